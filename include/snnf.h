@@ -450,6 +450,38 @@ int snnf_conv_blocked_tune(int T, int N, int Cin, int H, int W, int Cout, int KH
  * deterministic planner, and this is how a host reads its decision. The pointer stays valid for the thread's lifetime. */
 const char* snnf_conv_last_plan(void);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Sequence operators: the parts of a token model that is built from recurrences. The reference has no operators for these.
+ * ------------------------------------------------------------------------------------------------------------------ */
+
+typedef enum snnf_recurrence_form {
+    SNNF_RECURRENCE_LEAKY = 0,   /* a = sigmoid(gate), h_t = a h_{t-1} + (1 - a) x_t */
+    SNNF_RECURRENCE_LINEAR = 1   /* a = gate,          h_t = a h_{t-1} + x_t         */
+} snnf_recurrence_form;
+
+/* Gated linear recurrence over [T, N, D]. `x`, `gate` and `h` have elements of a row next to each other and any element strides over
+ * steps (`*_step`) and sequences (`*_row`); `gate` may have strides of 0. `h` overlaps neither input.
+ *   starts    NULL or a byte per (step, sequence), element strides as above: where it is not 0 the state is dropped before the step
+ *   lengths   NULL or N: steps from there on leave the state as it is and read 0 in `h`
+ *   state     NULL (zeros) or [N, D] float32; `state_out` [N, D] float32, not the same memory
+ *   marks     NULL, or snnf_gated_recurrence_marks_bytes(T, N, D) bytes that the backward pass will read
+ *   workspace snnf_gated_recurrence_workspace_bytes(...) bytes, 4-byte aligned (0: none needed), in use until the call's work is done
+ * T >= 1. Two launches where the sequences are few and long, else one. */
+size_t snnf_gated_recurrence_workspace_bytes(int T, int N, int D, int dtype, int backward);
+size_t snnf_gated_recurrence_marks_bytes(int T, int N, int D);
+int snnf_gated_recurrence(const void* x, int64_t x_step, int64_t x_row, const void* gate, int64_t gate_step, int64_t gate_row, int T, int N, int D,
+                          int dtype, int form, const void* starts, int64_t starts_step, int64_t starts_row, const int32_t* lengths,
+                          const float* state, void* h, int64_t h_step, int64_t h_row, float* state_out, float* marks, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* Its gradient: `dh` and `dstate` (NULL: zeros) are the gradients of `h` and of the last state, `dx`, `dgate` (not broadcast) and `dstate_in`
+ * those of `x`, `gate` and `state`. Steps from a sequence's length on get 0. `marks` as the forward call on the same operands left them. */
+int snnf_gated_recurrence_backward(const void* x, int64_t x_step, int64_t x_row, const void* gate, int64_t gate_step, int64_t gate_row, const void* dh,
+                                   int64_t dh_step, int64_t dh_row, int T, int N, int D, int dtype, int form, const void* starts,
+                                   int64_t starts_step, int64_t starts_row, const int32_t* lengths, const float* marks, const float* dstate,
+                                   void* dx, int64_t dx_step, int64_t dx_row, void* dgate, int64_t dgate_step, int64_t dgate_row, float* dstate_in,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

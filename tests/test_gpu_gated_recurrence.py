@@ -1,0 +1,321 @@
+"""Gated linear recurrence and its gradient against the formulas in float64 on the CPU.
+
+Tolerances: an output is rounded once, half a step of its type (`eps / 2` relative). Before that the kernels add float32 roundings: every step
+adds at most a few of 2^-24 relative to the largest state (decay, product, sum), a decay below 1 lets `memory` = 1 / (1 - largest decay)
+of them accumulate, and a decay that is itself off by a rounding acts like one more per step; runs of steps that are joined add one per
+joint. C = 8 covers decay (2), input gate (2), product and sum (1), joints (3)."""
+import pytest
+import torch
+
+from helpers import DEV, gen
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+U = 2.0 ** -24
+C = 8.0
+
+
+def reference(x, gate, state, form, starts=None, lengths=None, dh=None, dlast=None):
+    """float64, step by step: h, last and, with dh, (dx, dgate, dstate), and the largest |h| and |s|."""
+    x, gate = x.double().cpu(), gate.double().cpu()
+    T, N, D = x.shape
+    a, rest = (torch.sigmoid(gate), torch.sigmoid(-gate)) if form == "leaky" else (gate, torch.ones_like(gate))
+    h = torch.zeros(N, D, dtype=torch.float64) if state is None else state.double().cpu()
+    limit = torch.full((N,), T) if lengths is None else lengths.cpu().clamp(0, T)
+    inside = torch.arange(T)[:, None] < limit[None, :]
+    drop = torch.zeros(T, N, dtype=torch.bool) if starts is None else starts.cpu()
+    out, before = torch.zeros_like(x), torch.zeros_like(x)
+    peak = float(h.nan_to_num().abs().max()) if h.numel() else 0.0
+    for t in range(T):
+        before[t] = torch.where(drop[t][:, None], torch.zeros_like(h), h)
+        new = torch.where(drop[t][:, None], rest[t] * x[t], a[t] * h + rest[t] * x[t])
+        h = torch.where(inside[t][:, None], new, h)
+        out[t] = torch.where(inside[t][:, None], new, torch.zeros_like(new))
+        peak = max(peak, float(out[t].nan_to_num().abs().max()))
+    if dh is None:
+        return out, h, peak
+    dh = dh.double().cpu()
+    r = torch.zeros(N, D, dtype=torch.float64) if dlast is None else dlast.double().cpu()
+    dx, dgate = torch.zeros_like(x), torch.zeros_like(x)
+    most = float(r.abs().max())
+    for t in range(T - 1, -1, -1):
+        on = inside[t][:, None]
+        s = dh[t] + r
+        most = max(most, float(torch.where(on, s, torch.zeros_like(s)).nan_to_num().abs().max()))
+        dx[t] = torch.where(on, s * rest[t], torch.zeros_like(s))
+        dgate[t] = torch.where(on, s * (before[t] - x[t]) * a[t] * rest[t] if form == "leaky" else s * before[t], torch.zeros_like(s))
+        r = torch.where(on, torch.where(drop[t][:, None], torch.zeros_like(s), a[t] * s), r)
+    return out, h, peak, dx, dgate, r, most
+
+
+def operands(T, N, D, dtype, form, seed, batch_first=False):
+    g = gen(seed)
+    x, dh = torch.randn(T, N, D, generator=g), torch.randn(T, N, D, generator=g)
+    gate = (torch.randn(T, N, D, generator=g) * 1.5 + 1.0).clamp(-6.0, 4.0)                      # memory of at most 56 steps
+    if form == "linear":
+        gate = torch.sigmoid(gate) * torch.where(torch.rand(T, N, D, generator=g) < 0.1, -1.0, 1.0)
+    state, dlast = torch.randn(N, D, generator=g), torch.randn(N, D, generator=g)
+
+    def to(t):
+        if batch_first:
+            return t.transpose(0, 1).contiguous().to(DEV, dtype).transpose(0, 1)
+        return t.to(DEV, dtype)
+    return to(x), to(gate), state.to(DEV), to(dh), dlast.to(DEV)
+
+
+MEMORY = 60.0
+
+
+def near(got, want, dtype, extra, what):
+    got, want = got.double().cpu(), want.double()
+    room = torch.finfo(dtype).eps / 2 * (1 if dtype != torch.float32 else 0) * want.abs() + extra
+    if dtype == torch.float16:
+        room = room + 2.0 ** -25                                                                # half a step of the subnormals
+    off = (got - want).abs()
+    assert bool((off <= room).all()), f"{what}: off by {float((off - room).max()):.3g} over the tolerance, at most {float(off.max()):.3g}"
+
+
+def run(*args, **kwargs):
+    from triton_snn_fusion_amd.runtime.hip_gated_recurrence_backend import run_hip_gated_recurrence
+    return run_hip_gated_recurrence(*args, **kwargs)
+
+
+def check(T, N, D, dtype, form, seed, starts=None, lengths=None, batch_first=False, with_state=True, grad=True):
+    x, gate, state, dh, dlast = operands(T, N, D, dtype, form, seed, batch_first)
+    state = state if with_state else None
+    if not grad:
+        h, last = run(x, gate, state, form=form, starts=starts, lengths=lengths)
+        want = reference(x, gate, state, form, starts, lengths)
+    else:
+        leaves = [t.requires_grad_(True) for t in (x, gate, state) if t is not None]
+        h, last = run(x, gate, state, form=form, starts=starts, lengths=lengths)
+        got = torch.autograd.grad([h, last], leaves, [dh, dlast])
+        want = reference(x.detach(), gate.detach(), None if state is None else state.detach(), form, starts, lengths, dh, dlast)
+    torch.cuda.synchronize()
+    peak = want[2]
+    err = C * U * MEMORY * peak
+    near(h.detach(), want[0], dtype, err, "h")
+    near(last.detach(), want[1], torch.float32, err, "last state")
+    assert h.stride(2) == 1 and (N == 1 or T == 1 or (h.stride(1) > h.stride(0)) == batch_first)
+    if grad:
+        dx, dgate, dstate, most = want[3:]
+        top = float(x.detach().float().abs().max())
+        near(got[0], dx, dtype, C * U * MEMORY * most, "dx")
+        near(got[1], dgate, dtype, 2 * C * U * MEMORY * most * (peak + top), "dgate")
+        if state is not None:
+            near(got[2], dstate, torch.float32, C * U * MEMORY * most, "dstate")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["leaky", "linear"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,N,D", [(1, 1, 1), (1, 16, 1024), (2, 3, 65), (15, 2, 130), (16, 2, 128), (17, 1, 64), (33, 2, 192), (65, 1, 63),
+                                   (127, 2, 66), (257, 1, 320), (513, 2, 129), (1200, 1, 128)])
+def test_sizes(hip_ops, T, N, D, dtype, form):
+    check(T, N, D, dtype, form, 100 + T)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_columns_take_narrow_workgroups(hip_ops, dtype):
+    check(70, 40, 4096 if dtype == torch.float32 else 8192, dtype, "leaky", 7)      # 2560 waves of columns and more
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch_first", [False, True])
+@pytest.mark.parametrize("with_state", [False, True])
+def test_orders_in_memory_and_no_state(hip_ops, dtype, batch_first, with_state):
+    check(150, 3, 136, dtype, "leaky", 8, batch_first=batch_first, with_state=with_state)
+    check(5, 3, 136, dtype, "leaky", 9, batch_first=batch_first, with_state=with_state, grad=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["leaky", "linear"])
+@pytest.mark.parametrize("T,N,D", [(1, 4, 96), (16, 4, 96), (40, 4, 96), (700, 4, 96), (700, 4, 97)])
+def test_starts_and_lengths(hip_ops, T, N, D, form):
+    for dtype in DTYPES:
+        g = gen(T + D)
+        starts = torch.rand(T, N, generator=g) < 0.05
+        starts[0, 0] = True
+        starts[:, 3] = True                                                         # every step on its own
+        lengths = torch.tensor([T, max(0, T // 2), 0, T - 1], dtype=torch.int32)
+        check(T, N, D, dtype, form, 11, starts=starts.to(DEV))
+        check(T, N, D, dtype, form, 12, lengths=lengths.to(DEV))
+        check(T, N, D, dtype, form, 13, starts=starts.to(DEV), lengths=lengths.to(DEV), batch_first=True)
+        check(T, N, D, dtype, form, 14, starts=starts.t().contiguous().to(DEV).t(), lengths=torch.tensor([-5, 1 << 40, 1, T]).to(DEV), grad=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 20, 300])
+def test_what_is_masked_may_hold_anything(hip_ops, T):
+    """Padding full of NaN and infinities, and a state that overflowed in front of a start, change nothing."""
+    N, D = 3, 130
+    for dtype in DTYPES:
+        for form in ("leaky", "linear"):
+            x, gate, state, dh, dlast = operands(T, N, D, dtype, form, 15)
+            lengths = torch.tensor([T, T // 2, 0], dtype=torch.int32, device=DEV)
+            starts = torch.zeros(T, N, dtype=torch.bool, device=DEV)
+            starts[T // 3, 0] = True
+            outside = torch.arange(T, device=DEV)[:, None] >= lengths[None, :]
+            dirty = [t.clone() for t in (x, gate, dh)]
+            for t in dirty:
+                t[outside] = float("nan")
+                if T > 1:
+                    t[-1, 2] = float("inf")
+            dirty_state = state.clone()
+            answers = []
+            for xs, gs, ds in ((x, gate, dh), dirty):
+                leaves = [t.clone().requires_grad_(True) for t in (xs, gs, state)]
+                out = run(*leaves, form=form, starts=starts, lengths=lengths)
+                answers.append([*out, *torch.autograd.grad(out, leaves, [ds, dlast])])
+            for clean, got in zip(*answers):
+                assert torch.equal(clean, got)
+            # The first sequence's state is infinite before its start: from the start on it is as if it had been 0.
+            dirty_state[0] = float("inf")
+            after = run(x, gate, dirty_state, form=form, starts=starts)[0][T // 3:, 0]
+            assert torch.equal(after, run(x, gate, state, form=form, starts=starts)[0][T // 3:, 0])
+
+
+@pytest.mark.gpu
+def test_strided_operands_and_a_broadcast_gate(hip_ops):
+    """Slices of one projection and a gate per channel go in without copies; the expanded gate's gradient is summed."""
+    T, N, D = 90, 2, 96
+    g = gen(21)
+    wide = torch.randn(N, T, 2 * D + 1, generator=g).to(DEV, torch.bfloat16)
+    leak = torch.randn(D, generator=g).to(DEV, torch.bfloat16).requires_grad_(True)
+    x = wide[:, :, 1:D + 1].transpose(0, 1)                                         # odd offsets: no 4-byte accesses
+    h, last = run(x, leak.expand(T, N, D), None)
+    grad = torch.autograd.grad(h.float().sum(), leak)[0]
+    want = reference(x, leak.detach().expand(T, N, D), None, "leaky", dh=torch.ones(T, N, D), dlast=None)
+    near(h.detach(), want[0], torch.bfloat16, C * U * MEMORY * want[2], "h")
+    total = want[4].sum((0, 1))
+    # every element of the sum is rounded to bfloat16, and so is the sum, which autograd adds up in float32
+    room = torch.finfo(torch.bfloat16).eps / 2 * (want[4].abs().sum((0, 1)) + total.abs()) + T * N * 2 * C * U * MEMORY * want[6] * 10
+    assert bool(((grad.double().cpu() - total).abs() <= room).all())
+    assert torch.equal(run(wide[:, ::2, :D].transpose(0, 1), wide[:, ::2, D:2 * D].transpose(0, 1))[0],
+                       run(wide[:, ::2, :D].contiguous().transpose(0, 1), wide[:, ::2, D:2 * D].contiguous().transpose(0, 1))[0])
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences(hip_ops):
+    """One directional derivative per operand, float32, by central differences of the operator itself: truncation h^2 * third derivative
+    and rounding 2^-24 * memory * |loss terms| / h at h = 2^-6 stay below 2e-3 of the sum of the terms' sizes."""
+    T, N, D = 37, 2, 33
+    x, gate, state, dh, dlast = operands(T, N, D, torch.float32, "leaky", 31)
+    leaves = [t.requires_grad_(True) for t in (x, gate, state)]
+    out = run(*leaves)
+    grads = torch.autograd.grad(out, leaves, [dh, dlast])
+    step = 2.0 ** -6
+    for k in range(3):
+        way = torch.randn(leaves[k].shape, generator=gen(40 + k)).to(DEV)
+
+        def loss(sign):
+            moved = [t.detach() + (sign * step * way if i == k else 0) for i, t in enumerate(leaves)]
+            h, last = run(*moved)
+            return (h.double() * dh.double()).sum() + (last.double() * dlast.double()).sum()
+        slope = (loss(1) - loss(-1)) / (2 * step)
+        want = (grads[k].double() * way.double()).sum()
+        size = (grads[k].double() * way.double()).abs().sum()
+        assert abs(float(slope - want)) <= 2e-3 * float(size)
+
+
+@pytest.mark.gpu
+def test_a_sequence_in_pieces_and_repeated_calls(hip_ops):
+    """Handing the state over between pieces is the long call up to rounding, single tokens included; equal calls have equal bits."""
+    T, N, D = 400, 2, 128
+    x, gate, state, _, _ = operands(T, N, D, torch.float32, "leaky", 41)
+    whole, last = run(x, gate, state)
+    s, parts = state, []
+    for a, b in ((0, 1), (1, 2), (2, 30), (30, 300), (300, 400)):
+        h, s = run(x[a:b], gate[a:b], s)
+        parts.append(h)
+    err = 2 * C * U * MEMORY * float(whole.abs().max())
+    assert float((torch.cat(parts) - whole).abs().max()) <= err and float((s - last).abs().max()) <= err
+    for _ in range(3):
+        again = run(x, gate, state)
+        assert torch.equal(again[0], whole) and torch.equal(again[1], last)
+
+
+@pytest.mark.gpu
+def test_graph_replays_and_other_streams(hip_ops):
+    T, N, D = 300, 2, 128
+    x, gate, state, dh, dlast = operands(T, N, D, torch.bfloat16, "leaky", 51)
+    leaves = [t.requires_grad_(True) for t in (x, gate, state)]
+
+    def step():
+        out = run(*leaves)
+        return [*out, *torch.autograd.grad(out, leaves, [dh, dlast])]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        on_side = step()
+    torch.cuda.current_stream().wait_stream(side)
+    want = [t.clone() for t in step()]
+    assert all(torch.equal(a, b) for a, b in zip(on_side, want))
+    del on_side
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step())
+        graphs.append(graph)
+    for k in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(T, N, D, generator=gen(60 + k)).to(DEV, torch.bfloat16))
+        want = [t.clone() for t in step()]
+        for graph, out in zip(graphs, outs):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.gpu
+def test_empty(hip_ops):
+    for T, N, D in ((0, 2, 8), (3, 0, 8), (3, 2, 0)):
+        x = torch.empty(T, N, D, device=DEV, requires_grad=True)
+        state = torch.randn(N, D, device=DEV, requires_grad=True)
+        h, last = run(x, x, state)
+        assert h.shape == (T, N, D) and last.shape == (N, D)
+        if T == 0:
+            assert torch.equal(last, state)
+            assert torch.equal(torch.autograd.grad(last.sum(), state)[0], torch.ones_like(state))
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_gpu(hip_ops):
+    x = torch.zeros(4, 2, 8, device=DEV)
+    for args, kwargs, words in (((x, x[:3]), {}, "unsupported_shape"), ((x, x.half()), {}, "unsupported_dtype"), ((x, x, x[0].half()), {}, "unsupported_dtype"),
+                                ((x, x, x[0, :1]), {}, "unsupported_shape"), ((x[0], x[0]), {}, "unsupported_rank"), ((x.double(), x.double()), {}, "unsupported_dtype"),
+                                ((x, x), {"form": "other"}, "unsupported_form"), ((x, x), {"starts": torch.zeros(4, 2, device=DEV)}, "unsupported_dtype"),
+                                ((x, x), {"lengths": torch.zeros(2)}, "unsupported_device"), ((x, x.cpu()), {}, "unsupported_device")):
+        with pytest.raises(RuntimeError, match=words):
+            run(*args, **kwargs)
+    out = run(x.requires_grad_(True), x.detach() + 1)[0].sum()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(torch.autograd.grad(out, x, create_graph=True)[0].sum(), x)
+
+
+def test_refusals_without_a_gpu():
+    x = torch.zeros(4, 2, 8)
+    with pytest.raises(RuntimeError, match="unsupported_device"):
+        run(x, x)
+    with pytest.raises(RuntimeError, match="must be a tensor"):
+        run(None, x)
+
+
+def test_entry_points_refuse_before_any_gpu_work(snnf_lib):
+    f, b = snnf_lib.snnf_gated_recurrence, snnf_lib.snnf_gated_recurrence_backward
+
+    def forward(x=16, T=4, N=2, D=8, dtype=0, form=0, state_out=16, workspace=None, nbytes=0):
+        return f(x, 16, 8, 16, 16, 8, T, N, D, dtype, form, None, 0, 0, None, None, 16, 16, 8, state_out, None, workspace, nbytes, None)
+
+    assert forward(T=0) == -1 and forward(N=-1) == -1 and forward(dtype=9) == -1 and forward(form=2) == -1
+    assert forward(x=None) == -1 and b"non-null" in snnf_lib.snnf_last_error()
+    assert forward(state_out=None) == -1 and forward(N=0, x=None) == 0 and forward(D=0, x=None) == 0
+    assert forward(T=(1 << 30) + 1) == -2
+    assert snnf_lib.snnf_gated_recurrence_workspace_bytes(100000, 1, 64, 1, 0) > 0
+    assert forward(T=100000, N=1, D=64, dtype=1) == -4 and b"workspace" in snnf_lib.snnf_last_error()
+    assert b(16, 16, 8, 16, 16, 8, 16, 16, 8, 4, 2, 8, 0, 0, None, 0, 0, None, None, None, 16, 16, 8, 16, 16, 8, 16, None, 0, None) == -1    # no marks
+    assert b"marks" in snnf_lib.snnf_last_error()
+    assert snnf_lib.snnf_gated_recurrence_marks_bytes(0, 1, 1) == 0 and snnf_lib.snnf_gated_recurrence_marks_bytes(1, 3, 5) == 60

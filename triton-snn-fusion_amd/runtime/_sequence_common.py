@@ -1,0 +1,81 @@
+"""What the sequence operators (gated recurrence, block norm, token scores) share on the host side."""
+from __future__ import annotations
+
+import contextlib
+from typing import Iterable, List, Optional, Tuple
+
+import torch
+
+from .. import _lib
+
+SUPPORTED_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def refuse(operator: str, reasons: List[str]) -> None:
+    if reasons:
+        raise RuntimeError(f"{operator}: " + "; ".join(reasons))
+
+
+def check_activation(name: str, t, reasons: List[str]) -> bool:
+    """The tensor whose dtype and device the other operands have to match."""
+    if not isinstance(t, torch.Tensor):
+        reasons.append(f"{name} must be a tensor")
+        return False
+    if not t.is_cuda:
+        reasons.append(f"unsupported_device: {name} is not on the GPU")
+    if t.dtype not in SUPPORTED_DTYPES:
+        reasons.append(f"unsupported_dtype: {name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return not reasons
+
+
+def check_operand(name: str, t, device: torch.device, shape: Tuple[int, ...], dtypes: Iterable[torch.dtype], reasons: List[str]) -> None:
+    if not isinstance(t, torch.Tensor):
+        reasons.append(f"{name} must be a tensor")
+        return
+    if t.device != device:
+        reasons.append(f"unsupported_device: {name} is on {t.device}, not on {device}")
+    if tuple(t.shape) != tuple(shape):
+        reasons.append(f"unsupported_shape: {name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype not in tuple(dtypes):
+        reasons.append(f"unsupported_dtype: {name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+
+
+def wants_gradient(*tensors: Optional[torch.Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def on_device_of(t: torch.Tensor):
+    """Kernels launch on the current HIP device: a context that makes it the tensor's."""
+    if t.device.index is None or t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def unit_rows(t: torch.Tensor) -> torch.Tensor:
+    """The tensor itself where neighbouring elements of the last dimension lie next to each other, else a copy."""
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def workspace(nbytes: int, like: torch.Tensor) -> Optional[torch.Tensor]:
+    """Scratch memory from the caching allocator: of the current stream, and of the graph's own pool under capture, so that no two calls
+    in flight share it."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+
+
+def flat_rows(t: torch.Tensor) -> torch.Tensor:
+    """[..., D] as [rows, D] with any stride between rows: a view where the leading dimensions allow one, else a copy."""
+    t = unit_rows(t)
+    if t.dim() == 2:
+        return t
+    if t.dim() == 1:
+        return t.unsqueeze(0)
+    lead = 1
+    for n in t.shape[:-1]:
+        lead *= int(n)
+    try:
+        return t.view(lead, t.shape[-1])
+    except RuntimeError:
+        return t.contiguous().view(lead, t.shape[-1])
+
+
+__all__ = ["SUPPORTED_DTYPES", "check_activation", "check_operand", "flat_rows", "on_device_of", "refuse", "unit_rows", "wants_gradient", "workspace", "_lib"]
