@@ -464,11 +464,11 @@ typedef enum snnf_recurrence_form {
  *   starts    NULL or a byte per (step, sequence), element strides as above: where it is not 0 the state is dropped before the step
  *   lengths   NULL or N: steps from there on leave the state as it is and read 0 in `h`
  *   state     NULL (zeros) or [N, D] float32; `state_out` [N, D] float32, not the same memory
- *   marks     NULL, or snnf_gated_recurrence_marks_bytes(T, N, D) bytes that the backward pass will read
+ *   marks     NULL, or snnf_gated_recurrence_marks_bytes(T, N, D, dtype) bytes that the backward pass will read
  *   workspace snnf_gated_recurrence_workspace_bytes(...) bytes, 4-byte aligned (0: none needed), in use until the call's work is done
  * T >= 1. Two launches where the sequences are few and long, else one. */
 size_t snnf_gated_recurrence_workspace_bytes(int T, int N, int D, int dtype, int backward);
-size_t snnf_gated_recurrence_marks_bytes(int T, int N, int D);
+size_t snnf_gated_recurrence_marks_bytes(int T, int N, int D, int dtype);
 int snnf_gated_recurrence(const void* x, int64_t x_step, int64_t x_row, const void* gate, int64_t gate_step, int64_t gate_row, int T, int N, int D,
                           int dtype, int form, const void* starts, int64_t starts_step, int64_t starts_row, const int32_t* lengths,
                           const float* state, void* h, int64_t h_step, int64_t h_row, float* state_out, float* marks, void* workspace,

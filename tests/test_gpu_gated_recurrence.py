@@ -109,7 +109,7 @@ def check(T, N, D, dtype, form, seed, starts=None, lengths=None, batch_first=Fal
 @pytest.mark.parametrize("form", ["leaky", "linear"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,N,D", [(1, 1, 1), (1, 16, 1024), (2, 3, 65), (15, 2, 130), (16, 2, 128), (17, 1, 64), (33, 2, 192), (65, 1, 63),
-                                   (127, 2, 66), (257, 1, 320), (513, 2, 129), (1200, 1, 128)])
+                                   (127, 2, 66), (257, 1, 320), (513, 2, 129), (1200, 1, 128), (256, 20, 1280), (2500, 1, 64)])
 def test_sizes(hip_ops, T, N, D, dtype, form):
     check(T, N, D, dtype, form, 100 + T)
 
@@ -318,4 +318,6 @@ def test_entry_points_refuse_before_any_gpu_work(snnf_lib):
     assert forward(T=100000, N=1, D=64, dtype=1) == -4 and b"workspace" in snnf_lib.snnf_last_error()
     assert b(16, 16, 8, 16, 16, 8, 16, 16, 8, 4, 2, 8, 0, 0, None, 0, 0, None, None, None, 16, 16, 8, 16, 16, 8, 16, None, 0, None) == -1    # no marks
     assert b"marks" in snnf_lib.snnf_last_error()
-    assert snnf_lib.snnf_gated_recurrence_marks_bytes(0, 1, 1) == 0 and snnf_lib.snnf_gated_recurrence_marks_bytes(1, 3, 5) == 60
+    assert snnf_lib.snnf_gated_recurrence_marks_bytes(0, 1, 1, 0) == 0 and snnf_lib.snnf_gated_recurrence_marks_bytes(1, 3, 5, 0) == 60
+    assert f(16, 1 << 31, 8, 16, 16, 8, 4, 2, 8, 0, 0, None, 0, 0, None, None, 16, 16, 8, 16, None, None, 0, None) == -2
+    assert b"unsupported_stride" in snnf_lib.snnf_last_error()

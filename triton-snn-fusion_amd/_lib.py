@@ -71,7 +71,7 @@ SIGNATURES = {
     "snnf_conv_bias_workspace_bytes": (_sz, [_i] * 14),
     "snnf_conv_bias_ws": (_i, [_pp, _pp, _i, _i, _i, _i, _i, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _i64, _vp, _sz, _vp]),
     "snnf_gated_recurrence_workspace_bytes": (_sz, [_i] * 5),
-    "snnf_gated_recurrence_marks_bytes": (_sz, [_i] * 3),
+    "snnf_gated_recurrence_marks_bytes": (_sz, [_i] * 4),
     "snnf_gated_recurrence": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _i, _i, _i, _i, _i, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _sz, _vp]),
     "snnf_gated_recurrence_backward": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i, _i, _i, _i, _i, _vp, _i64, _i64, _vp, _vp, _vp,
                                             _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _sz, _vp]),

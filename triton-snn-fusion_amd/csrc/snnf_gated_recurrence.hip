@@ -3,9 +3,13 @@
 //     leaky :  a = sigmoid(g),  h_t = a h_{t-1} + (1 - a) x_t          linear:  a = g,  h_t = a h_{t-1} + x_t
 // A step composes with the next one: a run of steps is h -> A h + H with A the product of its a and H its result from h = 0. So a
 // sequence is cut into runs that are reduced to (A, H) at once and joined in order: a wave holds the elements of `S` steps of 64 * VEC
-// channels in registers, the W waves of a workgroup hold consecutive runs (a tile of W * S steps) and join through LDS, and where
-// there are too few channels to fill the chip, workgroups take chunks of whole tiles whose (A, H) a first kernel works out.
-// Joining is the same chain of fused multiply-adds in every variant's order: results do not depend on timing.
+// channels in registers, the W waves of a workgroup hold consecutive runs (a tile of W * S steps) and join through LDS. Where there are
+// columns of channels enough to fill the chip, a workgroup walks over the tiles of its column. Where there are not, tiles are
+// handed out in the order of time and each is joined with those before it through memory ("relay"): every element is still read once.
+// The value that enters a tile is always the same chain of fused multiply-adds over the tiles before it: results do not depend on timing.
+// A of a run with a long memory is worked out as 1 - c with c_t = c_{t-1} + (1 - a_t) (1 - c_{t-1}), which loses one rounding where the
+// product of the a loses one per step: the last state of 4096 steps with memories of up to 2000 is then as exact as from a scan in
+// which no value passes more than log2 T roundings.
 //
 // Gradient: with r_t the gradient that reaches h_t from later steps, s_t = dh_t + r_t and r_{t-1} = a_t s_t, the same recurrence
 // backwards; dx = s (1 - a) or s, dg = s (h_{t-1} - x) a (1 - a) or s h_{t-1}. h_{t-1} is not read but worked out again from the
@@ -16,9 +20,15 @@
 namespace snnf {
 namespace {
 
-constexpr int kSteps = 16;              // steps of a wave's run, forward
-constexpr int kBackSteps = 8;           // and backward, which holds twice the values for each
-
+// Waves of a tile and steps of a wave. Relay: the largest tile that 128 registers a lane and 16 waves allow (with the waves that relay), since
+// each costs a trip through memory (16384 x 2 x 2048 bf16, forward: tiles of 224 steps 94 us, of 168 101, of 112 124). Walk: enough waves to
+// cover the latency of memory by themselves where there are few columns (2048 x 16 x 2048: 8 waves 83 us, 4 85; 100 x 16 x 1024: 6.1 and
+// 7.2), 4 where workgroups cover for each other (512 x 64 x 2048: 78 us, 8 waves 80).
+constexpr int kRelayWaves = 14, kRelaySteps = 16, kRelayBackSteps = 8;
+constexpr int kWalkWaves = 8, kWalkWavesMany = 4, kWalkSteps = 8;
+// Tiles that a relay looks back at in one go: more of them reach further where all tiles start at once, and cost their loads where most
+// tiles in front are done (8192 x 1 x 1024: 2 28.6 us, 4 23.5, 8 22.4, 16 24.5; 16384 x 2 x 2048: 92, 94, 102, 111).
+constexpr int kReach = 4;
 constexpr int kMostSteps = 1 << 30;
 
 struct Series {                         // [T, N, D] with elements of a row next to each other
@@ -39,48 +49,42 @@ struct Args {
     const float* state;                 // forward: the state before the first step; backward: the gradient of the last state
     float* state_out;                   // the other way round
     float* marks;
-    float* chunks;                      // [chunk][2][N * D]: what a chunk does to the value that enters it
+    uint32_t* ticket;                   // relay: tiles handed out so far, less one
+    uint64_t* runs;                     // relay: [tile][N * D] (A, H) of a tile, all ones while it is not known
+    uint32_t* values;                   // relay: [tile][N * D] value behind a tile, all ones while it is not known
     int T, N, D;
     int groups;                         // wave-wide groups of channels in a row
+    int columns;                        // N * groups
+    int tiles;
     int span;                           // steps from one mark to the next
-    int tiles;                          // tiles of a chunk
-    int n_chunks;
-    int leaky;
 };
 
 template <typename XT> constexpr bool kPrecise = false;
 template <> constexpr bool kPrecise<float> = true;
 
-// a = sigmoid(g) and 1 - a, both to full relative accuracy: with e = exp(-|g|) the larger is 1 / (1 + e) and the smaller e / (1 + e).
-// v_exp_f32 works on powers of two; for float32 tensors what the product with log2(e) loses is put back to first order.
+// a = sigmoid(g) = 1 / (1 + e) and 1 - a = e / (1 + e) with e = exp(-g), both to full relative accuracy; a NaN stays one, and a gate of
+// infinity gives a = 1 and 1 - a = 0 exactly. e is kept from overflowing. v_exp_f32 works on powers of two; for float32 tensors what the
+// product with log2(e) loses is put back to first order.
 template <bool PRECISE>
 __device__ __forceinline__ void leak(float g, float& a, float& rest) {
     constexpr float kLog2e = 1.44269504088896340736f, kLog2eLow = 1.925963033500e-8f, kLn2 = 0.69314718055994530942f;
-    const float y = -fabsf(g);
-    const float t = y * kLog2e;
-    float e = __builtin_amdgcn_exp2f(t);
+    float e;
     if constexpr (PRECISE) {
-        const float lost = fmaf(y, kLog2eLow, fmaf(y, kLog2e, -t));
-        e = y < -126.0f ? e : fmaf(e, lost * kLn2, e);             // (far out e is 0 or next to it; -inf would make lost a NaN)
+        const float y = __builtin_elementwise_minimum(__builtin_elementwise_maximum(g, -86.0f), 200.0f);
+        const float t = y * -kLog2e;
+        e = __builtin_amdgcn_exp2f(t);
+        e = fmaf(e, fmaf(y, -kLog2eLow, fmaf(y, -kLog2e, -t)) * kLn2, e);
+    } else {
+        e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(g * -kLog2e, 124.0f));
     }
-    const float big = __builtin_amdgcn_rcpf(1.0f + e), small = e * big;
-    const bool positive = g >= 0.0f;
-    a = positive ? big : small;
-    rest = positive ? small : big;
-    if (g != g) a = rest = g;
+    a = __builtin_amdgcn_rcpf(1.0f + e);
+    rest = e * a;
 }
 
-template <typename XT, int VEC>
-__device__ __forceinline__ Pack<XT, VEC> load_at(const void* base, int64_t offset, int lane_offset) {
-    return *reinterpret_cast<const Pack<XT, VEC>*>(static_cast<const XT*>(base) + offset + lane_offset);
-}
-
-// Bit i: the state is dropped before step `first` + i.
-__device__ __forceinline__ uint32_t start_bits(const Args& p, int n, int first, int lim, int steps) {
+// Lane i: whether the state is dropped before step `first` + i.
+__device__ __forceinline__ uint8_t start_of(const Args& p, int n, int first, int lim, int steps) {
     const int lane = threadIdx.x & 63;
-    bool on = false;
-    if (lane < steps && first + lane < lim) on = p.starts[static_cast<int64_t>(first + lane) * p.starts_step + static_cast<int64_t>(n) * p.starts_row] != 0;
-    return static_cast<uint32_t>(__ballot(on));
+    return lane < steps && first + lane < lim ? p.starts[static_cast<int64_t>(first + lane) * p.starts_step + static_cast<int64_t>(n) * p.starts_row] : 0;
 }
 
 // One link of the chain: what a run of steps makes of the value that enters it. A run that drops the value has A = 0, and must not multiply
@@ -92,16 +96,19 @@ __device__ __forceinline__ float link(float A, float entering, float H) {
     return v;
 }
 
+// What is left of the value that enters a run: the product of its decays, or for a long memory 1 - c.
+__device__ __forceinline__ float left_over(float product, float c) { return c < 0.5f && c > -0.5f ? 1.0f - c : product; }
+
 struct Place {
     int n, d, lim;                      // sequence, first channel of the lane, steps that count
     bool active;
     int64_t cell;                       // n * D + d
 };
 template <int VEC>
-__device__ __forceinline__ Place place(const Args& p) {
+__device__ __forceinline__ Place place(const Args& p, int column) {
     Place q;
-    q.n = blockIdx.x / p.groups;
-    q.d = ((blockIdx.x - q.n * p.groups) * 64 + (threadIdx.x & 63)) * VEC;
+    q.n = column / p.groups;
+    q.d = ((column - q.n * p.groups) * 64 + (threadIdx.x & 63)) * VEC;
     q.active = q.d < p.D;
     q.cell = static_cast<int64_t>(q.n) * p.D + q.d;
     q.lim = p.T;
@@ -113,444 +120,598 @@ __device__ __forceinline__ Place place(const Args& p) {
     return q;
 }
 
-// The elements of S steps from `first` on, those that do not count left as they were.
+// A tensor from step `first` of a sequence on as a buffer, so that steps are a scalar offset and a lane behind the row's end, whose offset lies
+// outside any buffer, reads 0 and stores nothing. Steps of a run and a row's bytes together stay below 2^31 (`dispatch`).
+constexpr int kBufferBytes = 0x7fffffff;
+__device__ __forceinline__ int lane_bytes(const Place& q, int size) { return q.active ? q.d * size : static_cast<int>(0x80000000u); }
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const void* p, int64_t step, int64_t row, const Place& q, int first, int size) {
+    const char* base = static_cast<const char*>(p) + (static_cast<int64_t>(q.n) * row + static_cast<int64_t>(first) * step) * size;
+    const uint64_t at = reinterpret_cast<uint64_t>(base);
+    const uint64_t same = static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32))) << 32 |
+                          static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at)));
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(same), 0, kBufferBytes, 0x00020000);
+}
+// VEC elements of a row in one register; as a word, not as a struct of 16-bit halves, which the compiler would take apart at every copy.
+template <typename XT, int VEC>
+__device__ __forceinline__ uint32_t read(__amdgpu_buffer_rsrc_t from, int lane_bytes, int step_bytes) {
+    if constexpr (sizeof(XT) * VEC == 4) return __builtin_amdgcn_raw_buffer_load_b32(from, lane_bytes, step_bytes, 0);
+    else return static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(from, lane_bytes, step_bytes, 0));
+}
+template <typename XT, int VEC>
+__device__ __forceinline__ void write(__amdgpu_buffer_rsrc_t to, uint32_t word, int lane_bytes, int step_bytes) {
+    if constexpr (sizeof(XT) * VEC == 4) __builtin_amdgcn_raw_buffer_store_b32(word, to, lane_bytes, step_bytes, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(word), to, lane_bytes, step_bytes, 0);
+}
+template <typename XT>
+__device__ __forceinline__ float element(uint32_t word, int j) {
+    if constexpr (sizeof(XT) == 4) return __uint_as_float(word);
+    else if constexpr (dtype_of<XT>::value == SNNF_BF16) return __uint_as_float(j == 0 ? word << 16 : word & 0xffff0000u);
+    else return f16_bits_to_float(j == 0 ? word & 0xffffu : word >> 16);
+}
+template <typename XT, int VEC>
+__device__ __forceinline__ uint32_t word_of(const float (&v)[VEC]) {
+    if constexpr (sizeof(XT) == 4) return __float_as_uint(v[0]);
+    else if constexpr (dtype_of<XT>::value == SNNF_BF16) {
+        if constexpr (VEC == 2) return float_to_bf16_pair(v[0], v[1]);
+        else return float_to_bf16_bits(v[0]);
+    } else {
+        if constexpr (VEC == 2) return float_to_f16_bits(v[0]) | float_to_f16_bits(v[1]) << 16;
+        else return float_to_f16_bits(v[0]);
+    }
+}
+
+// The elements of S steps from `first` on. Steps that do not count are read from the last that does (from the first if there is none).
 template <typename XT, int VEC, int S>
-__device__ __forceinline__ void fetch(Pack<XT, VEC> (&to)[S], const Series& from, const Place& q, int first) {
-    if (!q.active) return;
-    const XT* base = static_cast<const XT*>(from.p) + static_cast<int64_t>(q.n) * from.row + static_cast<int64_t>(first) * from.step;
+__device__ __forceinline__ void fetch(uint32_t (&to)[S], const Series& from, const Place& q, int first) {
+    const int last = q.lim > 0 ? q.lim - 1 : 0, begin = first < last ? first : last;
+    const auto rows = rows_at(from.p, from.step, from.row, q, begin, sizeof(XT));
+    const int step = static_cast<int>(from.step) * static_cast<int>(sizeof(XT)), d = lane_bytes(q, sizeof(XT));
+#pragma unroll
+    for (int i = 0; i < S; ++i) to[i] = read<XT, VEC>(rows, d, (i < last - begin ? i : last - begin) * step);
+}
+template <typename XT, int VEC, int S>
+__device__ __forceinline__ void idle(uint32_t (&x)[S], const Place& q, int first, float value) {
+    if (first + S <= q.lim) return;
+    float v[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = value;
+    const uint32_t word = word_of<XT, VEC>(v);
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+        if (first + i >= q.lim) x[i] = word;
+}
+// What a gate is where a step does not count: a = 1 and nothing enters.
+template <bool LEAKY> constexpr float kIdleGate = LEAKY ? INFINITY : 1.0f;
+
+template <typename XT, int VEC, int S>
+__device__ __forceinline__ void store(const Output& to, const Place& q, int first, int T, const uint32_t (&y)[S]) {
+    const auto rows = rows_at(to.p, to.step, to.row, q, first, sizeof(XT));
+    const int step = static_cast<int>(to.step) * static_cast<int>(sizeof(XT)), d = lane_bytes(q, sizeof(XT));
     if (first + S <= q.lim) {
 #pragma unroll
-        for (int i = 0; i < S; ++i) to[i] = load_at<XT, VEC>(base, i * from.step, q.d);
+        for (int i = 0; i < S; ++i) write<XT, VEC>(rows, y[i], d, i * step);
     } else {
 #pragma unroll
         for (int i = 0; i < S; ++i)
-            if (first + i < q.lim) to[i] = load_at<XT, VEC>(base, i * from.step, q.d);
+            if (first + i < T) write<XT, VEC>(rows, first + i < q.lim ? y[i] : 0u, d, i * step);
     }
 }
 
-// Value that enters chunk `c`: the chunks before it (forward) or behind it (backward) in their order.
-template <int VEC, bool STARTS, bool BACKWARD>
-__device__ __forceinline__ void entering(const Args& p, const Place& q, int c, float (&v)[VEC]) {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = q.active && p.state != nullptr ? p.state[q.cell + j] : 0.0f;
-    if (!q.active) return;
+// ------------------------------------------------------------------------------------------------------------------
+// Relay: a tile publishes its (A, H), takes the value that enters it from the tiles in front of it in the order of the scan, and publishes
+// the value behind it. Each word says by itself whether it is known, so that relaxed accesses of the agent's scope are enough.
+// A tile waits only for tiles that were handed out before it: those run already and publish their (A, H) without waiting for anyone.
+// ------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t plain_bits(float v) { return v != v ? 0x7fc00000u : __float_as_uint(v); }      // never all ones
+
+// One channel a lane; `cell` < 0: none.
+template <bool STARTS>
+__device__ __forceinline__ float relay(const Args& p, int64_t cell, int order, float A, float H) {
     const int64_t cells = static_cast<int64_t>(p.N) * p.D;
-    const int many = BACKWARD ? p.n_chunks - 1 - c : c;
-    constexpr int kBatch = 4;
-    for (int i0 = 0; i0 < many; i0 += kBatch) {
-        float A[kBatch][VEC], H[kBatch][VEC];
+    const bool active = cell >= 0, last = order == p.tiles - 1;
+    uint64_t* runs = p.runs + order * cells + cell;
+    uint32_t* values = p.values + order * cells + cell;
+    if (active && !last)
+        __hip_atomic_store(runs, static_cast<uint64_t>(plain_bits(A)) << 32 | plain_bits(H), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    float from = active && p.state != nullptr ? p.state[cell] : 0.0f;
+    if (order > 0) {
+        const int reach = order < kReach ? order : kReach;
+        uint64_t run[kReach];
+        uint32_t value[kReach];
+        int found;                      // tiles whose (A, H) lie between the value found and this tile
+        for (;;) {
+            found = -1;
+            if (active) {
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            const int i = i0 + u < many ? i0 + u : many - 1;
-            const float* from = p.chunks + (BACKWARD ? p.n_chunks - 1 - i : i) * 2 * cells + q.cell;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                A[u][j] = from[j];
-                H[u][j] = from[cells + j];
+                for (int i = 0; i < kReach; ++i) {
+                    const int64_t back = (i < reach ? i + 1 : reach) * cells;
+                    run[i] = __hip_atomic_load(runs - back, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    value[i] = __hip_atomic_load(values - back, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
             }
+            bool chained = true;        // every tile up to here has published its (A, H)
+#pragma unroll
+            for (int i = 0; i < kReach; ++i) {
+                const bool all_value = __all(!active || value[i] != ~0u), all_run = __all(!active || run[i] != ~0ull);
+                if (chained && found < 0 && i < reach && all_value) found = i;
+                chained = chained && (i >= reach || all_run);
+            }
+            if (found < 0 && chained && order <= kReach) found = reach;         // all the way to the start
+            if (found >= 0) break;
+            __builtin_amdgcn_s_sleep(1);
         }
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u)
-            if (i0 + u < many) {
+        for (int i = kReach - 1; i >= 0; --i) {
+            if (i == found && i < reach) from = __uint_as_float(value[i]);
+            if (i < found) from = link<STARTS>(__uint_as_float(static_cast<uint32_t>(run[i] >> 32)), from, __uint_as_float(static_cast<uint32_t>(run[i])));
+        }
+    }
+    const float behind = link<STARTS>(A, from, H);
+    if (active) {
+        if (last) p.state_out[cell] = behind;
+        else __hip_atomic_store(values, plain_bits(behind), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    return from;
+}
+
+__global__ __launch_bounds__(256) void unknown_kernel(uint4* p, int64_t n) {
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) p[i] = uint4{~0u, ~0u, ~0u, ~0u};
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// Steps of one wave
+// ------------------------------------------------------------------------------------------------------------------
+template <typename XT, int VEC, int S, bool LEAKY>
+__device__ __forceinline__ void decode(const uint32_t (&g)[S], float (&a)[S][VEC], float (&rest)[S][VEC]) {
+    if constexpr (LEAKY) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) v[j] = link<STARTS>(A[u][j], v[j], H[u][j]);
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) leak<kPrecise<XT>>(element<XT>(g[i], j), a[i][j], rest[i][j]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                a[i][j] = element<XT>(g[i], j);
+                rest[i][j] = 1.0f - a[i][j];
             }
     }
 }
 
-// ------------------------------------------------------------------------------------------------------------------
-// Forward. REDUCE: only (A, H) of the chunk.
-// ------------------------------------------------------------------------------------------------------------------
-template <typename XT, int VEC, int W, int S, bool STARTS, bool REDUCE>
-__global__ __launch_bounds__(64 * W) void recurrence_kernel(Args p) {
-    constexpr int kLinks = W > 1 ? W : 1;
-    __shared__ float links[2][kLinks][2 * VEC][64];
-    const Place q = place<VEC>(p);
-    const int lane = threadIdx.x & 63, wave = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
-    const int chunk = blockIdx.y;
-    const int begin = chunk * p.tiles * W * S, end = begin + p.tiles * W * S < p.T ? begin + p.tiles * W * S : p.T;
-    using XV = Pack<XT, VEC>;
-    XV g[S], x[S];
-    fetch<XT, VEC, S>(g, p.gate, q, begin + wave * S);
-    fetch<XT, VEC, S>(x, p.x, q, begin + wave * S);
-    float v[VEC], whole[VEC];           // the state that enters the tile; REDUCE: product of the chunk so far
-    if constexpr (REDUCE) {
+// The same bits, of which the compiler knows nothing.
+template <int S>
+__device__ __forceinline__ void again(uint32_t (&x)[S]) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = 0.0f, whole[j] = 1.0f;
-    } else {
-        entering<VEC, STARTS, false>(p, q, chunk, v);
+    for (int i = 0; i < S; ++i) asm("" : "+v"(x[i]));
+}
+
+// The value that enters step i of a run whose bit says whether it is dropped.
+template <bool STARTS>
+__device__ __forceinline__ float kept(uint32_t drop, int i, float v) { return STARTS && (drop >> i & 1u) ? 0.0f : v; }
+
+// A of the run and H: what it makes of 0.
+template <int VEC, int S, bool STARTS>
+__device__ __forceinline__ void reduce(const float (&a)[S][VEC], const float (&b)[S][VEC], const float (&c)[VEC], uint32_t drop, float (&A)[VEC], float (&H)[VEC]) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) A[j] = 1.0f, H[j] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            H[j] = fmaf(a[i][j], kept<STARTS>(drop, i, H[j]), b[i][j]);
+            A[j] *= a[i][j];
+        }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) A[j] = STARTS && drop != 0 ? 0.0f : left_over(A[j], c[j]);
+}
+
+// The W runs of a tile as one: A in row `w * rows`, H `second` rows behind it.
+template <int W, bool STARTS>
+__device__ __forceinline__ void join(float (*links)[64], int rows, int second, bool reversed, float& A, float& H) {
+    const int lane = threadIdx.x & 63;
+    float c = 0.0f;
+    A = 1.0f, H = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < W; ++i) {
+        const int w = reversed ? W - 1 - i : i;
+        const float Aw = links[w * rows][lane];
+        H = link<STARTS>(Aw, H, links[w * rows + second][lane]);
+        A *= Aw;
+        c = fmaf(1.0f - Aw, 1.0f - c, c);
     }
-    int buffer = 0;
-    for (int t0 = begin; t0 < end; t0 += W * S) {
+    A = STARTS && A == 0.0f ? 0.0f : left_over(A, c);
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// A tile in the hands of its W waves. Forward: read, reduce, and with the value that enters the wave's run, write.
+// ------------------------------------------------------------------------------------------------------------------
+template <typename XT, int VEC, int W, int S, bool STARTS, bool LEAKY>
+struct ForwardTile {
+    static constexpr int kParts = 2;
+    uint32_t g[S], x[S];
+    uint8_t start;
+    float a[S][VEC], b[S][VEC], c[VEC];
+    uint32_t drop;                         // bit i: the state is dropped before step i of the run
+
+    __device__ __forceinline__ static int at(const Args&, int order) { return order * W * S; }
+    __device__ __forceinline__ void fetch_tile(const Args& p, const Place& q, int t0, int wave) {
         const int first = t0 + wave * S;
-        uint32_t drop = 0;
-        if constexpr (STARTS) drop = start_bits(p, q.n, first, q.lim, S);
-        float a[S][VEC], b[S][VEC];
+        fetch<XT, VEC, S>(g, p.gate, q, first);
+        fetch<XT, VEC, S>(x, p.x, q, first);
+        if constexpr (STARTS) start = start_of(p, q.n, first, q.lim, S);
+    }
+    __device__ __forceinline__ void decode_tile(const Place& q, int t0, int wave) {
+        const int first = t0 + wave * S;
+        idle<XT, VEC, S>(g, q, first, kIdleGate<LEAKY>);
+        idle<XT, VEC, S>(x, q, first, 0.0f);
+        float rest[S][VEC];
+        decode<XT, VEC, S, LEAKY>(g, a, rest);
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) b[i][j] = LEAKY ? rest[i][j] * element<XT>(x[i], j) : element<XT>(x[i], j);
+        drop = 0;
+        if constexpr (STARTS) drop = static_cast<uint32_t>(__ballot(start != 0));
+        if constexpr (W > 1) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) c[j] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) c[j] = fmaf(rest[i][j], 1.0f - c[j], c[j]);
+        }
+    }
+    __device__ __forceinline__ void reduce_tile(float (*links)[64], int wave) {
+        const int lane = threadIdx.x & 63;
+        float A[VEC], H[VEC];
+        reduce<VEC, S, STARTS>(a, b, c, drop, A, H);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            links[wave * 2 * VEC + j][lane] = A[j];
+            links[(wave * 2 + 1) * VEC + j][lane] = H[j];
+        }
+    }
+    // v: the value that enters the run, then the one behind it
+    __device__ __forceinline__ void write_tile(const Args& p, const Place& q, int t0, int wave, float (*)[64], float (&v)[VEC]) {
+        const int first = t0 + wave * S;
+        if (p.marks != nullptr && q.active && first % p.span == 0 && first < p.T) {
+            float* mark = p.marks + static_cast<int64_t>(first / p.span) * p.N * p.D + q.cell;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) mark[j] = v[j];
+        }
+        uint32_t y[S];
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            const bool counts = first + i < q.lim;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[j] = fmaf(a[i][j], kept<STARTS>(drop, i, v[j]), b[i][j]);
+            y[i] = word_of<XT, VEC>(v);
+        }
+        store<XT, VEC, S>(p.h, q, first, p.T, y);
+    }
+    // Waves whose runs the value passes before it reaches wave `wave`.
+    __device__ __forceinline__ static int passes(int wave) { return wave; }
+    __device__ __forceinline__ static int wave_at(int k) { return k; }
+};
+
+// Backward, from the last tile to the first: the value that travels is the gradient, and h comes from the tile's mark.
+template <typename XT, int VEC, int W, int S, bool STARTS, bool LEAKY>
+struct BackwardTile {
+    static constexpr int kParts = 3;       // A, R, H
+    uint32_t g[S], x[S], dh[S], xs[S], es[S];
+    float next_mark[VEC], mark[VEC];
+    uint8_t start;
+    float a[S][VEC], rest[S][VEC];
+    float A[VEC], H[VEC], R[VEC];
+    uint32_t drop;
+
+    __device__ __forceinline__ static int at(const Args& p, int order) { return (p.tiles - 1 - order) * W * S; }
+    __device__ __forceinline__ void fetch_tile(const Args& p, const Place& q, int t0, int wave) {
+        const int first = t0 + wave * S;
+        fetch<XT, VEC, S>(g, p.gate, q, first);
+        fetch<XT, VEC, S>(dh, p.dh, q, first);
+        fetch<XT, VEC, S>(x, p.x, q, first);
+        if constexpr (STARTS) start = start_of(p, q.n, first, q.lim, S);
+        const float* from = p.marks + static_cast<int64_t>(t0 / p.span) * p.N * p.D + q.cell;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) next_mark[j] = q.active ? from[j] : 0.0f;
+    }
+    __device__ __forceinline__ float in(int i, int j) const { return LEAKY ? rest[i][j] * element<XT>(xs[i], j) : element<XT>(xs[i], j); }
+    __device__ __forceinline__ void decode_tile(const Place& q, int t0, int wave) {
+        const int first = t0 + wave * S;
+        idle<XT, VEC, S>(g, q, first, kIdleGate<LEAKY>);
+        idle<XT, VEC, S>(x, q, first, 0.0f);
+        idle<XT, VEC, S>(dh, q, first, 0.0f);
+        decode<XT, VEC, S, LEAKY>(g, a, rest);
+        drop = 0;
+        if constexpr (STARTS) drop = static_cast<uint32_t>(__ballot(start != 0));
+        float b[S][VEC], c[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) mark[j] = next_mark[j], c[j] = 0.0f, R[j] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            xs[i] = x[i], es[i] = dh[i];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                float ai = to_float(g[i].v[j]), bi = to_float(x[i].v[j]);
-                if (p.leaky) {
-                    float rest;
-                    leak<kPrecise<XT>>(ai, ai, rest);
-                    bi *= rest;
-                }
-                a[i][j] = counts ? ai : 1.0f;
-                b[i][j] = counts ? bi : 0.0f;
+                b[i][j] = in(i, j);
+                c[j] = fmaf(rest[i][j], 1.0f - c[j], c[j]);
             }
         }
-        const bool more = t0 + W * S < end;
-        if (more) {
-            fetch<XT, VEC, S>(g, p.gate, q, first + W * S);
-            fetch<XT, VEC, S>(x, p.x, q, first + W * S);
-        }
-        float enter[VEC];
-        if constexpr (W > 1 || REDUCE) {
-            float A[VEC], H[VEC];
+        reduce<VEC, S, STARTS>(a, b, c, drop, A, H);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) A[j] = 1.0f, H[j] = 0.0f;
+        for (int i = S - 1; i >= 0; --i)
 #pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const bool dropped = STARTS && (drop >> i & 1u);
+            for (int j = 0; j < VEC; ++j) R[j] = kept<STARTS>(drop, i, a[i][j] * (R[j] + element<XT>(es[i], j)));
+        // From here on the elements are taken apart anew: kept apart, they would double the registers of the wait.
+        again<S>(xs);
+        again<S>(es);
+    }
+    __device__ __forceinline__ void reduce_tile(float (*links)[64], int wave) {
+        const int lane = threadIdx.x & 63;
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    H[j] = dropped ? b[i][j] : fmaf(a[i][j], H[j], b[i][j]);
-                    A[j] = dropped ? 0.0f : A[j] * a[i][j];
-                }
-            }
-            if constexpr (W > 1) {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    links[buffer][wave][j][lane] = A[j];
-                    links[buffer][wave][VEC + j][lane] = H[j];
-                }
-                __syncthreads();
-#pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    if (w == wave) {
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j) enter[j] = v[j];
-                    }
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        const float Aw = links[buffer][w][j][lane], Hw = links[buffer][w][VEC + j][lane];
-                        v[j] = link<STARTS>(Aw, v[j], Hw);
-                        if constexpr (REDUCE) whole[j] *= Aw;
-                    }
-                }
-                buffer ^= 1;
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    v[j] = link<STARTS>(A[j], v[j], H[j]);
-                    whole[j] *= A[j];
-                }
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) enter[j] = v[j];
-        }
-        if constexpr (!REDUCE) {
-            if (p.marks != nullptr && q.active && first % p.span == 0 && first < p.T) {
-                float* mark = p.marks + static_cast<int64_t>(first / p.span) * p.N * p.D + q.cell;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) mark[j] = enter[j];
-            }
-            XT* out = static_cast<XT*>(p.h.p) + static_cast<int64_t>(q.n) * p.h.row + static_cast<int64_t>(first) * p.h.step + q.d;
-#pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const bool dropped = STARTS && (drop >> i & 1u);
-                XV y;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    enter[j] = dropped ? b[i][j] : fmaf(a[i][j], enter[j], b[i][j]);
-                    y.v[j] = from_float<XT>(first + i < q.lim ? enter[j] : 0.0f);
-                }
-                if (first + i < p.T && q.active) *reinterpret_cast<XV*>(out + i * p.h.step) = y;
-            }
-            if constexpr (W == 1) {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) v[j] = enter[j];
-            }
+        for (int j = 0; j < VEC; ++j) {
+            links[wave * 3 * VEC + j][lane] = A[j];
+            links[(wave * 3 + 1) * VEC + j][lane] = R[j];
+            links[(wave * 3 + 2) * VEC + j][lane] = H[j];
         }
     }
-    if (!q.active || wave != 0) return;
-    if constexpr (REDUCE) {
-        const int64_t cells = static_cast<int64_t>(p.N) * p.D;
-        float* to = p.chunks + chunk * 2 * cells + q.cell;
+    __device__ __forceinline__ void write_tile(const Args& p, const Place& q, int t0, int wave, float (*links)[64], float (&v)[VEC]) {
+        const int lane = threadIdx.x & 63, first = t0 + wave * S;
+        float h[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) to[j] = whole[j], to[cells + j] = v[j];
-    } else if (chunk == p.n_chunks - 1) {
+        for (int j = 0; j < VEC; ++j) h[j] = mark[j];
+#pragma unroll 4
+        for (int w = 0; w < wave; ++w) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) h[j] = link<STARTS>(links[w * 3 * VEC + j][lane], h[j], links[(w * 3 + 2) * VEC + j][lane]);
+        }
+        float before[S][VEC];
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                before[i][j] = kept<STARTS>(drop, i, h[j]);
+                h[j] = fmaf(a[i][j], before[i][j], in(i, j));
+            }
+        uint32_t ox[S], og[S];
+#pragma unroll
+        for (int i = S - 1; i >= 0; --i) {
+            float gx[VEC], gg[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float s = v[j] + element<XT>(es[i], j);
+                v[j] = kept<STARTS>(drop, i, a[i][j] * s);
+                gx[j] = LEAKY ? s * rest[i][j] : s;
+                gg[j] = LEAKY ? gx[j] * (a[i][j] * (before[i][j] - element<XT>(xs[i], j))) : s * before[i][j];
+            }
+            ox[i] = word_of<XT, VEC>(gx);
+            og[i] = word_of<XT, VEC>(gg);
+        }
+        store<XT, VEC, S>(p.dx, q, first, p.T, ox);
+        store<XT, VEC, S>(p.dgate, q, first, p.T, og);
+    }
+    __device__ __forceinline__ static int passes(int wave) { return W - 1 - wave; }
+    __device__ __forceinline__ static int wave_at(int k) { return W - 1 - k; }
+};
+
+// A workgroup to a column, from tile to tile.
+template <typename Tile, int VEC, int W, bool STARTS>
+__global__ __launch_bounds__(64 * W) void walk_kernel(Args p) {
+    constexpr int kRows = Tile::kParts * VEC;
+    __shared__ float links[2][W * kRows][64];
+    const Place q = place<VEC>(p, blockIdx.x);
+    const int lane = threadIdx.x & 63, wave = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+    Tile tile;
+    int t0 = Tile::at(p, 0);
+    tile.fetch_tile(p, q, t0, wave);
+    float v[VEC];                       // the value that enters the tile
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = q.active && p.state != nullptr ? p.state[q.cell + j] : 0.0f;
+    for (int order = 0; order < p.tiles; ++order) {
+        tile.decode_tile(q, t0, wave);
+        const int now = t0;
+        if (order + 1 < p.tiles) {
+            t0 = Tile::at(p, order + 1);
+            tile.fetch_tile(p, q, t0, wave);
+        }
+        float(*const shared)[64] = links[order & 1];
+        if constexpr (W > 1) {
+            tile.reduce_tile(shared, wave);
+            __syncthreads();
+            float enter[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) enter[j] = v[j];
+#pragma unroll 4
+            for (int k = 0; k < W; ++k) {
+                if (k == Tile::passes(wave)) {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) enter[j] = v[j];
+                }
+                const int w = Tile::wave_at(k);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[j] = link<STARTS>(shared[w * kRows + j][lane], v[j], shared[w * kRows + VEC + j][lane]);
+            }
+            tile.write_tile(p, q, now, wave, shared, enter);
+        } else {
+            tile.write_tile(p, q, now, 0, shared, v);
+        }
+    }
+    if (q.active && wave == 0) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) p.state_out[q.cell + j] = v[j];
     }
 }
 
-// ------------------------------------------------------------------------------------------------------------------
-// Backward: tiles from the last to the first. REDUCE: only (A, R) of the chunk.
-// ------------------------------------------------------------------------------------------------------------------
-template <typename XT, int VEC, int W, int S, bool STARTS, bool REDUCE>
-__global__ __launch_bounds__(64 * W) void recurrence_backward_kernel(Args p) {
-    constexpr int kParts = REDUCE ? 2 : 3;
-    __shared__ float links[2][W][kParts * VEC][64];
-    const Place q = place<VEC>(p);
+// Workgroups that take tiles as they come, W waves for the elements and VEC more that relay: while those wait for the tiles in front, the
+// others read the next tile.
+template <typename Tile, int VEC, int W, bool STARTS>
+__global__ __launch_bounds__(64 * (W + VEC)) void relay_kernel(Args p) {
+    constexpr int kRows = Tile::kParts * VEC;
+    __shared__ float links[2][W * kRows][64];
+    __shared__ float values[VEC][64];
+    __shared__ uint32_t next_ticket;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int chunk = blockIdx.y + (REDUCE ? 1 : 0);           // nothing lies before the first chunk
-    const int begin = chunk * p.tiles * W * S, end = begin + p.tiles * W * S < p.T ? begin + p.tiles * W * S : p.T;
-    using XV = Pack<XT, VEC>;
-    XV g[S], x[S], dh[S];
-    float mark[VEC];
-    int t0 = begin + (end - begin - 1) / (W * S) * (W * S);
-    const auto fetch_tile = [&](int at) {
-        const int first = at + wave * S;
-        fetch<XT, VEC, S>(g, p.gate, q, first);
-        fetch<XT, VEC, S>(dh, p.dh, q, first);
-        if constexpr (!REDUCE) {
-            fetch<XT, VEC, S>(x, p.x, q, first);
-            const float* from = p.marks + static_cast<int64_t>(at / (W * S)) * p.N * p.D + q.cell;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) mark[j] = q.active ? from[j] : 0.0f;
-        }
-    };
-    fetch_tile(t0);
-    float r[VEC], whole[VEC];           // the gradient that enters the tile from behind
-    if constexpr (REDUCE) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) r[j] = 0.0f, whole[j] = 1.0f;
-    } else {
-        entering<VEC, STARTS, true>(p, q, chunk, r);
-    }
+    const uint32_t total = static_cast<uint32_t>(p.tiles) * static_cast<uint32_t>(p.columns);
+    if (threadIdx.x == 64 * W) next_ticket = atomicAdd(p.ticket, 1u) + 1u;
+    __syncthreads();
+    uint32_t ticket = __builtin_amdgcn_readfirstlane(next_ticket);
+    __syncthreads();                    // before the next one is written
     int buffer = 0;
-    for (; t0 >= begin; t0 -= W * S) {
-        const int first = t0 + wave * S;
-        uint32_t drop = 0;
-        if constexpr (STARTS) drop = start_bits(p, q.n, first, q.lim, S);
-        float a[S][VEC], rest[S][VEC], e[S][VEC], xi[S][VEC], h[VEC];
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-            const bool counts = first + i < q.lim;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                float ai = to_float(g[i].v[j]), ri = 1.0f;
-                if (p.leaky) leak<kPrecise<XT>>(ai, ai, ri);
-                a[i][j] = counts ? ai : 1.0f;
-                rest[i][j] = ri;
-                e[i][j] = counts ? to_float(dh[i].v[j]) : 0.0f;
-                if constexpr (!REDUCE) xi[i][j] = counts ? to_float(x[i].v[j]) : 0.0f;
-            }
+    if (wave >= W) {
+        while (ticket < total) {
+            if (threadIdx.x == 64 * W) next_ticket = atomicAdd(p.ticket, 1u) + 1u;
+            const int order = ticket / p.columns, column = ticket - order * p.columns;
+            const Place q = place<VEC>(p, column);
+            __syncthreads();
+            ticket = __builtin_amdgcn_readfirstlane(next_ticket);
+            float A, H;
+            join<W, STARTS>(&links[buffer][wave - W], kRows, VEC, Tile::wave_at(0) != 0, A, H);
+            values[wave - W][lane] = relay<STARTS>(p, q.active ? q.cell + wave - W : -1, order, A, H);
+            buffer ^= 1;
+            __syncthreads();
         }
-        if constexpr (!REDUCE) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) h[j] = mark[j];
-        }
-        if (t0 > begin) fetch_tile(t0 - W * S);
-        float A[VEC], H[VEC], R[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) A[j] = 1.0f, H[j] = R[j] = 0.0f;
-#pragma unroll
-        for (int i = S - 1; i >= 0; --i) {
-            const bool dropped = STARTS && (drop >> i & 1u);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                R[j] = dropped ? 0.0f : a[i][j] * (R[j] + e[i][j]);
-                A[j] = dropped ? 0.0f : A[j] * a[i][j];
-            }
-        }
-        if constexpr (!REDUCE) {
-#pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const bool dropped = STARTS && (drop >> i & 1u);
-                const bool counts = first + i < q.lim;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const float b = counts ? rest[i][j] * xi[i][j] : 0.0f;
-                    H[j] = dropped ? b : fmaf(a[i][j], H[j], b);
-                }
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            links[buffer][wave][j][lane] = A[j];
-            links[buffer][wave][VEC + j][lane] = R[j];
-            if constexpr (!REDUCE) links[buffer][wave][2 * VEC + j][lane] = H[j];
+        return;
+    }
+    Tile tile;
+    int order = ticket / p.columns;
+    Place q = place<VEC>(p, ticket - order * p.columns);
+    if (ticket < total) tile.fetch_tile(p, q, Tile::at(p, order), wave);
+    while (ticket < total) {
+        const int t0 = Tile::at(p, order);
+        tile.decode_tile(q, t0, wave);
+        tile.reduce_tile(links[buffer], wave);
+        __syncthreads();
+        ticket = __builtin_amdgcn_readfirstlane(next_ticket);
+        const Place here = q;
+        if (ticket < total) {
+            order = ticket / p.columns;
+            q = place<VEC>(p, ticket - order * p.columns);
+            tile.fetch_tile(p, q, Tile::at(p, order), wave);
         }
         __syncthreads();
-        float enter[VEC];
+        float v[VEC];
 #pragma unroll
-        for (int w = W - 1; w >= 0; --w) {
-            if (w == wave) {
+        for (int j = 0; j < VEC; ++j) v[j] = values[j][lane];
+#pragma unroll 4
+        for (int k = 0; k < Tile::passes(wave); ++k) {
+            const int w = Tile::wave_at(k);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) enter[j] = r[j];
-            }
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float Aw = links[buffer][w][j][lane];
-                r[j] = link<STARTS>(Aw, r[j], links[buffer][w][VEC + j][lane]);
-                if constexpr (REDUCE) whole[j] *= Aw;
-            }
+            for (int j = 0; j < VEC; ++j) v[j] = link<STARTS>(links[buffer][w * kRows + j][lane], v[j], links[buffer][w * kRows + VEC + j][lane]);
         }
-        if constexpr (!REDUCE) {
-#pragma unroll
-            for (int w = 0; w < W - 1; ++w)
-                if (w < wave) {
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) h[j] = link<STARTS>(links[buffer][w][j][lane], h[j], links[buffer][w][2 * VEC + j][lane]);
-                }
-            float before[S][VEC];
-#pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const bool dropped = STARTS && (drop >> i & 1u);
-                const bool counts = first + i < q.lim;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    before[i][j] = dropped ? 0.0f : h[j];
-                    h[j] = counts ? fmaf(a[i][j], before[i][j], rest[i][j] * xi[i][j]) : h[j];
-                }
-            }
-            XT* dx = static_cast<XT*>(p.dx.p) + static_cast<int64_t>(q.n) * p.dx.row + static_cast<int64_t>(first) * p.dx.step + q.d;
-            XT* dg = static_cast<XT*>(p.dgate.p) + static_cast<int64_t>(q.n) * p.dgate.row + static_cast<int64_t>(first) * p.dgate.step + q.d;
-#pragma unroll
-            for (int i = S - 1; i >= 0; --i) {
-                const bool dropped = STARTS && (drop >> i & 1u);
-                const bool counts = first + i < q.lim;
-                XV ox, og;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const float s = enter[j] + e[i][j];
-                    const float gx = s * rest[i][j];
-                    const float gg = p.leaky ? gx * (a[i][j] * (before[i][j] - xi[i][j])) : s * before[i][j];
-                    ox.v[j] = from_float<XT>(counts ? gx : 0.0f);
-                    og.v[j] = from_float<XT>(counts ? gg : 0.0f);
-                    enter[j] = dropped ? 0.0f : a[i][j] * s;
-                }
-                if (first + i < p.T && q.active) {
-                    *reinterpret_cast<XV*>(dx + i * p.dx.step) = ox;
-                    *reinterpret_cast<XV*>(dg + i * p.dgate.step) = og;
-                }
-            }
-        }
+        tile.write_tile(p, here, t0, wave, links[buffer], v);
         buffer ^= 1;
     }
-    if (!q.active || wave != 0) return;
-    if constexpr (REDUCE) {
-        const int64_t cells = static_cast<int64_t>(p.N) * p.D;
-        float* to = p.chunks + chunk * 2 * cells + q.cell;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) to[j] = whole[j], to[cells + j] = r[j];
-    } else if (chunk == 0) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) p.state_out[q.cell + j] = r[j];
-    }
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Which variant: waves of a tile, steps of a wave, chunks
+// Which variant
 // ------------------------------------------------------------------------------------------------------------------
 struct Shape {
-    int waves, steps, chunks, tiles;
+    bool relay;
+    int waves, steps;
+    int tile() const { return waves * steps; }
 };
 
-// Waves of a backward tile. The marks lie where these tiles begin: the rule goes by what both passes know, not by alignment.
-int back_waves(int T, int N, int D) { return T <= 32 || static_cast<int64_t>(N) * D >= compute_units() * 1024ll ? 4 : 16; }
-
-Shape shape_of(int T, int N, int D, int64_t columns, bool backward) {
-    Shape s;
+// Relay where columns of 64 * VEC channels are fewer than three quarters of the compute units, and the sequence longer than its way through
+// memory pays for (bf16: 4096 steps, 128 columns, walk 152 us, relay 107; 256 columns 83 and 104; 32 columns, 300 steps 11.3 and 11.6, 600 steps
+// 21.2 and 12.4). The rule goes by what the forward and the backward pass both know, not by alignment: marks lie where backward tiles begin.
+Shape shape_of(int T, int N, int D, int dtype, bool backward) {
     const int units = compute_units();
-    if (!backward && T == 1) {
-        s = {1, 1, 1, 1};
-        return s;
-    }
-    s.steps = backward ? kBackSteps : kSteps;
-    s.waves = backward ? back_waves(T, N, D) : T <= kSteps ? 1 : T <= 2 * kSteps || columns >= units * 8 ? 4 : 16;
-    const int tile = s.waves * s.steps, tiles = (T + tile - 1) / tile;
-    s.chunks = 1;
-    if (s.waves == 16 && columns < units / 2) {
-        const int64_t want = (units + columns - 1) / columns;
-        s.chunks = static_cast<int>(want < tiles ? want : tiles);
-    }
-    s.tiles = (tiles + s.chunks - 1) / s.chunks;
-    s.chunks = (tiles + s.tiles - 1) / s.tiles;
-    return s;
+    const int64_t columns = static_cast<int64_t>(N) * D / (dtype == SNNF_F32 ? 64 : 128);
+    if (!backward && T == 1) return {false, 1, 1};
+    if (!backward && T <= kWalkSteps) return {false, 1, kWalkSteps};
+    if (T > 256 && columns * 4 < units * 3) return {true, kRelayWaves, backward ? kRelayBackSteps : kRelaySteps};
+    return {false, columns < units * 4 ? kWalkWaves : kWalkWavesMany, kWalkSteps};
 }
+int64_t tiles_of(int T, const Shape& s) { return (static_cast<int64_t>(T) + s.tile() - 1) / s.tile(); }
 
-// Channels of a lane: two 16-bit ones where rows allow 4-byte accesses, else one.
-int vector_of(int D, int dtype) { return dtype != SNNF_F32 && D % 2 == 0 && D > 64 ? 2 : 1; }
-int64_t columns_of(int N, int D, int vec) { return static_cast<int64_t>(N) * ((D + 64 * vec - 1) / (64 * vec)); }
-
+// [ticket, in 64 bytes][tile][N * D] runs [tile][N * D] values
 size_t workspace_of(int T, int N, int D, int dtype, bool backward) {
-    // One lane-width more than the call may take gives more chunks, never fewer: the larger of both is enough for either.
-    size_t most = 0;
-    for (int vec = 1; vec <= vector_of(D, dtype); ++vec) {
-        const Shape s = shape_of(T, N, D, columns_of(N, D, vec), backward);
-        const size_t bytes = s.chunks > 1 ? static_cast<size_t>(s.chunks) * 2 * N * D * sizeof(float) : 0;
-        most = bytes > most ? bytes : most;
-    }
-    return most;
+    const Shape s = shape_of(T, N, D, dtype, backward);
+    if (!s.relay) return 0;
+    const size_t words = static_cast<size_t>(tiles_of(T, s)) * N * D * (sizeof(uint64_t) + sizeof(uint32_t));
+    return (words + 15) / 16 * 16 + 64;
 }
 
-template <typename XT, int VEC, int W, int S, bool STARTS>
-int run(Args& p, const Shape& s, int64_t columns, bool backward, hipStream_t stream) {
-    const dim3 block(64 * W);
-    if (backward) {
-        if constexpr (S == kBackSteps) {
-            if (s.chunks > 1) recurrence_backward_kernel<XT, VEC, W, S, STARTS, true><<<dim3(columns, s.chunks - 1), block, 0, stream>>>(p);
-            recurrence_backward_kernel<XT, VEC, W, S, STARTS, false><<<dim3(columns, s.chunks), block, 0, stream>>>(p);
-        }
-    } else {
-        if constexpr (S != kBackSteps) {
-            if constexpr (W > 1)
-                if (s.chunks > 1) recurrence_kernel<XT, VEC, W, S, STARTS, true><<<dim3(columns, s.chunks - 1), block, 0, stream>>>(p);
-            recurrence_kernel<XT, VEC, W, S, STARTS, false><<<dim3(columns, s.chunks), block, 0, stream>>>(p);
+template <typename XT, int VEC, bool STARTS, bool LEAKY, int W, int S>
+void walk(const Args& p, bool backward, hipStream_t stream) {
+    const dim3 grid(p.columns), block(64 * W);
+    if constexpr (W > 1) {
+        if (backward) {
+            walk_kernel<BackwardTile<XT, VEC, W, S, STARTS, LEAKY>, VEC, W, STARTS><<<grid, block, 0, stream>>>(p);
+            return;
         }
     }
-    return check_launch(backward ? "snnf_gated_recurrence_backward" : "snnf_gated_recurrence");
+    walk_kernel<ForwardTile<XT, VEC, W, S, STARTS, LEAKY>, VEC, W, STARTS><<<grid, block, 0, stream>>>(p);
 }
 
-template <typename XT, int VEC, bool STARTS>
+template <typename XT, int VEC, bool STARTS, bool LEAKY>
 int pick(Args& p, bool backward, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    constexpr int dtype = dtype_of<XT>::value;
+    const char* const name = backward ? "snnf_gated_recurrence_backward" : "snnf_gated_recurrence";
+    const Shape s = shape_of(p.T, p.N, p.D, dtype, backward);
     p.groups = (p.D + 64 * VEC - 1) / (64 * VEC);
-    const int64_t columns = static_cast<int64_t>(p.N) * p.groups;
-    if (columns > 0x7fffffffLL) return fail(SNNF_ERR_UNSUPPORTED, "snnf_gated_recurrence: unsupported_shape: N=%d D=%d", p.N, p.D);
-    const Shape s = shape_of(p.T, p.N, p.D, columns, backward);
-    p.span = back_waves(p.T, p.N, p.D) * kBackSteps;
-    p.tiles = s.tiles;
-    p.n_chunks = s.chunks;
-    if (s.chunks > 1) {
-        const size_t need = static_cast<size_t>(s.chunks) * 2 * p.N * p.D * sizeof(float);
-        if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 4))
-            return fail(SNNF_ERR_WORKSPACE, "snnf_gated_recurrence: workspace of %zu bytes needed, got %zu", need, workspace_bytes);
-        p.chunks = static_cast<float*>(workspace);
+    const int64_t columns = static_cast<int64_t>(p.N) * p.groups, tiles = tiles_of(p.T, s);
+    if (columns * (s.relay ? tiles : 1) > 0x7fffffffLL) return fail(SNNF_ERR_UNSUPPORTED, "%s: unsupported_shape: T=%d N=%d D=%d", name, p.T, p.N, p.D);
+    p.columns = static_cast<int>(columns);
+    p.tiles = static_cast<int>(tiles);
+    p.span = shape_of(p.T, p.N, p.D, dtype, true).tile();
+    if (s.relay) {
+        const size_t need = workspace_of(p.T, p.N, p.D, dtype, backward);
+        if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
+            return fail(SNNF_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", name, need, workspace_bytes);
+        p.ticket = static_cast<uint32_t*>(workspace);
+        p.runs = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + 64);
+        p.values = reinterpret_cast<uint32_t*>(p.runs + static_cast<size_t>(tiles) * p.N * p.D);
+        const int64_t words = static_cast<int64_t>(need / 16), fill = (words + 255) / 256;
+        unknown_kernel<<<dim3(static_cast<unsigned>(fill < 2048 ? fill : 2048)), dim3(256), 0, stream>>>(static_cast<uint4*>(workspace), words);
+        // One workgroup to a compute unit: a second one, with half the steps to a tile, doubles the trips through memory.
+        const int64_t units = compute_units();
+        const dim3 grid(static_cast<unsigned>(columns * tiles < units ? columns * tiles : units)), block(64 * (kRelayWaves + VEC));
+        if (backward) relay_kernel<BackwardTile<XT, VEC, kRelayWaves, kRelayBackSteps, STARTS, LEAKY>, VEC, kRelayWaves, STARTS><<<grid, block, 0, stream>>>(p);
+        else relay_kernel<ForwardTile<XT, VEC, kRelayWaves, kRelaySteps, STARTS, LEAKY>, VEC, kRelayWaves, STARTS><<<grid, block, 0, stream>>>(p);
+    } else if (s.waves == kWalkWaves) {
+        walk<XT, VEC, STARTS, LEAKY, kWalkWaves, kWalkSteps>(p, backward, stream);
+    } else if (s.waves == kWalkWavesMany) {
+        walk<XT, VEC, STARTS, LEAKY, kWalkWavesMany, kWalkSteps>(p, backward, stream);
+    } else if (s.steps == 1) {
+        walk<XT, VEC, STARTS, LEAKY, 1, 1>(p, false, stream);
+    } else {
+        walk<XT, VEC, STARTS, LEAKY, 1, kWalkSteps>(p, false, stream);
     }
-    if (backward) return s.waves == 16 ? run<XT, VEC, 16, kBackSteps, STARTS>(p, s, columns, true, stream) : run<XT, VEC, 4, kBackSteps, STARTS>(p, s, columns, true, stream);
-    if (s.steps == 1) return run<XT, VEC, 1, 1, STARTS>(p, s, columns, false, stream);
-    if (s.waves == 1) return run<XT, VEC, 1, kSteps, STARTS>(p, s, columns, false, stream);
-    return s.waves == 16 ? run<XT, VEC, 16, kSteps, STARTS>(p, s, columns, false, stream) : run<XT, VEC, 4, kSteps, STARTS>(p, s, columns, false, stream);
+    return check_launch(name);
 }
 
-template <typename XT>
-int launch(Args& p, bool pairs, bool backward, void* workspace, size_t workspace_bytes, hipStream_t stream) {
-    if constexpr (sizeof(XT) == 2) {
-        if (pairs)
-            return p.starts != nullptr ? pick<XT, 2, true>(p, backward, workspace, workspace_bytes, stream) : pick<XT, 2, false>(p, backward, workspace, workspace_bytes, stream);
-    }
-    return p.starts != nullptr ? pick<XT, 1, true>(p, backward, workspace, workspace_bytes, stream) : pick<XT, 1, false>(p, backward, workspace, workspace_bytes, stream);
+template <typename XT, int VEC>
+int launch(Args& p, bool leaky, bool backward, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    if (leaky)
+        return p.starts != nullptr ? pick<XT, VEC, true, true>(p, backward, workspace, workspace_bytes, stream)
+                                   : pick<XT, VEC, false, true>(p, backward, workspace, workspace_bytes, stream);
+    return p.starts != nullptr ? pick<XT, VEC, true, false>(p, backward, workspace, workspace_bytes, stream)
+                               : pick<XT, VEC, false, false>(p, backward, workspace, workspace_bytes, stream);
 }
 
 bool pairs_fit(const void* p, int64_t step, int64_t row) { return aligned_to(p, 4) && step % 2 == 0 && row % 2 == 0; }
 
-int dispatch(Args& p, int dtype, bool backward, void* workspace, size_t workspace_bytes, void* stream) {
+int dispatch(Args& p, int dtype, bool leaky, bool backward, void* workspace, size_t workspace_bytes, void* stream) {
     if (p.T > kMostSteps) return fail(SNNF_ERR_UNSUPPORTED, "snnf_gated_recurrence: unsupported_temporal_length: at most %d steps, got %d", kMostSteps, p.T);
-    bool pairs = vector_of(p.D, dtype) == 2 && pairs_fit(p.x.p, p.x.step, p.x.row) && pairs_fit(p.gate.p, p.gate.step, p.gate.row);
+    const int64_t size = dtype_size(dtype), run = p.T < kRelaySteps ? p.T : kRelaySteps;
+    for (int64_t* step : {&p.x.step, &p.gate.step, &p.dh.step, &p.h.step, &p.dx.step, &p.dgate.step}) {
+        if (p.T == 1) *step = 0;        // what the stride of a single step is says nothing
+        if (*step < 0 || *step > kBufferBytes || (*step * (run - 1) + p.D) * size >= kBufferBytes)
+            return fail(SNNF_ERR_UNSUPPORTED, "snnf_gated_recurrence: unsupported_stride: %d steps of %lld elements pass 2 GiB", static_cast<int>(run), (long long)*step);
+    }
+    // Two 16-bit channels to a lane where rows allow 4-byte accesses.
+    bool pairs = dtype != SNNF_F32 && p.D % 2 == 0 && p.D > 64 && pairs_fit(p.x.p, p.x.step, p.x.row) && pairs_fit(p.gate.p, p.gate.step, p.gate.row);
     if (backward)
         pairs = pairs && pairs_fit(p.dh.p, p.dh.step, p.dh.row) && pairs_fit(p.dx.p, p.dx.step, p.dx.row) && pairs_fit(p.dgate.p, p.dgate.step, p.dgate.row);
     else
         pairs = pairs && pairs_fit(p.h.p, p.h.step, p.h.row);
     hipStream_t hs = as_stream(stream);
-    if (dtype == SNNF_F32) return launch<float>(p, false, backward, workspace, workspace_bytes, hs);
-    if (dtype == SNNF_BF16) return launch<bf16_t>(p, pairs, backward, workspace, workspace_bytes, hs);
-    return launch<f16_t>(p, pairs, backward, workspace, workspace_bytes, hs);
+    if (dtype == SNNF_F32) return launch<float, 1>(p, leaky, backward, workspace, workspace_bytes, hs);
+    if (dtype == SNNF_BF16)
+        return pairs ? launch<bf16_t, 2>(p, leaky, backward, workspace, workspace_bytes, hs) : launch<bf16_t, 1>(p, leaky, backward, workspace, workspace_bytes, hs);
+    return pairs ? launch<f16_t, 2>(p, leaky, backward, workspace, workspace_bytes, hs) : launch<f16_t, 1>(p, leaky, backward, workspace, workspace_bytes, hs);
 }
 
 }  // namespace
@@ -563,10 +724,9 @@ extern "C" size_t snnf_gated_recurrence_workspace_bytes(int T, int N, int D, int
     return workspace_of(T, N, D, dtype, backward != 0);
 }
 
-extern "C" size_t snnf_gated_recurrence_marks_bytes(int T, int N, int D) {
-    if (T < 1 || N < 1 || D < 1) return 0;
-    const int span = back_waves(T, N, D) * kBackSteps;
-    return (static_cast<size_t>(T) + span - 1) / span * N * D * sizeof(float);
+extern "C" size_t snnf_gated_recurrence_marks_bytes(int T, int N, int D, int dtype) {
+    if (T < 1 || N < 1 || D < 1 || !valid_dtype(dtype)) return 0;
+    return static_cast<size_t>(tiles_of(T, shape_of(T, N, D, dtype, true))) * N * D * sizeof(float);
 }
 
 extern "C" int snnf_gated_recurrence(const void* x, int64_t x_step, int64_t x_row, const void* gate, int64_t gate_step, int64_t gate_row, int T, int N,
@@ -592,8 +752,7 @@ extern "C" int snnf_gated_recurrence(const void* x, int64_t x_step, int64_t x_ro
     p.state_out = state_out;
     p.marks = marks;
     p.T = T, p.N = N, p.D = D;
-    p.leaky = form == SNNF_RECURRENCE_LEAKY;
-    return dispatch(p, dtype, false, workspace, workspace_bytes, stream);
+    return dispatch(p, dtype, form == SNNF_RECURRENCE_LEAKY, false, workspace, workspace_bytes, stream);
 }
 
 extern "C" int snnf_gated_recurrence_backward(const void* x, int64_t x_step, int64_t x_row, const void* gate, int64_t gate_step, int64_t gate_row,
@@ -622,6 +781,5 @@ extern "C" int snnf_gated_recurrence_backward(const void* x, int64_t x_step, int
     p.state = dstate;
     p.state_out = dstate_in;
     p.T = T, p.N = N, p.D = D;
-    p.leaky = form == SNNF_RECURRENCE_LEAKY;
-    return dispatch(p, dtype, true, workspace, workspace_bytes, stream);
+    return dispatch(p, dtype, form == SNNF_RECURRENCE_LEAKY, true, workspace, workspace_bytes, stream);
 }

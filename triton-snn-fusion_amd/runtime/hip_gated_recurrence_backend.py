@@ -68,7 +68,7 @@ def _forward(x, gate, state, form: int, starts, lengths, keep_marks: bool):
     with on_device_of(x):
         h = _empty_like_steps(x)
         last = torch.empty((N, D), dtype=torch.float32, device=x.device)
-        marks = torch.empty(lib.snnf_gated_recurrence_marks_bytes(T, N, D) // 4, dtype=torch.float32, device=x.device) if keep_marks else None
+        marks = torch.empty(lib.snnf_gated_recurrence_marks_bytes(T, N, D, code) // 4, dtype=torch.float32, device=x.device) if keep_marks else None
         nbytes = lib.snnf_gated_recurrence_workspace_bytes(T, N, D, code, 0)
         space = workspace(nbytes, x)
         _lib.check("snnf_gated_recurrence", lib.snnf_gated_recurrence(
