@@ -482,6 +482,39 @@ int snnf_gated_recurrence_backward(const void* x, int64_t x_step, int64_t x_row,
                                    void* dx, int64_t dx_step, int64_t dx_row, void* dgate, int64_t dgate_step, int64_t dgate_row, float* dstate_in,
                                    void* workspace, size_t workspace_bytes, void* stream);
 
+typedef enum snnf_norm_kind {
+    SNNF_NORM_RMS = 0,           /* x / sqrt(mean(x^2) + eps) */
+    SNNF_NORM_LAYER = 1          /* the same after the mean is taken out */
+} snnf_norm_kind;
+
+typedef enum snnf_gate_form {
+    SNNF_GATE_NONE = 0,
+    SNNF_GATE_SIGMOID = 1,
+    SNNF_GATE_SILU = 2           /* gate * sigmoid(gate) */
+} snnf_gate_form;
+
+/* Norms behind and in front of a block with its gate, scale and residual, over rows of D <= 16384 elements:
+ *     residual_out = residual + factor * scale * act(gate) * norm(branch) * branch_weight,   normed = norm(residual_out) * next_weight
+ * Inputs have elements of a row next to each other and rows `*_row` elements apart; outputs have rows next to each other and overlap no input.
+ *   branch     NULL: residual_out is the residual (and not written), gate_form is SNNF_GATE_NONE
+ *   branch_weight, next_weight, scale   [D] of `vector_dtype` (the activations' dtype or float32), or NULL: ones
+ *   residual and residual_out are of `residual_dtype`: the activations' dtype or float32
+ *   stats      NULL, or 4 * rows floats (16-byte aligned) that the backward pass will read */
+int snnf_block_norm(const void* residual, int64_t residual_row, const void* branch, int64_t branch_row, const void* gate, int64_t gate_row,
+                    const void* branch_weight, const void* next_weight, const void* scale, float factor, int64_t rows, int D, int residual_dtype,
+                    int dtype, int vector_dtype, int kind, int gate_form, float eps, void* residual_out, void* normed, float* stats, void* stream);
+
+/* Its gradient. d_residual_out and d_normed are the gradients of the outputs (NULL: zeros); d_residual, d_branch and d_gate are written for the
+ * operands that are there, rows next to each other; d_branch_weight, d_next_weight and d_scale, of `vector_dtype`, may be NULL. rows >= 1.
+ * Workspace: snnf_block_norm_backward_workspace_bytes(rows, D) bytes, 16-byte aligned. Two launches; the sums over rows have a fixed order. */
+size_t snnf_block_norm_backward_workspace_bytes(int64_t rows, int D);
+int snnf_block_norm_backward(const void* residual, int64_t residual_row, const void* branch, int64_t branch_row, const void* gate, int64_t gate_row,
+                             const void* branch_weight, const void* next_weight, const void* scale, float factor, const void* d_residual_out,
+                             int64_t d_residual_out_row, const void* d_normed, int64_t d_normed_row, const float* stats, int64_t rows, int D,
+                             int residual_dtype, int dtype, int vector_dtype, int kind, int gate_form, void* d_residual, void* d_branch,
+                             void* d_gate, void* d_branch_weight, void* d_next_weight, void* d_scale, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
 #ifdef __cplusplus
 }
 #endif

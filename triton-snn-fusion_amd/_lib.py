@@ -75,6 +75,10 @@ SIGNATURES = {
     "snnf_gated_recurrence": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _i, _i, _i, _i, _i, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _sz, _vp]),
     "snnf_gated_recurrence_backward": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i, _i, _i, _i, _i, _vp, _i64, _i64, _vp, _vp, _vp,
                                             _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _sz, _vp]),
+    "snnf_block_norm": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _f, _i64, _i, _i, _i, _i, _i, _i, _f, _vp, _vp, _vp, _vp]),
+    "snnf_block_norm_backward_workspace_bytes": (_sz, [_i64, _i]),
+    "snnf_block_norm_backward": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _f, _vp, _i64, _vp, _i64, _vp, _i64, _i, _i, _i, _i, _i, _i,
+                                      _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "snnf_conv_bias": (_i, [_pp, _pp, _i, _i, _i, _i, _i, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _i64, _vp]),
 }
 

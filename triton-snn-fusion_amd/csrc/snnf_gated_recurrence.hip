@@ -15,7 +15,7 @@
 // backwards; dx = s (1 - a) or s, dg = s (h_{t-1} - x) a (1 - a) or s h_{t-1}. h_{t-1} is not read but worked out again from the
 // float32 state that the forward pass leaves where each tile of the backward pass begins ("marks"): less to read than h itself, and no
 // rounding of h to 16 bits enters the gradient.
-#include "snnf_common.h"
+#include "snnf_sequence.h"
 
 namespace snnf {
 namespace {
@@ -58,28 +58,6 @@ struct Args {
     int tiles;
     int span;                           // steps from one mark to the next
 };
-
-template <typename XT> constexpr bool kPrecise = false;
-template <> constexpr bool kPrecise<float> = true;
-
-// a = sigmoid(g) = 1 / (1 + e) and 1 - a = e / (1 + e) with e = exp(-g), both to full relative accuracy; a NaN stays one, and a gate of
-// infinity gives a = 1 and 1 - a = 0 exactly. e is kept from overflowing. v_exp_f32 works on powers of two; for float32 tensors what the
-// product with log2(e) loses is put back to first order.
-template <bool PRECISE>
-__device__ __forceinline__ void leak(float g, float& a, float& rest) {
-    constexpr float kLog2e = 1.44269504088896340736f, kLog2eLow = 1.925963033500e-8f, kLn2 = 0.69314718055994530942f;
-    float e;
-    if constexpr (PRECISE) {
-        const float y = __builtin_elementwise_minimum(__builtin_elementwise_maximum(g, -86.0f), 200.0f);
-        const float t = y * -kLog2e;
-        e = __builtin_amdgcn_exp2f(t);
-        e = fmaf(e, fmaf(y, -kLog2eLow, fmaf(y, -kLog2e, -t)) * kLn2, e);
-    } else {
-        e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(g * -kLog2e, 124.0f));
-    }
-    a = __builtin_amdgcn_rcpf(1.0f + e);
-    rest = e * a;
-}
 
 // Lane i: whether the state is dropped before step `first` + i.
 __device__ __forceinline__ uint8_t start_of(const Args& p, int n, int first, int lim, int steps) {
@@ -142,22 +120,11 @@ __device__ __forceinline__ void write(__amdgpu_buffer_rsrc_t to, uint32_t word, 
     if constexpr (sizeof(XT) * VEC == 4) __builtin_amdgcn_raw_buffer_store_b32(word, to, lane_bytes, step_bytes, 0);
     else __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(word), to, lane_bytes, step_bytes, 0);
 }
-template <typename XT>
-__device__ __forceinline__ float element(uint32_t word, int j) {
-    if constexpr (sizeof(XT) == 4) return __uint_as_float(word);
-    else if constexpr (dtype_of<XT>::value == SNNF_BF16) return __uint_as_float(j == 0 ? word << 16 : word & 0xffff0000u);
-    else return f16_bits_to_float(j == 0 ? word & 0xffffu : word >> 16);
-}
 template <typename XT, int VEC>
 __device__ __forceinline__ uint32_t word_of(const float (&v)[VEC]) {
     if constexpr (sizeof(XT) == 4) return __float_as_uint(v[0]);
-    else if constexpr (dtype_of<XT>::value == SNNF_BF16) {
-        if constexpr (VEC == 2) return float_to_bf16_pair(v[0], v[1]);
-        else return float_to_bf16_bits(v[0]);
-    } else {
-        if constexpr (VEC == 2) return float_to_f16_bits(v[0]) | float_to_f16_bits(v[1]) << 16;
-        else return float_to_f16_bits(v[0]);
-    }
+    else if constexpr (VEC == 2) return pair_word<XT>(v[0], v[1]);
+    else return from_float<XT>(v[0]).bits;
 }
 
 // The elements of S steps from `first` on. Steps that do not count are read from the last that does (from the first if there is none).
