@@ -515,6 +515,23 @@ int snnf_block_norm_backward(const void* residual, int64_t residual_row, const v
                              void* d_gate, void* d_branch_weight, void* d_next_weight, void* d_scale, void* workspace, size_t workspace_bytes,
                              void* stream);
 
+/* Scores of one given token a row of logits, rows of V elements next to each other, `row` elements apart:
+ *     logprob[r] = log softmax(row)[token], 0 where `tokens` is NULL or the token lies outside [0, V);   entropy[r] = -sum p log p
+ *     top_logprob, top_token   [rows, top_k]: the most likely alternatives, equal ones by the lower index; top_k <= 64 and <= V
+ *     stats                    NULL, or 2 * rows floats (8-byte aligned) that the backward pass will read
+ * Logits of minus infinity are masked; a row of nothing else has logprob -inf, entropy 0 and no gradient. A NaN or plus infinity makes the
+ * row's scores NaN; as an alternative a NaN comes last. Workspace: snnf_token_scores_workspace_bytes(...) bytes (0: none needed), 16-byte
+ * aligned. Two launches where rows are few and long, else one. */
+size_t snnf_token_scores_workspace_bytes(int64_t rows, int V, int top_k);
+int snnf_token_scores(const void* logits, int64_t row, int64_t rows, int V, int dtype, const int64_t* tokens, int top_k, float* logprob,
+                      float* entropy, float* top_logprob, int64_t* top_token, float* stats, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* Gradient of the logits, rows next to each other, from those of logprob and entropy (NULL: zeros); `stats` and `entropy` as the forward call
+ * left them. */
+int snnf_token_scores_backward(const void* logits, int64_t row, int64_t rows, int V, int dtype, const int64_t* tokens, const float* stats,
+                               const float* entropy, const float* d_logprob, const float* d_entropy, void* d_logits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

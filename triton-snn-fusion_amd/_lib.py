@@ -79,6 +79,9 @@ SIGNATURES = {
     "snnf_block_norm_backward_workspace_bytes": (_sz, [_i64, _i]),
     "snnf_block_norm_backward": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _f, _vp, _i64, _vp, _i64, _vp, _i64, _i, _i, _i, _i, _i, _i,
                                       _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "snnf_token_scores_workspace_bytes": (_sz, [_i64, _i, _i]),
+    "snnf_token_scores": (_i, [_vp, _i64, _i64, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "snnf_token_scores_backward": (_i, [_vp, _i64, _i64, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "snnf_conv_bias": (_i, [_pp, _pp, _i, _i, _i, _i, _i, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _i64, _vp]),
 }
 

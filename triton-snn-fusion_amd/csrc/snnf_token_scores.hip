@@ -1,0 +1,416 @@
+// Scores of given tokens: log probability, entropy of the row, the most likely alternatives, and the gradient of the first two.
+//     M = max x, s = sum exp(x - M), t = sum exp(x - M) (x - M);   logprob = (x_token - M) - log s,   entropy = log s - t / s
+//     d x_i = d_logprob (1[i = token] - p_i) - d_entropy p_i (log p_i + entropy)
+// One pass over the logits: every thread keeps (M, s, t) of its elements, rescaled when a batch brings a larger maximum, and the workgroup joins
+// them in a fixed order. Bound by memory with some 40 % of the issue slots free (v_exp_f32 is a quarter of them).
+// Alternatives: the threads' maxima, as 64 groups by lane, give a value that at least k elements reach (their k-th largest), and only threads
+// whose own maximum reaches it look through their elements again, which the caches still hold; a few dozen candidates are ranked by counting.
+// Ties go to the lower index: an element's key is its value, in an order of unsigned numbers, above the complement of its index.
+#include "snnf_sequence.h"
+
+namespace snnf {
+namespace {
+
+constexpr int kMostAlternatives = 64;
+constexpr int kCandidates = 1024;       // candidates that are ranked at once; rows with more (many equal values) select one by one
+constexpr int kBatch = 4;               // vectors a thread has in flight
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+struct ScoreArgs {
+    const void* logits;
+    int64_t row;                        // elements from one row to the next
+    int64_t rows;
+    int V, k;
+    int splits, span;                   // workgroups to a row, elements of each
+    const int64_t* tokens;
+    float *logprob, *entropy, *top_logprob;
+    int64_t* top_token;
+    float2* stats;                      // M, s
+    float4* parts;                      // [row][split] M, s, t
+    uint64_t* keys;                     // [row][split][k]
+    const float2* saved;
+    const float *saved_entropy, *d_logprob, *d_entropy;
+    void* d_logits;
+};
+
+template <typename T> constexpr int kVec = sizeof(T) == 4 ? 4 : 8;
+
+// M, s and t (in powers of two: t = sum e z with e = 2^z) of some elements.
+struct Stats {
+    float M, s, t;
+};
+// (x - M) in powers of two, kept where 2^z is 0 and z times it as well: masked elements are minus infinity.
+__device__ __forceinline__ float exponent(float x, float M) { return __builtin_elementwise_maximum((x - M) * kLog2e, -200.0f); }
+// What is subtracted where nothing but minus infinity has been seen.
+__device__ __forceinline__ float center(float M) { return M == -INFINITY ? 0.0f : M; }
+
+__device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
+    const float M = fmaxf(a.M, b.M), c = center(M);
+    const float za = exponent(a.M, c), zb = exponent(b.M, c);
+    const float fa = __builtin_amdgcn_exp2f(za), fb = __builtin_amdgcn_exp2f(zb);
+    return {M, a.s * fa + b.s * fb, fa * fmaf(za, a.s, a.t) + fb * fmaf(zb, b.s, b.t)};
+}
+
+template <int BLOCK>
+__device__ __forceinline__ Stats join_all(Stats v) {
+    __shared__ Stats shared[BLOCK / 64];
+#pragma unroll
+    for (int mask = 1; mask < 64; mask <<= 1) {
+        const Stats other{__shfl_xor(v.M, mask, 64), __shfl_xor(v.s, mask, 64), __shfl_xor(v.t, mask, 64)};
+        v = (threadIdx.x & mask) ? join(other, v) : join(v, other);
+    }
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = shared[0];
+    for (int w = 1; w < BLOCK / 64; ++w) v = join(v, shared[w]);
+    return v;
+}
+
+__device__ __forceinline__ uint32_t order_of(float x) {
+    const uint32_t bits = __float_as_uint(x);
+    if (x != x) return 0;               // a NaN comes last
+    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_float(order == 0 ? 0x7fc00000u : (order & 0x80000000u ? order & 0x7fffffffu : ~order)); }
+// -0 and 0 are the same value.
+__device__ __forceinline__ uint64_t key_of(float x, int index) { return static_cast<uint64_t>(order_of(x + 0.0f)) << 32 | static_cast<uint32_t>(~index); }
+
+template <typename T>
+__device__ __forceinline__ void load_vector(float (&v)[kVec<T>], const T* row, int at, int end) {
+    constexpr int VEC = kVec<T>;
+    if (at + VEC <= end) {
+        const auto w = *reinterpret_cast<const typename Words<T, VEC>::type*>(row + at);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            if constexpr (sizeof(T) == 4) v[j] = element<T>(w[j], 0);
+            else v[j] = element<T>(w[j / 2], j % 2);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = at + j < end ? to_float(row[at + j]) : -INFINITY;
+    }
+}
+
+// The k largest keys among `count` in LDS, in order, to `out`.
+template <int BLOCK>
+__device__ __forceinline__ void rank_keys(const uint64_t* keys, int count, int k, uint64_t* out) {
+    for (int i = threadIdx.x; i < count; i += BLOCK) {
+        const uint64_t mine = keys[i];
+        int rank = 0;
+        for (int j = 0; j < count; ++j) rank += keys[j] > mine ? 1 : 0;
+        if (rank < k) out[rank] = mine;
+    }
+}
+
+// The k largest keys of a workgroup's elements. `most`: the thread's own largest value.
+template <typename T, int BLOCK>
+__device__ __forceinline__ void alternatives(const T* row, int begin, int end, int k, float most, uint64_t* out) {
+    constexpr int VEC = kVec<T>, WAVES = BLOCK / 64;
+    __shared__ float maxima[WAVES][64];
+    __shared__ float reached;
+    __shared__ int count;
+    __shared__ uint64_t candidates[kCandidates];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    maxima[wave][lane] = most;
+    if (threadIdx.x == 0) count = 0;
+    __syncthreads();
+    if (wave == 0) {
+        float group = maxima[0][lane];
+        for (int w = 1; w < WAVES; ++w) group = fmaxf(group, maxima[w][lane]);
+        int rank = 0;
+#pragma unroll
+        for (int j = 0; j < 64; ++j) {
+            const float other = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(group), j));
+            rank += other > group || (other == group && j < lane) ? 1 : 0;
+        }
+        if (rank == k - 1) reached = group;
+    }
+    __syncthreads();
+    const float bound = reached;
+    if (most >= bound && bound > -INFINITY) {
+        for (int at = begin + static_cast<int>(threadIdx.x) * VEC; at < end; at += BLOCK * VEC) {
+            float v[VEC];
+            load_vector<T>(v, row, at, end);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (v[j] >= bound) {
+                    const int to = atomicAdd(&count, 1);
+                    if (to < kCandidates) candidates[to] = key_of(v[j], at + j);
+                }
+        }
+    }
+    __syncthreads();
+    const int found = count;
+    if (found >= k && found <= kCandidates) {
+        rank_keys<BLOCK>(candidates, found, k, out);
+        return;
+    }
+    // Few elements that count, or many equal ones: the largest key below the last, k times.
+    uint64_t last = ~0ull;
+    for (int i = 0; i < k; ++i) {
+        uint64_t best = 0;
+        for (int at = begin + static_cast<int>(threadIdx.x) * VEC; at < end; at += BLOCK * VEC) {
+            float v[VEC];
+            load_vector<T>(v, row, at, end);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const uint64_t key = key_of(v[j], at + j);
+                if (at + j < end && key < last && key > best) best = key;
+            }
+        }
+#pragma unroll
+        for (int mask = 32; mask > 0; mask >>= 1) {
+            const uint64_t other = static_cast<uint64_t>(__shfl_xor(static_cast<uint32_t>(best >> 32), mask, 64)) << 32 | __shfl_xor(static_cast<uint32_t>(best), mask, 64);
+            best = other > best ? other : best;
+        }
+        __syncthreads();
+        if (lane == 0) candidates[wave] = best;
+        __syncthreads();
+        for (int w = 0; w < WAVES; ++w) best = candidates[w] > best ? candidates[w] : best;
+        if (threadIdx.x == 0) out[i] = best;
+        last = best;
+    }
+}
+
+// Scores of a row from its statistics and its k keys.
+template <typename T>
+__device__ __forceinline__ void finish(const ScoreArgs& p, int64_t r, const Stats& v, const uint64_t* keys) {
+    const bool none = v.s == 0.0f;              // nothing is left of the row
+    const float log_s = none ? 0.0f : logf(v.s);
+    if (threadIdx.x == 0) {
+        const int64_t token = p.tokens == nullptr ? -1 : p.tokens[r];
+        float logprob = 0.0f;
+        if (token >= 0 && token < p.V) logprob = none ? -INFINITY : (to_float(static_cast<const T*>(p.logits)[r * p.row + token]) - v.M) - log_s;
+        p.logprob[r] = logprob;
+        p.entropy[r] = none ? 0.0f : log_s - kLn2 * (v.t / v.s);
+        if (p.stats != nullptr) p.stats[r] = make_float2(v.M, v.s);
+    }
+    if (static_cast<int>(threadIdx.x) < p.k) {
+        const uint64_t key = keys[threadIdx.x];
+        p.top_token[r * p.k + threadIdx.x] = static_cast<int64_t>(~static_cast<uint32_t>(key));
+        p.top_logprob[r * p.k + threadIdx.x] = none ? -INFINITY : (value_of(static_cast<uint32_t>(key >> 32)) - v.M) - log_s;
+    }
+}
+
+template <typename T, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void token_scores_kernel(ScoreArgs p) {
+    constexpr int VEC = kVec<T>;
+    __shared__ uint64_t top[kMostAlternatives];
+    const int64_t r = blockIdx.x / p.splits;
+    const int split = static_cast<int>(blockIdx.x - r * p.splits), begin = split * p.span, end = begin + p.span < p.V ? begin + p.span : p.V;
+    const T* row = static_cast<const T*>(p.logits) + r * p.row;
+    Stats mine{-INFINITY, 0.0f, 0.0f};
+    for (int at = begin + static_cast<int>(threadIdx.x) * VEC; at < end; at += kBatch * BLOCK * VEC) {
+        float v[kBatch][VEC];
+        float most = mine.M;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) load_vector<T>(v[u], row, at + u * BLOCK * VEC, end);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) most = fmaxf(most, v[u][j]);
+        const float c = center(most), z = exponent(mine.M, c), f = __builtin_amdgcn_exp2f(z);
+        mine.t = f * fmaf(z, mine.s, mine.t);
+        mine.s *= f;
+        mine.M = most;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float zj = exponent(v[u][j], c), e = __builtin_amdgcn_exp2f(zj);
+                mine.s += e;
+                mine.t = fmaf(e, zj, mine.t);
+            }
+    }
+    const Stats all = join_all<BLOCK>(mine);
+    if (p.k > 0) {
+        alternatives<T, BLOCK>(row, begin, end, p.k, mine.M, top);
+        __syncthreads();
+    }
+    if (p.splits == 1) {
+        finish<T>(p, r, all, top);
+        return;
+    }
+    if (threadIdx.x == 0) p.parts[blockIdx.x] = make_float4(all.M, all.s, all.t, 0.0f);
+    if (static_cast<int>(threadIdx.x) < p.k) p.keys[static_cast<int64_t>(blockIdx.x) * p.k + threadIdx.x] = top[threadIdx.x];
+}
+
+// Joins the splits of a row: one workgroup of 256 threads.
+constexpr int kMostSplits = 32;
+template <typename T>
+__global__ __launch_bounds__(256) void join_scores_kernel(ScoreArgs p) {
+    __shared__ uint64_t candidates[kMostSplits * kMostAlternatives], top[kMostAlternatives];
+    __shared__ int count;
+    const int64_t r = blockIdx.x;
+    const float4 first = p.parts[r * p.splits];
+    Stats all{first.x, first.y, first.z};
+    for (int i = 1; i < p.splits; ++i) {
+        const float4 part = p.parts[r * p.splits + i];
+        all = join(all, Stats{part.x, part.y, part.z});
+    }
+    if (p.k > 0) {
+        // Whatever is smaller than some split's k-th key has k larger ones.
+        const uint64_t* keys = p.keys + r * p.splits * p.k;
+        uint64_t bound = 0;
+        for (int i = 0; i < p.splits; ++i) bound = keys[i * p.k + p.k - 1] > bound ? keys[i * p.k + p.k - 1] : bound;
+        if (threadIdx.x == 0) count = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < p.splits * p.k; i += 256)
+            if (keys[i] >= bound) candidates[atomicAdd(&count, 1)] = keys[i];
+        __syncthreads();
+        rank_keys<256>(candidates, count, p.k, top);
+        __syncthreads();
+    }
+    finish<T>(p, r, all, top);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void token_scores_backward_kernel(ScoreArgs p) {
+    constexpr int VEC = kVec<T>;
+    const int64_t r = blockIdx.x / p.splits;
+    const int begin = static_cast<int>(blockIdx.x - r * p.splits) * p.span, end = begin + p.span < p.V ? begin + p.span : p.V;
+    const T* row = static_cast<const T*>(p.logits) + r * p.row;
+    T* out = static_cast<T*>(p.d_logits) + r * p.V;
+    const float2 stats = p.saved[r];
+    const int64_t token = p.tokens == nullptr ? -1 : p.tokens[r];
+    const bool given = token >= 0 && token < p.V && p.d_logprob != nullptr;
+    const float g = given ? p.d_logprob[r] : 0.0f, h = p.d_entropy != nullptr ? p.d_entropy[r] : 0.0f;
+    const bool none = stats.y == 0.0f;
+    const float c = center(stats.x), inverse = none ? 0.0f : 1.0f / stats.y;
+    // -p (g + h (log p + entropy)) with log p = ln2 z - log s
+    const float constant = none ? 0.0f : fmaf(h, p.saved_entropy[r] - logf(stats.y), g), slope = h * kLn2;
+    for (int at = begin + static_cast<int>(threadIdx.x) * VEC; at < end; at += 256 * VEC) {
+        float v[VEC];
+        load_vector<T>(v, row, at, end);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float z = exponent(v[j], c), probability = __builtin_amdgcn_exp2f(z) * inverse;
+            v[j] = -probability * fmaf(slope, z, constant);
+            if (given && !none && at + j == token) v[j] += g;
+        }
+        if (at + VEC <= end) {
+            typename Words<T, VEC>::type w;
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) w[j] = __float_as_uint(v[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; j += 2) w[j / 2] = pair_word<T>(v[j], v[j + 1]);
+            }
+            *reinterpret_cast<typename Words<T, VEC>::type*>(out + at) = w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (at + j < end) out[at + j] = from_float<T>(v[j]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// Launch
+// ------------------------------------------------------------------------------------------------------------------
+struct ScoreShape {
+    int block, splits, span;
+};
+
+// A workgroup to a row: 256 threads where there are rows enough to fill the chip or few elements, else 1024. Few long rows are split.
+ScoreShape score_shape(int64_t rows, int V) {
+    const int64_t units = compute_units();
+    ScoreShape s{rows >= units * 2 || V <= 8192 ? 256 : 1024, 1, V};
+    if (rows < units && V > 64 * 1024) {
+        int64_t splits = units / rows;
+        const int64_t useful = V / (16 * 1024);
+        splits = splits < useful ? splits : useful;
+        splits = splits < kMostSplits ? splits : kMostSplits;
+        if (splits > 1) {
+            s.span = static_cast<int>(((V + splits - 1) / splits + 1023) / 1024 * 1024);
+            s.splits = (V + s.span - 1) / s.span;
+        }
+    }
+    return s;
+}
+
+int check_scores(const char* name, int64_t rows, int V, int dtype, int k) {
+    if (rows < 0 || V < 1 || k < 0) return fail(SNNF_ERR_INVALID_ARGUMENT, "%s: rows=%lld V=%d top_k=%d", name, (long long)rows, V, k);
+    if (V > (1 << 30)) return fail(SNNF_ERR_UNSUPPORTED, "%s: unsupported_shape: rows of at most 2^30 elements", name);
+    if (k > V || k > kMostAlternatives)
+        return fail(SNNF_ERR_UNSUPPORTED, "%s: unsupported_top_k: at most %d alternatives and no more than elements, got %d of %d", name, kMostAlternatives, k, V);
+    if (!valid_dtype(dtype)) return fail(SNNF_ERR_INVALID_ARGUMENT, "%s: unknown dtype code %d", name, dtype);
+    return SNNF_OK;
+}
+
+template <typename T>
+void launch_scores(const ScoreArgs& p, const ScoreShape& s, hipStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(p.rows * s.splits));
+    if (s.block == 256) token_scores_kernel<T, 256><<<grid, dim3(256), 0, stream>>>(p);
+    else token_scores_kernel<T, 1024><<<grid, dim3(1024), 0, stream>>>(p);
+    if (s.splits > 1) join_scores_kernel<T><<<dim3(static_cast<unsigned>(p.rows)), dim3(256), 0, stream>>>(p);
+}
+
+}  // namespace
+}  // namespace snnf
+
+using namespace snnf;
+
+extern "C" size_t snnf_token_scores_workspace_bytes(int64_t rows, int V, int top_k) {
+    if (rows < 1 || V < 1 || top_k < 0) return 0;
+    const ScoreShape s = score_shape(rows, V);
+    return s.splits > 1 ? static_cast<size_t>(rows) * s.splits * (sizeof(float4) + sizeof(uint64_t) * top_k) : 0;
+}
+
+extern "C" int snnf_token_scores(const void* logits, int64_t row, int64_t rows, int V, int dtype, const int64_t* tokens, int top_k, float* logprob,
+                                 float* entropy, float* top_logprob, int64_t* top_token, float* stats, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+    const int rc = check_scores("snnf_token_scores", rows, V, dtype, top_k);
+    if (rc != SNNF_OK) return rc;
+    if (rows == 0) return SNNF_OK;
+    if (logits == nullptr || logprob == nullptr || entropy == nullptr || (top_k > 0 && (top_logprob == nullptr || top_token == nullptr)))
+        return fail(SNNF_ERR_INVALID_ARGUMENT, "snnf_token_scores: logits, logprob, entropy and what alternatives are written to must be non-null");
+    const ScoreShape s = score_shape(rows, V);
+    if (rows * s.splits > 0x7fffffffLL) return fail(SNNF_ERR_UNSUPPORTED, "snnf_token_scores: unsupported_shape: %lld rows", (long long)rows);
+    ScoreArgs p = {};
+    if (s.splits > 1) {
+        const size_t need = snnf_token_scores_workspace_bytes(rows, V, top_k);
+        if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
+            return fail(SNNF_ERR_WORKSPACE, "snnf_token_scores: workspace of %zu bytes needed, got %zu", need, workspace_bytes);
+        p.parts = static_cast<float4*>(workspace);
+        p.keys = reinterpret_cast<uint64_t*>(p.parts + rows * s.splits);
+    }
+    p.logits = logits, p.row = row, p.rows = rows;
+    p.V = V, p.k = top_k;
+    p.splits = s.splits, p.span = s.span;
+    p.tokens = tokens;
+    p.logprob = logprob, p.entropy = entropy, p.top_logprob = top_logprob, p.top_token = top_token;
+    p.stats = reinterpret_cast<float2*>(stats);
+    hipStream_t hs = as_stream(stream);
+    if (dtype == SNNF_F32) launch_scores<float>(p, s, hs);
+    else if (dtype == SNNF_BF16) launch_scores<bf16_t>(p, s, hs);
+    else launch_scores<f16_t>(p, s, hs);
+    return check_launch("snnf_token_scores");
+}
+
+extern "C" int snnf_token_scores_backward(const void* logits, int64_t row, int64_t rows, int V, int dtype, const int64_t* tokens, const float* stats,
+                                          const float* entropy, const float* d_logprob, const float* d_entropy, void* d_logits, void* stream) {
+    const int rc = check_scores("snnf_token_scores_backward", rows, V, dtype, 0);
+    if (rc != SNNF_OK) return rc;
+    if (rows == 0) return SNNF_OK;
+    if (logits == nullptr || stats == nullptr || entropy == nullptr || d_logits == nullptr)
+        return fail(SNNF_ERR_INVALID_ARGUMENT, "snnf_token_scores_backward: logits, stats, entropy and d_logits must be non-null");
+    ScoreArgs p = {};
+    p.logits = logits, p.row = row, p.rows = rows;
+    p.V = V;
+    p.span = 8192;
+    p.splits = (V + p.span - 1) / p.span;
+    if (rows * p.splits > 0x7fffffffLL) return fail(SNNF_ERR_UNSUPPORTED, "snnf_token_scores_backward: unsupported_shape: %lld rows", (long long)rows);
+    p.tokens = tokens;
+    p.saved = reinterpret_cast<const float2*>(stats);
+    p.saved_entropy = entropy;
+    p.d_logprob = d_logprob, p.d_entropy = d_entropy;
+    p.d_logits = d_logits;
+    const dim3 grid(static_cast<unsigned>(rows * p.splits)), block(256);
+    hipStream_t hs = as_stream(stream);
+    if (dtype == SNNF_F32) token_scores_backward_kernel<float><<<grid, block, 0, hs>>>(p);
+    else if (dtype == SNNF_BF16) token_scores_backward_kernel<bf16_t><<<grid, block, 0, hs>>>(p);
+    else token_scores_backward_kernel<f16_t><<<grid, block, 0, hs>>>(p);
+    return check_launch("snnf_token_scores_backward");
+}
