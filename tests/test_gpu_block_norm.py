@@ -303,6 +303,33 @@ def test_empty_and_refusals(hip_ops):
             run(*args, **kwargs)
 
 
+@pytest.mark.gpu
+def test_python_implementation(hip_ops, monkeypatch):
+    """What the dispatch module does not take runs in Python, on the same kernels: the same checks with the module out of the way, and equal bits."""
+    from triton_snn_fusion_amd.runtime import hip_block_norm_backend as backend
+    t, grads = operands((33,), 130, torch.bfloat16, torch.float32, torch.float32, True, True, 21)
+    dev = [t[n].to(DEV).requires_grad_(True) for n in NAMES]
+
+    def step():
+        out = run(dev[0], dev[1], gate=dev[2], branch_weight=dev[3], next_weight=dev[4], scale=dev[5])
+        return [*out, *torch.autograd.grad(out, dev, [g.to(DEV) for g in grads])]
+    dispatched = step()
+    monkeypatch.setattr(backend, "native", lambda t: None)
+    assert all(torch.equal(a, b) for a, b in zip(step(), dispatched))
+    for dtype in DTYPES:
+        check((2, 5), 200, dtype, seed=22)
+        check((9,), 77, dtype, kind="layer", gate=None, scale=0.5, seed=23)
+    test_empty_and_refusals(hip_ops)
+
+
+@pytest.mark.gpu
+def test_differentiated_once(hip_ops):
+    x = torch.randn(3, 16, device=DEV, requires_grad=True)
+    out = run(x, x.detach() + 1)[1].sum()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(torch.autograd.grad(out, x, create_graph=True)[0].sum(), x)
+
+
 def test_refusals_without_a_gpu():
     with pytest.raises(RuntimeError, match="unsupported_device"):
         run(torch.zeros(2, 8))

@@ -321,3 +321,37 @@ def test_entry_points_refuse_before_any_gpu_work(snnf_lib):
     assert snnf_lib.snnf_gated_recurrence_marks_bytes(0, 1, 1, 0) == 0 and snnf_lib.snnf_gated_recurrence_marks_bytes(1, 3, 5, 0) == 60
     assert f(16, 1 << 31, 8, 16, 16, 8, 4, 2, 8, 0, 0, None, 0, 0, None, None, 16, 16, 8, 16, None, None, 0, None) == -2
     assert b"unsupported_stride" in snnf_lib.snnf_last_error()
+
+
+@pytest.mark.gpu
+def test_python_implementation(hip_ops, monkeypatch):
+    """What the dispatch module does not take runs in Python, on the same kernels: the same checks with the module out of the way, and equal bits."""
+    from triton_snn_fusion_amd.runtime import hip_gated_recurrence_backend as backend
+    x, gate, state, dh, dlast = operands(300, 3, 130, torch.bfloat16, "leaky", 71)
+    leaves = [t.requires_grad_(True) for t in (x, gate, state)]
+    starts, lengths = (torch.rand(300, 3, generator=gen(1)) < 0.1).to(DEV), torch.tensor([300, 20, 299], dtype=torch.int32, device=DEV)
+
+    def step():
+        out = run(*leaves, starts=starts, lengths=lengths)
+        return [*out, *torch.autograd.grad(out, leaves, [dh, dlast])]
+    dispatched = step()
+    monkeypatch.setattr(backend, "native", lambda t: None)
+    assert all(torch.equal(a, b) for a, b in zip(step(), dispatched))
+    for dtype in DTYPES:
+        check(70, 3, 130, dtype, "leaky", 72, batch_first=True)
+        check(300, 2, 65, dtype, "linear", 73, starts=starts[:, :2].contiguous(), lengths=lengths[:2].long())
+    test_refusals_on_the_gpu(hip_ops)
+    test_empty(hip_ops)
+
+
+@pytest.mark.gpu
+def test_one_output_used_and_one_input_differentiated(hip_ops):
+    x, gate, state, dh, dlast = operands(40, 2, 70, torch.float32, "leaky", 74)
+    for k, leaf in enumerate((x, gate, state)):
+        args = [t.detach().requires_grad_(t is leaf) for t in (x, gate, state)]
+        alone = torch.autograd.grad(run(*args), args[k], [dh, dlast])[0]
+        every = [t.detach().requires_grad_(True) for t in (x, gate, state)]
+        assert torch.equal(alone, torch.autograd.grad(run(*every), every[k], [dh, dlast])[0])
+        for used, grads in ((0, [dh, torch.zeros_like(dlast)]), (1, [torch.zeros_like(dh), dlast])):
+            got = torch.autograd.grad(run(*every)[used], every[k], grads[used])[0]
+            assert torch.equal(got, torch.autograd.grad(run(*every), every[k], grads)[0])

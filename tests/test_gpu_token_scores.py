@@ -251,6 +251,33 @@ def test_empty_and_refusals(hip_ops):
             run(*args, **kwargs)
 
 
+@pytest.mark.gpu
+def test_python_implementation(hip_ops, monkeypatch):
+    """What the dispatch module does not take runs in Python, on the same kernels: the same checks with the module out of the way, and equal bits."""
+    from triton_snn_fusion_amd.runtime import hip_token_scores_backend as backend
+    x, tokens = logits((5,), 3001, torch.bfloat16, 31)
+    leaf, on_gpu, ones = x.to(DEV).requires_grad_(True), tokens.to(DEV), torch.ones(5, device=DEV)
+
+    def step():
+        out = run(leaf, on_gpu, top_k=6)
+        return [*out, torch.autograd.grad(out[:2], leaf, [ones, ones])[0]]
+    dispatched = step()
+    monkeypatch.setattr(backend, "native", lambda t: None)
+    assert all(torch.equal(a, b) for a, b in zip(step(), dispatched))
+    for dtype in DTYPES:
+        check(*logits((3,), 1001, dtype, 32), 7)
+        check(*logits((2,), 90000, dtype, 33), 0)
+    test_empty_and_refusals(hip_ops)
+
+
+@pytest.mark.gpu
+def test_differentiated_once(hip_ops):
+    x = torch.randn(3, 16, device=DEV, requires_grad=True)
+    out = run(x).entropy.sum()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(torch.autograd.grad(out, x, create_graph=True)[0].sum(), x)
+
+
 def test_refusals_without_a_gpu():
     with pytest.raises(RuntimeError, match="unsupported_device"):
         run(torch.zeros(2, 8))

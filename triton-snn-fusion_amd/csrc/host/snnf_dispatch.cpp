@@ -18,11 +18,14 @@
 #include <Python.h>
 
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/python/pybind_utils.h>
 #include <torch/extension.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <array>
 #include <atomic>
 #include <cstring>
@@ -1168,6 +1171,8 @@ PyObject* dense_pool(Args& a) {
     return ran ? THPVariable_Wrap(out) : none();
 }
 
+#include "snnf_sequence_ops.h"
+
 PyObject* py_conv(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(blocked_conv, args, n, 22); }
 PyObject* py_shortcut(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(blocked_shortcut, args, n, 27); }
 PyObject* py_avgpool(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(blocked_avgpool, args, n, 16); }
@@ -1177,6 +1182,10 @@ PyObject* py_head(PyObject*, PyObject* const* args, Py_ssize_t n) { return guard
 PyObject* py_conv_bias(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(dense_conv_bias, args, n, 6); }
 PyObject* py_dense_pool(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(dense_pool, args, n, 6); }
 
+PyObject* py_recurrence(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(gated_recurrence, args, n, 6); }
+PyObject* py_block_norm(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(block_norm, args, n, 10); }
+PyObject* py_scores(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(token_scores, args, n, 3); }
+
 PyMethodDef g_fast_methods[] = {
     {"blocked_conv", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_conv)), METH_FASTCALL, nullptr},
     {"blocked_shortcut", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_shortcut)), METH_FASTCALL, nullptr},
@@ -1185,6 +1194,9 @@ PyMethodDef g_fast_methods[] = {
     {"blocked_head", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_head)), METH_FASTCALL, nullptr},
     {"dense_conv_bias", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_conv_bias)), METH_FASTCALL, nullptr},
     {"dense_pool", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_dense_pool)), METH_FASTCALL, nullptr},
+    {"gated_recurrence", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_recurrence)), METH_FASTCALL, nullptr},
+    {"block_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_block_norm)), METH_FASTCALL, nullptr},
+    {"token_scores", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_scores)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -6,7 +6,7 @@ from typing import Iterable, List, Optional, Tuple
 
 import torch
 
-from .. import _lib
+from .. import _dispatch
 
 SUPPORTED_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -38,6 +38,11 @@ def check_operand(name: str, t, device: torch.device, shape: Tuple[int, ...], dt
         reasons.append(f"unsupported_shape: {name} must be {tuple(shape)}, got {tuple(t.shape)}")
     if t.dtype not in tuple(dtypes):
         reasons.append(f"unsupported_dtype: {name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+
+
+def native(t):
+    """The dispatch module where a call on `t` may be plain enough for it (it answers None where it is not), else None."""
+    return _dispatch.module() if isinstance(t, torch.Tensor) and t.is_cuda else None
 
 
 def wants_gradient(*tensors: Optional[torch.Tensor]) -> bool:
@@ -77,5 +82,3 @@ def flat_rows(t: torch.Tensor) -> torch.Tensor:
     except RuntimeError:
         return t.contiguous().view(lead, t.shape[-1])
 
-
-__all__ = ["SUPPORTED_DTYPES", "check_activation", "check_operand", "flat_rows", "on_device_of", "refuse", "unit_rows", "wants_gradient", "workspace", "_lib"]

@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._sequence_common import SUPPORTED_DTYPES, check_activation, check_operand, flat_rows, on_device_of, refuse, wants_gradient, workspace
+from ._sequence_common import SUPPORTED_DTYPES, check_activation, check_operand, flat_rows, native, on_device_of, refuse, wants_gradient, workspace
 
 KINDS = {"rms": 0, "layer": 1}
 GATE_FORMS = {"sigmoid": 1, "silu": 2}
@@ -132,9 +132,16 @@ def run_hip_block_norm(residual: torch.Tensor, branch: Optional[torch.Tensor] = 
     throughout (normed comes from residual' before its rounding), outputs are rounded once. Differentiable once, in all tensors; the
     vectors' gradients are sums in a fixed order.
     """
+    learnt = isinstance(scale, torch.Tensor)
+    module = native(residual)
+    if module is not None and kind in KINDS and gate_form in GATE_FORMS and eps >= 0.0:
+        known = module.block_norm(residual, branch, gate, branch_weight, next_weight, scale if learnt else None,
+                                  1.0 if learnt or scale is None else scale, KINDS[kind], GATE_FORMS[gate_form], eps)
+        if known is not None:
+            return known
     refuse("run_hip_block_norm", check_block_norm_support(residual, branch, gate, branch_weight, next_weight, scale, kind, gate_form, eps))
     factor = 1.0
-    if scale is not None and not isinstance(scale, torch.Tensor):
+    if not learnt and scale is not None:
         factor, scale = float(scale), None
     shape = residual.shape
     like = residual if branch is None else branch

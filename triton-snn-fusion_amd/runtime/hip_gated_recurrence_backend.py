@@ -17,7 +17,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._sequence_common import check_activation, check_operand, on_device_of, refuse, unit_rows, wants_gradient, workspace
+from ._sequence_common import check_activation, check_operand, native, on_device_of, refuse, unit_rows, wants_gradient, workspace
 
 FORMS = {"leaky": 0, "linear": 1}
 
@@ -121,6 +121,11 @@ def run_hip_gated_recurrence(x_seq: torch.Tensor, gate_seq: torch.Tensor, state:
 
     Arithmetic is float32 throughout, outputs are rounded once. Differentiable once, in x_seq, gate_seq and state.
     """
+    module = native(x_seq)
+    if module is not None and form in FORMS:
+        known = module.gated_recurrence(x_seq, gate_seq, state, starts, lengths, FORMS[form])
+        if known is not None:
+            return known
     refuse("run_hip_gated_recurrence", check_gated_recurrence_support(x_seq, gate_seq, state, form, starts, lengths))
     T, N, D = (int(n) for n in x_seq.shape)
     if T == 0:

@@ -12,7 +12,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._sequence_common import check_activation, check_operand, flat_rows, on_device_of, refuse, wants_gradient, workspace
+from ._sequence_common import check_activation, check_operand, flat_rows, native, on_device_of, refuse, wants_gradient, workspace
 
 MAX_ALTERNATIVES = 64
 
@@ -93,6 +93,11 @@ def run_hip_token_scores(logits: torch.Tensor, tokens: Optional[torch.Tensor] = 
 
     Arithmetic is float32; logprob and entropy are differentiable once, in the logits.
     """
+    module = native(logits)
+    if module is not None:
+        known = module.token_scores(logits, tokens, top_k)
+        if known is not None:
+            return TokenScores(*known)
     refuse("run_hip_token_scores", check_token_scores_support(logits, tokens, top_k))
     lead = logits.shape[:-1]
     if logits.numel() == 0:
