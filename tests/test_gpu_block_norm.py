@@ -306,6 +306,7 @@ def test_empty_and_refusals(hip_ops):
 @pytest.mark.gpu
 def test_python_implementation(hip_ops, monkeypatch):
     """What the dispatch module does not take runs in Python, on the same kernels: the same checks with the module out of the way, and equal bits."""
+    from triton_snn_fusion_amd import _dispatch
     from triton_snn_fusion_amd.runtime import hip_block_norm_backend as backend
     t, grads = operands((33,), 130, torch.bfloat16, torch.float32, torch.float32, True, True, 21)
     dev = [t[n].to(DEV).requires_grad_(True) for n in NAMES]
@@ -313,6 +314,7 @@ def test_python_implementation(hip_ops, monkeypatch):
     def step():
         out = run(dev[0], dev[1], gate=dev[2], branch_weight=dev[3], next_weight=dev[4], scale=dev[5])
         return [*out, *torch.autograd.grad(out, dev, [g.to(DEV) for g in grads])]
+    assert _dispatch.module().block_norm(*dev, 1.0, 0, 2, EPS)[0].grad_fn is not None
     dispatched = step()
     monkeypatch.setattr(backend, "native", lambda t: None)
     assert all(torch.equal(a, b) for a, b in zip(step(), dispatched))

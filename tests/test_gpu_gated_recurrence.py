@@ -326,6 +326,7 @@ def test_entry_points_refuse_before_any_gpu_work(snnf_lib):
 @pytest.mark.gpu
 def test_python_implementation(hip_ops, monkeypatch):
     """What the dispatch module does not take runs in Python, on the same kernels: the same checks with the module out of the way, and equal bits."""
+    from triton_snn_fusion_amd import _dispatch
     from triton_snn_fusion_amd.runtime import hip_gated_recurrence_backend as backend
     x, gate, state, dh, dlast = operands(300, 3, 130, torch.bfloat16, "leaky", 71)
     leaves = [t.requires_grad_(True) for t in (x, gate, state)]
@@ -334,6 +335,7 @@ def test_python_implementation(hip_ops, monkeypatch):
     def step():
         out = run(*leaves, starts=starts, lengths=lengths)
         return [*out, *torch.autograd.grad(out, leaves, [dh, dlast])]
+    assert _dispatch.module().gated_recurrence(*leaves, starts, lengths, 0)[0].grad_fn is not None
     dispatched = step()
     monkeypatch.setattr(backend, "native", lambda t: None)
     assert all(torch.equal(a, b) for a, b in zip(step(), dispatched))

@@ -254,6 +254,7 @@ def test_empty_and_refusals(hip_ops):
 @pytest.mark.gpu
 def test_python_implementation(hip_ops, monkeypatch):
     """What the dispatch module does not take runs in Python, on the same kernels: the same checks with the module out of the way, and equal bits."""
+    from triton_snn_fusion_amd import _dispatch
     from triton_snn_fusion_amd.runtime import hip_token_scores_backend as backend
     x, tokens = logits((5,), 3001, torch.bfloat16, 31)
     leaf, on_gpu, ones = x.to(DEV).requires_grad_(True), tokens.to(DEV), torch.ones(5, device=DEV)
@@ -261,6 +262,7 @@ def test_python_implementation(hip_ops, monkeypatch):
     def step():
         out = run(leaf, on_gpu, top_k=6)
         return [*out, torch.autograd.grad(out[:2], leaf, [ones, ones])[0]]
+    assert _dispatch.module().token_scores(leaf, on_gpu, 6)[0].grad_fn is not None
     dispatched = step()
     monkeypatch.setattr(backend, "native", lambda t: None)
     assert all(torch.equal(a, b) for a, b in zip(step(), dispatched))

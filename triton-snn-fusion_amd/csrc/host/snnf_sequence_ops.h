@@ -19,6 +19,11 @@ inline bool activation(const Tensor& t) {
 inline void* data_of(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 inline void check_status(int status) { TORCH_CHECK(status == 0, snnf_last_error()); }
 
+// Operands that a call may lack are handed to autograd as absent ones, which have no edge: the edge of operand i is its place among those there.
+using Maybe = std::optional<Tensor>;
+inline Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
+inline Tensor tensor_of(const Maybe& t) { return t.has_value() ? *t : Tensor(); }
+
 // The gradients are worked out by kernels that autograd does not see: a second differentiation has to fail, not to be silently zero.
 inline variable_list once(variable_list grads) {
     if (!at::GradMode::is_enabled()) return grads;
@@ -68,12 +73,13 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
                                            marks ? marks->data_ptr<float>() : nullptr, data_of(space), bytes, stream_of(x)));
         return {std::move(h), std::move(last)};
     }
-    static variable_list forward(AutogradContext* ctx, Tensor x, Tensor gate, Tensor state, Tensor starts, Tensor lengths, int64_t form) {
+    static variable_list forward(AutogradContext* ctx, Tensor x, Tensor gate, Maybe state, Maybe starts, Maybe lengths, int64_t form) {
         Tensor marks;
-        variable_list out = compute(x, gate, state, starts, lengths, form, &marks);
+        variable_list out = compute(x, gate, tensor_of(state), tensor_of(starts), tensor_of(lengths), form, &marks);
         ctx->set_materialize_grads(false);
         ctx->saved_data["form"] = form;
-        ctx->save_for_backward({x, gate, starts, lengths, marks});
+        ctx->saved_data["state"] = state.has_value();
+        ctx->save_for_backward({x, gate, tensor_of(starts), tensor_of(lengths), marks});
         return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -93,9 +99,9 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
             starts.defined() ? starts.stride(1) : 0, static_cast<const int32_t*>(data_of(lengths)), marks.data_ptr<float>(),
             static_cast<const float*>(data_of(dlast)), dx.data_ptr(), dx.stride(0), dx.stride(1), dgate.data_ptr(), dgate.stride(0), dgate.stride(1),
             dstate.data_ptr<float>(), data_of(space), bytes, stream_of(x)));
-        Tensor* const all[3] = {&dx, &dgate, &dstate};
-        for (int i = 0; i < 3; ++i)
-            if (!ctx->needs_input_grad(i)) *all[i] = Tensor();
+        if (!ctx->needs_input_grad(0)) dx = Tensor();
+        if (!ctx->needs_input_grad(1)) dgate = Tensor();
+        if (!ctx->saved_data["state"].toBool() || !ctx->needs_input_grad(2)) dstate = Tensor();
         return once({std::move(dx), std::move(dgate), std::move(dstate), Tensor(), Tensor(), Tensor()});
     }
 };
@@ -133,7 +139,7 @@ PyObject* gated_recurrence(Args& a) {
     if (lengths.defined() && (!like_of(lengths, x, at::kInt) || lengths.dim() != 1 || lengths.size(0) != N || !lengths.is_contiguous())) return none();
     variable_list out;
     unlocked([&] {
-        out = wants_gradient({&x, &gate, &state}) ? Recurrence::apply(x, gate, state, starts, lengths, form)
+        out = wants_gradient({&x, &gate, &state}) ? Recurrence::apply(x, gate, maybe(state), maybe(starts), maybe(lengths), form)
                                                   : Recurrence::compute(x, gate, state, starts, lengths, form, nullptr);
         return true;
     });
@@ -174,15 +180,16 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
                                      normed.data_ptr(), stats ? stats->data_ptr<float>() : nullptr, stream_of(residual)));
         return {std::move(out), std::move(normed)};
     }
-    static variable_list forward(AutogradContext* ctx, Tensor residual, Tensor branch, Tensor gate, Tensor wb, Tensor wn, Tensor scale, double factor,
-                                 int64_t kind, int64_t gate_form, double eps) {
+    static variable_list forward(AutogradContext* ctx, Tensor residual, Tensor branch, Maybe gate, Maybe branch_weight, Maybe next_weight, Maybe learnt,
+                                 double factor, int64_t kind, int64_t gate_form, double eps) {
+        const Tensor g = tensor_of(gate), wb = tensor_of(branch_weight), wn = tensor_of(next_weight), scale = tensor_of(learnt);
         Tensor stats;
-        variable_list out = compute(residual, branch, gate, wb, wn, scale, factor, kind, gate_form, eps, &stats);
+        variable_list out = compute(residual, branch, g, wb, wn, scale, factor, kind, gate_form, eps, &stats);
         ctx->set_materialize_grads(false);
         ctx->saved_data["factor"] = factor;
         ctx->saved_data["kind"] = kind;
         ctx->saved_data["gate_form"] = gate_form;
-        ctx->save_for_backward({residual, branch, gate, wb, wn, scale, stats});
+        ctx->save_for_backward({residual, branch, g, wb, wn, scale, stats});
         return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -195,8 +202,11 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
         variable_list d(10);
         for (int i = 0; i < 3; ++i)
             if (saved[i].defined()) d[i] = empty(saved[i].sizes(), saved[i].scalar_type(), residual);
+        std::array<bool, 6> needed{};
+        for (int i = 0, edge = 0; i < 6; ++i)
+            if (saved[i].defined()) needed[i] = ctx->needs_input_grad(edge++);
         for (int i = 3; i < 6; ++i)
-            if (saved[i].defined() && ctx->needs_input_grad(i)) d[i] = empty({s.D}, saved[i].scalar_type(), residual);
+            if (needed[i]) d[i] = empty({s.D}, saved[i].scalar_type(), residual);
         const size_t bytes = snnf_block_norm_backward_workspace_bytes(s.rows, s.D);
         const Tensor space = empty({static_cast<int64_t>(bytes)}, at::kByte, residual);
         check_status(snnf_block_norm_backward(
@@ -206,7 +216,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
             gate.defined() ? static_cast<int>(ctx->saved_data["gate_form"].toInt()) : 0, d[0].data_ptr(), d[1].data_ptr(), data_of(d[2]), data_of(d[3]),
             data_of(d[4]), data_of(d[5]), space.data_ptr(), bytes, stream_of(residual)));
         for (int i = 0; i < 3; ++i)
-            if (!ctx->needs_input_grad(i)) d[i] = Tensor();
+            if (!needed[i]) d[i] = Tensor();
         return once(std::move(d));
     }
 };
@@ -230,7 +240,7 @@ PyObject* block_norm(Args& a) {
     variable_list out;
     unlocked([&] {
         out = wants_gradient({&residual, &branch, &gate, &vectors[0], &vectors[1], &vectors[2]})
-                  ? BlockNorm::apply(residual, branch, gate, vectors[0], vectors[1], vectors[2], factor, kind, gate_form, eps)
+                  ? BlockNorm::apply(residual, branch, maybe(gate), maybe(vectors[0]), maybe(vectors[1]), maybe(vectors[2]), factor, kind, gate_form, eps)
                   : BlockNorm::compute(residual, branch, gate, vectors[0], vectors[1], vectors[2], factor, kind, gate_form, eps, nullptr);
         return true;
     });
@@ -264,11 +274,11 @@ struct Scores : torch::autograd::Function<Scores> {
                                        stats ? stats->data_ptr<float>() : nullptr, data_of(space), bytes, stream_of(logits)));
         return out;
     }
-    static variable_list forward(AutogradContext* ctx, Tensor logits, Tensor tokens, int64_t top_k) {
+    static variable_list forward(AutogradContext* ctx, Tensor logits, Maybe tokens, int64_t top_k) {
         Tensor stats;
-        variable_list out = compute(logits, tokens, top_k, &stats);
+        variable_list out = compute(logits, tensor_of(tokens), top_k, &stats);
         ctx->set_materialize_grads(false);
-        ctx->save_for_backward({logits, tokens, stats, out[1]});
+        ctx->save_for_backward({logits, tensor_of(tokens), stats, out[1]});
         if (top_k > 0) ctx->mark_non_differentiable({out[2], out[3]});
         return out;
     }
@@ -299,7 +309,7 @@ PyObject* token_scores(Args& a) {
     if (tokens.defined() && (!like_of(tokens, logits, at::kLong) || tokens.sizes() != logits.sizes().slice(0, logits.dim() - 1) || !tokens.is_contiguous())) return none();
     variable_list out;
     unlocked([&] {
-        out = wants_gradient({&logits}) ? Scores::apply(logits, tokens, top_k) : Scores::compute(logits, tokens, top_k, nullptr);
+        out = wants_gradient({&logits}) ? Scores::apply(logits, maybe(tokens), top_k) : Scores::compute(logits, tokens, top_k, nullptr);
         return true;
     });
     out.resize(4);
