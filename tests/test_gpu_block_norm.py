@@ -91,34 +91,34 @@ def check(lead, D, dtype, kind="rms", gate="silu", scale=True, residual_dtype=No
     want = reference(v, kind, form, factor)
     want_grads = torch.autograd.grad(want, [v[n] for n in leaves], [d_res.double(), d_norm.double()], retain_graph=True)
     with torch.no_grad():
-        # The sizes that enter, from the formulas
-        unit = norm64(v["branch"], kind)
+        # The sizes of the terms that enter, element by element, from the formulas
+        def center(x):
+            return x - x.mean(-1, keepdim=True) if kind == "layer" else x
+
+        def sigma(x):
+            return torch.sqrt((center(x) ** 2).mean(-1, keepdim=True) + EPS)
+
         act = 1.0 if v.get("gate") is None else (v["gate"].abs() + 1 if form == "silu" else torch.ones_like(v["gate"]))
         wb = v["branch_weight"].abs() if "branch_weight" in v else 1.0
         wn = v["next_weight"].abs() if "next_weight" in v else 1.0
         sc = (v["scale"].abs() if "scale" in v else 1.0) * abs(factor)
-        spread_b = v["branch"].abs().amax(-1, keepdim=True) / torch.sqrt(((v["branch"] - (v["branch"].mean(-1, keepdim=True) if kind == "layer" else 0)) ** 2).mean(-1, keepdim=True) + EPS)
-        size = v["residual"].abs() + spread_b * wb * act * sc
-        center = want[0] - (want[0].mean(-1, keepdim=True) if kind == "layer" else 0)
-        sigma = torch.sqrt((center ** 2).mean(-1, keepdim=True) + EPS)
-        top = size.amax(-1, keepdim=True) / sigma                                    # a unit row's error per rounding
-        room_n = C * U * top * (top + 1) * wn
+        unit = (v["branch"].abs() + v["branch"].abs().mean(-1, keepdim=True)) / sigma(v["branch"])
+        size = v["residual"].abs() + unit * wb * act * sc
+        unit2 = (size + size.mean(-1, keepdim=True)) / sigma(want[0])
         got_dtype[0] = residual_dtype
         near(out[0], want[0], C * U * size, "residual'")
         got_dtype[0] = dtype
-        near(out[1], want[1], room_n, "normed")
-        dn = d_norm.double().abs() * wn
-        d_size = d_res.double().abs() + (dn + (top + 1) * dn.mean(-1, keepdim=True) * (top + 1)) * (top + 1) / sigma
-        room = {"residual": C * U * d_size}
-        sig_b = torch.sqrt(((v["branch"] - (v["branch"].mean(-1, keepdim=True) if kind == "layer" else 0)) ** 2).mean(-1, keepdim=True) + EPS)
+        near(out[1], want[1], C * U * unit2 * wn, "normed")
+
+        def through_norm(d, unit, x):
+            return (d + unit * (d * unit).mean(-1, keepdim=True) + d.mean(-1, keepdim=True)) / sigma(x)
+        d_size = d_res.double().abs() + through_norm(d_norm.double().abs() * wn, unit2, want[0])
         du = d_size * sc * act
-        flow = du * wb
-        room["branch"] = C * U * (flow + (spread_b + 1) ** 2 * flow.mean(-1, keepdim=True)) * (spread_b + 1) / sig_b
-        room["gate"] = C * U * d_size * sc * wb * (spread_b + 1) * act
+        room = {"residual": C * U * d_size, "branch": C * U * through_norm(du * wb, unit, v["branch"]), "gate": C * U * d_size * sc * wb * unit * act}
         flat = lambda a: torch.broadcast_to(a, want[0].shape).reshape(-1, D).sum(0)  # noqa: E731
-        room["branch_weight"] = C * U * flat(du * (spread_b + 1))
-        room["next_weight"] = C * U * flat(d_norm.double().abs() * (top + 1) * (top + 1))
-        room["scale"] = C * U * flat(d_size * act * wb * (spread_b + 1)) * abs(factor)
+        room["branch_weight"] = C * U * flat(du * unit)
+        room["next_weight"] = C * U * flat(d_norm.double().abs() * unit2)
+        room["scale"] = C * U * flat(d_size * act * wb * unit) * abs(factor)
         for n, g, w in zip(leaves, grads, want_grads):
             assert g.dtype == t[n].dtype and g.shape == t[n].shape
             got_dtype[0] = t[n].dtype

@@ -6,6 +6,8 @@
 // sums over them, and the backward pass reads the row statistics that the forward pass leaves. What a program's vectors get as gradients is
 // summed over the rows a workgroup takes in registers, and over the workgroups by a second kernel, in a fixed order.
 // Bound by memory: 5 tensors forward, 8 backward.
+#include <type_traits>
+
 #include "snnf_sequence.h"
 
 namespace snnf {
@@ -29,86 +31,124 @@ struct NormArgs {
     int64_t rows;
     int D, per_row;                     // threads to a row
     int gate_form;
-    int vectors_f32;                    // the weights and the scale are float32
     float factor, eps;
 };
 
 template <typename T> constexpr int kVec = sizeof(T) == 4 ? 4 : 8;
 
-template <typename T, int VEC>
-__device__ __forceinline__ void load(float (&v)[VEC], const void* base, int64_t at, int left) {
-    const T* p = static_cast<const T*>(base) + at;
-    if (left >= VEC) {
-        const auto w = *reinterpret_cast<const typename Words<T, VEC>::type*>(p);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            if constexpr (sizeof(T) == 4) v[j] = element<T>(w[j], 0);
-            else v[j] = element<T>(w[j / 2], j % 2);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = j < left ? to_float(p[j]) : 0.0f;
+// VEC elements of T as they lie in memory; zeros behind the end of a row.
+template <typename T, int VEC> struct Raw {
+    static constexpr int kWords = VEC * static_cast<int>(sizeof(T)) / 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ float operator[](int j) const {
+        if constexpr (sizeof(T) == 4) return element<T>(w[j], 0);
+        else return element<T>(w[j / 2], j % 2);
     }
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void save(void* base, int64_t at, int left, const float (&v)[VEC]) {
-    T* p = static_cast<T*>(base) + at;
-    if (left >= VEC) {
-        typename Words<T, VEC>::type w;
-        if constexpr (sizeof(T) == 4) {
+    __device__ __forceinline__ void load(const void* base, int64_t at, int left) {
+        const T* p = static_cast<const T*>(base) + at;
+        if (left >= VEC) {
+            const auto words = *reinterpret_cast<const typename Words<T, VEC>::type*>(p);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) w[j] = __float_as_uint(v[j]);
+            for (int i = 0; i < kWords; ++i) w[i] = words[i];
         } else {
 #pragma unroll
-            for (int j = 0; j < VEC; j += 2) w[j / 2] = pair_word<T>(v[j], v[j + 1]);
+            for (int i = 0; i < kWords; ++i) {
+                if constexpr (sizeof(T) == 4) w[i] = i < left ? __float_as_uint(p[i]) : 0u;
+                else w[i] = (2 * i < left ? p[2 * i].bits : 0u) | (2 * i + 1 < left ? static_cast<uint32_t>(p[2 * i + 1].bits) << 16 : 0u);
+            }
         }
-        *reinterpret_cast<typename Words<T, VEC>::type*>(p) = w;
-    } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-            if (j < left) p[j] = from_float<T>(v[j]);
     }
+    // a vector of the program's, ones where it has none
+    __device__ __forceinline__ void load_vector(const void* base, int at, int left) {
+        if (base != nullptr) {
+            load(base, at, left);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = sizeof(T) == 4 ? __float_as_uint(1.0f) : pair_word_or_zero(1.0f);
+        }
+    }
+    __device__ __forceinline__ void store(void* base, int64_t at, int left) const {
+        T* p = static_cast<T*>(base) + at;
+        if (left >= VEC) {
+            typename Words<T, VEC>::type words;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) words[i] = w[i];
+            *reinterpret_cast<typename Words<T, VEC>::type*>(p) = words;
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                if constexpr (sizeof(T) == 4) {
+                    if (j < left) p[j] = __uint_as_float(w[j]);
+                } else {
+                    if (j < left) p[j].bits = static_cast<uint16_t>(j % 2 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void put(int j, float first, float second) {
+        if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(first), w[j + 1] = __float_as_uint(second);
+        else w[j / 2] = pair_word<T>(first, second);
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0u;
+    }
+    // The same bits, of which the compiler knows nothing: what was taken apart before is not kept for the next use.
+    __device__ __forceinline__ void again() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) asm("" : "+v"(w[i]));
+    }
+    __device__ __forceinline__ static uint32_t pair_word_or_zero(float v) {
+        if constexpr (sizeof(T) == 4) return 0u;
+        else return pair_word<T>(v, v);
+    }
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void save(void* base, int64_t at, int left, const float (&v)[VEC]) {
+    Raw<T, VEC> raw;
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) raw.put(j, v[j], v[j + 1]);
+    raw.store(base, at, left);
+}
+
+// What the gate lets through, and its slope. No gate is a sigmoid's at infinity: 1, and 0.
+template <typename T>
+__device__ __forceinline__ void gate_of(bool silu, float g, float& act, float& slope) {
+    float s, rest;
+    leak<kPrecise<T>>(g, s, rest);
+    const float from = __builtin_elementwise_maximum(g, -86.0f);        // a gate at the type's lowest value lets nothing through
+    act = s * (silu ? from : 1.0f);
+    slope = s * (silu ? fmaf(__builtin_elementwise_minimum(from, 200.0f), rest, 1.0f) : rest);
 }
 template <typename T, int VEC>
-__device__ __forceinline__ void load_vector(float (&v)[VEC], const void* base, bool f32, int at, int left) {
-    if (base == nullptr) {
+__device__ __forceinline__ void open_gate(Raw<T, VEC>& g) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = 1.0f;
-    } else if (f32) {
-        load<float, VEC>(v, base, at, left);
-    } else {
-        load<T, VEC>(v, base, at, left);
+    for (int i = 0; i < Raw<T, VEC>::kWords; ++i) {
+        if constexpr (sizeof(T) == 4) g.w[i] = __float_as_uint(INFINITY);
+        else g.w[i] = pair_word<T>(INFINITY, INFINITY);
     }
 }
+// Elements are worked out two at a time: all at once would hold more than the registers that are left.
+#define SNNF_ELEMENT_DONE(j) \
+    if ((j) % 2 == 1) __builtin_amdgcn_sched_barrier(0)
 
-// What the gate lets through and its slope.
-template <bool PRECISE>
-__device__ __forceinline__ void gate_of(int form, float g, float& act, float& slope) {
-    if (form == SNNF_GATE_NONE) {
-        act = 1.0f, slope = 0.0f;
-        return;
-    }
-    float s, rest;
-    leak<PRECISE>(g, s, rest);
-    if (form == SNNF_GATE_SIGMOID) {
-        act = s, slope = s * rest;
-    } else {
-        const float from = __builtin_elementwise_maximum(g, -86.0f);        // a gate at the type's lowest value lets nothing through
-        act = from * s;
-        slope = s * fmaf(__builtin_elementwise_minimum(from, 200.0f), rest, 1.0f);
-    }
-}
-
-// Sums over the threads of a row. Two buffers in turn, so that a sum costs one barrier.
+// Sums over the threads of a row: over the lanes of a wave, or of a part of one, and where a row takes several waves through LDS, two buffers in
+// turn so that a sum costs one barrier. Always in the same order.
 struct RowSum {
     float (*shared)[16][2];
-    int waves, first_wave, wave;
+    int lanes, waves, first_wave, wave;
     int buffer;
     template <int COUNT>
     __device__ __forceinline__ void operator()(float (&v)[COUNT]) {
 #pragma unroll
-        for (int i = 0; i < COUNT; ++i) v[i] = wave_sum(v[i]);
-        if (waves == 1) return;
+        for (int i = 0; i < COUNT; ++i) {
+#pragma unroll
+            for (int mask = 1; mask < 64; mask <<= 1) {
+                const float other = __shfl_xor(v[i], mask, 64);
+                v[i] += mask < lanes ? other : 0.0f;
+            }
+        }
+        if (waves <= 1) return;
         if ((threadIdx.x & 63) == 0) {
 #pragma unroll
             for (int i = 0; i < COUNT; ++i) shared[buffer][wave][i] = v[i];
@@ -124,186 +164,318 @@ struct RowSum {
     }
 };
 
-// Takes the mean out where asked, returns it, and 1 / sqrt(mean of squares + eps).
-template <bool LAYER, int K, int VEC>
-__device__ __forceinline__ void whiten(float (&x)[K][VEC], const int (&left)[K], int D, float eps, RowSum& sum, float& mean, float& r) {
-    mean = 0.0f;
-    if constexpr (LAYER) {
+// The thread's place in its row and its row's in the workgroup.
+template <int K, int VEC>
+struct Seat {
+    int slots, slot, thread;
+    int at[K], left[K];
+    RowSum sum;
+    __device__ __forceinline__ Seat(const NormArgs& p, float (*shared)[16][2]) {
+        slots = blockDim.x / p.per_row;
+        slot = threadIdx.x / p.per_row;
+        thread = threadIdx.x - slot * p.per_row;
+        const int waves = p.per_row >> 6;
+        sum = RowSum{shared, p.per_row < 64 ? p.per_row : 64, waves, slot * waves, static_cast<int>(threadIdx.x >> 6), 0};
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            at[k] = (k * p.per_row + thread) * VEC;
+            left[k] = p.D - at[k];
+        }
+    }
+};
+
+template <typename RT, typename XT, typename VT, int K, bool LAYER, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void block_norm_kernel(NormArgs p) {
+    constexpr int VEC = kVec<XT>;
+    __shared__ float shared[2][16][2];
+    Seat<K, VEC> seat(p, shared);
+    const int (&left)[K] = seat.left;
+    const bool branch = p.branch.p != nullptr, gated = p.gate_form != SNNF_GATE_NONE, silu = p.gate_form == SNNF_GATE_SILU;
+    const float part = 1.0f / p.D;
+    Raw<VT, VEC> wb[K], wn[K], sc[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        wn[k].load_vector(p.next_weight, seat.at[k], left[k]);
+        wb[k].load_vector(branch ? p.branch_weight : nullptr, seat.at[k], left[k]);
+        sc[k].load_vector(branch ? p.scale : nullptr, seat.at[k], left[k]);
+    }
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * seat.slots;
+    Raw<RT, VEC> r[K];
+    Raw<XT, VEC> o[K], g[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) open_gate(g[k]);
+    // The next row is on its way as soon as this one's elements are taken apart. (Slots behind the last row repeat it and write nothing.)
+    const auto fetch = [&](int64_t row) {
+        row = row < p.rows ? row : p.rows - 1;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if (branch) o[k].load(p.branch.p, row * p.branch.row + seat.at[k], left[k]);
+            if (gated) g[k].load(p.gate.p, row * p.gate.row + seat.at[k], left[k]);
+            r[k].load(p.residual.p, row * p.residual.row + seat.at[k], left[k]);
+        }
+    };
+    int64_t base = static_cast<int64_t>(blockIdx.x) * seat.slots;
+    fetch(base + seat.slot);
+    for (; base < p.rows; base += stride) {
+        const int64_t row = base + seat.slot;
+        const bool writes = row < p.rows;
+        float total[K][VEC];
+        float4 stats = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (branch) {
+            if constexpr (LAYER) {
+                float s[1] = {0.0f};
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) s[0] += o[k][j];
+                seat.sum(s);
+                stats.x = s[0] * part;
+            }
+            float s[1] = {0.0f};
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float v = LAYER && j >= left[k] ? 0.0f : o[k][j] - stats.x;
+                    s[0] = fmaf(v, v, s[0]);
+                }
+            seat.sum(s);
+            stats.y = 1.0f / sqrtf(s[0] * part + p.eps);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                o[k].again(), wb[k].again(), sc[k].again();
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    float act, slope;
+                    gate_of<XT>(silu, g[k][j], act, slope);
+                    const float more = ((o[k][j] - stats.x) * stats.y * wb[k][j]) * (act * (sc[k][j] * p.factor));
+                    total[k][j] = r[k][j] + (LAYER && j >= left[k] ? 0.0f : more);
+                }
+                if (writes) save<RT, VEC>(p.residual_out, row * p.D + seat.at[k], left[k], total[k]);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) total[k][j] = r[k][j];
+        }
+        if (base + stride < p.rows) fetch(row + stride);
+        if constexpr (LAYER) {
+            float s[1] = {0.0f};
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) s[0] += total[k][j];
+            seat.sum(s);
+            stats.z = s[0] * part;
+        }
         float s[1] = {0.0f};
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) s[0] += x[k][j];
-        sum(s);
-        mean = s[0] / D;
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) x[k][j] = j < left[k] ? x[k][j] - mean : 0.0f;
-    }
-    float s[1] = {0.0f};
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s[0] = fmaf(x[k][j], x[k][j], s[0]);
-    sum(s);
-    r = 1.0f / sqrtf(s[0] / D + eps);
-}
-
-template <typename RT, typename XT, int K, bool LAYER>
-__global__ __launch_bounds__(1024) void block_norm_kernel(NormArgs p) {
-    constexpr int VEC = kVec<XT>;
-    __shared__ float shared[2][16][2];
-    const int slots = blockDim.x / p.per_row, slot = threadIdx.x / p.per_row, thread = threadIdx.x - slot * p.per_row;
-    const int wave = threadIdx.x >> 6, waves = p.per_row >> 6;
-    RowSum sum{shared, waves, slot * waves, wave, 0};
-    int at[K], left[K];
-    float wb[K][VEC], wn[K][VEC], sc[K][VEC];
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        at[k] = (k * p.per_row + thread) * VEC;
-        left[k] = p.D - at[k];
-        load_vector<XT, VEC>(wn[k], p.next_weight, p.vectors_f32, at[k], left[k]);
-        if (p.branch.p != nullptr) {
-            load_vector<XT, VEC>(wb[k], p.branch_weight, p.vectors_f32, at[k], left[k]);
-            load_vector<XT, VEC>(sc[k], p.scale, p.vectors_f32, at[k], left[k]);
-        }
-    }
-    for (int64_t base = static_cast<int64_t>(blockIdx.x) * slots; base < p.rows; base += static_cast<int64_t>(gridDim.x) * slots) {
-        const int64_t row = base + slot < p.rows ? base + slot : p.rows - 1;       // (rows behind the last repeat it and are not written)
-        const bool writes = base + slot < p.rows;
-        float x[K][VEC], total[K][VEC], g[K][VEC];
-#pragma unroll
-        for (int k = 0; k < K; ++k) load<RT, VEC>(total[k], p.residual.p, row * p.residual.row + at[k], left[k]);
-        float4 stats = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (p.branch.p != nullptr) {
-#pragma unroll
-            for (int k = 0; k < K; ++k) load<XT, VEC>(x[k], p.branch.p, row * p.branch.row + at[k], left[k]);
-            if (p.gate_form != SNNF_GATE_NONE) {
-#pragma unroll
-                for (int k = 0; k < K; ++k) load<XT, VEC>(g[k], p.gate.p, row * p.gate.row + at[k], left[k]);
+            for (int j = 0; j < VEC; ++j) {
+                total[k][j] = LAYER && j >= left[k] ? 0.0f : total[k][j] - stats.z;
+                s[0] = fmaf(total[k][j], total[k][j], s[0]);
             }
-            whiten<LAYER, K, VEC>(x, left, p.D, p.eps, sum, stats.x, stats.y);
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    float act = 1.0f, slope;
-                    if (p.gate_form != SNNF_GATE_NONE) gate_of<kPrecise<XT>>(p.gate_form, g[k][j], act, slope);
-                    const float more = (x[k][j] * stats.y * wb[k][j]) * (act * (sc[k][j] * p.factor));
-                    total[k][j] = j < left[k] ? total[k][j] + more : 0.0f;
-                }
-                if (writes) save<RT, VEC>(p.residual_out, row * p.D + at[k], left[k], total[k]);
-            }
-        }
-        whiten<LAYER, K, VEC>(total, left, p.D, p.eps, sum, stats.z, stats.w);
+        seat.sum(s);
+        stats.w = 1.0f / sqrtf(s[0] * part + p.eps);
         if (!writes) continue;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
+            wn[k].again();
 #pragma unroll
             for (int j = 0; j < VEC; ++j) total[k][j] = total[k][j] * stats.w * wn[k][j];
-            save<XT, VEC>(p.normed, row * p.D + at[k], left[k], total[k]);
+            save<XT, VEC>(p.normed, row * p.D + seat.at[k], left[k], total[k]);
         }
-        if (p.stats != nullptr && thread == 0) p.stats[row] = stats;
+        if (p.stats != nullptr && seat.thread == 0) p.stats[row] = stats;
     }
 }
 
-template <typename RT, typename XT, int K, bool LAYER, int BLOCK>
-__global__ __launch_bounds__(BLOCK) void block_norm_backward_kernel(NormArgs p) {
+// Sums over a workgroup's rows, of the columns that a thread owns: in LDS, each read and written by its owner (registers would cost half the
+// waves: 32768 x 2048 bf16 250 -> 226 us), for the widest rows, whose sums LDS does not hold, in registers.
+constexpr bool sums_in_lds(int block, int elements) { return block * elements * 3 * 4 <= 100 * 1024; }
+typedef float Four __attribute__((ext_vector_type(4)));
+template <int BLOCK, int ELEMENTS, bool IN_LDS = sums_in_lds(BLOCK, ELEMENTS)>
+struct ColumnSums {
+    static constexpr int kShared = 1;
+    float v[3][ELEMENTS];
+    __device__ __forceinline__ ColumnSums(Four*) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+            for (int e = 0; e < ELEMENTS; ++e) v[i][e] = 0.0f;
+    }
+    __device__ __forceinline__ void add(int i, int first, const float (&more)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][first + e] += more[e];
+    }
+};
+template <int BLOCK, int ELEMENTS>
+struct ColumnSums<BLOCK, ELEMENTS, true> {
+    static constexpr int kShared = 3 * (ELEMENTS / 4) * BLOCK;         // [3][ELEMENTS / 4][BLOCK]
+    Four* mine;
+    __device__ __forceinline__ ColumnSums(Four* shared) : mine(shared + threadIdx.x) {
+#pragma unroll
+        for (int i = 0; i < 3 * (ELEMENTS / 4); ++i) mine[i * BLOCK] = Four{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    __device__ __forceinline__ void add(int i, int first, const float (&more)[4]) {
+        Four& at = mine[(i * (ELEMENTS / 4) + first / 4) * BLOCK];
+        at = at + Four{more[0], more[1], more[2], more[3]};
+    }
+};
+
+// Elements stay as they lie in memory and are taken apart where they are needed, the gate among them twice: what a thread would have to hold
+// otherwise costs the waves that cover the latency of memory.
+template <typename RT, typename XT, typename VT, int K, bool LAYER, int BLOCK>
+__global__ __launch_bounds__(BLOCK, BLOCK == 256 ? 3 : 1) void block_norm_backward_kernel(NormArgs p) {
     constexpr int VEC = kVec<XT>;
     __shared__ float shared[2][16][2];
-    const int slots = blockDim.x / p.per_row, slot = threadIdx.x / p.per_row, thread = threadIdx.x - slot * p.per_row;
-    const int wave = threadIdx.x >> 6, waves = p.per_row >> 6;
-    RowSum sum{shared, waves, slot * waves, wave, 0};
-    const bool branch = p.branch.p != nullptr, gated = p.gate_form != SNNF_GATE_NONE;
-    int at[K], left[K];
-    float wb[K][VEC], wn[K][VEC], sc[K][VEC], dwb[K][VEC], dwn[K][VEC], dsc[K][VEC];
+    constexpr int kElements = K * VEC;
+    __shared__ Four columns[ColumnSums<BLOCK, kElements>::kShared];
+    ColumnSums<BLOCK, kElements> sums(columns);
+    Seat<K, VEC> seat(p, shared);
+    const int (&left)[K] = seat.left;
+    const bool branch = p.branch.p != nullptr, gated = p.gate_form != SNNF_GATE_NONE, silu = p.gate_form == SNNF_GATE_SILU, from_out = p.d_residual_out.p != nullptr, from_normed = p.d_normed.p != nullptr;
+    const float part = 1.0f / p.D;
+    Raw<VT, VEC> wb[K], wn[K], sc[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        at[k] = (k * p.per_row + thread) * VEC;
-        left[k] = p.D - at[k];
-        load_vector<XT, VEC>(wn[k], p.next_weight, p.vectors_f32, at[k], left[k]);
-        load_vector<XT, VEC>(wb[k], branch ? p.branch_weight : nullptr, p.vectors_f32, at[k], left[k]);
-        load_vector<XT, VEC>(sc[k], branch ? p.scale : nullptr, p.vectors_f32, at[k], left[k]);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) dwb[k][j] = dwn[k][j] = dsc[k][j] = 0.0f;
+        wn[k].load_vector(p.next_weight, seat.at[k], left[k]);
+        wb[k].load_vector(branch ? p.branch_weight : nullptr, seat.at[k], left[k]);
+        sc[k].load_vector(branch ? p.scale : nullptr, seat.at[k], left[k]);
     }
-    for (int64_t base = static_cast<int64_t>(blockIdx.x) * slots; base < p.rows; base += static_cast<int64_t>(gridDim.x) * slots) {
-        const bool writes = base + slot < p.rows;
-        const int64_t row = writes ? base + slot : p.rows - 1;
-        float total[K][VEC], unit[K][VEC], g[K][VEC], d[K][VEC], dn[K][VEC];
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * seat.slots;
+    Raw<RT, VEC> r[K], d_out[K];
+    Raw<XT, VEC> o[K], g[K], dn[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {       // what is not there: a branch, whose statistics are 0 then, and gradients of 0
+        open_gate(g[k]);
+        o[k].clear(), dn[k].clear(), d_out[k].clear();
+    }
+    // The next row's elements are sent for as soon as this row's in their place are done with.
+    const auto fetch_total = [&](int64_t row) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            load<RT, VEC>(total[k], p.residual.p, row * p.residual.row + at[k], left[k]);
-            if (p.d_normed.p != nullptr) load<XT, VEC>(dn[k], p.d_normed.p, row * p.d_normed.row + at[k], left[k]);
-            if (p.d_residual_out.p != nullptr) load<RT, VEC>(d[k], p.d_residual_out.p, row * p.d_residual_out.row + at[k], left[k]);
-            if (branch) load<XT, VEC>(unit[k], p.branch.p, row * p.branch.row + at[k], left[k]);
-            if (gated) load<XT, VEC>(g[k], p.gate.p, row * p.gate.row + at[k], left[k]);
+            r[k].load(p.residual.p, row * p.residual.row + seat.at[k], left[k]);
+            if (from_normed) dn[k].load(p.d_normed.p, row * p.d_normed.row + seat.at[k], left[k]);
         }
-        const float4 stats = p.stats[row];
-        float act[K][VEC], slope[K][VEC], s[2] = {0.0f, 0.0f};
+    };
+    const auto fetch_gate = [&](int64_t row) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if (gated) g[k].load(p.gate.p, row * p.gate.row + seat.at[k], left[k]);
+            if (from_out) d_out[k].load(p.d_residual_out.p, row * p.d_residual_out.row + seat.at[k], left[k]);
+        }
+    };
+    const auto fetch_branch = [&](int64_t row) {
 #pragma unroll
         for (int k = 0; k < K; ++k)
+            if (branch) o[k].load(p.branch.p, row * p.branch.row + seat.at[k], left[k]);
+    };
+    const auto real = [&](int64_t row) { return row < p.rows ? row : p.rows - 1; };
+    int64_t base = static_cast<int64_t>(blockIdx.x) * seat.slots;
+    fetch_total(real(base + seat.slot));
+    fetch_branch(real(base + seat.slot));
+    fetch_gate(real(base + seat.slot));
+    float4 next_stats = p.stats[real(base + seat.slot)];
+    for (; base < p.rows; base += stride) {
+        const int64_t row = base + seat.slot, next = real(row + stride);
+        const bool writes = row < p.rows, more = base + stride < p.rows;
+        const float counts = writes ? 1.0f : 0.0f;
+        const float4 stats = next_stats;
+        float unit2[K][VEC], d[K][VEC], s[2] = {0.0f, 0.0f};           // the unit row of the second norm, the gradient in front of its weight
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            wb[k].again(), wn[k].again(), sc[k].again();
+            float more[4];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const bool in = j < left[k];
-                act[k][j] = 1.0f, slope[k][j] = 0.0f;
-                if (branch) {
-                    if (gated) gate_of<kPrecise<XT>>(p.gate_form, g[k][j], act[k][j], slope[k][j]);
-                    unit[k][j] = in ? (unit[k][j] - stats.x) * stats.y : 0.0f;
-                    total[k][j] += (unit[k][j] * wb[k][j]) * (act[k][j] * (sc[k][j] * p.factor));
-                }
-                total[k][j] = in ? (total[k][j] - stats.z) * stats.w : 0.0f;       // the unit row of the second norm
-                if (p.d_normed.p == nullptr) dn[k][j] = 0.0f;
-                if (p.d_residual_out.p == nullptr) d[k][j] = 0.0f;
-                if (writes) dwn[k][j] = fmaf(dn[k][j], total[k][j], dwn[k][j]);
-                dn[k][j] = in ? dn[k][j] * wn[k][j] : 0.0f;
-                s[0] = fmaf(dn[k][j], total[k][j], s[0]);
-                s[1] += dn[k][j];
+                float act, slope;
+                gate_of<XT>(silu, g[k][j], act, slope);
+                const float total = r[k][j] + ((o[k][j] - stats.x) * stats.y * wb[k][j]) * (act * (sc[k][j] * p.factor));
+                unit2[k][j] = LAYER && j >= left[k] ? 0.0f : (total - stats.z) * stats.w;
+                more[j % 4] = dn[k][j] * counts * unit2[k][j];
+                if (j % 4 == 3) sums.add(1, k * VEC + j - 3, more);
+                d[k][j] = dn[k][j] * wn[k][j];
+                s[0] = fmaf(d[k][j], unit2[k][j], s[0]);
+                s[1] += d[k][j];
+                SNNF_ELEMENT_DONE(j);
             }
-        sum(s);
-        s[0] /= p.D;
-        s[1] = LAYER ? s[1] / p.D : 0.0f;
+        }
+        if (more) fetch_total(next);
+        seat.sum(s);
+        s[0] *= part;
+        s[1] = LAYER ? s[1] * part : 0.0f;
         float q[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < K; ++k) {
 #pragma unroll
+            for (int j = 0; j < VEC; ++j) d[k][j] = LAYER && j >= left[k] ? 0.0f : stats.w * (d[k][j] - unit2[k][j] * s[0] - s[1]) + d_out[k][j];
+            if (writes) save<RT, VEC>(p.d_residual, row * p.D + seat.at[k], left[k], d[k]);
+            o[k].again(), g[k].again(), wb[k].again(), sc[k].again();
+            float more_weight[4], more_scale[4], gates[2];
+            Raw<XT, VEC> d_gate;
+#pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                d[k][j] += stats.w * (dn[k][j] - total[k][j] * s[0] - s[1]);
-                if (branch) {
-                    const float through = d[k][j] * p.factor, y = unit[k][j] * wb[k][j];
-                    if (writes) dsc[k][j] = fmaf(through * act[k][j], y, dsc[k][j]);
-                    slope[k][j] = through * sc[k][j] * y * slope[k][j];            // the gate's gradient
-                    const float du = through * sc[k][j] * act[k][j];
-                    if (writes) dwb[k][j] = fmaf(du, unit[k][j], dwb[k][j]);
-                    dn[k][j] = j < left[k] ? du * wb[k][j] : 0.0f;
-                    q[0] = fmaf(dn[k][j], unit[k][j], q[0]);
-                    q[1] += dn[k][j];
+                float act, slope;
+                gate_of<XT>(silu, g[k][j], act, slope);
+                const float unit = LAYER && j >= left[k] ? 0.0f : (o[k][j] - stats.x) * stats.y;
+                const float through = d[k][j] * p.factor, y = unit * wb[k][j], du = through * sc[k][j] * act;
+                more_scale[j % 4] = through * act * counts * y;
+                more_weight[j % 4] = du * counts * unit;
+                gates[j % 2] = through * sc[k][j] * y * slope;
+                if (j % 2 == 1) d_gate.put(j - 1, gates[0], gates[1]);
+                d[k][j] = du * wb[k][j];
+                q[0] = fmaf(d[k][j], unit, q[0]);
+                q[1] += d[k][j];
+                if (j % 4 == 3) {
+                    sums.add(0, k * VEC + j - 3, more_weight);
+                    sums.add(2, k * VEC + j - 3, more_scale);
                 }
+                SNNF_ELEMENT_DONE(j);
             }
-            if (writes) {
-                save<RT, VEC>(p.d_residual, row * p.D + at[k], left[k], d[k]);
-                if (gated) save<XT, VEC>(p.d_gate, row * p.D + at[k], left[k], slope[k]);
+            if (gated && writes) d_gate.store(p.d_gate, row * p.D + seat.at[k], left[k]);
+        }
+        if (more) {
+            fetch_gate(next);
+            next_stats = p.stats[next];
+        }
+        seat.sum(q);
+        q[0] *= part;
+        q[1] = LAYER ? q[1] * part : 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            o[k].again();
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) d[k][j] = stats.y * (d[k][j] - (o[k][j] - stats.x) * stats.y * q[0] - q[1]);
+            if (branch && writes) save<XT, VEC>(p.d_branch, row * p.D + seat.at[k], left[k], d[k]);
+        }
+        if (more) fetch_branch(next);
+    }
+    // A workgroup's rows as one part, slot by slot.
+    float* const to = p.parts + static_cast<int64_t>(blockIdx.x) * 3 * p.D;
+    if constexpr (sums_in_lds(BLOCK, kElements)) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < p.D; i += BLOCK) {
+            const int chunk = i / VEC, owner = chunk % p.per_row, e = chunk / p.per_row * VEC + i % VEC;
+#pragma unroll
+            for (int v = 0; v < 3; ++v) {
+                const float* const column = reinterpret_cast<const float*>(columns + (v * (kElements / 4) + e / 4) * BLOCK + owner) + e % 4;
+                float total = 0.0f;
+                for (int t = 0; t < seat.slots; ++t) total += column[t * p.per_row * 4];
+                to[v * p.D + i] = total;
             }
         }
-        if (branch) {
-            sum(q);
-            q[0] /= p.D;
-            q[1] = LAYER ? q[1] / p.D : 0.0f;
+    } else {
+#pragma unroll
+        for (int v = 0; v < 3; ++v)
 #pragma unroll
             for (int k = 0; k < K; ++k) {
+                float total[VEC];
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) dn[k][j] = stats.y * (dn[k][j] - unit[k][j] * q[0] - q[1]);
-                if (writes) save<XT, VEC>(p.d_branch, row * p.D + at[k], left[k], dn[k]);
+                for (int j = 0; j < VEC; ++j) total[j] = sums.v[v][k * VEC + j];
+                save<float, VEC>(to + v * p.D, seat.at[k], left[k], total);
             }
-        }
-    }
-    float* to = p.parts + (static_cast<int64_t>(blockIdx.x) * slots + slot) * 3 * p.D;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        save<float, VEC>(to, at[k], left[k], dwb[k]);
-        save<float, VEC>(to + p.D, at[k], left[k], dwn[k]);
-        save<float, VEC>(to + 2 * p.D, at[k], left[k], dsc[k]);
     }
 }
 
@@ -333,16 +505,20 @@ struct NormShape {
     int per_row, block, slots, chunks, grid;
 };
 
-// Threads to a row: 8 elements each, up to 1024 threads. Backward, a workgroup takes at least four rows to a slot where that leaves one for every
-// compute unit: its sums over rows cost as much memory as a row does.
+// Threads to a row: 8 elements each up to 512 threads, 16 from there on. Workgroups: as many as are resident at once, which walk over the rows.
+// Backward, a workgroup takes at least four rows to a slot where that leaves one for every compute unit: its sums over rows cost as much
+// memory as a row does.
 NormShape norm_shape(int64_t rows, int D, bool backward, int vec) {
     NormShape s;
-    s.per_row = 64;
-    while (s.per_row < 1024 && s.per_row * 8 < D) s.per_row *= 2;
+    s.per_row = 8;
+    while (s.per_row < 512 && s.per_row * 8 < D) s.per_row *= 2;
     s.chunks = s.per_row * 8 < D ? 16 / vec : 8 / vec;
+    if (s.per_row * 16 < D) s.per_row = 1024;
     s.block = s.per_row < 256 ? 256 : s.per_row;
     s.slots = s.block / s.per_row;
-    const int64_t units = compute_units(), resident = units * (backward ? (s.block == 256 ? 3 : 1) : 2048 / s.block);
+    const int64_t units = compute_units();
+    const int64_t fit = s.block == 1024 ? 1 : (backward ? (s.block == 512 ? 1 : 3) : (s.block == 512 ? (s.chunks * vec == 8 ? 3 : 2) : 6));
+    const int64_t resident = units * fit;
     int64_t grid = (rows + s.slots - 1) / s.slots;
     if (backward) {
         const int64_t few = (rows + s.slots * 4 - 1) / (s.slots * 4);
@@ -352,28 +528,44 @@ NormShape norm_shape(int64_t rows, int D, bool backward, int vec) {
     return s;
 }
 
-template <typename RT, typename XT, int K>
+template <typename RT, typename XT, typename VT, int K>
 void launch_norm(const NormArgs& p, const NormShape& s, bool layer, bool backward, hipStream_t stream) {
     const dim3 grid(s.grid), block(s.block);
-    if (backward) {
-        if (s.block > 512) {
-            if (layer) block_norm_backward_kernel<RT, XT, K, true, 1024><<<grid, block, 0, stream>>>(p);
-            else block_norm_backward_kernel<RT, XT, K, false, 1024><<<grid, block, 0, stream>>>(p);
-        } else if constexpr (K * kVec<XT> == 8) {
-            if (layer) block_norm_backward_kernel<RT, XT, K, true, 512><<<grid, block, 0, stream>>>(p);
-            else block_norm_backward_kernel<RT, XT, K, false, 512><<<grid, block, 0, stream>>>(p);
+    const auto go = [&](auto block_size) {
+        constexpr int BLOCK = decltype(block_size)::value;
+        if (backward) {
+            if (layer) block_norm_backward_kernel<RT, XT, VT, K, true, BLOCK><<<grid, block, 0, stream>>>(p);
+            else block_norm_backward_kernel<RT, XT, VT, K, false, BLOCK><<<grid, block, 0, stream>>>(p);
+        } else {
+            if (layer) block_norm_kernel<RT, XT, VT, K, true, BLOCK><<<grid, block, 0, stream>>>(p);
+            else block_norm_kernel<RT, XT, VT, K, false, BLOCK><<<grid, block, 0, stream>>>(p);
         }
+    };
+    if constexpr (K * kVec<XT> == 8) {
+        if (s.block == 512) go(std::integral_constant<int, 512>{});
+        else go(std::integral_constant<int, 256>{});
     } else {
-        if (layer) block_norm_kernel<RT, XT, K, true><<<grid, block, 0, stream>>>(p);
-        else block_norm_kernel<RT, XT, K, false><<<grid, block, 0, stream>>>(p);
+        if (s.block == 512) go(std::integral_constant<int, 512>{});
+        else go(std::integral_constant<int, 1024>{});
     }
 }
 
-template <typename RT, typename XT>
+template <typename RT, typename XT, typename VT>
 void launch_types(const NormArgs& p, const NormShape& s, bool layer, bool backward, hipStream_t stream) {
     constexpr int few = 8 / kVec<XT>;
-    if (s.chunks == few) launch_norm<RT, XT, few>(p, s, layer, backward, stream);
-    else launch_norm<RT, XT, 2 * few>(p, s, layer, backward, stream);
+    if (s.chunks == few) launch_norm<RT, XT, VT, few>(p, s, layer, backward, stream);
+    else launch_norm<RT, XT, VT, 2 * few>(p, s, layer, backward, stream);
+}
+
+template <typename XT>
+void launch_16(const NormArgs& p, const NormShape& s, bool wide_residual, bool wide_vectors, bool layer, bool backward, hipStream_t stream) {
+    if (wide_residual) {
+        if (wide_vectors) launch_types<float, XT, float>(p, s, layer, backward, stream);
+        else launch_types<float, XT, XT>(p, s, layer, backward, stream);
+    } else {
+        if (wide_vectors) launch_types<XT, XT, float>(p, s, layer, backward, stream);
+        else launch_types<XT, XT, XT>(p, s, layer, backward, stream);
+    }
 }
 
 int check_norm(const char* name, int64_t rows, int D, int residual_dtype, int dtype, int vector_dtype, int kind, int gate_form, float eps) {
@@ -390,13 +582,11 @@ int check_norm(const char* name, int64_t rows, int D, int residual_dtype, int dt
     return SNNF_OK;
 }
 
-int run_norm(const char* name, const NormArgs& p, int residual_dtype, int dtype, int kind, bool backward, const NormShape& s, hipStream_t stream) {
-    const bool layer = kind == SNNF_NORM_LAYER;
-    if (dtype == SNNF_F32) launch_types<float, float>(p, s, layer, backward, stream);
-    else if (dtype == SNNF_BF16 && residual_dtype == SNNF_F32) launch_types<float, bf16_t>(p, s, layer, backward, stream);
-    else if (dtype == SNNF_BF16) launch_types<bf16_t, bf16_t>(p, s, layer, backward, stream);
-    else if (residual_dtype == SNNF_F32) launch_types<float, f16_t>(p, s, layer, backward, stream);
-    else launch_types<f16_t, f16_t>(p, s, layer, backward, stream);
+int run_norm(const char* name, const NormArgs& p, int residual_dtype, int dtype, int vector_dtype, int kind, bool backward, const NormShape& s, hipStream_t stream) {
+    const bool layer = kind == SNNF_NORM_LAYER, wide_residual = residual_dtype == SNNF_F32, wide_vectors = vector_dtype == SNNF_F32;
+    if (dtype == SNNF_F32) launch_types<float, float, float>(p, s, layer, backward, stream);
+    else if (dtype == SNNF_BF16) launch_16<bf16_t>(p, s, wide_residual, wide_vectors, layer, backward, stream);
+    else launch_16<f16_t>(p, s, wide_residual, wide_vectors, layer, backward, stream);
     return check_launch(name);
 }
 
@@ -423,17 +613,16 @@ extern "C" int snnf_block_norm(const void* residual, int64_t residual_row, const
     p.stats = reinterpret_cast<float4*>(stats);
     p.rows = rows, p.D = D;
     p.gate_form = gate_form;
-    p.vectors_f32 = vector_dtype == SNNF_F32;
     p.factor = factor, p.eps = eps;
     const NormShape s = norm_shape(rows, D, false, dtype == SNNF_F32 ? 4 : 8);
     p.per_row = s.per_row;
-    return run_norm("snnf_block_norm", p, residual_dtype, dtype, kind, false, s, as_stream(stream));
+    return run_norm("snnf_block_norm", p, residual_dtype, dtype, vector_dtype, kind, false, s, as_stream(stream));
 }
 
 extern "C" size_t snnf_block_norm_backward_workspace_bytes(int64_t rows, int D) {
     if (rows < 1 || D < 1 || D > kMostWidth) return 0;
     const NormShape s = norm_shape(rows, D, true, 8);
-    return static_cast<size_t>(s.grid) * s.slots * 3 * D * sizeof(float);
+    return static_cast<size_t>(s.grid) * 3 * D * sizeof(float);
 }
 
 extern "C" int snnf_block_norm_backward(const void* residual, int64_t residual_row, const void* branch, int64_t branch_row, const void* gate,
@@ -464,15 +653,14 @@ extern "C" int snnf_block_norm_backward(const void* residual, int64_t residual_r
     p.parts = static_cast<float*>(workspace);
     p.rows = rows, p.D = D;
     p.gate_form = gate_form;
-    p.vectors_f32 = vector_dtype == SNNF_F32;
     p.factor = factor;
     const NormShape s = norm_shape(rows, D, true, dtype == SNNF_F32 ? 4 : 8);
     p.per_row = s.per_row;
     hipStream_t hs = as_stream(stream);
-    const int status = run_norm(name, p, residual_dtype, dtype, kind, true, s, hs);
+    const int status = run_norm(name, p, residual_dtype, dtype, vector_dtype, kind, true, s, hs);
     if (status != SNNF_OK || (d_branch_weight == nullptr && d_next_weight == nullptr && d_scale == nullptr)) return status;
     const dim3 grid((D + 63) / 64, 3), block(64 * kPhases);
-    const int n_parts = s.grid * s.slots;
+    const int n_parts = s.grid;
     if (vector_dtype == SNNF_F32)
         vector_gradient_kernel<<<grid, block, 0, hs>>>(p.parts, n_parts, D, static_cast<float*>(d_branch_weight), static_cast<float*>(d_next_weight), static_cast<float*>(d_scale));
     else if (vector_dtype == SNNF_BF16)
