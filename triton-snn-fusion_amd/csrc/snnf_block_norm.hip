@@ -34,75 +34,6 @@ struct NormArgs {
     float factor, eps;
 };
 
-template <typename T> constexpr int kVec = sizeof(T) == 4 ? 4 : 8;
-
-// VEC elements of T as they lie in memory; zeros behind the end of a row.
-template <typename T, int VEC> struct Raw {
-    static constexpr int kWords = VEC * static_cast<int>(sizeof(T)) / 4;
-    uint32_t w[kWords];
-    __device__ __forceinline__ float operator[](int j) const {
-        if constexpr (sizeof(T) == 4) return element<T>(w[j], 0);
-        else return element<T>(w[j / 2], j % 2);
-    }
-    __device__ __forceinline__ void load(const void* base, int64_t at, int left) {
-        const T* p = static_cast<const T*>(base) + at;
-        if (left >= VEC) {
-            const auto words = *reinterpret_cast<const typename Words<T, VEC>::type*>(p);
-#pragma unroll
-            for (int i = 0; i < kWords; ++i) w[i] = words[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < kWords; ++i) {
-                if constexpr (sizeof(T) == 4) w[i] = i < left ? __float_as_uint(p[i]) : 0u;
-                else w[i] = (2 * i < left ? p[2 * i].bits : 0u) | (2 * i + 1 < left ? static_cast<uint32_t>(p[2 * i + 1].bits) << 16 : 0u);
-            }
-        }
-    }
-    // a vector of the program's, ones where it has none
-    __device__ __forceinline__ void load_vector(const void* base, int at, int left) {
-        if (base != nullptr) {
-            load(base, at, left);
-        } else {
-#pragma unroll
-            for (int i = 0; i < kWords; ++i) w[i] = sizeof(T) == 4 ? __float_as_uint(1.0f) : pair_word_or_zero(1.0f);
-        }
-    }
-    __device__ __forceinline__ void store(void* base, int64_t at, int left) const {
-        T* p = static_cast<T*>(base) + at;
-        if (left >= VEC) {
-            typename Words<T, VEC>::type words;
-#pragma unroll
-            for (int i = 0; i < kWords; ++i) words[i] = w[i];
-            *reinterpret_cast<typename Words<T, VEC>::type*>(p) = words;
-        } else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                if constexpr (sizeof(T) == 4) {
-                    if (j < left) p[j] = __uint_as_float(w[j]);
-                } else {
-                    if (j < left) p[j].bits = static_cast<uint16_t>(j % 2 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu);
-                }
-            }
-        }
-    }
-    __device__ __forceinline__ void put(int j, float first, float second) {
-        if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(first), w[j + 1] = __float_as_uint(second);
-        else w[j / 2] = pair_word<T>(first, second);
-    }
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) w[i] = 0u;
-    }
-    // The same bits, of which the compiler knows nothing: what was taken apart before is not kept for the next use.
-    __device__ __forceinline__ void again() {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) asm("" : "+v"(w[i]));
-    }
-    __device__ __forceinline__ static uint32_t pair_word_or_zero(float v) {
-        if constexpr (sizeof(T) == 4) return 0u;
-        else return pair_word<T>(v, v);
-    }
-};
 template <typename T, int VEC>
 __device__ __forceinline__ void save(void* base, int64_t at, int left, const float (&v)[VEC]) {
     Raw<T, VEC> raw;
@@ -141,13 +72,7 @@ struct RowSum {
     template <int COUNT>
     __device__ __forceinline__ void operator()(float (&v)[COUNT]) {
 #pragma unroll
-        for (int i = 0; i < COUNT; ++i) {
-#pragma unroll
-            for (int mask = 1; mask < 64; mask <<= 1) {
-                const float other = __shfl_xor(v[i], mask, 64);
-                v[i] += mask < lanes ? other : 0.0f;
-            }
-        }
+        for (int i = 0; i < COUNT; ++i) v[i] = lane_sum(v[i], lanes);
         if (waves <= 1) return;
         if ((threadIdx.x & 63) == 0) {
 #pragma unroll

@@ -13,7 +13,7 @@ namespace {
 
 constexpr int kMostAlternatives = 64;
 constexpr int kCandidates = 1024;       // candidates that are ranked at once; rows with more (many equal values) select one by one
-constexpr int kBatch = 4;               // vectors a thread has in flight
+constexpr int kBatch = 2;               // vectors a thread works on while as many are on their way
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 struct ScoreArgs {
@@ -33,8 +33,6 @@ struct ScoreArgs {
     void* d_logits;
 };
 
-template <typename T> constexpr int kVec = sizeof(T) == 4 ? 4 : 8;
-
 // M, s and t (in powers of two: t = sum e z with e = 2^z) of some elements.
 struct Stats {
     float M, s, t;
@@ -51,18 +49,24 @@ __device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
     return {M, a.s * fa + b.s * fb, fa * fmaf(za, a.s, a.t) + fb * fmaf(zb, b.s, b.t)};
 }
 
+// All threads' statistics as one, in every thread.
 template <int BLOCK>
 __device__ __forceinline__ Stats join_all(Stats v) {
-    __shared__ Stats shared[BLOCK / 64];
-#pragma unroll
-    for (int mask = 1; mask < 64; mask <<= 1) {
-        const Stats other{__shfl_xor(v.M, mask, 64), __shfl_xor(v.s, mask, 64), __shfl_xor(v.t, mask, 64)};
-        v = (threadIdx.x & mask) ? join(other, v) : join(v, other);
-    }
-    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+    __shared__ float largest[BLOCK / 64], sums[2][BLOCK / 64];
+    const int wave = threadIdx.x >> 6;
+    float M = lane_max(v.M);
+    if ((threadIdx.x & 63) == 0) largest[wave] = M;
     __syncthreads();
-    v = shared[0];
-    for (int w = 1; w < BLOCK / 64; ++w) v = join(v, shared[w]);
+    M = largest[0];
+#pragma unroll
+    for (int w = 1; w < BLOCK / 64; ++w) M = fmaxf(M, largest[w]);
+    const float z = exponent(v.M, center(M)), f = __builtin_amdgcn_exp2f(z);
+    const float s = lane_sum(v.s * f), t = lane_sum(f * fmaf(z, v.s, v.t));
+    if ((threadIdx.x & 63) == 0) sums[0][wave] = s, sums[1][wave] = t;
+    __syncthreads();
+    v = {M, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < BLOCK / 64; ++w) v.s += sums[0][w], v.t += sums[1][w];
     return v;
 }
 
@@ -75,19 +79,14 @@ __device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_flo
 // -0 and 0 are the same value.
 __device__ __forceinline__ uint64_t key_of(float x, int index) { return static_cast<uint64_t>(order_of(x + 0.0f)) << 32 | static_cast<uint32_t>(~index); }
 
+// Elements `at` to `end` - 1 of a row; minus infinity behind them.
 template <typename T>
-__device__ __forceinline__ void load_vector(float (&v)[kVec<T>], const T* row, int at, int end) {
-    constexpr int VEC = kVec<T>;
-    if (at + VEC <= end) {
-        const auto w = *reinterpret_cast<const typename Words<T, VEC>::type*>(row + at);
+__device__ __forceinline__ void take(float (&v)[kVec<T>], const Raw<T, kVec<T>>& raw, int left) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            if constexpr (sizeof(T) == 4) v[j] = element<T>(w[j], 0);
-            else v[j] = element<T>(w[j / 2], j % 2);
-        }
-    } else {
+    for (int j = 0; j < kVec<T>; ++j) v[j] = raw[j];
+    if (left < kVec<T>) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = at + j < end ? to_float(row[at + j]) : -INFINITY;
+        for (int j = 0; j < kVec<T>; ++j) v[j] = j < left ? v[j] : -INFINITY;
     }
 }
 
@@ -97,6 +96,7 @@ __device__ __forceinline__ void rank_keys(const uint64_t* keys, int count, int k
     for (int i = threadIdx.x; i < count; i += BLOCK) {
         const uint64_t mine = keys[i];
         int rank = 0;
+#pragma unroll 8
         for (int j = 0; j < count; ++j) rank += keys[j] > mine ? 1 : 0;
         if (rank < k) out[rank] = mine;
     }
@@ -107,7 +107,7 @@ template <typename T, int BLOCK>
 __device__ __forceinline__ void alternatives(const T* row, int begin, int end, int k, float most, uint64_t* out) {
     constexpr int VEC = kVec<T>, WAVES = BLOCK / 64;
     __shared__ float maxima[WAVES][64];
-    __shared__ float reached;
+    __shared__ uint32_t reached;
     __shared__ int count;
     __shared__ uint64_t candidates[kCandidates];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -116,27 +116,34 @@ __device__ __forceinline__ void alternatives(const T* row, int begin, int end, i
     __syncthreads();
     if (wave == 0) {
         float group = maxima[0][lane];
-        for (int w = 1; w < WAVES; ++w) group = fmaxf(group, maxima[w][lane]);
-        int rank = 0;
 #pragma unroll
-        for (int j = 0; j < 64; ++j) {
-            const float other = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(group), j));
-            rank += other > group || (other == group && j < lane) ? 1 : 0;
+        for (int w = 1; w < WAVES; ++w) group = fmaxf(group, maxima[w][lane]);
+        // The k-th largest, bit by bit: the largest number that k of them reach.
+        const uint32_t mine = order_of(group + 0.0f);
+        uint32_t bound = 0;
+#pragma unroll
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t higher = bound | 1u << bit;
+            if (__popcll(__ballot(mine >= higher)) >= k) bound = higher;
         }
-        if (rank == k - 1) reached = group;
+        if (lane == 0) reached = bound;
     }
     __syncthreads();
-    const float bound = reached;
-    if (most >= bound && bound > -INFINITY) {
-        for (int at = begin + static_cast<int>(threadIdx.x) * VEC; at < end; at += BLOCK * VEC) {
-            float v[VEC];
-            load_vector<T>(v, row, at, end);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (v[j] >= bound) {
+    const float bound = value_of(reached);
+    // A wave looks through the elements of its threads that reach it, one thread after the other, a lane to an element.
+    uint64_t hot = __ballot(most >= bound && bound > -INFINITY);
+    while (hot != 0) {
+        const int thread = wave * 64 + __builtin_ctzll(hot);
+        hot &= hot - 1;
+        for (int first = begin + thread * VEC; first < end; first += 64 * BLOCK) {
+            const int at = first + lane / VEC * (BLOCK * VEC) + lane % VEC;
+            if (at < end) {
+                const float v = to_float(row[at]);
+                if (v >= bound) {
                     const int to = atomicAdd(&count, 1);
-                    if (to < kCandidates) candidates[to] = key_of(v[j], at + j);
+                    if (to < kCandidates) candidates[to] = key_of(v, at);
                 }
+            }
         }
     }
     __syncthreads();
@@ -150,8 +157,10 @@ __device__ __forceinline__ void alternatives(const T* row, int begin, int end, i
     for (int i = 0; i < k; ++i) {
         uint64_t best = 0;
         for (int at = begin + static_cast<int>(threadIdx.x) * VEC; at < end; at += BLOCK * VEC) {
+            Raw<T, VEC> raw;
             float v[VEC];
-            load_vector<T>(v, row, at, end);
+            raw.load(row, at, end - at);
+            take<T>(v, raw, end - at);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 const uint64_t key = key_of(v[j], at + j);
@@ -172,16 +181,24 @@ __device__ __forceinline__ void alternatives(const T* row, int begin, int end, i
     }
 }
 
-// Scores of a row from its statistics and its k keys.
+// The given token's logit, which the first thread sends for before the row is read.
+struct Given {
+    bool there;
+    float logit;
+};
 template <typename T>
-__device__ __forceinline__ void finish(const ScoreArgs& p, int64_t r, const Stats& v, const uint64_t* keys) {
+__device__ __forceinline__ Given given_token(const ScoreArgs& p, int64_t r) {
+    const int64_t token = p.tokens == nullptr ? -1 : p.tokens[r];
+    const bool there = token >= 0 && token < p.V;
+    return {there, there ? to_float(static_cast<const T*>(p.logits)[r * p.row + token]) : 0.0f};
+}
+
+// Scores of a row from its statistics and its k keys.
+__device__ __forceinline__ void finish(const ScoreArgs& p, int64_t r, const Stats& v, const Given& given, const uint64_t* keys) {
     const bool none = v.s == 0.0f;              // nothing is left of the row
     const float log_s = none ? 0.0f : logf(v.s);
     if (threadIdx.x == 0) {
-        const int64_t token = p.tokens == nullptr ? -1 : p.tokens[r];
-        float logprob = 0.0f;
-        if (token >= 0 && token < p.V) logprob = none ? -INFINITY : (to_float(static_cast<const T*>(p.logits)[r * p.row + token]) - v.M) - log_s;
-        p.logprob[r] = logprob;
+        p.logprob[r] = !given.there ? 0.0f : (none ? -INFINITY : (given.logit - v.M) - log_s);
         p.entropy[r] = none ? 0.0f : log_s - kLn2 * (v.t / v.s);
         if (p.stats != nullptr) p.stats[r] = make_float2(v.M, v.s);
     }
@@ -193,18 +210,30 @@ __device__ __forceinline__ void finish(const ScoreArgs& p, int64_t r, const Stat
 }
 
 template <typename T, int BLOCK>
-__global__ __launch_bounds__(BLOCK) void token_scores_kernel(ScoreArgs p) {
+__global__ __launch_bounds__(BLOCK, 8) void token_scores_kernel(ScoreArgs p) {
     constexpr int VEC = kVec<T>;
     __shared__ uint64_t top[kMostAlternatives];
     const int64_t r = blockIdx.x / p.splits;
     const int split = static_cast<int>(blockIdx.x - r * p.splits), begin = split * p.span, end = begin + p.span < p.V ? begin + p.span : p.V;
     const T* row = static_cast<const T*>(p.logits) + r * p.row;
+    Given given{false, 0.0f};
+    if (p.splits == 1 && threadIdx.x == 0) given = given_token<T>(p, r);
     Stats mine{-INFINITY, 0.0f, 0.0f};
-    for (int at = begin + static_cast<int>(threadIdx.x) * VEC; at < end; at += kBatch * BLOCK * VEC) {
+    Raw<T, VEC> now[kBatch], next[kBatch];
+    const auto fetch = [&](int at) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) next[u].load(row, at + u * BLOCK * VEC, end - at - u * BLOCK * VEC);
+    };
+    int at = begin + static_cast<int>(threadIdx.x) * VEC;
+    fetch(at);
+    for (; at < end; at += kBatch * BLOCK * VEC) {
         float v[kBatch][VEC];
         float most = mine.M;
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) load_vector<T>(v[u], row, at + u * BLOCK * VEC, end);
+        for (int u = 0; u < kBatch; ++u) now[u] = next[u];
+        if (at + kBatch * BLOCK * VEC < end) fetch(at + kBatch * BLOCK * VEC);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) take<T>(v[u], now[u], end - at - u * BLOCK * VEC);
 #pragma unroll
         for (int u = 0; u < kBatch; ++u)
 #pragma unroll
@@ -228,7 +257,7 @@ __global__ __launch_bounds__(BLOCK) void token_scores_kernel(ScoreArgs p) {
         __syncthreads();
     }
     if (p.splits == 1) {
-        finish<T>(p, r, all, top);
+        finish(p, r, all, given, top);
         return;
     }
     if (threadIdx.x == 0) p.parts[blockIdx.x] = make_float4(all.M, all.s, all.t, 0.0f);
@@ -242,6 +271,8 @@ __global__ __launch_bounds__(256) void join_scores_kernel(ScoreArgs p) {
     __shared__ uint64_t candidates[kMostSplits * kMostAlternatives], top[kMostAlternatives];
     __shared__ int count;
     const int64_t r = blockIdx.x;
+    Given given{false, 0.0f};
+    if (threadIdx.x == 0) given = given_token<T>(p, r);
     const float4 first = p.parts[r * p.splits];
     Stats all{first.x, first.y, first.z};
     for (int i = 1; i < p.splits; ++i) {
@@ -261,7 +292,7 @@ __global__ __launch_bounds__(256) void join_scores_kernel(ScoreArgs p) {
         rank_keys<256>(candidates, count, p.k, top);
         __syncthreads();
     }
-    finish<T>(p, r, all, top);
+    finish(p, r, all, given, top);
 }
 
 template <typename T>
@@ -280,29 +311,19 @@ __global__ __launch_bounds__(256) void token_scores_backward_kernel(ScoreArgs p)
     // -p (g + h (log p + entropy)) with log p = ln2 z - log s
     const float constant = none ? 0.0f : fmaf(h, p.saved_entropy[r] - logf(stats.y), g), slope = h * kLn2;
     for (int at = begin + static_cast<int>(threadIdx.x) * VEC; at < end; at += 256 * VEC) {
+        Raw<T, VEC> raw;
         float v[VEC];
-        load_vector<T>(v, row, at, end);
+        raw.load(row, at, end - at);
+        take<T>(v, raw, end - at);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             const float z = exponent(v[j], c), probability = __builtin_amdgcn_exp2f(z) * inverse;
             v[j] = -probability * fmaf(slope, z, constant);
             if (given && !none && at + j == token) v[j] += g;
         }
-        if (at + VEC <= end) {
-            typename Words<T, VEC>::type w;
-            if constexpr (sizeof(T) == 4) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) w[j] = __float_as_uint(v[j]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; j += 2) w[j / 2] = pair_word<T>(v[j], v[j + 1]);
-            }
-            *reinterpret_cast<typename Words<T, VEC>::type*>(out + at) = w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (at + j < end) out[at + j] = from_float<T>(v[j]);
-        }
+        for (int j = 0; j < VEC; j += 2) raw.put(j, v[j], v[j + 1]);
+        raw.store(out, at, end - at);
     }
 }
 
