@@ -1,0 +1,218 @@
+"""The sequence operators as they are used together: norm, projections, recurrence, gate and norm and residual, logits, scores. Training with its
+gradients, a prompt followed by single tokens, and both captured in graphs and replayed.
+
+Tolerances. Every stage by itself is off by at most 128 u (u = 2^-24) of its largest output, as the operators' own tests bound it, with a product
+over 64 channels at 64 u among them, and by half a step of its type where it rounds to 16 bits. What that comes to at the end is worked out in
+float64 on the CPU: the same run with each stage's output, and in the backward pass each stage's gradient, moved by that much with random signs,
+eight times. Those are worst cases of all stages at once, so four times the largest deviation seen bounds what a right run may be off by."""
+import pytest
+import torch
+
+from helpers import DEV, gen
+
+D, VOCABULARY = 64, 211
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+class Moved(torch.autograd.Function):
+    """y with each element, and its gradient, moved by `by` of the largest, in random directions."""
+
+    @staticmethod
+    def forward(ctx, y, by, g):
+        ctx.by, ctx.g = by, g
+        return Moved.move(y, by, g)
+
+    @staticmethod
+    def backward(ctx, d):
+        return Moved.move(d, ctx.by, ctx.g), None, None
+
+    @staticmethod
+    def move(y, by, g):
+        signs = torch.randint(0, 2, y.shape, generator=g).to(y.dtype) * 2 - 1
+        return y + signs * by * y.abs().max() if y.numel() else y
+
+
+def weights(dtype, seed):
+    g = gen(seed)
+    draw = lambda *shape: (torch.randn(*shape, generator=g) * shape[0] ** -0.5).to(dtype)
+    return {"w_in": draw(D, 3 * D), "w_out": draw(D, VOCABULARY), "n1": (1 + 0.1 * torch.randn(D, generator=g)).to(dtype),
+            "n2": (1 + 0.1 * torch.randn(D, generator=g)).to(dtype), "n3": (1 + 0.1 * torch.randn(D, generator=g)).to(dtype),
+            "scale": (0.5 + 0.1 * torch.randn(D, generator=g)).to(dtype)}
+
+
+def plain(p, residual, state, tokens, starts=None, lengths=None, moved=lambda y: y):
+    """float64, [T, N, D]."""
+    norm = lambda v: v * torch.rsqrt((v * v).mean(-1, keepdim=True) + 1e-6)
+    T = residual.shape[0]
+    both = moved(norm(residual) * p["n1"]) @ p["w_in"]
+    x, gate, out_gate = moved(both).split(D, -1)
+    h, hs = state, []
+    for t in range(T):
+        a = torch.sigmoid(gate[t])
+        before = h if starts is None else torch.where(starts[t][:, None], torch.zeros_like(h), h)
+        new = a * before + (1 - a) * x[t]
+        live = torch.ones(residual.shape[1], dtype=torch.bool) if lengths is None else t < lengths
+        h = torch.where(live[:, None], new, h)
+        hs.append(torch.where(live[:, None], new, torch.zeros_like(new)))
+    branch = moved(torch.stack(hs))
+    after = residual + p["scale"] * out_gate * torch.sigmoid(out_gate) * norm(branch) * p["n2"]
+    logits = moved(moved(norm(after) * p["n3"]) @ p["w_out"])
+    logp = torch.log_softmax(logits, -1)
+    given = tokens >= 0
+    logprob = torch.where(given, logp.gather(-1, tokens.clamp(min=0)[..., None])[..., 0], torch.zeros_like(logp[..., 0]))
+    return moved(logprob), moved(-(logp.exp() * logp).sum(-1)), moved(after), moved(h)
+
+
+def fused(p, residual, state, tokens, starts=None, lengths=None, top_k=0):
+    from triton_snn_fusion_amd.runtime.hip_block_norm_backend import run_hip_block_norm
+    from triton_snn_fusion_amd.runtime.hip_gated_recurrence_backend import run_hip_gated_recurrence
+    from triton_snn_fusion_amd.runtime.hip_token_scores_backend import run_hip_token_scores
+    _, normed = run_hip_block_norm(residual, next_weight=p["n1"])
+    x, gate, out_gate = (normed @ p["w_in"]).split(D, -1)
+    h, state = run_hip_gated_recurrence(x, gate, state, starts=starts, lengths=lengths)
+    after, normed = run_hip_block_norm(residual, h, out_gate, p["n2"], p["n3"], p["scale"])
+    return run_hip_token_scores(normed @ p["w_out"], tokens, top_k=top_k), after, state
+
+
+def operands(T, N, dtype, seed):
+    g = gen(seed)
+    residual = torch.randn(T, N, D, generator=g).to(dtype)
+    state = torch.randn(N, D, generator=g)
+    tokens = torch.randint(0, VOCABULARY, (T, N), generator=g)
+    tokens[torch.rand(T, N, generator=g) < 0.1] = -100
+    return residual, state, tokens
+
+
+def stage_error(dtype):
+    return 128 * 2.0 ** -24 + (torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0)
+
+
+def expected(p, residual, state, tokens, dtype, **masks):
+    """Float64 outputs and gradients, and what each may be off by."""
+    d = torch.randn(tokens.shape, generator=gen(5))
+
+    def once(moved):
+        leaves = {k: v.double().requires_grad_(True) for k, v in {**p, "residual": residual, "state": state}.items()}
+        w = {k: v for k, v in leaves.items() if k not in ("residual", "state")}
+        outs = plain(w, leaves["residual"], leaves["state"], tokens, moved=moved, **masks)
+        loss = (outs[0] * d).sum() + 0.1 * outs[1].sum() + (outs[3] ** 2).sum()
+        return list(outs), torch.autograd.grad(loss, list(leaves.values()))
+
+    outs, grads = once(lambda y: y)
+    off = [0.0] * (len(outs) + len(grads))
+    for k in range(8):
+        g = gen(100 + k)
+        o, q = once(lambda y: Moved.apply(y, stage_error(dtype), g))
+        off = [max(m, float((a - b).detach().abs().max())) for m, a, b in zip(off, [*o, *q], [*outs, *grads])]
+    return d, outs, grads, [4 * m for m in off]
+
+
+def near(got, want, off, what):
+    diff = (got.detach().double().cpu() - want.detach()).abs().max()
+    assert float(diff) <= off, f"{what}: off by {float(diff):.3e}, may be {off:.3e} (largest {float(want.abs().max()):.3e})"
+
+
+def cases(T, N, masks):
+    starts = (torch.rand(T, N, generator=gen(3)) < 0.1) if "starts" in masks else None
+    lengths = torch.randint(0, T + 1, (N,), generator=gen(4)) if "lengths" in masks else None
+    return starts, lengths
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,N,masks", [(1, 3, ""), (24, 5, ""), (24, 5, "starts"), (30, 4, "starts lengths"), (300, 2, "lengths")])
+def test_training(hip_ops, T, N, masks, dtype):
+    p, (residual, state, tokens) = weights(dtype, 1), operands(T, N, dtype, 2)
+    starts, lengths = cases(T, N, masks)
+    if lengths is not None:  # padding carries no token
+        tokens = torch.where(torch.arange(T)[:, None] < lengths, tokens, torch.full_like(tokens, -100))
+    d, outs, grads, off = expected(p, residual, state, tokens, dtype, starts=starts, lengths=lengths)
+    leaves = {k: v.to(DEV).requires_grad_(True) for k, v in {**p, "residual": residual, "state": state}.items()}
+    on = lambda t: None if t is None else t.to(DEV)
+    scores, after, last = fused(leaves, leaves["residual"], leaves["state"], tokens.to(DEV), on(starts), on(lengths))
+    loss = (scores.logprob * d.to(DEV)).sum() + 0.1 * scores.entropy.sum() + (last ** 2).sum()
+    got = torch.autograd.grad(loss, list(leaves.values()))
+    for what, a, b, m in zip(("logprob", "entropy", "residual", "state"), (scores.logprob, scores.entropy, after, last), outs, off):
+        near(a, b, m, what)
+    for what, a, b, m in zip(leaves, got, grads, off[4:]):
+        assert a.dtype == leaves[what].dtype and a.shape == leaves[what].shape
+        near(a, b, m, "gradient of " + what)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_prompt_and_then_single_tokens(hip_ops, dtype):
+    """One captured step replayed for every token, its state kept in place, against the whole sequence at once."""
+    T, N, prompt = 40, 6, 29
+    p, (residual, state, tokens) = weights(dtype, 1), operands(T, N, dtype, 7)
+    _, outs, _, off = expected(p, residual, state, tokens, dtype)
+    p, residual, state, tokens = {k: v.to(DEV) for k, v in p.items()}, residual.to(DEV), state.to(DEV), tokens.to(DEV)
+    with torch.no_grad():
+        whole, after, last = fused(p, residual, state, tokens)
+        near(whole.logprob, outs[0], off[0], "logprob")
+        head, _, kept = fused(p, residual[:prompt], state, tokens[:prompt])
+        near(head.logprob, outs[0][:prompt], off[0], "logprob of the prompt")
+        step_residual, step_token = residual[prompt:prompt + 1].clone(), tokens[prompt:prompt + 1].clone()
+        cell = kept.clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            fused(p, step_residual, cell, step_token, top_k=4)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            scores, step_after, new = fused(p, step_residual, cell, step_token, top_k=4)
+            cell.copy_(new)
+        eager = kept.clone()
+        for t in range(prompt, T):
+            step_residual.copy_(residual[t:t + 1])
+            step_token.copy_(tokens[t:t + 1])
+            graph.replay()
+            want, want_after, eager = fused(p, residual[t:t + 1], eager, tokens[t:t + 1], top_k=4)
+            torch.cuda.synchronize()
+            for a, b in zip((*scores, step_after, cell), (*want, want_after, eager)):
+                assert torch.equal(a, b)
+            near(scores.logprob[0], outs[0][t], off[0], f"logprob of token {t}")
+            near(scores.entropy[0], outs[1][t], off[1], f"entropy of token {t}")
+            near(step_after[0], outs[2][t], off[2], f"residual of token {t}")
+        near(cell, outs[3], off[3], "state")
+
+
+@pytest.mark.gpu
+def test_two_captured_training_steps(hip_ops):
+    """Two graphs of forward and backward, replayed in turn on their own streams with eager work between: each has scratch memory of its own."""
+    graphs = []
+    for seed, (T, N) in enumerate([(300, 2), (40, 64)]):
+        p, (residual, state, tokens) = weights(torch.bfloat16, seed), operands(T, N, torch.bfloat16, 20 + seed)
+        leaves = {k: v.to(DEV).requires_grad_(True) for k, v in {**p, "residual": residual, "state": state}.items()}
+        tokens = tokens.to(DEV)
+
+        def step(leaves=leaves, tokens=tokens):
+            scores, _, last = fused(leaves, leaves["residual"], leaves["state"], tokens)
+            ones = torch.ones_like(scores.logprob)
+            return torch.autograd.grad([scores.logprob, scores.entropy, last], list(leaves.values()), [ones, ones, torch.ones_like(last)])
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graphs.append((graph, out, step, side))
+    for _ in range(4):
+        for graph, out, _, side in graphs:
+            for t in out:
+                t.zero_()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                graph.replay()
+        torch.cuda.synchronize()
+        for graph, out, step, _ in graphs:
+            want = step()
+            torch.cuda.synchronize()
+            for a, b in zip(out, want):
+                assert torch.equal(a, b)
