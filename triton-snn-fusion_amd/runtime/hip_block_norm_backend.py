@@ -145,8 +145,11 @@ def run_hip_block_norm(residual: torch.Tensor, branch: Optional[torch.Tensor] = 
         factor, scale = float(scale), None
     shape = residual.shape
     like = residual if branch is None else branch
-    if residual.numel() == 0:
-        return (residual if branch is None else residual.clone()), torch.empty(shape, dtype=like.dtype, device=residual.device)
+    if residual.numel() == 0:        # no rows, but differentiable in every operand
+        none = like.clone()
+        for t in (residual, gate, branch_weight, next_weight, scale):
+            none = none if t is None else none * t.to(like.dtype)
+        return (residual if branch is None else none.to(residual.dtype)), none
     rows = [None if t is None else flat_rows(t) for t in (residual, branch, gate)]
     vectors = [None if t is None else t.contiguous() for t in (branch_weight, next_weight, scale)]
     options = (factor, KINDS[kind], GATE_FORMS[gate_form], float(eps))

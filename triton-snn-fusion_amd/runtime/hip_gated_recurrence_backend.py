@@ -116,8 +116,9 @@ def run_hip_gated_recurrence(x_seq: torch.Tensor, gate_seq: torch.Tensor, state:
         apart, and h_seq has x_seq's order in memory.
     state: [N, D] float32 before the first step (None: zeros). The returned state is float32 and new memory; T = 0 returns it unchanged.
     starts: [T, N] bool. Where set, the state is dropped before the step (several documents packed into one sequence); what the state
-        held, infinities and NaN among it, does not reach the steps from there on.
-    lengths: [N] int32 or int64, clamped to 0..T. Steps from there on are padding: x_seq and gate_seq are not read, h_seq is 0, the state stays.
+        held, infinities and NaN among it, does not reach the steps from there on. Nothing else ends a NaN.
+    lengths: [N] int32 or int64, clamped to 0..T. Steps from there on are padding: what x_seq, gate_seq and starts hold there does not
+        matter, h_seq is 0, the state stays.
 
     Arithmetic is float32 throughout, outputs are rounded once. Differentiable once, in x_seq, gate_seq and state.
     """
@@ -130,7 +131,7 @@ def run_hip_gated_recurrence(x_seq: torch.Tensor, gate_seq: torch.Tensor, state:
     T, N, D = (int(n) for n in x_seq.shape)
     if T == 0:
         last = torch.zeros((N, D), dtype=torch.float32, device=x_seq.device) if state is None else state.clone()
-        return x_seq.clone(), last
+        return x_seq * gate_seq, last        # nothing, but differentiable
     x, gate = unit_rows(x_seq), unit_rows(gate_seq)
     if state is not None:
         state = state.contiguous()

@@ -101,7 +101,7 @@ def run_hip_token_scores(logits: torch.Tensor, tokens: Optional[torch.Tensor] = 
     refuse("run_hip_token_scores", check_token_scores_support(logits, tokens, top_k))
     lead = logits.shape[:-1]
     if logits.numel() == 0:
-        zeros = logits.new_zeros(lead, dtype=torch.float32)
+        zeros = logits.sum(-1, dtype=torch.float32)        # no rows, but differentiable
         return TokenScores(zeros, zeros.clone(), logits.new_zeros((*lead, top_k), dtype=torch.float32) if top_k else None,
                            logits.new_zeros((*lead, top_k), dtype=torch.int64) if top_k else None)
     rows = flat_rows(logits)
