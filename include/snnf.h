@@ -460,12 +460,12 @@ typedef enum snnf_recurrence_form {
 } snnf_recurrence_form;
 
 /* Gated linear recurrence over [T, N, D]. `x`, `gate` and `h` have elements of a row next to each other and any element strides over
- * steps (`*_step`) and sequences (`*_row`); `gate` may have strides of 0. `h` overlaps neither input.
+ * steps (`*_step`, not negative, 16 steps within 2 GiB) and sequences (`*_row`); strides of 0 broadcast an input. `h` overlaps neither input.
  *   starts    NULL or a byte per (step, sequence), element strides as above: where it is not 0 the state is dropped before the step
  *   lengths   NULL or N: steps from there on leave the state as it is and read 0 in `h`
  *   state     NULL (zeros) or [N, D] float32; `state_out` [N, D] float32, not the same memory
  *   marks     NULL, or snnf_gated_recurrence_marks_bytes(T, N, D, dtype) bytes that the backward pass will read
- *   workspace snnf_gated_recurrence_workspace_bytes(...) bytes, 4-byte aligned (0: none needed), in use until the call's work is done
+ *   workspace snnf_gated_recurrence_workspace_bytes(...) bytes, 16-byte aligned (0: none needed), in use until the call's work is done
  * T >= 1. Two launches where the sequences are few and long, else one. */
 size_t snnf_gated_recurrence_workspace_bytes(int T, int N, int D, int dtype, int backward);
 size_t snnf_gated_recurrence_marks_bytes(int T, int N, int D, int dtype);
@@ -475,7 +475,7 @@ int snnf_gated_recurrence(const void* x, int64_t x_step, int64_t x_row, const vo
                           size_t workspace_bytes, void* stream);
 
 /* Its gradient: `dh` and `dstate` (NULL: zeros) are the gradients of `h` and of the last state, `dx`, `dgate` (not broadcast) and `dstate_in`
- * those of `x`, `gate` and `state`. Steps from a sequence's length on get 0. `marks` as the forward call on the same operands left them. */
+ * (not dstate's memory) those of `x`, `gate` and `state`. Steps from a sequence's length on get 0. `marks` as the forward call on the same operands left them. */
 int snnf_gated_recurrence_backward(const void* x, int64_t x_step, int64_t x_row, const void* gate, int64_t gate_step, int64_t gate_row, const void* dh,
                                    int64_t dh_step, int64_t dh_row, int T, int N, int D, int dtype, int form, const void* starts,
                                    int64_t starts_step, int64_t starts_row, const int32_t* lengths, const float* marks, const float* dstate,

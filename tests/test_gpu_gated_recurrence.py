@@ -177,6 +177,47 @@ def test_what_is_masked_may_hold_anything(hip_ops, T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,N", [(20, 3), (700, 2), (700, 64)])
+@pytest.mark.parametrize("form", ["leaky", "linear"])
+def test_what_is_not_a_number_stays_until_a_start(hip_ops, T, N, form):
+    """Decays whose product vanishes drop nothing: NaN lasts to the end of its sequence or to the next start, with starts given or not."""
+    D = 130
+    x, gate, state, _, _ = operands(T, N, D, torch.float32, form, 16)
+    gate = torch.full_like(gate, -30.0 if form == "leaky" else 1e-9)
+    x[3, 0, 5] = float("nan")
+    starts = torch.zeros(T, N, dtype=torch.bool, device=DEV)
+    without, given = run(x, gate, state, form=form), run(x, gate, state, form=form, starts=starts)
+    starts[T // 2, 0] = True
+    dropped = run(x, gate, state, form=form, starts=starts)
+    assert bool(without[0][3:, 0, 5].isnan().all()) and int(without[0].isnan().sum()) == T - 3 and int(without[1].isnan().sum()) == 1
+    for a, b in zip(without, given):
+        assert torch.allclose(a, b, rtol=0, atol=0, equal_nan=True)
+    assert bool(dropped[0][3:T // 2, 0, 5].isnan().all()) and int(dropped[0].isnan().sum()) == T // 2 - 3 and not bool(dropped[1].isnan().any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,N", [(20, 3), (700, 2), (700, 64)])
+def test_growth_of_nothing_is_nothing(hip_ops, T, N):
+    """Gates of 2 grow past the range of float32 over a run, and 0 stays 0; with a start, what grew is gone."""
+    D = 130
+    leaves = [torch.zeros(T, N, D, device=DEV), torch.full((T, N, D), 2.0, device=DEV), torch.zeros(N, D, device=DEV)]
+    starts = torch.zeros(T, N, dtype=torch.bool, device=DEV)
+    starts[T // 2] = True
+    for mask in (None, starts):
+        for t in leaves:
+            t.requires_grad_(True)
+        h, last = run(*leaves, form="linear", starts=mask)
+        got = torch.autograd.grad([h, last], leaves, [torch.zeros_like(h), torch.zeros_like(last)])
+        for t in (h, last, *got):
+            assert bool((t == 0).all())
+    x = torch.zeros(T, N, D, device=DEV)
+    x[0] = 1.0
+    h, last = run(x, leaves[1].detach(), form="linear", starts=starts)
+    want = torch.exp2(torch.arange(T // 2, dtype=torch.float64)).to(torch.float32).to(DEV)          # infinite from 2^128 on
+    assert torch.equal(h[:T // 2], want[:, None, None].expand(T // 2, N, D)) and bool((h[T // 2:] == 0).all()) and bool((last == 0).all())
+
+
+@pytest.mark.gpu
 def test_strided_operands_and_a_broadcast_gate(hip_ops):
     """Slices of one projection and a gate per channel go in without copies; the expanded gate's gradient is summed."""
     T, N, D = 90, 2, 96
@@ -313,6 +354,10 @@ def test_entry_points_refuse_before_any_gpu_work(snnf_lib):
     assert forward(T=0) == -1 and forward(N=-1) == -1 and forward(dtype=9) == -1 and forward(form=2) == -1
     assert forward(x=None) == -1 and b"non-null" in snnf_lib.snnf_last_error()
     assert forward(state_out=None) == -1 and forward(N=0, x=None) == 0 and forward(D=0, x=None) == 0
+    assert f(16, 16, 8, 16, 16, 8, 4, 2, 8, 0, 0, None, 0, 0, None, 32, 16, 16, 8, 32, None, None, 0, None) == -1        # the state in place
+    assert b"same memory" in snnf_lib.snnf_last_error()
+    assert b(16, 16, 8, 16, 16, 8, 16, 16, 8, 4, 2, 8, 0, 0, None, 0, 0, None, 16, 32, 16, 16, 8, 16, 16, 8, 32, None, 0, None) == -1
+    assert b"same memory" in snnf_lib.snnf_last_error()
     assert forward(T=(1 << 30) + 1) == -2
     assert snnf_lib.snnf_gated_recurrence_workspace_bytes(100000, 1, 64, 1, 0) > 0
     assert forward(T=100000, N=1, D=64, dtype=1) == -4 and b"workspace" in snnf_lib.snnf_last_error()

@@ -216,3 +216,104 @@ def test_two_captured_training_steps(hip_ops):
             torch.cuda.synchronize()
             for a, b in zip(out, want):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_no_rows_are_still_differentiable(hip_ops):
+    """A shard of a batch that got nothing: gradients of no elements, zeros for the parameters."""
+    from triton_snn_fusion_amd.runtime.hip_block_norm_backend import run_hip_block_norm
+    from triton_snn_fusion_amd.runtime.hip_gated_recurrence_backend import run_hip_gated_recurrence
+    from triton_snn_fusion_amd.runtime.hip_token_scores_backend import run_hip_token_scores
+    rows, vectors = [torch.empty(0, 8, device=DEV, requires_grad=True) for _ in range(3)], [torch.ones(8, device=DEV, requires_grad=True) for _ in range(3)]
+    out, normed = run_hip_block_norm(*rows, *vectors)
+    assert out.shape == normed.shape == (0, 8)
+    for k in (out, normed):
+        for t, g in zip((*rows, *vectors), torch.autograd.grad(k.sum(), (*rows, *vectors), retain_graph=True)):
+            assert g.shape == t.shape and bool((g == 0).all())
+    scores = run_hip_token_scores(rows[0], torch.empty(0, dtype=torch.int64, device=DEV), top_k=2)
+    assert torch.autograd.grad((scores.logprob + scores.entropy).sum(), rows[0])[0].shape == (0, 8)
+    for shape in ((0, 2, 8), (3, 0, 8)):
+        x, gate = torch.empty(shape, device=DEV, requires_grad=True), torch.empty(shape, device=DEV, requires_grad=True)
+        state = torch.ones(shape[1:], device=DEV, requires_grad=True)
+        h, last = run_hip_gated_recurrence(x, gate, state)
+        grads = torch.autograd.grad(h.sum() + last.sum(), (x, gate, state))
+        assert [g.shape for g in grads] == [x.shape, gate.shape, state.shape] and bool((grads[2] == 1).all())
+
+
+def far_apart(t, *strides):
+    """t's elements with these strides, in memory of its own."""
+    span = 1 + sum((n - 1) * s for n, s in zip(t.shape, strides))
+    out = torch.empty(span, dtype=t.dtype, device=DEV).as_strided(t.shape, strides)
+    out.copy_(t)
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("operator", ["steps", "sequences", "norm", "scores"])
+def test_offsets_past_32_bits(hip_ops, operator):
+    from triton_snn_fusion_amd.runtime.hip_block_norm_backend import run_hip_block_norm
+    from triton_snn_fusion_amd.runtime.hip_gated_recurrence_backend import run_hip_gated_recurrence
+    from triton_snn_fusion_amd.runtime.hip_token_scores_backend import run_hip_token_scores
+    g = gen(11)
+    far = 1 << 30
+    if operator in ("steps", "sequences"):
+        T, N, D = (70, 1, 96) if operator == "steps" else (20, 4, 96)
+        near_by = [torch.randn(T, N, D, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2)]
+        strides = (far >> 4, D, 1) if operator == "steps" else (D, far, 1)
+        call = run_hip_gated_recurrence
+    else:
+        near_by = [torch.randn(4, 200, generator=g).to(torch.bfloat16).to(DEV) for _ in range(1 if operator == "scores" else 2)]
+        strides = (far, 1)
+        tokens = torch.tensor([3, 199, 0, 7], device=DEV)
+        call = run_hip_block_norm if operator == "norm" else (lambda x: run_hip_token_scores(x, tokens, top_k=3))
+    answers = []
+    for operands_ in (near_by, [far_apart(t, *strides) for t in near_by]):
+        leaves = [t.requires_grad_(True) for t in operands_]
+        out = [t for t in call(*leaves) if t.is_floating_point()]
+        used = [t for t in out if t.requires_grad]
+        answers.append([*out, *torch.autograd.grad(used, leaves, [torch.ones_like(t) for t in used])])
+        del leaves, operands_
+    for a, b in zip(*answers):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_more_elements_than_32_bits_count(hip_ops):
+    """Rows of one tensor with more than 2^31 elements, against the last of them by themselves."""
+    from triton_snn_fusion_amd.runtime.hip_block_norm_backend import run_hip_block_norm
+    from triton_snn_fusion_amd.runtime.hip_gated_recurrence_backend import run_hip_gated_recurrence
+    from triton_snn_fusion_amd.runtime.hip_token_scores_backend import run_hip_token_scores
+    rows, width = (1 << 20) + 5, 2056
+    x = torch.empty(rows, width, dtype=torch.bfloat16, device=DEV)
+    x[:-9].fill_(0.25)
+    x[-9:] = torch.randn(9, width, generator=gen(12)).to(torch.bfloat16).to(DEV)
+    x.requires_grad_(True)
+    tail = x.detach()[-9:].clone().requires_grad_(True)
+    tokens = torch.arange(rows, device=DEV) % width
+    for call in (lambda t: run_hip_block_norm(t, t), lambda t: run_hip_token_scores(t, tokens[rows - t.shape[0]:])[:2],
+                 lambda t: run_hip_gated_recurrence(t[None], t[None])):
+        big, small = call(x), call(tail)
+        grad = torch.autograd.grad(big, x, [torch.ones_like(t) for t in big])[0][-9:]
+        want = torch.autograd.grad(small, tail, [torch.ones_like(t) for t in small])[0]
+        for a, b in zip(big, small):
+            assert torch.equal(a.reshape(-1, *a.shape[1:] if a.shape[0] == rows else a.shape[2:])[-9:], b.reshape(-1, *b.shape[1:] if b.shape[0] == 9 else b.shape[2:]))
+        assert torch.equal(grad, want)
+        del big, grad
+
+
+@pytest.mark.gpu
+def test_more_rows_than_a_launch_has_threads_for(hip_ops):
+    """17 million short rows, a workgroup each: the last of them as by themselves."""
+    from triton_snn_fusion_amd.runtime.hip_token_scores_backend import run_hip_token_scores
+    rows, width = (1 << 24) + 3, 10
+    x = torch.zeros(rows, width, device=DEV)
+    x[-9:] = torch.randn(9, width, generator=gen(13)).to(DEV)
+    x.requires_grad_(True)
+    tail = x.detach()[-9:].clone().requires_grad_(True)
+    tokens = torch.arange(rows, device=DEV) % width
+    big, small = run_hip_token_scores(x, tokens, top_k=2), run_hip_token_scores(tail, tokens[-9:], top_k=2)
+    for a, b in zip(big, small):
+        assert torch.equal(a[-9:], b)
+    ones = torch.ones(rows, device=DEV)
+    grad = torch.autograd.grad([big.logprob, big.entropy], x, [ones, ones])[0]
+    assert torch.equal(grad[-9:], torch.autograd.grad([small.logprob, small.entropy], tail, [ones[:9], ones[:9]])[0])

@@ -65,13 +65,20 @@ __device__ __forceinline__ uint8_t start_of(const Args& p, int n, int first, int
     return lane < steps && first + lane < lim ? p.starts[static_cast<int64_t>(first + lane) * p.starts_step + static_cast<int64_t>(n) * p.starts_row] : 0;
 }
 
-// One link of the chain: what a run of steps makes of the value that enters it. A run that drops the value has A = 0, and must not multiply
-// an infinity or NaN that belongs to what came before.
+// One link of the chain: what a run of steps makes of the value that enters it. Of 0 it makes H, whatever A may have grown to. A run that
+// drops the value says so by A = -0, which no other run has, and must not multiply an infinity or NaN that belongs to what came before; A = 0
+// from decays that vanish does.
+constexpr uint32_t kDropped = 0x80000000u;
+template <bool STARTS>
+__device__ __forceinline__ bool dropped(float A) { return STARTS && __float_as_uint(A) == kDropped; }
 template <bool STARTS>
 __device__ __forceinline__ float link(float A, float entering, float H) {
-    const float v = fmaf(A, entering, H);
-    if constexpr (STARTS) return A == 0.0f ? H : v;
-    return v;
+    return entering == 0.0f || dropped<STARTS>(A) ? H : fmaf(A, entering, H);
+}
+template <bool STARTS>
+__device__ __forceinline__ float run_of(float A, bool drops) {
+    if constexpr (STARTS) return drops ? __uint_as_float(kDropped) : A + 0.0f;      // -0 + 0 = 0
+    return A;
 }
 
 // What is left of the value that enters a run: the product of its decays, or for a long memory 1 - c.
@@ -270,7 +277,7 @@ __device__ __forceinline__ void reduce(const float (&a)[S][VEC], const float (&b
             A[j] *= a[i][j];
         }
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) A[j] = STARTS && drop != 0 ? 0.0f : left_over(A[j], c[j]);
+    for (int j = 0; j < VEC; ++j) A[j] = run_of<STARTS>(left_over(A[j], c[j]), drop != 0);
 }
 
 // The W runs of a tile as one: A in row `w * rows`, H `second` rows behind it.
@@ -278,6 +285,7 @@ template <int W, bool STARTS>
 __device__ __forceinline__ void join(float (*links)[64], int rows, int second, bool reversed, float& A, float& H) {
     const int lane = threadIdx.x & 63;
     float c = 0.0f;
+    bool drops = false;
     A = 1.0f, H = 0.0f;
 #pragma unroll 4
     for (int i = 0; i < W; ++i) {
@@ -286,8 +294,9 @@ __device__ __forceinline__ void join(float (*links)[64], int rows, int second, b
         H = link<STARTS>(Aw, H, links[w * rows + second][lane]);
         A *= Aw;
         c = fmaf(1.0f - Aw, 1.0f - c, c);
+        drops = drops || dropped<STARTS>(Aw);
     }
-    A = STARTS && A == 0.0f ? 0.0f : left_over(A, c);
+    A = run_of<STARTS>(left_over(A, c), drops);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -466,7 +475,9 @@ template <typename Tile, int VEC, int W, bool STARTS>
 __global__ __launch_bounds__(64 * W) void walk_kernel(Args p) {
     constexpr int kRows = Tile::kParts * VEC;
     __shared__ float links[2][W * kRows][64];
-    const Place q = place<VEC>(p, blockIdx.x);
+    const uint32_t column = group_index();
+    if (column >= static_cast<uint32_t>(p.columns)) return;
+    const Place q = place<VEC>(p, column);
     const int lane = threadIdx.x & 63, wave = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
     Tile tile;
     int t0 = Tile::at(p, 0);
@@ -602,7 +613,7 @@ size_t workspace_of(int T, int N, int D, int dtype, bool backward) {
 
 template <typename XT, int VEC, bool STARTS, bool LEAKY, int W, int S>
 void walk(const Args& p, bool backward, hipStream_t stream) {
-    const dim3 grid(p.columns), block(64 * W);
+    const dim3 grid = grid_of(p.columns), block(64 * W);
     if constexpr (W > 1) {
         if (backward) {
             walk_kernel<BackwardTile<XT, VEC, W, S, STARTS, LEAKY>, VEC, W, STARTS><<<grid, block, 0, stream>>>(p);
@@ -707,6 +718,7 @@ extern "C" int snnf_gated_recurrence(const void* x, int64_t x_step, int64_t x_ro
     if (N == 0 || D == 0) return SNNF_OK;
     if (x == nullptr || gate == nullptr || h == nullptr || state_out == nullptr)
         return fail(SNNF_ERR_INVALID_ARGUMENT, "snnf_gated_recurrence: x, gate, h and state_out must be non-null");
+    if (state == state_out) return fail(SNNF_ERR_INVALID_ARGUMENT, "snnf_gated_recurrence: state and state_out must not be the same memory");
     Args p = {};
     p.x = {x, x_step, x_row};
     p.gate = {gate, gate_step, gate_row};
@@ -734,6 +746,7 @@ extern "C" int snnf_gated_recurrence_backward(const void* x, int64_t x_step, int
     if (N == 0 || D == 0) return SNNF_OK;
     if (x == nullptr || gate == nullptr || dh == nullptr || marks == nullptr || dx == nullptr || dgate == nullptr || dstate_in == nullptr)
         return fail(SNNF_ERR_INVALID_ARGUMENT, "snnf_gated_recurrence_backward: x, gate, dh, marks, dx, dgate and dstate_in must be non-null");
+    if (dstate == dstate_in) return fail(SNNF_ERR_INVALID_ARGUMENT, "snnf_gated_recurrence_backward: dstate and dstate_in must not be the same memory");
     Args p = {};
     p.x = {x, x_step, x_row};
     p.gate = {gate, gate_step, gate_row};

@@ -26,6 +26,14 @@ __device__ __forceinline__ void leak(float g, float& a, float& rest) {
     rest = e * a;
 }
 
+// Workgroups that are as many as a long tensor has rows: a launch takes fewer than 2^32 threads along x, so that the rest goes along y. Those behind
+// the last one have nothing to do.
+inline dim3 grid_of(int64_t groups) {
+    constexpr int64_t kAlong = 1 << 21;
+    return groups <= kAlong ? dim3(static_cast<unsigned>(groups)) : dim3(kAlong, static_cast<unsigned>((groups + kAlong - 1) / kAlong));
+}
+__device__ __forceinline__ uint32_t group_index() { return blockIdx.y * gridDim.x + blockIdx.x; }
+
 // The value of the lane `MASK` apart, by exchange within the register file (a shuffle through LDS takes several times as long). Which lane
 // that is for 4 and 8, where rows of 8 and 16 lanes are mirrored, does not matter to a sum or maximum that has been taken over the smaller
 // distances before.

@@ -213,8 +213,10 @@ template <typename T, int BLOCK>
 __global__ __launch_bounds__(BLOCK, 8) void token_scores_kernel(ScoreArgs p) {
     constexpr int VEC = kVec<T>;
     __shared__ uint64_t top[kMostAlternatives];
-    const int64_t r = blockIdx.x / p.splits;
-    const int split = static_cast<int>(blockIdx.x - r * p.splits), begin = split * p.span, end = begin + p.span < p.V ? begin + p.span : p.V;
+    const uint32_t group = group_index();
+    if (group >= p.rows * p.splits) return;
+    const int64_t r = group / p.splits;
+    const int split = static_cast<int>(group - r * p.splits), begin = split * p.span, end = begin + p.span < p.V ? begin + p.span : p.V;
     const T* row = static_cast<const T*>(p.logits) + r * p.row;
     Given given{false, 0.0f};
     if (p.splits == 1 && threadIdx.x == 0) given = given_token<T>(p, r);
@@ -260,8 +262,8 @@ __global__ __launch_bounds__(BLOCK, 8) void token_scores_kernel(ScoreArgs p) {
         finish(p, r, all, given, top);
         return;
     }
-    if (threadIdx.x == 0) p.parts[blockIdx.x] = make_float4(all.M, all.s, all.t, 0.0f);
-    if (static_cast<int>(threadIdx.x) < p.k) p.keys[static_cast<int64_t>(blockIdx.x) * p.k + threadIdx.x] = top[threadIdx.x];
+    if (threadIdx.x == 0) p.parts[group] = make_float4(all.M, all.s, all.t, 0.0f);
+    if (static_cast<int>(threadIdx.x) < p.k) p.keys[static_cast<int64_t>(group) * p.k + threadIdx.x] = top[threadIdx.x];
 }
 
 // Joins the splits of a row: one workgroup of 256 threads.
@@ -270,7 +272,8 @@ template <typename T>
 __global__ __launch_bounds__(256) void join_scores_kernel(ScoreArgs p) {
     __shared__ uint64_t candidates[kMostSplits * kMostAlternatives], top[kMostAlternatives];
     __shared__ int count;
-    const int64_t r = blockIdx.x;
+    const int64_t r = group_index();
+    if (r >= p.rows) return;
     Given given{false, 0.0f};
     if (threadIdx.x == 0) given = given_token<T>(p, r);
     const float4 first = p.parts[r * p.splits];
@@ -298,8 +301,10 @@ __global__ __launch_bounds__(256) void join_scores_kernel(ScoreArgs p) {
 template <typename T>
 __global__ __launch_bounds__(256) void token_scores_backward_kernel(ScoreArgs p) {
     constexpr int VEC = kVec<T>;
-    const int64_t r = blockIdx.x / p.splits;
-    const int begin = static_cast<int>(blockIdx.x - r * p.splits) * p.span, end = begin + p.span < p.V ? begin + p.span : p.V;
+    const uint32_t group = group_index();
+    if (group >= p.rows * p.splits) return;
+    const int64_t r = group / p.splits;
+    const int begin = static_cast<int>(group - r * p.splits) * p.span, end = begin + p.span < p.V ? begin + p.span : p.V;
     const T* row = static_cast<const T*>(p.logits) + r * p.row;
     T* out = static_cast<T*>(p.d_logits) + r * p.V;
     const float2 stats = p.saved[r];
@@ -362,10 +367,10 @@ int check_scores(const char* name, int64_t rows, int V, int dtype, int k) {
 
 template <typename T>
 void launch_scores(const ScoreArgs& p, const ScoreShape& s, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(p.rows * s.splits));
+    const dim3 grid = grid_of(p.rows * s.splits);
     if (s.block == 256) token_scores_kernel<T, 256><<<grid, dim3(256), 0, stream>>>(p);
     else token_scores_kernel<T, 1024><<<grid, dim3(1024), 0, stream>>>(p);
-    if (s.splits > 1) join_scores_kernel<T><<<dim3(static_cast<unsigned>(p.rows)), dim3(256), 0, stream>>>(p);
+    if (s.splits > 1) join_scores_kernel<T><<<grid_of(p.rows), dim3(256), 0, stream>>>(p);
 }
 
 }  // namespace
@@ -428,7 +433,7 @@ extern "C" int snnf_token_scores_backward(const void* logits, int64_t row, int64
     p.saved_entropy = entropy;
     p.d_logprob = d_logprob, p.d_entropy = d_entropy;
     p.d_logits = d_logits;
-    const dim3 grid(static_cast<unsigned>(rows * p.splits)), block(256);
+    const dim3 grid = grid_of(rows * p.splits), block(256);
     hipStream_t hs = as_stream(stream);
     if (dtype == SNNF_F32) token_scores_backward_kernel<float><<<grid, block, 0, hs>>>(p);
     else if (dtype == SNNF_BF16) token_scores_backward_kernel<bf16_t><<<grid, block, 0, hs>>>(p);
