@@ -26,6 +26,8 @@ namespace {
 // 7.2), 4 where workgroups cover for each other (512 x 64 x 2048: 78 us, 8 waves 80).
 constexpr int kRelayWaves = 14, kRelaySteps = 16, kRelayBackSteps = 8;
 constexpr int kWalkWaves = 8, kWalkWavesMany = 4, kWalkSteps = 8;
+// Marks are left by the wave whose run begins where a tile of the backward pass does.
+static_assert(kRelayWaves * kRelayBackSteps % kRelaySteps == 0);
 // Tiles that a relay looks back at in one go: more of them reach further where all tiles start at once, and cost their loads where most
 // tiles in front are done (8192 x 1 x 1024: 2 28.6 us, 4 23.5, 8 22.4, 16 24.5; 16384 x 2 x 2048: 92, 94, 102, 111).
 constexpr int kReach = 4;
