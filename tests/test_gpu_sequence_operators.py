@@ -278,6 +278,61 @@ def test_offsets_past_32_bits(hip_ops, operator):
 
 
 @pytest.mark.gpu
+def test_steps_too_far_apart_are_refused(hip_ops, monkeypatch):
+    """Sixteen steps more than 2 GiB apart, from the dispatch module and from Python, with and without gradients."""
+    from triton_snn_fusion_amd.runtime import hip_gated_recurrence_backend as backend
+    x = torch.empty(19 * (1 << 27) + 8, dtype=torch.bfloat16, device=DEV).as_strided((20, 1, 8), (1 << 27, 8, 1))
+    for _ in range(2):
+        for gradient in (False, True):
+            with pytest.raises(RuntimeError, match="unsupported_stride"):
+                backend.run_hip_gated_recurrence(x.detach().requires_grad_(gradient), x)
+        monkeypatch.setattr(backend, "native", lambda t: None)
+    x = x[::10]
+    assert backend.run_hip_gated_recurrence(x[:1].zero_(), x[:1])[0].shape == (1, 1, 8)
+
+
+@pytest.mark.gpu
+def test_orders_that_differ_between_operands(hip_ops):
+    """x with steps outermost, the gate with sequences outermost, gradients with either, channels apart: the same bits."""
+    from triton_snn_fusion_amd.runtime.hip_gated_recurrence_backend import run_hip_gated_recurrence
+    g = gen(14)
+    T, N, D = 270, 3, 130
+    x, gate, dh = (torch.randn(T, N, D, generator=g).to(torch.bfloat16).to(DEV) for _ in range(3))
+    orders = [lambda t: t, lambda t: t.transpose(0, 1).contiguous().transpose(0, 1), lambda t: t.permute(2, 0, 1).contiguous().permute(1, 2, 0),
+              lambda t: torch.stack([t, t], -1)[..., 0]]
+    answers = []
+    for a, b, c in ((0, 0, 0), (0, 1, 1), (1, 0, 0), (2, 3, 2), (3, 1, 3), (1, 2, 0)):
+        leaves = [orders[a](x).detach().requires_grad_(True), orders[b](gate).detach().requires_grad_(True)]
+        h, last = run_hip_gated_recurrence(*leaves)
+        answers.append([h, last, *torch.autograd.grad([h, last], leaves, [orders[c](dh), torch.ones_like(last)])])
+    for other in answers[1:]:
+        for p, q in zip(answers[0], other):
+            assert torch.equal(p, q)
+
+
+@pytest.mark.gpu
+def test_one_tensor_in_several_places(hip_ops):
+    """The same leaf as x and gate, as residual, branch and gate, as all three vectors: its gradient is the sum."""
+    from triton_snn_fusion_amd.runtime.hip_block_norm_backend import run_hip_block_norm
+    from triton_snn_fusion_amd.runtime.hip_gated_recurrence_backend import run_hip_gated_recurrence
+    g = gen(15)
+    t = torch.randn(33, 2, 70, generator=g).to(DEV)
+    w = torch.rand(70, generator=g).to(DEV)
+    for call, roles in ((lambda *a: run_hip_gated_recurrence(*a), (t, t)),
+                        (lambda *a: run_hip_block_norm(*a), (t, t, t, w, w, w))):
+        one = {id(r): r.clone().requires_grad_(True) for r in roles}
+        apart = [r.clone().requires_grad_(True) for r in roles]
+        out, want = call(*(one[id(r)] for r in roles)), call(*apart)
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        got = torch.autograd.grad(out, list(one.values()), [torch.ones_like(a) for a in out])
+        separate = torch.autograd.grad(want, apart, [torch.ones_like(a) for a in want])
+        for k, grad in zip(one, got):
+            parts = [s for s, r in zip(separate, roles) if id(r) == k]
+            # sums of at most six terms in either order
+            assert bool(((grad - sum(parts)).abs() <= 6 * 2.0 ** -24 * sum(p.abs() for p in parts)).all())
+
+
+@pytest.mark.gpu
 def test_more_elements_than_32_bits_count(hip_ops):
     """Rows of one tensor with more than 2^31 elements, against the last of them by themselves."""
     from triton_snn_fusion_amd.runtime.hip_block_norm_backend import run_hip_block_norm
