@@ -261,9 +261,9 @@ def test_graph_replays_and_other_streams(hip_ops):
     dev = [t[n].to(DEV).requires_grad_(True) for n in NAMES]
     d_res, d_norm = d_res.to(DEV), d_norm.to(DEV)
 
-    def step():
+    def step():        # its autograd graph ends with it: none of the same leaves lives during a capture
         out = run(dev[0], dev[1], gate=dev[2], branch_weight=dev[3], next_weight=dev[4], scale=dev[5])
-        return [*out, *torch.autograd.grad(out, dev, [d_res, d_norm])]
+        return [*(t.detach() for t in out), *torch.autograd.grad(out, dev, [d_res, d_norm])]
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):

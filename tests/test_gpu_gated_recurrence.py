@@ -283,9 +283,9 @@ def test_graph_replays_and_other_streams(hip_ops):
     x, gate, state, dh, dlast = operands(T, N, D, torch.bfloat16, "leaky", 51)
     leaves = [t.requires_grad_(True) for t in (x, gate, state)]
 
-    def step():
+    def step():        # its autograd graph ends with it: none of the same leaves lives during a capture
         out = run(*leaves)
-        return [*out, *torch.autograd.grad(out, leaves, [dh, dlast])]
+        return [*(t.detach() for t in out), *torch.autograd.grad(out, leaves, [dh, dlast])]
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):

@@ -209,9 +209,9 @@ def test_graph_replays_and_other_streams(hip_ops, rows, V):
     leaf, tokens = x.to(DEV).requires_grad_(True), tokens.to(DEV)
     ones = torch.ones(rows, device=DEV)
 
-    def step():
+    def step():        # its autograd graph ends with it: none of the same leaves lives during a capture
         out = run(leaf, tokens, top_k=6)
-        return [*out, torch.autograd.grad(out[:2], leaf, [ones, ones])[0]]
+        return [*(t.detach() for t in out), torch.autograd.grad(out[:2], leaf, [ones, ones])[0]]
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
