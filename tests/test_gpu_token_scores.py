@@ -134,6 +134,33 @@ def test_equal_values_go_by_the_lower_index(hip_ops, dtype):
     check(x, torch.tensor([0, 8]), 30)
 
 
+FILLS = {"few": lambda x, g: x.masked_fill(torch.rand(x.shape, generator=g) >= 5.0 / x.shape[-1], -math.inf),
+         "lowest": lambda x, g: x.masked_fill(torch.rand(x.shape, generator=g) >= 5.0 / x.shape[-1], torch.finfo(x.dtype).min),
+         "neighbours": lambda x, g: torch.where((torch.arange(x.shape[-1]) >= 100) & (torch.arange(x.shape[-1]) < 290), x, torch.full_like(x, -math.inf)),
+         "same": lambda x, g: torch.full_like(x, 1.5),
+         "end": lambda x, g: torch.where(torch.arange(x.shape[-1]) < x.shape[-1] - 50, torch.full_like(x, -3.0), x.abs()),
+         "signs": lambda x, g: torch.where(torch.rand(x.shape, generator=g) < 0.5, torch.zeros_like(x), -torch.zeros_like(x)),
+         "first": lambda x, g: torch.where(torch.arange(x.shape[-1]) == 0, x, torch.full_like(x, -math.inf)),
+         "last": lambda x, g: torch.where(torch.arange(x.shape[-1]) == x.shape[-1] - 1, x, torch.full_like(x, -math.inf)),
+         "nan": lambda x, g: torch.full_like(x, -math.inf).masked_fill(torch.rand(x.shape, generator=g) < 0.9, math.nan)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fill", FILLS)
+@pytest.mark.parametrize("rows,V", [(3, 70), (5, 300), (3, 1000), (2, 9001), (600, 5003), (2, 33000), (2, 150001)])
+def test_alternatives_where_few_elements_count(hip_ops, rows, V, fill):
+    """Masks that leave fewer than top_k, masks of the type's lowest value, rows of one value: the lower index first, NaN behind everything."""
+    g = gen(31)
+    for dtype in (torch.bfloat16, torch.float32):
+        x = FILLS[fill](logits((rows,), V, dtype, 32)[0], g)
+        order = torch.sort(torch.where(x.isnan(), torch.full_like(x.double(), -math.inf), x.double()), dim=-1, descending=True, stable=True).indices
+        if fill == "nan":         # minus infinity first, then the others, each by the index
+            order = torch.sort(x.isnan().double(), dim=-1, stable=True).indices
+        for k in (1, 5, 20, 64):
+            got = run(x.to(DEV), top_k=k)
+            assert torch.equal(got.top_token.cpu(), order[:, :k]), (dtype, k)
+
+
 @pytest.mark.gpu
 def test_far_values(hip_ops):
     """Logits far from each other and far from 0: differences are what counts."""

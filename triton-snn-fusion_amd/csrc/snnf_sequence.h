@@ -46,13 +46,13 @@ __device__ __forceinline__ float across(float v) {
     else if constexpr (MASK == 8) return __int_as_float(__builtin_amdgcn_update_dpp(bits, bits, 0x140, 0xf, 0xf, false));  // 16 lanes mirrored
     else return __shfl_xor(v, MASK, 64);
 }
-// Over groups of `lanes` (8 to 64) neighbouring lanes, in every lane, always in the same order: with the rows of 16 lanes summed, the exchange of
+// Over groups of `lanes` (4 to 64) neighbouring lanes, in every lane, always in the same order: with the rows of 16 lanes summed, the exchange of
 // rows or halves leaves one half's value in one register and the other's in the other.
 template <typename Op>
 __device__ __forceinline__ float over_lanes(float v, int lanes, Op op) {
     v = op(v, across<1>(v));
     v = op(v, across<2>(v));
-    v = op(v, across<4>(v));
+    if (lanes >= 8) v = op(v, across<4>(v));
     if (lanes >= 16) v = op(v, across<8>(v));
     if (lanes >= 32) {
         const auto pair = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);

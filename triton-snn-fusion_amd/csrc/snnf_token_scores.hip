@@ -6,6 +6,8 @@
 // bound by latency: 16 x 32000 bf16 5.2 us, with 8 alternatives 7.9.
 // Alternatives: the threads' maxima, as 64 groups by lane, give a value that at least k elements reach (their k-th largest), and only threads
 // whose own maximum reaches it look through their elements again, which the caches still hold; a few dozen candidates are ranked by counting.
+// Where a mask leaves fewer than k, or many share the bound, those above it are ranked and the rest taken from those at it in order of the index
+// (500 x 50021 bf16 with 20 alternatives: 18 us, five elements left 24, with one maximum after the other 250; all of one value 24 and 281).
 // Ties go to the lower index: an element's key is its value, in an order of unsigned numbers, above the complement of its index.
 #include "snnf_sequence.h"
 
@@ -13,7 +15,8 @@ namespace snnf {
 namespace {
 
 constexpr int kMostAlternatives = 64;
-constexpr int kCandidates = 1024;       // candidates that are ranked at once; rows with more (many equal values) select one by one
+constexpr int kCandidates = 512;        // candidates that are ranked at once
+constexpr int kAtOnce = 4;              // elements a thread compares at once in the search for those equal to a bound
 constexpr int kBatch = 2;               // vectors a thread works on while as many are on their way
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
@@ -50,25 +53,21 @@ __device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
     return {M, a.s * fa + b.s * fb, fa * fmaf(za, a.s, a.t) + fb * fmaf(zb, b.s, b.t)};
 }
 
-// All threads' statistics as one, in every thread.
+// All threads' statistics as one, in every thread. A lane reads one wave's share, so that a few exchanges join 16 of them.
 template <int BLOCK>
 __device__ __forceinline__ Stats join_all(Stats v) {
-    __shared__ float largest[BLOCK / 64], sums[2][BLOCK / 64];
-    const int wave = threadIdx.x >> 6;
+    constexpr int WAVES = BLOCK / 64;
+    __shared__ float largest[WAVES], sums[2][WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, other = lane % WAVES;
     float M = lane_max(v.M);
-    if ((threadIdx.x & 63) == 0) largest[wave] = M;
+    if (lane == 0) largest[wave] = M;
     __syncthreads();
-    M = largest[0];
-#pragma unroll
-    for (int w = 1; w < BLOCK / 64; ++w) M = fmaxf(M, largest[w]);
+    M = lane_max(largest[other], WAVES);
     const float z = exponent(v.M, center(M)), f = __builtin_amdgcn_exp2f(z);
     const float s = lane_sum(v.s * f), t = lane_sum(f * fmaf(z, v.s, v.t));
-    if ((threadIdx.x & 63) == 0) sums[0][wave] = s, sums[1][wave] = t;
+    if (lane == 0) sums[0][wave] = s, sums[1][wave] = t;
     __syncthreads();
-    v = {M, 0.0f, 0.0f};
-#pragma unroll
-    for (int w = 0; w < BLOCK / 64; ++w) v.s += sums[0][w], v.t += sums[1][w];
-    return v;
+    return {M, lane_sum(sums[0][other], WAVES), lane_sum(sums[1][other], WAVES)};
 }
 
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -111,6 +110,7 @@ __device__ __forceinline__ void alternatives(const T* row, int begin, int end, i
     __shared__ uint32_t reached;
     __shared__ int count;
     __shared__ uint64_t candidates[kCandidates];
+    __shared__ int counts[kAtOnce][WAVES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     maxima[wave][lane] = most;
     if (threadIdx.x == 0) count = 0;
@@ -131,29 +131,64 @@ __device__ __forceinline__ void alternatives(const T* row, int begin, int end, i
     }
     __syncthreads();
     const float bound = value_of(reached);
-    // A wave looks through the elements of its threads that reach it, one thread after the other, a lane to an element.
-    uint64_t hot = __ballot(most >= bound && bound > -INFINITY);
-    while (hot != 0) {
-        const int thread = wave * 64 + __builtin_ctzll(hot);
-        hot &= hot - 1;
-        for (int first = begin + thread * VEC; first < end; first += 64 * BLOCK) {
-            const int at = first + lane / VEC * (BLOCK * VEC) + lane % VEC;
-            if (at < end) {
-                const float v = to_float(row[at]);
-                if (v >= bound) {
-                    const int to = atomicAdd(&count, 1);
-                    if (to < kCandidates) candidates[to] = key_of(v, at);
+    // A wave looks through the elements of its threads that reach it (or pass it), one thread after the other, a lane to an element.
+    const auto collect = [&](auto counts) {
+        uint64_t hot = __ballot(counts(most));
+        while (hot != 0) {
+            if (*const_cast<volatile int*>(&count) > kCandidates) break;
+            const int thread = wave * 64 + __builtin_ctzll(hot);
+            hot &= hot - 1;
+            for (int first = begin + thread * VEC; first < end; first += 64 * BLOCK) {
+                const int at = first + lane / VEC * (BLOCK * VEC) + lane % VEC;
+                if (at < end) {
+                    const float v = to_float(row[at]);
+                    if (counts(v)) {
+                        const int to = atomicAdd(&count, 1);
+                        if (to < kCandidates) candidates[to] = key_of(v, at);
+                    }
                 }
             }
         }
+        __syncthreads();
+        return count;
+    };
+    if (bound > -INFINITY) {
+        const int found = collect([&](float v) { return v >= bound; });
+        if (found >= k && found <= kCandidates) {
+            rank_keys<BLOCK>(candidates, found, k, out);
+            return;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) count = 0;
+        __syncthreads();
     }
-    __syncthreads();
-    const int found = count;
-    if (found >= k && found <= kCandidates) {
-        rank_keys<BLOCK>(candidates, found, k, out);
-        return;
+    // A mask leaves fewer than k, or many are equal (masked by a lowest value, say): those above the bound, then the first of those at it.
+    const int above = collect([&](float v) { return v > bound; });
+    if (above <= kCandidates) {
+        rank_keys<BLOCK>(candidates, above, k, out);
+        int filled = above;
+        for (int from = begin; from < end && filled < k; from += kAtOnce * BLOCK) {
+            uint64_t same[kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int at = from + u * BLOCK + static_cast<int>(threadIdx.x);
+                same[u] = __ballot(at < end && to_float(row[at < end ? at : begin]) == bound);
+                if (lane == 0) counts[u][wave] = __popcll(same[u]);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                for (int w = 0; w < WAVES; ++w) {
+                    const int to = filled + __popcll(same[u] & ((1ull << lane) - 1));
+                    if (w == wave && (same[u] >> lane & 1) && to < k) out[to] = key_of(bound, from + u * BLOCK + static_cast<int>(threadIdx.x));
+                    filled += counts[u][w];
+                }
+            }
+            __syncthreads();
+        }
+        if (filled >= k) return;
     }
-    // Few elements that count, or many equal ones: the largest key below the last, k times.
+    // Anything else (NaN among the few that count): the largest key below the last, k times.
     uint64_t last = ~0ull;
     for (int i = 0; i < k; ++i) {
         uint64_t best = 0;
