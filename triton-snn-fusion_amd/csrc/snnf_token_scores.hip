@@ -4,7 +4,7 @@
 // One pass over the logits: every thread keeps (M, s, t) of its elements, rescaled when a batch brings a larger maximum, and the workgroup joins
 // them in a fixed order. Bound by memory: 8192 x 32000 bf16 97 us (5.4 TB/s) and its gradient, which reads and writes, 184 us (5.7). A few rows are
 // bound by latency: 16 x 32000 bf16 5.2 us, with 8 alternatives 7.9.
-// Alternatives: the threads' maxima, as 64 groups by lane, give a value that at least k elements reach (their k-th largest), and only threads
+// Alternatives: the threads' maxima, as 64 or 256 groups, give a value that at least k elements reach (their k-th largest), and only threads
 // whose own maximum reaches it look through their elements again, which the caches still hold; a few dozen candidates are ranked by counting.
 // Where a mask leaves fewer than k, or many share the bound, those above it are ranked and the rest taken from those at it in order of the index
 // (500 x 50021 bf16 with 20 alternatives: 18 us, five elements left 24, with one maximum after the other 250; all of one value 24 and 281).
@@ -15,7 +15,8 @@ namespace snnf {
 namespace {
 
 constexpr int kMostAlternatives = 64;
-constexpr int kCandidates = 512;        // candidates that are ranked at once
+constexpr int kCandidates = 1024;       // candidates that are ranked at once
+constexpr int kEqual = 512;             // more than these at or above a bound: many may be equal to it
 constexpr int kAtOnce = 4;              // elements a thread compares at once in the search for those equal to a bound
 constexpr int kBatch = 2;               // vectors a thread works on while as many are on their way
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
@@ -116,26 +117,43 @@ __device__ __forceinline__ void alternatives(const T* row, int begin, int end, i
     if (threadIdx.x == 0) count = 0;
     __syncthreads();
     if (wave == 0) {
-        float group = maxima[0][lane];
+        // The k-th largest of 64 groups, or of 256 where 64 would be few for k (512 x 32000 bf16 with 64 alternatives 31 us, 102 by 64 groups, since
+        // several hundred elements reach the smallest maximum; with 20 the four counts for a bit cost more, 20.2 and 19.8), bit by bit: the largest number
+        // that k of them reach.
+        constexpr int kQuarters = 4;
+        float group[kQuarters];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) group = fmaxf(group, maxima[w][lane]);
-        // The k-th largest, bit by bit: the largest number that k of them reach.
-        const uint32_t mine = order_of(group + 0.0f);
+        for (int w = 0; w < WAVES; ++w) group[w % kQuarters] = w < kQuarters ? maxima[w][lane] : fmaxf(group[w % kQuarters], maxima[w][lane]);
         uint32_t bound = 0;
+        if (k <= 32) {
+            const uint32_t mine = order_of(fmaxf(fmaxf(group[0], group[1]), fmaxf(group[2], group[3])) + 0.0f);
 #pragma unroll
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t higher = bound | 1u << bit;
-            if (__popcll(__ballot(mine >= higher)) >= k) bound = higher;
+            for (int bit = 31; bit >= 0; --bit) {
+                const uint32_t higher = bound | 1u << bit;
+                if (__popcll(__ballot(mine >= higher)) >= k) bound = higher;
+            }
+        } else {
+            uint32_t mine[kQuarters];
+#pragma unroll
+            for (int q = 0; q < kQuarters; ++q) mine[q] = order_of(group[q] + 0.0f);
+#pragma unroll 4
+            for (int bit = 31; bit >= 0; --bit) {
+                const uint32_t higher = bound | 1u << bit;
+                int reach = 0;
+#pragma unroll
+                for (int q = 0; q < kQuarters; ++q) reach += __popcll(__ballot(mine[q] >= higher));
+                if (reach >= k) bound = higher;
+            }
         }
         if (lane == 0) reached = bound;
     }
     __syncthreads();
     const float bound = value_of(reached);
     // A wave looks through the elements of its threads that reach it (or pass it), one thread after the other, a lane to an element.
-    const auto collect = [&](auto counts) {
+    const auto collect = [&](int room, auto counts) {
         uint64_t hot = __ballot(counts(most));
         while (hot != 0) {
-            if (*const_cast<volatile int*>(&count) > kCandidates) break;
+            if (*const_cast<volatile int*>(&count) > room) break;
             const int thread = wave * 64 + __builtin_ctzll(hot);
             hot &= hot - 1;
             for (int first = begin + thread * VEC; first < end; first += 64 * BLOCK) {
@@ -153,8 +171,8 @@ __device__ __forceinline__ void alternatives(const T* row, int begin, int end, i
         return count;
     };
     if (bound > -INFINITY) {
-        const int found = collect([&](float v) { return v >= bound; });
-        if (found >= k && found <= kCandidates) {
+        const int found = collect(kEqual, [&](float v) { return v >= bound; });
+        if (found >= k && found <= kEqual) {
             rank_keys<BLOCK>(candidates, found, k, out);
             return;
         }
@@ -163,7 +181,7 @@ __device__ __forceinline__ void alternatives(const T* row, int begin, int end, i
         __syncthreads();
     }
     // A mask leaves fewer than k, or many are equal (masked by a lowest value, say): those above the bound, then the first of those at it.
-    const int above = collect([&](float v) { return v > bound; });
+    const int above = collect(kCandidates, [&](float v) { return v > bound; });
     if (above <= kCandidates) {
         rank_keys<BLOCK>(candidates, above, k, out);
         int filled = above;
@@ -188,7 +206,7 @@ __device__ __forceinline__ void alternatives(const T* row, int begin, int end, i
         }
         if (filled >= k) return;
     }
-    // Anything else (NaN among the few that count): the largest key below the last, k times.
+    // Anything else (more than fit above the bound, NaN among the few that count): the largest key below the last, k times.
     uint64_t last = ~0ull;
     for (int i = 0; i < k; ++i) {
         uint64_t best = 0;
