@@ -218,6 +218,25 @@ def test_growth_of_nothing_is_nothing(hip_ops, T, N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,N,D", [(1, 40, 3), (20, 33, 5), (300, 17, 24), (520, 2, 65), (40, 300, 1)])
+def test_narrow_rows_side_by_side(hip_ops, T, N, D, dtype):
+    """Sequences that lie next to each other run as one of more channels: the same bits as apart, whichever pass sees them so."""
+    check(T, N, D, dtype, "leaky", 17)
+    x, gate, state, dh, dlast = operands(T, N, D, dtype, "leaky", 18)
+    apart = lambda t: torch.cat([t, t], 2)[:, :, :D] if t.dim() == 3 else t
+    answers = []
+    for inputs, outputs in ((lambda t: t, lambda t: t), (apart, apart), (lambda t: t, apart), (apart, lambda t: t)):
+        leaves = [inputs(t).detach().requires_grad_(True) for t in (x, gate, state)]
+        out = run(*leaves)
+        answers.append([*out, *torch.autograd.grad(out, leaves, [outputs(dh), dlast])])
+    alone = run(x, gate, state, lengths=torch.full((N,), T, dtype=torch.int32, device=DEV))
+    for other in answers[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(answers[0], other))
+    assert all(torch.equal(a, b) for a, b in zip(answers[0], alone))
+
+
+@pytest.mark.gpu
 def test_strided_operands_and_a_broadcast_gate(hip_ops):
     """Slices of one projection and a gate per channel go in without copies; the expanded gate's gradient is summed."""
     T, N, D = 90, 2, 96
