@@ -153,7 +153,6 @@ __device__ __forceinline__ void alternatives(const T* row, int begin, int end, i
     const auto collect = [&](int room, auto counts) {
         uint64_t hot = __ballot(counts(most));
         while (hot != 0) {
-            if (*const_cast<volatile int*>(&count) > room) break;
             const int thread = wave * 64 + __builtin_ctzll(hot);
             hot &= hot - 1;
             for (int first = begin + thread * VEC; first < end; first += 64 * BLOCK) {
@@ -166,6 +165,7 @@ __device__ __forceinline__ void alternatives(const T* row, int begin, int end, i
                     }
                 }
             }
+            if (hot != 0 && *const_cast<volatile int*>(&count) > room) break;
         }
         __syncthreads();
         return count;
