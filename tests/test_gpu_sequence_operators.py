@@ -219,6 +219,33 @@ def test_two_captured_training_steps(hip_ops):
 
 
 @pytest.mark.gpu
+def test_calls_at_once_on_three_streams(hip_ops):
+    """Long sequences whose tiles wait for each other, training passes among them, with the chip shared: results as alone."""
+    runs = []
+    for seed, (T, N) in enumerate([(3000, 3), (2500, 9), (9000, 1)]):
+        p, (residual, state, tokens) = weights(torch.bfloat16, seed), operands(T, N, torch.bfloat16, 30 + seed)
+        leaves = {k: v.to(DEV).requires_grad_(True) for k, v in {**p, "residual": residual, "state": state}.items()}
+        tokens = tokens.to(DEV)
+
+        def step(leaves=leaves, tokens=tokens):
+            scores, after, last = fused(leaves, leaves["residual"], leaves["state"], tokens)
+            grads = torch.autograd.grad([scores.logprob, last], list(leaves.values()), [torch.ones_like(scores.logprob), torch.ones_like(last)])
+            return [scores.logprob.detach(), after.detach(), last.detach(), *grads]
+        want = step()
+        torch.cuda.synchronize()
+        runs.append((step, want, torch.cuda.Stream()))
+    for _ in range(3):
+        got = []
+        for step, _, side in runs:
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                got.append([step() for _ in range(3)][-1])
+        torch.cuda.synchronize()
+        for (_, want, _), out in zip(runs, got):
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.gpu
 def test_no_rows_are_still_differentiable(hip_ops):
     """A shard of a batch that got nothing: gradients of no elements, zeros for the parameters."""
     from triton_snn_fusion_amd.runtime.hip_block_norm_backend import run_hip_block_norm
