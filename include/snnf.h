@@ -475,7 +475,7 @@ int snnf_gated_recurrence(const void* x, int64_t x_step, int64_t x_row, const vo
                           size_t workspace_bytes, void* stream);
 
 /* Its gradient: `dh` and `dstate` (NULL: zeros) are the gradients of `h` and of the last state, `dx`, `dgate` (not broadcast) and `dstate_in`
- * (not dstate's memory) those of `x`, `gate` and `state`. Steps from a sequence's length on get 0. `marks` as the forward call on the same operands left them. */
+ * (not dstate's memory) those of `x`, `gate` and `state`; they overlap no input. Steps from a sequence's length on get 0. `marks` as the forward call on the same operands left them. */
 int snnf_gated_recurrence_backward(const void* x, int64_t x_step, int64_t x_row, const void* gate, int64_t gate_step, int64_t gate_row, const void* dh,
                                    int64_t dh_step, int64_t dh_row, int T, int N, int D, int dtype, int form, const void* starts,
                                    int64_t starts_step, int64_t starts_row, const int32_t* lengths, const float* marks, const float* dstate,

@@ -77,6 +77,8 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_float(order == 0 ? 0x7fc00000u : (order & 0x80000000u ? order & 0x7fffffffu : ~order)); }
+// Bits that can differ between numbers of a type begin here: those below are zeros of a 16-bit type's, ones below zero.
+template <typename T> inline constexpr int kLowest = sizeof(T) == 4 ? 0 : (dtype_of<T>::value == SNNF_BF16 ? 16 : 13);
 // -0 and 0 are the same value.
 __device__ __forceinline__ uint64_t key_of(float x, int index) { return static_cast<uint64_t>(order_of(x + 0.0f)) << 32 | static_cast<uint32_t>(~index); }
 
@@ -128,7 +130,7 @@ __device__ __forceinline__ void alternatives(const T* row, int begin, int end, i
         if (k <= 32) {
             const uint32_t mine = order_of(fmaxf(fmaxf(group[0], group[1]), fmaxf(group[2], group[3])) + 0.0f);
 #pragma unroll
-            for (int bit = 31; bit >= 0; --bit) {
+            for (int bit = 31; bit >= kLowest<T>; --bit) {
                 const uint32_t higher = bound | 1u << bit;
                 if (__popcll(__ballot(mine >= higher)) >= k) bound = higher;
             }
@@ -137,7 +139,7 @@ __device__ __forceinline__ void alternatives(const T* row, int begin, int end, i
 #pragma unroll
             for (int q = 0; q < kQuarters; ++q) mine[q] = order_of(group[q] + 0.0f);
 #pragma unroll 4
-            for (int bit = 31; bit >= 0; --bit) {
+            for (int bit = 31; bit >= kLowest<T>; --bit) {
                 const uint32_t higher = bound | 1u << bit;
                 int reach = 0;
 #pragma unroll
@@ -145,7 +147,7 @@ __device__ __forceinline__ void alternatives(const T* row, int begin, int end, i
                 if (reach >= k) bound = higher;
             }
         }
-        if (lane == 0) reached = bound;
+        if (lane == 0) reached = bound & 0x80000000u ? bound : bound | ((1u << kLowest<T>) - 1);
     }
     __syncthreads();
     const float bound = value_of(reached);
