@@ -3,7 +3,7 @@
 //     d x_i = d_logprob (1[i = token] - p_i) - d_entropy p_i (log p_i + entropy)
 // One pass over the logits: every thread keeps (M, s, t) of its elements, rescaled when a batch brings a larger maximum, and the workgroup joins
 // them in a fixed order. Bound by memory: 8192 x 32000 bf16 97 us (5.4 TB/s) and its gradient, which reads and writes, 184 us (5.7). A few rows are
-// bound by latency: 16 x 32000 bf16 5.2 us, with 8 alternatives 7.9.
+// bound by latency: 16 x 32000 bf16 5.2 us, with 8 alternatives 7.6.
 // Alternatives: the threads' maxima, as 64 or 256 groups, give a value that at least k elements reach (their k-th largest), and only threads
 // whose own maximum reaches it look through their elements again, which the caches still hold; a few dozen candidates are ranked by counting.
 // Where a mask leaves fewer than k, or many share the bound, those above it are ranked and the rest taken from those at it in order of the index
@@ -77,8 +77,8 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_float(order == 0 ? 0x7fc00000u : (order & 0x80000000u ? order & 0x7fffffffu : ~order)); }
-// Bits that can differ between numbers of a type begin here: those below are zeros of a 16-bit type's, ones below zero.
-template <typename T> inline constexpr int kLowest = sizeof(T) == 4 ? 0 : (dtype_of<T>::value == SNNF_BF16 ? 16 : 13);
+// Bits (an even one) from which on numbers of a type differ: those below are zeros in a 16-bit type's, ones where the order turns them.
+template <typename T> inline constexpr int kLowest = sizeof(T) == 4 ? 0 : (dtype_of<T>::value == SNNF_BF16 ? 16 : 12);
 // -0 and 0 are the same value.
 __device__ __forceinline__ uint64_t key_of(float x, int index) { return static_cast<uint64_t>(order_of(x + 0.0f)) << 32 | static_cast<uint32_t>(~index); }
 
@@ -120,8 +120,8 @@ __device__ __forceinline__ void alternatives(const T* row, int begin, int end, i
     __syncthreads();
     if (wave == 0) {
         // The k-th largest of 64 groups, or of 256 where 64 would be few for k (512 x 32000 bf16 with 64 alternatives 31 us, 102 by 64 groups, since
-        // several hundred elements reach the smallest maximum; with 20 the four counts for a bit cost more, 20.2 and 19.8), bit by bit: the largest number
-        // that k of them reach.
+        // several hundred elements reach the smallest maximum; with 20 the four counts for a bit cost more, 20.2 and 19.8), by its bits: the largest number
+        // that k of them reach, two bits at a time with one group to a lane.
         constexpr int kQuarters = 4;
         float group[kQuarters];
 #pragma unroll
@@ -130,9 +130,10 @@ __device__ __forceinline__ void alternatives(const T* row, int begin, int end, i
         if (k <= 32) {
             const uint32_t mine = order_of(fmaxf(fmaxf(group[0], group[1]), fmaxf(group[2], group[3])) + 0.0f);
 #pragma unroll
-            for (int bit = 31; bit >= kLowest<T>; --bit) {
-                const uint32_t higher = bound | 1u << bit;
-                if (__popcll(__ballot(mine >= higher)) >= k) bound = higher;
+            for (int bit = 30; bit >= kLowest<T>; bit -= 2) {
+                const int one = __popcll(__ballot(mine >= (bound | 1u << bit))), two = __popcll(__ballot(mine >= (bound | 2u << bit)));
+                const int three = __popcll(__ballot(mine >= (bound | 3u << bit)));
+                bound |= static_cast<uint32_t>((one >= k) + (two >= k) + (three >= k)) << bit;
             }
         } else {
             uint32_t mine[kQuarters];
@@ -396,7 +397,7 @@ struct ScoreShape {
 };
 
 // A workgroup to a row: 256 threads where there are rows enough to fill the chip or few elements (8192 x 32000 bf16 97 us, with 1024 threads 117;
-// 4096 x 6488 with 20 alternatives 28 and 60; 64 x 1000 float32 with 5 5.8 and 6.3), else 1024 (16 x 32000 bf16 with 8 alternatives 7.9 us, with 256
+// 4096 x 6488 with 20 alternatives 28 and 60; 64 x 1000 float32 with 5 5.8 and 6.3), else 1024 (16 x 32000 bf16 with 8 alternatives 7.6 us, with 256
 // threads 10.3; 500 x 50021 with 20 17.9 and 28.3). Few long rows are split over workgroups (1 x 200000 bf16 with 8 alternatives 14 us, in one
 // piece 20; 4 x 500000 23 and 45; about even at 128 x 100000), pieces of 16384 elements at least: a second launch joins them.
 ScoreShape score_shape(int64_t rows, int V) {
