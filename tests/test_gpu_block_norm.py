@@ -4,9 +4,13 @@ Tolerances: an output is rounded once, half a step of its type (`eps / 2` relati
 float32 values, each off by at most 2^-24 relative (sigmoid: 4), and row statistics are sums of D terms of one sign added in chains of 8 and a
 tree of at most 16 levels: 24 roundings. So C = 48 roundings of the largest magnitude that enters: of the sum for residual', of
 (|residual'| / sigma) * |weight| for normed, of r * (|d| + |unit| * mean |d unit|) for a gradient. Sums over rows add `rows` such terms."""
+import subprocess
+import sys
+
 import pytest
 import torch
 
+from conftest import ROOT
 from helpers import DEV, gen
 
 U = 2.0 ** -24
@@ -337,6 +341,25 @@ def test_refusals_without_a_gpu():
         run(torch.zeros(2, 8))
     with pytest.raises(RuntimeError, match="must be a tensor"):
         run(None)
+
+
+def test_rows_too_wide_are_left_to_the_python_implementation(snnf_lib):
+    """Widths that an int does not hold, 2^32 among them, which is 0 as an int: the dispatch module answers None before it divides by one."""
+    code = ("import torch, triton_snn_fusion_amd\nfrom triton_snn_fusion_amd import _dispatch\nfrom torch._subclasses import FakeTensorMode\n"
+            "module = _dispatch.module()\nwith FakeTensorMode():\n"
+            "    for width in (16385, 1 << 32, (1 << 32) + 8):\n"
+            "        x = torch.empty(2, width, dtype=torch.bfloat16, device='cuda')\n"
+            "        assert module.block_norm(x, x, None, None, None, None, 1.0, 0, 2, 1e-6) is None\n")
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, (done.returncode, done.stderr[-2000:])
+
+
+@pytest.mark.gpu
+def test_rows_too_wide_are_refused(hip_ops):
+    for width in (16385, 1 << 32, (1 << 32) + 8):
+        x = torch.empty(1, width, dtype=torch.bfloat16, device=DEV)
+        with pytest.raises(RuntimeError, match="run_hip_block_norm: unsupported_shape: rows of 1 to 16384"):
+            run(x, x)
 
 
 def test_entry_points_refuse_before_any_gpu_work(snnf_lib):

@@ -149,6 +149,8 @@ PyObject* gated_recurrence(Args& a) {
 // ------------------------------------------------------------------------------------------------------------------
 // Block norm
 // ------------------------------------------------------------------------------------------------------------------
+constexpr int64_t kWidestNorm = 16384;      // as the kernels take it; what follows divides by a width that fits an int
+
 struct BlockNorm : torch::autograd::Function<BlockNorm> {
     struct Shape {
         int64_t rows, row[3];
@@ -228,7 +230,7 @@ PyObject* block_norm(Args& a) {
     const double factor = a.real(6), eps = a.real(9);
     const int64_t kind = a.number(7), gate_form = a.number(8);
     int64_t stride;
-    if (!a.fine || !activation(residual) || !activation(branch) || residual.dim() < 1 || !row_stride(residual, &stride)) return none();
+    if (!a.fine || !activation(residual) || !activation(branch) || residual.dim() < 1 || residual.size(-1) > kWidestNorm || !row_stride(residual, &stride)) return none();
     if (branch.device() != residual.device() || (residual.scalar_type() != branch.scalar_type() && residual.scalar_type() != at::kFloat)) return none();
     for (const Tensor* t : {&branch, &gate})
         if (t->defined() && (!like_of(*t, residual, branch.scalar_type()) || t->sizes() != residual.sizes() || !row_stride(*t, &stride))) return none();
