@@ -399,3 +399,80 @@ def test_more_rows_than_a_launch_has_threads_for(hip_ops):
     ones = torch.ones(rows, device=DEV)
     grad = torch.autograd.grad([big.logprob, big.entropy], x, [ones, ones])[0]
     assert torch.equal(grad[-9:], torch.autograd.grad([small.logprob, small.entropy], tail, [ones[:9], ones[:9]])[0])
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# What the kernels do not see of a call
+# ------------------------------------------------------------------------------------------------------------------
+def _operators():
+    from triton_snn_fusion_amd.runtime.hip_block_norm_backend import run_hip_block_norm
+    from triton_snn_fusion_amd.runtime.hip_gated_recurrence_backend import run_hip_gated_recurrence
+    from triton_snn_fusion_amd.runtime.hip_token_scores_backend import run_hip_token_scores
+    return {"recurrence": (lambda x, other: run_hip_gated_recurrence(x, other)[0], (5, 2, 8)),
+            "norm": (lambda x, other: run_hip_block_norm(x, other)[1], (5, 8)),
+            "norm without a branch": (lambda x, other: run_hip_block_norm(x, next_weight=other[0].contiguous())[1], (5, 8)),
+            "scores": (lambda x, other: run_hip_token_scores(x * other).entropy, (5, 8))}
+
+
+def _observed(operator, device):
+    """Every way in which torch follows a call from outside, each refused by name."""
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, shape = _operators()[operator]
+    x, other = torch.randn(shape, generator=gen(1)).to(device), torch.randn(shape, generator=gen(2)).to(device)
+    for which in range(2):
+        for differentiated in (False, True):
+            leaves = [x.clone().requires_grad_(differentiated), other.clone().requires_grad_(differentiated)]
+            with forward_ad.dual_level():
+                leaves[which] = forward_ad.make_dual(leaves[which], torch.ones_like(x))
+                with pytest.raises(RuntimeError, match="unsupported_forward_ad"):
+                    call(*leaves)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="unsupported_forward_ad"):
+                    call(*leaves)
+    with pytest.raises(RuntimeError, match="unsupported_tracing"):
+        torch.jit.trace(call, (x, other), check_trace=False)
+    with pytest.raises(RuntimeError, match="unsupported_tracing"):
+        make_fx(call)(x, other)
+    stacked = torch.stack([x, x])
+    transformed = [lambda: torch.vmap(call, in_dims=(0, None))(stacked, other), lambda: torch.func.grad(lambda t: call(t, other).sum())(x),
+                   lambda: torch.vmap(call, in_dims=(None, 0))(x, stacked)]
+    for call_of in transformed:
+        with pytest.raises(RuntimeError, match="unsupported_transform"):
+            call_of()
+    if device == "cpu":
+        return
+    leaf = x.clone().requires_grad_(True)
+    out = call(leaf, other)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="unsupported_forward_ad"):
+            torch.autograd.grad(out, leaf, forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)), retain_graph=True)
+    with pytest.raises(RuntimeError, match="unsupported_transform"):
+        torch.autograd.grad(out, leaf, torch.ones(2, *out.shape, dtype=out.dtype, device=device), retain_graph=True, is_grads_batched=True)
+    with pytest.raises(RuntimeError, match="unsupported_tracing"):
+        make_fx(lambda d: torch.autograd.grad(out, leaf, d, retain_graph=True)[0])(torch.ones_like(out))
+    assert torch.autograd.grad(out, leaf, torch.ones_like(out))[0].shape == leaf.shape
+
+
+@pytest.mark.parametrize("operator", ["recurrence", "norm", "norm without a branch", "scores"])
+def test_what_follows_a_call_from_outside_is_refused_without_a_gpu(operator):
+    _observed(operator, "cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("operator", ["recurrence", "norm", "norm without a branch", "scores"])
+def test_what_follows_a_call_from_outside_is_refused(hip_ops, monkeypatch, operator):
+    """A tangent would be lost and a trace would hold memory that nothing fills; through the dispatch module and without it. Where forward-mode
+    differentiation is off a tangent is none, and the call runs."""
+    from torch.autograd import forward_ad
+    from triton_snn_fusion_amd.runtime import _sequence_common, hip_block_norm_backend, hip_gated_recurrence_backend, hip_token_scores_backend
+    call, shape = _operators()[operator]
+    x, other = torch.randn(shape, generator=gen(1)).to(DEV), torch.randn(shape, generator=gen(2)).to(DEV)
+    want = call(x, other)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with forward_ad._set_fwd_grad_enabled(False):
+            assert torch.equal(call(dual, other), want)
+    _observed(operator, DEV)
+    for backend in (_sequence_common, hip_block_norm_backend, hip_gated_recurrence_backend, hip_token_scores_backend):
+        monkeypatch.setattr(backend, "native", lambda t: None)
+    _observed(operator, DEV)

@@ -17,10 +17,12 @@
 // interpreter lock is requested.
 #include <Python.h>
 
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/jit/python/pybind_utils.h>
 #include <torch/extension.h>
 #include <torch/library.h>
@@ -1186,6 +1188,7 @@ PyObject* py_dense_pool(PyObject*, PyObject* const* args, Py_ssize_t n) { return
 PyObject* py_recurrence(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(gated_recurrence, args, n, 6); }
 PyObject* py_block_norm(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(block_norm, args, n, 10); }
 PyObject* py_scores(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(token_scores, args, n, 3); }
+PyObject* py_unobserved(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(are_unobserved, args, n, n); }
 
 PyMethodDef g_fast_methods[] = {
     {"blocked_conv", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_conv)), METH_FASTCALL, nullptr},
@@ -1198,6 +1201,7 @@ PyMethodDef g_fast_methods[] = {
     {"gated_recurrence", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_recurrence)), METH_FASTCALL, nullptr},
     {"block_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_block_norm)), METH_FASTCALL, nullptr},
     {"token_scores", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_scores)), METH_FASTCALL, nullptr},
+    {"unobserved", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_unobserved)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -16,6 +16,27 @@ inline bool activation(const Tensor& t) {
     int code;
     return t.defined() && t.is_cuda() && t.layout() == at::kStrided && dtype_code(t.scalar_type(), &code) && t.numel() > 0;
 }
+// Whether the kernels' work is all there is to a call: what traces torch's operations would record the outputs' allocation and nothing that fills them, a
+// tangent of forward-mode differentiation would be lost, and a tensor that a transform of torch.func wraps has no memory of its own.
+inline bool traced() {
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    return torch::jit::tracer::isTracing() || (Modes::any_modes_set() && Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value());
+}
+inline bool unobserved(c10::ArrayRef<const Tensor*> tensors) {
+    if (traced()) return false;
+    for (const Tensor* t : tensors)
+        if (t->defined() && (!t->has_storage() || t->_fw_grad(0).defined())) return false;
+    return true;
+}
+// The same of the gradients that autograd hands over: there is no other implementation to refuse them.
+inline void check_gradients(const char* name, const variable_list& grads) {
+    TORCH_CHECK(!traced(), name, ": unsupported_tracing: torch.jit.trace and make_fx record torch's own operations only");
+    for (const Tensor& d : grads) {
+        if (!d.defined()) continue;
+        TORCH_CHECK(d.has_storage(), name, ": unsupported_transform: a gradient is wrapped by a transform (torch.func, vmap) and has no memory of its own");
+        TORCH_CHECK(!d._fw_grad(0).defined(), name, ": unsupported_forward_ad: a gradient has a tangent, and there is no forward-mode derivative");
+    }
+}
 inline void* data_of(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 inline void check_status(int status) { TORCH_CHECK(status == 0, snnf_last_error()); }
 
@@ -83,6 +104,7 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
         return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_gradients("run_hip_gated_recurrence", grads);
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &gate = saved[1], &starts = saved[2], &lengths = saved[3], &marks = saved[4];
         const c10::DeviceGuard guard(x.device());
@@ -131,7 +153,7 @@ inline PyObject* tuple_of(const variable_list& tensors) {
 PyObject* gated_recurrence(Args& a) {
     const Tensor x = optional_tensor(a, 0), gate = optional_tensor(a, 1), state = optional_tensor(a, 2), starts = optional_tensor(a, 3), lengths = optional_tensor(a, 4);
     const int64_t form = a.number(5);
-    if (!a.fine || !activation(x) || x.dim() != 3 || !unit_rows(x) || !gate.defined()) return none();
+    if (!a.fine || !unobserved({&x, &gate, &state, &starts, &lengths}) || !activation(x) || x.dim() != 3 || !unit_rows(x) || !gate.defined()) return none();
     const int64_t T = x.size(0), N = x.size(1), D = x.size(2);
     if (std::max({T, N, D}) > (int64_t{1} << 30) || !like_of(gate, x, x.scalar_type()) || gate.sizes() != x.sizes() || !unit_rows(gate)) return none();
     if (state.defined() && (!like_of(state, x, at::kFloat) || state.dim() != 2 || state.size(0) != N || state.size(1) != D || !state.is_contiguous())) return none();
@@ -195,6 +217,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
         return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_gradients("run_hip_block_norm", grads);
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &residual = saved[0], &branch = saved[1], &gate = saved[2], &wb = saved[3], &wn = saved[4], &scale = saved[5], &stats = saved[6];
         const c10::DeviceGuard guard(residual.device());
@@ -230,7 +253,8 @@ PyObject* block_norm(Args& a) {
     const double factor = a.real(6), eps = a.real(9);
     const int64_t kind = a.number(7), gate_form = a.number(8);
     int64_t stride;
-    if (!a.fine || !activation(residual) || !activation(branch) || residual.dim() < 1 || residual.size(-1) > kWidestNorm || !row_stride(residual, &stride)) return none();
+    if (!a.fine || !unobserved({&residual, &branch, &gate, &vectors[0], &vectors[1], &vectors[2]})) return none();
+    if (!activation(residual) || !activation(branch) || residual.dim() < 1 || residual.size(-1) > kWidestNorm || !row_stride(residual, &stride)) return none();
     if (branch.device() != residual.device() || (residual.scalar_type() != branch.scalar_type() && residual.scalar_type() != at::kFloat)) return none();
     for (const Tensor* t : {&branch, &gate})
         if (t->defined() && (!like_of(*t, residual, branch.scalar_type()) || t->sizes() != residual.sizes() || !row_stride(*t, &stride))) return none();
@@ -285,6 +309,7 @@ struct Scores : torch::autograd::Function<Scores> {
         return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_gradients("run_hip_token_scores", grads);
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &logits = saved[0], &tokens = saved[1], &stats = saved[2], &entropy = saved[3];
         const c10::DeviceGuard guard(logits.device());
@@ -306,7 +331,7 @@ PyObject* token_scores(Args& a) {
     const Tensor logits = optional_tensor(a, 0), tokens = optional_tensor(a, 1);
     const int64_t top_k = a.number(2);
     int64_t stride;
-    if (!a.fine || !activation(logits) || logits.dim() < 1 || logits.size(-1) > (int64_t{1} << 30) || !row_stride(logits, &stride)) return none();
+    if (!a.fine || !unobserved({&logits, &tokens}) || !activation(logits) || logits.dim() < 1 || logits.size(-1) > (int64_t{1} << 30) || !row_stride(logits, &stride)) return none();
     if (top_k < 0 || top_k > 64 || top_k > logits.size(-1)) return none();
     if (tokens.defined() && (!like_of(tokens, logits, at::kLong) || tokens.sizes() != logits.sizes().slice(0, logits.dim() - 1) || !tokens.is_contiguous())) return none();
     variable_list out;
@@ -316,4 +341,13 @@ PyObject* token_scores(Args& a) {
     });
     out.resize(4);
     return tuple_of(out);
+}
+
+// Any number of arguments; what is no tensor counts for nothing
+PyObject* are_unobserved(Args& a) {
+    c10::SmallVector<const Tensor*, 8> tensors;
+    for (Py_ssize_t i = 0; i < a.n; ++i) {
+        if (THPVariable_Check(a.v[i])) tensors.push_back(&THPVariable_Unpack(a.v[i]));
+    }
+    return PyBool_FromLong(unobserved(tensors));
 }

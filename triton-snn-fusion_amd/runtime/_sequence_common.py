@@ -5,6 +5,8 @@ import contextlib
 from typing import Iterable, List, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from .. import _dispatch
 
@@ -14,6 +16,32 @@ SUPPORTED_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 def refuse(operator: str, reasons: List[str]) -> None:
     if reasons:
         raise RuntimeError(f"{operator}: " + "; ".join(reasons))
+
+
+def check_unobserved(reasons: List[str], names: Tuple[str, ...], *operands) -> None:
+    """A tensor is its memory to the kernels, and their work is all there is to a call: what else travels with a tensor would be lost (a tangent silently),
+    and a trace of torch's operations would hold the outputs' allocation and nothing that fills them."""
+    module = native(next((t for t in operands if t is not None), None))
+    if module is not None and module.unobserved(*operands):
+        return
+    if torch.jit.is_tracing() or get_proxy_mode() is not None:
+        reasons.append("unsupported_tracing: torch.jit.trace and make_fx record torch's own operations only")
+    for name, t in zip(names, operands):
+        if not isinstance(t, torch.Tensor):
+            continue
+        if forward_ad.unpack_dual(t).tangent is not None:
+            reasons.append(f"unsupported_forward_ad: {name} has a tangent, and there is no forward-mode derivative")
+        try:
+            t.untyped_storage()
+        except (NotImplementedError, RuntimeError):
+            reasons.append(f"unsupported_transform: {name} is wrapped by a transform (torch.func, vmap) and has no memory of its own")
+
+
+def refuse_observed(operator: str, names: Tuple[str, ...], *gradients) -> None:
+    """The same of the gradients that autograd hands over."""
+    reasons: List[str] = []
+    check_unobserved(reasons, names, *gradients)
+    refuse(operator, reasons)
 
 
 def check_activation(name: str, t, reasons: List[str]) -> bool:

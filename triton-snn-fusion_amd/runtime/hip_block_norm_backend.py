@@ -16,11 +16,12 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._sequence_common import SUPPORTED_DTYPES, check_activation, check_operand, flat_rows, native, on_device_of, refuse, wants_gradient, workspace
+from ._sequence_common import SUPPORTED_DTYPES, check_activation, check_operand, check_unobserved, flat_rows, native, on_device_of, refuse, refuse_observed, wants_gradient, workspace
 
 KINDS = {"rms": 0, "layer": 1}
 GATE_FORMS = {"sigmoid": 1, "silu": 2}
 MAX_WIDTH = 16384
+OPERANDS = ("residual", "branch", "gate", "branch_weight", "next_weight", "scale")
 
 
 def check_block_norm_support(residual, branch=None, gate=None, branch_weight=None, next_weight=None, scale=None, kind: str = "rms",
@@ -33,6 +34,7 @@ def check_block_norm_support(residual, branch=None, gate=None, branch_weight=Non
         reasons.append(f"unsupported_gate: gate_form must be one of {sorted(GATE_FORMS)}, got {gate_form!r}")
     if not eps >= 0.0:
         reasons.append(f"unsupported_eps: eps must not be negative, got {eps}")
+    check_unobserved(reasons, OPERANDS, residual, branch, gate, branch_weight, next_weight, scale)
     if not check_activation("residual", residual, reasons):
         return reasons
     if residual.dim() < 1 or not 1 <= residual.shape[-1] <= MAX_WIDTH:
@@ -96,6 +98,7 @@ class _BlockNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out, d_normed):
+        refuse_observed("run_hip_block_norm", ("the gradient of residual'", "the gradient of normed"), d_out, d_normed)
         residual, branch, gate, *vectors, stats = ctx.saved_tensors
         factor, kind, gate_form = ctx.options
         rows, D = residual.shape
@@ -129,8 +132,8 @@ def run_hip_block_norm(residual: torch.Tensor, branch: Optional[torch.Tensor] = 
     kind: "rms", or "layer" with the mean taken out.
 
     Leading dimensions that are one stride apart, slices of wider projections among them, go in without copies. Arithmetic is float32
-    throughout (normed comes from residual' before its rounding), outputs are rounded once. Differentiable once, in all tensors; the
-    vectors' gradients are sums in a fixed order.
+    throughout (normed comes from residual' before its rounding), outputs are rounded once. Differentiable once, backwards, in all tensors
+    (forward mode, torch.func and tracing are refused); the vectors' gradients are sums in a fixed order.
     """
     learnt = isinstance(scale, torch.Tensor)
     module = native(residual)

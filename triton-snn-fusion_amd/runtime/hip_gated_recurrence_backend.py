@@ -17,9 +17,10 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._sequence_common import check_activation, check_operand, native, on_device_of, refuse, unit_rows, wants_gradient, workspace
+from ._sequence_common import check_activation, check_operand, check_unobserved, native, on_device_of, refuse, refuse_observed, unit_rows, wants_gradient, workspace
 
 FORMS = {"leaky": 0, "linear": 1}
+OPERANDS = ("x_seq", "gate_seq", "state", "starts", "lengths")
 
 
 def check_gated_recurrence_support(x_seq, gate_seq, state=None, form: str = "leaky", starts=None, lengths=None) -> List[str]:
@@ -27,6 +28,7 @@ def check_gated_recurrence_support(x_seq, gate_seq, state=None, form: str = "lea
     reasons: List[str] = []
     if form not in FORMS:
         reasons.append(f"unsupported_form: form must be one of {sorted(FORMS)}, got {form!r}")
+    check_unobserved(reasons, OPERANDS, x_seq, gate_seq, state, starts, lengths)
     if not check_activation("x_seq", x_seq, reasons):
         return reasons
     if x_seq.dim() != 3:
@@ -89,6 +91,7 @@ class _GatedRecurrence(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dh, dlast):
+        refuse_observed("run_hip_gated_recurrence", ("the gradient of h_seq", "the gradient of the last state"), dh, dlast)
         x, gate, starts, lengths, marks = ctx.saved_tensors
         lib = _lib.lib()
         T, N, D = (int(n) for n in x.shape)
@@ -120,7 +123,8 @@ def run_hip_gated_recurrence(x_seq: torch.Tensor, gate_seq: torch.Tensor, state:
     lengths: [N] int32 or int64, clamped to 0..T. Steps from there on are padding: what x_seq, gate_seq and starts hold there does not
         matter, h_seq is 0, the state stays.
 
-    Arithmetic is float32 throughout, outputs are rounded once. Differentiable once, in x_seq, gate_seq and state.
+    Arithmetic is float32 throughout, outputs are rounded once. Differentiable once, backwards, in x_seq, gate_seq and state
+    (forward mode, torch.func and tracing are refused).
     """
     module = native(x_seq)
     if module is not None and form in FORMS:

@@ -12,7 +12,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._sequence_common import check_activation, check_operand, flat_rows, native, on_device_of, refuse, wants_gradient, workspace
+from ._sequence_common import check_activation, check_operand, check_unobserved, flat_rows, native, on_device_of, refuse, refuse_observed, wants_gradient, workspace
 
 MAX_ALTERNATIVES = 64
 
@@ -29,6 +29,7 @@ class TokenScores(NamedTuple):
 def check_token_scores_support(logits, tokens=None, top_k: int = 0) -> List[str]:
     """Reasons why a call is refused; empty if the kernels take it."""
     reasons: List[str] = []
+    check_unobserved(reasons, ("logits", "tokens"), logits, tokens)
     if not check_activation("logits", logits, reasons):
         return reasons
     if logits.dim() < 1 or not 1 <= logits.shape[-1] <= 1 << 30:
@@ -72,6 +73,7 @@ class _TokenScores(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_logprob, d_entropy, *_):
+        refuse_observed("run_hip_token_scores", ("the gradient of logprob", "the gradient of entropy"), d_logprob, d_entropy)
         logits, tokens, stats, entropy = ctx.saved_tensors
         rows, V = logits.shape
         with on_device_of(logits):
@@ -91,7 +93,7 @@ def run_hip_token_scores(logits: torch.Tensor, tokens: Optional[torch.Tensor] = 
     tokens: [...] int64 or int32, the token given for each row; outside [0, V) (-100, say), or without tokens, logprob is 0 and passes no gradient.
     top_k: alternatives a row, up to 64: the most likely first, equal ones by the lower index. They carry no gradient.
 
-    Arithmetic is float32; logprob and entropy are differentiable once, in the logits.
+    Arithmetic is float32; logprob and entropy are differentiable once, backwards, in the logits (forward mode, torch.func and tracing are refused).
     """
     module = native(logits)
     if module is not None:
