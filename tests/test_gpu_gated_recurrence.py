@@ -196,6 +196,28 @@ def test_what_is_not_a_number_stays_until_a_start(hip_ops, T, N, form):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,N", [(1, 3), (20, 3), (700, 2), (700, 64), (300, 200)])
+@pytest.mark.parametrize("form,value", [("leaky", -30.0), ("linear", 1e-9), ("linear", -1e-9), ("linear", 0.0)])
+def test_what_is_infinite_stays_until_a_start(hip_ops, T, N, form, value):
+    """Decays whose product vanishes leave an infinite state, or gradient, infinite, of the sign that the steps give it; a decay of 0 makes it NaN."""
+    D = 130
+    x, gate, state, dh, dlast = operands(T, N, D, torch.float32, form, 19)
+    gate = torch.full_like(gate, value)
+    at = min(3, T - 1)
+    x[at, 0, 5], dh[T - at - 1, 1, 7], state[1, 9], dlast[1, 9] = (float("inf"),) * 4
+    starts = torch.zeros(T, N, dtype=torch.bool, device=DEV)
+    for mask in (None, starts, starts.clone().index_fill_(0, torch.tensor([T // 2], device=DEV), True)):
+        leaves = [t.clone().requires_grad_(True) for t in (x, gate, state)]
+        h, last = run(*leaves, form=form, starts=mask)
+        dx, _, dstate = torch.autograd.grad([h, last], leaves, [dh, dlast])
+        want = reference(x, gate, state, form, mask, dh=dh, dlast=dlast)
+        for got, wanted in ((h, want[0]), (last, want[1]), (dx, want[3]), (dstate, want[5])):
+            got = got.detach().double().cpu()
+            assert torch.equal(got.isnan(), wanted.isnan())
+            assert torch.equal(torch.where(got.isinf(), got.sign(), 0.0), torch.where(wanted.isinf(), wanted.sign(), 0.0))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T,N", [(20, 3), (700, 2), (700, 64)])
 def test_growth_of_nothing_is_nothing(hip_ops, T, N):
     """Gates of 2 grow past the range of float32 over a run, and 0 stays 0; with a start, what grew is gone."""

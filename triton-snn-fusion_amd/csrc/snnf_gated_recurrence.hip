@@ -85,8 +85,16 @@ __device__ __forceinline__ float run_of(float A, bool drops) {
     return A;
 }
 
-// What is left of the value that enters a run: the product of its decays, or for a long memory 1 - c.
-__device__ __forceinline__ float left_over(float product, float c) { return c < 0.5f && c > -0.5f ? 1.0f - c : product; }
+// What is left of the value that enters a run: the product of its decays, or for a long memory 1 - c. Where the product of decays other than 0 vanishes
+// it is the smallest number there is: an infinite value stays infinite then, as it does step by step, and any other is off by 2^-149 of it at
+// most either way. `least`: the smallest decay's magnitude; a sigmoid is never 0.
+template <bool LEAKY>
+__device__ __forceinline__ float left_over(float product, float c, float least) {
+    constexpr float kSmallest = 0x1p-149f;
+    const float left = c < 0.5f && c > -0.5f ? 1.0f - c : product;
+    if constexpr (LEAKY) return __builtin_elementwise_maximum(left, kSmallest);
+    return left == 0.0f && least > 0.0f ? __builtin_copysignf(kSmallest, left) : left;
+}
 
 struct Place {
     int n, d, lim;                      // sequence, first channel of the lane, steps that count
@@ -269,26 +277,30 @@ template <bool STARTS>
 __device__ __forceinline__ float kept(uint32_t drop, int i, float v) { return STARTS && (drop >> i & 1u) ? 0.0f : v; }
 
 // A of the run and H: what it makes of 0.
-template <int VEC, int S, bool STARTS>
+template <int VEC, int S, bool STARTS, bool LEAKY>
 __device__ __forceinline__ void reduce(const float (&a)[S][VEC], const float (&b)[S][VEC], const float (&c)[VEC], uint32_t drop, float (&A)[VEC], float (&H)[VEC]) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) A[j] = 1.0f, H[j] = 0.0f;
+    float least[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) least[j] = 1.0f;
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             H[j] = fmaf(a[i][j], kept<STARTS>(drop, i, H[j]), b[i][j]);
             A[j] *= a[i][j];
+            if constexpr (!LEAKY) least[j] = fminf(least[j], fabsf(a[i][j]));
         }
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) A[j] = run_of<STARTS>(left_over(A[j], c[j]), drop != 0);
+    for (int j = 0; j < VEC; ++j) A[j] = run_of<STARTS>(left_over<LEAKY>(A[j], c[j], least[j]), drop != 0);
 }
 
 // The W runs of a tile as one: A in row `w * rows`, H `second` rows behind it.
-template <int W, bool STARTS>
+template <int W, bool STARTS, bool LEAKY>
 __device__ __forceinline__ void join(float (*links)[64], int rows, int second, bool reversed, float& A, float& H) {
     const int lane = threadIdx.x & 63;
-    float c = 0.0f;
+    float c = 0.0f, least = 1.0f;
     bool drops = false;
     A = 1.0f, H = 0.0f;
 #pragma unroll 4
@@ -298,9 +310,10 @@ __device__ __forceinline__ void join(float (*links)[64], int rows, int second, b
         H = link<STARTS>(Aw, H, links[w * rows + second][lane]);
         A *= Aw;
         c = fmaf(1.0f - Aw, 1.0f - c, c);
+        if constexpr (!LEAKY) least = fminf(least, fabsf(Aw));
         drops = drops || dropped<STARTS>(Aw);
     }
-    A = run_of<STARTS>(left_over(A, c), drops);
+    A = run_of<STARTS>(left_over<LEAKY>(A, c, least), drops);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -309,6 +322,7 @@ __device__ __forceinline__ void join(float (*links)[64], int rows, int second, b
 template <typename XT, int VEC, int W, int S, bool STARTS, bool LEAKY>
 struct ForwardTile {
     static constexpr int kParts = 2;
+    static constexpr bool kLeaky = LEAKY;
     uint32_t g[S], x[S];
     uint8_t start;
     float a[S][VEC], b[S][VEC], c[VEC];
@@ -345,7 +359,7 @@ struct ForwardTile {
     __device__ __forceinline__ void reduce_tile(float (*links)[64], int wave) {
         const int lane = threadIdx.x & 63;
         float A[VEC], H[VEC];
-        reduce<VEC, S, STARTS>(a, b, c, drop, A, H);
+        reduce<VEC, S, STARTS, LEAKY>(a, b, c, drop, A, H);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             links[wave * 2 * VEC + j][lane] = A[j];
@@ -378,6 +392,7 @@ struct ForwardTile {
 template <typename XT, int VEC, int W, int S, bool STARTS, bool LEAKY>
 struct BackwardTile {
     static constexpr int kParts = 3;       // A, R, H
+    static constexpr bool kLeaky = LEAKY;
     uint32_t g[S], x[S], dh[S], xs[S], es[S];
     float next_mark[VEC], mark[VEC];
     uint8_t start;
@@ -417,7 +432,7 @@ struct BackwardTile {
                 c[j] = fmaf(rest[i][j], 1.0f - c[j], c[j]);
             }
         }
-        reduce<VEC, S, STARTS>(a, b, c, drop, A, H);
+        reduce<VEC, S, STARTS, LEAKY>(a, b, c, drop, A, H);
 #pragma unroll
         for (int i = S - 1; i >= 0; --i)
 #pragma unroll
@@ -547,7 +562,7 @@ __global__ __launch_bounds__(64 * (W + VEC)) void relay_kernel(Args p) {
             __syncthreads();
             ticket = __builtin_amdgcn_readfirstlane(next_ticket);
             float A, H;
-            join<W, STARTS>(&links[buffer][wave - W], kRows, VEC, Tile::wave_at(0) != 0, A, H);
+            join<W, STARTS, Tile::kLeaky>(&links[buffer][wave - W], kRows, VEC, Tile::wave_at(0) != 0, A, H);
             values[wave - W][lane] = relay<STARTS>(p, q.active ? q.cell + wave - W : -1, order, A, H);
             buffer ^= 1;
             __syncthreads();

@@ -119,7 +119,7 @@ def run_hip_gated_recurrence(x_seq: torch.Tensor, gate_seq: torch.Tensor, state:
         apart, and h_seq has x_seq's order in memory.
     state: [N, D] float32 before the first step (None: zeros). The returned state is float32 and new memory; T = 0 returns it unchanged.
     starts: [T, N] bool. Where set, the state is dropped before the step (several documents packed into one sequence); what the state
-        held, infinities and NaN among it, does not reach the steps from there on. Nothing else ends a NaN.
+        held, infinities and NaN among it, does not reach the steps from there on. Nothing else ends either.
     lengths: [N] int32 or int64, clamped to 0..T. Steps from there on are padding: what x_seq, gate_seq and starts hold there does not
         matter, h_seq is 0, the state stays.
 
