@@ -466,7 +466,7 @@ typedef enum snnf_recurrence_form {
  *   state     NULL (zeros) or [N, D] float32; `state_out` [N, D] float32, not the same memory
  *   marks     NULL, or snnf_gated_recurrence_marks_bytes(T, N, D, dtype) bytes that the backward pass will read
  *   workspace snnf_gated_recurrence_workspace_bytes(...) bytes, 16-byte aligned (0: none needed), in use until the call's work is done
- * T >= 1. Two launches where the sequences are few and long, else one. */
+ * T >= 1. Two launches where the sequences are few and long, else one. Gates of the linear form beyond 1 in magnitude are walked step by step. */
 size_t snnf_gated_recurrence_workspace_bytes(int T, int N, int D, int dtype, int backward);
 size_t snnf_gated_recurrence_marks_bytes(int T, int N, int D, int dtype);
 int snnf_gated_recurrence(const void* x, int64_t x_step, int64_t x_row, const void* gate, int64_t gate_step, int64_t gate_row, int T, int N, int D,

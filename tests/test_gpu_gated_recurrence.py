@@ -239,6 +239,76 @@ def test_growth_of_nothing_is_nothing(hip_ops, T, N):
     assert torch.equal(h[:T // 2], want[:, None, None].expand(T // 2, N, D)) and bool((h[T // 2:] == 0).all()) and bool((last == 0).all())
 
 
+GROWTH = [(20, 3, 130), (20, 3, 33), (700, 2, 130), (700, 2, 65), (700, 64, 130), (300, 200, 130), (40, 2000, 130)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,N,D", GROWTH)
+def test_growth_past_the_range_of_float32_and_back(hip_ops, T, N, D, dtype):
+    """A state of 2^-110 that ten gates of 2^20 bring to 2^90, and four of 2^-10 to 2^50: every product is a power of two, so that nothing is
+    rounded, and no state leaves the range, though the product of the gates does. The gradient goes the same way back."""
+    gate = torch.ones(T, N, D)
+    gate[3:13], gate[14:18] = 2.0 ** 20, -(2.0 ** -10)
+    x, dh = torch.zeros(T, N, D), torch.zeros(T, N, D)
+    state, dlast = torch.full((N, D), 2.0 ** -110), torch.full((N, D), 2.0 ** -100)
+    want = reference(x, gate, state, "linear", dh=dh, dlast=dlast)
+    for mask in (None, torch.zeros(T, N, dtype=torch.bool, device=DEV)):
+        leaves = [t.to(DEV).requires_grad_(True) for t in (x.to(dtype), gate.to(dtype), state)]
+        h, last = run(*leaves, form="linear", starts=mask)
+        got = [h, last, *torch.autograd.grad([h, last], leaves, [dh.to(DEV, dtype), dlast.to(DEV)])]
+        for a, b in zip(got, (want[0], want[1], *want[3:6])):
+            assert torch.equal(a.detach().cpu(), b.to(a.dtype))         # a gradient of 2^-140 is 0 in bfloat16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,N,D", GROWTH)
+def test_gates_beyond_one_are_walked_step_by_step(hip_ops, T, N, D):
+    """Gates between -1.5 and 1.5: a prompt has the bits of the same prompt in single tokens, and gradients are as exact as a walk's, whose error is at
+    most 2^-24 of |a| |h| + |x| a step (8 of them: the state, its sum and product, the gradient's), carried on by |a|."""
+    g = gen(23)
+    x, dh = torch.randn(T, N, D, generator=g), torch.randn(T, N, D, generator=g)
+    gate = (torch.rand(T, N, D, generator=g) * 2 - 1) * 1.5
+    state, dlast = torch.randn(N, D, generator=g), torch.randn(N, D, generator=g)
+    starts, lengths = torch.rand(T, N, generator=g) < 0.02, torch.randint(0, T + 1, (N,), generator=g, dtype=torch.int32)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, gate, state)]
+    with torch.no_grad():
+        h, last = run(*leaves, form="linear")
+        s = leaves[2]
+        for t in range(T):
+            token, s = run(leaves[0][t:t + 1], leaves[1][t:t + 1], s, form="linear")
+            assert torch.equal(token[0], h[t]), t
+        assert torch.equal(s, last)
+    for masks in ({}, {"starts": starts, "lengths": lengths}):
+        h, last = run(*leaves, form="linear", **{k: m.to(DEV) for k, m in masks.items()})
+        got = [h, last, *torch.autograd.grad([h, last], leaves, [dh.to(DEV), dlast.to(DEV)])]
+        want = reference(x, gate, state, "linear", dh=dh, dlast=dlast, **masks)
+        a = gate.double().abs()
+        limit, drop = masks.get("lengths", torch.full((N,), T)), masks.get("starts", torch.zeros(T, N, dtype=torch.bool))
+        inside, keep = (torch.arange(T)[:, None] < limit[None, :])[:, :, None], (~drop)[:, :, None].double()
+        size, off = state.double().abs(), torch.zeros(N, D, dtype=torch.float64)
+        before, h_off = [], []
+        for t in range(T):
+            before.append((size * keep[t], off * keep[t]))
+            new = a[t] * before[t][0] + x[t].double().abs()
+            off = torch.where(inside[t], a[t] * before[t][1] + C * U * new, off)
+            size = torch.where(inside[t], new, size)
+            h_off.append(torch.where(inside[t], off, 0.0))
+        near(got[0], want[0], torch.float32, torch.stack(h_off), "h")
+        near(got[1], want[1], torch.float32, off, "last state")
+        size, off = dlast.double().abs(), torch.zeros(N, D, dtype=torch.float64)
+        x_off, gate_off = [None] * T, [None] * T
+        for t in range(T - 1, -1, -1):
+            new = size + dh[t].double().abs()
+            s_off = off + C * U * new
+            x_off[t] = torch.where(inside[t], s_off, 0.0)
+            gate_off[t] = torch.where(inside[t], s_off * (before[t][0] + before[t][1]) + new * before[t][1] + C * U * new * before[t][0], 0.0)
+            size, off = torch.where(inside[t], a[t] * new * keep[t], size), torch.where(inside[t], a[t] * s_off * keep[t], off)
+        near(got[2], want[3], torch.float32, torch.stack(x_off), "dx")
+        near(got[3], want[4], torch.float32, torch.stack(gate_off), "dgate")
+        near(got[4], want[5], torch.float32, off, "dstate")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,N,D", [(1, 40, 3), (20, 33, 5), (300, 17, 24), (520, 2, 65), (40, 300, 1)])

@@ -69,21 +69,26 @@ __device__ __forceinline__ uint8_t start_of(const Args& p, int n, int first, int
     return lane < steps && first + lane < lim ? p.starts[static_cast<int64_t>(first + lane) * p.starts_step + static_cast<int64_t>(n) * p.starts_row] : 0;
 }
 
-// One link of the chain: what a run of steps makes of the value that enters it. Of 0 it makes H, whatever A may have grown to. A run that
-// drops the value says so by A = -0, which no other run has, and must not multiply an infinity or NaN that belongs to what came before; A = 0
-// from decays that vanish does.
+// One link of the chain: what a run of steps makes of the value that enters it. A run that drops the value says so by A = -0, which no other run
+// has, and must not multiply an infinity or NaN that belongs to what came before; A = 0 from a decay of 0 does.
 constexpr uint32_t kDropped = 0x80000000u;
 template <bool STARTS>
 __device__ __forceinline__ bool dropped(float A) { return STARTS && __float_as_uint(A) == kDropped; }
 template <bool STARTS>
 __device__ __forceinline__ float link(float A, float entering, float H) {
-    return entering == 0.0f || dropped<STARTS>(A) ? H : fmaf(A, entering, H);
+    return dropped<STARTS>(A) ? H : fmaf(A, entering, H);
 }
 template <bool STARTS>
 __device__ __forceinline__ float run_of(float A, bool drops) {
     if constexpr (STARTS) return drops ? __uint_as_float(kDropped) : A + 0.0f;      // -0 + 0 = 0
     return A;
 }
+
+// A run of the linear form with a gate beyond 1 in magnitude, unless it drops the value, gets an infinite A: its product, or its result from 0, may
+// leave float32's range where the state itself does not. The runs of its tile then take the value one after the other, step by step, which costs little
+// where columns fill the chip (2048 x 16 x 2048 bf16, such a gate in every tile: forward 81 -> 87 us, backward 138 -> 172) and a chain of tiles where they do
+// not (8192 x 1 x 1024: 27 -> 145, 51 -> 350).
+constexpr float kInTurn = INFINITY;
 
 // What is left of the value that enters a run: the product of its decays, or for a long memory 1 - c. Where the product of decays other than 0 vanishes
 // it is the smallest number there is: an infinite value stays infinite then, as it does step by step, and any other is off by 2^-149 of it at
@@ -190,14 +195,20 @@ __device__ __forceinline__ void store(const Output& to, const Place& q, int firs
 // ------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t plain_bits(float v) { return v != v ? 0x7fc00000u : __float_as_uint(v); }      // never all ones
 
-// One channel a lane; `cell` < 0: none.
+// One channel a lane; `cell` < 0: none. A tile whose runs have to be taken in turn publishes no (A, H): those behind it wait for its value, which
+// `relay_value` publishes once the runs are done.
+__device__ __forceinline__ void relay_value(const Args& p, int64_t cell, int order, float behind) {
+    if (cell < 0) return;
+    if (order == p.tiles - 1) p.state_out[cell] = behind;
+    else __hip_atomic_store(p.values + order * (static_cast<int64_t>(p.N) * p.D) + cell, plain_bits(behind), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 template <bool STARTS>
-__device__ __forceinline__ float relay(const Args& p, int64_t cell, int order, float A, float H) {
+__device__ __forceinline__ float relay(const Args& p, int64_t cell, int order, float A, float H, bool in_turn) {
     const int64_t cells = static_cast<int64_t>(p.N) * p.D;
     const bool active = cell >= 0, last = order == p.tiles - 1;
     uint64_t* runs = p.runs + order * cells + cell;
     uint32_t* values = p.values + order * cells + cell;
-    if (active && !last)
+    if (active && !last && !in_turn)
         __hip_atomic_store(runs, static_cast<uint64_t>(plain_bits(A)) << 32 | plain_bits(H), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     float from = active && p.state != nullptr ? p.state[cell] : 0.0f;
     if (order > 0) {
@@ -232,11 +243,7 @@ __device__ __forceinline__ float relay(const Args& p, int64_t cell, int order, f
             if (i < found) from = link<STARTS>(__uint_as_float(static_cast<uint32_t>(run[i] >> 32)), from, __uint_as_float(static_cast<uint32_t>(run[i])));
         }
     }
-    const float behind = link<STARTS>(A, from, H);
-    if (active) {
-        if (last) p.state_out[cell] = behind;
-        else __hip_atomic_store(values, plain_bits(behind), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+    if (!in_turn) relay_value(p, cell, order, link<STARTS>(A, from, H));
     return from;
 }
 
@@ -281,19 +288,35 @@ template <int VEC, int S, bool STARTS, bool LEAKY>
 __device__ __forceinline__ void reduce(const float (&a)[S][VEC], const float (&b)[S][VEC], const float (&c)[VEC], uint32_t drop, float (&A)[VEC], float (&H)[VEC]) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) A[j] = 1.0f, H[j] = 0.0f;
-    float least[VEC];
+    float least[VEC], most[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) least[j] = 1.0f;
+    for (int j = 0; j < VEC; ++j) least[j] = 1.0f, most[j] = 1.0f;
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             H[j] = fmaf(a[i][j], kept<STARTS>(drop, i, H[j]), b[i][j]);
             A[j] *= a[i][j];
-            if constexpr (!LEAKY) least[j] = fminf(least[j], fabsf(a[i][j]));
+            if constexpr (!LEAKY) most[j] = fmaxf(most[j], fabsf(a[i][j]));
         }
+    if constexpr (!LEAKY) {
+        if (__any(A[0] == 0.0f || A[VEC - 1] == 0.0f)) {       // seldom
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) A[j] = run_of<STARTS>(left_over<LEAKY>(A[j], c[j], least[j]), drop != 0);
+            for (int i = 0; i < S; ++i)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) least[j] = fminf(least[j], fabsf(a[i][j]));
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) A[j] = run_of<STARTS>(most[j] > 1.0f ? kInTurn : left_over<LEAKY>(A[j], c[j], least[j]), drop != 0);
+}
+
+// Whether a run of the tile has to be taken in its turn.
+template <int W>
+__device__ __forceinline__ bool any_turn(const bool* turns) { return __any(turns[(threadIdx.x & 63) % W]); }
+__device__ __forceinline__ void say_turn(bool* turns, int wave, bool turn) {
+    turn = __any(turn);
+    if ((threadIdx.x & 63) == 0) turns[wave] = turn;
 }
 
 // The W runs of a tile as one: A in row `w * rows`, H `second` rows behind it.
@@ -356,7 +379,7 @@ struct ForwardTile {
                 for (int j = 0; j < VEC; ++j) c[j] = fmaf(rest[i][j], 1.0f - c[j], c[j]);
         }
     }
-    __device__ __forceinline__ void reduce_tile(float (*links)[64], int wave) {
+    __device__ __forceinline__ void reduce_tile(float (*links)[64], bool* turns, int wave) {
         const int lane = threadIdx.x & 63;
         float A[VEC], H[VEC];
         reduce<VEC, S, STARTS, LEAKY>(a, b, c, drop, A, H);
@@ -365,9 +388,20 @@ struct ForwardTile {
             links[wave * 2 * VEC + j][lane] = A[j];
             links[(wave * 2 + 1) * VEC + j][lane] = H[j];
         }
+        if constexpr (!LEAKY) say_turn(turns, wave, A[0] == kInTurn || A[VEC - 1] == kInTurn);
     }
+    // What enters the run besides the value that travels: nothing.
+    struct Entering {};
+    __device__ __forceinline__ Entering entering(float (*)[64], int) const { return {}; }
+    static constexpr int kTurns = 1;
     // v: the value that enters the run, then the one behind it
-    __device__ __forceinline__ void write_tile(const Args& p, const Place& q, int t0, int wave, float (*)[64], float (&v)[VEC]) {
+    __device__ __forceinline__ void step(int, float (&v)[VEC]) const {
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[j] = fmaf(a[i][j], kept<STARTS>(drop, i, v[j]), b[i][j]);
+    }
+    __device__ __forceinline__ void write_tile(const Args& p, const Place& q, int t0, int wave, Entering, float (&v)[VEC]) {
         const int first = t0 + wave * S;
         if (p.marks != nullptr && q.active && first % p.span == 0 && first < p.T) {
             float* mark = p.marks + static_cast<int64_t>(first / p.span) * p.N * p.D + q.cell;
@@ -441,7 +475,7 @@ struct BackwardTile {
         again<S>(xs);
         again<S>(es);
     }
-    __device__ __forceinline__ void reduce_tile(float (*links)[64], int wave) {
+    __device__ __forceinline__ void reduce_tile(float (*links)[64], bool* turns, int wave) {
         const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
@@ -449,17 +483,44 @@ struct BackwardTile {
             links[(wave * 3 + 1) * VEC + j][lane] = R[j];
             links[(wave * 3 + 2) * VEC + j][lane] = H[j];
         }
+        if constexpr (!LEAKY) say_turn(turns, wave, A[0] == kInTurn || A[VEC - 1] == kInTurn);
     }
-    __device__ __forceinline__ void write_tile(const Args& p, const Place& q, int t0, int wave, float (*links)[64], float (&v)[VEC]) {
-        const int lane = threadIdx.x & 63, first = t0 + wave * S;
+    // h that enters the run
+    struct Entering {
         float h[VEC];
+    };
+    __device__ __forceinline__ Entering entering(float (*links)[64], int wave) const {
+        const int lane = threadIdx.x & 63;
+        Entering e;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) h[j] = mark[j];
+        for (int j = 0; j < VEC; ++j) e.h[j] = mark[j];
 #pragma unroll 4
         for (int w = 0; w < wave; ++w) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) h[j] = link<STARTS>(links[w * 3 * VEC + j][lane], h[j], links[(w * 3 + 2) * VEC + j][lane]);
+            for (int j = 0; j < VEC; ++j) e.h[j] = link<STARTS>(links[w * 3 * VEC + j][lane], e.h[j], links[(w * 3 + 2) * VEC + j][lane]);
         }
+        return e;
+    }
+    // Turn 0: the gradient, from the last step to the first; turn 1: h.
+    static constexpr int kTurns = 2;
+    __device__ __forceinline__ void step(int turn, float (&v)[VEC]) const {
+        if (turn == 0) {
+#pragma unroll
+            for (int i = S - 1; i >= 0; --i)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[j] = kept<STARTS>(drop, i, a[i][j] * (v[j] + element<XT>(es[i], j)));
+        } else {
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[j] = fmaf(a[i][j], kept<STARTS>(drop, i, v[j]), in(i, j));
+        }
+    }
+    __device__ __forceinline__ void write_tile(const Args& p, const Place& q, int t0, int wave, const Entering& e, float (&v)[VEC]) {
+        const int first = t0 + wave * S;
+        float h[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) h[j] = e.h[j];
         float before[S][VEC];
 #pragma unroll
         for (int i = 0; i < S; ++i)
@@ -489,11 +550,52 @@ struct BackwardTile {
     __device__ __forceinline__ static int wave_at(int k) { return W - 1 - k; }
 };
 
+// The runs of a tile one after the other: in `enter` the value that enters this wave's, in v first the one that enters the tile, then the one behind it.
+// With two buffers in turn a round costs one barrier. All threads of the workgroup call it, those of other waves with `wave` < 0.
+template <typename Tile, int VEC, int W>
+__device__ __forceinline__ void take_turns(Tile& tile, int wave, float (*passed)[VEC][64], float (&v)[VEC], float (&enter)[VEC], typename Tile::Entering& e) {
+    static_assert(W % 2 == 0);          // the last round leaves the first buffer free
+    const int lane = threadIdx.x & 63;
+#pragma unroll 1
+    for (int k = 0; k < W; ++k) {
+        if (wave >= 0 && k == Tile::passes(wave)) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) enter[j] = v[j];
+            tile.step(0, v);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) passed[k & 1][j][lane] = v[j];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = passed[k & 1][j][lane];
+    }
+    if constexpr (Tile::kTurns == 2) {
+        float h[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) h[j] = tile.mark[j];
+#pragma unroll 1
+        for (int k = 0; k < W; ++k) {
+            if (k == wave) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) e.h[j] = h[j];
+                tile.step(1, h);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) passed[k & 1][j][lane] = h[j];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) h[j] = passed[k & 1][j][lane];
+        }
+    }
+}
+
 // A workgroup to a column, from tile to tile.
 template <typename Tile, int VEC, int W, bool STARTS>
 __global__ __launch_bounds__(64 * W) void walk_kernel(Args p) {
     constexpr int kRows = Tile::kParts * VEC;
     __shared__ float links[2][W * kRows][64];
+    __shared__ float passed[Tile::kLeaky ? 1 : 2][VEC][64];
+    __shared__ bool turns[2][W];
     const uint32_t column = group_index();
     if (column >= static_cast<uint32_t>(p.columns)) return;
     const Place q = place<VEC>(p, column);
@@ -513,24 +615,30 @@ __global__ __launch_bounds__(64 * W) void walk_kernel(Args p) {
         }
         float(*const shared)[64] = links[order & 1];
         if constexpr (W > 1) {
-            tile.reduce_tile(shared, wave);
+            tile.reduce_tile(shared, turns[order & 1], wave);
             __syncthreads();
             float enter[VEC];
+            typename Tile::Entering e;
+            if (Tile::kLeaky || !any_turn<W>(turns[order & 1])) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) enter[j] = v[j];
+                for (int j = 0; j < VEC; ++j) enter[j] = v[j];
 #pragma unroll 4
-            for (int k = 0; k < W; ++k) {
-                if (k == Tile::passes(wave)) {
+                for (int k = 0; k < W; ++k) {
+                    if (k == Tile::passes(wave)) {
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) enter[j] = v[j];
+                        for (int j = 0; j < VEC; ++j) enter[j] = v[j];
+                    }
+                    const int w = Tile::wave_at(k);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) v[j] = link<STARTS>(shared[w * kRows + j][lane], v[j], shared[w * kRows + VEC + j][lane]);
                 }
-                const int w = Tile::wave_at(k);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) v[j] = link<STARTS>(shared[w * kRows + j][lane], v[j], shared[w * kRows + VEC + j][lane]);
+                e = tile.entering(shared, wave);
+            } else {
+                take_turns<Tile, VEC, W>(tile, wave, passed, v, enter, e);
             }
-            tile.write_tile(p, q, now, wave, shared, enter);
+            tile.write_tile(p, q, now, wave, e, enter);
         } else {
-            tile.write_tile(p, q, now, 0, shared, v);
+            tile.write_tile(p, q, now, 0, tile.entering(shared, 0), v);
         }
     }
     if (q.active && wave == 0) {
@@ -547,6 +655,8 @@ __global__ __launch_bounds__(64 * (W + VEC)) void relay_kernel(Args p) {
     __shared__ float links[2][W * kRows][64];
     __shared__ float values[VEC][64];
     __shared__ uint32_t next_ticket;
+    __shared__ float passed[Tile::kLeaky ? 1 : 2][VEC][64];
+    __shared__ bool turns[2][W];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t total = static_cast<uint32_t>(p.tiles) * static_cast<uint32_t>(p.columns);
     if (threadIdx.x == 64 * W) next_ticket = atomicAdd(p.ticket, 1u) + 1u;
@@ -563,9 +673,20 @@ __global__ __launch_bounds__(64 * (W + VEC)) void relay_kernel(Args p) {
             ticket = __builtin_amdgcn_readfirstlane(next_ticket);
             float A, H;
             join<W, STARTS, Tile::kLeaky>(&links[buffer][wave - W], kRows, VEC, Tile::wave_at(0) != 0, A, H);
-            values[wave - W][lane] = relay<STARTS>(p, q.active ? q.cell + wave - W : -1, order, A, H);
+            const bool turn = !Tile::kLeaky && any_turn<W>(turns[buffer]);
+            const int64_t cell = q.active ? q.cell + wave - W : -1;
+            values[wave - W][lane] = relay<STARTS>(p, cell, order, A, H, turn);
             buffer ^= 1;
             __syncthreads();
+            if constexpr (!Tile::kLeaky) {
+                if (turn) {
+                    float v[VEC] = {}, enter[VEC];
+                    typename Tile::Entering e;
+                    Tile none;
+                    take_turns<Tile, VEC, W>(none, -1, passed, v, enter, e);
+                    relay_value(p, cell, order, wave == W ? v[0] : v[VEC - 1]);
+                }
+            }
         }
         return;
     }
@@ -576,7 +697,7 @@ __global__ __launch_bounds__(64 * (W + VEC)) void relay_kernel(Args p) {
     while (ticket < total) {
         const int t0 = Tile::at(p, order);
         tile.decode_tile(q, t0, wave);
-        tile.reduce_tile(links[buffer], wave);
+        tile.reduce_tile(links[buffer], turns[buffer], wave);
         __syncthreads();
         ticket = __builtin_amdgcn_readfirstlane(next_ticket);
         const Place here = q;
@@ -589,13 +710,30 @@ __global__ __launch_bounds__(64 * (W + VEC)) void relay_kernel(Args p) {
         float v[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[j] = values[j][lane];
+        const auto chain = [&] {
 #pragma unroll 4
-        for (int k = 0; k < Tile::passes(wave); ++k) {
-            const int w = Tile::wave_at(k);
+            for (int k = 0; k < Tile::passes(wave); ++k) {
+                const int w = Tile::wave_at(k);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[j] = link<STARTS>(links[buffer][w * kRows + j][lane], v[j], links[buffer][w * kRows + VEC + j][lane]);
+                for (int j = 0; j < VEC; ++j) v[j] = link<STARTS>(links[buffer][w * kRows + j][lane], v[j], links[buffer][w * kRows + VEC + j][lane]);
+            }
+            return tile.entering(links[buffer], wave);
+        };
+        if constexpr (Tile::kLeaky) {
+            const auto e = chain();
+            tile.write_tile(p, here, t0, wave, e, v);
+        } else {
+            typename Tile::Entering e;
+            if (any_turn<W>(turns[buffer])) {
+                float enter[VEC];
+                take_turns<Tile, VEC, W>(tile, wave, passed, v, enter, e);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[j] = enter[j];
+            } else {
+                e = chain();
+            }
+            tile.write_tile(p, here, t0, wave, e, v);
         }
-        tile.write_tile(p, here, t0, wave, links[buffer], v);
         buffer ^= 1;
     }
 }
