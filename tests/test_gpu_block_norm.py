@@ -4,6 +4,7 @@ Tolerances: an output is rounded once, half a step of its type (`eps / 2` relati
 float32 values, each off by at most 2^-24 relative (sigmoid: 4), and row statistics are sums of D terms of one sign added in chains of 8 and a
 tree of at most 16 levels: 24 roundings. So C = 48 roundings of the largest magnitude that enters: of the sum for residual', of
 (|residual'| / sigma) * |weight| for normed, of r * (|d| + |unit| * mean |d unit|) for a gradient. Sums over rows add `rows` such terms."""
+import gc
 import subprocess
 import sys
 
@@ -360,6 +361,9 @@ def test_rows_too_wide_are_refused(hip_ops):
         x = torch.empty(1, width, dtype=torch.bfloat16, device=DEV)
         with pytest.raises(RuntimeError, match="run_hip_block_norm: unsupported_shape: rows of 1 to 16384"):
             run(x, x)
+        del x
+    gc.collect()                        # the refusals' frames hold the tensors of 8 GB
+    torch.cuda.empty_cache()
 
 
 def test_entry_points_refuse_before_any_gpu_work(snnf_lib):
