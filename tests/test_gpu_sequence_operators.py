@@ -476,3 +476,33 @@ def test_what_follows_a_call_from_outside_is_refused(hip_ops, monkeypatch, opera
     for backend in (_sequence_common, hip_block_norm_backend, hip_gated_recurrence_backend, hip_token_scores_backend):
         monkeypatch.setattr(backend, "native", lambda t: None)
     _observed(operator, DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("python", [False, True])
+def test_outputs_may_be_written_over(hip_ops, monkeypatch, python):
+    """An addition or a mask in place on an output is the one out of place, whichever implementation ran the call."""
+    from triton_snn_fusion_amd.runtime import hip_block_norm_backend, hip_gated_recurrence_backend, hip_token_scores_backend
+    if python:
+        for backend in (hip_block_norm_backend, hip_gated_recurrence_backend, hip_token_scores_backend):
+            monkeypatch.setattr(backend, "native", lambda t: None)
+    g = gen(5)
+    x, gate, logits = (torch.randn(2, 40, 64, generator=g).to(DEV).requires_grad_(True) for _ in range(3))
+    tokens = torch.randint(0, 64, (2, 40), generator=g).to(DEV)
+    mask = (torch.rand(2, 40, generator=g) < 0.5).to(DEV)
+
+    def recurrence(batch_first):
+        order = (lambda t: t.transpose(0, 1)) if batch_first else (lambda t: t)
+        return hip_gated_recurrence_backend.run_hip_gated_recurrence(order(x), order(gate))
+    calls = [(lambda: recurrence(True), [x, gate], 2), (lambda: recurrence(False), [x, gate], 2),
+             (lambda: hip_block_norm_backend.run_hip_block_norm(x, gate), [x, gate], 2),
+             (lambda: hip_token_scores_backend.run_hip_token_scores(logits, tokens, 3), [logits], 1)]      # entropy is saved for the gradient
+    for call, leaves, n_written in calls:
+        for k in range(n_written):
+            answers = []
+            for in_place in (False, True):
+                out = call()[k]
+                cover = mask if out.shape == mask.shape else torch.ones_like(out, dtype=torch.bool).tril()
+                out = (out.add_(1.0).masked_fill_(cover, 0.0) if in_place else (out + 1.0).masked_fill(cover, 0.0))
+                answers.append([out.detach(), *torch.autograd.grad((out * out).sum(), leaves)])
+            assert all(torch.equal(a, b) for a, b in zip(*answers))

@@ -48,11 +48,10 @@ def check_gated_recurrence_support(x_seq, gate_seq, state=None, form: str = "lea
 
 
 def _empty_like_steps(x: torch.Tensor) -> torch.Tensor:
-    """[T, N, D] whose memory has steps and sequences in x's order: a batch-first tensor seen steps-first gives one again."""
+    """[T, N, D] whose memory has steps and sequences in x's order: a batch-first tensor seen steps-first gives one again. No view of another
+    tensor: autograd lets several outputs of a function be written over only if they are none."""
     T, N, D = x.shape
-    if x.stride(1) > x.stride(0):
-        return torch.empty((N, T, D), dtype=x.dtype, device=x.device).transpose(0, 1)
-    return torch.empty((T, N, D), dtype=x.dtype, device=x.device)
+    return torch.empty_strided((T, N, D), (D, T * D, 1) if x.stride(1) > x.stride(0) else (N * D, D, 1), dtype=x.dtype, device=x.device)
 
 
 def _series(t: torch.Tensor) -> Tuple[int, int, int]:

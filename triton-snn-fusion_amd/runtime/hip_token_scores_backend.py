@@ -46,17 +46,17 @@ def _forward(logits, tokens, top_k: int, keep_stats: bool):
     lib = _lib.lib()
     rows, V = logits.shape
     with on_device_of(logits):
-        scores = torch.empty((2, rows), dtype=torch.float32, device=logits.device)
+        logprob, entropy = (torch.empty(rows, dtype=torch.float32, device=logits.device) for _ in range(2))
         top_logprob = torch.empty((rows, top_k), dtype=torch.float32, device=logits.device) if top_k else None
         top_token = torch.empty((rows, top_k), dtype=torch.int64, device=logits.device) if top_k else None
         stats = torch.empty((rows, 2), dtype=torch.float32, device=logits.device) if keep_stats else None
         nbytes = lib.snnf_token_scores_workspace_bytes(rows, V, top_k)
         space = workspace(nbytes, logits)
         _lib.check("snnf_token_scores", lib.snnf_token_scores(
-            logits.data_ptr(), logits.stride(0), rows, V, _lib.dtype_code(logits.dtype), _lib.ptr(tokens), top_k, scores[0].data_ptr(),
-            scores[1].data_ptr(), _lib.ptr(top_logprob), _lib.ptr(top_token), _lib.ptr(stats), _lib.ptr(space), nbytes,
+            logits.data_ptr(), logits.stride(0), rows, V, _lib.dtype_code(logits.dtype), _lib.ptr(tokens), top_k, logprob.data_ptr(),
+            entropy.data_ptr(), _lib.ptr(top_logprob), _lib.ptr(top_token), _lib.ptr(stats), _lib.ptr(space), nbytes,
             _lib.current_stream(logits.device)))
-    return scores[0], scores[1], top_logprob, top_token, stats
+    return logprob, entropy, top_logprob, top_token, stats
 
 
 class _TokenScores(torch.autograd.Function):
