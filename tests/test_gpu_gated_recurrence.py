@@ -448,6 +448,38 @@ def test_refusals_on_the_gpu(hip_ops):
         torch.autograd.grad(torch.autograd.grad(out, x, create_graph=True)[0].sum(), x)
 
 
+def test_steps_too_far_apart_are_among_the_reasons():
+    """What the kernels refuse of strides is listed beforehand, of the tensor that h_seq will be as well."""
+    from torch._subclasses import FakeTensorMode
+    from triton_snn_fusion_amd.runtime.hip_gated_recurrence_backend import check_gated_recurrence_support as reasons
+    with FakeTensorMode():
+        far = torch.empty(16, 65536, 2048, dtype=torch.bfloat16, device="cuda")
+        near_by = torch.empty(65536, 16, 2048, dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+        assert len(reasons(far, far)) == 3 and all("unsupported_stride" in r for r in reasons(far, far))
+        assert len(reasons(near_by, far)) == 1 and "unsupported_stride: gate_seq" in reasons(near_by, far)[0]
+        one = torch.empty(1, 1, 2048, dtype=torch.bfloat16, device="cuda").expand(16, 65536, 2048)
+        assert len(reasons(one, near_by)) == 1 and "unsupported_stride: h_seq" in reasons(one, near_by)[0]
+        apart = torch.empty(2048, 16, 65536, dtype=torch.bfloat16, device="cuda").permute(1, 2, 0)     # channels apart: copied to steps outermost
+        assert sum("unsupported_stride: gate_seq" in r for r in reasons(near_by, apart)) == 1
+        assert reasons(near_by, near_by) == [] and reasons(far[:1], far[:1]) == [] and reasons(far[:, :1], far[:, :1]) != []
+
+
+@pytest.mark.gpu
+def test_a_gradient_whose_steps_lie_far_apart(hip_ops):
+    """Sequences outermost go in whatever their size; a gradient with the steps outermost, 2 GiB within 16 steps, is brought into their order."""
+    T, N, D = 16, 4096, 17600
+    g = torch.Generator(device=DEV).manual_seed(5)
+    draw = lambda *shape: torch.randn(shape, generator=g, device=DEV, dtype=torch.bfloat16)
+    x, gate = (draw(N, T, D).transpose(0, 1).requires_grad_(True) for _ in range(2))
+    dh = draw(T, N, D)
+    h, _ = run(x, gate)
+    got = torch.autograd.grad(h, [x, gate], dh, retain_graph=True)
+    want = torch.autograd.grad(h, [x, gate], dh.transpose(0, 1).contiguous().transpose(0, 1))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del x, gate, dh, h, got, want
+    torch.cuda.empty_cache()
+
+
 def test_refusals_without_a_gpu():
     x = torch.zeros(4, 2, 8)
     with pytest.raises(RuntimeError, match="unsupported_device"):

@@ -79,6 +79,11 @@ inline Tensor empty_steps(const Tensor& x) {
     return at::empty_strided({T, N, D}, batch_first ? std::array<int64_t, 3>{D, T * D, 1} : std::array<int64_t, 3>{N * D, D, 1}, x.options().requires_grad(false));
 }
 
+// The kernels reach the steps that a thread takes at once, up to 16, by offsets of 31 bits.
+inline bool within_reach(const Tensor& t) {
+    return (t.stride(0) * (std::min<int64_t>(t.size(0), 16) - 1) + t.size(2)) * static_cast<int64_t>(t.element_size()) < 0x7fffffff;
+}
+
 struct Recurrence : torch::autograd::Function<Recurrence> {
     static variable_list compute(const Tensor& x, const Tensor& gate, const Tensor& state, const Tensor& starts, const Tensor& lengths, int64_t form, Tensor* marks) {
         const c10::DeviceGuard guard(x.device());
@@ -110,7 +115,10 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
         const c10::DeviceGuard guard(x.device());
         const int T = static_cast<int>(x.size(0)), N = static_cast<int>(x.size(1)), D = static_cast<int>(x.size(2)), code = code_of(x.scalar_type());
         Tensor dh = grads[0].defined() ? grads[0] : at::zeros({D}, x.options().requires_grad(false)).expand({T, N, D});
-        if (!unit_rows(dh)) dh = dh.contiguous();
+        if (!unit_rows(dh) || !within_reach(dh)) {
+            Tensor near_by = empty_steps(x);
+            dh = near_by.copy_(dh);
+        }
         const Tensor dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
         Tensor dx = empty_steps(x), dgate = empty_steps(x), dstate = empty({N, D}, at::kFloat, x);
         const size_t bytes = snnf_gated_recurrence_workspace_bytes(T, N, D, code, 1);

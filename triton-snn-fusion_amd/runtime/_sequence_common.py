@@ -84,9 +84,14 @@ def on_device_of(t: torch.Tensor):
     return torch.cuda.device(t.device)
 
 
+def unit_rows_in_place(t: torch.Tensor) -> bool:
+    """Whether neighbouring elements of the last dimension lie next to each other."""
+    return t.shape[-1] <= 1 or t.stride(-1) == 1
+
+
 def unit_rows(t: torch.Tensor) -> torch.Tensor:
-    """The tensor itself where neighbouring elements of the last dimension lie next to each other, else a copy."""
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    """The tensor itself where they do, else a copy."""
+    return t if unit_rows_in_place(t) else t.contiguous()
 
 
 def workspace(nbytes: int, like: torch.Tensor) -> Optional[torch.Tensor]:

@@ -17,7 +17,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._sequence_common import check_activation, check_operand, check_unobserved, native, on_device_of, refuse, refuse_observed, unit_rows, wants_gradient, workspace
+from ._sequence_common import check_activation, check_operand, check_unobserved, native, on_device_of, refuse, refuse_observed, unit_rows, unit_rows_in_place, wants_gradient, workspace
 
 FORMS = {"leaky": 0, "linear": 1}
 OPERANDS = ("x_seq", "gate_seq", "state", "starts", "lengths")
@@ -44,14 +44,31 @@ def check_gated_recurrence_support(x_seq, gate_seq, state=None, form: str = "lea
         check_operand("starts", starts, x_seq.device, (T, N), (torch.bool,), reasons)
     if lengths is not None:
         check_operand("lengths", lengths, x_seq.device, (N,), (torch.int32, torch.int64), reasons)
+    if not reasons:
+        for name, step in (("x_seq", _step_of(x_seq)), ("gate_seq", _step_of(gate_seq)), ("h_seq", _steps_like(x_seq)[0])):
+            if not _within_reach(x_seq, step):
+                reasons.append(f"unsupported_stride: {name} has steps {step} elements apart, of which 16 may not pass 2 GiB")
     return reasons
 
 
-def _empty_like_steps(x: torch.Tensor) -> torch.Tensor:
-    """[T, N, D] whose memory has steps and sequences in x's order: a batch-first tensor seen steps-first gives one again. No view of another
-    tensor: autograd lets several outputs of a function be written over only if they are none."""
+def _steps_like(x: torch.Tensor) -> Tuple[int, int, int]:
+    """Strides of a [T, N, D] tensor whose memory has steps and sequences in x's order: a batch-first tensor seen steps-first gives one again."""
     T, N, D = x.shape
-    return torch.empty_strided((T, N, D), (D, T * D, 1) if x.stride(1) > x.stride(0) else (N * D, D, 1), dtype=x.dtype, device=x.device)
+    return (D, T * D, 1) if unit_rows_in_place(x) and x.stride(1) > x.stride(0) else (N * D, D, 1)
+
+
+def _step_of(t: torch.Tensor) -> int:
+    return t.stride(0) if unit_rows_in_place(t) else t.shape[1] * t.shape[2]        # of the copy
+
+
+def _within_reach(x: torch.Tensor, step: int) -> bool:
+    """The kernels reach the steps that a thread takes at once, up to 16, by offsets of 31 bits."""
+    return (step * (min(x.shape[0], 16) - 1) + x.shape[2]) * x.element_size() < 0x7FFFFFFF
+
+
+def _empty_like_steps(x: torch.Tensor) -> torch.Tensor:
+    """A tensor of x's shape and order in memory. No view of another: autograd lets several outputs of a function be written over only if they are none."""
+    return torch.empty_strided(x.shape, _steps_like(x), dtype=x.dtype, device=x.device)
 
 
 def _series(t: torch.Tensor) -> Tuple[int, int, int]:
@@ -96,7 +113,10 @@ class _GatedRecurrence(torch.autograd.Function):
         T, N, D = (int(n) for n in x.shape)
         code = _lib.dtype_code(x.dtype)
         with on_device_of(x):
-            dh = torch.zeros(D, dtype=x.dtype, device=x.device).expand(T, N, D) if dh is None else unit_rows(dh)
+            if dh is None:
+                dh = torch.zeros(D, dtype=x.dtype, device=x.device).expand(T, N, D)
+            elif not (unit_rows_in_place(dh) and _within_reach(dh, dh.stride(0))):
+                dh = _empty_like_steps(x).copy_(dh)
             dlast = None if dlast is None else dlast.contiguous()
             dx, dgate = _empty_like_steps(x), _empty_like_steps(x)
             dstate = torch.empty((N, D), dtype=torch.float32, device=x.device)
@@ -115,7 +135,7 @@ def run_hip_gated_recurrence(x_seq: torch.Tensor, gate_seq: torch.Tensor, state:
 
     x_seq, gate_seq: [T, N, D], float32, bfloat16 or float16, steps outermost as everywhere here; a batch-first tensor goes in as
         `t.transpose(0, 1)`, a slice of a wider projection or an expanded gate as it is: nothing is copied unless neighbouring channels lie
-        apart, and h_seq has x_seq's order in memory.
+        apart, and h_seq has x_seq's order in memory. 16 steps may not pass 2 GiB: where sequences are that many, they go in batch-first.
     state: [N, D] float32 before the first step (None: zeros). The returned state is float32 and new memory; T = 0 returns it unchanged.
     starts: [T, N] bool. Where set, the state is dropped before the step (several documents packed into one sequence); what the state
         held, infinities and NaN among it, does not reach the steps from there on. Nothing else ends either.
