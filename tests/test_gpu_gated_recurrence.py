@@ -115,6 +115,39 @@ def test_sizes(hip_ops, T, N, D, dtype, form):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,T,N", [(torch.float32, 1500, 96), (torch.bfloat16, 1500, 192), (torch.float32, 4096, 2), (torch.bfloat16, 4096, 2)])
+def test_long_memories(hip_ops, dtype, T, N):
+    """Channels that remember over m = 300 to 2000 steps, each with one decay for all steps, so that what a step's decay loses to rounding is the same
+    every time: the state and the gradient come from runs of S = 8 steps (16 forward where tiles are relayed, N = 2) whose decay is worked out as 1 - c.
+
+    A run adds half a step of 1 - c, 2^-25, and one of its sum, 2^-24; m / S of them are remembered. Inside a run a step adds 2^-24 of the sum and up to 2.5 of the
+    decay (1 + e, its reciprocal). 64 for the exponential (16 in 16 bits, twice: decay and input) and the join of a tile (14 runs, each
+    half a step of 1 - c, and their sums): 1.5 m / S + 3.5 S + 64 in units of 2^-24 of the largest state. A decay worked out as a product of rounded
+    decays instead loses up to 2.5 a step: in float32 arithmetic on the CPU these cases are off by 50 to 100 units so and by 1400 to 2200 as a product."""
+    D = 128
+    g = gen(29)
+    memory = torch.exp(torch.empty(D).uniform_(5.704, 7.6, generator=g))            # 300 to 2000
+    gate = torch.log(memory - 1).to(dtype)[None, None].expand(T, N, D).contiguous()
+    x, dh = (1 + 0.1 * torch.randn(T, N, D, generator=g)).to(dtype), (1 + 0.1 * torch.randn(T, N, D, generator=g)).to(dtype)
+    state, dlast = torch.ones(N, D), 300 * torch.ones(N, D)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, gate, state)]
+    h, last = run(*leaves)
+    dx, dgate, dstate = torch.autograd.grad([h, last], leaves, [dh.to(DEV), dlast.to(DEV)])
+    want_h, want_last, peak, want_dx, want_dgate, want_dstate, most = reference(x, gate, state, "leaky", dh=dh, dlast=dlast)
+    units = lambda S: U * (1.5 * 2048 / S + 3.5 * S + 64)                           # 2048: a gate in bfloat16 may be half a step of 2^-6 more
+    h_off, s_off = units(16 if N == 2 else 8) * peak, units(8) * most
+    near(h.detach(), want_h, dtype, h_off, "h")
+    near(last.detach(), want_last, torch.float32, h_off, "last state")
+    near(dstate, want_dstate, torch.float32, s_off, "dstate")
+    rest = torch.sigmoid(-gate.double())
+    near(dx, want_dx, dtype, rest * s_off + 32 * U * want_dx.abs(), "dx")
+    before = torch.cat([state.double()[None], want_h[:-1]])
+    # h of the gradient's pass comes from runs of 8 steps whatever the forward pass did
+    room = want_dx.abs() * units(8) * peak + rest * s_off * ((before - x.double()).abs() + units(8) * peak) + 32 * U * want_dgate.abs()
+    near(dgate, want_dgate, dtype, room, "dgate")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_many_columns_take_narrow_workgroups(hip_ops, dtype):
     check(70, 40, 4096 if dtype == torch.float32 else 8192, dtype, "leaky", 7)      # 2560 waves of columns and more
