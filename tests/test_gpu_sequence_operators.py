@@ -506,3 +506,50 @@ def test_outputs_may_be_written_over(hip_ops, monkeypatch, python):
                 out = (out.add_(1.0).masked_fill_(cover, 0.0) if in_place else (out + 1.0).masked_fill(cover, 0.0))
                 answers.append([out.detach(), *torch.autograd.grad((out * out).sum(), leaves)])
             assert all(torch.equal(a, b) for a, b in zip(*answers))
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# torch.fx
+# ------------------------------------------------------------------------------------------------------------------
+class Block(torch.nn.Module):
+    """One layer of a token model with its scores."""
+
+    def __init__(self, seed=7):
+        super().__init__()
+        for name, value in weights(torch.float32, seed).items():
+            setattr(self, name, torch.nn.Parameter(value))
+
+    def forward(self, residual, tokens, state=None):
+        from triton_snn_fusion_amd.runtime.hip_block_norm_backend import run_hip_block_norm
+        from triton_snn_fusion_amd.runtime.hip_gated_recurrence_backend import run_hip_gated_recurrence
+        from triton_snn_fusion_amd.runtime.hip_token_scores_backend import run_hip_token_scores
+        _, normed = run_hip_block_norm(residual, next_weight=self.n1)
+        x, gate, out_gate = (normed @ self.w_in).split(D, -1)
+        h, state = run_hip_gated_recurrence(x, gate, state, form="leaky")
+        residual, normed = run_hip_block_norm(residual, h, out_gate, self.n2, self.n3, self.scale, gate_form="silu")
+        scores = run_hip_token_scores(normed @ self.w_out, tokens, top_k=3)
+        return scores.logprob, scores.entropy, scores.top_token, state
+
+
+def test_a_symbolic_trace_holds_the_operators():
+    """torch.fx records each call as one node, as it does torch's own functions; a module that uses them can be traced without a GPU."""
+    traced = torch.fx.symbolic_trace(Block())
+    names = [node.target.__name__ for node in traced.graph.nodes if node.op == "call_function" and node.target.__name__.startswith("run_hip")]
+    assert names == ["run_hip_block_norm", "run_hip_gated_recurrence", "run_hip_block_norm", "run_hip_token_scores"]
+    from triton_snn_fusion_amd.runtime.hip_token_scores_backend import run_hip_token_scores
+    with pytest.raises(RuntimeError, match="must be a tensor"):
+        run_hip_token_scores("no tensor")
+
+
+@pytest.mark.gpu
+def test_a_traced_module_runs_as_it_is_written(hip_ops):
+    block = Block().to(DEV)
+    traced = torch.fx.symbolic_trace(block)
+    g = gen(3)
+    residual, tokens = torch.randn(6, 2, D, generator=g).to(DEV).requires_grad_(True), torch.randint(0, VOCABULARY, (6, 2), generator=g).to(DEV)
+    state = torch.randn(2, D, generator=g).to(DEV)
+    answers = []
+    for module in (block, traced):
+        out = module(residual, tokens, state)
+        answers.append([*out, *torch.autograd.grad(out[0].sum() + out[1].sum() + out[3].sum(), [residual, *block.parameters()])])
+    assert all(torch.equal(a, b) for a, b in zip(*answers))

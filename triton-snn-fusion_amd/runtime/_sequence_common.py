@@ -5,12 +5,20 @@ import contextlib
 from typing import Iterable, List, Optional, Tuple
 
 import torch
+import torch.fx
 from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from .. import _dispatch
 
 SUPPORTED_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def recorded(function, operands: tuple, options: dict):
+    """A call that the kernels do not take: None, or where torch.fx traces the program, which hands it stand-ins for tensors, the node that records it."""
+    if any(isinstance(t, torch.fx.Proxy) for t in operands):
+        return torch.overrides.handle_torch_function(function, operands, *operands, **options)
+    return None
 
 
 def refuse(operator: str, reasons: List[str]) -> None:

@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._sequence_common import SUPPORTED_DTYPES, check_activation, check_operand, check_unobserved, flat_rows, native, on_device_of, refuse, refuse_observed, wants_gradient, workspace
+from ._sequence_common import SUPPORTED_DTYPES, check_activation, check_operand, check_unobserved, flat_rows, native, on_device_of, recorded, refuse, refuse_observed, wants_gradient, workspace
 
 KINDS = {"rms": 0, "layer": 1}
 GATE_FORMS = {"sigmoid": 1, "silu": 2}
@@ -142,7 +142,12 @@ def run_hip_block_norm(residual: torch.Tensor, branch: Optional[torch.Tensor] = 
                                   1.0 if learnt or scale is None else scale, KINDS[kind], GATE_FORMS[gate_form], eps)
         if known is not None:
             return known
-    refuse("run_hip_block_norm", check_block_norm_support(residual, branch, gate, branch_weight, next_weight, scale, kind, gate_form, eps))
+    reasons = check_block_norm_support(residual, branch, gate, branch_weight, next_weight, scale, kind, gate_form, eps)
+    if reasons:
+        node = recorded(run_hip_block_norm, (residual, branch, gate, branch_weight, next_weight, scale), {"kind": kind, "gate_form": gate_form, "eps": eps})
+        if node is not None:
+            return node
+        refuse("run_hip_block_norm", reasons)
     factor = 1.0
     if not learnt and scale is not None:
         factor, scale = float(scale), None

@@ -17,7 +17,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._sequence_common import check_activation, check_operand, check_unobserved, native, on_device_of, refuse, refuse_observed, unit_rows, unit_rows_in_place, wants_gradient, workspace
+from ._sequence_common import check_activation, check_operand, check_unobserved, native, on_device_of, recorded, refuse, refuse_observed, unit_rows, unit_rows_in_place, wants_gradient, workspace
 
 FORMS = {"leaky": 0, "linear": 1}
 OPERANDS = ("x_seq", "gate_seq", "state", "starts", "lengths")
@@ -152,7 +152,12 @@ def run_hip_gated_recurrence(x_seq: torch.Tensor, gate_seq: torch.Tensor, state:
         known = module.gated_recurrence(x_seq, gate_seq, state, starts, lengths, FORMS[form])
         if known is not None:
             return known
-    refuse("run_hip_gated_recurrence", check_gated_recurrence_support(x_seq, gate_seq, state, form, starts, lengths))
+    reasons = check_gated_recurrence_support(x_seq, gate_seq, state, form, starts, lengths)
+    if reasons:
+        node = recorded(run_hip_gated_recurrence, (x_seq, gate_seq, state), {"form": form, "starts": starts, "lengths": lengths})
+        if node is not None:
+            return node
+        refuse("run_hip_gated_recurrence", reasons)
     T, N, D = (int(n) for n in x_seq.shape)
     if T == 0:
         last = torch.zeros((N, D), dtype=torch.float32, device=x_seq.device) if state is None else state.clone()

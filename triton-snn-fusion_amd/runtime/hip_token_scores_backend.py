@@ -12,7 +12,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._sequence_common import check_activation, check_operand, check_unobserved, flat_rows, native, on_device_of, refuse, refuse_observed, wants_gradient, workspace
+from ._sequence_common import check_activation, check_operand, check_unobserved, flat_rows, native, on_device_of, recorded, refuse, refuse_observed, wants_gradient, workspace
 
 MAX_ALTERNATIVES = 64
 
@@ -100,7 +100,12 @@ def run_hip_token_scores(logits: torch.Tensor, tokens: Optional[torch.Tensor] = 
         known = module.token_scores(logits, tokens, top_k)
         if known is not None:
             return TokenScores(*known)
-    refuse("run_hip_token_scores", check_token_scores_support(logits, tokens, top_k))
+    reasons = check_token_scores_support(logits, tokens, top_k)
+    if reasons:
+        node = recorded(run_hip_token_scores, (logits, tokens), {"top_k": top_k})
+        if node is not None:
+            return node
+        refuse("run_hip_token_scores", reasons)
     lead = logits.shape[:-1]
     if logits.numel() == 0:
         zeros = logits.sum(-1, dtype=torch.float32)        # no rows, but differentiable
