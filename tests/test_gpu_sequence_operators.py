@@ -553,3 +553,23 @@ def test_a_traced_module_runs_as_it_is_written(hip_ops):
         out = module(residual, tokens, state)
         answers.append([*out, *torch.autograd.grad(out[0].sum() + out[1].sum() + out[3].sum(), [residual, *block.parameters()])])
     assert all(torch.equal(a, b) for a, b in zip(*answers))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("python", [False, True])
+def test_operands_whose_elements_lie_elsewhere_are_refused(hip_ops, monkeypatch, python):
+    """A subclass that wraps other tensors has no address, and an operand without one must not pass for one that a call lacks."""
+    from torch.testing._internal.two_tensor import TwoTensor
+    from triton_snn_fusion_amd.runtime import _sequence_common, hip_block_norm_backend, hip_gated_recurrence_backend, hip_token_scores_backend
+    if python:
+        for backend in (_sequence_common, hip_block_norm_backend, hip_gated_recurrence_backend, hip_token_scores_backend):
+            monkeypatch.setattr(backend, "native", lambda t: None)
+    x, vector, rows = torch.randn(4, 2, 8, device=DEV), torch.randn(8, device=DEV), torch.randn(2, 8, device=DEV)
+    wrap = lambda t: TwoTensor(t, t.clone())
+    recurrence, norm = hip_gated_recurrence_backend.run_hip_gated_recurrence, hip_block_norm_backend.run_hip_block_norm
+    for call in (lambda: recurrence(x, x, wrap(rows)), lambda: recurrence(x, x, starts=wrap(torch.ones(4, 2, dtype=torch.bool, device=DEV))),
+                 lambda: recurrence(x, x, lengths=wrap(torch.ones(2, dtype=torch.int32, device=DEV))), lambda: recurrence(wrap(x), x),
+                 lambda: norm(x, x, gate=wrap(x)), lambda: norm(x, x, next_weight=wrap(vector)), lambda: norm(x, x, scale=wrap(vector)),
+                 lambda: hip_token_scores_backend.run_hip_token_scores(rows, wrap(torch.zeros(2, dtype=torch.int64, device=DEV)))):
+        with pytest.raises(RuntimeError, match="unsupported_subclass"):
+            call()

@@ -17,7 +17,8 @@ inline bool activation(const Tensor& t) {
     return t.defined() && t.is_cuda() && t.layout() == at::kStrided && dtype_code(t.scalar_type(), &code) && t.numel() > 0;
 }
 // Whether the kernels' work is all there is to a call: what traces torch's operations would record the outputs' allocation and nothing that fills them, a
-// tangent of forward-mode differentiation would be lost, and a tensor that a transform of torch.func wraps has no memory of its own.
+// tangent of forward-mode differentiation would be lost, a tensor that a transform of torch.func wraps has no memory of its own, and a subclass may be a
+// wrapper without an address.
 inline bool traced() {
     using Modes = c10::impl::TorchDispatchModeTLS;
     return torch::jit::tracer::isTracing() || (Modes::any_modes_set() && Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value());
@@ -25,7 +26,7 @@ inline bool traced() {
 inline bool unobserved(c10::ArrayRef<const Tensor*> tensors) {
     if (traced()) return false;
     for (const Tensor* t : tensors)
-        if (t->defined() && (!t->has_storage() || t->_fw_grad(0).defined())) return false;
+        if (t->defined() && (!t->has_storage() || t->unsafeGetTensorImpl()->is_python_dispatch() || t->_fw_grad(0).defined())) return false;
     return true;
 }
 // The same of the gradients that autograd hands over: there is no other implementation to refuse them.
@@ -34,6 +35,7 @@ inline void check_gradients(const char* name, const variable_list& grads) {
     for (const Tensor& d : grads) {
         if (!d.defined()) continue;
         TORCH_CHECK(d.has_storage(), name, ": unsupported_transform: a gradient is wrapped by a transform (torch.func, vmap) and has no memory of its own");
+        TORCH_CHECK(d.const_data_ptr() != nullptr || d.numel() == 0, name, ": unsupported_subclass: a gradient wraps other tensors");
         TORCH_CHECK(!d._fw_grad(0).defined(), name, ": unsupported_forward_ad: a gradient has a tangent, and there is no forward-mode derivative");
     }
 }

@@ -8,6 +8,7 @@ import torch
 import torch.fx
 from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import get_proxy_mode
+from torch.utils._python_dispatch import is_traceable_wrapper_subclass
 
 from .. import _dispatch
 
@@ -43,6 +44,8 @@ def check_unobserved(reasons: List[str], names: Tuple[str, ...], *operands) -> N
             t.untyped_storage()
         except (NotImplementedError, RuntimeError):
             reasons.append(f"unsupported_transform: {name} is wrapped by a transform (torch.func, vmap) and has no memory of its own")
+        if is_traceable_wrapper_subclass(t):
+            reasons.append(f"unsupported_subclass: {name} is a {type(t).__name__}, which wraps other tensors and has no address")
 
 
 def refuse_observed(operator: str, names: Tuple[str, ...], *gradients) -> None:
