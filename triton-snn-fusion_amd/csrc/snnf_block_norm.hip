@@ -2,7 +2,7 @@
 //     y = norm(branch) * branch_weight;   residual' = residual + factor * scale * act(gate) * y;   normed = norm(residual') * next_weight
 // norm takes the mean out (LAYER) or not and divides by sqrt(mean of squares + eps); without a branch residual' is the residual. With unit = the
 // divided row and r = 1 / sqrt(...), the gradient through a norm is r * (d - unit * mean(d * unit) [- mean(d)]).
-// A row lies in the registers of P threads (8 elements each, 16 where rows pass 8192), so that every tensor is read once; its statistics are
+// A row lies in the registers of P threads (8 elements each, 16 where rows pass 4096), so that every tensor is read once; its statistics are
 // sums over them, and the backward pass reads the row statistics that the forward pass leaves. What a program's vectors get as gradients is
 // summed over the rows a workgroup takes in registers, and over the workgroups by a second kernel, in a fixed order.
 // Bound by memory: 5 tensors forward, 8 backward (32768 x 2048 bf16, gated: 128 us, 5.2 TB/s, and 224 us, 4.8 TB/s); few rows by the sums over
@@ -435,7 +435,9 @@ struct NormShape {
 // 4096 x 8192 107 in place of 63, and the backward pass no longer fits the registers). Workgroups: as many as are resident at once, which walk
 // over the rows (four times as many: 8192 x 4096 65 -> 68 us forward, 131 -> 157 backward; 8192 x 2048 33 -> 31, 77 -> 86). Backward, a
 // workgroup takes at least four rows to a slot where that leaves one for every compute unit: its sums over rows cost as much memory as a
-// row does (1000 x 1024: 14.6 us, without 16.7; 1531 x 777 float32 19.2 and 21.0; the other way 2000 x 2048 28.3 and 25.2).
+// row does (1000 x 1024: 14.6 us, without 16.7; 1531 x 777 float32 19.2 and 21.0; the other way 2000 x 2048 28.3 and 25.2). Rows past 8192 take 1024 threads,
+// whose 128 registers do not hold 16 elements of everything: all 18 backward kernels of that size keep up to 1032 bytes a lane in scratch memory, and 10 of the 18
+// forward ones, whose vectors are float32, up to 304 (2048 x 12288 bf16 forward 67 us, of which 47 are its bytes, backward 870, of which 75 are).
 NormShape norm_shape(int64_t rows, int D, bool backward, int vec) {
     NormShape s;
     s.per_row = 8;

@@ -191,7 +191,9 @@ __device__ __forceinline__ void store(const Output& to, const Place& q, int firs
 // ------------------------------------------------------------------------------------------------------------------
 // Relay: a tile publishes its (A, H), takes the value that enters it from the tiles in front of it in the order of the scan, and publishes
 // the value behind it. Each word says by itself whether it is known, so that relaxed accesses of the agent's scope are enough.
-// A tile waits only for tiles that were handed out before it: those run already and publish their (A, H) without waiting for anyone.
+// Every wait ends whatever else shares the chip: a tile waits only for tiles that were handed out before it, and of those that are not done the one
+// handed out first waits for none, since all before it have published their value. (A workgroup takes its next tile while its last one may still wait, so
+// that a tile handed out need not have published anything yet.)
 // ------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t plain_bits(float v) { return v != v ? 0x7fc00000u : __float_as_uint(v); }      // never all ones
 
@@ -749,7 +751,8 @@ struct Shape {
 
 // Relay where columns of 64 * VEC channels are fewer than three quarters of the compute units, and the sequence longer than its way through
 // memory pays for (bf16: 4096 steps, 128 columns, walk 152 us, relay 107; 256 columns 83 and 104; 32 columns, 300 steps 11.3 and 11.6, 600 steps
-// 21.2 and 12.4). The rule goes by what the forward and the backward pass both know, not by alignment: marks lie where backward tiles begin.
+// 21.2 and 12.4). The rule goes by what the forward and the backward pass both know, not by alignment: marks lie where backward tiles begin. It counts
+// columns as if every lane had a channel, which sequences of few channels that starts or lengths keep apart do not come to.
 Shape shape_of(int T, int N, int D, int dtype, bool backward) {
     const int units = compute_units();
     const int64_t columns = static_cast<int64_t>(N) * D / (dtype == SNNF_F32 ? 64 : 128);
