@@ -157,7 +157,7 @@ def _plain_delta_forward(s, query, key, value, gate, beta, state):
     case = s["case"]
     t, n, dk = case["t"], case["n"], case["dk"]
     inside = torch.ones(t, n, dtype=torch.bool, device=DEVICE) if s["lengths"] is None else torch.arange(t, device=DEVICE)[:, None] < s["lengths"][None, :]
-    starts = torch.zeros(t, n, dtype=torch.bool, device=DEVICE) if s["starts"] is None else s["starts"]
+    starts = torch.zeros(t, n, dtype=torch.bool, device=DEVICE) if s["starts"] is None else s["starts"] & inside
     chunk = min(CHUNK, 1 << (t - 1).bit_length())
     count = -(-t // chunk)
 
