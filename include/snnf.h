@@ -532,6 +532,47 @@ int snnf_token_scores(const void* logits, int64_t row, int64_t rows, int V, int 
 int snnf_token_scores_backward(const void* logits, int64_t row, int64_t rows, int V, int dtype, const int64_t* tokens, const float* stats,
                                const float* entropy, const float* d_logprob, const float* d_entropy, void* d_logits, void* stream);
 
+/* Heads of [T, N, heads, D] (or gates of [T, N, heads]): elements of a head next to each other, steps, sequences and heads any number of elements apart. */
+typedef struct snnf_heads {
+    void* data;
+    int64_t step, row, head;
+} snnf_heads;
+
+#define SNNF_DELTA_RULE_MAX_KEY 128
+#define SNNF_DELTA_RULE_MAX_VALUE 1024
+
+/* Gated delta rule: per sequence and value head a state S of [key_size, value_size], at every step
+ *     S <- exp(gate) S,   S <- S + beta key (value - S^T key)^T,   out = scale S^T query
+ * with value head j on head j / (value_heads / heads) of query and key. */
+typedef struct snnf_delta_rule_call {
+    int T, N, heads, value_heads, key_size, value_size;
+    int dtype, gate_dtype;                   /* gate_dtype: dtype or SNNF_F32 */
+    float scale;
+    snnf_heads query, key, value, gate, beta;  /* gate.data NULL: no decay; beta.data NULL: 1 */
+    const void* starts;                      /* NULL or a byte per (step, sequence): where it is not 0 the state is dropped before the step */
+    int64_t starts_step, starts_row;
+    const int32_t* lengths;                  /* NULL or N: steps from there on leave the state as it is and read 0 in out; clamped to 0..T */
+    const float* state;                      /* NULL (zeros) or [N, value_heads, key_size, value_size] */
+} snnf_delta_rule_call;
+
+/*   state_out  as state; may be the same memory, and overlaps it in no other way      out  overlaps no input
+ *   marks      NULL, or snnf_delta_rule_marks_bytes(call) bytes that the backward pass will read
+ *   workspace  snnf_delta_rule_workspace_bytes(call, marks != NULL) bytes, 16-byte aligned (0: none needed), in use until the call's work is done
+ * A gate below -104 drops the state as a start does. Two launches, one for up to 16 steps without marks. */
+size_t snnf_delta_rule_workspace_bytes(const snnf_delta_rule_call* call, int training);
+size_t snnf_delta_rule_marks_bytes(const snnf_delta_rule_call* call);
+int snnf_delta_rule(const snnf_delta_rule_call* call, const snnf_heads* out, float* state_out, float* marks, void* workspace, size_t workspace_bytes,
+                    void* stream);
+
+/* Its gradient: `dout` and `dstate` (NULL: zeros) are the gradients of `out` and of the last state; dquery, dkey, dvalue, dgate, dbeta (data NULL: not wanted) and
+ * dstate_in (not dstate's memory) those of the operands, of their types; they overlap no input. Steps from a sequence's length on get 0, as does a gate that
+ * a start or its own value makes meaningless. `marks` as the forward call on the same operands left them; call->state is not read.
+ * Workspace: snnf_delta_rule_backward_workspace_bytes(call) bytes, 16-byte aligned. Three launches; sums have a fixed order. */
+size_t snnf_delta_rule_backward_workspace_bytes(const snnf_delta_rule_call* call);
+int snnf_delta_rule_backward(const snnf_delta_rule_call* call, const float* marks, const snnf_heads* dout, const float* dstate, const snnf_heads* dquery,
+                             const snnf_heads* dkey, const snnf_heads* dvalue, const snnf_heads* dgate, const snnf_heads* dbeta, float* dstate_in,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

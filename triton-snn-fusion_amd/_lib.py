@@ -27,6 +27,21 @@ _f = ctypes.c_float
 _sz = ctypes.c_size_t
 _pp = ctypes.POINTER(ctypes.c_void_p)
 
+
+
+class Heads(ctypes.Structure):
+    _fields_ = [("data", _vp), ("step", _i64), ("row", _i64), ("head", _i64)]
+
+
+class DeltaRuleCall(ctypes.Structure):
+    _fields_ = [*((name, _i) for name in ("T", "N", "heads", "value_heads", "key_size", "value_size", "dtype", "gate_dtype")), ("scale", _f),
+                *((name, Heads) for name in ("query", "key", "value", "gate", "beta")), ("starts", _vp), ("starts_step", _i64), ("starts_row", _i64), ("lengths", _vp),
+                ("state", _vp)]
+
+
+_heads = ctypes.POINTER(Heads)
+_delta = ctypes.POINTER(DeltaRuleCall)
+
 # name -> (restype, argtypes); must list every function declared in include/snnf.h.
 SIGNATURES = {
     "snnf_abi_version": (_i, []),
@@ -82,6 +97,11 @@ SIGNATURES = {
     "snnf_token_scores_workspace_bytes": (_sz, [_i64, _i, _i]),
     "snnf_token_scores": (_i, [_vp, _i64, _i64, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "snnf_token_scores_backward": (_i, [_vp, _i64, _i64, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "snnf_delta_rule_workspace_bytes": (_sz, [_delta, _i]),
+    "snnf_delta_rule_marks_bytes": (_sz, [_delta]),
+    "snnf_delta_rule": (_i, [_delta, _heads, _vp, _vp, _vp, _sz, _vp]),
+    "snnf_delta_rule_backward_workspace_bytes": (_sz, [_delta]),
+    "snnf_delta_rule_backward": (_i, [_delta, _vp, _heads, _vp, _heads, _heads, _heads, _heads, _heads, _vp, _vp, _sz, _vp]),
     "snnf_conv_bias": (_i, [_pp, _pp, _i, _i, _i, _i, _i, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _i64, _vp]),
 }
 

@@ -1,0 +1,523 @@
+// Gated delta rule, forward: per value head with a state S of [DK x DV]
+//     S <- exp(gate_t) S,   delta_t = v_t - S^T k_t,   S <- S + beta_t k_t delta_t^T,   out_t = scale S^T q_t
+// Chunks of 64 steps at once. With G the running sum of gates inside a chunk, D_ij = exp(G_i - G_j) for j <= i and L_ij = D_ij k_i . k_j for j < i:
+//     delta = (I + L diag(beta))^-1 (V - diag(e^G) K S),   out = scale (diag(e^G) Q S + (Q K^T o D) diag(beta) delta),
+//     S <- e^(G_64) S + K^T diag(e^(G_64 - G)) diag(beta) delta
+#include "snnf_delta_rule.h"
+
+namespace snnf {
+namespace {
+
+// ------------------------------------------------------------------------------------------------------------------
+// What chunks need that does not depend on the state
+// ------------------------------------------------------------------------------------------------------------------
+// The backward pass wants transposes: of the scores, and of (I + diag(beta) L)^-1, whose transpose turns a gradient of beta delta into that of the rows in front.
+constexpr int kPitch = 68;              // of a [64 x 64] matrix in LDS: rows start 4 banks apart
+
+// rows 16 a.., columns 16 b + 4 (lane / 16) + 0..3 of lane % 16's row
+__device__ __forceinline__ f32x4 block_row(const float* m, int a, int b) {
+    const int lane = threadIdx.x & 63;
+    return *reinterpret_cast<const f32x4*>(m + (16 * a + lane % 16) * kPitch + 16 * b + 4 * (lane / 16));
+}
+__device__ __forceinline__ f32x4 multiply_f32(const f32x4& a, const f32x4& b, f32x4 c) {       // 16 places, place 4 (lane / 16) + s in step s
+#pragma unroll
+    for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], c, 0, 0, 0);
+    return c;
+}
+
+template <typename T, int KS, bool BACKWARD>
+__global__ __launch_bounds__(256, 2) void delta_chunk_kernel(DeltaArgs p) {
+    constexpr int RANKS = BACKWARD ? 3 : kOutputRanks<T>;
+    __shared__ float lower[kChunk * kPitch], inverse[kChunk * kPitch], scores[kChunk * kPitch];
+    __shared__ double total[kChunk];
+    __shared__ int part[kChunk];
+    __shared__ float beta[kChunk];
+    const uint32_t index = group_index();
+    if (index >= static_cast<uint32_t>(p.N) * p.HV * p.chunks) return;
+    const int chunk = index % p.chunks, head = index / p.chunks, n = head / p.HV, hv = head % p.HV, h = hv / (p.HV / p.H);
+    const int first = chunk * kChunk, limit = length_of(p, n);
+    if (first >= limit) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane / 16, column = lane % 16;
+    float* vectors = p.vectors + static_cast<int64_t>(index) * 3 * kChunk;
+
+    if (wave == 0) {
+        const int t = first + lane;
+        const bool there = t < limit;
+        float g = there ? gate_value<T>(p.gate, p.gate_float, t, n, hv, 0.0f) : 0.0f;
+        const float b = there ? gate_value<T>(p.beta, p.gate_float, t, n, hv, 1.0f) : 0.0f;
+        const bool fresh = there && (g < kForgotten || (p.starts != nullptr && p.starts[t * p.starts_step + n * p.starts_row] != 0));
+        double sum = fresh ? 0.0 : static_cast<double>(g) * 1.4426950408889634074;
+        const int mine = __popcll(__ballot(fresh) & (~0ull >> (63 - lane)));
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const double before = __shfl_up(sum, d, 64);
+            if (lane >= d) sum += before;
+        }
+        total[lane] = sum, part[lane] = mine, beta[lane] = b;
+        const double all = __shfl(sum, 63, 64);
+        const int last = __shfl(mine, 63, 64);
+        vectors[lane] = mine == 0 ? decay_of(sum) : 0.0f;
+        vectors[kChunk + lane] = mine == last ? decay_of(all - sum) : 0.0f;
+        vectors[2 * kChunk + lane] = b;
+    }
+    const T* keys = static_cast<const T*>(p.k.data) + n * p.k.row + h * p.k.head;
+    const T* queries = static_cast<const T*>(p.q.data) + n * p.q.row + h * p.q.head;
+    f32x4 kk[4], qk[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) kk[j] = qk[j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        const int at = 32 * s + 8 * group, t = first + 16 * wave + column;
+        const bool there = t < limit && at < p.DK;
+        const auto k = there ? row_terms<T>(keys + t * p.k.step, at, p.DK) : no_terms<kTerms<T>>();
+        const auto q = there ? row_terms<T>(queries + t * p.q.step, at, p.DK) : no_terms<kTerms<T>>();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j > wave) break;
+            const int other = first + 16 * j + column;
+            const auto b = other < limit && at < p.DK ? row_terms<T>(keys + other * p.k.step, at, p.DK) : no_terms<kTerms<T>>();
+            kk[j] = product<3>(k, b, kk[j]);
+            qk[j] = product<3>(q, b, qk[j]);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int c = 16 * j + column;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int i = 16 * wave + 4 * group + r;
+            float d = 0.0f;
+            if (j <= wave && c <= i && part[i] == part[c]) d = decay_of(total[i] - total[c]);
+            const bool below = c < i && d != 0.0f;
+            lower[i * kPitch + c] = below ? d * kk[j][r] * beta[BACKWARD ? i : c] : 0.0f;
+            scores[i * kPitch + c] = d != 0.0f ? d * qk[j][r] * p.scale : 0.0f;
+            inverse[i * kPitch + c] = 0.0f;
+        }
+    }
+    __syncthreads();
+    // Diagonal blocks by substitution, a column of the inverse to a lane (four lanes to the same).
+    {
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float v = i == column ? 1.0f : 0.0f;
+            const float* row = lower + (16 * wave + i) * kPitch + 16 * wave;
+#pragma unroll
+            for (int j = 0; j < i; ++j) v = fmaf(-row[j], x[j], v);
+            x[i] = v;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (i / 4 == group) inverse[(16 * wave + i) * kPitch + 16 * wave + column] = x[i];
+    }
+    __syncthreads();
+    // Blocks below: T_ij = -T_ii sum_k A_ik T_kj, one diagonal of blocks after the other.
+#pragma unroll
+    for (int d = 1; d < 4; ++d) {
+        f32x4 corner{0, 0, 0, 0};
+        const int j = wave - d;
+        if (j >= 0) {
+            f32x4 sum{0, 0, 0, 0};
+            for (int k = j; k < wave; ++k) {
+                f32x4 b;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) b[s] = inverse[(16 * k + 4 * group + s) * kPitch + 16 * j + column];
+                sum = multiply_f32(block_row(lower, wave, k), b, sum);
+            }
+            corner = multiply_f32(block_row(inverse, wave, wave), sum, corner);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) inverse[(16 * wave + 4 * group + r) * kPitch + 16 * j + column] = -corner[r];
+        }
+        __syncthreads();
+    }
+    // Fragments as the other kernels load them.
+    uint32_t* blocks = p.blocks + static_cast<int64_t>(index) * block_words(RANKS);
+    const auto fragment = [&](const float* m, int f) {
+        if constexpr (BACKWARD) {
+            const float* from = m + (32 * upper_half(f) + 4 * group) * kPitch + 16 * upper_tile(f) + column;
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = from[(e < 4 ? e : 12 + e) * kPitch];
+            return split<3>(x);
+        } else {
+            const float* from = m + (16 * lower_tile(f) + column) * kPitch + 32 * lower_half(f) + 4 * group;
+            return split<3>(*reinterpret_cast<const f32x4*>(from), *reinterpret_cast<const f32x4*>(from + 16));
+        }
+    };
+    for (int f = wave; f < kBlocks; f += 4) {
+        const Terms<3> x = fragment(inverse, f), y = fragment(scores, f);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) *reinterpret_cast<u32x4a*>(blocks + (f * 3 + i) * 256 + lane * 4) = x.t[i];
+#pragma unroll
+        for (int i = 0; i < RANKS; ++i) *reinterpret_cast<u32x4a*>(blocks + (kBlocks * 3 + f * RANKS + i) * 256 + lane * 4) = y.t[i];
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// The walk over the chunks
+// ------------------------------------------------------------------------------------------------------------------
+// A wave owns 16 columns of the state, in accumulators, and of everything that is multiplied from it on: products go over the heads' elements
+// or over steps, whose place in an accumulator is a matter of the other operand's order, so that nothing but keys and queries passes through LDS.
+template <typename T, int KS, bool TRAIN>
+__global__ __launch_bounds__(256, 1) void delta_walk_kernel(DeltaArgs p) {
+    using Lds = Rows<T, KS>;
+    constexpr int RANKS = kOutputRanks<T>, BUFFERS = kTerms<T> == 1 ? 2 : 1;
+    __shared__ uint16_t lds[BUFFERS][2][Lds::kSize];
+    int head, columns;
+    if (!part_of_head(p.N * p.HV, (p.DV + 63) / 64, &head, &columns)) return;
+    const int n = head / p.HV, hv = head % p.HV, h = hv / (p.HV / p.H), limit = length_of(p, n), live = (limit + kChunk - 1) / kChunk;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane / 16, column = columns * 64 + wave * 16 + lane % 16;
+    const bool there = column < p.DV;
+    const int64_t cell = static_cast<int64_t>(head) * p.DK * p.DV + column;
+    f32x4 state[2 * KS];
+#pragma unroll
+    for (int d = 0; d < 2 * KS; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = 16 * d + 4 * group + r;
+            state[d][r] = p.state != nullptr && there && row < p.DK ? p.state[cell + static_cast<int64_t>(row) * p.DV] : 0.0f;
+        }
+    const T* values = static_cast<const T*>(p.v.data) + n * p.v.row + hv * p.v.head + column;
+    T* outs = static_cast<T*>(const_cast<void*>(p.out.data)) + n * p.out.row + hv * p.out.head + column;
+    T v[16];
+    const auto fetch = [&](int chunk) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int t = chunk * kChunk + 16 * (i / 4) + 4 * group + i % 4;
+            v[i] = there && t < limit ? values[t * p.v.step] : from_float<T>(0.0f);
+        }
+    };
+    Staged<T, KS, 256> k_next, q_next;
+    k_next.load(p.k, 0, limit, n, h, p.DK);
+    q_next.load(p.q, 0, limit, n, h, p.DK);
+    fetch(0);
+    for (int chunk = 0; chunk < live; ++chunk) {
+        const int64_t index = static_cast<int64_t>(head) * p.chunks + chunk;
+        uint16_t *keys = lds[chunk % BUFFERS][0], *queries = lds[chunk % BUFFERS][1];
+        if constexpr (BUFFERS == 1) __syncthreads();        // with two, the barrier of the chunk before says that the one before that is done
+        k_next.store(keys);
+        q_next.store(queries);
+        __syncthreads();
+        const uint32_t* blocks = p.blocks + index * block_words(RANKS) + lane * 4;
+        const float* vectors = p.vectors + index * 3 * kChunk + 4 * group;
+        f32x4 since[4], until[4], beta[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            since[i] = *reinterpret_cast<const f32x4*>(vectors + 16 * i);
+            until[i] = *reinterpret_cast<const f32x4*>(vectors + kChunk + 16 * i);
+            beta[i] = *reinterpret_cast<const f32x4*>(vectors + 2 * kChunk + 16 * i);
+        }
+        const float rest = p.vectors[index * 3 * kChunk + kChunk - 1];
+        Terms<3> inverse[kBlocks];
+#pragma unroll
+        for (int f = 0; f < kBlocks; ++f)
+#pragma unroll
+            for (int i = 0; i < 3; ++i) inverse[f].t[i] = *reinterpret_cast<const u32x4a*>(blocks + (f * 3 + i) * 256);
+        f32x4 right[4];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) right[i / 4][i % 4] = to_float(v[i]);
+        if (chunk + 1 < live) {
+            k_next.load(p.k, (chunk + 1) * kChunk, limit, n, h, p.DK);
+            q_next.load(p.q, (chunk + 1) * kChunk, limit, n, h, p.DK);
+            fetch(chunk + 1);
+        }
+        if constexpr (TRAIN) {
+            float* marks = p.marks + index * p.DK * p.DV + column;
+#pragma unroll
+            for (int d = 0; d < 2 * KS; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 16 * d + 4 * group + r;
+                    if (there && row < p.DK) marks[row * p.DV] = state[d][r];
+                }
+        }
+        f32x4 ks[4], out[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ks[i] = out[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const Terms<3> x = split<3>(state[2 * s], state[2 * s + 1]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                ks[i] = product<3>(Lds::rows(keys, i, s), x, ks[i]);
+                out[i] = product<RANKS>(Lds::rows(queries, i, s), x, out[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                right[i][r] -= kept(since[i][r], ks[i][r]);
+                out[i][r] = kept(since[i][r] * p.scale, out[i][r]);
+            }
+        f32x4 delta[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) delta[i] = f32x4{0, 0, 0, 0};
+        {
+            const Terms<3> x[2] = {split<3>(right[0], right[1]), split<3>(right[2], right[3])};
+#pragma unroll
+            for (int f = 0; f < kBlocks; ++f) delta[lower_tile(f)] = product<3>(inverse[f], x[lower_half(f)], delta[lower_tile(f)]);
+        }
+        if constexpr (TRAIN) {
+            float* deltas = p.deltas + index * kChunk * p.DV + column;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (there) deltas[(16 * (i / 4) + 4 * group + i % 4) * p.DV] = delta[i / 4][i % 4];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) delta[i] *= beta[i];
+        {
+            const Terms<RANKS> x[2] = {split<RANKS>(delta[0], delta[1]), split<RANKS>(delta[2], delta[3])};
+#pragma unroll
+            for (int f = 0; f < kBlocks; ++f) {
+                Terms<RANKS> scores;
+#pragma unroll
+                for (int i = 0; i < RANKS; ++i) scores.t[i] = *reinterpret_cast<const u32x4a*>(blocks + (kBlocks * 3 + f * RANKS + i) * 256);
+                out[lower_tile(f)] = product<RANKS>(scores, x[lower_half(f)], out[lower_tile(f)]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) delta[i][r] = kept(until[i][r], delta[i][r]);
+        {
+            const Terms<3> x[2] = {split<3>(delta[0], delta[1]), split<3>(delta[2], delta[3])};
+#pragma unroll
+            for (int d = 0; d < 2 * KS; ++d) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) state[d][r] = kept(rest, state[d][r]);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) state[d] = product<3>(Lds::columns(keys, d, half), x[half], state[d]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int t = chunk * kChunk + 16 * (i / 4) + 4 * group + i % 4;
+            if (there && t < p.T) outs[t * p.out.step] = from_float<T>(t < limit ? out[i / 4][i % 4] : 0.0f);
+        }
+    }
+    for (int t = live * kChunk + wave * 4 + group; t < p.T; t += 16)      // padding
+        for (int c = columns * 64 + lane % 16; c < p.DV && c < columns * 64 + 64; c += 16)
+            outs[t * p.out.step + c - column] = from_float<T>(0.0f);
+#pragma unroll
+    for (int d = 0; d < 2 * KS; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = 16 * d + 4 * group + r;
+            if (there && row < p.DK) p.state_out[cell + static_cast<int64_t>(row) * p.DV] = state[d][r];
+        }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// A few steps
+// ------------------------------------------------------------------------------------------------------------------
+// Step by step, in float32: 64 columns of the state to a workgroup, 8 rows and 4 columns to a thread. k . S and q . S are summed over the rows in one
+// exchange; out = scale (q . S + (q . k) beta delta).
+__device__ __forceinline__ float sum_of_rows(float v) {      // over the four rows of 16 lanes
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+template <typename T, int KS>
+__global__ __launch_bounds__(64 * KS) void delta_step_kernel(DeltaArgs p) {
+    __shared__ float sums[2][KS][16][9];
+    int head, columns;
+    if (!part_of_head(p.N * p.HV, (p.DV + 63) / 64, &head, &columns)) return;
+    const int n = head / p.HV, hv = head % p.HV, h = hv / (p.HV / p.H), limit = length_of(p, n);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, column = columns * 64 + 4 * (lane % 16), row = 8 * (threadIdx.x / 16);
+    const int left = p.DV - column;
+    const int64_t cell = static_cast<int64_t>(head) * p.DK * p.DV + column;
+    Raw<float, 4> state[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (p.state != nullptr && row + i < p.DK && left > 0) state[i].load(p.state + cell, static_cast<int64_t>(row + i) * p.DV, left);
+        else state[i].clear();
+    }
+    float s[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[i][c] = state[i][c];
+    const T* keys = static_cast<const T*>(p.k.data) + n * p.k.row + h * p.k.head;
+    const T* queries = static_cast<const T*>(p.q.data) + n * p.q.row + h * p.q.head;
+    const T* values = static_cast<const T*>(p.v.data) + n * p.v.row + hv * p.v.head + column;
+    T* outs = static_cast<T*>(const_cast<void*>(p.out.data)) + n * p.out.row + hv * p.out.head + column;
+    for (int t = 0; t < limit; ++t) {
+        Raw<T, 8> k, q;
+        k.clear();
+        q.clear();
+        if (row < p.DK) {
+            k.load(keys, t * p.k.step + row, p.DK - row);
+            q.load(queries, t * p.q.step + row, p.DK - row);
+        }
+        float v[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] = c < left ? to_float(values[t * p.v.step + c]) : 0.0f;
+        const float g = gate_value<T>(p.gate, p.gate_float, t, n, hv, 0.0f), b = gate_value<T>(p.beta, p.gate_float, t, n, hv, 1.0f);
+        const bool fresh = g < kForgotten || (p.starts != nullptr && p.starts[t * p.starts_step + n * p.starts_row] != 0);
+        const float a = fresh ? 0.0f : expf(g);
+        float part[9];
+#pragma unroll
+        for (int c = 0; c < 9; ++c) part[c] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            part[8] = fmaf(k[i], q[i], part[8]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                s[i][c] = kept(a, s[i][c]);
+                part[c] = fmaf(k[i], s[i][c], part[c]);
+                part[4 + c] = fmaf(q[i], s[i][c], part[4 + c]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 9; ++c) {
+            part[c] = sum_of_rows(part[c]);
+            if (lane < 16) sums[t & 1][wave][lane][c] = part[c];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < 9; ++c) {
+            part[c] = sums[t & 1][0][lane % 16][c];
+#pragma unroll
+            for (int w = 1; w < KS; ++w) part[c] += sums[t & 1][w][lane % 16][c];
+        }
+        float u[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            u[c] = b * (v[c] - part[c]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i][c] = fmaf(k[i], u[c], s[i][c]);
+        }
+        if (threadIdx.x < 16) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (c < left) outs[t * p.out.step + c] = from_float<T>(p.scale * fmaf(part[8], u[c], part[4 + c]));
+        }
+    }
+    for (int t = limit; t < p.T; ++t)
+        if (threadIdx.x < 16) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (c < left) outs[t * p.out.step + c] = from_float<T>(0.0f);
+        }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        state[i].put(0, s[i][0], s[i][1]);
+        state[i].put(2, s[i][2], s[i][3]);
+        if (row + i < p.DK && left > 0) state[i].store(p.state_out + cell, static_cast<int64_t>(row + i) * p.DV, left);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// Launch
+// ------------------------------------------------------------------------------------------------------------------
+constexpr int kFewSteps = 16;
+
+template <typename T, int KS>
+void launch_forward(const DeltaArgs& p, hipStream_t stream) {
+    const dim3 grid(head_groups(p.N * p.HV, (p.DV + 63) / 64));
+    if (p.blocks == nullptr) {
+        delta_step_kernel<T, KS><<<grid, dim3(64 * KS), 0, stream>>>(p);
+        return;
+    }
+    launch_chunks<T, KS, false>(p, stream);
+    if (p.marks != nullptr) delta_walk_kernel<T, KS, true><<<grid, dim3(256), 0, stream>>>(p);
+    else delta_walk_kernel<T, KS, false><<<grid, dim3(256), 0, stream>>>(p);
+}
+
+}  // namespace
+
+template <typename T, int KS, bool BACKWARD>
+void launch_chunks(const DeltaArgs& p, hipStream_t stream) {
+    delta_chunk_kernel<T, KS, BACKWARD><<<grid_of(static_cast<int64_t>(p.N) * p.HV * p.chunks), dim3(256), 0, stream>>>(p);
+}
+template void launch_chunks<float, 2, true>(const DeltaArgs&, hipStream_t);
+template void launch_chunks<float, 4, true>(const DeltaArgs&, hipStream_t);
+template void launch_chunks<bf16_t, 2, true>(const DeltaArgs&, hipStream_t);
+template void launch_chunks<bf16_t, 4, true>(const DeltaArgs&, hipStream_t);
+template void launch_chunks<f16_t, 2, true>(const DeltaArgs&, hipStream_t);
+template void launch_chunks<f16_t, 4, true>(const DeltaArgs&, hipStream_t);
+
+int check_delta(const char* name, const snnf_delta_rule_call* c) {
+    if (c == nullptr) return fail(SNNF_ERR_INVALID_ARGUMENT, "%s: no call", name);
+    if (c->T < 0 || c->N < 0 || c->heads < 0 || c->value_heads < 0 || c->key_size < 0 || c->value_size < 0)
+        return fail(SNNF_ERR_INVALID_ARGUMENT, "%s: T=%d N=%d heads=%d value_heads=%d key_size=%d value_size=%d", name, c->T, c->N, c->heads, c->value_heads,
+                    c->key_size, c->value_size);
+    if (!valid_dtype(c->dtype) || (c->gate_dtype != c->dtype && c->gate_dtype != SNNF_F32))
+        return fail(SNNF_ERR_INVALID_ARGUMENT, "%s: dtype codes %d and, for gates, %d", name, c->dtype, c->gate_dtype);
+    if (c->heads == 0 || c->value_heads % c->heads != 0)
+        return fail(SNNF_ERR_UNSUPPORTED, "%s: unsupported_shape: value heads (%d) must be a multiple of heads (%d)", name, c->value_heads, c->heads);
+    if (c->key_size < 1 || c->key_size > SNNF_DELTA_RULE_MAX_KEY || c->value_size < 1 || c->value_size > SNNF_DELTA_RULE_MAX_VALUE)
+        return fail(SNNF_ERR_UNSUPPORTED, "%s: unsupported_shape: keys of 1 to %d and values of 1 to %d elements, got %d and %d", name, SNNF_DELTA_RULE_MAX_KEY,
+                    SNNF_DELTA_RULE_MAX_VALUE, c->key_size, c->value_size);
+    if (c->T > (1 << 30) || static_cast<int64_t>(c->N) * c->value_heads > (1 << 20) ||
+        static_cast<int64_t>(c->N) * c->value_heads * ((c->T + kChunk - 1) / kChunk) > (1 << 30))
+        return fail(SNNF_ERR_UNSUPPORTED, "%s: unsupported_shape: at most 2^20 heads of all sequences and 2^30 steps of 64 of them, got N=%d, %d heads, T=%d", name, c->N,
+                    c->value_heads, c->T);
+    return SNNF_OK;
+}
+
+DeltaArgs delta_args(const snnf_delta_rule_call* c) {
+    const auto view = [](const snnf_heads& x) { return HeadView{x.data, x.step, x.row, x.head}; };
+    DeltaArgs p = {};
+    p.q = view(c->query), p.k = view(c->key), p.v = view(c->value), p.gate = view(c->gate), p.beta = view(c->beta);
+    p.T = c->T, p.N = c->N, p.H = c->heads, p.HV = c->value_heads, p.DK = c->key_size, p.DV = c->value_size;
+    p.chunks = (c->T + kChunk - 1) / kChunk;
+    p.scale = c->scale;
+    p.gate_float = c->gate_dtype == SNNF_F32;
+    p.starts = static_cast<const uint8_t*>(c->starts), p.starts_step = c->starts_step, p.starts_row = c->starts_row;
+    p.lengths = c->lengths;
+    p.state = c->state;
+    return p;
+}
+
+int64_t delta_chunks(const snnf_delta_rule_call* c) {
+    return static_cast<int64_t>(c->N) * c->value_heads * ((c->T + kChunk - 1) / kChunk);
+}
+
+}  // namespace snnf
+
+using namespace snnf;
+
+extern "C" size_t snnf_delta_rule_workspace_bytes(const snnf_delta_rule_call* call, int training) {
+    if (check_delta("snnf_delta_rule_workspace_bytes", call) != SNNF_OK || (!training && call->T <= kFewSteps)) return 0;
+    const int ranks = call->dtype == SNNF_F32 ? kOutputRanks<float> : kOutputRanks<bf16_t>;
+    return static_cast<size_t>(delta_chunks(call)) * (block_words(ranks) + 3 * kChunk) * 4;
+}
+
+extern "C" size_t snnf_delta_rule_marks_bytes(const snnf_delta_rule_call* call) {
+    if (check_delta("snnf_delta_rule_marks_bytes", call) != SNNF_OK) return 0;
+    return static_cast<size_t>(delta_chunks(call)) * (call->key_size + kChunk) * call->value_size * sizeof(float);
+}
+
+extern "C" int snnf_delta_rule(const snnf_delta_rule_call* call, const snnf_heads* out, float* state_out, float* marks, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+    const int rc = check_delta("snnf_delta_rule", call);
+    if (rc != SNNF_OK) return rc;
+    if (call->T == 0 || call->N == 0) return SNNF_OK;
+    if (call->query.data == nullptr || call->key.data == nullptr || call->value.data == nullptr || out == nullptr || out->data == nullptr || state_out == nullptr)
+        return fail(SNNF_ERR_INVALID_ARGUMENT, "snnf_delta_rule: query, key, value, out and state_out must be non-null");
+    DeltaArgs p = delta_args(call);
+    p.out = HeadView{out->data, out->step, out->row, out->head};
+    p.state_out = state_out;
+    const size_t need = snnf_delta_rule_workspace_bytes(call, marks != nullptr);
+    if (need > 0) {
+        if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
+            return fail(SNNF_ERR_WORKSPACE, "snnf_delta_rule: workspace of %zu bytes needed, got %zu", need, workspace_bytes);
+        p.vectors = static_cast<float*>(workspace);
+        p.blocks = reinterpret_cast<uint32_t*>(p.vectors + delta_chunks(call) * 3 * kChunk);
+    }
+    if (marks != nullptr) {
+        p.marks = marks;
+        p.deltas = marks + delta_chunks(call) * call->key_size * call->value_size;
+    }
+    hipStream_t hs = as_stream(stream);
+    const bool small = call->key_size <= 64;
+    if (call->dtype == SNNF_F32) small ? launch_forward<float, 2>(p, hs) : launch_forward<float, 4>(p, hs);
+    else if (call->dtype == SNNF_BF16) small ? launch_forward<bf16_t, 2>(p, hs) : launch_forward<bf16_t, 4>(p, hs);
+    else small ? launch_forward<f16_t, 2>(p, hs) : launch_forward<f16_t, 4>(p, hs);
+    return check_launch("snnf_delta_rule");
+}
