@@ -573,6 +573,19 @@ int snnf_delta_rule_backward(const snnf_delta_rule_call* call, const float* mark
                              const snnf_heads* dkey, const snnf_heads* dvalue, const snnf_heads* dgate, const snnf_heads* dbeta, float* dstate_in,
                              void* workspace, size_t workspace_bytes, void* stream);
 
+/* Verification of drafted tokens against the target's logits [N, K + 1, V]: requests `*_row`, places `*_step` elements apart, a row's elements next to each other.
+ *     p = softmax(logits / t), q = softmax(draft_logits / t) (draft_logits NULL: 1 at the draft); draft x stands while uniforms * q(x) < p(x)
+ *     the token behind the accepted ones: the largest r / noise, r = p behind all drafts, else max(p - q, 0), or p where that leaves nothing
+ *   temperatures  NULL (every request has `temperature`) or N; where it is not above 0: greedily, by the largest logit
+ *   drafts, uniforms [N, K], noise [N, V] with rows `noise_row` apart, lengths NULL or N (drafts of each request, clamped to 0..K)
+ *   tokens [N, K + 1]: accepted drafts, the token, then -100 (as the token where nothing of the row can be drawn);  accepted [N]
+ * K <= 64. Workspace: snnf_draft_verification_workspace_bytes(N, K, V, draft_logits != NULL) bytes, 16-byte aligned, in use until the call's work is done. Two launches. */
+size_t snnf_draft_verification_workspace_bytes(int N, int K, int V, int draft_logits);
+int snnf_draft_verification(const void* logits, int64_t logits_row, int64_t logits_step, const void* draft_logits, int64_t draft_row, int64_t draft_step, int N, int K,
+                            int V, int dtype, const int64_t* drafts, const float* uniforms, const float* noise, int64_t noise_row, const int32_t* lengths,
+                            float temperature, const float* temperatures, int64_t* tokens, int32_t* accepted, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

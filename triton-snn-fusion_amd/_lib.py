@@ -102,6 +102,8 @@ SIGNATURES = {
     "snnf_delta_rule": (_i, [_delta, _heads, _vp, _vp, _vp, _sz, _vp]),
     "snnf_delta_rule_backward_workspace_bytes": (_sz, [_delta]),
     "snnf_delta_rule_backward": (_i, [_delta, _vp, _heads, _vp, _heads, _heads, _heads, _heads, _heads, _vp, _vp, _sz, _vp]),
+    "snnf_draft_verification_workspace_bytes": (_sz, [_i] * 4),
+    "snnf_draft_verification": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _i, _i, _i, _i, _vp, _vp, _vp, _i64, _vp, _f, _vp, _vp, _vp, _vp, _sz, _vp]),
     "snnf_conv_bias": (_i, [_pp, _pp, _i, _i, _i, _i, _i, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _i64, _vp]),
 }
 

@@ -1,0 +1,443 @@
+// Verification of drafted tokens. With p = softmax(logits / temperature) of the target at a place and q that of the draft (1 at the drafted token where it has no
+// distribution), token x is accepted while u q(x) < p(x); the place behind the accepted ones gets argmax_i r_i / e_i over exponential noise e, which draws i with
+// probability r_i / sum r: r = p behind all drafts, max(p - q, 0) where one was turned down. So every token is distributed as p.
+// Two launches: (M, s) = (max x, sum exp((x - M) / temperature)) of every row, then the decisions and one more pass over the row that is drawn from. Bound by memory; few rows are
+// split over workgroups.
+// A decision is that of exact arithmetic: float32 gives each number with a bound of its error, and where two cannot be told apart (one test in some 10^5) the
+// workgroup goes over the rows again in float64.
+#include "snnf_sequence.h"
+
+namespace snnf {
+namespace {
+
+constexpr int kMostDrafts = 64;
+constexpr int kMostSplits = 64;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct VerifyArgs {
+    const void *logits, *draft_logits;
+    int64_t logits_row, logits_step, draft_row, draft_step, noise_row;      // row: of a request
+    const int64_t* drafts;
+    const float *uniforms, *noise, *temperatures;
+    const int32_t* lengths;
+    float temperature;
+    int N, K, V, rows;                  // rows of a request: K + 1 of the target, then the draft's
+    int splits, span;                   // of a row in the first launch
+    int draw_splits, draw_span;         // and in the second
+    float2* stats;                      // [request][row][split]: M, s
+    uint64_t* largest;                  // [request][row][split]: key of the largest logit
+    float4* parts;                      // [request][split]: the two largest upper bounds, the largest lower bound, index
+    uint32_t* arrived;                  // [request]
+    int64_t* tokens;
+    int32_t* accepted;
+};
+
+__device__ __forceinline__ float temperature_of(const VerifyArgs& p, int n) { return p.temperatures == nullptr ? p.temperature : p.temperatures[n]; }
+__device__ __forceinline__ int drafts_of(const VerifyArgs& p, int n) {
+    if (p.lengths == nullptr) return p.K;
+    const int length = p.lengths[n];
+    return length < 0 ? 0 : (length < p.K ? length : p.K);
+}
+template <typename T>
+__device__ __forceinline__ const T* row_of(const VerifyArgs& p, int n, int row) {
+    return row <= p.K ? static_cast<const T*>(p.logits) + n * p.logits_row + row * p.logits_step
+                      : static_cast<const T*>(p.draft_logits) + n * p.draft_row + (row - p.K - 1) * p.draft_step;
+}
+
+// What is subtracted where nothing but minus infinity has been seen.
+__device__ __forceinline__ float center(float M) { return M == -INFINITY ? 0.0f : M; }
+
+// A key orders by value, equal ones by the lower index; 0: nothing that could be drawn (minus infinity and NaN).
+__device__ __forceinline__ uint64_t key_of(float x, int index) {
+    if (!(x > -INFINITY)) return 0;
+    const uint32_t bits = __float_as_uint(x + 0.0f), order = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+    return static_cast<uint64_t>(order) << 32 | static_cast<uint32_t>(~index);
+}
+__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint64_t lane_largest(uint64_t v) {
+#pragma unroll
+    for (int mask = 32; mask > 0; mask >>= 1)
+        v = larger(v, static_cast<uint64_t>(__shfl_xor(static_cast<uint32_t>(v >> 32), mask, 64)) << 32 | __shfl_xor(static_cast<uint32_t>(v), mask, 64));
+    return v;
+}
+
+// Elements from `at` on, minus infinity behind the row's end.
+template <typename T>
+__device__ __forceinline__ void take(float (&v)[kVec<T>], const Raw<T, kVec<T>>& raw, int left) {
+#pragma unroll
+    for (int j = 0; j < kVec<T>; ++j) v[j] = left >= kVec<T> || j < left ? raw[j] : -INFINITY;
+}
+template <int VEC>
+__device__ __forceinline__ float sum_of(const float (&v)[VEC]) {        // in pairs: a thread adds few of these
+    if constexpr (VEC == 8) return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    else return (v[0] + v[1]) + (v[2] + v[3]);
+}
+
+template <typename T, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void verify_rows_kernel(VerifyArgs p) {
+    constexpr int VEC = kVec<T>, WAVES = BLOCK / 64, BATCH = 2;
+    __shared__ float maxima[WAVES], sums[WAVES];
+    __shared__ uint64_t keys[WAVES];
+    const uint32_t group = group_index();
+    const int split = group % p.splits, place = group / p.splits, row = place % p.rows, n = place / p.rows;
+    if (n >= p.N) return;
+    if (row == 0 && split == 0 && threadIdx.x == 0) p.arrived[n] = 0;
+    const int length = drafts_of(p, n);
+    const float temperature = temperature_of(p, n);
+    const bool greedy = !(temperature > 0.0f);
+    if (row <= p.K ? row > length : greedy || row - p.K - 1 >= length) return;
+    const T* x = row_of<T>(p, n, row);
+    const int begin = split * p.span, end = begin + p.span < p.V ? begin + p.span : p.V, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    Raw<T, VEC> now[BATCH], next[BATCH];
+    const auto fetch = [&](int at) {
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) next[u].load(x, at + u * BLOCK * VEC, end - at - u * BLOCK * VEC);
+    };
+    int at = begin + static_cast<int>(threadIdx.x) * VEC;
+    fetch(at);
+    if (greedy) {
+        uint64_t best = 0;
+        for (; at < end; at += BATCH * BLOCK * VEC) {
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) now[u] = next[u];
+            if (at + BATCH * BLOCK * VEC < end) fetch(at + BATCH * BLOCK * VEC);
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                float v[VEC];
+                take<T>(v, now[u], end - at - u * BLOCK * VEC);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) best = larger(best, key_of(v[j], at + u * BLOCK * VEC + j));
+            }
+        }
+        best = lane_largest(best);
+        if (lane == 0) keys[wave] = best;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < WAVES; ++w) best = larger(best, keys[w]);
+            p.largest[static_cast<int64_t>(place) * p.splits + split] = best;
+        }
+        return;
+    }
+    const float slope = kLog2e / temperature;
+    float M = -INFINITY, s = 0.0f;
+    for (; at < end; at += BATCH * BLOCK * VEC) {
+        float v[BATCH][VEC], most = M;
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) now[u] = next[u];
+        if (at + BATCH * BLOCK * VEC < end) fetch(at + BATCH * BLOCK * VEC);
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) take<T>(v[u], now[u], end - at - u * BLOCK * VEC);
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) most = fmaxf(most, v[u][j]);
+        const float c = center(most);
+        s *= __builtin_amdgcn_exp2f((M - c) * slope);
+        M = most;
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[u][j] = __builtin_amdgcn_exp2f((v[u][j] - c) * slope);
+            s += sum_of<VEC>(v[u]);
+        }
+    }
+    const float most = lane_max(M);
+    if (lane == 0) maxima[wave] = most;
+    __syncthreads();
+    const float all = lane_max(maxima[lane % WAVES], WAVES < 4 ? 4 : WAVES);
+    s = lane_sum(s * __builtin_amdgcn_exp2f((M - center(all)) * slope));
+    if (lane == 0) sums[wave] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = sums[0];
+        for (int w = 1; w < WAVES; ++w) s += sums[w];
+        p.stats[static_cast<int64_t>(place) * p.splits + split] = make_float2(all, s);
+    }
+}
+
+// Relative error of exp2(z) / s in float32: 62 or 125 additions of a thread's vectors, the exponent's roundings.
+__device__ __forceinline__ float doubt(float z) { return 1.6e-5f + 2.4e-7f * fminf(fabsf(z), 1000.0f); }
+
+// ------------------------------------------------------------------------------------------------------------------
+// In float64, by a workgroup
+// ------------------------------------------------------------------------------------------------------------------
+template <int BLOCK, typename V, typename Op>
+__device__ __forceinline__ V over_block(V v, Op op) {
+    __shared__ V shared[BLOCK];
+    __syncthreads();
+    shared[threadIdx.x] = v;
+    __syncthreads();
+    for (int half = BLOCK / 2; half > 0; half /= 2) {
+        if (static_cast<int>(threadIdx.x) < half) shared[threadIdx.x] = op(shared[threadIdx.x], shared[threadIdx.x + half]);
+        __syncthreads();
+    }
+    return shared[0];
+}
+template <typename T, int BLOCK>
+__device__ double exact_sum(const T* x, int V, float M, double temperature) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < V; i += BLOCK) s += exp((static_cast<double>(to_float(x[i])) - M) / temperature);
+    return over_block<BLOCK>(s, [](double a, double b) { return a + b; });
+}
+struct Candidate {
+    double value;
+    int index;
+};
+template <typename T, int BLOCK>
+__device__ int exact_draw(const T* x, const T* y, int taken, int V, float M, float M2, double temperature, const float* noise) {
+    const double s = exact_sum<T, BLOCK>(x, V, M, temperature), s2 = y != nullptr ? exact_sum<T, BLOCK>(y, V, M2, temperature) : 1.0;
+    for (int round = 0; round < 2; ++round) {       // where nothing is left beside the draft's share: from p
+        Candidate best{0.0, -1};
+        for (int i = threadIdx.x; i < V; i += BLOCK) {
+            double r = exp((static_cast<double>(to_float(x[i])) - M) / temperature) / s;
+            if (round == 0) r -= y != nullptr ? exp((static_cast<double>(to_float(y[i])) - M2) / temperature) / s2 : (i == taken ? 1.0 : 0.0);
+            const double v = r > 0.0 ? r / static_cast<double>(noise[i]) : 0.0;
+            if (v > best.value) best = Candidate{v, i};
+        }
+        best = over_block<BLOCK>(best, [](const Candidate& a, const Candidate& b) {
+            return b.value > a.value || (b.value == a.value && b.index >= 0 && (a.index < 0 || b.index < a.index)) ? b : a;
+        });
+        if (best.index >= 0) return best.index;
+    }
+    return -100;
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// Decisions and the draw
+// ------------------------------------------------------------------------------------------------------------------
+struct Race {                           // upper bounds of r / e: the two largest; the largest lower bound; index of the first
+    float first, second, lower;
+    int index;
+};
+__device__ __forceinline__ Race join(const Race& a, const Race& b) {
+    const bool other = b.first > a.first || (b.first == a.first && b.index < a.index);
+    const Race& w = other ? b : a;
+    return {w.first, fmaxf(w.second, other ? a.first : b.first), fmaxf(a.lower, b.lower), w.index};
+}
+__device__ __forceinline__ Race lane_race(Race v) {
+#pragma unroll
+    for (int mask = 32; mask > 0; mask >>= 1)
+        v = join(v, Race{__shfl_xor(v.first, mask, 64), __shfl_xor(v.second, mask, 64), __shfl_xor(v.lower, mask, 64), __shfl_xor(v.index, mask, 64)});
+    return v;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
+    constexpr int BLOCK = 256, VEC = kVec<T>;
+    enum { kTaken, kRefused, kDoubtful };
+    __shared__ float2 stats[2 * kMostDrafts + 1];
+    __shared__ int verdicts[kMostDrafts];
+    __shared__ uint64_t largest[kMostDrafts + 1];
+    __shared__ Race races[4];
+    __shared__ int last;
+    const uint32_t group = group_index();
+    const int split = group % p.draw_splits, n = group / p.draw_splits;
+    if (n >= p.N) return;
+    const int length = drafts_of(p, n), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const float temperature = temperature_of(p, n);
+    const bool greedy = !(temperature > 0.0f);
+    const float slope = greedy ? 0.0f : kLog2e / temperature;
+    // Statistics of the request's rows, a thread to a row.
+    for (int row = threadIdx.x; row < p.rows; row += BLOCK) {
+        if (row <= p.K ? row > length : greedy || row - p.K - 1 >= length) continue;
+        const int64_t at = (static_cast<int64_t>(n) * p.rows + row) * p.splits;
+        if (greedy) {
+            uint64_t best = p.largest[at];
+            for (int i = 1; i < p.splits; ++i) best = larger(best, p.largest[at + i]);
+            largest[row] = best;
+        } else {
+            float M = -INFINITY, s = 0.0f;
+            for (int i = 0; i < p.splits; ++i) M = fmaxf(M, p.stats[at + i].x);
+            for (int i = 0; i < p.splits; ++i) s += p.stats[at + i].y * __builtin_amdgcn_exp2f((p.stats[at + i].x - center(M)) * slope);
+            stats[row] = make_float2(M, s);
+        }
+    }
+    __syncthreads();
+    // The verdict on each draft.
+    if (static_cast<int>(threadIdx.x) < length) {
+        const int j = threadIdx.x;
+        const int64_t x = p.drafts[static_cast<int64_t>(n) * p.K + j];
+        int verdict = kRefused;
+        if (x >= 0 && x < p.V) {
+            if (greedy) {
+                verdict = largest[j] != 0 && static_cast<int64_t>(~static_cast<uint32_t>(largest[j])) == x ? kTaken : kRefused;
+            } else {
+                const float z = (to_float(row_of<T>(p, n, j)[x]) - center(stats[j].x)) * slope;
+                const float mine = __builtin_amdgcn_exp2f(z) / stats[j].y, u = p.uniforms[static_cast<int64_t>(n) * p.K + j];
+                float theirs = u, unsure = doubt(z);
+                if (p.draft_logits != nullptr) {
+                    const float2 q = stats[p.K + 1 + j];
+                    const float z2 = (to_float(row_of<T>(p, n, p.K + 1 + j)[x]) - center(q.x)) * slope;
+                    theirs *= __builtin_amdgcn_exp2f(z2) / q.y;
+                    unsure += doubt(z2);
+                }
+                verdict = theirs < mine ? kTaken : kRefused;
+                if (fabsf(theirs - mine) <= unsure * (theirs + mine)) verdict = kDoubtful;
+            }
+        }
+        verdicts[j] = verdict;
+    }
+    __syncthreads();
+    int taken = 0;
+    for (; taken < length; ++taken) {
+        int verdict = verdicts[taken];
+        if (verdict == kDoubtful) {
+            const int64_t x = p.drafts[static_cast<int64_t>(n) * p.K + taken];
+            const T *a = row_of<T>(p, n, taken), *b = p.draft_logits == nullptr ? nullptr : row_of<T>(p, n, p.K + 1 + taken);
+            const float M = stats[taken].x;
+            const double mine = exp((static_cast<double>(to_float(a[x])) - M) / temperature) / exact_sum<T, BLOCK>(a, p.V, M, temperature);
+            double theirs = p.uniforms[static_cast<int64_t>(n) * p.K + taken];
+            if (b != nullptr) {
+                const float M2 = stats[p.K + 1 + taken].x;
+                theirs *= exp((static_cast<double>(to_float(b[x])) - M2) / temperature) / exact_sum<T, BLOCK>(b, p.V, M2, temperature);
+            }
+            verdict = theirs < mine ? kTaken : kRefused;
+        }
+        if (verdict != kTaken) break;
+    }
+    int64_t token = -100;
+    if (greedy) {
+        if (split != 0) return;
+        if (largest[taken] != 0) token = static_cast<int64_t>(~static_cast<uint32_t>(largest[taken]));
+    } else {
+        const T *x = row_of<T>(p, n, taken), *y = taken < length && p.draft_logits != nullptr ? row_of<T>(p, n, p.K + 1 + taken) : nullptr;
+        const int64_t drafted = taken < length ? p.drafts[static_cast<int64_t>(n) * p.K + taken] : -1;
+        const float* noise = p.noise + n * p.noise_row;
+        const float2 a = stats[taken], b = y != nullptr ? stats[p.K + 1 + taken] : make_float2(0.0f, 1.0f);
+        const float c = center(a.x), c2 = center(b.x), part = 1.0f / a.y, part2 = 1.0f / b.y;
+        const int begin = split * p.draw_span, end = begin + p.draw_span < p.V ? begin + p.draw_span : p.V;
+        Race mine{0.0f, 0.0f, 0.0f, 0x7fffffff};
+        for (int at = begin + static_cast<int>(threadIdx.x) * VEC; at < end; at += BLOCK * VEC) {
+            Raw<T, VEC> raw, raw2;
+            Raw<float, 4> e[VEC / 4];
+            raw.load(x, at, end - at);
+            if (y != nullptr) raw2.load(y, at, end - at);
+#pragma unroll
+            for (int u = 0; u < VEC / 4; ++u) e[u].load(noise, at + 4 * u, end - at - 4 * u);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float z = (raw[j] - c) * slope, share = __builtin_amdgcn_exp2f(z) * part;
+                float r = share, unsure = share * doubt(z);
+                if (y != nullptr) {
+                    const float z2 = (raw2[j] - c2) * slope, theirs = __builtin_amdgcn_exp2f(z2) * part2;
+                    r -= theirs;
+                    unsure = share > 0.0f ? fmaf(theirs, doubt(z2), unsure) : 0.0f;
+                } else if (at + j == drafted) {
+                    r = unsure = 0.0f;                       // p is at most 1
+                }
+                const float inverse = 1.0f / e[j / 4][j % 4], upper = (r + unsure) * inverse;
+                if (at + j < end && upper > 0.0f) mine = join(mine, Race{upper, 0.0f, (r - unsure) * inverse, at + j});
+            }
+        }
+        mine = lane_race(mine);
+        if (lane == 0) races[wave] = mine;
+        __syncthreads();
+        mine = join(join(races[0], races[1]), join(races[2], races[3]));
+        if (p.draw_splits > 1) {
+            float4* parts = p.parts + static_cast<int64_t>(n) * p.draw_splits;
+            if (threadIdx.x == 0) {
+                parts[split] = make_float4(mine.first, mine.second, mine.lower, __int_as_float(mine.index));
+                last = __hip_atomic_fetch_add(p.arrived + n, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == static_cast<uint32_t>(p.draw_splits - 1);
+            }
+            __syncthreads();
+            if (!last) return;
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+            mine = Race{0.0f, 0.0f, 0.0f, 0x7fffffff};
+            if (lane < p.draw_splits) {
+                const float4 other = parts[lane];
+                mine = Race{other.x, other.y, other.z, __float_as_int(other.w)};
+            }
+            mine = lane_race(mine);
+        }
+        if (mine.first > 0.0f && mine.second < mine.lower) token = mine.index;
+        else if (a.y > 0.0f && a.y < INFINITY) token = exact_draw<T, BLOCK>(x, y, static_cast<int>(y == nullptr && drafted >= 0 && drafted < p.V ? drafted : -1), p.V, a.x, b.x, temperature, noise);
+    }
+    if (static_cast<int>(threadIdx.x) <= p.K) {
+        const int j = threadIdx.x;
+        p.tokens[static_cast<int64_t>(n) * (p.K + 1) + j] = j < taken ? p.drafts[static_cast<int64_t>(n) * p.K + j] : (j == taken ? token : -100);
+    }
+    if (threadIdx.x == 0) p.accepted[n] = taken;
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// Launch
+// ------------------------------------------------------------------------------------------------------------------
+struct VerifyShape {
+    int splits, span, draw_splits, draw_span;
+};
+void split_row(int64_t rows, int64_t wanted, int least, int V, int* splits, int* span) {
+    int64_t pieces = (wanted + rows - 1) / rows;
+    const int64_t useful = (V + least - 1) / least;
+    pieces = pieces < useful ? pieces : useful;
+    pieces = pieces < kMostSplits ? (pieces < 1 ? 1 : pieces) : kMostSplits;
+    *span = static_cast<int>(((V + pieces - 1) / pieces + 1023) / 1024 * 1024);
+    *splits = (V + *span - 1) / *span;
+}
+VerifyShape verify_shape(int64_t N, int rows, int V) {
+    VerifyShape s;
+    split_row(N * rows, compute_units() * 4, 8192, V, &s.splits, &s.span);
+    split_row(N, compute_units() * 4, 4096, V, &s.draw_splits, &s.draw_span);
+    return s;
+}
+int check_verification(const char* name, int N, int K, int V, int dtype) {
+    if (N < 0 || K < 0 || V < 1) return fail(SNNF_ERR_INVALID_ARGUMENT, "%s: N=%d K=%d V=%d", name, N, K, V);
+    if (!valid_dtype(dtype)) return fail(SNNF_ERR_INVALID_ARGUMENT, "%s: unknown dtype code %d", name, dtype);
+    if (K > kMostDrafts || N > (1 << 20) || V > (1 << 30))
+        return fail(SNNF_ERR_UNSUPPORTED, "%s: unsupported_shape: at most %d drafts of 2^20 requests and 2^30 logits, got K=%d N=%d V=%d", name, kMostDrafts, K, N, V);
+    return SNNF_OK;
+}
+size_t rounded(size_t bytes) { return (bytes + 15) / 16 * 16; }
+
+template <typename T>
+void launch_verification(const VerifyArgs& p, hipStream_t stream) {
+    verify_rows_kernel<T, 256><<<grid_of(static_cast<int64_t>(p.N) * p.rows * p.splits), dim3(256), 0, stream>>>(p);
+    verify_draw_kernel<T><<<grid_of(static_cast<int64_t>(p.N) * p.draw_splits), dim3(256), 0, stream>>>(p);
+}
+
+}  // namespace
+}  // namespace snnf
+
+using namespace snnf;
+
+extern "C" size_t snnf_draft_verification_workspace_bytes(int N, int K, int V, int draft_logits) {
+    if (check_verification("snnf_draft_verification_workspace_bytes", N, K, V, SNNF_F32) != SNNF_OK) return 0;
+    const int rows = draft_logits ? 2 * K + 1 : K + 1;
+    const VerifyShape s = verify_shape(N, rows, V);
+    const size_t pieces = static_cast<size_t>(N) * rows * s.splits;
+    return rounded(pieces * 8) + rounded(pieces * 8) + static_cast<size_t>(N) * s.draw_splits * 16 + rounded(static_cast<size_t>(N) * 4);
+}
+
+extern "C" int snnf_draft_verification(const void* logits, int64_t logits_row, int64_t logits_step, const void* draft_logits, int64_t draft_row, int64_t draft_step, int N,
+                                       int K, int V, int dtype, const int64_t* drafts, const float* uniforms, const float* noise, int64_t noise_row, const int32_t* lengths,
+                                       float temperature, const float* temperatures, int64_t* tokens, int32_t* accepted, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+    const int rc = check_verification("snnf_draft_verification", N, K, V, dtype);
+    if (rc != SNNF_OK) return rc;
+    if (N == 0) return SNNF_OK;
+    if (logits == nullptr || noise == nullptr || tokens == nullptr || accepted == nullptr || (K > 0 && (drafts == nullptr || uniforms == nullptr)))
+        return fail(SNNF_ERR_INVALID_ARGUMENT, "snnf_draft_verification: logits, drafts, uniforms, noise, tokens and accepted must be non-null");
+    if (K == 0) draft_logits = nullptr;
+    const size_t need = snnf_draft_verification_workspace_bytes(N, K, V, draft_logits != nullptr);
+    if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
+        return fail(SNNF_ERR_WORKSPACE, "snnf_draft_verification: workspace of %zu bytes needed, got %zu", need, workspace_bytes);
+    VerifyArgs p = {};
+    p.logits = logits, p.logits_row = logits_row, p.logits_step = logits_step;
+    p.draft_logits = draft_logits, p.draft_row = draft_row, p.draft_step = draft_step;
+    p.drafts = drafts, p.uniforms = uniforms, p.noise = noise, p.noise_row = noise_row;
+    p.lengths = lengths, p.temperature = temperature, p.temperatures = temperatures;
+    p.N = N, p.K = K, p.V = V, p.rows = draft_logits != nullptr ? 2 * K + 1 : K + 1;
+    const VerifyShape s = verify_shape(N, p.rows, V);
+    p.splits = s.splits, p.span = s.span, p.draw_splits = s.draw_splits, p.draw_span = s.draw_span;
+    const size_t pieces = static_cast<size_t>(N) * p.rows * s.splits;
+    char* space = static_cast<char*>(workspace);
+    p.stats = reinterpret_cast<float2*>(space);
+    p.largest = reinterpret_cast<uint64_t*>(space += rounded(pieces * 8));
+    p.parts = reinterpret_cast<float4*>(space += rounded(pieces * 8));
+    p.arrived = reinterpret_cast<uint32_t*>(space + static_cast<size_t>(N) * s.draw_splits * 16);
+    p.tokens = tokens, p.accepted = accepted;
+    hipStream_t hs = as_stream(stream);
+    if (dtype == SNNF_F32) launch_verification<float>(p, hs);
+    else if (dtype == SNNF_BF16) launch_verification<bf16_t>(p, hs);
+    else launch_verification<f16_t>(p, hs);
+    return check_launch("snnf_draft_verification");
+}
