@@ -30,6 +30,7 @@
 #include <algorithm>
 #include <array>
 #include <atomic>
+#include <cmath>
 #include <cstring>
 #include <list>
 #include <memory>
@@ -746,7 +747,7 @@ struct Args {
     PyObject* const* v;
     Py_ssize_t n;
     bool fine = true;
-    std::array<Tensor, 8> held;
+    std::array<Tensor, 12> held;
     int n_held = 0;
 
     int64_t number(Py_ssize_t i) {
@@ -1188,6 +1189,8 @@ PyObject* py_dense_pool(PyObject*, PyObject* const* args, Py_ssize_t n) { return
 PyObject* py_recurrence(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(gated_recurrence, args, n, 6); }
 PyObject* py_block_norm(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(block_norm, args, n, 10); }
 PyObject* py_scores(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(token_scores, args, n, 3); }
+PyObject* py_delta_rule(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(delta_rule, args, n, 10); }
+PyObject* py_verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(verify_drafts, args, n, 7); }
 PyObject* py_unobserved(PyObject*, PyObject* const* args, Py_ssize_t n) { return guarded(are_unobserved, args, n, n); }
 
 PyMethodDef g_fast_methods[] = {
@@ -1201,6 +1204,8 @@ PyMethodDef g_fast_methods[] = {
     {"gated_recurrence", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_recurrence)), METH_FASTCALL, nullptr},
     {"block_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_block_norm)), METH_FASTCALL, nullptr},
     {"token_scores", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_scores)), METH_FASTCALL, nullptr},
+    {"delta_rule", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_delta_rule)), METH_FASTCALL, nullptr},
+    {"verify_drafts", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_verify_drafts)), METH_FASTCALL, nullptr},
     {"unobserved", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_unobserved)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -1,4 +1,4 @@
-// The sequence operators (gated recurrence, block norm, token scores) from C++: calls on tensors that the kernels read in place, with and without
+// The sequence operators (gated recurrence, delta rule, block norm, token scores, verification of drafts) from C++: calls on tensors that the kernels read in place, with and without
 // gradients. Included by snnf_dispatch.cpp, inside its namespace.
 //
 // A training step on a small batch is bound by the host: through the Python implementations forward and backward take 130 to 170 us of it, from
@@ -350,6 +350,165 @@ PyObject* token_scores(Args& a) {
         return true;
     });
     out.resize(4);
+    return tuple_of(out);
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// Gated delta rule
+// ------------------------------------------------------------------------------------------------------------------
+inline Tensor empty_heads(const Tensor& t) {     // steps and sequences in t's order in memory
+    const int64_t T = t.size(0), N = t.size(1), inner = t.numel() / (T * N);
+    c10::SmallVector<int64_t, 4> strides(t.dim(), 1);
+    if (t.dim() == 4) strides[2] = t.size(3);
+    strides[0] = t.stride(1) > t.stride(0) ? inner : N * inner;
+    strides[1] = t.stride(1) > t.stride(0) ? T * inner : inner;
+    return at::empty_strided(t.sizes(), strides, t.options().requires_grad(false));
+}
+
+struct DeltaRule : torch::autograd::Function<DeltaRule> {
+    static snnf_heads heads(const Tensor& t) {
+        return t.defined() ? snnf_heads{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)} : snnf_heads{nullptr, 0, 0, 0};
+    }
+    static snnf_delta_rule_call call_of(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& gate, const Tensor& beta, const Tensor& starts,
+                                        const Tensor& lengths, double scale) {
+        snnf_delta_rule_call c = {};
+        c.T = static_cast<int>(q.size(0)), c.N = static_cast<int>(q.size(1)), c.heads = static_cast<int>(q.size(2)), c.value_heads = static_cast<int>(v.size(2));
+        c.key_size = static_cast<int>(q.size(3)), c.value_size = static_cast<int>(v.size(3));
+        c.dtype = code_of(q.scalar_type());
+        c.gate_dtype = gate.defined() ? code_of(gate.scalar_type()) : (beta.defined() ? code_of(beta.scalar_type()) : c.dtype);
+        c.scale = static_cast<float>(scale);
+        c.query = heads(q), c.key = heads(k), c.value = heads(v), c.gate = heads(gate), c.beta = heads(beta);
+        c.starts = data_of(starts);
+        if (starts.defined()) c.starts_step = starts.stride(0), c.starts_row = starts.stride(1);
+        c.lengths = static_cast<const int32_t*>(data_of(lengths));
+        return c;
+    }
+    static variable_list compute(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& gate, const Tensor& beta, const Tensor& state, const Tensor& starts,
+                                 const Tensor& lengths, double scale, const Tensor& state_out, Tensor* marks) {
+        const c10::DeviceGuard guard(q.device());
+        snnf_delta_rule_call c = call_of(q, k, v, gate, beta, starts, lengths, scale);
+        c.state = static_cast<const float*>(data_of(state));
+        Tensor out = empty_heads(v), last = state_out.defined() ? state_out : empty({v.size(1), v.size(2), q.size(3), v.size(3)}, at::kFloat, q);
+        if (marks) *marks = empty({static_cast<int64_t>(snnf_delta_rule_marks_bytes(&c) / 4)}, at::kFloat, q);
+        const size_t bytes = snnf_delta_rule_workspace_bytes(&c, marks != nullptr);
+        const Tensor space = bytes ? empty({static_cast<int64_t>(bytes)}, at::kByte, q) : Tensor();
+        const snnf_heads view = heads(out);
+        check_status(snnf_delta_rule(&c, &view, last.data_ptr<float>(), marks ? marks->data_ptr<float>() : nullptr, data_of(space), bytes, stream_of(q)));
+        return {std::move(out), std::move(last)};
+    }
+    static variable_list forward(AutogradContext* ctx, Tensor q, Tensor k, Tensor v, Maybe gate, Maybe beta, Maybe state, Maybe starts, Maybe lengths, double scale) {
+        const Tensor g = tensor_of(gate), b = tensor_of(beta), m = tensor_of(starts), l = tensor_of(lengths);
+        Tensor marks;
+        variable_list out = compute(q, k, v, g, b, tensor_of(state), m, l, scale, Tensor(), &marks);
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["state"] = state.has_value();
+        ctx->save_for_backward({q, k, v, g, b, m, l, marks});
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_gradients("run_hip_delta_rule", grads);
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &marks = saved[7];
+        const c10::DeviceGuard guard(q.device());
+        const snnf_delta_rule_call c = call_of(q, k, v, saved[3], saved[4], saved[5], saved[6], ctx->saved_data["scale"].toDouble());
+        Tensor dout = grads[0].defined() ? grads[0] : at::zeros({v.size(3)}, v.options().requires_grad(false)).expand(v.sizes());
+        if (!unit_rows(dout)) dout = dout.contiguous();
+        const Tensor dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+        variable_list d(9);
+        std::array<snnf_heads, 5> views;
+        for (int i = 0; i < 5; ++i) {
+            if (saved[i].defined()) d[i] = empty_heads(saved[i]);
+            views[i] = heads(d[i]);
+        }
+        d[5] = empty({v.size(1), v.size(2), q.size(3), v.size(3)}, at::kFloat, q);
+        const size_t bytes = snnf_delta_rule_backward_workspace_bytes(&c);
+        const Tensor space = empty({static_cast<int64_t>(bytes)}, at::kByte, q);
+        const snnf_heads dout_view = heads(dout);
+        check_status(snnf_delta_rule_backward(&c, marks.data_ptr<float>(), &dout_view, static_cast<const float*>(data_of(dlast)), &views[0], &views[1], &views[2], &views[3],
+                                              &views[4], d[5].data_ptr<float>(), space.data_ptr(), bytes, stream_of(q)));
+        for (int i = 0, edge = 0; i < 6; ++i) {
+            const bool there = i == 5 ? ctx->saved_data["state"].toBool() : saved[i].defined();
+            if (!there || !ctx->needs_input_grad(edge)) d[i] = Tensor();
+            edge += there;
+        }
+        return once(std::move(d));
+    }
+};
+
+// query, key, value, gate | None, beta | None, state | None, scale | None, starts | None, lengths | None, state_out | None
+PyObject* delta_rule(Args& a) {
+    const Tensor q = optional_tensor(a, 0), k = optional_tensor(a, 1), v = optional_tensor(a, 2), gate = optional_tensor(a, 3), beta = optional_tensor(a, 4);
+    const Tensor state = optional_tensor(a, 5), starts = optional_tensor(a, 7), lengths = optional_tensor(a, 8), state_out = optional_tensor(a, 9);
+    if (!a.fine || !unobserved({&q, &k, &v, &gate, &beta, &state, &starts, &lengths, &state_out}) || !activation(q) || q.dim() != 4 || !unit_rows(q)) return none();
+    if (a.v[6] != Py_None && !PyFloat_Check(a.v[6]) && !PyLong_Check(a.v[6])) return none();
+    const int64_t T = q.size(0), N = q.size(1), H = q.size(2), DK = q.size(3);
+    if (!k.defined() || !like_of(k, q, q.scalar_type()) || k.sizes() != q.sizes() || !unit_rows(k)) return none();
+    if (!v.defined() || !like_of(v, q, q.scalar_type()) || v.dim() != 4 || v.size(0) != T || v.size(1) != N || !unit_rows(v)) return none();
+    const int64_t HV = v.size(2), DV = v.size(3);
+    if (HV < 1 || HV % H != 0 || DK > SNNF_DELTA_RULE_MAX_KEY || DV < 1 || DV > SNNF_DELTA_RULE_MAX_VALUE || T > (int64_t{1} << 30) || N > (int64_t{1} << 20) ||
+        HV > (int64_t{1} << 20) || N * HV > (int64_t{1} << 20) || N * HV * ((T + 63) / 64) > (int64_t{1} << 30))
+        return none();
+    for (const Tensor* t : {&gate, &beta})
+        if (t->defined() && (t->dim() != 3 || t->size(0) != T || t->size(1) != N || t->size(2) != HV || !(like_of(*t, q, q.scalar_type()) || like_of(*t, q, at::kFloat)))) return none();
+    if (gate.defined() && beta.defined() && gate.scalar_type() != beta.scalar_type()) return none();
+    for (const Tensor* t : {&state, &state_out})
+        if (t->defined() && (!like_of(*t, q, at::kFloat) || t->dim() != 4 || t->size(0) != N || t->size(1) != HV || t->size(2) != DK || t->size(3) != DV || !t->is_contiguous()))
+            return none();
+    if (starts.defined() && (!like_of(starts, q, at::kBool) || starts.dim() != 2 || starts.size(0) != T || starts.size(1) != N)) return none();
+    if (lengths.defined() && (!like_of(lengths, q, at::kInt) || lengths.dim() != 1 || lengths.size(0) != N || !lengths.is_contiguous())) return none();
+    const bool gradient = wants_gradient({&q, &k, &v, &gate, &beta, &state});
+    if (state_out.defined()) {
+        if (gradient || state_out.requires_grad()) return none();
+        for (const Tensor* t : {&q, &k, &v, &gate, &beta, &state, &starts, &lengths})
+            if (t->defined() && t->is_alias_of(state_out) && !(t == &state && t->data_ptr() == state_out.data_ptr())) return none();
+    }
+    const double scale = a.v[6] == Py_None ? std::pow(static_cast<double>(DK), -0.5) : a.real(6);
+    if (!a.fine) return none();
+    variable_list out;
+    unlocked([&] {
+        out = gradient ? DeltaRule::apply(q, k, v, maybe(gate), maybe(beta), maybe(state), maybe(starts), maybe(lengths), scale)
+                       : DeltaRule::compute(q, k, v, gate, beta, state, starts, lengths, scale, state_out, nullptr);
+        return true;
+    });
+    return tuple_of(out);
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// Verification of drafts
+// ------------------------------------------------------------------------------------------------------------------
+// logits, drafts, uniforms, noise, draft_logits | None, temperature, lengths | None
+PyObject* verify_drafts(Args& a) {
+    const bool number = PyFloat_Check(a.v[5]) || PyLong_Check(a.v[5]);
+    const Tensor logits = optional_tensor(a, 0), drafts = optional_tensor(a, 1), uniforms = optional_tensor(a, 2), noise = optional_tensor(a, 3), theirs = optional_tensor(a, 4);
+    const Tensor each = number ? Tensor() : optional_tensor(a, 5), lengths = optional_tensor(a, 6);
+    if (!a.fine || !unobserved({&logits, &drafts, &uniforms, &noise, &theirs, &each, &lengths}) || !activation(logits) || logits.dim() != 3 || !unit_rows(logits)) return none();
+    if (!number && !each.defined()) return none();
+    const int64_t N = logits.size(0), K = logits.size(1) - 1, V = logits.size(2);
+    if (K < 1 || K > 64 || N > (int64_t{1} << 20) || V > (int64_t{1} << 30)) return none();
+    const auto rows = [&](const Tensor& t, at::ScalarType dtype) { return t.defined() && like_of(t, logits, dtype) && t.dim() == 2 && t.size(0) == N; };
+    if (!rows(drafts, at::kLong) || drafts.size(1) != K || !drafts.is_contiguous() || !rows(uniforms, at::kFloat) || uniforms.size(1) != K || !uniforms.is_contiguous()) return none();
+    if (!rows(noise, at::kFloat) || noise.size(1) != V || !unit_rows(noise)) return none();
+    if (theirs.defined() && (!like_of(theirs, logits, logits.scalar_type()) || theirs.dim() != 3 || theirs.size(0) != N || theirs.size(1) != K || theirs.size(2) != V || !unit_rows(theirs)))
+        return none();
+    if (each.defined() && (!like_of(each, logits, at::kFloat) || each.dim() != 1 || each.size(0) != N || !each.is_contiguous())) return none();
+    if (lengths.defined() && (!like_of(lengths, logits, at::kInt) || lengths.dim() != 1 || lengths.size(0) != N || !lengths.is_contiguous())) return none();
+    const double temperature = number ? a.real(5) : 1.0;
+    if (!a.fine) return none();
+    variable_list out;
+    unlocked([&] {
+        const c10::DeviceGuard guard(logits.device());
+        out = {empty({N, K + 1}, at::kLong, logits), empty({N}, at::kInt, logits)};
+        const int n = static_cast<int>(N), k = static_cast<int>(K), v = static_cast<int>(V);
+        const size_t bytes = snnf_draft_verification_workspace_bytes(n, k, v, theirs.defined());
+        const Tensor space = empty({static_cast<int64_t>(bytes)}, at::kByte, logits);
+        check_status(snnf_draft_verification(logits.data_ptr(), logits.stride(0), logits.stride(1), data_of(theirs), theirs.defined() ? theirs.stride(0) : 0,
+                                             theirs.defined() ? theirs.stride(1) : 0, n, k, v, code_of(logits.scalar_type()), drafts.data_ptr<int64_t>(),
+                                             uniforms.data_ptr<float>(), noise.data_ptr<float>(), noise.stride(0), static_cast<const int32_t*>(data_of(lengths)),
+                                             static_cast<float>(temperature), static_cast<const float*>(data_of(each)), out[0].data_ptr<int64_t>(),
+                                             out[1].data_ptr<int32_t>(), space.data_ptr(), bytes, stream_of(logits)));
+        return true;
+    });
     return tuple_of(out);
 }
 

@@ -15,7 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._sequence_common import check_activation, check_operand, check_unobserved, native, on_device_of, recorded, refuse, refuse_observed, unit_rows, unit_rows_in_place, wants_gradient, workspace
+from ._sequence_common import check_activation, check_operand, check_unobserved, native, on_device_of, recorded, refuse, refuse_observed, unit_rows, wants_gradient, workspace
 
 MAX_KEY, MAX_VALUE = 128, 1024
 OPERANDS = ("query", "key", "value", "gate", "beta", "state", "starts", "lengths", "state_out")
@@ -59,10 +59,9 @@ def check_delta_rule_support(query, key, value, gate=None, beta=None, state=None
             reasons.append("unsupported_stride: state_out must be contiguous")
         elif wants_gradient(query, key, value, gate, beta, state) or state_out.requires_grad:
             reasons.append("unsupported_gradient: state_out is for calls without gradients")
-        elif T == 0 or any(_overlap(state_out, t) and not (t is state and state.is_contiguous() and state.data_ptr() == state_out.data_ptr())
-                           for t in (query, key, value, gate, beta, state, starts, lengths) if t is not None):
-            if T:
-                reasons.append("unsupported_overlap: state_out may be the state itself and overlap nothing else that is read")
+        elif any(_overlap(state_out, t) and not (t is state and state.is_contiguous() and state.data_ptr() == state_out.data_ptr())
+                 for t in (query, key, value, gate, beta, state, starts, lengths) if t is not None):
+            reasons.append("unsupported_overlap: state_out may be the state itself and overlap nothing else that is read")
     return reasons
 
 
@@ -168,6 +167,11 @@ def run_hip_delta_rule(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
     Sums, states and decays are float32 or more, out is rounded once. Differentiable once, backwards, in query, key, value, gate, beta and state (forward
     mode, torch.func and tracing are refused); the gradients of a head's queries and keys are summed over its value heads in a fixed order.
     """
+    module = native(query)
+    if module is not None:
+        known = module.delta_rule(query, key, value, gate, beta, state, scale, starts, lengths, state_out)
+        if known is not None:
+            return known
     reasons = check_delta_rule_support(query, key, value, gate, beta, state, scale, starts, lengths, state_out)
     if reasons:
         node = recorded(run_hip_delta_rule, (query, key, value, gate, beta, state),

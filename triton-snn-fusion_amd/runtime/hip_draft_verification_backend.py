@@ -68,6 +68,11 @@ def run_hip_draft_verification(logits: torch.Tensor, drafts: torch.Tensor, unifo
     which nothing is left (masked, or not finite) lets no draft stand, and its token is -100. What a recurrent state takes of such a step is `lengths=accepted + 1`.
     Nothing is differentiable.
     """
+    module = native(logits)
+    if module is not None:
+        known = module.verify_drafts(logits, drafts, uniforms, noise, draft_logits, temperature, lengths)
+        if known is not None:
+            return DraftVerification(*known)
     reasons = check_draft_verification_support(logits, drafts, uniforms, noise, draft_logits, temperature, lengths)
     if reasons:
         node = recorded(run_hip_draft_verification, (logits, drafts, uniforms, noise), {"draft_logits": draft_logits, "temperature": temperature, "lengths": lengths})
