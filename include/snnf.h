@@ -556,12 +556,12 @@ typedef struct snnf_delta_rule_call {
 } snnf_delta_rule_call;
 
 /*   state_out  as state; may be the same memory, and overlaps it in no other way      out  overlaps no input
- *   marks      NULL, or snnf_delta_rule_marks_bytes(call) bytes that the backward pass will read
+ *   marks      NULL, or snnf_delta_rule_marks_bytes(call) bytes, 16-byte aligned, that the backward pass will read
  *   workspace  snnf_delta_rule_workspace_bytes(call, marks != NULL) bytes, 16-byte aligned (0: none needed), in use until the call's work is done
  * A gate below -104 drops the state as a start does. Two launches, one for up to 16 steps without marks. */
 size_t snnf_delta_rule_workspace_bytes(const snnf_delta_rule_call* call, int training);
 size_t snnf_delta_rule_marks_bytes(const snnf_delta_rule_call* call);
-int snnf_delta_rule(const snnf_delta_rule_call* call, const snnf_heads* out, float* state_out, float* marks, void* workspace, size_t workspace_bytes,
+int snnf_delta_rule(const snnf_delta_rule_call* call, const snnf_heads* out, float* state_out, void* marks, void* workspace, size_t workspace_bytes,
                     void* stream);
 
 /* Its gradient: `dout` and `dstate` (NULL: zeros) are the gradients of `out` and of the last state; dquery, dkey, dvalue, dgate, dbeta (data NULL: not wanted) and
@@ -569,7 +569,7 @@ int snnf_delta_rule(const snnf_delta_rule_call* call, const snnf_heads* out, flo
  * a start or its own value makes meaningless. `marks` as the forward call on the same operands left them; call->state is not read.
  * Workspace: snnf_delta_rule_backward_workspace_bytes(call) bytes, 16-byte aligned. Three launches; sums have a fixed order. */
 size_t snnf_delta_rule_backward_workspace_bytes(const snnf_delta_rule_call* call);
-int snnf_delta_rule_backward(const snnf_delta_rule_call* call, const float* marks, const snnf_heads* dout, const float* dstate, const snnf_heads* dquery,
+int snnf_delta_rule_backward(const snnf_delta_rule_call* call, const void* marks, const snnf_heads* dout, const float* dstate, const snnf_heads* dquery,
                              const snnf_heads* dkey, const snnf_heads* dvalue, const snnf_heads* dgate, const snnf_heads* dbeta, float* dstate_in,
                              void* workspace, size_t workspace_bytes, void* stream);
 

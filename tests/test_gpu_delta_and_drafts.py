@@ -165,10 +165,13 @@ def test_greedy_decoding_with_drafts_and_without(hip_ops):
     first = torch.randint(0, VOCABULARY, (N,), generator=gen(3)).to(DEV)
     state = torch.randn(N, HV, DK, DV, generator=gen(4)).to(DEV)
     none = lambda done, last: torch.zeros(N, 0, dtype=torch.long, device=DEV)
-    want, _, _, rounds = decode(p, embedding, first, state, count + 8, none, 0.0)
-    assert rounds == count + 8
+    long = 5 * count + 8                                        # as far as a request may get while the slowest one gets to `count`
+    want, _, _, rounds = decode(p, embedding, first, state, long, none, 0.0)
+    assert rounds == long
+    g = torch.Generator(device=DEV)
+    g.manual_seed(9)
     right = lambda done, last: torch.stack([want[n, int(done[n]):][:4] if int(done[n]) + 4 <= want.shape[1] else torch.zeros(4, dtype=torch.long, device=DEV) for n in range(N)])
-    half = lambda done, last: torch.where(torch.rand(N, 4, device=DEV) < 0.6, right(done, last), 7)
+    half = lambda done, last: torch.where(torch.rand(N, 4, generator=g, device=DEV) < 0.6, right(done, last), 7)
     for drafted, most in ((right, count // 4), (half, count), (lambda done, last: torch.full((N, 3), 5, device=DEV), count)):
         got, last_state, done, rounds = decode(p, embedding, first, state, count, drafted, 0.0)
         assert torch.equal(got, want[:, :count]) and rounds <= most

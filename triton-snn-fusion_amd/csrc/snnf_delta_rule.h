@@ -1,6 +1,8 @@
 // Parts of the gated delta rule's kernels: numbers as sums of bfloat16 terms for the matrix units, fragments, what forward and backward pass share.
 #pragma once
 
+#include <type_traits>
+
 #include "snnf_sequence.h"
 
 namespace snnf {
@@ -23,13 +25,20 @@ template <int N> struct Terms {
 };
 template <typename T> inline constexpr int kTerms = sizeof(T) == 4 ? 3 : (dtype_of<T>::value == SNNF_F16 ? 2 : 1);
 
+// What a term leaves comes from a dot product with (-1, 0) or (0, -1), which saves taking the pair apart (7 instructions for three terms of two numbers, 11 with shifts and
+// subtractions). The differences are exact.
 template <int N>
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&out)[N]) {
+    // (-1, 0) and (0, -1), from registers: as an inline constant of the instruction -1.0 does not mean the first
+    uint32_t lower = 0x0000bf80u, upper = 0xbf800000u;
+    asm("" : "+s"(lower), "+s"(upper));
+    const snnf_bf16x2 first = __builtin_bit_cast(snnf_bf16x2, lower), second = __builtin_bit_cast(snnf_bf16x2, upper);
     out[0] = float_to_bf16_pair(a, b);
 #pragma unroll
     for (int n = 1; n < N; ++n) {
-        a -= __uint_as_float(out[n - 1] << 16);
-        b -= __uint_as_float(out[n - 1] & 0xffff0000u);
+        const snnf_bf16x2 term = __builtin_bit_cast(snnf_bf16x2, out[n - 1]);
+        a = __builtin_amdgcn_fdot2_f32_bf16(term, first, a, false);
+        b = __builtin_amdgcn_fdot2_f32_bf16(term, second, b, false);
         out[n] = float_to_bf16_pair(a, b);
     }
 }
@@ -66,9 +75,13 @@ __device__ __forceinline__ f32x4 product(const Terms<NA>& a, const Terms<NB>& b,
     return c;
 }
 
-// Which of 32 places of a contraction group `g` holds as its element j: in order where both operands come from memory, or where one is an accumulator
-// (two tiles of 16 rows, of which a group has 4g to 4g + 3) and is multiplied where it lies, without a way through LDS.
-__device__ __forceinline__ constexpr int accumulated_place(int g, int j) { return j < 4 ? 4 * g + j : 12 + 4 * g + j; }
+// Nothing is moved across by the compiler, which would put loads off until their values are needed.
+__device__ __forceinline__ void now() { __builtin_amdgcn_sched_barrier(0); }
+
+// An accumulator multiplied next lies where the second operand of a product does: a lane has a column and, of two tiles of 16 rows, 4 (l / 16) to 4 (l / 16) + 3 each, 8 places out of 32. What they are
+// places of is up to the first operand. Over steps, a tile's rows are 16 steps, and the first operand takes its places in that order. Over a head's elements, the rows
+// of two tiles are chosen so that the places are 32 elements in order:
+__device__ __forceinline__ int head_element(int tile, int r) { return 32 * (tile / 2) + 8 * ((threadIdx.x & 63) / 16) + 4 * (tile % 2) + r; }
 
 constexpr int kChunk = 64;              // steps that are taken at once
 constexpr int kBlocks = 6;              // fragments [16 x 32] of a triangular matrix [64 x 64] that are not zero
@@ -85,7 +98,8 @@ struct DeltaArgs {
     HeadView q, k, v, gate, beta, out, dout, dq, dk, dv, dgate, dbeta;
     int T, N, H, HV, DK, DV, chunks;
     float scale;
-    int gate_float, beta_there;         // gates in float32 beside 16-bit tensors
+    int gate_float;                     // gates in float32 beside 16-bit tensors
+    int near_keys, near_values;         // whether a chunk's rows are whole vectors within reach of 31 bits
     const uint8_t* starts;
     int64_t starts_step, starts_row;
     const int32_t* lengths;
@@ -94,13 +108,29 @@ struct DeltaArgs {
     const float* dstate;
     float* dstate_in;
     // per chunk of a value head
-    uint32_t* blocks;                   // fragments of the inverse, then of the scores
-    float* vectors;                     // since, until, beta [64] each
-    float* marks;                       // state before the chunk [DK][DV]
-    float* deltas;                      // v - S k [64][DV]
-    float* later;                       // gradient of the state behind the chunk [DK][DV]
-    float* pulls;                       // gradient of beta delta's cause [64][DV]
+    uint32_t* blocks;                   // fragments of the inverse, then of the scores, then vectors
+    uint16_t* marks;                    // state before the chunk, as planes (below)
+    uint16_t* deltas;                   // v - S k, [rank][64][value columns]
+    uint16_t* later;                    // gradient of the state behind the chunk, as marks
+    uint16_t* pulls;                    // Z, as deltas
 };
+
+// Of a chunk's block: 3 terms of the inverse's fragments, `ranks` of the scores', then exp(G), exp(G_64 - G), beta [64] each, whether any of the first two is 0, and zeros.
+constexpr int kSince = 0, kUntil = kChunk, kBeta = 2 * kChunk, kBroken = 3 * kChunk, kZeros = 3 * kChunk + 4;
+__host__ __device__ __forceinline__ constexpr int block_pieces(int ranks) { return kBlocks * (3 + ranks) + 1; }      // of 256 words
+__host__ __device__ __forceinline__ constexpr int block_words(int ranks) { return block_pieces(ranks) * 256; }
+__host__ __device__ __forceinline__ constexpr int block_vectors(int ranks) { return kBlocks * (3 + ranks) * 256; }
+
+// Terms of what the output alone depends on: scores, and the state and corrections that they multiply. What the gradients of queries and keys are made of, too.
+template <typename T> inline constexpr int kOutputRanks = sizeof(T) == 4 ? 3 : 2;
+
+// What the walks leave for the gradients, as the terms of which those are products. States [rank][value column][32 KS elements of a key], value columns up to what a walk's workgroups have; the 32 bytes
+// of 16 elements lie at a place that depends on the column, so that columns read side by side from LDS come from different banks.
+__host__ __device__ __forceinline__ constexpr int padded_values(int DV) { return DV <= 64 ? 64 : (DV + 127) / 128 * 128; }
+template <int KS>
+__device__ __forceinline__ int mark_place(int column, int tile) { return (tile ^ (KS == 4 ? column & 7 : column >> 1 & 3)) * 16; }
+inline int64_t mark_elements(int ranks, int KS, int DV) { return static_cast<int64_t>(ranks) * padded_values(DV) * 32 * KS; }
+inline int64_t delta_elements(int ranks, int DV) { return static_cast<int64_t>(ranks) * kChunk * padded_values(DV); }
 
 __device__ __forceinline__ int length_of(const DeltaArgs& p, int n) {
     if (p.lengths == nullptr) return p.T;
@@ -140,42 +170,39 @@ __device__ __forceinline__ constexpr int lower_half(int f) { return f == 3 || f 
 __device__ __forceinline__ constexpr int upper_tile(int f) { return f < 2 ? 0 : (f < 4 ? 1 : f - 2); }
 __device__ __forceinline__ constexpr int upper_half(int f) { return f == 0 || f == 2 ? 0 : 1; }
 
-// Words of a chunk's fragments: 3 terms of the inverse, `ranks` of the scores.
-__host__ __device__ __forceinline__ constexpr int block_words(int ranks) { return kBlocks * (3 + ranks) * 256; }
-
 // ------------------------------------------------------------------------------------------------------------------
 // Keys and queries of a chunk in LDS
 // ------------------------------------------------------------------------------------------------------------------
-// [term][64 rows][32 KS + 8], the elements of every 32 in the order of `accumulated_place`, so that a row's 16 bytes are an operand against an accumulator over
-// the head's elements, and 4 rows x 16 elements, transposed on their way by the LDS unit, one over the steps.
+// [term][64 rows][32 KS], the 16 bytes of 8 elements at a place that depends on the row, so that 16 rows side by side are read from all banks and rows can
+// come straight from memory, past the registers.
+template <int SLOTS>                    // of 16 bytes in a row
+__device__ __forceinline__ int slot_of(int row, int slot) {
+    static_assert(SLOTS == 4 || SLOTS == 8 || SLOTS == 16, "rows of 64, 128 or 256 bytes");
+    return slot ^ (SLOTS == 16 ? row & 15 : (SLOTS == 8 ? row >> 1 & 7 : row >> 2 & 3));
+}
 template <typename T, int KS> struct Rows {
-    static constexpr int kStride = 32 * KS + 8, kPlane = kChunk * kStride, kSize = kTerms<T> * kPlane;      // in elements
-    static constexpr int kPieces = kChunk * 4 * KS;                                                    // of 8 elements
+    static constexpr int kSlots = 4 * KS, kStride = 32 * KS, kPlane = kChunk * kStride, kSize = kTerms<T> * kPlane;      // in elements
 
     __device__ __forceinline__ static void put(uint16_t* lds, int piece, const Terms<kTerms<T>>& x) {
-        const int row = piece / (4 * KS), at = piece % (4 * KS), s = at / 4, quad = 2 * (at % 4);
-        const int place = quad < 4 ? 8 * quad : 8 * (quad - 4) + 4;                                     // the next quad lies 8 further
-        uint16_t* to = lds + row * kStride + 32 * s + place;
+        const int row = piece / kSlots;
+        uint16_t* to = lds + row * kStride + 8 * slot_of<kSlots>(row, piece % kSlots);
 #pragma unroll
-        for (int n = 0; n < kTerms<T>; ++n) {
-            *reinterpret_cast<u32x2a*>(to + n * kPlane) = u32x2a{x.t[n][0], x.t[n][1]};
-            *reinterpret_cast<u32x2a*>(to + n * kPlane + 8) = u32x2a{x.t[n][2], x.t[n][3]};
-        }
+        for (int n = 0; n < kTerms<T>; ++n) *reinterpret_cast<u32x4a*>(to + n * kPlane) = x.t[n];
     }
     // rows 16 tile.., elements 32 s..
     __device__ __forceinline__ static Terms<kTerms<T>> rows(const uint16_t* lds, int tile, int s) {
-        const int lane = threadIdx.x & 63;
-        const uint16_t* from = lds + (16 * tile + lane % 16) * kStride + 32 * s + 8 * (lane / 16);
+        const int lane = threadIdx.x & 63, row = lane % 16;
+        const uint16_t* from = lds + 16 * tile * kStride + row * kStride + 8 * slot_of<kSlots>(row, 4 * s + lane / 16);
         Terms<kTerms<T>> r;
 #pragma unroll
         for (int n = 0; n < kTerms<T>; ++n) r.t[n] = *reinterpret_cast<const u32x4a*>(from + n * kPlane);
         return r;
     }
-    // elements 16 tile.. as rows, steps of half `half` as places
+    // the elements of `head_element(tile, ..)` as rows, steps of half `half` as places: four rows of 16 elements, transposed on their way by the LDS unit
     __device__ __forceinline__ static Terms<kTerms<T>> columns(const uint16_t* lds, int tile, int half) {
         typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-        const int lane = threadIdx.x & 63, l = lane % 16;
-        const uint16_t* from = lds + (32 * half + 4 * (lane / 16) + l / 4) * kStride + 32 * (tile / 2) + 8 * (l % 4) + 4 * (tile % 2);
+        const int lane = threadIdx.x & 63, row = 4 * (lane / 16) + lane % 16 / 4;
+        const uint16_t* from = lds + (32 * half + row) * kStride + 8 * slot_of<kSlots>(row, 4 * (tile / 2) + lane % 4) + 4 * (tile % 2);
         Terms<kTerms<T>> r;
 #pragma unroll
         for (int n = 0; n < kTerms<T>; ++n) {
@@ -185,10 +212,9 @@ template <typename T, int KS> struct Rows {
         }
         return r;
     }
-    // elements 16 tile + 4 (lane / 16) + 0..3 of a row
+    // elements head_element(tile, 0..3) of a row
     __device__ __forceinline__ static f32x4 four(const uint16_t* lds, int row, int tile) {
-        const int lane = threadIdx.x & 63;
-        const uint16_t* from = lds + row * kStride + 32 * (tile / 2) + 8 * (lane / 16) + 4 * (tile % 2);
+        const uint16_t* from = lds + row * kStride + 8 * slot_of<kSlots>(row, 4 * (tile / 2) + (threadIdx.x & 63) / 16) + 4 * (tile % 2);
         f32x4 r{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int n = kTerms<T> - 1; n >= 0; --n) {
@@ -200,36 +226,305 @@ template <typename T, int KS> struct Rows {
     }
 };
 
-// Pieces of a chunk's rows on their way from memory to LDS, `COUNT` to a thread of `THREADS`.
-template <typename T, int KS, int THREADS> struct Staged {
-    static constexpr int kCount = Rows<T, KS>::kPieces / THREADS;
-    Raw<T, 8> raw[kCount];
-    __device__ __forceinline__ void load(const HeadView& x, int first, int limit, int n, int head, int width) {
-        const T* base = static_cast<const T*>(x.data) + n * x.row + head * x.head;
+// 16 bytes a lane from memory to LDS, a lane's behind the one before it: `lds` is the first lane's byte address. Written out, since the compiler lets every later read of LDS wait for what it
+// knows to be on its way there; whoever reads waits (`arrived`) and passes a barrier first.
+__device__ __forceinline__ void to_lds(const void* from, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void to_lds(const void* base, uint32_t offset, uint32_t lds) {        // base: the same in all lanes
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)(p))));
+}
+// A chunk's rows of 16 bytes times SLOTS to LDS in the order of `slot_of`; zeros for rows from `rows` on and behind `width` elements, from 16 bytes of them.
+template <int SLOTS, int WAVES>
+__device__ __forceinline__ void rows_to_lds(const uint16_t* base, int64_t step, int rows, int width, const void* zeros, uint16_t* lds) {
+    constexpr int ROWS = 64 / SLOTS;    // of one instruction
+    static_assert(ROWS * WAVES % 16 == 0, "a lane's place in a row is the same in all of its rows");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = wave * ROWS + lane / SLOTS, at = 8 * slot_of<SLOTS>(row, lane % SLOTS);
+    const uint32_t to = lds_address(lds) + wave * 1024, offset = static_cast<uint32_t>(row * static_cast<int>(step) + at) * 2;
+    const bool whole = rows >= kChunk && width >= 8 * SLOTS;
 #pragma unroll
-        for (int i = 0; i < kCount; ++i) {
-            const int piece = threadIdx.x + i * THREADS, t = first + piece / (4 * KS), at = 8 * (piece % (4 * KS));
-            if (t < limit && at < width) raw[i].load(base + t * x.step, at, width - at);
-            else raw[i].clear();
+    for (int i = 0; i < kChunk / ROWS / WAVES; ++i) {
+        const uint16_t* from = base + i * WAVES * ROWS * step;
+        if (whole) {
+            to_lds(from, offset, to + i * WAVES * 1024);
+        } else {
+            const bool there = i * WAVES * ROWS + row < rows && at < width;
+            to_lds(there ? reinterpret_cast<const char*>(from) + offset : reinterpret_cast<const char*>(zeros), to + i * WAVES * 1024);
         }
     }
-    __device__ __forceinline__ void store(uint16_t* lds) const {
+}
+
+// Pieces of 8 elements of a chunk's rows on their way from memory, PER_ROW of a row, COUNT to a thread of THREADS: neighbouring threads take neighbouring pieces. Where
+// rows are whole vectors within reach a thread has one offset for all of them; else, and in the last rows of a sequence, each element is looked at.
+template <typename T, int PER_ROW, int THREADS> struct Staged {
+    static constexpr int kCount = kChunk * PER_ROW / THREADS, kRows = THREADS / PER_ROW;      // rows from one of a thread's pieces to the next
+    static_assert(THREADS % PER_ROW == 0 && kChunk % kRows == 0, "a thread's pieces lie in one column");
+    Raw<T, 8> raw[kCount];
+    // base: the chunk's first row; rows, width: how many rows and elements there are
+    __device__ __forceinline__ void load(const T* base, int64_t step, int rows, int width, bool near) {
+        const int row = threadIdx.x / PER_ROW, at = 8 * (threadIdx.x % PER_ROW);
+        if (near && rows >= kChunk) {
+            const uint32_t offset = at < width ? static_cast<uint32_t>(row * static_cast<int>(step) + at) * sizeof(T) : 0u;
 #pragma unroll
-        for (int i = 0; i < kCount; ++i) {
-            Terms<kTerms<T>> r;
-            if constexpr (dtype_of<T>::value == SNNF_BF16) {
+            for (int i = 0; i < kCount; ++i) {
+                const char* from = reinterpret_cast<const char*>(base + i * kRows * step);
+                const auto words = *reinterpret_cast<const typename Words<T, 8>::type*>(from + offset);
 #pragma unroll
-                for (int w = 0; w < 4; ++w) r.t[0][w] = raw[i].w[w];
-            } else {
-                float x[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = raw[i][j];
-                r = split<kTerms<T>>(x);
+                for (int w = 0; w < Raw<T, 8>::kWords; ++w) raw[i].w[w] = words[w];
             }
-            Rows<T, KS>::put(lds, threadIdx.x + i * THREADS, r);
+            if (width < 8 * PER_ROW) {
+#pragma unroll
+                for (int i = 0; i < kCount; ++i)
+#pragma unroll
+                    for (int w = 0; w < Raw<T, 8>::kWords; ++w) raw[i].w[w] = at < width ? raw[i].w[w] : 0u;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) {
+                if (row + i * kRows < rows && at < width) raw[i].load(base, (row + i * kRows) * step + at, width - at);
+                else raw[i].clear();
+            }
         }
     }
 };
+template <typename T, int KS, int THREADS>
+__device__ __forceinline__ void put_rows(const Staged<T, 4 * KS, THREADS>& x, uint16_t* lds) {
+#pragma unroll
+    for (int i = 0; i < x.kCount; ++i) {
+        Terms<kTerms<T>> r;
+        if constexpr (dtype_of<T>::value == SNNF_BF16) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) r.t[0][w] = x.raw[i].w[w];
+        } else {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = x.raw[i][j];
+            r = split<kTerms<T>>(v);
+        }
+        Rows<T, KS>::put(lds, threadIdx.x + i * THREADS, r);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// Values of a chunk in LDS
+// ------------------------------------------------------------------------------------------------------------------
+// [64][16 WAVES], 16-bit elements as above, float32 ones with a pitch of their own. A wave reads its 16 columns in the accumulators' layout and, once it has them, uses the room to
+// turn what it writes into rows.
+template <typename T, int WAVES> struct Tile {
+    static constexpr int kColumns = 16 * WAVES, kSlots = 2 * WAVES, kStride = sizeof(T) == 4 ? kColumns + 8 : kColumns, kSize = kChunk * kStride;
+    // byte address of a column's 16-bit (32-bit: its) element within the wave's 16
+    template <typename E>
+    __device__ __forceinline__ static uint32_t place(int row, int column) {
+        const int wave = threadIdx.x >> 6;
+        if constexpr (sizeof(T) == 4) return (row * kStride + 16 * wave) * 4 + column * sizeof(E);
+        else return row * kStride * 2 + 16 * slot_of<kSlots>(row, 2 * wave + column / 8) + 2 * (column % 8);
+    }
+    __device__ __forceinline__ static void put(T* lds, const Staged<T, 2 * WAVES, 64 * WAVES>& x) {
+#pragma unroll
+        for (int i = 0; i < x.kCount; ++i) {
+            const int row = threadIdx.x / kSlots + i * x.kRows, slot = threadIdx.x % kSlots;
+            T* to = lds + row * kStride + 8 * (sizeof(T) == 4 ? slot : slot_of<kSlots>(row, slot));
+#pragma unroll
+            for (int w = 0; w < Raw<T, 8>::kWords; w += 4)
+                reinterpret_cast<u32x4a*>(to)[w / 4] = u32x4a{x.raw[i].w[w], x.raw[i].w[w + 1], x.raw[i].w[w + 2], x.raw[i].w[w + 3]};
+        }
+    }
+    // rows 16 i + 4 (lane / 16) + 0..3 of the lane's column
+    __device__ __forceinline__ static f32x4 get(const T* lds, int i) {
+        const int lane = threadIdx.x & 63, l = lane % 16, row = 4 * (lane / 16);
+        f32x4 r;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(lds) + place<float>(16 * i + row + j, l));
+        } else {
+            typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+            const char* from = reinterpret_cast<const char*>(lds) + place<T>(row + l / 4, 4 * (l % 4)) + 16 * i * kStride * 2;
+            const u32x2a words = __builtin_bit_cast(u32x2a, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(from)));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = element<T>(words[j / 2], j % 2);
+        }
+        return r;
+    }
+    // The wave's 16 columns of x as E, in the room of 16 columns of T.
+    template <typename E>
+    __device__ __forceinline__ static void turn(T* lds, const E (&x)[16]) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            *reinterpret_cast<E*>(reinterpret_cast<char*>(lds) + place<E>(4 * (lane / 16) + i % 4, lane % 16) + 16 * (i / 4) * kStride * sizeof(T)) = x[i];
+    }
+    // 16 bytes of them: piece `lane + 64 i` of row (...) / pieces a row
+    template <typename E>
+    __device__ __forceinline__ static u32x4a piece(const T* lds, int i, int* row, int* at) {
+        constexpr int EACH = 16 / sizeof(E), PER_ROW = 16 / EACH;
+        const int lane = threadIdx.x & 63, index = lane + 64 * i;
+        *row = index / PER_ROW, *at = EACH * (index % PER_ROW);
+        return *reinterpret_cast<const u32x4a*>(reinterpret_cast<const char*>(lds) + place<E>(*row, *at));
+    }
+    // The wave's 16 columns into its room...
+    __device__ __forceinline__ static void turn_values(T* lds, const f32x4 (&x)[4]) {
+        T y[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y[i] = from_float<T>(x[i / 4][i % 4]);
+        turn<T>(lds, y);
+    }
+    // ... and from there to rows of memory; `rows` are written, those from `live` on as zeros.
+    __device__ __forceinline__ static void write(const T* lds, T* base, int64_t step, int rows, int live, int width, bool near) {
+        __builtin_amdgcn_wave_barrier();
+        constexpr int EACH = 16 / sizeof(T), COUNT = kChunk / 64 * 16 / EACH;
+        const bool whole = near && live >= kChunk && width >= 16;
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            int row, at;
+            const u32x4a words = piece<T>(lds, i, &row, &at);
+            if (whole) {
+                *reinterpret_cast<typename Words<T, kVec<T>>::type*>(reinterpret_cast<char*>(base) + static_cast<uint32_t>(row * static_cast<int>(step) + at) * sizeof(T)) = words;
+            } else if (row < rows) {
+                T* to = base + row * step + at;
+#pragma unroll
+                for (int j = 0; j < EACH; ++j) {
+                    const uint32_t word = row < live ? words[j * sizeof(T) / 4] : 0u;
+                    if (at + j >= width) continue;
+                    if constexpr (sizeof(T) == 4) to[j] = __uint_as_float(word);
+                    else to[j].bits = static_cast<uint16_t>(j % 2 ? word >> 16 : word);
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    // The terms of the wave's 16 columns to planes [rank][64][columns].
+    template <int RANKS>
+    __device__ __forceinline__ static void write_terms(T* lds, const f32x4 (&x)[4], uint16_t* base, int columns) {
+        uint32_t words[8][RANKS];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) split_pair<RANKS>(x[i / 2][2 * (i % 2)], x[i / 2][2 * (i % 2) + 1], words[i]);
+#pragma unroll
+        for (int n = 0; n < RANKS; ++n) {
+            uint16_t y[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] = static_cast<uint16_t>(i % 2 ? words[i / 2][n] >> 16 : words[i / 2][n]);
+            turn<uint16_t>(lds, y);
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                int row, at;
+                const u32x4a piece16 = piece<uint16_t>(lds, i, &row, &at);
+                *reinterpret_cast<u32x4a*>(base + static_cast<uint32_t>((n * kChunk + row) * columns + at)) = piece16;
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+};
+
+// A chunk's block on its way to LDS.
+template <int PIECES, int WAVES> struct StagedBlock {
+    static constexpr int kCount = (PIECES + WAVES - 1) / WAVES;
+    u32x4a words[kCount];
+    __device__ __forceinline__ void load(const uint32_t* from) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (int i = 0; i < kCount; ++i)
+            if (wave + i * WAVES < PIECES) words[i] = *reinterpret_cast<const u32x4a*>(from + (wave + i * WAVES) * 256 + lane * 4);
+    }
+    __device__ __forceinline__ void store(uint32_t* lds) const {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (int i = 0; i < kCount; ++i)
+            if (wave + i * WAVES < PIECES) *reinterpret_cast<u32x4a*>(lds + (wave + i * WAVES) * 256 + lane * 4) = words[i];
+    }
+};
+// What a walk reads of a chunk: keys, queries, values (or the gradient of what is read) and the chunk's block; through registers...
+template <typename T, int KS, int WAVES, int PIECES> struct StagedChunk {
+    Staged<T, 4 * KS, 64 * WAVES> k, q;
+    Staged<T, 2 * WAVES, 64 * WAVES> v;
+    StagedBlock<PIECES, WAVES> block;
+    __device__ __forceinline__ void load(const DeltaArgs& p, const T* keys, const T* queries, const T* values, int64_t step, int rows, int width, const uint32_t* from) {
+        k.load(keys, p.k.step, rows, p.DK, p.near_keys);
+        q.load(queries, p.q.step, rows, p.DK, p.near_keys);
+        v.load(values, step, rows, width, p.near_values);
+        block.load(from);
+    }
+    __device__ __forceinline__ void store(uint16_t* keys, uint16_t* queries, T* tile, uint32_t* to) const {
+        put_rows<T, KS, 64 * WAVES>(k, keys);
+        put_rows<T, KS, 64 * WAVES>(q, queries);
+        Tile<T, WAVES>::put(tile, v);
+        block.store(to);
+    }
+};
+// ... or, with one term to an element, as they are, a chunk ahead into the other buffer: past the registers where rows are whole vectors, else through them at once.
+template <typename T, int KS, int WAVES, int PIECES> struct ChunkReader {
+    static constexpr bool kDirect = kTerms<T> == 1;
+    static constexpr int kBuffers = kDirect ? 2 : 1;
+    struct Buffers {
+        uint16_t keys[Rows<T, KS>::kSize], queries[Rows<T, KS>::kSize];
+        T tile[Tile<T, WAVES>::kSize];
+        uint32_t block[PIECES * 256];
+    };
+    struct Nothing {};
+    std::conditional_t<kDirect, Nothing, StagedChunk<T, KS, WAVES, PIECES>> next;
+
+    __device__ __forceinline__ void fetch(const DeltaArgs& p, const T* keys, const T* queries, const T* values, int64_t step, int rows, int width, const uint32_t* block, Buffers& to) {
+        if constexpr (!kDirect) {
+            next.load(p, keys, queries, values, step, rows, width, block);
+        } else {
+            const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+            const uint32_t* zeros = block + block_vectors((PIECES - 1) / kBlocks - 3) + kZeros;
+            if (p.near_keys) {
+                rows_to_lds<4 * KS, WAVES>(reinterpret_cast<const uint16_t*>(keys), p.k.step, rows, p.DK, zeros, to.keys);
+                rows_to_lds<4 * KS, WAVES>(reinterpret_cast<const uint16_t*>(queries), p.q.step, rows, p.DK, zeros, to.queries);
+            } else {
+                Staged<T, 4 * KS, 64 * WAVES> x;
+                x.load(keys, p.k.step, rows, p.DK, false);
+                put_rows<T, KS, 64 * WAVES>(x, to.keys);
+                x.load(queries, p.q.step, rows, p.DK, false);
+                put_rows<T, KS, 64 * WAVES>(x, to.queries);
+            }
+            if (p.near_values) {
+                rows_to_lds<2 * WAVES, WAVES>(reinterpret_cast<const uint16_t*>(values), step, rows, width, zeros, reinterpret_cast<uint16_t*>(to.tile));
+            } else {
+                Staged<T, 2 * WAVES, 64 * WAVES> x;
+                x.load(values, step, rows, width, false);
+                Tile<T, WAVES>::put(to.tile, x);
+            }
+            const uint32_t at = lds_address(to.block) + wave * 1024;
+#pragma unroll
+            for (int i = 0; i < (PIECES + WAVES - 1) / WAVES; ++i)
+                if (wave + i * WAVES < PIECES) to_lds(block + (wave + i * WAVES) * 256, lane * 16u, at + i * WAVES * 1024);
+        }
+    }
+    // Has the chunk that was fetched last in LDS, for all waves; the one before it may be overwritten from then on.
+    __device__ __forceinline__ void wait(Buffers& to) {
+        if constexpr (kDirect) {
+            arrived();
+            __syncthreads();
+        } else {
+            __syncthreads();
+            next.store(to.keys, to.queries, to.tile, to.block);
+            __syncthreads();
+        }
+    }
+};
+template <int N>
+__device__ __forceinline__ Terms<N> block_terms(const uint32_t* lds, int fragment) {
+    Terms<N> r;
+#pragma unroll
+    for (int n = 0; n < N; ++n) r.t[n] = *reinterpret_cast<const u32x4a*>(lds + (fragment * N + n) * 256 + (threadIdx.x & 63) * 4);
+    return r;
+}
+// Of a vector of a chunk: rows 16 i + 4 (lane / 16) + 0..3
+__device__ __forceinline__ f32x4 row_factors(const uint32_t* vectors, int which, int i) {
+    return *reinterpret_cast<const f32x4*>(vectors + which + 16 * i + 4 * ((threadIdx.x & 63) / 16));
+}
+// What a vanished decay would multiply is dropped, infinities and NaN as well.
+__device__ __forceinline__ void drop(f32x4& x, const f32x4& factor) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = factor[r] == 0.0f ? 0.0f : x[r];
+}
 
 // Gates: of the activations' type or float32; none: no decay, every step learnt in full.
 template <typename T>
@@ -266,10 +561,16 @@ inline unsigned head_groups(int heads, int parts) { return static_cast<unsigned>
 // Fragments, decays and inverses of all chunks; transposed for the backward pass.
 template <typename T, int KS, bool BACKWARD> void launch_chunks(const DeltaArgs& p, hipStream_t stream);
 
-// Terms of what the output alone depends on: scores, and the state and corrections that they multiply.
-template <typename T> inline constexpr int kOutputRanks = sizeof(T) == 4 ? 3 : 2;
-
 int check_delta(const char* name, const snnf_delta_rule_call* call);
 DeltaArgs delta_args(const snnf_delta_rule_call* call);
 int64_t delta_chunks(const snnf_delta_rule_call* call);
+int delta_ranks(const snnf_delta_rule_call* call);
+int64_t delta_mark_elements(const snnf_delta_rule_call* call);
+// Whether a chunk's rows lie within reach of 31-bit offsets, and, where they go to LDS as they are, on 16 bytes.
+inline bool near_by(const HeadView& x, int dtype, bool read) {
+    const bool reach = x.step >= 0 && x.step <= 0x7fffffff / (kChunk * dtype_size(dtype)) - 1024;
+    return reach && (!read || dtype != SNNF_BF16 || (aligned_to(x.data, 16) && (x.step | x.row | x.head) % 8 == 0));
+}
+// Eight waves share a head's keys in LDS where heads alone fill the chip, else four.
+inline bool eight_waves(const DeltaArgs& p) { return p.DV > 64 && p.N * p.HV >= compute_units(); }
 }  // namespace snnf

@@ -38,7 +38,8 @@ __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(DeltaArgs p) {
     const int first = chunk * kChunk, limit = length_of(p, n);
     if (first >= limit) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane / 16, column = lane % 16;
-    float* vectors = p.vectors + static_cast<int64_t>(index) * 3 * kChunk;
+    uint32_t* blocks = p.blocks + static_cast<int64_t>(index) * block_words(RANKS);
+    float* vectors = reinterpret_cast<float*>(blocks + block_vectors(RANKS));
 
     if (wave == 0) {
         const int t = first + lane;
@@ -56,9 +57,12 @@ __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(DeltaArgs p) {
         total[lane] = sum, part[lane] = mine, beta[lane] = b;
         const double all = __shfl(sum, 63, 64);
         const int last = __shfl(mine, 63, 64);
-        vectors[lane] = mine == 0 ? decay_of(sum) : 0.0f;
-        vectors[kChunk + lane] = mine == last ? decay_of(all - sum) : 0.0f;
-        vectors[2 * kChunk + lane] = b;
+        const float since = mine == 0 ? decay_of(sum) : 0.0f, until = mine == last ? decay_of(all - sum) : 0.0f;
+        vectors[kSince + lane] = since;
+        vectors[kUntil + lane] = until;
+        vectors[kBeta + lane] = b;
+        const bool broken = __ballot(since == 0.0f || until == 0.0f) != 0;
+        vectors[kBroken + lane] = broken && lane == 0 ? 1.0f : 0.0f;
     }
     const T* keys = static_cast<const T*>(p.k.data) + n * p.k.row + h * p.k.head;
     const T* queries = static_cast<const T*>(p.q.data) + n * p.q.row + h * p.q.head;
@@ -132,7 +136,6 @@ __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(DeltaArgs p) {
         __syncthreads();
     }
     // Fragments as the other kernels load them.
-    uint32_t* blocks = p.blocks + static_cast<int64_t>(index) * block_words(RANKS);
     const auto fragment = [&](const float* m, int f) {
         if constexpr (BACKWARD) {
             const float* from = m + (32 * upper_half(f) + 4 * group) * kPitch + 16 * upper_tile(f) + column;
@@ -158,16 +161,19 @@ __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(DeltaArgs p) {
 // The walk over the chunks
 // ------------------------------------------------------------------------------------------------------------------
 // A wave owns 16 columns of the state, in accumulators, and of everything that is multiplied from it on: products go over the heads' elements
-// or over steps, whose place in an accumulator is a matter of the other operand's order, so that nothing but keys and queries passes through LDS.
-template <typename T, int KS, bool TRAIN>
-__global__ __launch_bounds__(256, 1) void delta_walk_kernel(DeltaArgs p) {
+// or over steps, whose place in an accumulator is a matter of the other operand's order, so that nothing but keys, queries and what crosses the kernel's edge passes through LDS.
+template <typename T, int KS, int WAVES, bool TRAIN>
+__global__ __launch_bounds__(kTerms<T> == 1 && !TRAIN ? 512 : 64 * WAVES) void delta_walk_kernel(DeltaArgs p) {
     using Lds = Rows<T, KS>;
-    constexpr int RANKS = kOutputRanks<T>, BUFFERS = kTerms<T> == 1 ? 2 : 1;
-    __shared__ uint16_t lds[BUFFERS][2][Lds::kSize];
+    using Values = Tile<T, WAVES>;
+    constexpr int RANKS = kOutputRanks<T>, TERMS = kTerms<T>, PIPE = TERMS == 1 ? 2 : 1;
+    using Reader = ChunkReader<T, KS, WAVES, block_pieces(RANKS)>;
+    __shared__ alignas(16) typename Reader::Buffers lds[Reader::kBuffers];
     int head, columns;
-    if (!part_of_head(p.N * p.HV, (p.DV + 63) / 64, &head, &columns)) return;
+    if (!part_of_head(p.N * p.HV, (p.DV + Values::kColumns - 1) / Values::kColumns, &head, &columns)) return;
     const int n = head / p.HV, hv = head % p.HV, h = hv / (p.HV / p.H), limit = length_of(p, n), live = (limit + kChunk - 1) / kChunk;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane / 16, column = columns * 64 + wave * 16 + lane % 16;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane / 16;
+    const int left = columns * Values::kColumns, mine = left + 16 * wave, column = mine + lane % 16;
     const bool there = column < p.DV;
     const int64_t cell = static_cast<int64_t>(head) * p.DK * p.DV + column;
     f32x4 state[2 * KS];
@@ -175,136 +181,171 @@ __global__ __launch_bounds__(256, 1) void delta_walk_kernel(DeltaArgs p) {
     for (int d = 0; d < 2 * KS; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = 16 * d + 4 * group + r;
+            const int row = head_element(d, r);
             state[d][r] = p.state != nullptr && there && row < p.DK ? p.state[cell + static_cast<int64_t>(row) * p.DV] : 0.0f;
         }
-    const T* values = static_cast<const T*>(p.v.data) + n * p.v.row + hv * p.v.head + column;
-    T* outs = static_cast<T*>(const_cast<void*>(p.out.data)) + n * p.out.row + hv * p.out.head + column;
-    T v[16];
+    const T* k_base = static_cast<const T*>(p.k.data) + n * p.k.row + h * p.k.head;
+    const T* q_base = static_cast<const T*>(p.q.data) + n * p.q.row + h * p.q.head;
+    const T* v_base = static_cast<const T*>(p.v.data) + n * p.v.row + hv * p.v.head + left;
+    T* out_base = static_cast<T*>(const_cast<void*>(p.out.data)) + n * p.out.row + hv * p.out.head + mine;
+    Reader reader;
     const auto fetch = [&](int chunk) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int t = chunk * kChunk + 16 * (i / 4) + 4 * group + i % 4;
-            v[i] = there && t < limit ? values[t * p.v.step] : from_float<T>(0.0f);
-        }
+        const int64_t first = static_cast<int64_t>(chunk) * kChunk;
+        if (chunk < live) reader.fetch(p, k_base + first * p.k.step, q_base + first * p.q.step, v_base + first * p.v.step, p.v.step, limit - chunk * kChunk, p.DV - left,
+                     p.blocks + (static_cast<int64_t>(head) * p.chunks + chunk) * block_words(RANKS), lds[chunk % Reader::kBuffers]);
     };
-    Staged<T, KS, 256> k_next, q_next;
-    k_next.load(p.k, 0, limit, n, h, p.DK);
-    q_next.load(p.q, 0, limit, n, h, p.DK);
     fetch(0);
     for (int chunk = 0; chunk < live; ++chunk) {
         const int64_t index = static_cast<int64_t>(head) * p.chunks + chunk;
-        uint16_t *keys = lds[chunk % BUFFERS][0], *queries = lds[chunk % BUFFERS][1];
-        if constexpr (BUFFERS == 1) __syncthreads();        // with two, the barrier of the chunk before says that the one before that is done
-        k_next.store(keys);
-        q_next.store(queries);
-        __syncthreads();
-        const uint32_t* blocks = p.blocks + index * block_words(RANKS) + lane * 4;
-        const float* vectors = p.vectors + index * 3 * kChunk + 4 * group;
-        f32x4 since[4], until[4], beta[4];
+        typename Reader::Buffers& here = lds[chunk % Reader::kBuffers];
+        const uint16_t *keys = here.keys, *queries = here.queries;
+        T* tile = here.tile;
+        const uint32_t *block = here.block, *vectors = block + block_vectors(RANKS);
+        reader.wait(here);
+        fetch(chunk + 1);
+        now();
+        // S k and S q, the state's terms a step ahead of the products that take them
+        f32x4 ks[4], out[4], right[4], delta[4], since[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            since[i] = *reinterpret_cast<const f32x4*>(vectors + 16 * i);
-            until[i] = *reinterpret_cast<const f32x4*>(vectors + kChunk + 16 * i);
-            beta[i] = *reinterpret_cast<const f32x4*>(vectors + 2 * kChunk + 16 * i);
-        }
-        const float rest = p.vectors[index * 3 * kChunk + kChunk - 1];
-        Terms<3> inverse[kBlocks];
+        for (int i = 0; i < 4; ++i) ks[i] = out[i] = delta[i] = f32x4{0, 0, 0, 0};
+        Terms<TERMS> a[PIPE][8];
+        Terms<3> x[2] = {split<3>(state[0], state[1]), {}}, inverse[kBlocks];
+        const auto load = [&](int s) {
 #pragma unroll
-        for (int f = 0; f < kBlocks; ++f)
-#pragma unroll
-            for (int i = 0; i < 3; ++i) inverse[f].t[i] = *reinterpret_cast<const u32x4a*>(blocks + (f * 3 + i) * 256);
-        f32x4 right[4];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) right[i / 4][i % 4] = to_float(v[i]);
-        if (chunk + 1 < live) {
-            k_next.load(p.k, (chunk + 1) * kChunk, limit, n, h, p.DK);
-            q_next.load(p.q, (chunk + 1) * kChunk, limit, n, h, p.DK);
-            fetch(chunk + 1);
-        }
-        if constexpr (TRAIN) {
-            float* marks = p.marks + index * p.DK * p.DV + column;
-#pragma unroll
-            for (int d = 0; d < 2 * KS; ++d)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * d + 4 * group + r;
-                    if (there && row < p.DK) marks[row * p.DV] = state[d][r];
-                }
-        }
-        f32x4 ks[4], out[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ks[i] = out[i] = f32x4{0, 0, 0, 0};
+            for (int i = 0; i < 4; ++i) a[s % PIPE][i] = Lds::rows(keys, i, s), a[s % PIPE][4 + i] = Lds::rows(queries, i, s);
+        };
+        load(0);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            const Terms<3> x = split<3>(state[2 * s], state[2 * s + 1]);
+            now();
+            if (PIPE == 2 && s + 1 < KS) load(s + 1);
+            if (s + 1 < KS) x[(s + 1) % 2] = split<3>(state[2 * s + 2], state[2 * s + 3]);
+            if (s + 1 == KS) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) right[i] = Values::get(tile, i), since[i] = row_factors(vectors, kSince, i);
+                if constexpr (PIPE == 2) {
+#pragma unroll
+                    for (int f = 0; f < 2; ++f) inverse[f] = block_terms<3>(block, f);
+                }
+            }
+#pragma unroll
+            for (int rank = 2; rank >= 0; --rank)
+#pragma unroll
+                for (int j = 0; j <= rank; ++j)
+                    if (j < TERMS) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) ks[i] = mfma(a[s % PIPE][i].t[j], x[s % 2].t[rank - j], ks[i]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (rank < RANKS) out[i] = mfma(a[s % PIPE][4 + i].t[j], x[s % 2].t[rank - j], out[i]);
+                    }
+            if constexpr (TRAIN) {
+                uint16_t* marks = p.marks + index * (RANKS * padded_values(p.DV) * 32 * KS);
+#pragma unroll
+                for (int r = 0; r < RANKS; ++r)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+                        *reinterpret_cast<u32x2a*>(marks + static_cast<uint32_t>((r * padded_values(p.DV) + column) * 32 * KS + mark_place<KS>(column, 2 * s + half) + 4 * group)) =
+                            u32x2a{x[s % 2].t[r][2 * half], x[s % 2].t[r][2 * half + 1]};
+            }
+            if (PIPE == 1 && s + 1 < KS) load(s + 1);
+        }
+        const bool broken = __builtin_amdgcn_readfirstlane(vectors[kBroken]) != 0;
+        const float rest = __uint_as_float(__builtin_amdgcn_readfirstlane(vectors[kSince + kChunk - 1]));
+        if (broken) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) drop(ks[i], since[i]), drop(out[i], since[i]);
+#pragma unroll
+            for (int d = 0; d < 2 * KS; ++d) drop(state[d], f32x4{rest, rest, rest, rest});
+        }
+        // delta
+        now();
+        Terms<RANKS> scores[kBlocks];
+        f32x4 beta[4];
+        {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) right[i] -= since[i] * ks[i];
+#pragma unroll
+            for (int f = PIPE == 2 ? 2 : 0; f < kBlocks; ++f) inverse[f] = block_terms<3>(block, f);
+            const Terms<3> y[2] = {split<3>(right[0], right[1]), split<3>(right[2], right[3])};
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int rank = 2; rank >= 0; --rank)
+#pragma unroll
+                    for (int j = 0; j <= rank; ++j)
+#pragma unroll
+                        for (int f = 0; f < kBlocks; ++f)
+                            if (lower_half(f) == half) delta[lower_tile(f)] = mfma(inverse[f].t[j], y[half].t[rank - j], delta[lower_tile(f)]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[i] *= since[i] * p.scale, beta[i] = row_factors(vectors, kBeta, i);
+#pragma unroll
+            for (int d = 0; d < 2 * KS; ++d) state[d] *= rest;
+#pragma unroll
+            for (int f = 0; f < kBlocks; ++f) scores[f] = block_terms<RANKS>(block + kBlocks * 3 * 256, f);
+        }
+        if constexpr (TRAIN) Values::template write_terms<RANKS>(tile, delta, p.deltas + index * (RANKS * kChunk * padded_values(p.DV)) + mine, padded_values(p.DV));
+        // What the steps read of each other, and the state behind them
+        f32x4 until[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) until[i] = row_factors(vectors, kUntil, i), delta[i] *= beta[i];
+        if (broken) {
+            f32x4 left_over[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                ks[i] = product<3>(Lds::rows(keys, i, s), x, ks[i]);
-                out[i] = product<RANKS>(Lds::rows(queries, i, s), x, out[i]);
+                left_over[i] = delta[i];
+                drop(left_over[i], until[i]);
+                right[i] = left_over[i];
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) right[i] = delta[i];
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                right[i][r] -= kept(since[i][r], ks[i][r]);
-                out[i][r] = kept(since[i][r] * p.scale, out[i][r]);
-            }
-        f32x4 delta[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) delta[i] = f32x4{0, 0, 0, 0};
+        now();
         {
-            const Terms<3> x[2] = {split<3>(right[0], right[1]), split<3>(right[2], right[3])};
+            Terms<TERMS> k[PIPE][2 * KS];
+            const auto columns_of = [&](int half) {
 #pragma unroll
-            for (int f = 0; f < kBlocks; ++f) delta[lower_tile(f)] = product<3>(inverse[f], x[lower_half(f)], delta[lower_tile(f)]);
-        }
-        if constexpr (TRAIN) {
-            float* deltas = p.deltas + index * kChunk * p.DV + column;
+                for (int d = 0; d < 2 * KS; ++d) k[half % PIPE][d] = Lds::columns(keys, d, half);
+            };
+            columns_of(0);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (there) deltas[(16 * (i / 4) + 4 * group + i % 4) * p.DV] = delta[i / 4][i % 4];
-        }
+            for (int half = 0; half < 2; ++half) {
+                const Terms<RANKS> y = split<RANKS>(delta[2 * half], delta[2 * half + 1]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) delta[i] *= beta[i];
-        {
-            const Terms<RANKS> x[2] = {split<RANKS>(delta[0], delta[1]), split<RANKS>(delta[2], delta[3])};
+                for (int rank = RANKS - 1; rank >= 0; --rank)
 #pragma unroll
-            for (int f = 0; f < kBlocks; ++f) {
-                Terms<RANKS> scores;
+                    for (int j = 0; j <= rank; ++j)
 #pragma unroll
-                for (int i = 0; i < RANKS; ++i) scores.t[i] = *reinterpret_cast<const u32x4a*>(blocks + (kBlocks * 3 + f * RANKS + i) * 256);
-                out[lower_tile(f)] = product<RANKS>(scores, x[lower_half(f)], out[lower_tile(f)]);
+                        for (int f = 0; f < kBlocks; ++f)
+                            if (lower_half(f) == half) out[lower_tile(f)] = mfma(scores[f].t[j], y.t[rank - j], out[lower_tile(f)]);
             }
-        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+            for (int half = 0; half < 2; ++half) {
+                if (PIPE == 2 && half == 0) columns_of(1);
+                if (PIPE == 1 && half == 1) columns_of(1);
+                const Terms<3> y = split<3>(right[2 * half] * until[2 * half], right[2 * half + 1] * until[2 * half + 1]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) delta[i][r] = kept(until[i][r], delta[i][r]);
-        {
-            const Terms<3> x[2] = {split<3>(delta[0], delta[1]), split<3>(delta[2], delta[3])};
+                for (int rank = 2; rank >= 0; --rank)
 #pragma unroll
-            for (int d = 0; d < 2 * KS; ++d) {
+                    for (int j = 0; j <= rank; ++j)
+                        if (j < TERMS) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) state[d][r] = kept(rest, state[d][r]);
-#pragma unroll
-                for (int half = 0; half < 2; ++half) state[d] = product<3>(Lds::columns(keys, d, half), x[half], state[d]);
+                            for (int d = 0; d < 2 * KS; ++d) state[d] = mfma(k[half % PIPE][d].t[j], y.t[rank - j], state[d]);
+                        }
             }
+            Values::turn_values(tile, out);
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int t = chunk * kChunk + 16 * (i / 4) + 4 * group + i % 4;
-            if (there && t < p.T) outs[t * p.out.step] = from_float<T>(t < limit ? out[i / 4][i % 4] : 0.0f);
-        }
+        now();
+        Values::write(tile, out_base + static_cast<int64_t>(chunk) * kChunk * p.out.step, p.out.step, p.T - chunk * kChunk, limit - chunk * kChunk, p.DV - mine, p.near_values);
     }
-    for (int t = live * kChunk + wave * 4 + group; t < p.T; t += 16)      // padding
-        for (int c = columns * 64 + lane % 16; c < p.DV && c < columns * 64 + 64; c += 16)
-            outs[t * p.out.step + c - column] = from_float<T>(0.0f);
+    for (int t = live * kChunk + wave * 4 + group; t < p.T; t += 4 * WAVES)      // padding
+        for (int c = left + lane % 16; c < p.DV && c < left + Values::kColumns; c += 16) out_base[t * p.out.step + c - mine] = from_float<T>(0.0f);
 #pragma unroll
     for (int d = 0; d < 2 * KS; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = 16 * d + 4 * group + r;
+            const int row = head_element(d, r);
             if (there && row < p.DK) p.state_out[cell + static_cast<int64_t>(row) * p.DV] = state[d][r];
         }
 }
@@ -416,16 +457,27 @@ __global__ __launch_bounds__(64 * KS) void delta_step_kernel(DeltaArgs p) {
 // ------------------------------------------------------------------------------------------------------------------
 constexpr int kFewSteps = 16;
 
+template <typename T, int KS, int WAVES>
+void launch_walk(const DeltaArgs& p, hipStream_t stream) {
+    const dim3 grid(head_groups(p.N * p.HV, (p.DV + 16 * WAVES - 1) / (16 * WAVES))), block(64 * WAVES);
+    if (p.marks != nullptr) delta_walk_kernel<T, KS, WAVES, true><<<grid, block, 0, stream>>>(p);
+    else delta_walk_kernel<T, KS, WAVES, false><<<grid, block, 0, stream>>>(p);
+}
+
 template <typename T, int KS>
 void launch_forward(const DeltaArgs& p, hipStream_t stream) {
-    const dim3 grid(head_groups(p.N * p.HV, (p.DV + 63) / 64));
     if (p.blocks == nullptr) {
-        delta_step_kernel<T, KS><<<grid, dim3(64 * KS), 0, stream>>>(p);
+        delta_step_kernel<T, KS><<<dim3(head_groups(p.N * p.HV, (p.DV + 63) / 64)), dim3(64 * KS), 0, stream>>>(p);
         return;
     }
     launch_chunks<T, KS, false>(p, stream);
-    if (p.marks != nullptr) delta_walk_kernel<T, KS, true><<<grid, dim3(256), 0, stream>>>(p);
-    else delta_walk_kernel<T, KS, false><<<grid, dim3(256), 0, stream>>>(p);
+    if constexpr (sizeof(T) == 2) {
+        if (eight_waves(p)) {
+            launch_walk<T, KS, 8>(p, stream);
+            return;
+        }
+    }
+    launch_walk<T, KS, 4>(p, stream);
 }
 
 }  // namespace
@@ -471,9 +523,13 @@ DeltaArgs delta_args(const snnf_delta_rule_call* c) {
     p.starts = static_cast<const uint8_t*>(c->starts), p.starts_step = c->starts_step, p.starts_row = c->starts_row;
     p.lengths = c->lengths;
     p.state = c->state;
+    p.near_keys = c->key_size % 8 == 0 && near_by(p.q, c->dtype, true) && near_by(p.k, c->dtype, true);
+    p.near_values = c->value_size % 8 == 0 && near_by(p.v, c->dtype, true);
     return p;
 }
 
+int delta_ranks(const snnf_delta_rule_call* c) { return c->dtype == SNNF_F32 ? kOutputRanks<float> : kOutputRanks<bf16_t>; }
+int64_t delta_mark_elements(const snnf_delta_rule_call* c) { return mark_elements(delta_ranks(c), c->key_size <= 64 ? 2 : 4, c->value_size); }
 int64_t delta_chunks(const snnf_delta_rule_call* c) {
     return static_cast<int64_t>(c->N) * c->value_heads * ((c->T + kChunk - 1) / kChunk);
 }
@@ -484,16 +540,15 @@ using namespace snnf;
 
 extern "C" size_t snnf_delta_rule_workspace_bytes(const snnf_delta_rule_call* call, int training) {
     if (check_delta("snnf_delta_rule_workspace_bytes", call) != SNNF_OK || (!training && call->T <= kFewSteps)) return 0;
-    const int ranks = call->dtype == SNNF_F32 ? kOutputRanks<float> : kOutputRanks<bf16_t>;
-    return static_cast<size_t>(delta_chunks(call)) * (block_words(ranks) + 3 * kChunk) * 4;
+    return static_cast<size_t>(delta_chunks(call)) * block_words(delta_ranks(call)) * 4;
 }
 
 extern "C" size_t snnf_delta_rule_marks_bytes(const snnf_delta_rule_call* call) {
     if (check_delta("snnf_delta_rule_marks_bytes", call) != SNNF_OK) return 0;
-    return static_cast<size_t>(delta_chunks(call)) * (call->key_size + kChunk) * call->value_size * sizeof(float);
+    return static_cast<size_t>(delta_chunks(call)) * (delta_mark_elements(call) + delta_elements(delta_ranks(call), call->value_size)) * sizeof(uint16_t);
 }
 
-extern "C" int snnf_delta_rule(const snnf_delta_rule_call* call, const snnf_heads* out, float* state_out, float* marks, void* workspace, size_t workspace_bytes,
+extern "C" int snnf_delta_rule(const snnf_delta_rule_call* call, const snnf_heads* out, float* state_out, void* marks, void* workspace, size_t workspace_bytes,
                                void* stream) {
     const int rc = check_delta("snnf_delta_rule", call);
     if (rc != SNNF_OK) return rc;
@@ -507,13 +562,13 @@ extern "C" int snnf_delta_rule(const snnf_delta_rule_call* call, const snnf_head
     if (need > 0) {
         if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
             return fail(SNNF_ERR_WORKSPACE, "snnf_delta_rule: workspace of %zu bytes needed, got %zu", need, workspace_bytes);
-        p.vectors = static_cast<float*>(workspace);
-        p.blocks = reinterpret_cast<uint32_t*>(p.vectors + delta_chunks(call) * 3 * kChunk);
+        p.blocks = static_cast<uint32_t*>(workspace);
     }
     if (marks != nullptr) {
-        p.marks = marks;
-        p.deltas = marks + delta_chunks(call) * call->key_size * call->value_size;
+        p.marks = static_cast<uint16_t*>(marks);
+        p.deltas = p.marks + delta_chunks(call) * delta_mark_elements(call);
     }
+    p.near_values = p.near_values && near_by(p.out, call->dtype, false);
     hipStream_t hs = as_stream(stream);
     const bool small = call->key_size <= 64;
     if (call->dtype == SNNF_F32) small ? launch_forward<float, 2>(p, hs) : launch_forward<float, 4>(p, hs);

@@ -16,14 +16,17 @@ namespace {
 // The walk back
 // ------------------------------------------------------------------------------------------------------------------
 template <typename T, int KS>
-__global__ __launch_bounds__(256, 1) void delta_walk_back_kernel(DeltaArgs p) {
+__global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_kernel(DeltaArgs p) {
+    constexpr int WAVES = 4, RANKS = kOutputRanks<T>, TERMS = kTerms<T>, PIPE = TERMS == 1 ? 2 : 1;
     using Lds = Rows<T, KS>;
-    constexpr int BUFFERS = kTerms<T> == 1 ? 2 : 1;
-    __shared__ uint16_t lds[BUFFERS][2][Lds::kSize];
+    using Values = Tile<T, WAVES>;
+    using Reader = ChunkReader<T, KS, WAVES, block_pieces(3)>;
+    __shared__ alignas(16) typename Reader::Buffers lds[Reader::kBuffers];
     int head, columns;
     if (!part_of_head(p.N * p.HV, (p.DV + 63) / 64, &head, &columns)) return;
     const int n = head / p.HV, hv = head % p.HV, h = hv / (p.HV / p.H), limit = length_of(p, n), live = (limit + kChunk - 1) / kChunk;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane / 16, column = columns * 64 + wave * 16 + lane % 16;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane / 16;
+    const int left = columns * Values::kColumns, mine = left + 16 * wave, column = mine + lane % 16;
     const bool there = column < p.DV;
     const int64_t cell = static_cast<int64_t>(head) * p.DK * p.DV + column;
     f32x4 later[2 * KS];
@@ -31,133 +34,143 @@ __global__ __launch_bounds__(256, 1) void delta_walk_back_kernel(DeltaArgs p) {
     for (int d = 0; d < 2 * KS; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = 16 * d + 4 * group + r;
+            const int row = head_element(d, r);
             later[d][r] = p.dstate != nullptr && there && row < p.DK ? p.dstate[cell + static_cast<int64_t>(row) * p.DV] : 0.0f;
         }
-    const T* douts = static_cast<const T*>(p.dout.data) + n * p.dout.row + hv * p.dout.head + column;
-    T* dvalues = static_cast<T*>(const_cast<void*>(p.dv.data)) + n * p.dv.row + hv * p.dv.head + column;
-    T o[16];
+    const T* k_base = static_cast<const T*>(p.k.data) + n * p.k.row + h * p.k.head;
+    const T* q_base = static_cast<const T*>(p.q.data) + n * p.q.row + h * p.q.head;
+    const T* o_base = static_cast<const T*>(p.dout.data) + n * p.dout.row + hv * p.dout.head + left;
+    T* v_base = static_cast<T*>(const_cast<void*>(p.dv.data)) + n * p.dv.row + hv * p.dv.head + mine;
+    Reader reader;
     const auto fetch = [&](int chunk) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int t = chunk * kChunk + 16 * (i / 4) + 4 * group + i % 4;
-            o[i] = there && t < limit ? douts[t * p.dout.step] : from_float<T>(0.0f);
-        }
+        const int64_t first = static_cast<int64_t>(chunk) * kChunk;
+        if (chunk >= 0) reader.fetch(p, k_base + first * p.k.step, q_base + first * p.q.step, o_base + first * p.dout.step, p.dout.step, limit - chunk * kChunk, p.DV - left,
+                                     p.blocks + (static_cast<int64_t>(head) * p.chunks + chunk) * block_words(3), lds[chunk % Reader::kBuffers]);
     };
-    Staged<T, KS, 256> k_next, q_next;
-    if (live > 0) {
-        k_next.load(p.k, (live - 1) * kChunk, limit, n, h, p.DK);
-        q_next.load(p.q, (live - 1) * kChunk, limit, n, h, p.DK);
-        fetch(live - 1);
-    }
+    fetch(live - 1);
     for (int chunk = live - 1; chunk >= 0; --chunk) {
         const int64_t index = static_cast<int64_t>(head) * p.chunks + chunk;
-        uint16_t *keys = lds[chunk % BUFFERS][0], *queries = lds[chunk % BUFFERS][1];
-        if constexpr (BUFFERS == 1) __syncthreads();
-        k_next.store(keys);
-        q_next.store(queries);
-        __syncthreads();
-        const uint32_t* blocks = p.blocks + index * block_words(3) + lane * 4;
-        const float* vectors = p.vectors + index * 3 * kChunk + 4 * group;
-        f32x4 since[4], until[4], beta[4];
+        typename Reader::Buffers& here = lds[chunk % Reader::kBuffers];
+        const uint16_t *keys = here.keys, *queries = here.queries;
+        T* tile = here.tile;
+        const uint32_t *block = here.block, *vectors = block + block_vectors(3);
+        reader.wait(here);
+        fetch(chunk - 1);
+        now();
+        // K R
+        f32x4 pull[4], dout[4], z[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            since[i] = *reinterpret_cast<const f32x4*>(vectors + 16 * i);
-            until[i] = *reinterpret_cast<const f32x4*>(vectors + kChunk + 16 * i);
-            beta[i] = *reinterpret_cast<const f32x4*>(vectors + 2 * kChunk + 16 * i);
-        }
-        const float rest = p.vectors[index * 3 * kChunk + kChunk - 1];
-        f32x4 dout[4];
+        for (int i = 0; i < 4; ++i) pull[i] = z[i] = f32x4{0, 0, 0, 0};
+        Terms<TERMS> a[PIPE][4];
+        const auto load = [&](int s) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) dout[i / 4][i % 4] = to_float(o[i]);
-        if (chunk > 0) {
-            k_next.load(p.k, (chunk - 1) * kChunk, limit, n, h, p.DK);
-            q_next.load(p.q, (chunk - 1) * kChunk, limit, n, h, p.DK);
-            fetch(chunk - 1);
-        }
-        {
-            float* marks = p.later + index * p.DK * p.DV + column;
-#pragma unroll
-            for (int d = 0; d < 2 * KS; ++d)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * d + 4 * group + r;
-                    if (there && row < p.DK) marks[row * p.DV] = later[d][r];
-                }
-        }
-        f32x4 pull[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pull[i] = f32x4{0, 0, 0, 0};
+            for (int i = 0; i < 4; ++i) a[s % PIPE][i] = Lds::rows(keys, i, s);
+        };
+        load(0);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
+            if (PIPE == 2 && s + 1 < KS) load(s + 1);
+            now();
             const Terms<3> x = split<3>(later[2 * s], later[2 * s + 1]);
+            uint16_t* marks = p.later + index * (RANKS * padded_values(p.DV) * 32 * KS);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) pull[i] = product<3>(Lds::rows(keys, i, s), x, pull[i]);
+            for (int r = 0; r < RANKS; ++r)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+                    *reinterpret_cast<u32x2a*>(marks + static_cast<uint32_t>((r * padded_values(p.DV) + column) * 32 * KS + mark_place<KS>(column, 2 * s + half) + 4 * group)) =
+                        u32x2a{x.t[r][2 * half], x.t[r][2 * half + 1]};
+#pragma unroll
+            for (int rank = 2; rank >= 0; --rank)
+#pragma unroll
+                for (int j = 0; j <= rank; ++j)
+                    if (j < TERMS) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) pull[i] = mfma(a[s % PIPE][i].t[j], x.t[rank - j], pull[i]);
+                    }
+            if (PIPE == 1 && s + 1 < KS) load(s + 1);
         }
+        const bool broken = __builtin_amdgcn_readfirstlane(vectors[kBroken]) != 0;
+        const float rest = __uint_as_float(__builtin_amdgcn_readfirstlane(vectors[kSince + kChunk - 1]));
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) pull[i][r] = kept(until[i][r], pull[i][r]);
-        {
-            const Terms<kTerms<T>> x[2] = {split<kTerms<T>>(dout[0], dout[1]), split<kTerms<T>>(dout[2], dout[3])};
-#pragma unroll
-            for (int f = 0; f < kBlocks; ++f) {
-                Terms<3> scores;
-#pragma unroll
-                for (int i = 0; i < 3; ++i) scores.t[i] = *reinterpret_cast<const u32x4a*>(blocks + ((kBlocks + f) * 3 + i) * 256);
-                pull[upper_tile(f)] = product<3>(scores, x[upper_half(f)], pull[upper_tile(f)]);
-            }
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 until = row_factors(vectors, kUntil, i);
+            if (broken) drop(pull[i], until);
+            pull[i] *= until;
+            dout[i] = Values::get(tile, i);
         }
-        f32x4 z[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) z[i] = f32x4{0, 0, 0, 0};
+        // dU, then Z
         {
+            const Terms<TERMS> x[2] = {split<TERMS>(dout[0], dout[1]), split<TERMS>(dout[2], dout[3])};
+            Terms<3> scores[kBlocks];
+#pragma unroll
+            for (int f = 0; f < kBlocks; ++f) scores[f] = block_terms<3>(block + kBlocks * 3 * 256, f);
+            now();
+#pragma unroll
+            for (int rank = 2; rank >= 0; --rank)
+#pragma unroll
+                for (int j = 0; j <= rank; ++j)
+                    if (rank - j < TERMS) {
+#pragma unroll
+                        for (int f = 0; f < kBlocks; ++f) pull[upper_tile(f)] = mfma(scores[f].t[j], x[upper_half(f)].t[rank - j], pull[upper_tile(f)]);
+                    }
+        }
+        {
+            Terms<3> inverse[kBlocks];
+#pragma unroll
+            for (int f = 0; f < kBlocks; ++f) inverse[f] = block_terms<3>(block, f);
+            now();
             const Terms<3> x[2] = {split<3>(pull[0], pull[1]), split<3>(pull[2], pull[3])};
 #pragma unroll
-            for (int f = 0; f < kBlocks; ++f) {
-                Terms<3> inverse;
+            for (int rank = 2; rank >= 0; --rank)
 #pragma unroll
-                for (int i = 0; i < 3; ++i) inverse.t[i] = *reinterpret_cast<const u32x4a*>(blocks + (f * 3 + i) * 256);
-                z[upper_tile(f)] = product<3>(inverse, x[upper_half(f)], z[upper_tile(f)]);
-            }
+                for (int j = 0; j <= rank; ++j)
+#pragma unroll
+                    for (int f = 0; f < kBlocks; ++f) z[upper_tile(f)] = mfma(inverse[f].t[j], x[upper_half(f)].t[rank - j], z[upper_tile(f)]);
         }
-        float* pulls = p.pulls + index * kChunk * p.DV + column;
+        Values::template write_terms<RANKS>(tile, z, p.pulls + index * (RANKS * kChunk * padded_values(p.DV)) + mine, padded_values(p.DV));
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int at = 16 * (i / 4) + 4 * group + i % 4, t = chunk * kChunk + at;
-            if (there) pulls[at * p.DV] = z[i / 4][i % 4];
-            z[i / 4][i % 4] *= beta[i / 4][i % 4];
-            if (there && t < p.T) dvalues[t * p.dv.step] = from_float<T>(t < limit ? z[i / 4][i % 4] : 0.0f);
+        for (int i = 0; i < 4; ++i) z[i] *= row_factors(vectors, kBeta, i);
+        Values::turn_values(tile, z);
+        Values::write(tile, v_base + static_cast<int64_t>(chunk) * kChunk * p.dv.step, p.dv.step, p.T - chunk * kChunk, limit - chunk * kChunk, p.DV - mine, p.near_values);
+        // R in front of the chunk
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 since = row_factors(vectors, kSince, i);
+            if (broken) drop(z[i], since), drop(dout[i], since);
+            z[i] *= -since;
+            dout[i] *= since * p.scale;
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                z[i][r] = kept(since[i][r], -z[i][r]);
-                dout[i][r] = kept(since[i][r] * p.scale, dout[i][r]);
-            }
-        {
-            const Terms<3> x[2] = {split<3>(z[0], z[1]), split<3>(z[2], z[3])}, y[2] = {split<3>(dout[0], dout[1]), split<3>(dout[2], dout[3])};
-#pragma unroll
-            for (int d = 0; d < 2 * KS; ++d) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) later[d][r] = kept(rest, later[d][r]);
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    later[d] = product<3>(Lds::columns(keys, d, half), x[half], later[d]);
-                    later[d] = product<3>(Lds::columns(queries, d, half), y[half], later[d]);
-                }
-            }
+        for (int d = 0; d < 2 * KS; ++d) {
+            if (broken) drop(later[d], f32x4{rest, rest, rest, rest});
+            later[d] *= rest;
         }
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                Terms<TERMS> c[2 * KS];
+#pragma unroll
+                for (int d = 0; d < 2 * KS; ++d) c[d] = Lds::columns(which == 0 ? keys : queries, d, half);
+                now();
+                const Terms<3> x = which == 0 ? split<3>(z[2 * half], z[2 * half + 1]) : split<3>(dout[2 * half], dout[2 * half + 1]);
+#pragma unroll
+                for (int rank = 2; rank >= 0; --rank)
+#pragma unroll
+                    for (int j = 0; j <= rank; ++j)
+                        if (j < TERMS) {
+#pragma unroll
+                            for (int d = 0; d < 2 * KS; ++d) later[d] = mfma(c[d].t[j], x.t[rank - j], later[d]);
+                        }
+            }
     }
-    for (int t = live * kChunk + wave * 4 + group; t < p.T; t += 16)      // padding
-        for (int c = columns * 64 + lane % 16; c < p.DV && c < columns * 64 + 64; c += 16)
-            dvalues[t * p.dv.step + c - column] = from_float<T>(0.0f);
+    for (int t = live * kChunk + wave * 4 + group; t < p.T; t += 4 * WAVES)      // padding
+        for (int c = left + lane % 16; c < p.DV && c < left + Values::kColumns; c += 16) v_base[t * p.dv.step + c - mine] = from_float<T>(0.0f);
 #pragma unroll
     for (int d = 0; d < 2 * KS; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = 16 * d + 4 * group + r;
+            const int row = head_element(d, r);
             if (there && row < p.DK) p.dstate_in[cell + static_cast<int64_t>(row) * p.DV] = later[d][r];
         }
 }
@@ -173,12 +186,44 @@ __device__ __forceinline__ float over_groups(float v) {
     const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
-__device__ __forceinline__ void floats_of(float (&x)[8], const float* row, int at, int width, bool there) {
-    Raw<float, 8> raw;
-    if (there && at < width) raw.load(row, at, width - at);
-    else raw.clear();
+// A row of 32 value columns in LDS: [term][64 rows][32], 16 bytes at a place that depends on the row.
+__device__ __forceinline__ uint32_t value_place(int row, int slot) { return static_cast<uint32_t>(row * 32 + 8 * slot_of<4>(row, slot)); }
+template <int N>
+__device__ __forceinline__ Terms<N> value_rows(const uint16_t* lds, int tile) {
+    const int lane = threadIdx.x & 63;
+    const uint16_t* from = lds + 16 * tile * 32 + value_place(lane % 16, lane / 16);
+    Terms<N> r;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = raw[j];
+    for (int n = 0; n < N; ++n) r.t[n] = *reinterpret_cast<const u32x4a*>(from + n * kChunk * 32);
+    return r;
+}
+// Rows of a plane [64][columns] to there: four instructions, one to a wave.
+__device__ __forceinline__ void value_rows_to_lds(const uint16_t* plane, int columns, uint16_t* lds) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = 16 * wave + lane / 4;
+    to_lds(plane, static_cast<uint32_t>(row * columns + 8 * slot_of<4>(row, lane % 4)) * 2, lds_address(lds) + wave * 1024);
+}
+// Of a state's 32 value columns [32][32 KS]: elements of `head_element(tile, ..)` as rows, value columns as places, in order.
+template <int N, int KS>
+__device__ __forceinline__ Terms<N> state_columns(const uint16_t* lds, int tile) {
+    typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+    const int lane = threadIdx.x & 63, column = 8 * (lane / 16) + lane % 16 / 4;
+    const uint16_t* low = lds + column * 32 * KS + mark_place<KS>(column, tile) + 4 * (lane % 4);
+    const uint16_t* high = lds + (column + 4) * 32 * KS + mark_place<KS>(column + 4, tile) + 4 * (lane % 4);
+    Terms<N> r;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const u32x2a a = __builtin_bit_cast(u32x2a, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(low + n * 1024 * KS)));
+        const u32x2a b = __builtin_bit_cast(u32x2a, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(high + n * 1024 * KS)));
+        r.t[n] = u32x4a{a[0], a[1], b[0], b[1]};
+    }
+    return r;
+}
+template <int N>
+__device__ __forceinline__ float term_sum(const Terms<N>& x, int j) {
+    float v = 0.0f;
+#pragma unroll
+    for (int n = N - 1; n >= 0; --n) v += element<bf16_t>(x.t[n][j / 2], j % 2);
+    return v;
 }
 template <typename T>
 __device__ __forceinline__ void store_four(T* to, int left, const f32x4& x) {
@@ -187,18 +232,26 @@ __device__ __forceinline__ void store_four(T* to, int left, const f32x4& x) {
         if (r < left) to[r] = from_float<T>(x[r]);
 }
 
-template <typename T, int KS>
-__global__ __launch_bounds__(256, 1) void delta_gradient_kernel(DeltaArgs p) {
+// GROUPED: several value heads to a key head, whose gradients are summed one after the other.
+template <typename T, int KS, bool GROUPED>
+__global__ __launch_bounds__(256, sizeof(T) == 4 || GROUPED ? 1 : 2) void delta_gradient_kernel(DeltaArgs p) {
     using Lds = Rows<T, KS>;
-    constexpr int RANKS = kOutputRanks<T>, TILES = 2 * KS;
-    __shared__ uint16_t keys[Lds::kSize], queries[Lds::kSize];
+    constexpr int RANKS = kOutputRanks<T>, TERMS = kTerms<T>, TILES = 2 * KS;
+    __shared__ union {
+        struct {                        // 32 value columns of everything
+            uint16_t marks[RANKS][1024 * KS], later[RANKS][1024 * KS], deltas[RANKS][kChunk * 32], pulls[RANKS][kChunk * 32], douts[TERMS][kChunk * 32];
+        };
+        struct {
+            uint16_t keys[Lds::kSize], queries[Lds::kSize];
+        };
+    } lds;
     __shared__ double total[kChunk];
     __shared__ int part[kChunk];
     __shared__ float betas[kChunk], dsums[kChunk], tails[kChunk], dots[4];
     const uint32_t place = group_index();
     if (place >= static_cast<uint32_t>(p.N) * p.H * p.chunks) return;
     const int chunk = place % p.chunks, n = place / p.chunks / p.H, h = place / p.chunks % p.H, first = chunk * kChunk, limit = length_of(p, n);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane / 16, column = lane % 16, own = 16 * wave + column, t_own = first + own;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane / 16, column = lane % 16, own = 16 * wave + column, t_own = first + own;
     const bool there = t_own < limit;
     const int members = p.HV / p.H, gate_size = p.gate_float ? 4 : static_cast<int>(sizeof(T));
     const auto store_gate = [&](const HeadView& x, int t, int hv, float v) {
@@ -212,13 +265,7 @@ __global__ __launch_bounds__(256, 1) void delta_gradient_kernel(DeltaArgs p) {
     f32x4 dq_all[TILES], dk_all[TILES];
 #pragma unroll
     for (int d = 0; d < TILES; ++d) dq_all[d] = dk_all[d] = f32x4{0, 0, 0, 0};
-    if (first < limit) {
-        Staged<T, KS, 256> k_rows, q_rows;
-        k_rows.load(p.k, first, limit, n, h, p.DK);
-        q_rows.load(p.q, first, limit, n, h, p.DK);
-        k_rows.store(keys);
-        q_rows.store(queries);
-    }
+    const int columns = padded_values(p.DV);
     for (int member = 0; member < members; ++member) {
         const int hv = h * members + member;
         if (first >= limit) {
@@ -226,6 +273,7 @@ __global__ __launch_bounds__(256, 1) void delta_gradient_kernel(DeltaArgs p) {
             continue;
         }
         const int64_t index = (static_cast<int64_t>(n) * p.HV + hv) * p.chunks + chunk;
+        const float* vectors = reinterpret_cast<const float*>(p.blocks + index * block_words(3) + block_vectors(3));
         __syncthreads();
         if (wave == 0) {
             const int t = first + lane;
@@ -240,12 +288,11 @@ __global__ __launch_bounds__(256, 1) void delta_gradient_kernel(DeltaArgs p) {
                 if (lane >= d) sum += before;
             }
             total[lane] = sum;
-            betas[lane] = p.vectors[index * 3 * kChunk + 2 * kChunk + lane];
+            betas[lane] = vectors[kBeta + lane];
         }
-        const float since = p.vectors[index * 3 * kChunk + own], until = p.vectors[index * 3 * kChunk + kChunk + own];
-        const float beta = p.vectors[index * 3 * kChunk + 2 * kChunk + own];
-        const float *marks = p.marks + index * p.DK * p.DV, *later = p.later + index * p.DK * p.DV;
-        const float *deltas = p.deltas + index * kChunk * p.DV, *pulls = p.pulls + index * kChunk * p.DV;
+        const float since = vectors[kSince + own], until = vectors[kUntil + own], beta = vectors[kBeta + own];
+        const uint16_t *marks = p.marks + index * (RANKS * columns * 32 * KS), *later = p.later + index * (RANKS * columns * 32 * KS);
+        const uint16_t *deltas = p.deltas + index * (RANKS * kChunk * columns), *pulls = p.pulls + index * (RANKS * kChunk * columns);
         const T* douts = static_cast<const T*>(p.dout.data) + n * p.dout.row + hv * p.dout.head;
         const T* values = static_cast<const T*>(p.v.data) + n * p.v.row + hv * p.v.head;
         f32x4 score_row[4], score_column[4], pull_row[4], pull_column[4], dq[TILES], ds[TILES], dk[TILES];
@@ -255,54 +302,74 @@ __global__ __launch_bounds__(256, 1) void delta_gradient_kernel(DeltaArgs p) {
         for (int d = 0; d < TILES; ++d) dq[d] = ds[d] = dk[d] = f32x4{0, 0, 0, 0};
         float dbeta = 0.0f, zv = 0.0f, dot = 0.0f;
         for (int s = 0; 32 * s < p.DV; ++s) {
-            const int at = 32 * s + 8 * group;
-            float z[8], delta[8];
-            floats_of(z, pulls + own * p.DV, at, p.DV, true);
-            floats_of(delta, deltas + own * p.DV, at, p.DV, true);
-            const auto o_own = there && at < p.DV ? row_terms<T>(douts + t_own * p.dout.step, at, p.DV) : no_terms<kTerms<T>>();
-            const Terms<RANKS> z_own = split<RANKS>(z), delta_own = split<RANKS>(delta);
+            if (s > 0) __syncthreads();
+#pragma unroll
+            for (int r = 0; r < RANKS; ++r) {
+#pragma unroll
+                for (int i = wave; i < 2 * KS; i += 4) {
+                    const uint32_t from = static_cast<uint32_t>((r * columns + 32 * s) * 32 * KS + 512 * i) * 2 + lane * 16;
+                    to_lds(marks, from, lds_address(lds.marks[r]) + i * 1024);
+                    to_lds(later, from, lds_address(lds.later[r]) + i * 1024);
+                }
+                value_rows_to_lds(deltas + r * kChunk * columns + 32 * s, columns, lds.deltas[r]);
+                value_rows_to_lds(pulls + r * kChunk * columns + 32 * s, columns, lds.pulls[r]);
+            }
+            {
+                const int row = threadIdx.x / 4, at = 32 * s + 8 * (threadIdx.x % 4);
+                const auto o = first + row < limit && at < p.DV ? row_terms<T>(douts + (first + row) * p.dout.step, at, p.DV) : no_terms<TERMS>();
+#pragma unroll
+                for (int r = 0; r < TERMS; ++r) *reinterpret_cast<u32x4a*>(lds.douts[r] + value_place(row, threadIdx.x % 4)) = o.t[r];
+            }
             Raw<T, 8> v;
+            const int at = 32 * s + 8 * group;
             if (there && at < p.DV) v.load(values + t_own * p.v.step, at, p.DV - at);
             else v.clear();
+            arrived();
+            __syncthreads();
+            const Terms<TERMS> o_own = value_rows<TERMS>(lds.douts[0], wave);
+            const Terms<RANKS> z_own = value_rows<RANKS>(lds.pulls[0], wave), delta_own = value_rows<RANKS>(lds.deltas[0], wave);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                dbeta = fmaf(z[j], delta[j], dbeta);
-                zv = fmaf(z[j], v[j], zv);
+                const float z = term_sum(z_own, j);
+                dbeta = fmaf(z, term_sum(delta_own, j), dbeta);
+                zv = fmaf(z, v[j], zv);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                float x[8];
                 if (j <= wave) {
-                    floats_of(x, deltas + (16 * j + column) * p.DV, at, p.DV, true);
-                    const Terms<RANKS> a = split<RANKS>(x);
-                    score_row[j] = product<RANKS>(a, o_own, score_row[j]);
-                    pull_row[j] = product<RANKS>(a, z_own, pull_row[j]);
+                    const Terms<RANKS> x = value_rows<RANKS>(lds.deltas[0], j);
+                    score_row[j] = product<RANKS>(x, o_own, score_row[j]);
+                    pull_row[j] = product<RANKS>(x, z_own, pull_row[j]);
                 }
                 if (j >= wave) {
-                    const int t = first + 16 * j + column;
-                    const auto o = t < limit && at < p.DV ? row_terms<T>(douts + t * p.dout.step, at, p.DV) : no_terms<kTerms<T>>();
-                    score_column[j] = product<RANKS>(o, delta_own, score_column[j]);
-                    floats_of(x, pulls + (16 * j + column) * p.DV, at, p.DV, true);
-                    pull_column[j] = product<RANKS>(split<RANKS>(x), delta_own, pull_column[j]);
+                    score_column[j] = product<RANKS>(value_rows<TERMS>(lds.douts[0], j), delta_own, score_column[j]);
+                    pull_column[j] = product<RANKS>(value_rows<RANKS>(lds.pulls[0], j), delta_own, pull_column[j]);
                 }
             }
 #pragma unroll
             for (int d = 0; d < TILES; ++d) {
-                const int row = 16 * d + column;
-                float x[8], y[8];
-                floats_of(x, marks + row * p.DV, at, p.DV, row < p.DK);
-                floats_of(y, later + row * p.DV, at, p.DV, row < p.DK);
+                const Terms<RANKS> x = state_columns<RANKS, KS>(lds.marks[0], d), y = state_columns<RANKS, KS>(lds.later[0], d);
                 if (d % 4 == wave) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) dot = fmaf(x[j], y[j], dot);
+                    for (int j = 0; j < 8; ++j) dot = fmaf(term_sum(x, j), term_sum(y, j), dot);
                 }
-                const Terms<RANKS> a = split<RANKS>(x), b = split<RANKS>(y);
-                dq[d] = product<RANKS>(a, o_own, dq[d]);
-                ds[d] = product<RANKS>(a, z_own, ds[d]);
-                dk[d] = product<RANKS>(b, delta_own, dk[d]);
+                dq[d] = product<RANKS>(x, o_own, dq[d]);
+                ds[d] = product<RANKS>(x, z_own, ds[d]);
+                dk[d] = product<RANKS>(y, delta_own, dk[d]);
             }
         }
         __syncthreads();
+        {
+            Staged<T, 4 * KS, 256> x;
+            const T* from = static_cast<const T*>(p.k.data) + static_cast<int64_t>(first) * p.k.step + n * p.k.row + h * p.k.head;
+            x.load(from, p.k.step, limit - first, p.DK, p.near_keys);
+            put_rows<T, KS, 256>(x, lds.keys);
+            from = static_cast<const T*>(p.q.data) + static_cast<int64_t>(first) * p.q.step + n * p.q.row + h * p.q.head;
+            x.load(from, p.q.step, limit - first, p.DK, p.near_keys);
+            put_rows<T, KS, 256>(x, lds.queries);
+        }
+        __syncthreads();
+        const uint16_t *keys = lds.keys, *queries = lds.queries;
         float tail = 0.0f;
 #pragma unroll
         for (int d = 0; d < TILES; ++d) {
@@ -345,8 +412,8 @@ __global__ __launch_bounds__(256, 1) void delta_gradient_kernel(DeltaArgs p) {
             const f32x4 k = Lds::four(keys, own, d), q = Lds::four(queries, own, d);
 #pragma unroll
             for (int r = 0; r < 4; ++r) sum += q[r] * dq[d][r] - k[r] * dk[d][r];
-            dq_all[d] += dq[d];
-            dk_all[d] += dk[d];
+            if constexpr (GROUPED) dq_all[d] += dq[d], dk_all[d] += dk[d];
+            else dq_all[d] = dq[d], dk_all[d] = dk[d];
         }
         sum = over_groups(sum);
         tail = over_groups(tail);
@@ -362,7 +429,7 @@ __global__ __launch_bounds__(256, 1) void delta_gradient_kernel(DeltaArgs p) {
         __syncthreads();
         if (wave == 0) {
             const int mine = part[lane], before = lane == 0 ? 0 : part[lane - 1], last = part[kChunk - 1], t = first + lane;
-            const float rest = p.vectors[index * 3 * kChunk + kChunk - 1];
+            const float rest = vectors[kSince + kChunk - 1];
             const float behind = kept(rest, dots[0] + dots[1] + dots[2] + dots[3]) + lane_sum(tails[lane]);
             float v = dsums[lane];
 #pragma unroll
@@ -378,7 +445,7 @@ __global__ __launch_bounds__(256, 1) void delta_gradient_kernel(DeltaArgs p) {
     if (t_own < p.T) {
 #pragma unroll
         for (int d = 0; d < TILES; ++d) {
-            const int at = 16 * d + 4 * group;
+            const int at = head_element(d, 0);
             store_four<T>(dquery + at, p.DK - at, dq_all[d]);
             store_four<T>(dkey + at, p.DK - at, dk_all[d]);
         }
@@ -389,7 +456,9 @@ template <typename T, int KS>
 void launch_backward(const DeltaArgs& p, hipStream_t stream) {
     launch_chunks<T, KS, true>(p, stream);
     delta_walk_back_kernel<T, KS><<<dim3(head_groups(p.N * p.HV, (p.DV + 63) / 64)), dim3(256), 0, stream>>>(p);
-    delta_gradient_kernel<T, KS><<<grid_of(static_cast<int64_t>(p.N) * p.H * p.chunks), dim3(256), 0, stream>>>(p);
+    const dim3 grid = grid_of(static_cast<int64_t>(p.N) * p.H * p.chunks);
+    if (p.HV > p.H) delta_gradient_kernel<T, KS, true><<<grid, dim3(256), 0, stream>>>(p);
+    else delta_gradient_kernel<T, KS, false><<<grid, dim3(256), 0, stream>>>(p);
 }
 
 }  // namespace
@@ -399,10 +468,11 @@ using namespace snnf;
 
 extern "C" size_t snnf_delta_rule_backward_workspace_bytes(const snnf_delta_rule_call* call) {
     if (check_delta("snnf_delta_rule_backward_workspace_bytes", call) != SNNF_OK) return 0;
-    return static_cast<size_t>(delta_chunks(call)) * (block_words(3) + 3 * kChunk + (call->key_size + kChunk) * call->value_size) * 4;
+    return static_cast<size_t>(delta_chunks(call)) *
+           (block_words(3) * 4 + (delta_mark_elements(call) + delta_elements(delta_ranks(call), call->value_size)) * sizeof(uint16_t));
 }
 
-extern "C" int snnf_delta_rule_backward(const snnf_delta_rule_call* call, const float* marks, const snnf_heads* dout, const float* dstate, const snnf_heads* dquery,
+extern "C" int snnf_delta_rule_backward(const snnf_delta_rule_call* call, const void* marks, const snnf_heads* dout, const float* dstate, const snnf_heads* dquery,
                                         const snnf_heads* dkey, const snnf_heads* dvalue, const snnf_heads* dgate, const snnf_heads* dbeta, float* dstate_in,
                                         void* workspace, size_t workspace_bytes, void* stream) {
     const int rc = check_delta("snnf_delta_rule_backward", call);
@@ -420,12 +490,12 @@ extern "C" int snnf_delta_rule_backward(const snnf_delta_rule_call* call, const 
     p.dout = view(dout), p.dq = view(dquery), p.dk = view(dkey), p.dv = view(dvalue), p.dgate = view(dgate), p.dbeta = view(dbeta);
     p.dstate = dstate, p.dstate_in = dstate_in;
     const int64_t chunks = delta_chunks(call);
-    p.marks = const_cast<float*>(marks);
-    p.deltas = p.marks + chunks * call->key_size * call->value_size;
-    p.vectors = static_cast<float*>(workspace);
-    p.blocks = reinterpret_cast<uint32_t*>(p.vectors + chunks * 3 * kChunk);
-    p.later = reinterpret_cast<float*>(p.blocks + chunks * block_words(3));
-    p.pulls = p.later + chunks * call->key_size * call->value_size;
+    p.near_values = call->value_size % 8 == 0 && near_by(p.dout, call->dtype, true) && near_by(p.dv, call->dtype, false);
+    p.marks = static_cast<uint16_t*>(const_cast<void*>(marks));
+    p.deltas = p.marks + chunks * delta_mark_elements(call);
+    p.blocks = static_cast<uint32_t*>(workspace);
+    p.later = reinterpret_cast<uint16_t*>(p.blocks + chunks * block_words(3));
+    p.pulls = p.later + chunks * delta_mark_elements(call);
     hipStream_t hs = as_stream(stream);
     const bool small = call->key_size <= 64;
     if (call->dtype == SNNF_F32) small ? launch_backward<float, 2>(p, hs) : launch_backward<float, 4>(p, hs);
