@@ -240,13 +240,10 @@ __global__ __launch_bounds__(kTerms<T> == 1 && !TRAIN ? 512 : 64 * WAVES) void d
                             if (rank < RANKS) out[i] = mfma(a[s % PIPE][4 + i].t[j], x[s % 2].t[rank - j], out[i]);
                     }
             if constexpr (TRAIN) {
-                uint16_t* marks = p.marks + index * (RANKS * padded_values(p.DV) * 32 * KS);
+                uint16_t* marks = p.marks + index * (kMarkRanks<T> * padded_values(p.DV) * 32 * KS);
 #pragma unroll
-                for (int r = 0; r < RANKS; ++r)
-#pragma unroll
-                    for (int half = 0; half < 2; ++half)
-                        *reinterpret_cast<u32x2a*>(marks + static_cast<uint32_t>((r * padded_values(p.DV) + column) * 32 * KS + mark_place<KS>(column, 2 * s + half) + 4 * group)) =
-                            u32x2a{x[s % 2].t[r][2 * half], x[s % 2].t[r][2 * half + 1]};
+                for (int r = 0; r < kMarkRanks<T>; ++r)
+                    *reinterpret_cast<u32x4a*>(marks + static_cast<uint32_t>((r * padded_values(p.DV) + column) * 32 * KS + mark_place<KS>(column, 2 * s) + 8 * group)) = x[s % 2].t[r];
             }
             if (PIPE == 1 && s + 1 < KS) load(s + 1);
         }
@@ -529,7 +526,7 @@ DeltaArgs delta_args(const snnf_delta_rule_call* c) {
 }
 
 int delta_ranks(const snnf_delta_rule_call* c) { return c->dtype == SNNF_F32 ? kOutputRanks<float> : kOutputRanks<bf16_t>; }
-int64_t delta_mark_elements(const snnf_delta_rule_call* c) { return mark_elements(delta_ranks(c), c->key_size <= 64 ? 2 : 4, c->value_size); }
+int64_t delta_mark_elements(const snnf_delta_rule_call* c) { return mark_elements(c->dtype == SNNF_F32 ? kMarkRanks<float> : (c->dtype == SNNF_F16 ? kMarkRanks<f16_t> : kMarkRanks<bf16_t>), c->key_size <= 64 ? 2 : 4, c->value_size); }
 int64_t delta_chunks(const snnf_delta_rule_call* c) {
     return static_cast<int64_t>(c->N) * c->value_heads * ((c->T + kChunk - 1) / kChunk);
 }

@@ -72,13 +72,10 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
             if (PIPE == 2 && s + 1 < KS) load(s + 1);
             now();
             const Terms<3> x = split<3>(later[2 * s], later[2 * s + 1]);
-            uint16_t* marks = p.later + index * (RANKS * padded_values(p.DV) * 32 * KS);
+            uint16_t* marks = p.later + index * (kMarkRanks<T> * padded_values(p.DV) * 32 * KS);
 #pragma unroll
-            for (int r = 0; r < RANKS; ++r)
-#pragma unroll
-                for (int half = 0; half < 2; ++half)
-                    *reinterpret_cast<u32x2a*>(marks + static_cast<uint32_t>((r * padded_values(p.DV) + column) * 32 * KS + mark_place<KS>(column, 2 * s + half) + 4 * group)) =
-                        u32x2a{x.t[r][2 * half], x.t[r][2 * half + 1]};
+            for (int r = 0; r < kMarkRanks<T>; ++r)
+                *reinterpret_cast<u32x4a*>(marks + static_cast<uint32_t>((r * padded_values(p.DV) + column) * 32 * KS + mark_place<KS>(column, 2 * s) + 8 * group)) = x.t[r];
 #pragma unroll
             for (int rank = 2; rank >= 0; --rank)
 #pragma unroll
@@ -197,18 +194,18 @@ __device__ __forceinline__ Terms<N> value_rows(const uint16_t* lds, int tile) {
     for (int n = 0; n < N; ++n) r.t[n] = *reinterpret_cast<const u32x4a*>(from + n * kChunk * 32);
     return r;
 }
-// Rows of a plane [64][columns] to there: four instructions, one to a wave.
-__device__ __forceinline__ void value_rows_to_lds(const uint16_t* plane, int columns, uint16_t* lds) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = 16 * wave + lane / 4;
-    to_lds(plane, static_cast<uint32_t>(row * columns + 8 * slot_of<4>(row, lane % 4)) * 2, lds_address(lds) + wave * 1024);
+// Rows of a plane [64][columns] to there, instruction `part` of four.
+__device__ __forceinline__ void value_rows_to_lds(const uint16_t* plane, int columns, uint16_t* lds, int part) {
+    const int lane = threadIdx.x & 63, row = 16 * part + lane / 4;
+    to_lds(plane, static_cast<uint32_t>(row * columns + 8 * slot_of<4>(row, lane % 4)) * 2, lds_address(lds) + part * 1024);
 }
 // Of a state's 32 value columns [32][32 KS]: elements of `head_element(tile, ..)` as rows, value columns as places, in order.
 template <int N, int KS>
 __device__ __forceinline__ Terms<N> state_columns(const uint16_t* lds, int tile) {
     typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
     const int lane = threadIdx.x & 63, column = 8 * (lane / 16) + lane % 16 / 4;
-    const uint16_t* low = lds + column * 32 * KS + mark_place<KS>(column, tile) + 4 * (lane % 4);
-    const uint16_t* high = lds + (column + 4) * 32 * KS + mark_place<KS>(column + 4, tile) + 4 * (lane % 4);
+    const uint16_t* low = lds + column * 32 * KS + mark_place<KS>(column, tile) + 8 * (lane % 4);
+    const uint16_t* high = lds + (column + 4) * 32 * KS + mark_place<KS>(column + 4, tile) + 8 * (lane % 4);
     Terms<N> r;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -225,131 +222,223 @@ __device__ __forceinline__ float term_sum(const Terms<N>& x, int j) {
     for (int n = N - 1; n >= 0; --n) v += element<bf16_t>(x.t[n][j / 2], j % 2);
     return v;
 }
+// Eight elements next to each other
 template <typename T>
-__device__ __forceinline__ void store_four(T* to, int left, const f32x4& x) {
+__device__ __forceinline__ void store_eight(T* to, int left, const f32x4& x, const f32x4& y) {
+    Raw<T, 8> raw;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-        if (r < left) to[r] = from_float<T>(x[r]);
+    for (int r = 0; r < 4; r += 2) raw.put(r, x[r], x[r + 1]), raw.put(4 + r, y[r], y[r + 1]);
+    if (left > 0) raw.store(to, 0, left);
+}
+template <typename T>
+__device__ __forceinline__ void store_gate(const DeltaArgs& p, const HeadView& x, int t, int n, int hv, float v) {
+    if (x.data == nullptr) return;
+    const int64_t at = t * x.step + n * x.row + hv * x.head;
+    if (p.gate_float) static_cast<float*>(const_cast<void*>(x.data))[at] = v;
+    else static_cast<T*>(const_cast<void*>(x.data))[at] = from_float<T>(v);
 }
 
-// GROUPED: several value heads to a key head, whose gradients are summed one after the other.
-template <typename T, int KS, bool GROUPED>
-__global__ __launch_bounds__(256, sizeof(T) == 4 || GROUPED ? 1 : 2) void delta_gradient_kernel(DeltaArgs p) {
-    using Lds = Rows<T, KS>;
-    constexpr int RANKS = kOutputRanks<T>, TERMS = kTerms<T>, TILES = 2 * KS;
-    __shared__ union {
-        struct {                        // 32 value columns of everything
-            uint16_t marks[RANKS][1024 * KS], later[RANKS][1024 * KS], deltas[RANKS][kChunk * 32], pulls[RANKS][kChunk * 32], douts[TERMS][kChunk * 32];
-        };
-        struct {
-            uint16_t keys[Lds::kSize], queries[Lds::kSize];
-        };
-    } lds;
-    __shared__ double total[kChunk];
-    __shared__ int part[kChunk];
-    __shared__ float betas[kChunk], dsums[kChunk], tails[kChunk], dots[4];
-    const uint32_t place = group_index();
-    if (place >= static_cast<uint32_t>(p.N) * p.H * p.chunks) return;
-    const int chunk = place % p.chunks, n = place / p.chunks / p.H, h = place / p.chunks % p.H, first = chunk * kChunk, limit = length_of(p, n);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane / 16, column = lane % 16, own = 16 * wave + column, t_own = first + own;
-    const bool there = t_own < limit;
-    const int members = p.HV / p.H, gate_size = p.gate_float ? 4 : static_cast<int>(sizeof(T));
-    const auto store_gate = [&](const HeadView& x, int t, int hv, float v) {
-        if (x.data == nullptr) return;
-        const int64_t at = t * x.step + n * x.row + hv * x.head;
-        if (gate_size == 4) static_cast<float*>(const_cast<void*>(x.data))[at] = v;
-        else static_cast<T*>(const_cast<void*>(x.data))[at] = from_float<T>(v);
+// Of tensors of 16 bits the logarithm is rounded to float32: a decay by 2^-10 is off by 2^-21 then.
+template <typename T>
+__device__ __forceinline__ float decay_between(double x) {
+    if constexpr (sizeof(T) == 4) return decay_of(x);
+    else return __builtin_amdgcn_exp2f(static_cast<float>(x));
+}
+
+// Two waves to 16 steps: the first works out dL, the second dP, and each has half of the head's elements of everything else; they exchange dL and dP through LDS. A workgroup takes one chunk after the
+// other, each in pieces of 32 value columns and then a last one of keys and queries; with bfloat16 the next piece is on its way while one is worked on.
+template <typename T, int KS> struct GradientPieces {
+    static constexpr int RANKS = kOutputRanks<T>, TERMS = kTerms<T>, MARKS = kMarkRanks<T>, BUFFERS = TERMS == 1 ? 2 : 1;     // by the room in LDS
+    struct Slice {                      // 32 value columns of everything
+        uint16_t marks[MARKS][1024 * KS], later[MARKS][1024 * KS], deltas[RANKS][kChunk * 32], pulls[RANKS][kChunk * 32], douts[TERMS][kChunk * 32];
     };
-    T* dquery = static_cast<T*>(const_cast<void*>(p.dq.data)) + t_own * p.dq.step + n * p.dq.row + h * p.dq.head;
-    T* dkey = static_cast<T*>(const_cast<void*>(p.dk.data)) + t_own * p.dk.step + n * p.dk.row + h * p.dk.head;
-    f32x4 dq_all[TILES], dk_all[TILES];
-#pragma unroll
-    for (int d = 0; d < TILES; ++d) dq_all[d] = dk_all[d] = f32x4{0, 0, 0, 0};
-    const int columns = padded_values(p.DV);
-    for (int member = 0; member < members; ++member) {
-        const int hv = h * members + member;
-        if (first >= limit) {
-            if (group == 0 && t_own < p.T) store_gate(p.dgate, t_own, hv, 0.0f), store_gate(p.dbeta, t_own, hv, 0.0f);
-            continue;
-        }
-        const int64_t index = (static_cast<int64_t>(n) * p.HV + hv) * p.chunks + chunk;
-        const float* vectors = reinterpret_cast<const float*>(p.blocks + index * block_words(3) + block_vectors(3));
-        __syncthreads();
-        if (wave == 0) {
-            const int t = first + lane;
-            const bool inside = t < limit;
-            const float g = inside ? gate_value<T>(p.gate, p.gate_float, t, n, hv, 0.0f) : 0.0f;
-            const bool fresh = inside && (g < kForgotten || (p.starts != nullptr && p.starts[t * p.starts_step + n * p.starts_row] != 0));
-            double sum = fresh ? 0.0 : static_cast<double>(g) * 1.4426950408889634074;
-            part[lane] = __popcll(__ballot(fresh) & (~0ull >> (63 - lane)));
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-                const double before = __shfl_up(sum, d, 64);
-                if (lane >= d) sum += before;
+    struct Heads {
+        uint16_t keys[Rows<T, KS>::kSize], queries[Rows<T, KS>::kSize];
+        uint32_t between[2][4][2][RANKS][256];     // of 16 steps: dL and dP by rows, then dP by columns; halves of the other steps
+    };
+    union Piece {
+        Slice slice;
+        Heads heads;
+    };
+};
+
+template <typename T, int KS>
+__global__ __launch_bounds__(512) void delta_gradient_kernel(DeltaArgs p) {
+    using Lds = Rows<T, KS>;
+    using Pieces = GradientPieces<T, KS>;
+    constexpr int RANKS = Pieces::RANKS, TERMS = Pieces::TERMS, MARKS = Pieces::MARKS, BUFFERS = Pieces::BUFFERS;
+    __shared__ alignas(16) typename Pieces::Piece lds[BUFFERS];
+    __shared__ alignas(16) double total[kChunk];
+    __shared__ alignas(16) int part[kChunk];
+    __shared__ alignas(16) float betas[kChunk], dsums[2][kChunk], tails[2][kChunk], own_sums[kChunk], dots[8];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), team = wave / 4, w = wave % 4, group = lane / 16, column = lane % 16;
+    const int own = 16 * w + column, members = p.HV / p.H, columns = padded_values(p.DV), slices = (p.DV + 31) / 32;
+    const int places = p.N * p.H * p.chunks;
+    struct Item {                       // a chunk of a value head
+        int place, member, chunk, n, h, rows;
+    };
+    const auto settle = [&](Item& x) {
+        const int head = x.place / p.chunks;
+        x.chunk = x.place - head * p.chunks, x.n = head / p.H, x.h = head % p.H;
+        x.rows = length_of(p, x.n) - x.chunk * kChunk;
+    };
+    // The first chunk from there on that has steps; those that have none get their zeros on the way.
+    const auto find = [&](Item& x) {
+        for (; x.place < places; x.place += static_cast<int>(gridDim.x)) {
+            settle(x);
+            if (x.rows > 0) return;
+            const int steps = p.T - x.chunk * kChunk < kChunk ? p.T - x.chunk * kChunk : kChunk;
+            T* dquery = static_cast<T*>(const_cast<void*>(p.dq.data)) + static_cast<int64_t>(x.chunk) * kChunk * p.dq.step + x.n * p.dq.row + x.h * p.dq.head;
+            T* dkey = static_cast<T*>(const_cast<void*>(p.dk.data)) + static_cast<int64_t>(x.chunk) * kChunk * p.dk.step + x.n * p.dk.row + x.h * p.dk.head;
+            for (int i = threadIdx.x; i < steps * p.DK; i += 512) {
+                const int t = i / p.DK, e = i - t * p.DK;
+                dquery[t * p.dq.step + e] = dkey[t * p.dk.step + e] = from_float<T>(0.0f);
             }
-            total[lane] = sum;
-            betas[lane] = vectors[kBeta + lane];
+            for (int i = threadIdx.x; i < steps * members; i += 512)
+                store_gate<T>(p, p.dgate, x.chunk * kChunk + i / members, x.n, x.h * members + i % members, 0.0f),
+                    store_gate<T>(p, p.dbeta, x.chunk * kChunk + i / members, x.n, x.h * members + i % members, 0.0f);
         }
-        const float since = vectors[kSince + own], until = vectors[kUntil + own], beta = vectors[kBeta + own];
-        const uint16_t *marks = p.marks + index * (RANKS * columns * 32 * KS), *later = p.later + index * (RANKS * columns * 32 * KS);
-        const uint16_t *deltas = p.deltas + index * (RANKS * kChunk * columns), *pulls = p.pulls + index * (RANKS * kChunk * columns);
-        const T* douts = static_cast<const T*>(p.dout.data) + n * p.dout.row + hv * p.dout.head;
-        const T* values = static_cast<const T*>(p.v.data) + n * p.v.row + hv * p.v.head;
-        f32x4 score_row[4], score_column[4], pull_row[4], pull_column[4], dq[TILES], ds[TILES], dk[TILES];
+    };
+    const auto index_of = [&](const Item& x) { return (static_cast<int64_t>(x.n) * p.HV + x.h * members + x.member) * p.chunks + x.chunk; };
+
+    Raw<T, 8> o_next, v_next;           // a piece to each of the first 256 threads; the values of the lane's own step
+    const auto fetch_slice = [&](const Item& x, int s, typename Pieces::Slice& to) {
+        const int64_t index = index_of(x);
+        const int hv = x.h * members + x.member;
+        const uint16_t *marks = p.marks + index * (MARKS * columns * 32 * KS), *later = p.later + index * (MARKS * columns * 32 * KS);
+        const uint16_t* own_rows = (team == 0 ? p.deltas : p.pulls) + index * (RANKS * kChunk * columns) + 32 * s;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) score_row[j] = score_column[j] = pull_row[j] = pull_column[j] = f32x4{0, 0, 0, 0};
+        for (int r = 0; r < MARKS; ++r)
 #pragma unroll
-        for (int d = 0; d < TILES; ++d) dq[d] = ds[d] = dk[d] = f32x4{0, 0, 0, 0};
-        float dbeta = 0.0f, zv = 0.0f, dot = 0.0f;
-        for (int s = 0; 32 * s < p.DV; ++s) {
-            if (s > 0) __syncthreads();
-#pragma unroll
-            for (int r = 0; r < RANKS; ++r) {
-#pragma unroll
-                for (int i = wave; i < 2 * KS; i += 4) {
-                    const uint32_t from = static_cast<uint32_t>((r * columns + 32 * s) * 32 * KS + 512 * i) * 2 + lane * 16;
-                    to_lds(marks, from, lds_address(lds.marks[r]) + i * 1024);
-                    to_lds(later, from, lds_address(lds.later[r]) + i * 1024);
+            for (int i = 0; i < (2 * KS + 7) / 8; ++i)
+                if (wave + 8 * i < 2 * KS) {
+                    const uint32_t from = static_cast<uint32_t>((r * columns + 32 * s) * 32 * KS + 512 * (wave + 8 * i)) * 2 + lane * 16;
+                    to_lds(marks, from, lds_address(to.marks[r]) + (wave + 8 * i) * 1024);
+                    to_lds(later, from, lds_address(to.later[r]) + (wave + 8 * i) * 1024);
                 }
-                value_rows_to_lds(deltas + r * kChunk * columns + 32 * s, columns, lds.deltas[r]);
-                value_rows_to_lds(pulls + r * kChunk * columns + 32 * s, columns, lds.pulls[r]);
-            }
-            {
-                const int row = threadIdx.x / 4, at = 32 * s + 8 * (threadIdx.x % 4);
-                const auto o = first + row < limit && at < p.DV ? row_terms<T>(douts + (first + row) * p.dout.step, at, p.DV) : no_terms<TERMS>();
 #pragma unroll
-                for (int r = 0; r < TERMS; ++r) *reinterpret_cast<u32x4a*>(lds.douts[r] + value_place(row, threadIdx.x % 4)) = o.t[r];
+        for (int r = 0; r < RANKS; ++r) value_rows_to_lds(own_rows + r * kChunk * columns, columns, team == 0 ? to.deltas[r] : to.pulls[r], w);
+        o_next.clear();
+        v_next.clear();
+        const T* douts = static_cast<const T*>(p.dout.data) + static_cast<int64_t>(x.chunk) * kChunk * p.dout.step + x.n * p.dout.row + hv * p.dout.head;
+        const T* values = static_cast<const T*>(p.v.data) + static_cast<int64_t>(x.chunk) * kChunk * p.v.step + x.n * p.v.row + hv * p.v.head;
+        const int row = threadIdx.x / 4, at = 32 * s + 8 * (threadIdx.x % 4), own_at = 32 * s + 8 * group;
+        if (row < x.rows && row < kChunk && at < p.DV) o_next.load(douts, row * p.dout.step + at, p.DV - at);
+        if (team == 0 && own < x.rows && own_at < p.DV) v_next.load(values, own * p.v.step + own_at, p.DV - own_at);
+    };
+    // What a chunk's steps have of their own: exp(G), exp(G_64 - G), beta and exp(G_64) of the lane's own step; gate, start and beta of the first wave's
+    float since_next, until_next, beta_next, rest_next, gate_next, row_beta_next;
+    bool start_next;
+    const auto fetch_steps = [&](const Item& x) {
+        const int hv = x.h * members + x.member;
+        const float* vectors = reinterpret_cast<const float*>(p.blocks + index_of(x) * block_words(3) + block_vectors(3));
+        since_next = vectors[kSince + own], until_next = vectors[kUntil + own], beta_next = vectors[kBeta + own], rest_next = vectors[kSince + kChunk - 1];
+        if (wave == 0) {
+            const int t = x.chunk * kChunk + (lane < x.rows ? lane : 0);
+            gate_next = gate_value<T>(p.gate, p.gate_float, t, x.n, hv, 0.0f);
+            start_next = p.starts != nullptr && p.starts[t * p.starts_step + x.n * p.starts_row] != 0;
+            row_beta_next = vectors[kBeta + lane];
+        }
+    };
+    const auto fetch_heads = [&](const Item& x, typename Pieces::Heads& to) {
+        const T* keys = static_cast<const T*>(p.k.data) + static_cast<int64_t>(x.chunk) * kChunk * p.k.step + x.n * p.k.row + x.h * p.k.head;
+        const T* queries = static_cast<const T*>(p.q.data) + static_cast<int64_t>(x.chunk) * kChunk * p.q.step + x.n * p.q.row + x.h * p.q.head;
+        if constexpr (TERMS == 1) {
+            if (p.near_keys) {
+                const uint32_t* zeros = p.blocks + index_of(x) * block_words(3) + block_vectors(3) + kZeros;
+                rows_to_lds<4 * KS, 8>(reinterpret_cast<const uint16_t*>(keys), p.k.step, x.rows, p.DK, zeros, to.keys);
+                rows_to_lds<4 * KS, 8>(reinterpret_cast<const uint16_t*>(queries), p.q.step, x.rows, p.DK, zeros, to.queries);
+                return;
             }
-            Raw<T, 8> v;
-            const int at = 32 * s + 8 * group;
-            if (there && at < p.DV) v.load(values + t_own * p.v.step, at, p.DV - at);
-            else v.clear();
+        }
+        Staged<T, 4 * KS, 512> k_rows, q_rows;
+        k_rows.load(keys, p.k.step, x.rows, p.DK, p.near_keys);
+        q_rows.load(queries, p.q.step, x.rows, p.DK, p.near_keys);
+        put_rows<T, KS, 512>(k_rows, to.keys);
+        put_rows<T, KS, 512>(q_rows, to.queries);
+    };
+
+    Item item{static_cast<int>(blockIdx.x), 0, 0, 0, 0, 0};
+    find(item);
+    if (item.place >= places) return;
+    int turn = 0;                       // pieces so far
+    fetch_slice(item, 0, lds[0].slice);
+    fetch_steps(item);
+    f32x4 dq_all[KS], dk_all[KS];
+    for (;;) {
+        if (item.member == 0) {
+#pragma unroll
+            for (int d = 0; d < KS; ++d) dq_all[d] = dk_all[d] = f32x4{0, 0, 0, 0};
+        }
+        const float since = since_next, until = until_next, beta = beta_next, rest = rest_next;
+        // by_row: the wave's steps are rows of dL (dP), the others, up to them, its columns; by_column: the other way round
+        f32x4 by_row[4], by_column[4], dq[KS], ds[KS], dk[KS];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) by_row[j] = by_column[j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int d = 0; d < KS; ++d) dq[d] = ds[d] = dk[d] = f32x4{0, 0, 0, 0};
+        float dbeta = 0.0f, zv = 0.0f, dot = 0.0f;
+        for (int s = 0; s < slices; ++s, ++turn) {
+            typename Pieces::Slice& here = lds[turn % BUFFERS].slice;
+            if (threadIdx.x < 256) {
+                Terms<TERMS> o;
+                if constexpr (TERMS == 1) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o.t[0][i] = o_next.w[i];
+                } else {
+                    float x[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = o_next[j];
+                    o = split<TERMS>(x);
+                }
+#pragma unroll
+                for (int r = 0; r < TERMS; ++r) *reinterpret_cast<u32x4a*>(here.douts[r] + value_place(threadIdx.x / 4, threadIdx.x % 4)) = o.t[r];
+            }
+            const Raw<T, 8> v = v_next;
+            if (s == 0 && wave == 0) {
+                const bool fresh = lane < item.rows && (start_next || gate_next < kForgotten);
+                double sum = fresh || lane >= item.rows ? 0.0 : static_cast<double>(gate_next) * 1.4426950408889634074;
+                part[lane] = __popcll(__ballot(fresh) & (~0ull >> (63 - lane)));
+#pragma unroll
+                for (int d = 1; d < 64; d *= 2) {
+                    const double before = __shfl_up(sum, d, 64);
+                    if (lane >= d) sum += before;
+                }
+                total[lane] = sum;
+                betas[lane] = row_beta_next;
+            }
             arrived();
             __syncthreads();
-            const Terms<TERMS> o_own = value_rows<TERMS>(lds.douts[0], wave);
-            const Terms<RANKS> z_own = value_rows<RANKS>(lds.pulls[0], wave), delta_own = value_rows<RANKS>(lds.deltas[0], wave);
+            if constexpr (BUFFERS == 2) {
+                if (s + 1 < slices) fetch_slice(item, s + 1, lds[(turn + 1) % BUFFERS].slice);
+                else fetch_heads(item, lds[(turn + 1) % BUFFERS].heads);
+            }
+            const Terms<TERMS> o_own = value_rows<TERMS>(here.douts[0], w);
+            const Terms<RANKS> z_own = value_rows<RANKS>(here.pulls[0], w), delta_own = value_rows<RANKS>(here.deltas[0], w);
+            if (team == 0) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float z = term_sum(z_own, j);
-                dbeta = fmaf(z, term_sum(delta_own, j), dbeta);
-                zv = fmaf(z, v[j], zv);
+                for (int j = 0; j < 8; ++j) {
+                    const float z = term_sum(z_own, j);
+                    dbeta = fmaf(z, term_sum(delta_own, j), dbeta);
+                    zv = fmaf(z, v[j], zv);
+                }
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (j <= wave) {
-                    const Terms<RANKS> x = value_rows<RANKS>(lds.deltas[0], j);
-                    score_row[j] = product<RANKS>(x, o_own, score_row[j]);
-                    pull_row[j] = product<RANKS>(x, z_own, pull_row[j]);
+                if (j <= w) {
+                    const Terms<RANKS> x = value_rows<RANKS>(here.deltas[0], j);
+                    if (team == 0) by_row[j] = product<RANKS>(x, z_own, by_row[j]);
+                    else by_row[j] = product<RANKS>(x, o_own, by_row[j]);
                 }
-                if (j >= wave) {
-                    score_column[j] = product<RANKS>(value_rows<TERMS>(lds.douts[0], j), delta_own, score_column[j]);
-                    pull_column[j] = product<RANKS>(value_rows<RANKS>(lds.pulls[0], j), delta_own, pull_column[j]);
+                if (j >= w) {
+                    if (team == 0) by_column[j] = product<RANKS>(value_rows<RANKS>(here.pulls[0], j), delta_own, by_column[j]);
+                    else by_column[j] = product<RANKS>(value_rows<TERMS>(here.douts[0], j), delta_own, by_column[j]);
                 }
             }
 #pragma unroll
-            for (int d = 0; d < TILES; ++d) {
-                const Terms<RANKS> x = state_columns<RANKS, KS>(lds.marks[0], d), y = state_columns<RANKS, KS>(lds.later[0], d);
-                if (d % 4 == wave) {
+            for (int d = 0; d < KS; ++d) {
+                const Terms<MARKS> x = state_columns<MARKS, KS>(here.marks[0], team * KS + d), y = state_columns<MARKS, KS>(here.later[0], team * KS + d);
+                if (d == w) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) dot = fmaf(term_sum(x, j), term_sum(y, j), dot);
                 }
@@ -357,23 +446,70 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || GROUPED ? 1 : 2) void delta_
                 ds[d] = product<RANKS>(x, z_own, ds[d]);
                 dk[d] = product<RANKS>(y, delta_own, dk[d]);
             }
+            if constexpr (BUFFERS == 1) {
+                __syncthreads();
+                if (s + 1 < slices) fetch_slice(item, s + 1, lds[0].slice);
+                else fetch_heads(item, lds[0].heads);
+            }
         }
+        typename Pieces::Heads& here = lds[turn % BUFFERS].heads;
+        const uint16_t *keys = here.keys, *queries = here.queries;
+        arrived();
         __syncthreads();
-        {
-            Staged<T, 4 * KS, 256> x;
-            const T* from = static_cast<const T*>(p.k.data) + static_cast<int64_t>(first) * p.k.step + n * p.k.row + h * p.k.head;
-            x.load(from, p.k.step, limit - first, p.DK, p.near_keys);
-            put_rows<T, KS, 256>(x, lds.keys);
-            from = static_cast<const T*>(p.q.data) + static_cast<int64_t>(first) * p.q.step + n * p.q.row + h * p.q.head;
-            x.load(from, p.q.step, limit - first, p.DK, p.near_keys);
-            put_rows<T, KS, 256>(x, lds.queries);
+        Item next = item;
+        if (++next.member == members) {
+            next.member = 0;
+            next.place += static_cast<int>(gridDim.x);
+            find(next);
         }
-        __syncthreads();
-        const uint16_t *keys = lds.keys, *queries = lds.queries;
+        ++turn;
+        if (BUFFERS == 2 && next.place < places) {
+            fetch_slice(next, 0, lds[turn % BUFFERS].slice);
+            fetch_steps(next);
+        }
+        // The other steps are rows 4 group + r of the tiles
+        const double mine_total = total[own];
+        const int mine_part = part[own];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int at = 16 * j + 4 * group;
+            typedef double f64x2 __attribute__((ext_vector_type(2)));
+            typedef int i32x4 __attribute__((ext_vector_type(4)));
+            const f64x2 sums[2] = {*reinterpret_cast<const f64x2*>(total + at), *reinterpret_cast<const f64x2*>(total + at + 2)};
+            const i32x4 parts = *reinterpret_cast<const i32x4*>(part + at);
+            const f32x4 others = *reinterpret_cast<const f32x4*>(betas + at);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int x = at + r;
+                const double since_then = mine_total - sums[r / 2][r % 2];
+                const float d = parts[r] == mine_part ? decay_between<T>(x <= own ? since_then : -since_then) : 0.0f;
+                if (team == 0) {
+                    by_row[j][r] = x == own ? 0.0f : kept(-d * beta * others[r], x < own ? by_row[j][r] : by_column[j][r]);
+                } else {
+                    by_row[j][r] = x <= own ? kept(p.scale * d * others[r], by_row[j][r]) : 0.0f;
+                    by_column[j][r] = x >= own ? kept(p.scale * d * beta, by_column[j][r]) : 0.0f;
+                }
+            }
+        }
+        const auto publish = [&](int where, const f32x4 (&x)[4]) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const Terms<RANKS> y = split<RANKS>(x[2 * half], x[2 * half + 1]);
+#pragma unroll
+                for (int r = 0; r < RANKS; ++r) *reinterpret_cast<u32x4a*>(&here.between[where][w][half][r][lane * 4]) = y.t[r];
+            }
+        };
+        const auto published = [&](int where, int half) {
+            Terms<RANKS> x;
+#pragma unroll
+            for (int r = 0; r < RANKS; ++r) x.t[r] = *reinterpret_cast<const u32x4a*>(&here.between[where][w][half][r][lane * 4]);
+            return x;
+        };
+        publish(team, by_row);
         float tail = 0.0f;
 #pragma unroll
-        for (int d = 0; d < TILES; ++d) {
-            const f32x4 k = Lds::four(keys, own, d);
+        for (int d = 0; d < KS; ++d) {
+            const f32x4 k = Lds::four(keys, own, team * KS + d);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float behind = kept(until * beta, dk[d][r]);
@@ -382,56 +518,68 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || GROUPED ? 1 : 2) void delta_
                 dq[d][r] = kept(since * p.scale, dq[d][r]);
             }
         }
-        // x: the other step, row of the tile
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int x = 16 * j + 4 * group + r;
-                const float d = part[x] == part[own] ? decay_of(x <= own ? total[own] - total[x] : total[x] - total[own]) : 0.0f;
-                const float both = -d * beta * betas[x];
-                score_row[j][r] = x <= own ? kept(p.scale * d * betas[x], score_row[j][r]) : 0.0f;
-                score_column[j][r] = x >= own ? kept(p.scale * d * beta, score_column[j][r]) : 0.0f;
-                pull_row[j][r] = x < own ? kept(both, pull_row[j][r]) : (x > own ? kept(both, pull_column[j][r]) : 0.0f);
-            }
+        __syncthreads();
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const Terms<RANKS> a = split<RANKS>(score_row[2 * half], score_row[2 * half + 1]), b = split<RANKS>(score_column[2 * half], score_column[2 * half + 1]);
-            const Terms<RANKS> c = split<RANKS>(pull_row[2 * half], pull_row[2 * half + 1]);
+            const Terms<RANKS> x = published(0, half), y = published(1, half);
 #pragma unroll
-            for (int d = 0; d < TILES; ++d) {
-                const auto k = Lds::columns(keys, d, half), q = Lds::columns(queries, d, half);
-                dq[d] = product<RANKS>(k, a, dq[d]);
-                dk[d] = product<RANKS>(q, b, dk[d]);
-                dk[d] = product<RANKS>(k, c, dk[d]);
+            for (int d = 0; d < KS; ++d) {
+                const auto k = Lds::columns(keys, team * KS + d, half);
+                dk[d] = product<RANKS>(k, x, dk[d]);
+                dq[d] = product<RANKS>(k, y, dq[d]);
             }
+        }
+        __syncthreads();
+        if (team == 1) publish(0, by_column);
+        __syncthreads();
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const Terms<RANKS> x = published(0, half);
+#pragma unroll
+            for (int d = 0; d < KS; ++d) dk[d] = product<RANKS>(Lds::columns(queries, team * KS + d, half), x, dk[d]);
         }
         float sum = 0.0f;
 #pragma unroll
-        for (int d = 0; d < TILES; ++d) {
-            const f32x4 k = Lds::four(keys, own, d), q = Lds::four(queries, own, d);
+        for (int d = 0; d < KS; ++d) {
+            const f32x4 k = Lds::four(keys, own, team * KS + d), q = Lds::four(queries, own, team * KS + d);
 #pragma unroll
             for (int r = 0; r < 4; ++r) sum += q[r] * dq[d][r] - k[r] * dk[d][r];
-            if constexpr (GROUPED) dq_all[d] += dq[d], dk_all[d] += dk[d];
-            else dq_all[d] = dq[d], dk_all[d] = dk[d];
+            dq_all[d] += dq[d];
+            dk_all[d] += dk[d];
         }
         sum = over_groups(sum);
         tail = over_groups(tail);
         dbeta = over_groups(dbeta);
         zv = over_groups(zv);
         dot = lane_sum(dot);
+        const int first = item.chunk * kChunk, hv = item.h * members + item.member, t_own = first + own;
         if (group == 0) {
-            dsums[own] = sum + 2.0f * beta * (dbeta - zv);
-            tails[own] = tail;
-            if (t_own < p.T) store_gate(p.dbeta, t_own, hv, there ? dbeta : 0.0f);
+            dsums[team][own] = sum;
+            tails[team][own] = tail;
+            if (team == 0) {
+                own_sums[own] = 2.0f * beta * (dbeta - zv);
+                if (t_own < p.T) store_gate<T>(p, p.dbeta, t_own, item.n, hv, own < item.rows ? dbeta : 0.0f);
+            }
         }
         if (lane == 0) dots[wave] = dot;
+        if (item.member == members - 1 && t_own < p.T) {
+            T* dquery = static_cast<T*>(const_cast<void*>(p.dq.data)) + t_own * p.dq.step + item.n * p.dq.row + item.h * p.dq.head;
+            T* dkey = static_cast<T*>(const_cast<void*>(p.dk.data)) + t_own * p.dk.step + item.n * p.dk.row + item.h * p.dk.head;
+#pragma unroll
+            for (int d = 0; d < KS; d += 2) {
+                const int at = head_element(team * KS + d, 0);
+                store_eight<T>(dquery + at, p.DK - at, dq_all[d], dq_all[d + 1]);
+                store_eight<T>(dkey + at, p.DK - at, dk_all[d], dk_all[d + 1]);
+            }
+        }
         __syncthreads();
         if (wave == 0) {
             const int mine = part[lane], before = lane == 0 ? 0 : part[lane - 1], last = part[kChunk - 1], t = first + lane;
-            const float rest = vectors[kSince + kChunk - 1];
-            const float behind = kept(rest, dots[0] + dots[1] + dots[2] + dots[3]) + lane_sum(tails[lane]);
-            float v = dsums[lane];
+            float all = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) all += dots[i];
+            const float behind = kept(rest, all) + lane_sum(tails[0][lane] + tails[1][lane]);
+            float v = dsums[0][lane] + dsums[1][lane] + own_sums[lane];
 #pragma unroll
             for (int d = 1; d < 64; d *= 2) {
                 const float more = __shfl_down(v, d, 64);
@@ -439,15 +587,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || GROUPED ? 1 : 2) void delta_
                 if (lane + d < 64 && theirs == mine) v += more;
             }
             if (mine == last) v += behind;
-            if (t < p.T) store_gate(p.dgate, t, hv, t < limit && mine == before ? v : 0.0f);
+            if (t < p.T) store_gate<T>(p, p.dgate, t, item.n, hv, lane < item.rows && mine == before ? v : 0.0f);
         }
-    }
-    if (t_own < p.T) {
-#pragma unroll
-        for (int d = 0; d < TILES; ++d) {
-            const int at = head_element(d, 0);
-            store_four<T>(dquery + at, p.DK - at, dq_all[d]);
-            store_four<T>(dkey + at, p.DK - at, dk_all[d]);
+        if (next.place >= places) return;
+        item = next;
+        if constexpr (BUFFERS == 1) {
+            fetch_slice(item, 0, lds[0].slice);
+            fetch_steps(item);
         }
     }
 }
@@ -456,9 +602,8 @@ template <typename T, int KS>
 void launch_backward(const DeltaArgs& p, hipStream_t stream) {
     launch_chunks<T, KS, true>(p, stream);
     delta_walk_back_kernel<T, KS><<<dim3(head_groups(p.N * p.HV, (p.DV + 63) / 64)), dim3(256), 0, stream>>>(p);
-    const dim3 grid = grid_of(static_cast<int64_t>(p.N) * p.H * p.chunks);
-    if (p.HV > p.H) delta_gradient_kernel<T, KS, true><<<grid, dim3(256), 0, stream>>>(p);
-    else delta_gradient_kernel<T, KS, false><<<grid, dim3(256), 0, stream>>>(p);
+    const int64_t places = static_cast<int64_t>(p.N) * p.H * p.chunks, units = compute_units();
+    delta_gradient_kernel<T, KS><<<dim3(static_cast<unsigned>(places < units ? places : units)), dim3(512), 0, stream>>>(p);
 }
 
 }  // namespace
