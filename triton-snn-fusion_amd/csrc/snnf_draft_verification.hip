@@ -3,8 +3,9 @@
 // probability r_i / sum r: r = p behind all drafts, max(p - q, 0) where one was turned down. So every token is distributed as p.
 // Two launches: (M, s) = (max x, sum exp((x - M) / temperature)) of every row, then the decisions and one more pass over the row that is drawn from. Bound by memory; few rows are
 // split over workgroups.
-// A decision is that of exact arithmetic: float32 gives each number with a bound of its error, and where two cannot be told apart (one test in some 10^5) the
-// workgroup goes over the rows again in float64.
+// A decision is that of exact arithmetic: float32 gives each number with a bound of its error, 10^-6, and where two cannot be told apart the workgroup goes over the rows again in
+// float64. That takes several times as long as the rest, so that the bound matters: exponents are products in two parts, sums are compensated. (In the sums, plain exponents will do: the slope's rounding is the same
+// for all and makes 2^-25.5 of the exponent, of which a sum has at most log2 V on average.)
 #include "snnf_sequence.h"
 
 namespace snnf {
@@ -12,7 +13,6 @@ namespace {
 
 constexpr int kMostDrafts = 64;
 constexpr int kMostSplits = 64;
-constexpr float kLog2e = 1.44269504088896340736f;
 
 struct VerifyArgs {
     const void *logits, *draft_logits;
@@ -26,7 +26,7 @@ struct VerifyArgs {
     int draw_splits, draw_span;         // and in the second
     float2* stats;                      // [request][row][split]: M, s
     uint64_t* largest;                  // [request][row][split]: key of the largest logit
-    float4* parts;                      // [request][split]: the two largest upper bounds, the largest lower bound, index
+    uint64_t* parts;                    // [request][split]: the two largest upper bounds; the largest lower bound, index
     uint32_t* arrived;                  // [request]
     int64_t* tokens;
     int32_t* accepted;
@@ -71,6 +71,22 @@ template <int VEC>
 __device__ __forceinline__ float sum_of(const float (&v)[VEC]) {        // in pairs: a thread adds few of these
     if constexpr (VEC == 8) return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
     else return (v[0] + v[1]) + (v[2] + v[3]);
+}
+
+// 1 / temperature in powers of two, as the sum of two numbers.
+struct Slope {
+    float high, low;
+};
+__device__ __forceinline__ Slope slope_of(float temperature) {
+    const double slope = 1.4426950408889634074 / temperature;
+    const float high = static_cast<float>(slope);
+    return {high, static_cast<float>(slope - high)};
+}
+// exp((x - M) / temperature): what the exponent's rounding loses is put back to first order. Off by some 2^-22, and by 2^-24 of the exponent where x - M is rounded.
+__device__ __forceinline__ float share_of(float x, float c, const Slope& slope) {
+    constexpr float kLn2 = 0.69314718055994530942f;
+    const float d = x - c, z = d * slope.high, e = __builtin_amdgcn_exp2f(z);
+    return e == 0.0f ? 0.0f : fmaf(e, fmaf(d, slope.low, fmaf(d, slope.high, -z)) * kLn2, e);
 }
 
 template <typename T, int BLOCK>
@@ -118,8 +134,8 @@ __global__ __launch_bounds__(BLOCK) void verify_rows_kernel(VerifyArgs p) {
         }
         return;
     }
-    const float slope = kLog2e / temperature;
-    float M = -INFINITY, s = 0.0f;
+    const Slope slope = slope_of(temperature);
+    float M = -INFINITY, s = 0.0f, lost = 0.0f;
     for (; at < end; at += BATCH * BLOCK * VEC) {
         float v[BATCH][VEC], most = M;
 #pragma unroll
@@ -132,20 +148,23 @@ __global__ __launch_bounds__(BLOCK) void verify_rows_kernel(VerifyArgs p) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) most = fmaxf(most, v[u][j]);
         const float c = center(most);
-        s *= __builtin_amdgcn_exp2f((M - c) * slope);
+        const float f = share_of(M, c, slope);
+        s *= f, lost *= f;
         M = most;
 #pragma unroll
         for (int u = 0; u < BATCH; ++u) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[u][j] = __builtin_amdgcn_exp2f((v[u][j] - c) * slope);
-            s += sum_of<VEC>(v[u]);
+            for (int j = 0; j < VEC; ++j) v[u][j] = __builtin_amdgcn_exp2f((v[u][j] - c) * slope.high);
+            const float more = sum_of<VEC>(v[u]) - lost, now_s = s + more;
+            lost = (now_s - s) - more;
+            s = now_s;
         }
     }
     const float most = lane_max(M);
     if (lane == 0) maxima[wave] = most;
     __syncthreads();
     const float all = lane_max(maxima[lane % WAVES], WAVES < 4 ? 4 : WAVES);
-    s = lane_sum(s * __builtin_amdgcn_exp2f((M - center(all)) * slope));
+    s = lane_sum(s * share_of(M, center(all), slope));
     if (lane == 0) sums[wave] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -155,8 +174,8 @@ __global__ __launch_bounds__(BLOCK) void verify_rows_kernel(VerifyArgs p) {
     }
 }
 
-// Relative error of exp2(z) / s in float32: 62 or 125 additions of a thread's vectors, the exponent's roundings.
-__device__ __forceinline__ float doubt(float z) { return 1.6e-5f + 2.4e-7f * fminf(fabsf(z), 1000.0f); }
+// Relative error of a share over the sum: 4 x 10^-7 of the sum's exponents, some 8 roundings, and that of x - M (of float32 logits).
+__device__ __forceinline__ float doubt(float d, const Slope& slope) { return 1.2e-6f + 6e-8f * fminf(fabsf(d * slope.high), 1000.0f); }
 
 // ------------------------------------------------------------------------------------------------------------------
 // In float64, by a workgroup
@@ -205,7 +224,7 @@ __device__ int exact_draw(const T* x, const T* y, int taken, int V, float M, flo
 // ------------------------------------------------------------------------------------------------------------------
 // Decisions and the draw
 // ------------------------------------------------------------------------------------------------------------------
-struct Race {                           // upper bounds of r / e: the two largest; the largest lower bound; index of the first
+struct Race {                           // upper bounds of r / e: the two largest; the largest lower bound; index of the first, the lowest of equal ones
     float first, second, lower;
     int index;
 };
@@ -220,6 +239,8 @@ __device__ __forceinline__ Race lane_race(Race v) {
         v = join(v, Race{__shfl_xor(v.first, mask, 64), __shfl_xor(v.second, mask, 64), __shfl_xor(v.lower, mask, 64), __shfl_xor(v.index, mask, 64)});
     return v;
 }
+
+__device__ __forceinline__ uint64_t two_words(float a, float b) { return static_cast<uint64_t>(__float_as_uint(b)) << 32 | __float_as_uint(a); }
 
 template <typename T>
 __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
@@ -236,19 +257,34 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
     const int length = drafts_of(p, n), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const float temperature = temperature_of(p, n);
     const bool greedy = !(temperature > 0.0f);
-    const float slope = greedy ? 0.0f : kLog2e / temperature;
+    const Slope slope = slope_of(greedy ? 1.0f : temperature);
+    // What the verdicts need of the drafts, sent for before the statistics.
+    int64_t drafted_here = -1;
+    float logit = 0.0f, theirs_logit = 0.0f, uniform = 0.0f;
+    if (static_cast<int>(threadIdx.x) < length) {
+        const int j = threadIdx.x;
+        drafted_here = p.drafts[static_cast<int64_t>(n) * p.K + j];
+        if (drafted_here >= 0 && drafted_here < p.V && !greedy) {
+            uniform = p.uniforms[static_cast<int64_t>(n) * p.K + j];
+            logit = to_float(row_of<T>(p, n, j)[drafted_here]);
+            if (p.draft_logits != nullptr) theirs_logit = to_float(row_of<T>(p, n, p.K + 1 + j)[drafted_here]);
+        }
+    }
     // Statistics of the request's rows, a thread to a row.
     for (int row = threadIdx.x; row < p.rows; row += BLOCK) {
         if (row <= p.K ? row > length : greedy || row - p.K - 1 >= length) continue;
         const int64_t at = (static_cast<int64_t>(n) * p.rows + row) * p.splits;
         if (greedy) {
             uint64_t best = p.largest[at];
+#pragma unroll 4
             for (int i = 1; i < p.splits; ++i) best = larger(best, p.largest[at + i]);
             largest[row] = best;
         } else {
             float M = -INFINITY, s = 0.0f;
+#pragma unroll 4
             for (int i = 0; i < p.splits; ++i) M = fmaxf(M, p.stats[at + i].x);
-            for (int i = 0; i < p.splits; ++i) s += p.stats[at + i].y * __builtin_amdgcn_exp2f((p.stats[at + i].x - center(M)) * slope);
+#pragma unroll 4
+            for (int i = 0; i < p.splits; ++i) s += p.stats[at + i].y * share_of(p.stats[at + i].x, center(M), slope);
             stats[row] = make_float2(M, s);
         }
     }
@@ -256,20 +292,17 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
     // The verdict on each draft.
     if (static_cast<int>(threadIdx.x) < length) {
         const int j = threadIdx.x;
-        const int64_t x = p.drafts[static_cast<int64_t>(n) * p.K + j];
         int verdict = kRefused;
-        if (x >= 0 && x < p.V) {
+        if (drafted_here >= 0 && drafted_here < p.V) {
             if (greedy) {
-                verdict = largest[j] != 0 && static_cast<int64_t>(~static_cast<uint32_t>(largest[j])) == x ? kTaken : kRefused;
+                verdict = largest[j] != 0 && static_cast<int64_t>(~static_cast<uint32_t>(largest[j])) == drafted_here ? kTaken : kRefused;
             } else {
-                const float z = (to_float(row_of<T>(p, n, j)[x]) - center(stats[j].x)) * slope;
-                const float mine = __builtin_amdgcn_exp2f(z) / stats[j].y, u = p.uniforms[static_cast<int64_t>(n) * p.K + j];
-                float theirs = u, unsure = doubt(z);
+                const float c = center(stats[j].x), mine = share_of(logit, c, slope) / stats[j].y;
+                float theirs = uniform, unsure = doubt(logit - c, slope);
                 if (p.draft_logits != nullptr) {
                     const float2 q = stats[p.K + 1 + j];
-                    const float z2 = (to_float(row_of<T>(p, n, p.K + 1 + j)[x]) - center(q.x)) * slope;
-                    theirs *= __builtin_amdgcn_exp2f(z2) / q.y;
-                    unsure += doubt(z2);
+                    theirs *= share_of(theirs_logit, center(q.x), slope) / q.y;
+                    unsure += doubt(theirs_logit - center(q.x), slope);
                 }
                 verdict = theirs < mine ? kTaken : kRefused;
                 if (fabsf(theirs - mine) <= unsure * (theirs + mine)) verdict = kDoubtful;
@@ -304,29 +337,51 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
         const int64_t drafted = taken < length ? p.drafts[static_cast<int64_t>(n) * p.K + taken] : -1;
         const float* noise = p.noise + n * p.noise_row;
         const float2 a = stats[taken], b = y != nullptr ? stats[p.K + 1 + taken] : make_float2(0.0f, 1.0f);
+        // A draft without a distribution that was turned down: p without it, since p is at most 1.
+        const int64_t passed = y == nullptr ? drafted : -1;
         const float c = center(a.x), c2 = center(b.x), part = 1.0f / a.y, part2 = 1.0f / b.y;
         const int begin = split * p.draw_span, end = begin + p.draw_span < p.V ? begin + p.draw_span : p.V;
         Race mine{0.0f, 0.0f, 0.0f, 0x7fffffff};
-        for (int at = begin + static_cast<int>(threadIdx.x) * VEC; at < end; at += BLOCK * VEC) {
-            Raw<T, VEC> raw, raw2;
-            Raw<float, 4> e[VEC / 4];
-            raw.load(x, at, end - at);
-            if (y != nullptr) raw2.load(y, at, end - at);
+        Raw<T, VEC> raw, raw2;
+        Raw<float, 4> e[VEC / 4];
+        float bar = 0.0f;
+        int at = begin + static_cast<int>(threadIdx.x) * VEC;
+        const auto fetch = [&](int from) {
+            raw.load(x, from, end - from);
+            if (y != nullptr) raw2.load(y, from, end - from);
 #pragma unroll
-            for (int u = 0; u < VEC / 4; ++u) e[u].load(noise, at + 4 * u, end - at - 4 * u);
+            for (int u = 0; u < VEC / 4; ++u) e[u].load(noise, from + 4 * u, end - from - 4 * u);
+        };
+        fetch(at);
+        for (int from = begin; from < end; from += BLOCK * VEC, at += BLOCK * VEC) {        // together: the wave shares what it has seen
+            float v[VEC], v2[VEC], inverse[VEC], rough[VEC];
+            const int left = end - at;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const float z = (raw[j] - c) * slope, share = __builtin_amdgcn_exp2f(z) * part;
-                float r = share, unsure = share * doubt(z);
-                if (y != nullptr) {
-                    const float z2 = (raw2[j] - c2) * slope, theirs = __builtin_amdgcn_exp2f(z2) * part2;
-                    r -= theirs;
-                    unsure = share > 0.0f ? fmaf(theirs, doubt(z2), unsure) : 0.0f;
-                } else if (at + j == drafted) {
-                    r = unsure = 0.0f;                       // p is at most 1
+                v[j] = j < left ? raw[j] : -INFINITY;
+                v2[j] = y != nullptr && j < left ? raw2[j] : -INFINITY;
+                inverse[j] = j < left ? __builtin_amdgcn_rcpf(e[j / 4][j % 4]) : 0.0f;
+            }
+            if (from + BLOCK * VEC < end) fetch(at + BLOCK * VEC);
+            // What the wave has seen beats most elements by far, by their shares without corrections, off by less than 2^-14.
+            constexpr float kRough = 6.2e-5f;
+            float least = 0.0f;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float share = __builtin_amdgcn_exp2f((v[j] - c) * slope.high) * part, theirs = y != nullptr ? __builtin_amdgcn_exp2f((v2[j] - c2) * slope.high) * part2 : 0.0f;
+                const float middle = at + j == passed ? 0.0f : (share - theirs) * inverse[j], width = (share + theirs) * (inverse[j] * kRough);
+                least = fmaxf(least, middle - width);
+                rough[j] = middle + width;
+            }
+            bar = fmaxf(bar, lane_max(least));
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                if (rough[j] >= bar && rough[j] > 0.0f && at + j != passed) {
+                    const float p1 = share_of(v[j], c, slope) * part, p2 = y != nullptr ? share_of(v2[j], c2, slope) * part2 : 0.0f;
+                    const float r = p1 - p2, unsure = fmaf(p1, doubt(v[j] - c, slope), p2 > 0.0f ? p2 * doubt(v2[j] - c2, slope) : 0.0f);
+                    const float upper = (r + unsure) * inverse[j];
+                    if (p1 > 0.0f && upper > 0.0f) mine = join(mine, Race{upper, 0.0f, (r - unsure) * inverse[j], at + j});
                 }
-                const float inverse = 1.0f / e[j / 4][j % 4], upper = (r + unsure) * inverse;
-                if (at + j < end && upper > 0.0f) mine = join(mine, Race{upper, 0.0f, (r - unsure) * inverse, at + j});
             }
         }
         mine = lane_race(mine);
@@ -334,18 +389,23 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
         __syncthreads();
         mine = join(join(races[0], races[1]), join(races[2], races[3]));
         if (p.draw_splits > 1) {
-            float4* parts = p.parts + static_cast<int64_t>(n) * p.draw_splits;
+            // Parts are written and read past the dies' own caches and counted once they have arrived (a fence in place of that, which empties a die's cache, took 23 of 45 us a
+            // workgroup at 256 x 128000).
+            uint64_t* parts = p.parts + static_cast<int64_t>(n) * p.draw_splits * 2;
             if (threadIdx.x == 0) {
-                parts[split] = make_float4(mine.first, mine.second, mine.lower, __int_as_float(mine.index));
-                last = __hip_atomic_fetch_add(p.arrived + n, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == static_cast<uint32_t>(p.draw_splits - 1);
+                __hip_atomic_store(parts + 2 * split, two_words(mine.first, mine.second), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(parts + 2 * split + 1, two_words(mine.lower, __int_as_float(mine.index)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+                last = __hip_atomic_fetch_add(p.arrived + n, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == static_cast<uint32_t>(p.draw_splits - 1);
             }
             __syncthreads();
             if (!last) return;
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
             mine = Race{0.0f, 0.0f, 0.0f, 0x7fffffff};
             if (lane < p.draw_splits) {
-                const float4 other = parts[lane];
-                mine = Race{other.x, other.y, other.z, __float_as_int(other.w)};
+                const uint64_t one = __hip_atomic_load(parts + 2 * lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                const uint64_t two = __hip_atomic_load(parts + 2 * lane + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                mine = Race{__uint_as_float(static_cast<uint32_t>(one)), __uint_as_float(static_cast<uint32_t>(one >> 32)), __uint_as_float(static_cast<uint32_t>(two)),
+                            static_cast<int>(two >> 32)};
             }
             mine = lane_race(mine);
         }
@@ -432,7 +492,7 @@ extern "C" int snnf_draft_verification(const void* logits, int64_t logits_row, i
     char* space = static_cast<char*>(workspace);
     p.stats = reinterpret_cast<float2*>(space);
     p.largest = reinterpret_cast<uint64_t*>(space += rounded(pieces * 8));
-    p.parts = reinterpret_cast<float4*>(space += rounded(pieces * 8));
+    p.parts = reinterpret_cast<uint64_t*>(space += rounded(pieces * 8));
     p.arrived = reinterpret_cast<uint32_t*>(space + static_cast<size_t>(N) * s.draw_splits * 16);
     p.tokens = tokens, p.accepted = accepted;
     hipStream_t hs = as_stream(stream);
