@@ -1,6 +1,7 @@
 // Parts of the gated delta rule's kernels: numbers as sums of bfloat16 terms for the matrix units, fragments, what forward and backward pass share.
 #pragma once
 
+#include <algorithm>
 #include <type_traits>
 
 #include "snnf_sequence.h"
@@ -113,6 +114,10 @@ struct DeltaArgs {
     uint16_t* deltas;                   // v - S k, [rank][64][value columns]
     uint16_t* later;                    // gradient of the state behind the chunk, as marks
     uint16_t* pulls;                    // Z, as deltas
+    // Few heads: chunks in segments of `per`, walked side by side
+    int segments, per;
+    float* transfers;                   // per head and segment but the last walked: what it makes of a state (below)
+    float* between;                     // per head and segment but the first: the state before it
 };
 
 // Of a chunk's block: 3 terms of the inverse's fragments, `ranks` of the scores', then exp(G), exp(G_64 - G), beta [64] each, whether any of the first two is 0, and zeros.
@@ -134,6 +139,9 @@ __host__ __device__ __forceinline__ constexpr int padded_values(int DV) { return
 template <int KS>
 __device__ __forceinline__ int mark_place(int column, int tile) { return (tile / 2 ^ (column & (KS - 1))) * 32 + 4 * (tile % 2); }
 inline int64_t mark_elements(int ranks, int KS, int DV) { return static_cast<int64_t>(ranks) * padded_values(DV) * 32 * KS; }
+// Of a segment: [32 KS rows][32 KS columns of the matrix that takes the state before it to the state behind it, then the value columns of what it adds], then whether the state before it is forgotten.
+__host__ __device__ __forceinline__ constexpr int transfer_columns(int KS, int DV) { return 32 * KS + padded_values(DV); }
+__host__ __device__ __forceinline__ constexpr int transfer_floats(int KS, int DV) { return 32 * KS * transfer_columns(KS, DV) + 4; }
 inline int64_t delta_elements(int ranks, int DV) { return static_cast<int64_t>(ranks) * kChunk * padded_values(DV); }
 
 __device__ __forceinline__ int length_of(const DeltaArgs& p, int n) {
@@ -142,11 +150,8 @@ __device__ __forceinline__ int length_of(const DeltaArgs& p, int n) {
     return length < 0 ? 0 : (length < p.T ? length : p.T);
 }
 
-// 8 elements of a row from `at` on, zeros behind its end.
 template <typename T>
-__device__ __forceinline__ Terms<kTerms<T>> row_terms(const T* row, int at, int width) {
-    Raw<T, 8> raw;
-    raw.load(row, at, width - at);
+__device__ __forceinline__ Terms<kTerms<T>> terms_of(const Raw<T, 8>& raw) {
     if constexpr (dtype_of<T>::value == SNNF_BF16) {
         Terms<1> r;
 #pragma unroll
@@ -158,6 +163,13 @@ __device__ __forceinline__ Terms<kTerms<T>> row_terms(const T* row, int at, int 
         for (int j = 0; j < 8; ++j) x[j] = raw[j];
         return split<kTerms<T>>(x);
     }
+}
+// 8 elements of a row from `at` on, zeros behind its end.
+template <typename T>
+__device__ __forceinline__ Terms<kTerms<T>> row_terms(const T* row, int at, int width) {
+    Raw<T, 8> raw;
+    raw.load(row, at, width - at);
+    return terms_of(raw);
 }
 template <int N>
 __device__ __forceinline__ Terms<N> no_terms() {
@@ -300,17 +312,7 @@ template <typename T, int KS, int THREADS>
 __device__ __forceinline__ void put_rows(const Staged<T, 4 * KS, THREADS>& x, uint16_t* lds) {
 #pragma unroll
     for (int i = 0; i < x.kCount; ++i) {
-        Terms<kTerms<T>> r;
-        if constexpr (dtype_of<T>::value == SNNF_BF16) {
-#pragma unroll
-            for (int w = 0; w < 4; ++w) r.t[0][w] = x.raw[i].w[w];
-        } else {
-            float v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = x.raw[i][j];
-            r = split<kTerms<T>>(v);
-        }
-        Rows<T, KS>::put(lds, threadIdx.x + i * THREADS, r);
+        Rows<T, KS>::put(lds, threadIdx.x + i * THREADS, terms_of(x.raw[i]));
     }
 }
 
@@ -442,26 +444,26 @@ template <int PIECES, int WAVES> struct StagedBlock {
             if (wave + i * WAVES < PIECES) *reinterpret_cast<u32x4a*>(lds + (wave + i * WAVES) * 256 + lane * 4) = words[i];
     }
 };
-// What a walk reads of a chunk: keys, queries, values (or the gradient of what is read) and the chunk's block; through registers...
-template <typename T, int KS, int WAVES, int PIECES> struct StagedChunk {
+// What a walk reads of a chunk: keys, queries, values (or the gradient of what is read) and the chunk's block, without queries and scores if not ALL; through registers...
+template <typename T, int KS, int WAVES, int PIECES, bool ALL> struct StagedChunk {
     Staged<T, 4 * KS, 64 * WAVES> k, q;
     Staged<T, 2 * WAVES, 64 * WAVES> v;
     StagedBlock<PIECES, WAVES> block;
     __device__ __forceinline__ void load(const DeltaArgs& p, const T* keys, const T* queries, const T* values, int64_t step, int rows, int width, const uint32_t* from) {
         k.load(keys, p.k.step, rows, p.DK, p.near_keys);
-        q.load(queries, p.q.step, rows, p.DK, p.near_keys);
+        if constexpr (ALL) q.load(queries, p.q.step, rows, p.DK, p.near_keys);
         v.load(values, step, rows, width, p.near_values);
         block.load(from);
     }
     __device__ __forceinline__ void store(uint16_t* keys, uint16_t* queries, T* tile, uint32_t* to) const {
         put_rows<T, KS, 64 * WAVES>(k, keys);
-        put_rows<T, KS, 64 * WAVES>(q, queries);
+        if constexpr (ALL) put_rows<T, KS, 64 * WAVES>(q, queries);
         Tile<T, WAVES>::put(tile, v);
         block.store(to);
     }
 };
 // ... or, with one term to an element, as they are, a chunk ahead into the other buffer: past the registers where rows are whole vectors, else through them at once.
-template <typename T, int KS, int WAVES, int PIECES> struct ChunkReader {
+template <typename T, int KS, int WAVES, int PIECES, bool ALL = true> struct ChunkReader {
     static constexpr bool kDirect = kTerms<T> == 1;
     static constexpr int kBuffers = kDirect ? 2 : 1;
     struct Buffers {
@@ -470,7 +472,7 @@ template <typename T, int KS, int WAVES, int PIECES> struct ChunkReader {
         uint32_t block[PIECES * 256];
     };
     struct Nothing {};
-    std::conditional_t<kDirect, Nothing, StagedChunk<T, KS, WAVES, PIECES>> next;
+    std::conditional_t<kDirect, Nothing, StagedChunk<T, KS, WAVES, PIECES, ALL>> next;
 
     __device__ __forceinline__ void fetch(const DeltaArgs& p, const T* keys, const T* queries, const T* values, int64_t step, int rows, int width, const uint32_t* block, Buffers& to) {
         if constexpr (!kDirect) {
@@ -480,13 +482,15 @@ template <typename T, int KS, int WAVES, int PIECES> struct ChunkReader {
             const uint32_t* zeros = block + block_vectors((PIECES - 1) / kBlocks - 3) + kZeros;
             if (p.near_keys) {
                 rows_to_lds<4 * KS, WAVES>(reinterpret_cast<const uint16_t*>(keys), p.k.step, rows, p.DK, zeros, to.keys);
-                rows_to_lds<4 * KS, WAVES>(reinterpret_cast<const uint16_t*>(queries), p.q.step, rows, p.DK, zeros, to.queries);
+                if constexpr (ALL) rows_to_lds<4 * KS, WAVES>(reinterpret_cast<const uint16_t*>(queries), p.q.step, rows, p.DK, zeros, to.queries);
             } else {
                 Staged<T, 4 * KS, 64 * WAVES> x;
                 x.load(keys, p.k.step, rows, p.DK, false);
                 put_rows<T, KS, 64 * WAVES>(x, to.keys);
-                x.load(queries, p.q.step, rows, p.DK, false);
-                put_rows<T, KS, 64 * WAVES>(x, to.queries);
+                if constexpr (ALL) {
+                    x.load(queries, p.q.step, rows, p.DK, false);
+                    put_rows<T, KS, 64 * WAVES>(x, to.queries);
+                }
             }
             if (p.near_values) {
                 rows_to_lds<2 * WAVES, WAVES>(reinterpret_cast<const uint16_t*>(values), step, rows, width, zeros, reinterpret_cast<uint16_t*>(to.tile));
@@ -498,7 +502,8 @@ template <typename T, int KS, int WAVES, int PIECES> struct ChunkReader {
             const uint32_t at = lds_address(to.block) + wave * 1024;
 #pragma unroll
             for (int i = 0; i < (PIECES + WAVES - 1) / WAVES; ++i)
-                if (wave + i * WAVES < PIECES) to_lds(block + (wave + i * WAVES) * 256, lane * 16u, at + i * WAVES * 1024);
+                if (wave + i * WAVES < PIECES && (ALL || wave + i * WAVES < kBlocks * 3 || wave + i * WAVES == PIECES - 1))
+                    to_lds(block + (wave + i * WAVES) * 256, lane * 16u, at + i * WAVES * 1024);
         }
     }
     // Has the chunk that was fetched last in LDS, for all waves; the one before it may be overwritten from then on.
@@ -548,6 +553,21 @@ __device__ __forceinline__ float decay_of(double x) {
     return ldexpf(__builtin_amdgcn_exp2f(static_cast<float>(x - whole)), static_cast<int>(whole < 1000.0 ? whole : 1000.0));
 }
 
+// The same for two sums as pairs of float32, without float64: the difference of the larger parts and what its rounding lost, exactly, then the smaller parts.
+struct Sum {
+    float large, small;
+};
+__device__ __forceinline__ Sum sum_of(double x) {
+    const float large = static_cast<float>(x);
+    return {large, static_cast<float>(x - large)};
+}
+__device__ __forceinline__ float decay_between(const Sum& from, const Sum& to) {
+    const float x = to.large - from.large, back = x - to.large;
+    const float lost = (to.large - (x - back)) - (from.large + back);
+    const float whole = __builtin_rintf(x), rest = (x - whole) + (lost + (to.small - from.small));
+    return x <= -160.0f ? 0.0f : ldexpf(__builtin_amdgcn_exp2f(rest), static_cast<int>(fminf(whole, 1000.0f)));
+}
+
 // Row i of a factor that a vanished decay has made 0 drops what it would multiply, infinities and NaN as well.
 __device__ __forceinline__ float kept(float factor, float x) { return factor == 0.0f ? 0.0f : factor * x; }
 
@@ -564,6 +584,13 @@ inline unsigned head_groups(int heads, int parts) { return static_cast<unsigned>
 
 // Fragments, decays and inverses of all chunks; transposed for the backward pass.
 template <typename T, int KS, bool BACKWARD> void launch_chunks(const DeltaArgs& p, hipStream_t stream);
+
+// Workgroups to a segment on its first walk, and what joins the states (backward: from the last segment on).
+inline int transfer_parts(int waves, int KS, int DV) { return (DV + 16 * waves - 1) / (16 * waves) + (2 * KS + waves - 1) / waves; }
+template <int KS> void launch_join(const DeltaArgs& p, bool backward, hipStream_t stream);
+int delta_segments(const snnf_delta_rule_call* call, bool backward);
+size_t delta_segment_floats(const snnf_delta_rule_call* call, bool backward);
+void set_segments(DeltaArgs& p, const snnf_delta_rule_call* call, bool backward, float* workspace);
 
 int check_delta(const char* name, const snnf_delta_rule_call* call);
 DeltaArgs delta_args(const snnf_delta_rule_call* call);

@@ -26,11 +26,14 @@ __device__ __forceinline__ f32x4 multiply_f32(const f32x4& a, const f32x4& b, f3
 }
 
 template <typename T, int KS, bool BACKWARD>
-__global__ __launch_bounds__(256, 2) void delta_chunk_kernel(DeltaArgs p) {
-    constexpr int RANKS = BACKWARD ? 3 : kOutputRanks<T>;
-    __shared__ float lower[kChunk * kPitch], inverse[kChunk * kPitch], scores[kChunk * kPitch];
-    __shared__ double total[kChunk];
-    __shared__ int part[kChunk];
+__global__ __launch_bounds__(256, kTerms<T> == 3 ? 2 : 4) void delta_chunk_kernel(DeltaArgs p) {
+    constexpr int RANKS = BACKWARD ? 3 : kOutputRanks<T>, TERMS = kTerms<T>;
+    constexpr int kMatrix = kChunk * kPitch, kFragments = 4 * KS * TERMS * 256;
+    __shared__ alignas(16) uint32_t shared[kFragments > 2 * kMatrix ? kFragments : 2 * kMatrix];     // keys, then the matrices
+    // L below the diagonal, the scores transposed above it, four columns to the right: score [i][c] at [c][i + 4]
+    float *both = reinterpret_cast<float*>(shared), *inverse = both + kMatrix;
+    __shared__ Sum total[kChunk];
+    __shared__ alignas(16) int part[kChunk];
     __shared__ float beta[kChunk];
     const uint32_t index = group_index();
     if (index >= static_cast<uint32_t>(p.N) * p.HV * p.chunks) return;
@@ -41,6 +44,34 @@ __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(DeltaArgs p) {
     uint32_t* blocks = p.blocks + static_cast<int64_t>(index) * block_words(RANKS);
     float* vectors = reinterpret_cast<float*>(blocks + block_vectors(RANKS));
 
+    // The wave's 16 rows; out of reach: the chunk's first, which is there, and zeros in their place
+    const T* keys = static_cast<const T*>(p.k.data) + n * p.k.row + h * p.k.head;
+    const T* queries = static_cast<const T*>(p.q.data) + n * p.q.row + h * p.q.head;
+    Raw<T, 8> k_raw[KS], q_raw[KS];
+    {
+        const int row = first + 16 * wave + column;
+        const auto rows = [&](const T* base, int64_t step, Raw<T, 8> (&x)[KS]) {
+            if (p.DK % 8 == 0) {
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const int at = 32 * s + 8 * group;
+                    x[s].load(base, row < limit && at < p.DK ? row * step + at : first * step, 8);
+                }
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+                    if (row >= limit || 32 * s + 8 * group >= p.DK) x[s].clear();
+            } else {
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const int at = 32 * s + 8 * group;
+                    if (row < limit && at < p.DK) x[s].load(base, row * step + at, p.DK - at);
+                    else x[s].clear();
+                }
+            }
+        };
+        rows(keys, p.k.step, k_raw);
+        rows(queries, p.q.step, q_raw);
+    }
     if (wave == 0) {
         const int t = first + lane;
         const bool there = t < limit;
@@ -54,7 +85,7 @@ __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(DeltaArgs p) {
             const double before = __shfl_up(sum, d, 64);
             if (lane >= d) sum += before;
         }
-        total[lane] = sum, part[lane] = mine, beta[lane] = b;
+        total[lane] = sum_of(sum), part[lane] = mine, beta[lane] = b;
         const double all = __shfl(sum, 63, 64);
         const int last = __shfl(mine, 63, 64);
         const float since = mine == 0 ? decay_of(sum) : 0.0f, until = mine == last ? decay_of(all - sum) : 0.0f;
@@ -64,39 +95,65 @@ __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(DeltaArgs p) {
         const bool broken = __ballot(since == 0.0f || until == 0.0f) != 0;
         vectors[kBroken + lane] = broken && lane == 0 ? 1.0f : 0.0f;
     }
-    const T* keys = static_cast<const T*>(p.k.data) + n * p.k.row + h * p.k.head;
-    const T* queries = static_cast<const T*>(p.q.data) + n * p.q.row + h * p.q.head;
     f32x4 kk[4], qk[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) kk[j] = qk[j] = f32x4{0, 0, 0, 0};
+    {
+        Terms<TERMS> k[KS], q[KS];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-        const int at = 32 * s + 8 * group, t = first + 16 * wave + column;
-        const bool there = t < limit && at < p.DK;
-        const auto k = there ? row_terms<T>(keys + t * p.k.step, at, p.DK) : no_terms<kTerms<T>>();
-        const auto q = there ? row_terms<T>(queries + t * p.q.step, at, p.DK) : no_terms<kTerms<T>>();
+        for (int s = 0; s < KS; ++s) {
+            k[s] = terms_of(k_raw[s]), q[s] = terms_of(q_raw[s]);
+#pragma unroll
+            for (int i = 0; i < TERMS; ++i) *reinterpret_cast<u32x4a*>(shared + ((wave * KS + s) * TERMS + i) * 256 + lane * 4) = k[s].t[i];
+        }
+        __syncthreads();
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (j > wave) break;
-            const int other = first + 16 * j + column;
-            const auto b = other < limit && at < p.DK ? row_terms<T>(keys + other * p.k.step, at, p.DK) : no_terms<kTerms<T>>();
-            kk[j] = product<3>(k, b, kk[j]);
-            qk[j] = product<3>(q, b, qk[j]);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                if (s % 2 == 0) now();
+                const Terms<TERMS> other = block_terms<TERMS>(shared, j * KS + s);
+                kk[j] = product<3>(k[s], other, kk[j]);
+                qk[j] = product<3>(q[s], other, qk[j]);
+            }
         }
     }
     __syncthreads();
+    {
+        const int row = 16 * wave + 4 * group;
+        Sum mine[4];
+        int segment[4];
+        float rate[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int c = 16 * j + column;
+        for (int r = 0; r < 4; ++r) mine[r] = total[row + r], segment[r] = part[row + r], rate[r] = beta[row + r];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int i = 16 * wave + 4 * group + r;
-            float d = 0.0f;
-            if (j <= wave && c <= i && part[i] == part[c]) d = decay_of(total[i] - total[c]);
-            const bool below = c < i && d != 0.0f;
-            lower[i * kPitch + c] = below ? d * kk[j][r] * beta[BACKWARD ? i : c] : 0.0f;
-            scores[i * kPitch + c] = d != 0.0f ? d * qk[j][r] * p.scale : 0.0f;
-            inverse[i * kPitch + c] = 0.0f;
+        for (int j = 0; j < 4; ++j) {
+            const int c = 16 * j + column;
+            if (j <= wave) {
+                const Sum other = total[c];
+                const int theirs = part[c];
+                const float theirs_rate = beta[c];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float d = decay_between(other, mine[r]);
+                    d = c <= row + r && segment[r] == theirs ? d : 0.0f;
+                    const float below = d * kk[j][r] * (BACKWARD ? rate[r] : theirs_rate);
+                    if (c < row + r) both[(row + r) * kPitch + c] = d != 0.0f ? below : 0.0f;
+                    qk[j][r] = d != 0.0f ? d * qk[j][r] * p.scale : 0.0f;
+                }
+                float* score = both + c * kPitch + row + 4;
+                if (j < wave) {
+                    *reinterpret_cast<f32x4*>(score) = qk[j];
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (c <= row + r) score[r] = qk[j][r];
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) inverse[(row + r) * kPitch + c] = 0.0f;
+            now();
         }
     }
     __syncthreads();
@@ -104,12 +161,13 @@ __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(DeltaArgs p) {
     {
         float x[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float v = i == column ? 1.0f : 0.0f;
-            const float* row = lower + (16 * wave + i) * kPitch + 16 * wave;
+        for (int i = 0; i < 16; ++i) x[i] = i == column ? 1.0f : 0.0f;
+        // four columns of the block at a time
 #pragma unroll
-            for (int j = 0; j < i; ++j) v = fmaf(-row[j], x[j], v);
-            x[i] = v;
+        for (int j = 0; j < 15; ++j) {
+            if (j % 4 == 0) now();
+#pragma unroll
+            for (int i = j + 1; i < 16; ++i) x[i] = fmaf(-both[(16 * wave + i) * kPitch + 16 * wave + j], x[j], x[i]);
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -127,7 +185,7 @@ __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(DeltaArgs p) {
                 f32x4 b;
 #pragma unroll
                 for (int s = 0; s < 4; ++s) b[s] = inverse[(16 * k + 4 * group + s) * kPitch + 16 * j + column];
-                sum = multiply_f32(block_row(lower, wave, k), b, sum);
+                sum = multiply_f32(block_row(both, wave, k), b, sum);
             }
             corner = multiply_f32(block_row(inverse, wave, wave), sum, corner);
 #pragma unroll
@@ -135,21 +193,21 @@ __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(DeltaArgs p) {
         }
         __syncthreads();
     }
-    // Fragments as the other kernels load them.
-    const auto fragment = [&](const float* m, int f) {
-        if constexpr (BACKWARD) {
-            const float* from = m + (32 * upper_half(f) + 4 * group) * kPitch + 16 * upper_tile(f) + column;
-            float x[8];
+    // Fragments as the other kernels load them: a row of one matrix, a column of the other
+    const auto place = [&](int e) { return 4 * group + (e < 4 ? e : 12 + e); };
+    const auto fragment = [&](const float* m, int f, bool transposed, int shift) {
+        const int line = 16 * (BACKWARD ? upper_tile(f) : lower_tile(f)) + column, from = 32 * (BACKWARD ? upper_half(f) : lower_half(f));
+        float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = from[(e < 4 ? e : 12 + e) * kPitch];
-            return split<3>(x);
-        } else {
-            const float* from = m + (16 * lower_tile(f) + column) * kPitch + 32 * lower_half(f) + 4 * group;
-            return split<3>(*reinterpret_cast<const f32x4*>(from), *reinterpret_cast<const f32x4*>(from + 16));
+        for (int e = 0; e < 8; ++e) x[e] = transposed ? m[(from + place(e)) * kPitch + line + shift] : m[line * kPitch + from + place(e) + shift];
+        if (shift > 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = (BACKWARD ? line <= from + place(e) : from + place(e) <= line) ? x[e] : 0.0f;
         }
+        return split<3>(x);
     };
     for (int f = wave; f < kBlocks; f += 4) {
-        const Terms<3> x = fragment(inverse, f), y = fragment(scores, f);
+        const Terms<3> x = fragment(inverse, f, BACKWARD, 0), y = fragment(both, f, !BACKWARD, 4);
 #pragma unroll
         for (int i = 0; i < 3; ++i) *reinterpret_cast<u32x4a*>(blocks + (f * 3 + i) * 256 + lane * 4) = x.t[i];
 #pragma unroll
@@ -162,40 +220,54 @@ __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(DeltaArgs p) {
 // ------------------------------------------------------------------------------------------------------------------
 // A wave owns 16 columns of the state, in accumulators, and of everything that is multiplied from it on: products go over the heads' elements
 // or over steps, whose place in an accumulator is a matter of the other operand's order, so that nothing but keys, queries and what crosses the kernel's edge passes through LDS.
-template <typename T, int KS, int WAVES, bool TRAIN>
-__global__ __launch_bounds__(kTerms<T> == 1 && !TRAIN ? 512 : 64 * WAVES) void delta_walk_kernel(DeltaArgs p) {
+// Few heads leave most of the chip idle, so that their chunks are cut into segments. What a segment does to a state S is A S + B: A is where it takes the identity, with values of 0, B where it
+// takes no state at all. kTransfer walks the segments for both, side by side; the states between them follow (`delta_join_kernel`), and a second walk over all segments has its states at once.
+enum Walk { kOutputs, kTraining, kTransfer };
+
+template <typename T, int KS, int WAVES, Walk WALK>
+__global__ __launch_bounds__(kTerms<T> == 1 && WALK != kTraining ? 512 : 64 * WAVES) void delta_walk_kernel(DeltaArgs p) {
     using Lds = Rows<T, KS>;
     using Values = Tile<T, WAVES>;
     constexpr int RANKS = kOutputRanks<T>, TERMS = kTerms<T>, PIPE = TERMS == 1 ? 2 : 1;
-    using Reader = ChunkReader<T, KS, WAVES, block_pieces(RANKS)>;
+    constexpr bool TRAIN = WALK == kTraining, TRANSFER = WALK == kTransfer;
+    using Reader = ChunkReader<T, KS, WAVES, block_pieces(RANKS), !TRANSFER>;
     __shared__ alignas(16) typename Reader::Buffers lds[Reader::kBuffers];
-    int head, columns;
-    if (!part_of_head(p.N * p.HV, (p.DV + Values::kColumns - 1) / Values::kColumns, &head, &columns)) return;
-    const int n = head / p.HV, hv = head % p.HV, h = hv / (p.HV / p.H), limit = length_of(p, n), live = (limit + kChunk - 1) / kChunk;
+    const int value_parts = (p.DV + Values::kColumns - 1) / Values::kColumns, segments = TRANSFER ? p.segments - 1 : p.segments;
+    int item, columns;
+    if (!part_of_head(p.N * p.HV * segments, TRANSFER ? value_parts + (32 * KS + Values::kColumns - 1) / Values::kColumns : value_parts, &item, &columns)) return;
+    const int head = item / segments, segment = item % segments, n = head / p.HV, hv = head % p.HV, h = hv / (p.HV / p.H), limit = length_of(p, n);
+    const int chunks = (limit + kChunk - 1) / kChunk, begin = segment * p.per, last = chunks == 0 ? 0 : (chunks - 1) / p.per;
+    const int live = segment < last ? begin + p.per : chunks;
+    const bool matrix = TRANSFER && columns >= value_parts;
+    if (segment > last || (TRANSFER && (segment == last || (matrix && segment == 0)))) return;      // the first segment's state is known
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane / 16;
-    const int left = columns * Values::kColumns, mine = left + 16 * wave, column = mine + lane % 16;
-    const bool there = column < p.DV;
+    const int left = (matrix ? columns - value_parts : columns) * Values::kColumns, mine = left + 16 * wave, column = mine + lane % 16;
+    const bool there = column < (matrix ? 32 * KS : p.DV);
     const int64_t cell = static_cast<int64_t>(head) * p.DK * p.DV + column;
+    const float* before = nullptr;
+    if (segment == 0) before = p.state == nullptr ? nullptr : p.state + cell;
+    else if constexpr (!TRANSFER) before = p.between + (static_cast<int64_t>(head) * (segments - 1) + segment - 1) * p.DK * p.DV + column;
     f32x4 state[2 * KS];
 #pragma unroll
     for (int d = 0; d < 2 * KS; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int row = head_element(d, r);
-            state[d][r] = p.state != nullptr && there && row < p.DK ? p.state[cell + static_cast<int64_t>(row) * p.DV] : 0.0f;
+            state[d][r] = before != nullptr && there && row < p.DK ? before[static_cast<int64_t>(row) * p.DV] : (matrix && row == column ? 1.0f : 0.0f);
         }
+    bool forgotten = false;
     const T* k_base = static_cast<const T*>(p.k.data) + n * p.k.row + h * p.k.head;
     const T* q_base = static_cast<const T*>(p.q.data) + n * p.q.row + h * p.q.head;
-    const T* v_base = static_cast<const T*>(p.v.data) + n * p.v.row + hv * p.v.head + left;
+    const T* v_base = static_cast<const T*>(p.v.data) + n * p.v.row + hv * p.v.head + (matrix ? 0 : left);
     T* out_base = static_cast<T*>(const_cast<void*>(p.out.data)) + n * p.out.row + hv * p.out.head + mine;
     Reader reader;
     const auto fetch = [&](int chunk) {
         const int64_t first = static_cast<int64_t>(chunk) * kChunk;
-        if (chunk < live) reader.fetch(p, k_base + first * p.k.step, q_base + first * p.q.step, v_base + first * p.v.step, p.v.step, limit - chunk * kChunk, p.DV - left,
+        if (chunk < live) reader.fetch(p, k_base + first * p.k.step, q_base + first * p.q.step, v_base + first * p.v.step, p.v.step, limit - chunk * kChunk, matrix ? 0 : p.DV - left,
                      p.blocks + (static_cast<int64_t>(head) * p.chunks + chunk) * block_words(RANKS), lds[chunk % Reader::kBuffers]);
     };
-    fetch(0);
-    for (int chunk = 0; chunk < live; ++chunk) {
+    fetch(begin);
+    for (int chunk = begin; chunk < live; ++chunk) {
         const int64_t index = static_cast<int64_t>(head) * p.chunks + chunk;
         typename Reader::Buffers& here = lds[chunk % Reader::kBuffers];
         const uint16_t *keys = here.keys, *queries = here.queries;
@@ -212,7 +284,10 @@ __global__ __launch_bounds__(kTerms<T> == 1 && !TRAIN ? 512 : 64 * WAVES) void d
         Terms<3> x[2] = {split<3>(state[0], state[1]), {}}, inverse[kBlocks];
         const auto load = [&](int s) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a[s % PIPE][i] = Lds::rows(keys, i, s), a[s % PIPE][4 + i] = Lds::rows(queries, i, s);
+            for (int i = 0; i < 4; ++i) {
+                a[s % PIPE][i] = Lds::rows(keys, i, s);
+                if constexpr (!TRANSFER) a[s % PIPE][4 + i] = Lds::rows(queries, i, s);
+            }
         };
         load(0);
 #pragma unroll
@@ -237,7 +312,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 && !TRAIN ? 512 : 64 * WAVES) void d
                         for (int i = 0; i < 4; ++i) ks[i] = mfma(a[s % PIPE][i].t[j], x[s % 2].t[rank - j], ks[i]);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (rank < RANKS) out[i] = mfma(a[s % PIPE][4 + i].t[j], x[s % 2].t[rank - j], out[i]);
+                            if (!TRANSFER && rank < RANKS) out[i] = mfma(a[s % PIPE][4 + i].t[j], x[s % 2].t[rank - j], out[i]);
                     }
             if constexpr (TRAIN) {
                 uint16_t* marks = p.marks + index * (kMarkRanks<T> * padded_values(p.DV) * 32 * KS);
@@ -249,6 +324,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 && !TRAIN ? 512 : 64 * WAVES) void d
         }
         const bool broken = __builtin_amdgcn_readfirstlane(vectors[kBroken]) != 0;
         const float rest = __uint_as_float(__builtin_amdgcn_readfirstlane(vectors[kSince + kChunk - 1]));
+        if constexpr (TRANSFER) forgotten = forgotten || rest == 0.0f;
         if (broken) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) drop(ks[i], since[i]), drop(out[i], since[i]);
@@ -279,7 +355,8 @@ __global__ __launch_bounds__(kTerms<T> == 1 && !TRAIN ? 512 : 64 * WAVES) void d
 #pragma unroll
             for (int d = 0; d < 2 * KS; ++d) state[d] *= rest;
 #pragma unroll
-            for (int f = 0; f < kBlocks; ++f) scores[f] = block_terms<RANKS>(block + kBlocks * 3 * 256, f);
+            for (int f = 0; f < kBlocks; ++f)
+                if constexpr (!TRANSFER) scores[f] = block_terms<RANKS>(block + kBlocks * 3 * 256, f);
         }
         if constexpr (TRAIN) Values::template write_terms<RANKS>(tile, delta, p.deltas + index * (RANKS * kChunk * padded_values(p.DV)) + mine, padded_values(p.DV));
         // What the steps read of each other, and the state behind them
@@ -307,7 +384,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 && !TRAIN ? 512 : 64 * WAVES) void d
             };
             columns_of(0);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
+            for (int half = 0; half < 2 && !TRANSFER; ++half) {
                 const Terms<RANKS> y = split<RANKS>(delta[2 * half], delta[2 * half + 1]);
 #pragma unroll
                 for (int rank = RANKS - 1; rank >= 0; --rank)
@@ -331,20 +408,110 @@ __global__ __launch_bounds__(kTerms<T> == 1 && !TRAIN ? 512 : 64 * WAVES) void d
                             for (int d = 0; d < 2 * KS; ++d) state[d] = mfma(k[half % PIPE][d].t[j], y.t[rank - j], state[d]);
                         }
             }
-            Values::turn_values(tile, out);
+            if constexpr (!TRANSFER) Values::turn_values(tile, out);
         }
         now();
-        Values::write(tile, out_base + static_cast<int64_t>(chunk) * kChunk * p.out.step, p.out.step, p.T - chunk * kChunk, limit - chunk * kChunk, p.DV - mine, p.near_values);
+        if constexpr (!TRANSFER) Values::write(tile, out_base + static_cast<int64_t>(chunk) * kChunk * p.out.step, p.out.step, p.T - chunk * kChunk, limit - chunk * kChunk, p.DV - mine, p.near_values);
     }
-    for (int t = live * kChunk + wave * 4 + group; t < p.T; t += 4 * WAVES)      // padding
-        for (int c = left + lane % 16; c < p.DV && c < left + Values::kColumns; c += 16) out_base[t * p.out.step + c - mine] = from_float<T>(0.0f);
+    if constexpr (TRANSFER) {
+        float* to = p.transfers + static_cast<int64_t>(item) * transfer_floats(KS, p.DV);
+        const int at = matrix ? column : 32 * KS + column;
 #pragma unroll
-    for (int d = 0; d < 2 * KS; ++d)
+        for (int d = 0; d < 2 * KS; ++d)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = head_element(d, r);
-            if (there && row < p.DK) p.state_out[cell + static_cast<int64_t>(row) * p.DV] = state[d][r];
+            for (int r = 0; r < 4; ++r)
+                if (there) to[head_element(d, r) * transfer_columns(KS, p.DV) + at] = state[d][r];
+        if (matrix && columns == value_parts && threadIdx.x == 0) to[transfer_floats(KS, p.DV) - 4] = forgotten ? 1.0f : 0.0f;
+    } else if (segment == last) {
+        for (int t = chunks * kChunk + wave * 4 + group; t < p.T; t += 4 * WAVES)      // padding
+            for (int c = left + lane % 16; c < p.DV && c < left + Values::kColumns; c += 16) out_base[t * p.out.step + c - mine] = from_float<T>(0.0f);
+#pragma unroll
+        for (int d = 0; d < 2 * KS; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = head_element(d, r);
+                if (there && row < p.DK) p.state_out[cell + static_cast<int64_t>(row) * p.DV] = state[d][r];
+            }
+    }
+}
+
+// The states between a head's segments, one after the other: 16 columns to a workgroup, 32 of the rows that are summed over to a wave. Products in float32, whose operands are what
+// memory and accumulators hold.
+template <int KS>
+__global__ __launch_bounds__(64 * KS) void delta_join_kernel(DeltaArgs p, int backward) {
+    __shared__ f32x4 parts[2][KS][2 * KS][64];
+    int head, tile;
+    if (!part_of_head(p.N * p.HV, (p.DV + 15) / 16, &head, &tile)) return;
+    const int n = head / p.HV, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, column = 16 * tile + lane % 16, width = transfer_columns(KS, p.DV);
+    const int chunks = (length_of(p, n) + kChunk - 1) / kChunk, last = chunks == 0 ? 0 : (chunks - 1) / p.per;
+    const float* transfers = p.transfers + static_cast<int64_t>(head) * (p.segments - 1) * transfer_floats(KS, p.DV);
+    float* between = p.between + static_cast<int64_t>(head) * (p.segments - 1) * p.DK * p.DV;
+    // Rows of the matrix as the accumulators have them, the wave's columns of it as they lie in the other operand; what the segment adds to the wave's own rows
+    struct Segment {
+        f32x4 matrix[2 * KS][2];
+        f32x4 added[2];
+        float forgotten;
+    };
+    const auto load = [&](Segment& x, int step) {
+        step = step < last ? step : last - 1;
+        const float* from = transfers + static_cast<int64_t>(backward ? last - 1 - step : step) * transfer_floats(KS, p.DV);
+        x.forgotten = from[transfer_floats(KS, p.DV) - 4];
+#pragma unroll
+        for (int d = 0; d < 2 * KS; ++d)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int row = 32 * (d / 2) + 8 * (lane % 16 / 4) + 4 * (d % 2) + lane % 4;
+                x.matrix[d][i] = *reinterpret_cast<const f32x4*>(from + row * width + 32 * wave + 8 * (lane / 16) + 4 * i);
+            }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x.added[i][r] = from[head_element(2 * wave + i, r) * width + 32 * KS + column];
+        now();
+    };
+    f32x4 state[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    const auto advance = [&](const Segment& x, int step) {
+        if (step >= last) return;
+        if (step > 0) {
+            f32x4 sums[2 * KS];
+#pragma unroll
+            for (int d = 0; d < 2 * KS; ++d) sums[d] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float s = x.forgotten == 0.0f ? state[i][r] : 0.0f;       // an infinite state as well
+#pragma unroll
+                    for (int d = 0; d < 2 * KS; ++d) sums[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.matrix[d][i][r], s, sums[d], 0, 0, 0);
+                }
+#pragma unroll
+            for (int d = 0; d < 2 * KS; ++d) parts[step % 2][wave][d][lane] = sums[d];
         }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            state[i] = x.added[i];
+            if (step > 0) {
+#pragma unroll
+                for (int w = 0; w < KS; ++w) state[i] += parts[step % 2][w][2 * wave + i][lane];
+            }
+            float* to = between + static_cast<int64_t>(backward ? last - 1 - step : step) * p.DK * p.DV;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = head_element(2 * wave + i, r);
+                if (row < p.DK && column < p.DV) to[row * p.DV + column] = state[i][r];
+            }
+        }
+    };
+    if (last == 0) return;
+    Segment even, odd;
+    load(even, 0);
+    for (int step = 0; step < last; step += 2) {
+        load(odd, step + 1);
+        advance(even, step);
+        load(even, step + 2);
+        advance(odd, step + 1);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -456,9 +623,9 @@ constexpr int kFewSteps = 16;
 
 template <typename T, int KS, int WAVES>
 void launch_walk(const DeltaArgs& p, hipStream_t stream) {
-    const dim3 grid(head_groups(p.N * p.HV, (p.DV + 16 * WAVES - 1) / (16 * WAVES))), block(64 * WAVES);
-    if (p.marks != nullptr) delta_walk_kernel<T, KS, WAVES, true><<<grid, block, 0, stream>>>(p);
-    else delta_walk_kernel<T, KS, WAVES, false><<<grid, block, 0, stream>>>(p);
+    const dim3 grid(head_groups(p.N * p.HV * p.segments, (p.DV + 16 * WAVES - 1) / (16 * WAVES))), block(64 * WAVES);
+    if (p.marks != nullptr) delta_walk_kernel<T, KS, WAVES, kTraining><<<grid, block, 0, stream>>>(p);
+    else delta_walk_kernel<T, KS, WAVES, kOutputs><<<grid, block, 0, stream>>>(p);
 }
 
 template <typename T, int KS>
@@ -468,6 +635,11 @@ void launch_forward(const DeltaArgs& p, hipStream_t stream) {
         return;
     }
     launch_chunks<T, KS, false>(p, stream);
+    if (p.segments > 1) {
+        constexpr int WAVES = sizeof(T) == 2 ? 8 : 4;
+        delta_walk_kernel<T, KS, WAVES, kTransfer><<<dim3(head_groups(p.N * p.HV * (p.segments - 1), transfer_parts(WAVES, KS, p.DV))), dim3(64 * WAVES), 0, stream>>>(p);
+        launch_join<KS>(p, false, stream);
+    }
     if constexpr (sizeof(T) == 2) {
         if (eight_waves(p)) {
             launch_walk<T, KS, 8>(p, stream);
@@ -478,6 +650,36 @@ void launch_forward(const DeltaArgs& p, hipStream_t stream) {
 }
 
 }  // namespace
+
+template <int KS>
+void launch_join(const DeltaArgs& p, bool backward, hipStream_t stream) {
+    delta_join_kernel<KS><<<dim3(head_groups(p.N * p.HV, (p.DV + 15) / 16)), dim3(64 * KS), 0, stream>>>(p, backward);
+}
+template void launch_join<2>(const DeltaArgs&, bool, hipStream_t);
+template void launch_join<4>(const DeltaArgs&, bool, hipStream_t);
+
+int delta_segments(const snnf_delta_rule_call* c, bool backward) {
+    const int64_t heads = static_cast<int64_t>(c->N) * c->value_heads, chunks = (c->T + kChunk - 1) / kChunk, units = compute_units();
+    if (heads == 0 || heads > units) return 1;
+    const int waves = dtype_size(c->dtype) == 2 && !backward ? 8 : 4;
+    int64_t segments = 1 + units / (heads * transfer_parts(waves, c->key_size <= 64 ? 2 : 4, c->value_size));
+    segments = std::min(segments, units / (heads * ((c->value_size + 63) / 64)));
+    segments = std::min(segments, chunks / 3);
+    while (segments * segments > 8 * chunks) --segments;
+    if (segments < 3) return 1;
+    const int64_t per = (chunks + segments - 1) / segments;
+    return static_cast<int>((chunks + per - 1) / per);
+}
+size_t delta_segment_floats(const snnf_delta_rule_call* c, bool backward) {
+    return static_cast<size_t>(c->N) * c->value_heads * (delta_segments(c, backward) - 1) *
+           (transfer_floats(c->key_size <= 64 ? 2 : 4, c->value_size) + static_cast<size_t>(c->key_size) * c->value_size);
+}
+void set_segments(DeltaArgs& p, const snnf_delta_rule_call* c, bool backward, float* workspace) {
+    p.segments = delta_segments(c, backward);
+    p.per = (p.chunks + p.segments - 1) / p.segments;
+    p.transfers = workspace;
+    p.between = workspace + static_cast<int64_t>(p.N) * p.HV * (p.segments - 1) * transfer_floats(c->key_size <= 64 ? 2 : 4, p.DV);
+}
 
 template <typename T, int KS, bool BACKWARD>
 void launch_chunks(const DeltaArgs& p, hipStream_t stream) {
@@ -537,7 +739,7 @@ using namespace snnf;
 
 extern "C" size_t snnf_delta_rule_workspace_bytes(const snnf_delta_rule_call* call, int training) {
     if (check_delta("snnf_delta_rule_workspace_bytes", call) != SNNF_OK || (!training && call->T <= kFewSteps)) return 0;
-    return static_cast<size_t>(delta_chunks(call)) * block_words(delta_ranks(call)) * 4;
+    return static_cast<size_t>(delta_chunks(call)) * block_words(delta_ranks(call)) * 4 + delta_segment_floats(call, false) * 4;
 }
 
 extern "C" size_t snnf_delta_rule_marks_bytes(const snnf_delta_rule_call* call) {
@@ -560,6 +762,7 @@ extern "C" int snnf_delta_rule(const snnf_delta_rule_call* call, const snnf_head
         if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
             return fail(SNNF_ERR_WORKSPACE, "snnf_delta_rule: workspace of %zu bytes needed, got %zu", need, workspace_bytes);
         p.blocks = static_cast<uint32_t*>(workspace);
+        set_segments(p, call, false, reinterpret_cast<float*>(p.blocks + delta_chunks(call) * block_words(delta_ranks(call))));
     }
     if (marks != nullptr) {
         p.marks = static_cast<uint16_t*>(marks);

@@ -15,40 +15,51 @@ namespace {
 // ------------------------------------------------------------------------------------------------------------------
 // The walk back
 // ------------------------------------------------------------------------------------------------------------------
-template <typename T, int KS>
+// In segments where heads are few, as the walk forward: a segment's effect on R is A^T R + B, and a first walk (TRANSFER) takes the identity and no gradient of its outputs for A^T, the
+// gradient of its outputs and no R for B.
+template <typename T, int KS, bool TRANSFER>
 __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_kernel(DeltaArgs p) {
     constexpr int WAVES = 4, RANKS = kOutputRanks<T>, TERMS = kTerms<T>, PIPE = TERMS == 1 ? 2 : 1;
     using Lds = Rows<T, KS>;
     using Values = Tile<T, WAVES>;
     using Reader = ChunkReader<T, KS, WAVES, block_pieces(3)>;
     __shared__ alignas(16) typename Reader::Buffers lds[Reader::kBuffers];
-    int head, columns;
-    if (!part_of_head(p.N * p.HV, (p.DV + 63) / 64, &head, &columns)) return;
-    const int n = head / p.HV, hv = head % p.HV, h = hv / (p.HV / p.H), limit = length_of(p, n), live = (limit + kChunk - 1) / kChunk;
+    const int value_parts = (p.DV + Values::kColumns - 1) / Values::kColumns, segments = TRANSFER ? p.segments - 1 : p.segments;
+    int item, columns;
+    if (!part_of_head(p.N * p.HV * segments, TRANSFER ? value_parts + (2 * KS + WAVES - 1) / WAVES : value_parts, &item, &columns)) return;
+    const int head = item / segments, segment = item % segments + TRANSFER, n = head / p.HV, hv = head % p.HV, h = hv / (p.HV / p.H), limit = length_of(p, n);
+    const int chunks = (limit + kChunk - 1) / kChunk, begin = segment * p.per, last = chunks == 0 ? 0 : (chunks - 1) / p.per;
+    const int live = segment < last ? begin + p.per : chunks;
+    const bool matrix = TRANSFER && columns >= value_parts;
+    if (segment > last || (matrix && segment == last)) return;      // what comes behind the last segment is known
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane / 16;
-    const int left = columns * Values::kColumns, mine = left + 16 * wave, column = mine + lane % 16;
-    const bool there = column < p.DV;
+    const int left = (matrix ? columns - value_parts : columns) * Values::kColumns, mine = left + 16 * wave, column = mine + lane % 16;
+    const bool there = column < (matrix ? 32 * KS : p.DV);
     const int64_t cell = static_cast<int64_t>(head) * p.DK * p.DV + column;
+    const float* behind = nullptr;
+    if (segment == last) behind = p.dstate == nullptr ? nullptr : p.dstate + cell;
+    else if constexpr (!TRANSFER) behind = p.between + (static_cast<int64_t>(head) * (segments - 1) + segment) * p.DK * p.DV + column;
     f32x4 later[2 * KS];
 #pragma unroll
     for (int d = 0; d < 2 * KS; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int row = head_element(d, r);
-            later[d][r] = p.dstate != nullptr && there && row < p.DK ? p.dstate[cell + static_cast<int64_t>(row) * p.DV] : 0.0f;
+            later[d][r] = behind != nullptr && there && row < p.DK ? behind[static_cast<int64_t>(row) * p.DV] : (matrix && row == column ? 1.0f : 0.0f);
         }
+    bool forgotten = false;
     const T* k_base = static_cast<const T*>(p.k.data) + n * p.k.row + h * p.k.head;
     const T* q_base = static_cast<const T*>(p.q.data) + n * p.q.row + h * p.q.head;
-    const T* o_base = static_cast<const T*>(p.dout.data) + n * p.dout.row + hv * p.dout.head + left;
+    const T* o_base = static_cast<const T*>(p.dout.data) + n * p.dout.row + hv * p.dout.head + (matrix ? 0 : left);
     T* v_base = static_cast<T*>(const_cast<void*>(p.dv.data)) + n * p.dv.row + hv * p.dv.head + mine;
     Reader reader;
     const auto fetch = [&](int chunk) {
         const int64_t first = static_cast<int64_t>(chunk) * kChunk;
-        if (chunk >= 0) reader.fetch(p, k_base + first * p.k.step, q_base + first * p.q.step, o_base + first * p.dout.step, p.dout.step, limit - chunk * kChunk, p.DV - left,
+        if (chunk >= begin) reader.fetch(p, k_base + first * p.k.step, q_base + first * p.q.step, o_base + first * p.dout.step, p.dout.step, limit - chunk * kChunk, matrix ? 0 : p.DV - left,
                                      p.blocks + (static_cast<int64_t>(head) * p.chunks + chunk) * block_words(3), lds[chunk % Reader::kBuffers]);
     };
     fetch(live - 1);
-    for (int chunk = live - 1; chunk >= 0; --chunk) {
+    for (int chunk = live - 1; chunk >= begin; --chunk) {
         const int64_t index = static_cast<int64_t>(head) * p.chunks + chunk;
         typename Reader::Buffers& here = lds[chunk % Reader::kBuffers];
         const uint16_t *keys = here.keys, *queries = here.queries;
@@ -72,10 +83,12 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
             if (PIPE == 2 && s + 1 < KS) load(s + 1);
             now();
             const Terms<3> x = split<3>(later[2 * s], later[2 * s + 1]);
-            uint16_t* marks = p.later + index * (kMarkRanks<T> * padded_values(p.DV) * 32 * KS);
+            if constexpr (!TRANSFER) {
+                uint16_t* marks = p.later + index * (kMarkRanks<T> * padded_values(p.DV) * 32 * KS);
 #pragma unroll
-            for (int r = 0; r < kMarkRanks<T>; ++r)
-                *reinterpret_cast<u32x4a*>(marks + static_cast<uint32_t>((r * padded_values(p.DV) + column) * 32 * KS + mark_place<KS>(column, 2 * s) + 8 * group)) = x.t[r];
+                for (int r = 0; r < kMarkRanks<T>; ++r)
+                    *reinterpret_cast<u32x4a*>(marks + static_cast<uint32_t>((r * padded_values(p.DV) + column) * 32 * KS + mark_place<KS>(column, 2 * s) + 8 * group)) = x.t[r];
+            }
 #pragma unroll
             for (int rank = 2; rank >= 0; --rank)
 #pragma unroll
@@ -88,6 +101,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
         }
         const bool broken = __builtin_amdgcn_readfirstlane(vectors[kBroken]) != 0;
         const float rest = __uint_as_float(__builtin_amdgcn_readfirstlane(vectors[kSince + kChunk - 1]));
+        forgotten = forgotten || rest == 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const f32x4 until = row_factors(vectors, kUntil, i);
@@ -96,7 +110,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
             dout[i] = Values::get(tile, i);
         }
         // dU, then Z
-        {
+        if (!matrix) {
             const Terms<TERMS> x[2] = {split<TERMS>(dout[0], dout[1]), split<TERMS>(dout[2], dout[3])};
             Terms<3> scores[kBlocks];
 #pragma unroll
@@ -124,11 +138,11 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
 #pragma unroll
                     for (int f = 0; f < kBlocks; ++f) z[upper_tile(f)] = mfma(inverse[f].t[j], x[upper_half(f)].t[rank - j], z[upper_tile(f)]);
         }
-        Values::template write_terms<RANKS>(tile, z, p.pulls + index * (RANKS * kChunk * padded_values(p.DV)) + mine, padded_values(p.DV));
+        if constexpr (!TRANSFER) Values::template write_terms<RANKS>(tile, z, p.pulls + index * (RANKS * kChunk * padded_values(p.DV)) + mine, padded_values(p.DV));
 #pragma unroll
         for (int i = 0; i < 4; ++i) z[i] *= row_factors(vectors, kBeta, i);
-        Values::turn_values(tile, z);
-        Values::write(tile, v_base + static_cast<int64_t>(chunk) * kChunk * p.dv.step, p.dv.step, p.T - chunk * kChunk, limit - chunk * kChunk, p.DV - mine, p.near_values);
+        if constexpr (!TRANSFER) Values::turn_values(tile, z);
+        if constexpr (!TRANSFER) Values::write(tile, v_base + static_cast<int64_t>(chunk) * kChunk * p.dv.step, p.dv.step, p.T - chunk * kChunk, limit - chunk * kChunk, p.DV - mine, p.near_values);
         // R in front of the chunk
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -146,6 +160,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
         for (int half = 0; half < 2; ++half)
 #pragma unroll
             for (int which = 0; which < 2; ++which) {
+                if (matrix && which == 1) continue;
                 Terms<TERMS> c[2 * KS];
 #pragma unroll
                 for (int d = 0; d < 2 * KS; ++d) c[d] = Lds::columns(which == 0 ? keys : queries, d, half);
@@ -161,15 +176,30 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
                         }
             }
     }
-    for (int t = live * kChunk + wave * 4 + group; t < p.T; t += 4 * WAVES)      // padding
-        for (int c = left + lane % 16; c < p.DV && c < left + Values::kColumns; c += 16) v_base[t * p.dv.step + c - mine] = from_float<T>(0.0f);
+    if constexpr (TRANSFER) {
+        float* to = p.transfers + static_cast<int64_t>(item) * transfer_floats(KS, p.DV);
+        const int at = matrix ? column : 32 * KS + column;
 #pragma unroll
-    for (int d = 0; d < 2 * KS; ++d)
+        for (int d = 0; d < 2 * KS; ++d)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = head_element(d, r);
-            if (there && row < p.DK) p.dstate_in[cell + static_cast<int64_t>(row) * p.DV] = later[d][r];
-        }
+            for (int r = 0; r < 4; ++r)
+                if (there) to[head_element(d, r) * transfer_columns(KS, p.DV) + at] = later[d][r];
+        if (matrix && columns == value_parts && threadIdx.x == 0) to[transfer_floats(KS, p.DV) - 4] = forgotten ? 1.0f : 0.0f;
+        return;
+    }
+    if (segment == last) {
+        for (int t = chunks * kChunk + wave * 4 + group; t < p.T; t += 4 * WAVES)      // padding
+            for (int c = left + lane % 16; c < p.DV && c < left + Values::kColumns; c += 16) v_base[t * p.dv.step + c - mine] = from_float<T>(0.0f);
+    }
+    if (segment == 0) {
+#pragma unroll
+        for (int d = 0; d < 2 * KS; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = head_element(d, r);
+                if (there && row < p.DK) p.dstate_in[cell + static_cast<int64_t>(row) * p.DV] = later[d][r];
+            }
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -601,7 +631,11 @@ __global__ __launch_bounds__(512) void delta_gradient_kernel(DeltaArgs p) {
 template <typename T, int KS>
 void launch_backward(const DeltaArgs& p, hipStream_t stream) {
     launch_chunks<T, KS, true>(p, stream);
-    delta_walk_back_kernel<T, KS><<<dim3(head_groups(p.N * p.HV, (p.DV + 63) / 64)), dim3(256), 0, stream>>>(p);
+    if (p.segments > 1) {
+        delta_walk_back_kernel<T, KS, true><<<dim3(head_groups(p.N * p.HV * (p.segments - 1), transfer_parts(4, KS, p.DV))), dim3(256), 0, stream>>>(p);
+        launch_join<KS>(p, true, stream);
+    }
+    delta_walk_back_kernel<T, KS, false><<<dim3(head_groups(p.N * p.HV * p.segments, (p.DV + 63) / 64)), dim3(256), 0, stream>>>(p);
     const int64_t places = static_cast<int64_t>(p.N) * p.H * p.chunks, units = compute_units();
     delta_gradient_kernel<T, KS><<<dim3(static_cast<unsigned>(places < units ? places : units)), dim3(512), 0, stream>>>(p);
 }
@@ -614,7 +648,8 @@ using namespace snnf;
 extern "C" size_t snnf_delta_rule_backward_workspace_bytes(const snnf_delta_rule_call* call) {
     if (check_delta("snnf_delta_rule_backward_workspace_bytes", call) != SNNF_OK) return 0;
     return static_cast<size_t>(delta_chunks(call)) *
-           (block_words(3) * 4 + (delta_mark_elements(call) + delta_elements(delta_ranks(call), call->value_size)) * sizeof(uint16_t));
+           (block_words(3) * 4 + (delta_mark_elements(call) + delta_elements(delta_ranks(call), call->value_size)) * sizeof(uint16_t)) +
+           delta_segment_floats(call, true) * 4;
 }
 
 extern "C" int snnf_delta_rule_backward(const snnf_delta_rule_call* call, const void* marks, const snnf_heads* dout, const float* dstate, const snnf_heads* dquery,
@@ -641,6 +676,7 @@ extern "C" int snnf_delta_rule_backward(const snnf_delta_rule_call* call, const 
     p.blocks = static_cast<uint32_t*>(workspace);
     p.later = reinterpret_cast<uint16_t*>(p.blocks + chunks * block_words(3));
     p.pulls = p.later + chunks * delta_mark_elements(call);
+    set_segments(p, call, true, reinterpret_cast<float*>(p.pulls + chunks * delta_elements(delta_ranks(call), call->value_size)));
     hipStream_t hs = as_stream(stream);
     const bool small = call->key_size <= 64;
     if (call->dtype == SNNF_F32) small ? launch_backward<float, 2>(p, hs) : launch_backward<float, 4>(p, hs);
