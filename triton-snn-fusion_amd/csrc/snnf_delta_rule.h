@@ -139,9 +139,21 @@ __host__ __device__ __forceinline__ constexpr int padded_values(int DV) { return
 template <int KS>
 __device__ __forceinline__ int mark_place(int column, int tile) { return (tile / 2 ^ (column & (KS - 1))) * 32 + 4 * (tile % 2); }
 inline int64_t mark_elements(int ranks, int KS, int DV) { return static_cast<int64_t>(ranks) * padded_values(DV) * 32 * KS; }
-// Of a segment: [32 KS rows][32 KS columns of the matrix that takes the state before it to the state behind it, then the value columns of what it adds], then whether the state before it is forgotten.
-__host__ __device__ __forceinline__ constexpr int transfer_columns(int KS, int DV) { return 32 * KS + padded_values(DV); }
-__host__ __device__ __forceinline__ constexpr int transfer_floats(int KS, int DV) { return 32 * KS * transfer_columns(KS, DV) + 4; }
+// Of a segment: the matrix that takes the state before it to the state behind it, what it adds ([32 KS rows][value columns]), and whether the state before it is forgotten. The matrix lies as
+// the products that take it load it: [32 columns][tile of rows][half of 8 columns][lane][4 columns].
+__host__ __device__ __forceinline__ constexpr int transfer_matrix(int KS) { return 32 * KS * 32 * KS; }
+__host__ __device__ __forceinline__ constexpr int transfer_floats(int KS, int DV) { return transfer_matrix(KS) + 32 * KS * padded_values(DV) + 4; }
+template <int KS>
+__device__ __forceinline__ int transfer_place(int tile, int r, int column) {      // row head_element(tile, r)
+    return (((column / 32 * 2 * KS + tile) * 2 + column % 8 / 4) * 64 + column % 32 / 8 * 16 + (threadIdx.x & 63) / 16 * 4 + r) * 4 + column % 4;
+}
+template <int KS>
+__device__ __forceinline__ void store_transfer(float* to, const f32x4 (&x)[2 * KS], bool matrix, int column, int values) {
+#pragma unroll
+    for (int d = 0; d < 2 * KS; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) to[matrix ? transfer_place<KS>(d, r, column) : transfer_matrix(KS) + head_element(d, r) * values + column] = x[d][r];
+}
 inline int64_t delta_elements(int ranks, int DV) { return static_cast<int64_t>(ranks) * kChunk * padded_values(DV); }
 
 __device__ __forceinline__ int length_of(const DeltaArgs& p, int n) {

@@ -415,12 +415,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 && WALK != kTraining ? 512 : 64 * WA
     }
     if constexpr (TRANSFER) {
         float* to = p.transfers + static_cast<int64_t>(item) * transfer_floats(KS, p.DV);
-        const int at = matrix ? column : 32 * KS + column;
-#pragma unroll
-        for (int d = 0; d < 2 * KS; ++d)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (there) to[head_element(d, r) * transfer_columns(KS, p.DV) + at] = state[d][r];
+        if (there) store_transfer<KS>(to, state, matrix, column, padded_values(p.DV));
         if (matrix && columns == value_parts && threadIdx.x == 0) to[transfer_floats(KS, p.DV) - 4] = forgotten ? 1.0f : 0.0f;
     } else if (segment == last) {
         for (int t = chunks * kChunk + wave * 4 + group; t < p.T; t += 4 * WAVES)      // padding
@@ -442,7 +437,7 @@ __global__ __launch_bounds__(64 * KS) void delta_join_kernel(DeltaArgs p, int ba
     __shared__ f32x4 parts[2][KS][2 * KS][64];
     int head, tile;
     if (!part_of_head(p.N * p.HV, (p.DV + 15) / 16, &head, &tile)) return;
-    const int n = head / p.HV, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, column = 16 * tile + lane % 16, width = transfer_columns(KS, p.DV);
+    const int n = head / p.HV, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, column = 16 * tile + lane % 16;
     const int chunks = (length_of(p, n) + kChunk - 1) / kChunk, last = chunks == 0 ? 0 : (chunks - 1) / p.per;
     const float* transfers = p.transfers + static_cast<int64_t>(head) * (p.segments - 1) * transfer_floats(KS, p.DV);
     float* between = p.between + static_cast<int64_t>(head) * (p.segments - 1) * p.DK * p.DV;
@@ -459,14 +454,11 @@ __global__ __launch_bounds__(64 * KS) void delta_join_kernel(DeltaArgs p, int ba
 #pragma unroll
         for (int d = 0; d < 2 * KS; ++d)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int row = 32 * (d / 2) + 8 * (lane % 16 / 4) + 4 * (d % 2) + lane % 4;
-                x.matrix[d][i] = *reinterpret_cast<const f32x4*>(from + row * width + 32 * wave + 8 * (lane / 16) + 4 * i);
-            }
+            for (int i = 0; i < 2; ++i) x.matrix[d][i] = *reinterpret_cast<const f32x4*>(from + (((wave * 2 * KS + d) * 2 + i) * 64 + lane) * 4);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x.added[i][r] = from[head_element(2 * wave + i, r) * width + 32 * KS + column];
+            for (int r = 0; r < 4; ++r) x.added[i][r] = from[transfer_matrix(KS) + head_element(2 * wave + i, r) * padded_values(p.DV) + column];
         now();
     };
     f32x4 state[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};

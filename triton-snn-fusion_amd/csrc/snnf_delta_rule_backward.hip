@@ -178,12 +178,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
     }
     if constexpr (TRANSFER) {
         float* to = p.transfers + static_cast<int64_t>(item) * transfer_floats(KS, p.DV);
-        const int at = matrix ? column : 32 * KS + column;
-#pragma unroll
-        for (int d = 0; d < 2 * KS; ++d)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (there) to[head_element(d, r) * transfer_columns(KS, p.DV) + at] = later[d][r];
+        if (there) store_transfer<KS>(to, later, matrix, column, padded_values(p.DV));
         if (matrix && columns == value_parts && threadIdx.x == 0) to[transfer_floats(KS, p.DV) - 4] = forgotten ? 1.0f : 0.0f;
         return;
     }
