@@ -266,13 +266,12 @@ __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" : 
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
     return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)(p))));
 }
-// A chunk's rows of 16 bytes times SLOTS to LDS in the order of `slot_of`; zeros for rows from `rows` on and behind `width` elements, from 16 bytes of them.
+// A chunk's rows of 16 bytes times SLOTS to LDS in the order of `slot_of`, by WAVES waves; zeros for rows from `rows` on and behind `width` elements, from 16 bytes of them.
 template <int SLOTS, int WAVES>
-__device__ __forceinline__ void rows_to_lds(const uint16_t* base, int64_t step, int rows, int width, const void* zeros, uint16_t* lds) {
+__device__ __forceinline__ void rows_to_lds(int wave, const uint16_t* base, int64_t step, int rows, int width, const void* zeros, uint16_t* lds) {
     constexpr int ROWS = 64 / SLOTS;    // of one instruction
     static_assert(ROWS * WAVES % 16 == 0, "a lane's place in a row is the same in all of its rows");
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int row = wave * ROWS + lane / SLOTS, at = 8 * slot_of<SLOTS>(row, lane % SLOTS);
+    const int lane = threadIdx.x & 63, row = wave * ROWS + lane / SLOTS, at = 8 * slot_of<SLOTS>(row, lane % SLOTS);
     const uint32_t to = lds_address(lds) + wave * 1024, offset = static_cast<uint32_t>(row * static_cast<int>(step) + at) * 2;
     const bool whole = rows >= kChunk && width >= 8 * SLOTS;
 #pragma unroll
@@ -295,7 +294,7 @@ template <typename T, int PER_ROW, int THREADS> struct Staged {
     Raw<T, 8> raw[kCount];
     // base: the chunk's first row; rows, width: how many rows and elements there are
     __device__ __forceinline__ void load(const T* base, int64_t step, int rows, int width, bool near) {
-        const int row = threadIdx.x / PER_ROW, at = 8 * (threadIdx.x % PER_ROW);
+        const int row = threadIdx.x % THREADS / PER_ROW, at = 8 * (threadIdx.x % PER_ROW);
         if (near && rows >= kChunk) {
             const uint32_t offset = at < width ? static_cast<uint32_t>(row * static_cast<int>(step) + at) * sizeof(T) : 0u;
 #pragma unroll
@@ -324,7 +323,7 @@ template <typename T, int KS, int THREADS>
 __device__ __forceinline__ void put_rows(const Staged<T, 4 * KS, THREADS>& x, uint16_t* lds) {
 #pragma unroll
     for (int i = 0; i < x.kCount; ++i) {
-        Rows<T, KS>::put(lds, threadIdx.x + i * THREADS, terms_of(x.raw[i]));
+        Rows<T, KS>::put(lds, threadIdx.x % THREADS + i * THREADS, terms_of(x.raw[i]));
     }
 }
 
@@ -345,7 +344,7 @@ template <typename T, int WAVES> struct Tile {
     __device__ __forceinline__ static void put(T* lds, const Staged<T, 2 * WAVES, 64 * WAVES>& x) {
 #pragma unroll
         for (int i = 0; i < x.kCount; ++i) {
-            const int row = threadIdx.x / kSlots + i * x.kRows, slot = threadIdx.x % kSlots;
+            const int row = threadIdx.x % (64 * WAVES) / kSlots + i * x.kRows, slot = threadIdx.x % kSlots;
             T* to = lds + row * kStride + 8 * (sizeof(T) == 4 ? slot : slot_of<kSlots>(row, slot));
 #pragma unroll
             for (int w = 0; w < Raw<T, 8>::kWords; w += 4)
@@ -474,54 +473,62 @@ template <typename T, int KS, int WAVES, int PIECES, bool ALL> struct StagedChun
         block.store(to);
     }
 };
-// ... or, with one term to an element, as they are, a chunk ahead into the other buffer: past the registers where rows are whole vectors, else through them at once.
+// ... or, with one term to an element, as they are, a chunk ahead into the other buffer: past the registers where rows are whole vectors, else through them at once. Loads past the registers wait for
+// room on their way, some 3000 of a walk's 13000 cycles a chunk: where four waves walk, four more do nothing but load.
 template <typename T, int KS, int WAVES, int PIECES, bool ALL = true> struct ChunkReader {
-    static constexpr bool kDirect = kTerms<T> == 1;
+    static constexpr bool kDirect = kTerms<T> == 1, kLoaders = kDirect && WAVES == 4;
     static constexpr int kBuffers = kDirect ? 2 : 1;
     struct Buffers {
         uint16_t keys[Rows<T, KS>::kSize], queries[Rows<T, KS>::kSize];
         T tile[Tile<T, WAVES>::kSize];
         uint32_t block[PIECES * 256];
     };
+    struct Chunk {                      // its first row of keys, queries and values, and how many rows and values there are
+        const T *keys, *queries, *values;
+        int64_t step;
+        int rows, width;
+        const uint32_t* block;
+    };
     struct Nothing {};
     std::conditional_t<kDirect, Nothing, StagedChunk<T, KS, WAVES, PIECES, ALL>> next;
 
-    __device__ __forceinline__ void fetch(const DeltaArgs& p, const T* keys, const T* queries, const T* values, int64_t step, int rows, int width, const uint32_t* block, Buffers& to) {
+    __device__ __forceinline__ void fetch(const DeltaArgs& p, const Chunk& c, Buffers& to) {
         if constexpr (!kDirect) {
-            next.load(p, keys, queries, values, step, rows, width, block);
+            next.load(p, c.keys, c.queries, c.values, c.step, c.rows, c.width, c.block);
         } else {
-            const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-            const uint32_t* zeros = block + block_vectors((PIECES - 1) / kBlocks - 3) + kZeros;
+            const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % WAVES;
+            const uint32_t* zeros = c.block + block_vectors((PIECES - 1) / kBlocks - 3) + kZeros;
             if (p.near_keys) {
-                rows_to_lds<4 * KS, WAVES>(reinterpret_cast<const uint16_t*>(keys), p.k.step, rows, p.DK, zeros, to.keys);
-                if constexpr (ALL) rows_to_lds<4 * KS, WAVES>(reinterpret_cast<const uint16_t*>(queries), p.q.step, rows, p.DK, zeros, to.queries);
+                rows_to_lds<4 * KS, WAVES>(wave, reinterpret_cast<const uint16_t*>(c.keys), p.k.step, c.rows, p.DK, zeros, to.keys);
+                if constexpr (ALL) rows_to_lds<4 * KS, WAVES>(wave, reinterpret_cast<const uint16_t*>(c.queries), p.q.step, c.rows, p.DK, zeros, to.queries);
             } else {
                 Staged<T, 4 * KS, 64 * WAVES> x;
-                x.load(keys, p.k.step, rows, p.DK, false);
+                x.load(c.keys, p.k.step, c.rows, p.DK, false);
                 put_rows<T, KS, 64 * WAVES>(x, to.keys);
                 if constexpr (ALL) {
-                    x.load(queries, p.q.step, rows, p.DK, false);
+                    x.load(c.queries, p.q.step, c.rows, p.DK, false);
                     put_rows<T, KS, 64 * WAVES>(x, to.queries);
                 }
             }
             if (p.near_values) {
-                rows_to_lds<2 * WAVES, WAVES>(reinterpret_cast<const uint16_t*>(values), step, rows, width, zeros, reinterpret_cast<uint16_t*>(to.tile));
+                rows_to_lds<2 * WAVES, WAVES>(wave, reinterpret_cast<const uint16_t*>(c.values), c.step, c.rows, c.width, zeros, reinterpret_cast<uint16_t*>(to.tile));
             } else {
                 Staged<T, 2 * WAVES, 64 * WAVES> x;
-                x.load(values, step, rows, width, false);
+                x.load(c.values, c.step, c.rows, c.width, false);
                 Tile<T, WAVES>::put(to.tile, x);
             }
             const uint32_t at = lds_address(to.block) + wave * 1024;
 #pragma unroll
-            for (int i = 0; i < (PIECES + WAVES - 1) / WAVES; ++i)
-                if (wave + i * WAVES < PIECES && (ALL || wave + i * WAVES < kBlocks * 3 || wave + i * WAVES == PIECES - 1))
-                    to_lds(block + (wave + i * WAVES) * 256, lane * 16u, at + i * WAVES * 1024);
+            for (int i = 0; i < (PIECES + WAVES - 1) / WAVES; ++i) {
+                const int piece = wave + i * WAVES;
+                if (piece < PIECES && (ALL || piece < kBlocks * 3 || piece == PIECES - 1)) to_lds(c.block + piece * 256, lane * 16u, at + i * WAVES * 1024);
+            }
         }
     }
     // Has the chunk that was fetched last in LDS, for all waves; the one before it may be overwritten from then on.
     __device__ __forceinline__ void wait(Buffers& to) {
         if constexpr (kDirect) {
-            arrived();
+            if constexpr (!kLoaders) arrived();
             __syncthreads();
         } else {
             __syncthreads();
@@ -597,6 +604,8 @@ inline unsigned head_groups(int heads, int parts) { return static_cast<unsigned>
 // Fragments, decays and inverses of all chunks; transposed for the backward pass.
 template <typename T, int KS, bool BACKWARD> void launch_chunks(const DeltaArgs& p, hipStream_t stream);
 
+// Threads of a walk's workgroup, with the waves that load.
+template <typename T> inline int walk_threads(int waves) { return 64 * waves * (kTerms<T> == 1 && waves == 4 ? 2 : 1); }
 // Workgroups to a segment on its first walk, and what joins the states (backward: from the last segment on).
 inline int transfer_parts(int waves, int KS, int DV) { return (DV + 16 * waves - 1) / (16 * waves) + (2 * KS + waves - 1) / waves; }
 template <int KS> void launch_join(const DeltaArgs& p, bool backward, hipStream_t stream);

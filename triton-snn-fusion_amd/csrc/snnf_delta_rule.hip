@@ -225,7 +225,7 @@ __global__ __launch_bounds__(256, kTerms<T> == 3 ? 2 : 4) void delta_chunk_kerne
 enum Walk { kOutputs, kTraining, kTransfer };
 
 template <typename T, int KS, int WAVES, Walk WALK>
-__global__ __launch_bounds__(kTerms<T> == 1 && WALK != kTraining ? 512 : 64 * WAVES) void delta_walk_kernel(DeltaArgs p) {
+__global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 64 * WAVES) void delta_walk_kernel(DeltaArgs p) {
     using Lds = Rows<T, KS>;
     using Values = Tile<T, WAVES>;
     constexpr int RANKS = kOutputRanks<T>, TERMS = kTerms<T>, PIPE = TERMS == 1 ? 2 : 1;
@@ -243,6 +243,29 @@ __global__ __launch_bounds__(kTerms<T> == 1 && WALK != kTraining ? 512 : 64 * WA
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane / 16;
     const int left = (matrix ? columns - value_parts : columns) * Values::kColumns, mine = left + 16 * wave, column = mine + lane % 16;
     const bool there = column < (matrix ? 32 * KS : p.DV);
+    const T* k_base = static_cast<const T*>(p.k.data) + n * p.k.row + h * p.k.head;
+    const T* q_base = static_cast<const T*>(p.q.data) + n * p.q.row + h * p.q.head;
+    const T* v_base = static_cast<const T*>(p.v.data) + n * p.v.row + hv * p.v.head + (matrix ? 0 : left);
+    T* out_base = static_cast<T*>(const_cast<void*>(p.out.data)) + n * p.out.row + hv * p.out.head + mine;
+    const auto place = [&](int chunk) {
+        const int64_t first = static_cast<int64_t>(chunk) * kChunk;
+        return typename Reader::Chunk{k_base + first * p.k.step, q_base + first * p.q.step, v_base + first * p.v.step, p.v.step, limit - chunk * kChunk, matrix ? 0 : p.DV - left,
+                                      p.blocks + (static_cast<int64_t>(head) * p.chunks + chunk) * block_words(RANKS)};
+    };
+    Reader reader;
+    const auto fetch = [&](int chunk) {
+        if (chunk < live) reader.fetch(p, place(chunk), lds[chunk % Reader::kBuffers]);
+    };
+    if constexpr (Reader::kLoaders)
+        if (wave >= WAVES) {
+            fetch(begin);
+            for (int chunk = begin; chunk < live; ++chunk) {
+                arrived();
+                __syncthreads();
+                fetch(chunk + 1);
+            }
+            return;
+        }
     const int64_t cell = static_cast<int64_t>(head) * p.DK * p.DV + column;
     const float* before = nullptr;
     if (segment == 0) before = p.state == nullptr ? nullptr : p.state + cell;
@@ -256,17 +279,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 && WALK != kTraining ? 512 : 64 * WA
             state[d][r] = before != nullptr && there && row < p.DK ? before[static_cast<int64_t>(row) * p.DV] : (matrix && row == column ? 1.0f : 0.0f);
         }
     bool forgotten = false;
-    const T* k_base = static_cast<const T*>(p.k.data) + n * p.k.row + h * p.k.head;
-    const T* q_base = static_cast<const T*>(p.q.data) + n * p.q.row + h * p.q.head;
-    const T* v_base = static_cast<const T*>(p.v.data) + n * p.v.row + hv * p.v.head + (matrix ? 0 : left);
-    T* out_base = static_cast<T*>(const_cast<void*>(p.out.data)) + n * p.out.row + hv * p.out.head + mine;
-    Reader reader;
-    const auto fetch = [&](int chunk) {
-        const int64_t first = static_cast<int64_t>(chunk) * kChunk;
-        if (chunk < live) reader.fetch(p, k_base + first * p.k.step, q_base + first * p.q.step, v_base + first * p.v.step, p.v.step, limit - chunk * kChunk, matrix ? 0 : p.DV - left,
-                     p.blocks + (static_cast<int64_t>(head) * p.chunks + chunk) * block_words(RANKS), lds[chunk % Reader::kBuffers]);
-    };
-    fetch(begin);
+    if constexpr (!Reader::kLoaders) fetch(begin);
     for (int chunk = begin; chunk < live; ++chunk) {
         const int64_t index = static_cast<int64_t>(head) * p.chunks + chunk;
         typename Reader::Buffers& here = lds[chunk % Reader::kBuffers];
@@ -274,7 +287,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 && WALK != kTraining ? 512 : 64 * WA
         T* tile = here.tile;
         const uint32_t *block = here.block, *vectors = block + block_vectors(RANKS);
         reader.wait(here);
-        fetch(chunk + 1);
+        if constexpr (!Reader::kLoaders) fetch(chunk + 1);
         now();
         // S k and S q, the state's terms a step ahead of the products that take them
         f32x4 ks[4], out[4], right[4], delta[4], since[4];
@@ -356,9 +369,15 @@ __global__ __launch_bounds__(kTerms<T> == 1 && WALK != kTraining ? 512 : 64 * WA
             for (int d = 0; d < 2 * KS; ++d) state[d] *= rest;
 #pragma unroll
             for (int f = 0; f < kBlocks; ++f)
-                if constexpr (!TRANSFER) scores[f] = block_terms<RANKS>(block + kBlocks * 3 * 256, f);
+                if constexpr (WALK == kOutputs) scores[f] = block_terms<RANKS>(block + kBlocks * 3 * 256, f);
         }
-        if constexpr (TRAIN) Values::template write_terms<RANKS>(tile, delta, p.deltas + index * (RANKS * kChunk * padded_values(p.DV)) + mine, padded_values(p.DV));
+        if constexpr (TRAIN) {
+            now();
+            Values::template write_terms<RANKS>(tile, delta, p.deltas + index * (RANKS * kChunk * padded_values(p.DV)) + mine, padded_values(p.DV));
+            now();
+#pragma unroll
+            for (int f = 0; f < kBlocks; ++f) scores[f] = block_terms<RANKS>(block + kBlocks * 3 * 256, f);
+        }
         // What the steps read of each other, and the state behind them
         f32x4 until[4];
 #pragma unroll
@@ -615,7 +634,7 @@ constexpr int kFewSteps = 16;
 
 template <typename T, int KS, int WAVES>
 void launch_walk(const DeltaArgs& p, hipStream_t stream) {
-    const dim3 grid(head_groups(p.N * p.HV * p.segments, (p.DV + 16 * WAVES - 1) / (16 * WAVES))), block(64 * WAVES);
+    const dim3 grid(head_groups(p.N * p.HV * p.segments, (p.DV + 16 * WAVES - 1) / (16 * WAVES))), block(walk_threads<T>(WAVES));
     if (p.marks != nullptr) delta_walk_kernel<T, KS, WAVES, kTraining><<<grid, block, 0, stream>>>(p);
     else delta_walk_kernel<T, KS, WAVES, kOutputs><<<grid, block, 0, stream>>>(p);
 }
@@ -629,7 +648,7 @@ void launch_forward(const DeltaArgs& p, hipStream_t stream) {
     launch_chunks<T, KS, false>(p, stream);
     if (p.segments > 1) {
         constexpr int WAVES = sizeof(T) == 2 ? 8 : 4;
-        delta_walk_kernel<T, KS, WAVES, kTransfer><<<dim3(head_groups(p.N * p.HV * (p.segments - 1), transfer_parts(WAVES, KS, p.DV))), dim3(64 * WAVES), 0, stream>>>(p);
+        delta_walk_kernel<T, KS, WAVES, kTransfer><<<dim3(head_groups(p.N * p.HV * (p.segments - 1), transfer_parts(WAVES, KS, p.DV))), dim3(walk_threads<T>(WAVES)), 0, stream>>>(p);
         launch_join<KS>(p, false, stream);
     }
     if constexpr (sizeof(T) == 2) {

@@ -35,6 +35,29 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane / 16;
     const int left = (matrix ? columns - value_parts : columns) * Values::kColumns, mine = left + 16 * wave, column = mine + lane % 16;
     const bool there = column < (matrix ? 32 * KS : p.DV);
+    const T* k_base = static_cast<const T*>(p.k.data) + n * p.k.row + h * p.k.head;
+    const T* q_base = static_cast<const T*>(p.q.data) + n * p.q.row + h * p.q.head;
+    const T* o_base = static_cast<const T*>(p.dout.data) + n * p.dout.row + hv * p.dout.head + (matrix ? 0 : left);
+    T* v_base = static_cast<T*>(const_cast<void*>(p.dv.data)) + n * p.dv.row + hv * p.dv.head + mine;
+    const auto place = [&](int chunk) {
+        const int64_t first = static_cast<int64_t>(chunk) * kChunk;
+        return typename Reader::Chunk{k_base + first * p.k.step, q_base + first * p.q.step, o_base + first * p.dout.step, p.dout.step, limit - chunk * kChunk, matrix ? 0 : p.DV - left,
+                                      p.blocks + (static_cast<int64_t>(head) * p.chunks + chunk) * block_words(3)};
+    };
+    Reader reader;
+    const auto fetch = [&](int chunk) {
+        if (chunk >= begin) reader.fetch(p, place(chunk), lds[chunk % Reader::kBuffers]);
+    };
+    if constexpr (Reader::kLoaders)
+        if (wave >= WAVES) {
+            fetch(live - 1);
+            for (int chunk = live - 1; chunk >= begin; --chunk) {
+                arrived();
+                __syncthreads();
+                fetch(chunk - 1);
+            }
+            return;
+        }
     const int64_t cell = static_cast<int64_t>(head) * p.DK * p.DV + column;
     const float* behind = nullptr;
     if (segment == last) behind = p.dstate == nullptr ? nullptr : p.dstate + cell;
@@ -48,17 +71,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
             later[d][r] = behind != nullptr && there && row < p.DK ? behind[static_cast<int64_t>(row) * p.DV] : (matrix && row == column ? 1.0f : 0.0f);
         }
     bool forgotten = false;
-    const T* k_base = static_cast<const T*>(p.k.data) + n * p.k.row + h * p.k.head;
-    const T* q_base = static_cast<const T*>(p.q.data) + n * p.q.row + h * p.q.head;
-    const T* o_base = static_cast<const T*>(p.dout.data) + n * p.dout.row + hv * p.dout.head + (matrix ? 0 : left);
-    T* v_base = static_cast<T*>(const_cast<void*>(p.dv.data)) + n * p.dv.row + hv * p.dv.head + mine;
-    Reader reader;
-    const auto fetch = [&](int chunk) {
-        const int64_t first = static_cast<int64_t>(chunk) * kChunk;
-        if (chunk >= begin) reader.fetch(p, k_base + first * p.k.step, q_base + first * p.q.step, o_base + first * p.dout.step, p.dout.step, limit - chunk * kChunk, matrix ? 0 : p.DV - left,
-                                     p.blocks + (static_cast<int64_t>(head) * p.chunks + chunk) * block_words(3), lds[chunk % Reader::kBuffers]);
-    };
-    fetch(live - 1);
+    if constexpr (!Reader::kLoaders) fetch(live - 1);
     for (int chunk = live - 1; chunk >= begin; --chunk) {
         const int64_t index = static_cast<int64_t>(head) * p.chunks + chunk;
         typename Reader::Buffers& here = lds[chunk % Reader::kBuffers];
@@ -66,7 +79,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
         T* tile = here.tile;
         const uint32_t *block = here.block, *vectors = block + block_vectors(3);
         reader.wait(here);
-        fetch(chunk - 1);
+        if constexpr (!Reader::kLoaders) fetch(chunk - 1);
         now();
         // K R
         f32x4 pull[4], dout[4], z[4];
@@ -371,8 +384,8 @@ __global__ __launch_bounds__(512) void delta_gradient_kernel(DeltaArgs p) {
         if constexpr (TERMS == 1) {
             if (p.near_keys) {
                 const uint32_t* zeros = p.blocks + index_of(x) * block_words(3) + block_vectors(3) + kZeros;
-                rows_to_lds<4 * KS, 8>(reinterpret_cast<const uint16_t*>(keys), p.k.step, x.rows, p.DK, zeros, to.keys);
-                rows_to_lds<4 * KS, 8>(reinterpret_cast<const uint16_t*>(queries), p.q.step, x.rows, p.DK, zeros, to.queries);
+                rows_to_lds<4 * KS, 8>(wave, reinterpret_cast<const uint16_t*>(keys), p.k.step, x.rows, p.DK, zeros, to.keys);
+                rows_to_lds<4 * KS, 8>(wave, reinterpret_cast<const uint16_t*>(queries), p.q.step, x.rows, p.DK, zeros, to.queries);
                 return;
             }
         }
@@ -627,10 +640,10 @@ template <typename T, int KS>
 void launch_backward(const DeltaArgs& p, hipStream_t stream) {
     launch_chunks<T, KS, true>(p, stream);
     if (p.segments > 1) {
-        delta_walk_back_kernel<T, KS, true><<<dim3(head_groups(p.N * p.HV * (p.segments - 1), transfer_parts(4, KS, p.DV))), dim3(256), 0, stream>>>(p);
+        delta_walk_back_kernel<T, KS, true><<<dim3(head_groups(p.N * p.HV * (p.segments - 1), transfer_parts(4, KS, p.DV))), dim3(walk_threads<T>(4)), 0, stream>>>(p);
         launch_join<KS>(p, true, stream);
     }
-    delta_walk_back_kernel<T, KS, false><<<dim3(head_groups(p.N * p.HV * p.segments, (p.DV + 63) / 64)), dim3(256), 0, stream>>>(p);
+    delta_walk_back_kernel<T, KS, false><<<dim3(head_groups(p.N * p.HV * p.segments, (p.DV + 63) / 64)), dim3(walk_threads<T>(4)), 0, stream>>>(p);
     const int64_t places = static_cast<int64_t>(p.N) * p.H * p.chunks, units = compute_units();
     delta_gradient_kernel<T, KS><<<dim3(static_cast<unsigned>(places < units ? places : units)), dim3(512), 0, stream>>>(p);
 }
