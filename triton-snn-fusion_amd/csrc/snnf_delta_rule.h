@@ -138,6 +138,26 @@ template <typename T> inline constexpr int kMarkRanks = kOutputRanks<T>;
 __host__ __device__ __forceinline__ constexpr int padded_values(int DV) { return DV <= 64 ? 64 : (DV + 127) / 128 * 128; }
 template <int KS>
 __device__ __forceinline__ int mark_place(int column, int tile) { return (tile / 2 ^ (column & (KS - 1))) * 32 + 4 * (tile % 2); }
+// The terms of a wave's 16 columns from column `left` on, elements 32 s to 32 s + 31 and the 32 behind them, which lie in one line of 128 bytes: lanes swap halves so that an instruction writes whole ones.
+template <int KS, int RANKS>
+__device__ __forceinline__ void store_marks(uint16_t* marks, int DV, int left, int s, const u32x4a (&first)[3], const u32x4a (&second)[3]) {
+    const int lane = threadIdx.x & 63, low = lane % 8;
+    const bool upper = lane % 16 >= 8;
+    const int column = left + low, at = mark_place<KS>(column, 2 * (s + upper)) + 8 * (lane / 16);
+#pragma unroll
+    for (int r = 0; r < RANKS; ++r) {
+        u32x4a x, y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t other = static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(upper ? first[r][i] : second[r][i]), 0x128, 0xf, 0xf, false));     // from 8 lanes on
+            x[i] = upper ? other : first[r][i];
+            y[i] = upper ? second[r][i] : other;
+        }
+        uint16_t* to = marks + static_cast<uint32_t>((r * padded_values(DV) + column) * 32 * KS + at);
+        *reinterpret_cast<u32x4a*>(to) = x;
+        *reinterpret_cast<u32x4a*>(to + 8 * 32 * KS) = y;      // column + 8, whose place is the same
+    }
+}
 inline int64_t mark_elements(int ranks, int KS, int DV) { return static_cast<int64_t>(ranks) * padded_values(DV) * 32 * KS; }
 // Of a segment: the matrix that takes the state before it to the state behind it, what it adds ([32 KS rows][value columns]), and whether the state before it is forgotten. The matrix lies as
 // the products that take it load it: [32 columns][tile of rows][half of 8 columns][lane][4 columns].

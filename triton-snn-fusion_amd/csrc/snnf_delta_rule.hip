@@ -307,6 +307,8 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 64 * WAVES) void delta_walk_
         for (int s = 0; s < KS; ++s) {
             now();
             if (PIPE == 2 && s + 1 < KS) load(s + 1);
+            if constexpr (TRAIN)
+                if (s % 2 == 1) store_marks<KS, kMarkRanks<T>>(p.marks + index * (kMarkRanks<T> * padded_values(p.DV) * 32 * KS), p.DV, mine, s - 1, x[0].t, x[1].t);
             if (s + 1 < KS) x[(s + 1) % 2] = split<3>(state[2 * s + 2], state[2 * s + 3]);
             if (s + 1 == KS) {
 #pragma unroll
@@ -327,12 +329,6 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 64 * WAVES) void delta_walk_
                         for (int i = 0; i < 4; ++i)
                             if (!TRANSFER && rank < RANKS) out[i] = mfma(a[s % PIPE][4 + i].t[j], x[s % 2].t[rank - j], out[i]);
                     }
-            if constexpr (TRAIN) {
-                uint16_t* marks = p.marks + index * (kMarkRanks<T> * padded_values(p.DV) * 32 * KS);
-#pragma unroll
-                for (int r = 0; r < kMarkRanks<T>; ++r)
-                    *reinterpret_cast<u32x4a*>(marks + static_cast<uint32_t>((r * padded_values(p.DV) + column) * 32 * KS + mark_place<KS>(column, 2 * s) + 8 * group)) = x[s % 2].t[r];
-            }
             if (PIPE == 1 && s + 1 < KS) load(s + 1);
         }
         const bool broken = __builtin_amdgcn_readfirstlane(vectors[kBroken]) != 0;

@@ -86,6 +86,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
 #pragma unroll
         for (int i = 0; i < 4; ++i) pull[i] = z[i] = f32x4{0, 0, 0, 0};
         Terms<TERMS> a[PIPE][4];
+        Terms<3> x[2];
         const auto load = [&](int s) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) a[s % PIPE][i] = Lds::rows(keys, i, s);
@@ -95,20 +96,16 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
         for (int s = 0; s < KS; ++s) {
             if (PIPE == 2 && s + 1 < KS) load(s + 1);
             now();
-            const Terms<3> x = split<3>(later[2 * s], later[2 * s + 1]);
-            if constexpr (!TRANSFER) {
-                uint16_t* marks = p.later + index * (kMarkRanks<T> * padded_values(p.DV) * 32 * KS);
-#pragma unroll
-                for (int r = 0; r < kMarkRanks<T>; ++r)
-                    *reinterpret_cast<u32x4a*>(marks + static_cast<uint32_t>((r * padded_values(p.DV) + column) * 32 * KS + mark_place<KS>(column, 2 * s) + 8 * group)) = x.t[r];
-            }
+            x[s % 2] = split<3>(later[2 * s], later[2 * s + 1]);
+            if constexpr (!TRANSFER)
+                if (s % 2 == 1) store_marks<KS, kMarkRanks<T>>(p.later + index * (kMarkRanks<T> * padded_values(p.DV) * 32 * KS), p.DV, mine, s - 1, x[0].t, x[1].t);
 #pragma unroll
             for (int rank = 2; rank >= 0; --rank)
 #pragma unroll
                 for (int j = 0; j <= rank; ++j)
                     if (j < TERMS) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) pull[i] = mfma(a[s % PIPE][i].t[j], x.t[rank - j], pull[i]);
+                        for (int i = 0; i < 4; ++i) pull[i] = mfma(a[s % PIPE][i].t[j], x[s % 2].t[rank - j], pull[i]);
                     }
             if (PIPE == 1 && s + 1 < KS) load(s + 1);
         }
