@@ -111,7 +111,7 @@ struct DeltaArgs {
     // per chunk of a value head
     uint32_t* blocks;                   // fragments of the inverse, then of the scores, then vectors
     uint16_t* marks;                    // state before the chunk, as planes (below)
-    uint16_t* deltas;                   // v - S k, [rank][64][value columns]
+    uint16_t* deltas;                   // v - S k, [rank][16 value columns][64][16], so that a wave writes whole lines
     uint16_t* later;                    // gradient of the state behind the chunk, as marks
     uint16_t* pulls;                    // Z, as deltas
     // Few heads: chunks in segments of `per`, walked side by side
@@ -434,7 +434,7 @@ template <typename T, int WAVES> struct Tile {
         }
         __builtin_amdgcn_wave_barrier();
     }
-    // The terms of the wave's 16 columns to planes [rank][64][columns].
+    // The terms of the wave's 16 columns to where those are in planes [rank][16 columns][64][16].
     template <int RANKS>
     __device__ __forceinline__ static void write_terms(T* lds, const f32x4 (&x)[4], uint16_t* base, int columns) {
         uint32_t words[8][RANKS];
@@ -451,7 +451,7 @@ template <typename T, int WAVES> struct Tile {
             for (int i = 0; i < 2; ++i) {
                 int row, at;
                 const u32x4a piece16 = piece<uint16_t>(lds, i, &row, &at);
-                *reinterpret_cast<u32x4a*>(base + static_cast<uint32_t>((n * kChunk + row) * columns + at)) = piece16;
+                *reinterpret_cast<u32x4a*>(base + static_cast<uint32_t>(n * kChunk * columns + row * 16 + at)) = piece16;
             }
             __builtin_amdgcn_wave_barrier();
         }

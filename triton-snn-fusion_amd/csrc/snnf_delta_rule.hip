@@ -369,7 +369,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 64 * WAVES) void delta_walk_
         }
         if constexpr (TRAIN) {
             now();
-            Values::template write_terms<RANKS>(tile, delta, p.deltas + index * (RANKS * kChunk * padded_values(p.DV)) + mine, padded_values(p.DV));
+            Values::template write_terms<RANKS>(tile, delta, p.deltas + index * (RANKS * kChunk * padded_values(p.DV)) + mine * kChunk, padded_values(p.DV));
             now();
 #pragma unroll
             for (int f = 0; f < kBlocks; ++f) scores[f] = block_terms<RANKS>(block + kBlocks * 3 * 256, f);

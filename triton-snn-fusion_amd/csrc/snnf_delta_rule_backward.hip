@@ -148,7 +148,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
 #pragma unroll
                     for (int f = 0; f < kBlocks; ++f) z[upper_tile(f)] = mfma(inverse[f].t[j], x[upper_half(f)].t[rank - j], z[upper_tile(f)]);
         }
-        if constexpr (!TRANSFER) Values::template write_terms<RANKS>(tile, z, p.pulls + index * (RANKS * kChunk * padded_values(p.DV)) + mine, padded_values(p.DV));
+        if constexpr (!TRANSFER) Values::template write_terms<RANKS>(tile, z, p.pulls + index * (RANKS * kChunk * padded_values(p.DV)) + mine * kChunk, padded_values(p.DV));
 #pragma unroll
         for (int i = 0; i < 4; ++i) z[i] *= row_factors(vectors, kBeta, i);
         if constexpr (!TRANSFER) Values::turn_values(tile, z);
@@ -229,10 +229,10 @@ __device__ __forceinline__ Terms<N> value_rows(const uint16_t* lds, int tile) {
     for (int n = 0; n < N; ++n) r.t[n] = *reinterpret_cast<const u32x4a*>(from + n * kChunk * 32);
     return r;
 }
-// Rows of a plane [64][columns] to there, instruction `part` of four.
-__device__ __forceinline__ void value_rows_to_lds(const uint16_t* plane, int columns, uint16_t* lds, int part) {
-    const int lane = threadIdx.x & 63, row = 16 * part + lane / 4;
-    to_lds(plane, static_cast<uint32_t>(row * columns + 8 * slot_of<4>(row, lane % 4)) * 2, lds_address(lds) + part * 1024);
+// Two times 16 columns of 64 steps to there, instruction `part` of four.
+__device__ __forceinline__ void value_rows_to_lds(const uint16_t* from, uint16_t* lds, int part) {
+    const int lane = threadIdx.x & 63, row = 16 * part + lane / 4, slot = slot_of<4>(row, lane % 4);
+    to_lds(from, static_cast<uint32_t>(slot / 2 * kChunk * 16 + row * 16 + slot % 2 * 8) * 2, lds_address(lds) + part * 1024);
 }
 // Of a state's 32 value columns [32][32 KS]: elements of `head_element(tile, ..)` as rows, value columns as places, in order.
 template <int N, int KS>
@@ -341,7 +341,7 @@ __global__ __launch_bounds__(512) void delta_gradient_kernel(DeltaArgs p) {
         const int64_t index = index_of(x);
         const int hv = x.h * members + x.member;
         const uint16_t *marks = p.marks + index * (MARKS * columns * 32 * KS), *later = p.later + index * (MARKS * columns * 32 * KS);
-        const uint16_t* own_rows = (team == 0 ? p.deltas : p.pulls) + index * (RANKS * kChunk * columns) + 32 * s;
+        const uint16_t* own_rows = (team == 0 ? p.deltas : p.pulls) + index * (RANKS * kChunk * columns) + 32 * kChunk * s;
 #pragma unroll
         for (int r = 0; r < MARKS; ++r)
 #pragma unroll
@@ -352,7 +352,7 @@ __global__ __launch_bounds__(512) void delta_gradient_kernel(DeltaArgs p) {
                     to_lds(later, from, lds_address(to.later[r]) + (wave + 8 * i) * 1024);
                 }
 #pragma unroll
-        for (int r = 0; r < RANKS; ++r) value_rows_to_lds(own_rows + r * kChunk * columns, columns, team == 0 ? to.deltas[r] : to.pulls[r], w);
+        for (int r = 0; r < RANKS; ++r) value_rows_to_lds(own_rows + r * kChunk * columns, team == 0 ? to.deltas[r] : to.pulls[r], w);
         o_next.clear();
         v_next.clear();
         const T* douts = static_cast<const T*>(p.dout.data) + static_cast<int64_t>(x.chunk) * kChunk * p.dout.step + x.n * p.dout.row + hv * p.dout.head;
