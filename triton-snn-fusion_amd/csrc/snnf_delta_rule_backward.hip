@@ -275,15 +275,20 @@ __device__ __forceinline__ void store_gate(const DeltaArgs& p, const HeadView& x
 
 // Of tensors of 16 bits the logarithm is rounded to float32: a decay by 2^-10 is off by 2^-21 then.
 template <typename T>
-__device__ __forceinline__ float decay_between(double x) {
-    if constexpr (sizeof(T) == 4) return decay_of(x);
-    else return __builtin_amdgcn_exp2f(static_cast<float>(x));
+__device__ __forceinline__ float decay_apart(const Sum& one, const Sum& other, bool ahead) {
+    if constexpr (sizeof(T) == 4) {
+        return ahead ? decay_between(other, one) : decay_between(one, other);
+    } else {
+        const float x = (one.large - other.large) + (one.small - other.small);
+        return __builtin_amdgcn_exp2f(ahead ? x : -x);
+    }
 }
 
 // Two waves to 16 steps: the first works out dL, the second dP, and each has half of the head's elements of everything else; they exchange dL and dP through LDS. A workgroup takes one chunk after the
-// other, each in pieces of 32 value columns and then a last one of keys and queries; with bfloat16 the next piece is on its way while one is worked on.
+// other, each in pieces of 32 value columns and then a last one of keys and queries; with bfloat16 four more waves load the next piece while one is worked on.
 template <typename T, int KS> struct GradientPieces {
     static constexpr int RANKS = kOutputRanks<T>, TERMS = kTerms<T>, MARKS = kMarkRanks<T>, BUFFERS = TERMS == 1 ? 2 : 1;     // by the room in LDS
+    static constexpr int THREADS = BUFFERS == 2 ? 768 : 512;
     struct Slice {                      // 32 value columns of everything
         uint16_t marks[MARKS][1024 * KS], later[MARKS][1024 * KS], deltas[RANKS][kChunk * 32], pulls[RANKS][kChunk * 32], douts[TERMS][kChunk * 32];
     };
@@ -297,17 +302,19 @@ template <typename T, int KS> struct GradientPieces {
     };
 };
 
-template <typename T, int KS>
-__global__ __launch_bounds__(512) void delta_gradient_kernel(DeltaArgs p) {
+// SHARED: whether value heads share queries and keys, whose gradients are their sums then, held over the chunks of a head's members.
+template <typename T, int KS, bool SHARED>
+__global__ __launch_bounds__((GradientPieces<T, KS>::THREADS)) void delta_gradient_kernel(DeltaArgs p) {
     using Lds = Rows<T, KS>;
     using Pieces = GradientPieces<T, KS>;
     constexpr int RANKS = Pieces::RANKS, TERMS = Pieces::TERMS, MARKS = Pieces::MARKS, BUFFERS = Pieces::BUFFERS;
+    constexpr bool LOADERS = BUFFERS == 2;
     __shared__ alignas(16) typename Pieces::Piece lds[BUFFERS];
-    __shared__ alignas(16) double total[kChunk];
+    __shared__ alignas(16) Sum total[kChunk];
     __shared__ alignas(16) int part[kChunk];
     __shared__ alignas(16) float betas[kChunk], dsums[2][kChunk], tails[2][kChunk], own_sums[kChunk], dots[8];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), team = wave / 4, w = wave % 4, group = lane / 16, column = lane % 16;
-    const int own = 16 * w + column, members = p.HV / p.H, columns = padded_values(p.DV), slices = (p.DV + 31) / 32;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), team = wave / 4 % 2, w = wave % 4, group = lane / 16, column = lane % 16;
+    const int own = 16 * w + column, members = SHARED ? p.HV / p.H : 1, columns = padded_values(p.DV), slices = (p.DV + 31) / 32;
     const int places = p.N * p.H * p.chunks;
     struct Item {                       // a chunk of a value head
         int place, member, chunk, n, h, rows;
@@ -322,6 +329,7 @@ __global__ __launch_bounds__(512) void delta_gradient_kernel(DeltaArgs p) {
         for (; x.place < places; x.place += static_cast<int>(gridDim.x)) {
             settle(x);
             if (x.rows > 0) return;
+            if (wave >= 8) continue;
             const int steps = p.T - x.chunk * kChunk < kChunk ? p.T - x.chunk * kChunk : kChunk;
             T* dquery = static_cast<T*>(const_cast<void*>(p.dq.data)) + static_cast<int64_t>(x.chunk) * kChunk * p.dq.step + x.n * p.dq.row + x.h * p.dq.head;
             T* dkey = static_cast<T*>(const_cast<void*>(p.dk.data)) + static_cast<int64_t>(x.chunk) * kChunk * p.dk.step + x.n * p.dk.row + x.h * p.dk.head;
@@ -336,29 +344,42 @@ __global__ __launch_bounds__(512) void delta_gradient_kernel(DeltaArgs p) {
     };
     const auto index_of = [&](const Item& x) { return (static_cast<int64_t>(x.n) * p.HV + x.h * members + x.member) * p.chunks + x.chunk; };
 
-    Raw<T, 8> o_next, v_next;           // a piece to each of the first 256 threads; the values of the lane's own step
+    Raw<T, 8> o_next, v_next;           // a piece to each of 256 threads; the values of the lane's own step
     const auto fetch_slice = [&](const Item& x, int s, typename Pieces::Slice& to) {
+        constexpr int WAVES = LOADERS ? 4 : 8;
+        const int from_wave = wave % WAVES;
         const int64_t index = index_of(x);
-        const int hv = x.h * members + x.member;
         const uint16_t *marks = p.marks + index * (MARKS * columns * 32 * KS), *later = p.later + index * (MARKS * columns * 32 * KS);
-        const uint16_t* own_rows = (team == 0 ? p.deltas : p.pulls) + index * (RANKS * kChunk * columns) + 32 * kChunk * s;
 #pragma unroll
         for (int r = 0; r < MARKS; ++r)
 #pragma unroll
-            for (int i = 0; i < (2 * KS + 7) / 8; ++i)
-                if (wave + 8 * i < 2 * KS) {
-                    const uint32_t from = static_cast<uint32_t>((r * columns + 32 * s) * 32 * KS + 512 * (wave + 8 * i)) * 2 + lane * 16;
-                    to_lds(marks, from, lds_address(to.marks[r]) + (wave + 8 * i) * 1024);
-                    to_lds(later, from, lds_address(to.later[r]) + (wave + 8 * i) * 1024);
+            for (int i = 0; i < (2 * KS + WAVES - 1) / WAVES; ++i)
+                if (from_wave + WAVES * i < 2 * KS) {
+                    const uint32_t from = static_cast<uint32_t>((r * columns + 32 * s) * 32 * KS + 512 * (from_wave + WAVES * i)) * 2 + lane * 16;
+                    to_lds(marks, from, lds_address(to.marks[r]) + (from_wave + WAVES * i) * 1024);
+                    to_lds(later, from, lds_address(to.later[r]) + (from_wave + WAVES * i) * 1024);
                 }
+        const int64_t rows_at = index * (RANKS * kChunk * columns) + 32 * kChunk * s;
 #pragma unroll
-        for (int r = 0; r < RANKS; ++r) value_rows_to_lds(own_rows + r * kChunk * columns, team == 0 ? to.deltas[r] : to.pulls[r], w);
+        for (int r = 0; r < RANKS; ++r) {
+            if (LOADERS || team == 0) value_rows_to_lds(p.deltas + rows_at + r * kChunk * columns, to.deltas[r], w);
+            if (LOADERS || team == 1) value_rows_to_lds(p.pulls + rows_at + r * kChunk * columns, to.pulls[r], w);
+        }
         o_next.clear();
+        const T* douts = static_cast<const T*>(p.dout.data) + static_cast<int64_t>(x.chunk) * kChunk * p.dout.step + x.n * p.dout.row + (x.h * members + x.member) * p.dout.head;
+        const int row = threadIdx.x % 256 / 4, at = 32 * s + 8 * (threadIdx.x % 4);
+        if (row < x.rows && (LOADERS || team == 0) && at < p.DV) o_next.load(douts, row * p.dout.step + at, p.DV - at);
+    };
+    const auto put_slice = [&](typename Pieces::Slice& to) {
+        if (!LOADERS && team == 1) return;
+        const Terms<TERMS> o = terms_of(o_next);
+#pragma unroll
+        for (int r = 0; r < TERMS; ++r) *reinterpret_cast<u32x4a*>(to.douts[r] + value_place(threadIdx.x % 256 / 4, threadIdx.x % 4)) = o.t[r];
+    };
+    const auto fetch_values = [&](const Item& x, int s) {
         v_next.clear();
-        const T* douts = static_cast<const T*>(p.dout.data) + static_cast<int64_t>(x.chunk) * kChunk * p.dout.step + x.n * p.dout.row + hv * p.dout.head;
-        const T* values = static_cast<const T*>(p.v.data) + static_cast<int64_t>(x.chunk) * kChunk * p.v.step + x.n * p.v.row + hv * p.v.head;
-        const int row = threadIdx.x / 4, at = 32 * s + 8 * (threadIdx.x % 4), own_at = 32 * s + 8 * group;
-        if (row < x.rows && row < kChunk && at < p.DV) o_next.load(douts, row * p.dout.step + at, p.DV - at);
+        const T* values = static_cast<const T*>(p.v.data) + static_cast<int64_t>(x.chunk) * kChunk * p.v.step + x.n * p.v.row + (x.h * members + x.member) * p.v.head;
+        const int own_at = 32 * s + 8 * group;
         if (team == 0 && own < x.rows && own_at < p.DV) v_next.load(values, own * p.v.step + own_at, p.DV - own_at);
     };
     // What a chunk's steps have of their own: exp(G), exp(G_64 - G), beta and exp(G_64) of the lane's own step; gate, start and beta of the first wave's
@@ -376,32 +397,71 @@ __global__ __launch_bounds__(512) void delta_gradient_kernel(DeltaArgs p) {
         }
     };
     const auto fetch_heads = [&](const Item& x, typename Pieces::Heads& to) {
+        constexpr int THREADS = LOADERS ? 256 : 512;
         const T* keys = static_cast<const T*>(p.k.data) + static_cast<int64_t>(x.chunk) * kChunk * p.k.step + x.n * p.k.row + x.h * p.k.head;
         const T* queries = static_cast<const T*>(p.q.data) + static_cast<int64_t>(x.chunk) * kChunk * p.q.step + x.n * p.q.row + x.h * p.q.head;
         if constexpr (TERMS == 1) {
             if (p.near_keys) {
                 const uint32_t* zeros = p.blocks + index_of(x) * block_words(3) + block_vectors(3) + kZeros;
-                rows_to_lds<4 * KS, 8>(wave, reinterpret_cast<const uint16_t*>(keys), p.k.step, x.rows, p.DK, zeros, to.keys);
-                rows_to_lds<4 * KS, 8>(wave, reinterpret_cast<const uint16_t*>(queries), p.q.step, x.rows, p.DK, zeros, to.queries);
+                rows_to_lds<4 * KS, THREADS / 64>(w, reinterpret_cast<const uint16_t*>(keys), p.k.step, x.rows, p.DK, zeros, to.keys);
+                rows_to_lds<4 * KS, THREADS / 64>(w, reinterpret_cast<const uint16_t*>(queries), p.q.step, x.rows, p.DK, zeros, to.queries);
                 return;
             }
         }
-        Staged<T, 4 * KS, 512> k_rows, q_rows;
+        Staged<T, 4 * KS, THREADS> k_rows, q_rows;
         k_rows.load(keys, p.k.step, x.rows, p.DK, p.near_keys);
         q_rows.load(queries, p.q.step, x.rows, p.DK, p.near_keys);
-        put_rows<T, KS, 512>(k_rows, to.keys);
-        put_rows<T, KS, 512>(q_rows, to.queries);
+        put_rows<T, KS, THREADS>(k_rows, to.keys);
+        put_rows<T, KS, THREADS>(q_rows, to.queries);
     };
 
     Item item{static_cast<int>(blockIdx.x), 0, 0, 0, 0, 0};
     find(item);
     if (item.place >= places) return;
     int turn = 0;                       // pieces so far
-    fetch_slice(item, 0, lds[0].slice);
+    const auto after = [&](const Item& x) {
+        Item next = x;
+        if (++next.member == members) {
+            next.member = 0;
+            next.place += static_cast<int>(gridDim.x);
+            find(next);
+        }
+        return next;
+    };
+    if constexpr (LOADERS)
+        if (wave >= 8) {
+            fetch_slice(item, 0, lds[0].slice);
+            put_slice(lds[0].slice);
+            for (;;) {
+                for (int s = 0; s < slices; ++s) {
+                    arrived();
+                    __syncthreads();
+                    ++turn;
+                    if (s + 1 < slices) {
+                        fetch_slice(item, s + 1, lds[turn % BUFFERS].slice);
+                        put_slice(lds[turn % BUFFERS].slice);
+                    } else {
+                        fetch_heads(item, lds[turn % BUFFERS].heads);
+                    }
+                }
+                arrived();
+                __syncthreads();
+                item = after(item);
+                ++turn;
+                if (item.place < places) {
+                    fetch_slice(item, 0, lds[turn % BUFFERS].slice);
+                    put_slice(lds[turn % BUFFERS].slice);
+                }
+                for (int i = 0; i < 4; ++i) __syncthreads();      // of the others, below
+                if (item.place >= places) return;
+            }
+        }
+    if constexpr (!LOADERS) fetch_slice(item, 0, lds[0].slice);
+    fetch_values(item, 0);
     fetch_steps(item);
     f32x4 dq_all[KS], dk_all[KS];
     for (;;) {
-        if (item.member == 0) {
+        if (SHARED && item.member == 0) {
 #pragma unroll
             for (int d = 0; d < KS; ++d) dq_all[d] = dk_all[d] = f32x4{0, 0, 0, 0};
         }
@@ -415,20 +475,7 @@ __global__ __launch_bounds__(512) void delta_gradient_kernel(DeltaArgs p) {
         float dbeta = 0.0f, zv = 0.0f, dot = 0.0f;
         for (int s = 0; s < slices; ++s, ++turn) {
             typename Pieces::Slice& here = lds[turn % BUFFERS].slice;
-            if (threadIdx.x < 256) {
-                Terms<TERMS> o;
-                if constexpr (TERMS == 1) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o.t[0][i] = o_next.w[i];
-                } else {
-                    float x[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] = o_next[j];
-                    o = split<TERMS>(x);
-                }
-#pragma unroll
-                for (int r = 0; r < TERMS; ++r) *reinterpret_cast<u32x4a*>(here.douts[r] + value_place(threadIdx.x / 4, threadIdx.x % 4)) = o.t[r];
-            }
+            if constexpr (!LOADERS) put_slice(here);
             const Raw<T, 8> v = v_next;
             if (s == 0 && wave == 0) {
                 const bool fresh = lane < item.rows && (start_next || gate_next < kForgotten);
@@ -439,15 +486,12 @@ __global__ __launch_bounds__(512) void delta_gradient_kernel(DeltaArgs p) {
                     const double before = __shfl_up(sum, d, 64);
                     if (lane >= d) sum += before;
                 }
-                total[lane] = sum;
+                total[lane] = sum_of(sum);
                 betas[lane] = row_beta_next;
             }
-            arrived();
+            if constexpr (!LOADERS) arrived();
             __syncthreads();
-            if constexpr (BUFFERS == 2) {
-                if (s + 1 < slices) fetch_slice(item, s + 1, lds[(turn + 1) % BUFFERS].slice);
-                else fetch_heads(item, lds[(turn + 1) % BUFFERS].heads);
-            }
+            if (s + 1 < slices) fetch_values(item, s + 1);
             const Terms<TERMS> o_own = value_rows<TERMS>(here.douts[0], w);
             const Terms<RANKS> z_own = value_rows<RANKS>(here.pulls[0], w), delta_own = value_rows<RANKS>(here.deltas[0], w);
             if (team == 0) {
@@ -489,35 +533,29 @@ __global__ __launch_bounds__(512) void delta_gradient_kernel(DeltaArgs p) {
         }
         typename Pieces::Heads& here = lds[turn % BUFFERS].heads;
         const uint16_t *keys = here.keys, *queries = here.queries;
-        arrived();
+        if constexpr (!LOADERS) arrived();
         __syncthreads();
-        Item next = item;
-        if (++next.member == members) {
-            next.member = 0;
-            next.place += static_cast<int>(gridDim.x);
-            find(next);
-        }
+        const Item next = after(item);
         ++turn;
-        if (BUFFERS == 2 && next.place < places) {
-            fetch_slice(next, 0, lds[turn % BUFFERS].slice);
+        if (next.place < places) {
+            fetch_values(next, 0);
             fetch_steps(next);
         }
         // The other steps are rows 4 group + r of the tiles
-        const double mine_total = total[own];
+        const Sum mine_total = total[own];
         const int mine_part = part[own];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int at = 16 * j + 4 * group;
-            typedef double f64x2 __attribute__((ext_vector_type(2)));
             typedef int i32x4 __attribute__((ext_vector_type(4)));
-            const f64x2 sums[2] = {*reinterpret_cast<const f64x2*>(total + at), *reinterpret_cast<const f64x2*>(total + at + 2)};
+            const f32x4 sums[2] = {*reinterpret_cast<const f32x4*>(total + at), *reinterpret_cast<const f32x4*>(total + at + 2)};
             const i32x4 parts = *reinterpret_cast<const i32x4*>(part + at);
             const f32x4 others = *reinterpret_cast<const f32x4*>(betas + at);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int x = at + r;
-                const double since_then = mine_total - sums[r / 2][r % 2];
-                const float d = parts[r] == mine_part ? decay_between<T>(x <= own ? since_then : -since_then) : 0.0f;
+                const Sum other = {sums[r / 2][r % 2 * 2], sums[r / 2][r % 2 * 2 + 1]};
+                const float d = parts[r] == mine_part ? decay_apart<T>(mine_total, other, x <= own) : 0.0f;
                 if (team == 0) {
                     by_row[j][r] = x == own ? 0.0f : kept(-d * beta * others[r], x < own ? by_row[j][r] : by_column[j][r]);
                 } else {
@@ -579,8 +617,10 @@ __global__ __launch_bounds__(512) void delta_gradient_kernel(DeltaArgs p) {
             const f32x4 k = Lds::four(keys, own, team * KS + d), q = Lds::four(queries, own, team * KS + d);
 #pragma unroll
             for (int r = 0; r < 4; ++r) sum += q[r] * dq[d][r] - k[r] * dk[d][r];
-            dq_all[d] += dq[d];
-            dk_all[d] += dk[d];
+            if constexpr (SHARED) {
+                dq_all[d] += dq[d];
+                dk_all[d] += dk[d];
+            }
         }
         sum = over_groups(sum);
         tail = over_groups(tail);
@@ -603,8 +643,13 @@ __global__ __launch_bounds__(512) void delta_gradient_kernel(DeltaArgs p) {
 #pragma unroll
             for (int d = 0; d < KS; d += 2) {
                 const int at = head_element(team * KS + d, 0);
-                store_eight<T>(dquery + at, p.DK - at, dq_all[d], dq_all[d + 1]);
-                store_eight<T>(dkey + at, p.DK - at, dk_all[d], dk_all[d + 1]);
+                if constexpr (SHARED) {
+                    store_eight<T>(dquery + at, p.DK - at, dq_all[d], dq_all[d + 1]);
+                    store_eight<T>(dkey + at, p.DK - at, dk_all[d], dk_all[d + 1]);
+                } else {
+                    store_eight<T>(dquery + at, p.DK - at, dq[d], dq[d + 1]);
+                    store_eight<T>(dkey + at, p.DK - at, dk[d], dk[d + 1]);
+                }
             }
         }
         __syncthreads();
@@ -628,7 +673,6 @@ __global__ __launch_bounds__(512) void delta_gradient_kernel(DeltaArgs p) {
         item = next;
         if constexpr (BUFFERS == 1) {
             fetch_slice(item, 0, lds[0].slice);
-            fetch_steps(item);
         }
     }
 }
@@ -642,7 +686,9 @@ void launch_backward(const DeltaArgs& p, hipStream_t stream) {
     }
     delta_walk_back_kernel<T, KS, false><<<dim3(head_groups(p.N * p.HV * p.segments, (p.DV + 63) / 64)), dim3(walk_threads<T>(4)), 0, stream>>>(p);
     const int64_t places = static_cast<int64_t>(p.N) * p.H * p.chunks, units = compute_units();
-    delta_gradient_kernel<T, KS><<<dim3(static_cast<unsigned>(places < units ? places : units)), dim3(512), 0, stream>>>(p);
+    const dim3 grid(static_cast<unsigned>(places < units ? places : units)), block(GradientPieces<T, KS>::THREADS);
+    if (p.HV > p.H) delta_gradient_kernel<T, KS, true><<<grid, block, 0, stream>>>(p);
+    else delta_gradient_kernel<T, KS, false><<<grid, block, 0, stream>>>(p);
 }
 
 }  // namespace
