@@ -361,10 +361,11 @@ template <typename T, int WAVES> struct Tile {
         if constexpr (sizeof(T) == 4) return (row * kStride + 16 * wave) * 4 + column * sizeof(E);
         else return row * kStride * 2 + 16 * slot_of<kSlots>(row, 2 * wave + column / 8) + 2 * (column % 8);
     }
-    __device__ __forceinline__ static void put(T* lds, const Staged<T, 2 * WAVES, 64 * WAVES>& x) {
+    template <int THREADS>
+    __device__ __forceinline__ static void put(T* lds, const Staged<T, 2 * WAVES, THREADS>& x) {
 #pragma unroll
         for (int i = 0; i < x.kCount; ++i) {
-            const int row = threadIdx.x % (64 * WAVES) / kSlots + i * x.kRows, slot = threadIdx.x % kSlots;
+            const int row = threadIdx.x % THREADS / kSlots + i * x.kRows, slot = threadIdx.x % kSlots;
             T* to = lds + row * kStride + 8 * (sizeof(T) == 4 ? slot : slot_of<kSlots>(row, slot));
 #pragma unroll
             for (int w = 0; w < Raw<T, 8>::kWords; w += 4)
@@ -493,10 +494,12 @@ template <typename T, int KS, int WAVES, int PIECES, bool ALL> struct StagedChun
         block.store(to);
     }
 };
+template <typename T> __host__ __device__ __forceinline__ constexpr bool loads_apart(int waves, bool all) { return kTerms<T> == 1 && (waves <= 4 || !all); }
+template <typename T> __host__ __device__ __forceinline__ constexpr int walk_threads(int waves, bool all = true) { return 64 * (waves + (loads_apart<T>(waves, all) ? 4 : 0)); }
 // ... or, with one term to an element, as they are, a chunk ahead into the other buffer: past the registers where rows are whole vectors, else through them at once. Loads past the registers wait for
 // room on their way, some 3000 of a walk's 13000 cycles a chunk: where four waves walk, four more do nothing but load.
 template <typename T, int KS, int WAVES, int PIECES, bool ALL = true> struct ChunkReader {
-    static constexpr bool kDirect = kTerms<T> == 1, kLoaders = kDirect && WAVES == 4;
+    static constexpr bool kDirect = kTerms<T> == 1, kLoaders = loads_apart<T>(WAVES, ALL);
     static constexpr int kBuffers = kDirect ? 2 : 1;
     struct Buffers {
         uint16_t keys[Rows<T, KS>::kSize], queries[Rows<T, KS>::kSize];
@@ -516,32 +519,33 @@ template <typename T, int KS, int WAVES, int PIECES, bool ALL = true> struct Chu
         if constexpr (!kDirect) {
             next.load(p, c.keys, c.queries, c.values, c.step, c.rows, c.width, c.block);
         } else {
-            const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % WAVES;
+            constexpr int W = kLoaders ? 4 : WAVES;       // that load
+            const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % W;
             const uint32_t* zeros = c.block + block_vectors((PIECES - 1) / kBlocks - 3) + kZeros;
             if (p.near_keys) {
-                rows_to_lds<4 * KS, WAVES>(wave, reinterpret_cast<const uint16_t*>(c.keys), p.k.step, c.rows, p.DK, zeros, to.keys);
-                if constexpr (ALL) rows_to_lds<4 * KS, WAVES>(wave, reinterpret_cast<const uint16_t*>(c.queries), p.q.step, c.rows, p.DK, zeros, to.queries);
+                rows_to_lds<4 * KS, W>(wave, reinterpret_cast<const uint16_t*>(c.keys), p.k.step, c.rows, p.DK, zeros, to.keys);
+                if constexpr (ALL) rows_to_lds<4 * KS, W>(wave, reinterpret_cast<const uint16_t*>(c.queries), p.q.step, c.rows, p.DK, zeros, to.queries);
             } else {
-                Staged<T, 4 * KS, 64 * WAVES> x;
+                Staged<T, 4 * KS, 64 * W> x;
                 x.load(c.keys, p.k.step, c.rows, p.DK, false);
-                put_rows<T, KS, 64 * WAVES>(x, to.keys);
+                put_rows<T, KS, 64 * W>(x, to.keys);
                 if constexpr (ALL) {
                     x.load(c.queries, p.q.step, c.rows, p.DK, false);
-                    put_rows<T, KS, 64 * WAVES>(x, to.queries);
+                    put_rows<T, KS, 64 * W>(x, to.queries);
                 }
             }
             if (p.near_values) {
-                rows_to_lds<2 * WAVES, WAVES>(wave, reinterpret_cast<const uint16_t*>(c.values), c.step, c.rows, c.width, zeros, reinterpret_cast<uint16_t*>(to.tile));
+                rows_to_lds<2 * WAVES, W>(wave, reinterpret_cast<const uint16_t*>(c.values), c.step, c.rows, c.width, zeros, reinterpret_cast<uint16_t*>(to.tile));
             } else {
-                Staged<T, 2 * WAVES, 64 * WAVES> x;
+                Staged<T, 2 * WAVES, 64 * W> x;
                 x.load(c.values, c.step, c.rows, c.width, false);
                 Tile<T, WAVES>::put(to.tile, x);
             }
             const uint32_t at = lds_address(to.block) + wave * 1024;
 #pragma unroll
-            for (int i = 0; i < (PIECES + WAVES - 1) / WAVES; ++i) {
-                const int piece = wave + i * WAVES;
-                if (piece < PIECES && (ALL || piece < kBlocks * 3 || piece == PIECES - 1)) to_lds(c.block + piece * 256, lane * 16u, at + i * WAVES * 1024);
+            for (int i = 0; i < (PIECES + W - 1) / W; ++i) {
+                const int piece = wave + i * W;
+                if (piece < PIECES && (ALL || piece < kBlocks * 3 || piece == PIECES - 1)) to_lds(c.block + piece * 256, lane * 16u, at + i * W * 1024);
             }
         }
     }
@@ -624,8 +628,6 @@ inline unsigned head_groups(int heads, int parts) { return static_cast<unsigned>
 // Fragments, decays and inverses of all chunks; transposed for the backward pass.
 template <typename T, int KS, bool BACKWARD> void launch_chunks(const DeltaArgs& p, hipStream_t stream);
 
-// Threads of a walk's workgroup, with the waves that load.
-template <typename T> inline int walk_threads(int waves) { return 64 * waves * (kTerms<T> == 1 && waves == 4 ? 2 : 1); }
 // Workgroups to a segment on its first walk, and what joins the states (backward: from the last segment on).
 inline int transfer_parts(int waves, int KS, int DV) { return (DV + 16 * waves - 1) / (16 * waves) + (2 * KS + waves - 1) / waves; }
 template <int KS> void launch_join(const DeltaArgs& p, bool backward, hipStream_t stream);
@@ -645,4 +647,6 @@ inline bool near_by(const HeadView& x, int dtype, bool read) {
 }
 // Eight waves share a head's keys in LDS where heads alone fill the chip, else four.
 inline bool eight_waves(const DeltaArgs& p) { return p.DV > 64 && p.N * p.HV >= compute_units(); }
+// Two waves of 16 columns where four leave half of the chip idle
+inline bool two_waves(const DeltaArgs& p) { return p.DV > 32 && 2 * p.N * p.HV * p.segments * ((p.DV + 63) / 64) <= compute_units(); }
 }  // namespace snnf

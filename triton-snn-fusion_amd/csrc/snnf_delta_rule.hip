@@ -225,7 +225,7 @@ __global__ __launch_bounds__(256, kTerms<T> == 3 ? 2 : 4) void delta_chunk_kerne
 enum Walk { kOutputs, kTraining, kTransfer };
 
 template <typename T, int KS, int WAVES, Walk WALK>
-__global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 64 * WAVES) void delta_walk_kernel(DeltaArgs p) {
+__global__ __launch_bounds__(kTerms<T> == 1 && walk_threads<T>(WAVES, WALK != kTransfer) <= 512 ? 512 : walk_threads<T>(WAVES, WALK != kTransfer)) void delta_walk_kernel(DeltaArgs p) {
     using Lds = Rows<T, KS>;
     using Values = Tile<T, WAVES>;
     constexpr int RANKS = kOutputRanks<T>, TERMS = kTerms<T>, PIPE = TERMS == 1 ? 2 : 1;
@@ -644,12 +644,18 @@ void launch_forward(const DeltaArgs& p, hipStream_t stream) {
     launch_chunks<T, KS, false>(p, stream);
     if (p.segments > 1) {
         constexpr int WAVES = sizeof(T) == 2 ? 8 : 4;
-        delta_walk_kernel<T, KS, WAVES, kTransfer><<<dim3(head_groups(p.N * p.HV * (p.segments - 1), transfer_parts(WAVES, KS, p.DV))), dim3(walk_threads<T>(WAVES)), 0, stream>>>(p);
+        delta_walk_kernel<T, KS, WAVES, kTransfer><<<dim3(head_groups(p.N * p.HV * (p.segments - 1), transfer_parts(WAVES, KS, p.DV))), dim3(walk_threads<T>(WAVES, false)), 0, stream>>>(p);
         launch_join<KS>(p, false, stream);
     }
     if constexpr (sizeof(T) == 2) {
         if (eight_waves(p)) {
             launch_walk<T, KS, 8>(p, stream);
+            return;
+        }
+    }
+    if constexpr (kTerms<T> == 1) {
+        if (two_waves(p)) {
+            launch_walk<T, KS, 2>(p, stream);
             return;
         }
     }

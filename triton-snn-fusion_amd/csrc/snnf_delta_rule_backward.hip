@@ -17,9 +17,9 @@ namespace {
 // ------------------------------------------------------------------------------------------------------------------
 // In segments where heads are few, as the walk forward: a segment's effect on R is A^T R + B, and a first walk (TRANSFER) takes the identity and no gradient of its outputs for A^T, the
 // gradient of its outputs and no R for B.
-template <typename T, int KS, bool TRANSFER>
+template <typename T, int KS, int WAVES, bool TRANSFER>
 __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_kernel(DeltaArgs p) {
-    constexpr int WAVES = 4, RANKS = kOutputRanks<T>, TERMS = kTerms<T>, PIPE = TERMS == 1 ? 2 : 1;
+    constexpr int RANKS = kOutputRanks<T>, TERMS = kTerms<T>, PIPE = TERMS == 1 ? 2 : 1;
     using Lds = Rows<T, KS>;
     using Values = Tile<T, WAVES>;
     using Reader = ChunkReader<T, KS, WAVES, block_pieces(3)>;
@@ -681,10 +681,15 @@ template <typename T, int KS>
 void launch_backward(const DeltaArgs& p, hipStream_t stream) {
     launch_chunks<T, KS, true>(p, stream);
     if (p.segments > 1) {
-        delta_walk_back_kernel<T, KS, true><<<dim3(head_groups(p.N * p.HV * (p.segments - 1), transfer_parts(4, KS, p.DV))), dim3(walk_threads<T>(4)), 0, stream>>>(p);
+        delta_walk_back_kernel<T, KS, 4, true><<<dim3(head_groups(p.N * p.HV * (p.segments - 1), transfer_parts(4, KS, p.DV))), dim3(walk_threads<T>(4)), 0, stream>>>(p);
         launch_join<KS>(p, true, stream);
     }
-    delta_walk_back_kernel<T, KS, false><<<dim3(head_groups(p.N * p.HV * p.segments, (p.DV + 63) / 64)), dim3(walk_threads<T>(4)), 0, stream>>>(p);
+    bool narrow = false;
+    if constexpr (kTerms<T> == 1) {
+        narrow = two_waves(p);
+        if (narrow) delta_walk_back_kernel<T, KS, 2, false><<<dim3(head_groups(p.N * p.HV * p.segments, (p.DV + 31) / 32)), dim3(walk_threads<T>(2)), 0, stream>>>(p);
+    }
+    if (!narrow) delta_walk_back_kernel<T, KS, 4, false><<<dim3(head_groups(p.N * p.HV * p.segments, (p.DV + 63) / 64)), dim3(walk_threads<T>(4)), 0, stream>>>(p);
     const int64_t places = static_cast<int64_t>(p.N) * p.H * p.chunks, units = compute_units();
     const dim3 grid(static_cast<unsigned>(places < units ? places : units)), block(GradientPieces<T, KS>::THREADS);
     if (p.HV > p.H) delta_gradient_kernel<T, KS, true><<<grid, block, 0, stream>>>(p);
