@@ -133,19 +133,11 @@ def test_sizes(hip_ops, shape, dtype):
     check(shape, dtype, 200 + shape[0], grad=False)
 
 
-@pytest.mark.gpu
-@pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("T", [1, 3, 16, 17, 70, 150])
-def test_starts_and_lengths(hip_ops, T, dtype):
-    """Padding holds NaN in every operand, and starts of its own."""
-    N, shape = 5, (T, 5, 1, 2, 40, 24)
-    lengths = torch.tensor([0, T, (T + 1) // 2, -3, T + 9], dtype=torch.int32)
-    starts = torch.rand(T, N, generator=gen(T)) < 0.1
-    starts[0, 1] = True
+def check_padded(shape, lengths, starts, dtype):
     for grad, wide in ((False, torch.int32), (True, torch.int64)):
-        leaves, dout, dlast = operands(*shape, dtype, 300 + T)
+        leaves, dout, dlast = operands(*shape, dtype, 300 + shape[0])
         want, most = reference(*leaves, 0.2, starts, lengths, dout, dlast)
-        dead = (torch.arange(T)[:, None] >= lengths.clamp(0, T)[None, :]).to(DEV)
+        dead = (torch.arange(shape[0])[:, None] >= lengths.clamp(0, shape[0])[None, :]).to(DEV)
         for t in (*leaves[:5], dout):
             t[dead] = float("nan")
         leaves = [t.requires_grad_(grad) for t in leaves]
@@ -158,7 +150,80 @@ def test_starts_and_lengths(hip_ops, T, dtype):
             near(a, want[i], kinds[i], ((128 if i < 2 else 256) * U + coarse) * most[i], NAMES[i])
             if i not in (1, 7):
                 assert bool((a[dead] == 0).all()), NAMES[i]
-        assert torch.equal(last[0], leaves[5][0]) and torch.equal(last[3], leaves[5][3])
+        empty = lengths <= 0
+        assert torch.equal(last[empty], leaves[5][empty])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [1, 3, 16, 17, 70, 150])
+def test_starts_and_lengths(hip_ops, T, dtype):
+    """Padding holds NaN in every operand, and starts of its own."""
+    N, shape = 5, (T, 5, 1, 2, 40, 24)
+    lengths = torch.tensor([0, T, (T + 1) // 2, -3, T + 9], dtype=torch.int32)
+    starts = torch.rand(T, N, generator=gen(T)) < 0.1
+    starts[0, 1] = True
+    check_padded(shape, lengths, starts, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(700, 5, 1, 2, 40, 24), (1234, 4, 2, 2, 17, 33), (777, 2, 1, 1, 128, 70)])
+def test_long_sequences_of_few_heads(hip_ops, shape, dtype):
+    """Chunks in segments of some, of which sequences have all, some, one or none; starts in few of them. A segment's matrix times a state adds 128 u of what is left of that after 3 chunks
+    at least, 3 % with these gates."""
+    T, N = shape[:2]
+    lengths = torch.tensor([T, 449, 0, T - 1, 5][:N], dtype=torch.int32)
+    starts = torch.rand(T, N, generator=gen(T)) < 0.003
+    check_padded(shape, lengths, starts, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(70, 260, 1, 1, 17, 73), (65, 130, 1, 1, 24, 48), (65, 130, 1, 1, 70, 40), (66, 256, 1, 1, 72, 72)])
+def test_many_heads(hip_ops, shape, dtype):
+    check(shape, dtype, 400 + shape[4])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_sequences_forget(hip_ops, dtype):
+    """An infinite state is gone behind a start, whichever segment that is in, and a vanishing gate."""
+    T = 1000
+    leaves, dout, dlast = operands(T, 2, 1, 1, 32, 32, dtype, 41)
+    starts = torch.zeros(T, 2, dtype=torch.bool, device=DEV)
+    starts[500, 0] = True
+    leaves[3][300, 1] = -200.0
+    state = leaves[5].clone()
+    state[0, 0, 3], state[1, 0, 5] = float("inf"), float("nan")
+    with torch.no_grad():
+        a, b = run(*leaves[:5], state, starts=starts), run(*leaves[:5], None, starts=starts)
+    assert torch.equal(a[0][500:, 0], b[0][500:, 0]) and torch.equal(a[0][300:, 1], b[0][300:, 1]) and torch.equal(a[1], b[1])
+    assert not bool(torch.isfinite(a[0][499, 0]).all()) and bool(torch.isfinite(a[1]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [12, 100, 260])
+def test_infinities_end_at_starts(hip_ops, T, dtype):
+    """What a state and values hold of infinities and NaN reaches the steps of its own part, from the first of them on, and no others, in their own columns."""
+    leaves, _, _ = operands(T, 2, 1, 2, 16, 40, dtype, 43)
+    starts = torch.rand(T, 2, generator=gen(T)) < 0.15
+    starts[4], starts[7, 0], starts[8, 1] = True, True, True
+    parts = starts.cumsum(0)
+    value, state = leaves[2].clone(), leaves[5].clone()
+    state[1, :, :, 2] = float("inf")
+    value[5, 0, 0, 3], value[5, 0, 1, 30], value[T - 2, 1, 0, 7] = float("nan"), float("inf"), -float("inf")
+    with torch.no_grad():
+        want, last = run(*leaves, starts=starts.to(DEV))
+        out, state_out = run(leaves[0], leaves[1], value, *leaves[3:5], state, starts=starts.to(DEV))
+    reached = torch.zeros(T, 2, 2, 40, dtype=torch.bool)
+    reached[:, 1, :, 2] = (parts[:, 1] == 0)[:, None]
+    for t, n, h, c in ((5, 0, 0, 3), (5, 0, 1, 30), (T - 2, 1, 0, 7)):
+        reached[t:, n, h, c] |= parts[t:, n] == parts[t, n]
+    assert torch.equal(out.isfinite().cpu(), ~reached)
+    assert torch.equal(out[~reached.to(DEV)], want[~reached.to(DEV)])
+    assert torch.equal(state_out.isfinite().all(2).cpu(), ~reached[-1])
 
 
 @pytest.mark.gpu

@@ -120,8 +120,8 @@ struct DeltaArgs {
     float* between;                     // per head and segment but the first: the state before it
 };
 
-// Of a chunk's block: 3 terms of the inverse's fragments, `ranks` of the scores', then exp(G), exp(G_64 - G), beta [64] each, whether any of the first two is 0, and zeros.
-constexpr int kSince = 0, kUntil = kChunk, kBeta = 2 * kChunk, kBroken = 3 * kChunk, kZeros = 3 * kChunk + 4;
+// Of a chunk's block: 3 terms of the inverse's fragments, `ranks` of the scores', then exp(G), exp(G_64 - G), beta [64] each, whether any of the first two is 0, the steps that start anew as 64 bits, and zeros.
+constexpr int kSince = 0, kUntil = kChunk, kBeta = 2 * kChunk, kBroken = 3 * kChunk, kFresh = 3 * kChunk + 2, kZeros = 3 * kChunk + 4;
 __host__ __device__ __forceinline__ constexpr int block_pieces(int ranks) { return kBlocks * (3 + ranks) + 1; }      // of 256 words
 __host__ __device__ __forceinline__ constexpr int block_words(int ranks) { return block_pieces(ranks) * 256; }
 __host__ __device__ __forceinline__ constexpr int block_vectors(int ranks) { return kBlocks * (3 + ranks) * 256; }
@@ -576,6 +576,43 @@ __device__ __forceinline__ f32x4 row_factors(const uint32_t* vectors, int which,
 __device__ __forceinline__ void drop(f32x4& x, const f32x4& factor) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) x[r] = factor[r] == 0.0f ? 0.0f : x[r];
+}
+
+// In a matrix product the zeros above the diagonal and between two parts of a chunk do not keep infinities and NaN from steps that they do not concern. Where there are any (times 0 they are
+// not 0), they are taken out of x, rows in the accumulators' layout, and the rows that they are to reach, their own and those behind them in the same part, come back as bits 4 i + r.
+__device__ __forceinline__ bool all_finite(const f32x4 (&x)[4]) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum = fmaf(x[i / 4][i % 4], 0.0f, sum);
+    return __ballot(sum != 0.0f) == 0;
+}
+__device__ __forceinline__ uint32_t take_out(f32x4 (&x)[4], uint64_t fresh) {
+    const int first = 4 * ((threadIdx.x & 63) / 16);
+    uint32_t own = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const bool finite = fabsf(x[i / 4][i % 4]) < __builtin_inff();
+        own |= finite ? 0u : 1u << i;
+        x[i / 4][i % 4] = finite ? x[i / 4][i % 4] : 0.0f;
+    }
+    // bit t: step t of the lane's column
+    uint64_t rows = static_cast<uint64_t>((own & 15u) | (own & 240u) << 12 ) << first | static_cast<uint64_t>((own >> 8 & 15u) | (own >> 12) << 16) << (32 + first);
+    rows |= __shfl_xor(rows, 16, 64);
+    rows |= __shfl_xor(rows, 32, 64);
+    uint64_t open = ~fresh;             // bit t: no start among the last d steps up to t
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        rows |= open & rows << d;
+        open &= open << d;
+    }
+    const uint32_t low = static_cast<uint32_t>(rows >> first), high = static_cast<uint32_t>(rows >> (32 + first));
+    return (low & 15u) | (low >> 12 & 240u) | (high & 15u) << 8 | (high >> 16 & 15u) << 12;
+}
+__device__ __forceinline__ void put_back(f32x4 (&x)[4], uint32_t rows) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[i][r] = rows >> (4 * i + r) & 1 ? __builtin_nanf("") : x[i][r];
 }
 
 // Gates: of the activations' type or float32; none: no decay, every step learnt in full.

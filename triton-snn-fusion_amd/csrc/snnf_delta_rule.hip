@@ -93,7 +93,9 @@ __global__ __launch_bounds__(256, kTerms<T> == 3 ? 2 : 4) void delta_chunk_kerne
         vectors[kUntil + lane] = until;
         vectors[kBeta + lane] = b;
         const bool broken = __ballot(since == 0.0f || until == 0.0f) != 0;
-        vectors[kBroken + lane] = broken && lane == 0 ? 1.0f : 0.0f;
+        const uint64_t starts = __ballot(fresh);
+        const uint32_t word = lane == 0 ? __float_as_uint(broken ? 1.0f : 0.0f) : (lane == 2 ? static_cast<uint32_t>(starts) : (lane == 3 ? static_cast<uint32_t>(starts >> 32) : 0u));
+        vectors[kBroken + lane] = __uint_as_float(word);
     }
     f32x4 kk[4], qk[4];
 #pragma unroll
@@ -342,11 +344,15 @@ __global__ __launch_bounds__(kTerms<T> == 1 && walk_threads<T>(WAVES, WALK != kT
         }
         // delta
         now();
+        uint32_t infinite = 0;
+        bool finite;
         Terms<RANKS> scores[kBlocks];
         f32x4 beta[4];
         {
 #pragma unroll
             for (int i = 0; i < 4; ++i) right[i] -= since[i] * ks[i];
+            finite = all_finite(right);
+            if (!finite) infinite = take_out(right, vectors[kFresh] | static_cast<uint64_t>(vectors[kFresh + 1]) << 32);
 #pragma unroll
             for (int f = PIPE == 2 ? 2 : 0; f < kBlocks; ++f) inverse[f] = block_terms<3>(block, f);
             const Terms<3> y[2] = {split<3>(right[0], right[1]), split<3>(right[2], right[3])};
@@ -378,17 +384,12 @@ __global__ __launch_bounds__(kTerms<T> == 1 && walk_threads<T>(WAVES, WALK != kT
         f32x4 until[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) until[i] = row_factors(vectors, kUntil, i), delta[i] *= beta[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) right[i] = delta[i];
+        if (!finite) put_back(right, infinite);
         if (broken) {
-            f32x4 left_over[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                left_over[i] = delta[i];
-                drop(left_over[i], until[i]);
-                right[i] = left_over[i];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) right[i] = delta[i];
+            for (int i = 0; i < 4; ++i) drop(right[i], until[i]);
         }
         now();
         {
@@ -423,6 +424,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 && walk_threads<T>(WAVES, WALK != kT
                             for (int d = 0; d < 2 * KS; ++d) state[d] = mfma(k[half % PIPE][d].t[j], y.t[rank - j], state[d]);
                         }
             }
+            if (!TRANSFER && !finite) put_back(out, infinite);
             if constexpr (!TRANSFER) Values::turn_values(tile, out);
         }
         now();
