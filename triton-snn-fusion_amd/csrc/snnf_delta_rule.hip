@@ -535,9 +535,24 @@ __device__ __forceinline__ float sum_of_rows(float v) {      // over the four ro
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Of four numbers at once: row g of 16 lanes gets the sum of the g-th.
+__device__ __forceinline__ float sums_of_rows(float a, float b, float c, float d) {
+    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(c), __float_as_uint(d), false, false);
+    const float ab = __uint_as_float(x[0]) + __uint_as_float(x[1]), cd = __uint_as_float(y[0]) + __uint_as_float(y[1]);
+    const auto z = __builtin_amdgcn_permlane32_swap(__float_as_uint(ab), __float_as_uint(cd), false, false);
+    return __uint_as_float(z[0]) + __uint_as_float(z[1]);
+}
+
+constexpr int kFewSteps = 16;
+
 template <typename T, int KS>
 __global__ __launch_bounds__(64 * KS) void delta_step_kernel(DeltaArgs p) {
-    __shared__ float sums[2][KS][16][9];
+    constexpr int PER = 4 * KS, COLUMNS = 64 / PER;     // pieces of 8 elements of a head, of which a thread has one of one step, and columns that it has of that
+    static_assert(kFewSteps * PER == 64 * KS, "a thread to a piece");
+    __shared__ alignas(16) float keys[kFewSteps][32 * KS], queries[kFewSteps][32 * KS], values[kFewSteps][64];
+    __shared__ float decays[kFewSteps], rates[kFewSteps];
+    __shared__ f32x4 sums[2][KS][16][3];
     int head, columns;
     if (!part_of_head(p.N * p.HV, (p.DV + 63) / 64, &head, &columns)) return;
     const int n = head / p.HV, hv = head % p.HV, h = hv / (p.HV / p.H), limit = length_of(p, n);
@@ -550,29 +565,52 @@ __global__ __launch_bounds__(64 * KS) void delta_step_kernel(DeltaArgs p) {
         if (p.state != nullptr && row + i < p.DK && left > 0) state[i].load(p.state + cell, static_cast<int64_t>(row + i) * p.DV, left);
         else state[i].clear();
     }
+    // All steps' keys, queries, values and gates at once, to LDS
+    {
+        const int t = threadIdx.x / PER, piece = threadIdx.x % PER, at = 8 * piece, first = columns * 64 + COLUMNS * piece;
+        Raw<T, 8> k, q;
+        float v[COLUMNS];
+        k.clear();
+        q.clear();
+        if (t < limit && at < p.DK) {
+            k.load(static_cast<const T*>(p.k.data) + n * p.k.row + h * p.k.head, t * p.k.step + at, p.DK - at);
+            q.load(static_cast<const T*>(p.q.data) + n * p.q.row + h * p.q.head, t * p.q.step + at, p.DK - at);
+        }
+#pragma unroll
+        for (int c = 0; c < COLUMNS; ++c)
+            v[c] = t < limit && first + c < p.DV ? to_float(static_cast<const T*>(p.v.data)[n * p.v.row + hv * p.v.head + t * p.v.step + first + c]) : 0.0f;
+        if (static_cast<int>(threadIdx.x) < limit) {
+            const int64_t step = threadIdx.x;
+            const float g = gate_value<T>(p.gate, p.gate_float, threadIdx.x, n, hv, 0.0f);
+            const bool fresh = g < kForgotten || (p.starts != nullptr && p.starts[step * p.starts_step + n * p.starts_row] != 0);
+            decays[threadIdx.x] = fresh ? 0.0f : expf(g);
+            rates[threadIdx.x] = gate_value<T>(p.beta, p.gate_float, threadIdx.x, n, hv, 1.0f);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) keys[t][at + j] = k[j], queries[t][at + j] = q[j];
+#pragma unroll
+        for (int c = 0; c < COLUMNS; ++c) values[t][COLUMNS * piece + c] = v[c];
+    }
+    __syncthreads();
     float s[8][4];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[i][c] = state[i][c];
-    const T* keys = static_cast<const T*>(p.k.data) + n * p.k.row + h * p.k.head;
-    const T* queries = static_cast<const T*>(p.q.data) + n * p.q.row + h * p.q.head;
-    const T* values = static_cast<const T*>(p.v.data) + n * p.v.row + hv * p.v.head + column;
     T* outs = static_cast<T*>(const_cast<void*>(p.out.data)) + n * p.out.row + hv * p.out.head + column;
     for (int t = 0; t < limit; ++t) {
-        Raw<T, 8> k, q;
-        k.clear();
-        q.clear();
-        if (row < p.DK) {
-            k.load(keys, t * p.k.step + row, p.DK - row);
-            q.load(queries, t * p.q.step + row, p.DK - row);
-        }
-        float v[4];
+        const float a = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(decays[t]))), b = rates[t];
+        float k[8], q[8], v[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = c < left ? to_float(values[t * p.v.step + c]) : 0.0f;
-        const float g = gate_value<T>(p.gate, p.gate_float, t, n, hv, 0.0f), b = gate_value<T>(p.beta, p.gate_float, t, n, hv, 1.0f);
-        const bool fresh = g < kForgotten || (p.starts != nullptr && p.starts[t * p.starts_step + n * p.starts_row] != 0);
-        const float a = fresh ? 0.0f : expf(g);
+        for (int i = 0; i < 8; ++i) k[i] = keys[t][row + i], q[i] = queries[t][row + i];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] = values[t][4 * (lane % 16) + c];
+        if (a == 0.0f) {                // infinities and NaN as well
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s[i][c] = 0.0f;
+        }
         float part[9];
 #pragma unroll
         for (int c = 0; c < 9; ++c) part[c] = 0.0f;
@@ -581,22 +619,28 @@ __global__ __launch_bounds__(64 * KS) void delta_step_kernel(DeltaArgs p) {
             part[8] = fmaf(k[i], q[i], part[8]);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                s[i][c] = kept(a, s[i][c]);
+                s[i][c] *= a;
                 part[c] = fmaf(k[i], s[i][c], part[c]);
                 part[4 + c] = fmaf(q[i], s[i][c], part[4 + c]);
             }
         }
 #pragma unroll
-        for (int c = 0; c < 9; ++c) {
-            part[c] = sum_of_rows(part[c]);
-            if (lane < 16) sums[t & 1][wave][lane][c] = part[c];
-        }
+        for (int i = 0; i < 2; ++i) sums[t & 1][wave][lane % 16][i][lane / 16] = sums_of_rows(part[4 * i], part[4 * i + 1], part[4 * i + 2], part[4 * i + 3]);
+        sums[t & 1][wave][lane % 16][2][0] = sum_of_rows(part[8]);
         __syncthreads();
+        f32x4 all[KS][2];
+        float dots[KS];
+#pragma unroll
+        for (int w = 0; w < KS; ++w) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) all[w][i] = sums[t & 1][w][lane % 16][i];
+            dots[w] = sums[t & 1][w][lane % 16][2][0];
+        }
 #pragma unroll
         for (int c = 0; c < 9; ++c) {
-            part[c] = sums[t & 1][0][lane % 16][c];
+            part[c] = c < 8 ? all[0][c / 4][c % 4] : dots[0];
 #pragma unroll
-            for (int w = 1; w < KS; ++w) part[c] += sums[t & 1][w][lane % 16][c];
+            for (int w = 1; w < KS; ++w) part[c] += c < 8 ? all[w][c / 4][c % 4] : dots[w];
         }
         float u[4];
 #pragma unroll
@@ -628,8 +672,6 @@ __global__ __launch_bounds__(64 * KS) void delta_step_kernel(DeltaArgs p) {
 // ------------------------------------------------------------------------------------------------------------------
 // Launch
 // ------------------------------------------------------------------------------------------------------------------
-constexpr int kFewSteps = 16;
-
 template <typename T, int KS, int WAVES>
 void launch_walk(const DeltaArgs& p, hipStream_t stream) {
     const dim3 grid(head_groups(p.N * p.HV * p.segments, (p.DV + 16 * WAVES - 1) / (16 * WAVES))), block(walk_threads<T>(WAVES));
