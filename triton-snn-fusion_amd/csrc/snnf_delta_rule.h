@@ -682,8 +682,8 @@ inline bool near_by(const HeadView& x, int dtype, bool read) {
     const bool reach = x.step >= 0 && x.step <= 0x7fffffff / (kChunk * dtype_size(dtype)) - 1024;
     return reach && (!read || dtype != SNNF_BF16 || (aligned_to(x.data, 16) && (x.step | x.row | x.head) % 8 == 0));
 }
-// Eight waves share a head's keys in LDS where heads alone fill the chip, else four.
-inline bool eight_waves(const DeltaArgs& p) { return p.DV > 64 && p.N * p.HV >= compute_units(); }
-// Two waves of 16 columns where four leave half of the chip idle
+// Workgroups of 32 value columns where those of 64 leave half of the chip idle: half as much to read and write for each (4096 x 4 x 16 heads of 128 bfloat16, forward and backward: 1109 us, with 64 columns
+// 1187). Of 128, with eight waves, a head's keys are read once, but no room is left for waves that load: 16, 20 and 32 x 16 heads of 1024 steps take 216, 335 and 400 us, with 64 columns 214, 268
+// and 384.
 inline bool two_waves(const DeltaArgs& p) { return p.DV > 32 && 2 * p.N * p.HV * p.segments * ((p.DV + 63) / 64) <= compute_units(); }
 }  // namespace snnf

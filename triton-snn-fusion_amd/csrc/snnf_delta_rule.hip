@@ -691,12 +691,6 @@ void launch_forward(const DeltaArgs& p, hipStream_t stream) {
         delta_walk_kernel<T, KS, WAVES, kTransfer><<<dim3(head_groups(p.N * p.HV * (p.segments - 1), transfer_parts(WAVES, KS, p.DV))), dim3(walk_threads<T>(WAVES, false)), 0, stream>>>(p);
         launch_join<KS>(p, false, stream);
     }
-    if constexpr (sizeof(T) == 2) {
-        if (eight_waves(p)) {
-            launch_walk<T, KS, 8>(p, stream);
-            return;
-        }
-    }
     if constexpr (kTerms<T> == 1) {
         if (two_waves(p)) {
             launch_walk<T, KS, 2>(p, stream);
@@ -715,9 +709,12 @@ void launch_join(const DeltaArgs& p, bool backward, hipStream_t stream) {
 template void launch_join<2>(const DeltaArgs&, bool, hipStream_t);
 template void launch_join<4>(const DeltaArgs&, bool, hipStream_t);
 
+// As many as fill the chip on both walks, of 3 chunks at least, no more than the states between them are worth (a step there costs a third of a chunk), and 3 at least: with 2 the
+// first walk takes the time that the second saves. Two more launches cost what 6 to 10 chunks of a walk do (16 heads of 128, with and without segments: bfloat16 16 chunks 67 and 66 us,
+// 20 72 and 81, 32 82 and 115; float16 9 chunks 78 and 73, 12 82 and 93; float32 9 chunks 89 and 105).
 int delta_segments(const snnf_delta_rule_call* c, bool backward) {
     const int64_t heads = static_cast<int64_t>(c->N) * c->value_heads, chunks = (c->T + kChunk - 1) / kChunk, units = compute_units();
-    if (heads == 0 || heads > units) return 1;
+    if (heads == 0 || heads > units || chunks <= (c->dtype == SNNF_BF16 ? 16 : 9)) return 1;
     const int waves = dtype_size(c->dtype) == 2 && !backward ? 8 : 4;
     int64_t segments = 1 + units / (heads * transfer_parts(waves, c->key_size <= 64 ? 2 : 4, c->value_size));
     segments = std::min(segments, units / (heads * ((c->value_size + 63) / 64)));
