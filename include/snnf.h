@@ -558,7 +558,8 @@ typedef struct snnf_delta_rule_call {
 /*   state_out  as state; may be the same memory, and overlaps it in no other way      out  overlaps no input
  *   marks      NULL, or snnf_delta_rule_marks_bytes(call) bytes, 16-byte aligned, that the backward pass will read
  *   workspace  snnf_delta_rule_workspace_bytes(call, marks != NULL) bytes, 16-byte aligned (0: none needed), in use until the call's work is done
- * A gate below -104 drops the state as a start does. Two launches, one for up to 16 steps without marks. */
+ * A gate below -104 drops the state as a start does. Infinities and NaN of states and values reach no step before them and none behind a start;
+ * those of keys, beta and gates any step of the same 64. Two launches, four where heads are few and steps many, one for up to 16 steps without marks. */
 size_t snnf_delta_rule_workspace_bytes(const snnf_delta_rule_call* call, int training);
 size_t snnf_delta_rule_marks_bytes(const snnf_delta_rule_call* call);
 int snnf_delta_rule(const snnf_delta_rule_call* call, const snnf_heads* out, float* state_out, void* marks, void* workspace, size_t workspace_bytes,
@@ -567,7 +568,7 @@ int snnf_delta_rule(const snnf_delta_rule_call* call, const snnf_heads* out, flo
 /* Its gradient: `dout` and `dstate` (NULL: zeros) are the gradients of `out` and of the last state; dquery, dkey, dvalue, dgate, dbeta (data NULL: not wanted) and
  * dstate_in (not dstate's memory) those of the operands, of their types; they overlap no input. Steps from a sequence's length on get 0, as does a gate that
  * a start or its own value makes meaningless. `marks` as the forward call on the same operands left them; call->state is not read.
- * Workspace: snnf_delta_rule_backward_workspace_bytes(call) bytes, 16-byte aligned. Three launches; sums have a fixed order. */
+ * Workspace: snnf_delta_rule_backward_workspace_bytes(call) bytes, 16-byte aligned. Three launches, five where heads are few and steps many; sums have a fixed order. */
 size_t snnf_delta_rule_backward_workspace_bytes(const snnf_delta_rule_call* call);
 int snnf_delta_rule_backward(const snnf_delta_rule_call* call, const void* marks, const snnf_heads* dout, const float* dstate, const snnf_heads* dquery,
                              const snnf_heads* dkey, const snnf_heads* dvalue, const snnf_heads* dgate, const snnf_heads* dbeta, float* dstate_in,

@@ -359,6 +359,18 @@ def test_state_in_place(hip_ops, T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_state_in_place_of_long_sequences(hip_ops, dtype):
+    leaves, _, _ = operands(1200, 2, 1, 2, 50, 70, dtype, 62)
+    lengths = torch.tensor([1200, 130], dtype=torch.int32, device=DEV)
+    want = run(*leaves, lengths=lengths)
+    for _ in range(3):
+        state = leaves[5].clone()
+        out, last = run(*leaves[:5], state, lengths=lengths, state_out=state)
+        assert last is state and torch.equal(out, want[0]) and torch.equal(state, want[1])
+
+
+@pytest.mark.gpu
 def test_steps_one_by_one_and_together(hip_ops):
     """A sequence in pieces, the state handed on: each piece is right for itself, so the whole is."""
     leaves, _, _ = operands(100, 2, 1, 2, 64, 32, torch.float32, 71)

@@ -117,7 +117,7 @@ struct DeltaArgs {
     // Few heads: chunks in segments of `per`, walked side by side
     int segments, per;
     float* transfers;                   // per head and segment but the last walked: what it makes of a state (below)
-    float* between;                     // per head and segment but the first: the state before it
+    float* between;                     // per head and segment: the state before it (backward: the gradient of the state behind it, of all but the last)
 };
 
 // Of a chunk's block: 3 terms of the inverse's fragments, `ranks` of the scores', then exp(G), exp(G_64 - G), beta [64] each, whether any of the first two is 0, the steps that start anew as 64 bits, and zeros.

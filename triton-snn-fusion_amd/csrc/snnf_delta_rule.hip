@@ -269,9 +269,11 @@ __global__ __launch_bounds__(kTerms<T> == 1 && walk_threads<T>(WAVES, WALK != kT
             return;
         }
     const int64_t cell = static_cast<int64_t>(head) * p.DK * p.DV + column;
+    // The first of several segments has its state from a copy: the last one's may take its place meanwhile.
+    float* slot = p.segments > 1 ? p.between + (static_cast<int64_t>(head) * p.segments + segment) * p.DK * p.DV + column : nullptr;
     const float* before = nullptr;
-    if (segment == 0) before = p.state == nullptr ? nullptr : p.state + cell;
-    else if constexpr (!TRANSFER) before = p.between + (static_cast<int64_t>(head) * (segments - 1) + segment - 1) * p.DK * p.DV + column;
+    if (TRANSFER || last == 0) before = segment > 0 || p.state == nullptr ? nullptr : p.state + cell;
+    else before = slot;
     f32x4 state[2 * KS];
 #pragma unroll
     for (int d = 0; d < 2 * KS; ++d)
@@ -280,6 +282,13 @@ __global__ __launch_bounds__(kTerms<T> == 1 && walk_threads<T>(WAVES, WALK != kT
             const int row = head_element(d, r);
             state[d][r] = before != nullptr && there && row < p.DK ? before[static_cast<int64_t>(row) * p.DV] : (matrix && row == column ? 1.0f : 0.0f);
         }
+    if (TRANSFER && segment == 0) {
+#pragma unroll
+        for (int d = 0; d < 2 * KS; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (there && head_element(d, r) < p.DK) slot[static_cast<int64_t>(head_element(d, r)) * p.DV] = state[d][r];
+    }
     bool forgotten = false;
     if constexpr (!Reader::kLoaders) fetch(begin);
     for (int chunk = begin; chunk < live; ++chunk) {
@@ -457,7 +466,7 @@ __global__ __launch_bounds__(64 * KS) void delta_join_kernel(DeltaArgs p, int ba
     const int n = head / p.HV, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, column = 16 * tile + lane % 16;
     const int chunks = (length_of(p, n) + kChunk - 1) / kChunk, last = chunks == 0 ? 0 : (chunks - 1) / p.per;
     const float* transfers = p.transfers + static_cast<int64_t>(head) * (p.segments - 1) * transfer_floats(KS, p.DV);
-    float* between = p.between + static_cast<int64_t>(head) * (p.segments - 1) * p.DK * p.DV;
+    float* between = p.between + static_cast<int64_t>(head) * p.segments * p.DK * p.DV;
     // Rows of the matrix as the accumulators have them, the wave's columns of it as they lie in the other operand; what the segment adds to the wave's own rows
     struct Segment {
         f32x4 matrix[2 * KS][2];
@@ -504,7 +513,7 @@ __global__ __launch_bounds__(64 * KS) void delta_join_kernel(DeltaArgs p, int ba
 #pragma unroll
                 for (int w = 0; w < KS; ++w) state[i] += parts[step % 2][w][2 * wave + i][lane];
             }
-            float* to = between + static_cast<int64_t>(backward ? last - 1 - step : step) * p.DK * p.DV;
+            float* to = between + static_cast<int64_t>(backward ? last - 1 - step : step + 1) * p.DK * p.DV;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int row = head_element(2 * wave + i, r);
@@ -725,8 +734,8 @@ int delta_segments(const snnf_delta_rule_call* c, bool backward) {
     return static_cast<int>((chunks + per - 1) / per);
 }
 size_t delta_segment_floats(const snnf_delta_rule_call* c, bool backward) {
-    return static_cast<size_t>(c->N) * c->value_heads * (delta_segments(c, backward) - 1) *
-           (transfer_floats(c->key_size <= 64 ? 2 : 4, c->value_size) + static_cast<size_t>(c->key_size) * c->value_size);
+    const int64_t heads = static_cast<int64_t>(c->N) * c->value_heads, segments = delta_segments(c, backward);
+    return segments == 1 ? 0 : static_cast<size_t>(heads * ((segments - 1) * transfer_floats(c->key_size <= 64 ? 2 : 4, c->value_size) + segments * c->key_size * c->value_size));
 }
 void set_segments(DeltaArgs& p, const snnf_delta_rule_call* c, bool backward, float* workspace) {
     p.segments = delta_segments(c, backward);

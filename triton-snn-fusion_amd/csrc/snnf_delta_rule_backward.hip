@@ -61,7 +61,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
     const int64_t cell = static_cast<int64_t>(head) * p.DK * p.DV + column;
     const float* behind = nullptr;
     if (segment == last) behind = p.dstate == nullptr ? nullptr : p.dstate + cell;
-    else if constexpr (!TRANSFER) behind = p.between + (static_cast<int64_t>(head) * (segments - 1) + segment) * p.DK * p.DV + column;
+    else if constexpr (!TRANSFER) behind = p.between + (static_cast<int64_t>(head) * segments + segment) * p.DK * p.DV + column;
     f32x4 later[2 * KS];
 #pragma unroll
     for (int d = 0; d < 2 * KS; ++d)

@@ -162,8 +162,8 @@ def run_hip_delta_rule(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
         tokens that are not accepted are left out this way: lengths is their number and one.
     state_out: memory for the returned state, contiguous, without gradients; may be state itself.
 
-    Up to 16 steps without gradients are taken one by one, others in chunks of 64. A value that is not finite, or overflows, makes the outputs of its chunk, those before it
-    among them, and the state from there on NaN, across starts inside that chunk; a later start drops it.
+    Up to 16 steps without gradients are taken one by one, others in chunks of 64. Infinities and NaN of states and values stay in their columns, reach no
+    step before them and none behind a start; those of keys, beta and gates, and of any operand in the gradients, may reach every step of their chunk.
     Sums, states and decays are float32 or more, out is rounded once. Differentiable once, backwards, in query, key, value, gate, beta and state (forward
     mode, torch.func and tracing are refused); the gradients of a head's queries and keys are summed over its value heads in a fixed order.
     """
