@@ -371,6 +371,29 @@ def test_state_in_place_of_long_sequences(hip_ops, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_sequences_in_a_graph(hip_ops, dtype):
+    """Replays with other work and another call of the same kind between them."""
+    leaves, _, _ = operands(1200, 1, 1, 2, 30, 40, dtype, 63)
+    other, _, _ = operands(1300, 2, 1, 1, 30, 40, dtype, 64)
+    with torch.no_grad():
+        expected = run(*other)
+        run(*leaves)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out, last = run(*leaves)
+        for i in range(4):
+            for t in leaves[2:3] + leaves[5:]:
+                t.mul_(0.5)
+            graph.replay()
+            again = run(*other)
+            want = run(*leaves)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want[0]) and torch.equal(last, want[1]) and torch.equal(again[0], expected[0]) and torch.equal(again[1], expected[1])
+
+
+@pytest.mark.gpu
 def test_steps_one_by_one_and_together(hip_ops):
     """A sequence in pieces, the state handed on: each piece is right for itself, so the whole is."""
     leaves, _, _ = operands(100, 2, 1, 2, 64, 32, torch.float32, 71)
@@ -423,6 +446,29 @@ def test_refusals():
         run_hip_delta_rule(t, t, t)
     assert check_delta_rule_support(t.to(torch.float64), t, t)
     assert check_delta_rule_support(None, t, t)
+
+
+def test_refusals_of_the_c_entries():
+    """Before anything is launched: no address here is one of memory."""
+    import ctypes
+
+    from triton_snn_fusion_amd import _lib
+    lib = _lib.lib()
+    heads = lambda at: _lib.Heads(at, 64, 64, 32)
+    call = _lib.DeltaRuleCall(2000, 1, 2, 2, 32, 32, _lib.dtype_code(torch.bfloat16), _lib.dtype_code(torch.float32), 1.0, heads(4096), heads(4096), heads(4096), heads(None), heads(None),
+                              None, 0, 0, None, None)
+    need, back = lib.snnf_delta_rule_workspace_bytes(ctypes.byref(call), 1), lib.snnf_delta_rule_backward_workspace_bytes(ctypes.byref(call))
+    assert need % 4 == 0 and back % 4 == 0 and need > 0 and back > need
+    out = [heads(8192) for _ in range(6)]
+    forward = lambda marks, space, size, o=out[0], last=8192: lib.snnf_delta_rule(ctypes.byref(call), ctypes.byref(o), last, marks, space, size, None)
+    backward = lambda marks, space, size, o=out[0]: lib.snnf_delta_rule_backward(ctypes.byref(call), marks, ctypes.byref(o), None, *(ctypes.byref(x) for x in out[1:]), 8192, space, size, None)
+    for rc in (forward(8200, 4096, need), forward(8192, 4096, need - 1), forward(8192, 4100, need), forward(8192, None, need), forward(None, 4096, need, heads(None)), forward(8192, 4096, need, last=None),
+               backward(8200, 4096, back), backward(8192, 4096, back - 1), backward(8192, 4104, back), backward(None, 4096, back), backward(8192, 4096, back, heads(None))):
+        assert rc != 0
+    call.value_heads = 3
+    assert forward(8192, 4096, need) != 0 and lib.snnf_delta_rule_workspace_bytes(ctypes.byref(call), 1) == 0
+    call.value_heads, call.key_size = 2, 129
+    assert forward(8192, 4096, need) != 0 and backward(8192, 4096, back) != 0
 
 
 @pytest.mark.gpu

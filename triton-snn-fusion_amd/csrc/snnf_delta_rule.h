@@ -655,12 +655,12 @@ __device__ __forceinline__ float kept(float factor, float x) { return factor == 
 // different dies. False: nothing to do.
 __device__ __forceinline__ bool part_of_head(int heads, int parts, int* head, int* part) {
     constexpr int kDies = 8;
-    const int die = blockIdx.x % kDies, order = blockIdx.x / kDies;
+    const int index = static_cast<int>(group_index()), die = index % kDies, order = index / kDies;
     *part = order % parts;
     *head = order / parts * kDies + die;
     return *head < heads;
 }
-inline unsigned head_groups(int heads, int parts) { return static_cast<unsigned>((heads + 7) / 8 * 8 * parts); }
+inline dim3 head_grid(int heads, int parts) { return grid_of(static_cast<int64_t>((heads + 7) / 8 * 8) * parts); }
 
 // Fragments, decays and inverses of all chunks; transposed for the backward pass.
 template <typename T, int KS, bool BACKWARD> void launch_chunks(const DeltaArgs& p, hipStream_t stream);

@@ -690,7 +690,7 @@ __global__ __launch_bounds__(64 * KS) void delta_step_kernel(DeltaArgs p) {
 // ------------------------------------------------------------------------------------------------------------------
 template <typename T, int KS, int WAVES>
 void launch_walk(const DeltaArgs& p, hipStream_t stream) {
-    const dim3 grid(head_groups(p.N * p.HV * p.segments, (p.DV + 16 * WAVES - 1) / (16 * WAVES))), block(walk_threads<T>(WAVES));
+    const dim3 grid(head_grid(p.N * p.HV * p.segments, (p.DV + 16 * WAVES - 1) / (16 * WAVES))), block(walk_threads<T>(WAVES));
     if (p.marks != nullptr) delta_walk_kernel<T, KS, WAVES, kTraining><<<grid, block, 0, stream>>>(p);
     else delta_walk_kernel<T, KS, WAVES, kOutputs><<<grid, block, 0, stream>>>(p);
 }
@@ -698,13 +698,13 @@ void launch_walk(const DeltaArgs& p, hipStream_t stream) {
 template <typename T, int KS>
 void launch_forward(const DeltaArgs& p, hipStream_t stream) {
     if (p.blocks == nullptr) {
-        delta_step_kernel<T, KS><<<dim3(head_groups(p.N * p.HV, (p.DV + 63) / 64)), dim3(64 * KS), 0, stream>>>(p);
+        delta_step_kernel<T, KS><<<head_grid(p.N * p.HV, (p.DV + 63) / 64), dim3(64 * KS), 0, stream>>>(p);
         return;
     }
     launch_chunks<T, KS, false>(p, stream);
     if (p.segments > 1) {
         constexpr int WAVES = sizeof(T) == 2 ? 8 : 4;
-        delta_walk_kernel<T, KS, WAVES, kTransfer><<<dim3(head_groups(p.N * p.HV * (p.segments - 1), transfer_parts(WAVES, KS, p.DV))), dim3(walk_threads<T>(WAVES, false)), 0, stream>>>(p);
+        delta_walk_kernel<T, KS, WAVES, kTransfer><<<head_grid(p.N * p.HV * (p.segments - 1), transfer_parts(WAVES, KS, p.DV)), dim3(walk_threads<T>(WAVES, false)), 0, stream>>>(p);
         launch_join<KS>(p, false, stream);
     }
     if constexpr (kTerms<T> == 1) {
@@ -720,7 +720,7 @@ void launch_forward(const DeltaArgs& p, hipStream_t stream) {
 
 template <int KS>
 void launch_join(const DeltaArgs& p, bool backward, hipStream_t stream) {
-    delta_join_kernel<KS><<<dim3(head_groups(p.N * p.HV, (p.DV + 15) / 16)), dim3(64 * KS), 0, stream>>>(p, backward);
+    delta_join_kernel<KS><<<head_grid(p.N * p.HV, (p.DV + 15) / 16), dim3(64 * KS), 0, stream>>>(p, backward);
 }
 template void launch_join<2>(const DeltaArgs&, bool, hipStream_t);
 template void launch_join<4>(const DeltaArgs&, bool, hipStream_t);
@@ -835,6 +835,7 @@ extern "C" int snnf_delta_rule(const snnf_delta_rule_call* call, const snnf_head
         set_segments(p, call, false, reinterpret_cast<float*>(p.blocks + delta_chunks(call) * block_words(delta_ranks(call))));
     }
     if (marks != nullptr) {
+        if (!aligned_to(marks, 16)) return fail(SNNF_ERR_INVALID_ARGUMENT, "snnf_delta_rule: marks must lie on 16 bytes");
         p.marks = static_cast<uint16_t*>(marks);
         p.deltas = p.marks + delta_chunks(call) * delta_mark_elements(call);
     }

@@ -683,15 +683,15 @@ template <typename T, int KS>
 void launch_backward(const DeltaArgs& p, hipStream_t stream) {
     launch_chunks<T, KS, true>(p, stream);
     if (p.segments > 1) {
-        delta_walk_back_kernel<T, KS, 4, true><<<dim3(head_groups(p.N * p.HV * (p.segments - 1), transfer_parts(4, KS, p.DV))), dim3(walk_threads<T>(4)), 0, stream>>>(p);
+        delta_walk_back_kernel<T, KS, 4, true><<<head_grid(p.N * p.HV * (p.segments - 1), transfer_parts(4, KS, p.DV)), dim3(walk_threads<T>(4)), 0, stream>>>(p);
         launch_join<KS>(p, true, stream);
     }
     bool narrow = false;
     if constexpr (kTerms<T> == 1) {
         narrow = two_waves(p);
-        if (narrow) delta_walk_back_kernel<T, KS, 2, false><<<dim3(head_groups(p.N * p.HV * p.segments, (p.DV + 31) / 32)), dim3(walk_threads<T>(2)), 0, stream>>>(p);
+        if (narrow) delta_walk_back_kernel<T, KS, 2, false><<<head_grid(p.N * p.HV * p.segments, (p.DV + 31) / 32), dim3(walk_threads<T>(2)), 0, stream>>>(p);
     }
-    if (!narrow) delta_walk_back_kernel<T, KS, 4, false><<<dim3(head_groups(p.N * p.HV * p.segments, (p.DV + 63) / 64)), dim3(walk_threads<T>(4)), 0, stream>>>(p);
+    if (!narrow) delta_walk_back_kernel<T, KS, 4, false><<<head_grid(p.N * p.HV * p.segments, (p.DV + 63) / 64), dim3(walk_threads<T>(4)), 0, stream>>>(p);
     const int64_t places = static_cast<int64_t>(p.N) * p.H * p.chunks, units = compute_units();
     const dim3 grid(static_cast<unsigned>(places < units ? places : units)), block(GradientPieces<T, KS>::THREADS);
     if (p.HV > p.H) delta_gradient_kernel<T, KS, true><<<grid, block, 0, stream>>>(p);
@@ -720,6 +720,7 @@ extern "C" int snnf_delta_rule_backward(const snnf_delta_rule_call* call, const 
     if (call->query.data == nullptr || call->key.data == nullptr || call->value.data == nullptr || marks == nullptr || missing(dout) || missing(dquery) || missing(dkey) ||
         missing(dvalue) || dgate == nullptr || dbeta == nullptr || dstate_in == nullptr)
         return fail(SNNF_ERR_INVALID_ARGUMENT, "snnf_delta_rule_backward: operands, marks, dout and what gradients are written to must be non-null");
+    if (!aligned_to(marks, 16)) return fail(SNNF_ERR_INVALID_ARGUMENT, "snnf_delta_rule_backward: marks must lie on 16 bytes");
     const size_t need = snnf_delta_rule_backward_workspace_bytes(call);
     if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
         return fail(SNNF_ERR_WORKSPACE, "snnf_delta_rule_backward: workspace of %zu bytes needed, got %zu", need, workspace_bytes);
