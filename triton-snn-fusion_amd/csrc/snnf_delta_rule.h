@@ -196,21 +196,6 @@ __device__ __forceinline__ Terms<kTerms<T>> terms_of(const Raw<T, 8>& raw) {
         return split<kTerms<T>>(x);
     }
 }
-// 8 elements of a row from `at` on, zeros behind its end.
-template <typename T>
-__device__ __forceinline__ Terms<kTerms<T>> row_terms(const T* row, int at, int width) {
-    Raw<T, 8> raw;
-    raw.load(row, at, width - at);
-    return terms_of(raw);
-}
-template <int N>
-__device__ __forceinline__ Terms<N> no_terms() {
-    Terms<N> r;
-#pragma unroll
-    for (int n = 0; n < N; ++n) r.t[n] = u32x4a{0, 0, 0, 0};
-    return r;
-}
-
 // Fragment f = 0..5 of a lower triangular [64 x 64] matrix: rows of tile 0, 1, 2, 2, 3, 3, columns of half 0, 0, 0, 1, 0, 1. Of an upper one
 // (a transposed lower one): rows of tile 0, 0, 1, 1, 2, 3, columns of half 0, 1, 0, 1, 1, 1.
 __device__ __forceinline__ constexpr int lower_tile(int f) { return f < 2 ? f : (f < 4 ? 2 : 3); }
