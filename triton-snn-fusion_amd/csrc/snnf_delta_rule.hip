@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256, kTerms<T> == 3 ? 2 : 4) void delta_chunk_kerne
     const int chunk = index % p.chunks, head = index / p.chunks, n = head / p.HV, hv = head % p.HV, h = hv / (p.HV / p.H);
     const int first = chunk * kChunk, limit = length_of(p, n);
     if (first >= limit) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane / 16, column = lane % 16;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane / 16, column = lane % 16;
     uint32_t* blocks = p.blocks + static_cast<int64_t>(index) * block_words(RANKS);
     float* vectors = reinterpret_cast<float*>(blocks + block_vectors(RANKS));
 
