@@ -187,6 +187,46 @@ def test_many_heads(hip_ops, shape, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(40, 1, 1, 64, 16, 16), (70, 1, 1, 1, 1, 1024), (1200, 1, 1, 1, 1, 700), (1200, 1, 1, 1, 128, 96), (20, 700, 1, 1, 8, 8), (65, 1, 64, 64, 4, 4)])
+def test_extremes(hip_ops, shape, dtype):
+    check(shape, dtype, 500 + shape[5])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_sequences_on_two_streams(hip_ops, dtype):
+    one, _, _ = operands(1400, 1, 2, 4, 64, 64, dtype, 44)
+    two, _, _ = operands(1500, 2, 1, 1, 128, 128, dtype, 45)
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.no_grad():
+        want = [*run(*one), *run(*two)]
+        for _ in range(3):
+            torch.cuda.synchronize()
+            got = []
+            for leaves, stream in zip((one, two), streams):
+                with torch.cuda.stream(stream):
+                    got += run(*leaves)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_long_sequence_in_pieces(hip_ops):
+    """60000 steps at once, in segments, and in pieces of 8 chunks that are walked in one go: either way a state is off by 128 u of its size at most."""
+    leaves, _, _ = operands(60000, 1, 1, 1, 32, 32, torch.float32, 46)
+    with torch.no_grad():
+        out, last = run(*leaves)
+        state, outs = leaves[5], []
+        for i in range(0, 60000, 500):
+            piece, state = run(*(t[i:i + 500] for t in leaves[:5]), state)
+            outs.append(piece)
+    size = float(torch.linalg.matrix_norm(last).max().clamp(min=8.0))
+    near(torch.cat(outs), out.cpu(), torch.float32, 256 * U * size, "out")
+    near(state, last.cpu(), torch.float32, 256 * U * size, "last state")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_long_sequences_forget(hip_ops, dtype):
     """An infinite state is gone behind a start, whichever segment that is in, and a vanishing gate."""
     T = 1150
