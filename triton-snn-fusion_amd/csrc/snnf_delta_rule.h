@@ -461,6 +461,8 @@ template <int PIECES, int WAVES> struct StagedBlock {
             if (wave + i * WAVES < PIECES) *reinterpret_cast<u32x4a*>(lds + (wave + i * WAVES) * 256 + lane * 4) = words[i];
     }
 };
+// Threads of a walk's workgroup: with one term to an element four waves more, which load.
+template <typename T> __host__ __device__ __forceinline__ constexpr int walk_threads(int waves) { return 64 * (waves + (kTerms<T> == 1 ? 4 : 0)); }
 // What a walk reads of a chunk: keys, queries, values (or the gradient of what is read) and the chunk's block, without queries and scores if not ALL; through registers...
 template <typename T, int KS, int WAVES, int PIECES, bool ALL> struct StagedChunk {
     Staged<T, 4 * KS, 64 * WAVES> k, q;
@@ -479,13 +481,11 @@ template <typename T, int KS, int WAVES, int PIECES, bool ALL> struct StagedChun
         block.store(to);
     }
 };
-template <typename T> __host__ __device__ __forceinline__ constexpr bool loads_apart(int waves, bool all) { return kTerms<T> == 1 && (waves <= 4 || !all); }
-template <typename T> __host__ __device__ __forceinline__ constexpr int walk_threads(int waves, bool all = true) { return 64 * (waves + (loads_apart<T>(waves, all) ? 4 : 0)); }
 // ... or, with one term to an element, as they are, a chunk ahead into the other buffer: past the registers where rows are whole vectors, else through them at once. Loads past the registers wait for
-// room on their way, some 3000 of a walk's 13000 cycles a chunk: where four waves walk, four more do nothing but load.
+// room on their way, some 3000 of 13000 cycles a chunk where the waves that walk do it: four more do nothing but load.
 template <typename T, int KS, int WAVES, int PIECES, bool ALL = true> struct ChunkReader {
-    static constexpr bool kDirect = kTerms<T> == 1, kLoaders = loads_apart<T>(WAVES, ALL);
-    static constexpr int kBuffers = kDirect ? 2 : 1;
+    static constexpr bool kDirect = kTerms<T> == 1;
+    static constexpr int kLoaders = kDirect ? 4 : 0, kBuffers = kDirect ? 2 : 1;
     struct Buffers {
         uint16_t keys[Rows<T, KS>::kSize], queries[Rows<T, KS>::kSize];
         T tile[Tile<T, WAVES>::kSize];
@@ -504,7 +504,7 @@ template <typename T, int KS, int WAVES, int PIECES, bool ALL = true> struct Chu
         if constexpr (!kDirect) {
             next.load(p, c.keys, c.queries, c.values, c.step, c.rows, c.width, c.block);
         } else {
-            constexpr int W = kLoaders ? 4 : WAVES;       // that load
+            constexpr int W = kLoaders;
             const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % W;
             const uint32_t* zeros = c.block + block_vectors((PIECES - 1) / kBlocks - 3) + kZeros;
             if (p.near_keys) {
@@ -537,7 +537,6 @@ template <typename T, int KS, int WAVES, int PIECES, bool ALL = true> struct Chu
     // Has the chunk that was fetched last in LDS, for all waves; the one before it may be overwritten from then on.
     __device__ __forceinline__ void wait(Buffers& to) {
         if constexpr (kDirect) {
-            if constexpr (!kLoaders) arrived();
             __syncthreads();
         } else {
             __syncthreads();

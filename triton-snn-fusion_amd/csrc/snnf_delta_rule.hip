@@ -233,7 +233,7 @@ __global__ __launch_bounds__(256, kTerms<T> == 3 ? 2 : 4) void delta_chunk_kerne
 enum Walk { kOutputs, kTraining, kTransfer };
 
 template <typename T, int KS, int WAVES, Walk WALK>
-__global__ __launch_bounds__(kTerms<T> == 1 && walk_threads<T>(WAVES, WALK != kTransfer) <= 512 ? 512 : walk_threads<T>(WAVES, WALK != kTransfer)) void delta_walk_kernel(DeltaArgs p) {
+__global__ __launch_bounds__(kTerms<T> == 1 && walk_threads<T>(WAVES) <= 512 ? 512 : walk_threads<T>(WAVES)) void delta_walk_kernel(DeltaArgs p) {
     using Lds = Rows<T, KS>;
     using Values = Tile<T, WAVES>;
     constexpr int RANKS = kOutputRanks<T>, TERMS = kTerms<T>, PIPE = TERMS == 1 ? 2 : 1;
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 && walk_threads<T>(WAVES, WALK != kT
     const auto fetch = [&](int chunk) {
         if (chunk < live) reader.fetch(p, place(chunk), lds[chunk % Reader::kBuffers]);
     };
-    if constexpr (Reader::kLoaders)
+    if constexpr (Reader::kDirect)
         if (wave >= WAVES) {
             fetch(begin);
             for (int chunk = begin; chunk < live; ++chunk) {
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 && walk_threads<T>(WAVES, WALK != kT
                 if (there && head_element(d, r) < p.DK) slot[static_cast<int64_t>(head_element(d, r)) * p.DV] = state[d][r];
     }
     bool forgotten = false;
-    if constexpr (!Reader::kLoaders) fetch(begin);
+    if constexpr (!Reader::kDirect) fetch(begin);
     for (int chunk = begin; chunk < live; ++chunk) {
         const int64_t index = static_cast<int64_t>(head) * p.chunks + chunk;
         typename Reader::Buffers& here = lds[chunk % Reader::kBuffers];
@@ -304,7 +304,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 && walk_threads<T>(WAVES, WALK != kT
         T* tile = here.tile;
         const uint32_t *block = here.block, *vectors = block + block_vectors(RANKS);
         reader.wait(here);
-        if constexpr (!Reader::kLoaders) fetch(chunk + 1);
+        if constexpr (!Reader::kDirect) fetch(chunk + 1);
         now();
         // S k and S q, the state's terms a step ahead of the products that take them
         f32x4 ks[4], out[4], right[4], delta[4], since[4];
@@ -704,7 +704,7 @@ void launch_forward(const DeltaArgs& p, hipStream_t stream) {
     launch_chunks<T, KS, false>(p, stream);
     if (p.segments > 1) {
         constexpr int WAVES = sizeof(T) == 2 ? 8 : 4;
-        delta_walk_kernel<T, KS, WAVES, kTransfer><<<head_grid(p.N * p.HV * (p.segments - 1), transfer_parts(WAVES, KS, p.DV)), dim3(walk_threads<T>(WAVES, false)), 0, stream>>>(p);
+        delta_walk_kernel<T, KS, WAVES, kTransfer><<<head_grid(p.N * p.HV * (p.segments - 1), transfer_parts(WAVES, KS, p.DV)), dim3(walk_threads<T>(WAVES)), 0, stream>>>(p);
         launch_join<KS>(p, false, stream);
     }
     if constexpr (kTerms<T> == 1) {

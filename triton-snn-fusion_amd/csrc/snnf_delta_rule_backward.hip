@@ -49,7 +49,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
     const auto fetch = [&](int chunk) {
         if (chunk >= begin) reader.fetch(p, place(chunk), lds[chunk % Reader::kBuffers]);
     };
-    if constexpr (Reader::kLoaders)
+    if constexpr (Reader::kDirect)
         if (wave >= WAVES) {
             fetch(live - 1);
             for (int chunk = live - 1; chunk >= begin; --chunk) {
@@ -72,7 +72,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
             later[d][r] = behind != nullptr && there && row < p.DK ? behind[static_cast<int64_t>(row) * p.DV] : (matrix && row == column ? 1.0f : 0.0f);
         }
     bool forgotten = false;
-    if constexpr (!Reader::kLoaders) fetch(live - 1);
+    if constexpr (!Reader::kDirect) fetch(live - 1);
     for (int chunk = live - 1; chunk >= begin; --chunk) {
         const int64_t index = static_cast<int64_t>(head) * p.chunks + chunk;
         typename Reader::Buffers& here = lds[chunk % Reader::kBuffers];
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
         T* tile = here.tile;
         const uint32_t *block = here.block, *vectors = block + block_vectors(3);
         reader.wait(here);
-        if constexpr (!Reader::kLoaders) fetch(chunk - 1);
+        if constexpr (!Reader::kDirect) fetch(chunk - 1);
         now();
         // K R
         f32x4 pull[4], dout[4], z[4];
