@@ -123,12 +123,12 @@ def prepare(case, seed):
     logits.scatter_add_(2, peaks, 11.0 * uniform(n, k + 1, 4))
     draft = logits[:, :k] + 0.8 * normal(n, k, v)                                    # a smaller model's idea of them
     state.update(logits=logits.to(dtype), draft_logits=draft.to(dtype) if case["draft"] else None, temperature=1.0, lengths=None,
-                 uniforms=uniform(n, k), noise=(-torch.log(1.0 - uniform(n, v))).clamp(min=1e-12))
+                 uniforms=uniform(n, k), noise=-torch.log(1.0 - uniform(n, v)).clamp(min=1e-12))
     if case["temperature"] == "each":                                                # a quarter of the requests are answered greedily
         state["temperature"] = torch.where(uniform(n) < 0.25, 0.0, 0.5 + uniform(n))
     if case["lengths"]:
         state["lengths"] = torch.randint(0, k + 1, (n,), generator=g, device=DEVICE, dtype=torch.int32)
-    state["drafts"] = (draft - torch.log((-torch.log(uniform(n, k, v).clamp(min=1e-12))).clamp(min=1e-12))).argmax(2)       # drawn from it
+    state["drafts"] = (draft - torch.log(-torch.log(uniform(n, k, v).clamp(min=1e-12)).clamp(min=1e-12))).argmax(2)       # drawn from it
     if not case["draft"]:
         state["drafts"] = torch.where(uniform(n, k) < 0.7, logits[:, :k].argmax(2), state["drafts"])
     return state
