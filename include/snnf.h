@@ -577,7 +577,8 @@ int snnf_delta_rule_backward(const snnf_delta_rule_call* call, const void* marks
 /* Verification of drafted tokens against the target's logits [N, K + 1, V]: requests `*_row`, places `*_step` elements apart, a row's elements next to each other.
  *     p = softmax(logits / t), q = softmax(draft_logits / t) (draft_logits NULL: 1 at the draft); draft x stands while uniforms * q(x) < p(x)
  *     the token behind the accepted ones: the largest r / noise, r = p behind all drafts, else max(p - q, 0), or p where that leaves nothing
- *   temperatures  NULL (every request has `temperature`) or N; where it is not above 0: greedily, by the largest logit
+ *     (noise of any sign: an entry of r = 0 has 0; one of r > 0 over NaN is left out); a row of q of which nothing is left takes nothing from p, and its draft does not stand
+ *   temperatures  NULL (every request has `temperature`) or N; where it is not above 0: greedily, p is 1 at the largest logit (q at the draft) and 0 elsewhere
  *   drafts, uniforms [N, K], noise [N, V] with rows `noise_row` apart, lengths NULL or N (drafts of each request, clamped to 0..K)
  *   tokens [N, K + 1]: accepted drafts, the token, then -100 (as the token where nothing of the row can be drawn);  accepted [N]
  * K <= 64. Workspace: snnf_draft_verification_workspace_bytes(N, K, V, draft_logits != NULL) bytes, 16-byte aligned, in use until the call's work is done. Two launches. */

@@ -1,6 +1,7 @@
 // Verification of drafted tokens. With p = softmax(logits / temperature) of the target at a place and q that of the draft (1 at the drafted token where it has no
 // distribution), token x is accepted while u q(x) < p(x); the place behind the accepted ones gets argmax_i r_i / e_i over exponential noise e, which draws i with
-// probability r_i / sum r: r = p behind all drafts, max(p - q, 0) where one was turned down. So every token is distributed as p.
+// probability r_i / sum r: r = p behind all drafts, max(p - q, 0) where one was turned down. So every token is distributed as p. The argmax is taken as it is written, whatever the noise: an
+// entry of r = 0 has 0 and is the largest where no entry has noise above 0.
 // Two launches: (M, s) = (max x, sum exp((x - M) / temperature)) of every row, then the decisions and one more pass over the row that is drawn from. Bound by memory; few rows are
 // split over workgroups. 256 requests of 4 drafts x 128000 bfloat16 with both distributions take 168 us, of them 120 the first launch: 590 MB at 4.9 TB/s, next to what 295 million exponents
 // take of the vector units; one request of 4 x 32000 takes 12, the second launch's chain of statistics, drafted logits, verdicts, row and join.
@@ -27,7 +28,7 @@ struct VerifyArgs {
     int draw_splits, draw_span;         // and in the second
     float2* stats;                      // [request][row][split]: M, s
     uint64_t* largest;                  // [request][row][split]: key of the largest logit
-    uint64_t* parts;                    // [request][split]: the two largest upper bounds; the largest lower bound, index
+    uint64_t* parts;                    // [request][split]: the two largest upper bounds; the largest lower bound, index; the lowest index of those that are 0
     uint32_t* arrived;                  // [request]
     int64_t* tokens;
     int32_t* accepted;
@@ -204,20 +205,23 @@ struct Candidate {
     int index;
 };
 template <typename T, int BLOCK>
-__device__ int exact_draw(const T* x, const T* y, int taken, int V, float M, float M2, double temperature, const float* noise) {
+__device__ int exact_draw(const T* x, const T* y, int passed, int V, float M, float M2, double temperature, const float* noise) {
     const double s = exact_sum<T, BLOCK>(x, V, M, temperature), s2 = y != nullptr ? exact_sum<T, BLOCK>(y, V, M2, temperature) : 1.0;
     for (int round = 0; round < 2; ++round) {       // where nothing is left beside the draft's share: from p
         Candidate best{0.0, -1};
+        int some = 0;
         for (int i = threadIdx.x; i < V; i += BLOCK) {
             double r = exp((static_cast<double>(to_float(x[i])) - M) / temperature) / s;
-            if (round == 0) r -= y != nullptr ? exp((static_cast<double>(to_float(y[i])) - M2) / temperature) / s2 : (i == taken ? 1.0 : 0.0);
+            if (round == 0) r -= y != nullptr ? exp((static_cast<double>(to_float(y[i])) - M2) / temperature) / s2 : (i == passed ? 1.0 : 0.0);
             const double v = r > 0.0 ? r / static_cast<double>(noise[i]) : 0.0;
-            if (v > best.value) best = Candidate{v, i};
+            some |= r > 0.0;
+            if (best.index < 0 ? v == v : v > best.value) best = Candidate{v, i};
         }
+        if (!__syncthreads_or(some)) continue;
         best = over_block<BLOCK>(best, [](const Candidate& a, const Candidate& b) {
-            return b.value > a.value || (b.value == a.value && b.index >= 0 && (a.index < 0 || b.index < a.index)) ? b : a;
+            return b.index >= 0 && (a.index < 0 || b.value > a.value || (b.value == a.value && b.index < a.index)) ? b : a;
         });
-        if (best.index >= 0) return best.index;
+        return best.index >= 0 ? best.index : -100;
     }
     return -100;
 }
@@ -225,21 +229,40 @@ __device__ int exact_draw(const T* x, const T* y, int taken, int V, float M, flo
 // ------------------------------------------------------------------------------------------------------------------
 // Decisions and the draw
 // ------------------------------------------------------------------------------------------------------------------
-struct Race {                           // upper bounds of r / e: the two largest; the largest lower bound; index of the first, the lowest of equal ones
+// Of the values r / e that are not known to be 0: the two largest upper bounds; the largest lower bound; index of the first, the lowest of equal ones. The lowest index of those that are.
+constexpr int kNone = 0x7fffffff;
+struct Race {
     float first, second, lower;
-    int index;
+    int index, zero;
 };
+__device__ __forceinline__ Race nobody() { return {-INFINITY, -INFINITY, -INFINITY, kNone, kNone}; }
 __device__ __forceinline__ Race join(const Race& a, const Race& b) {
     const bool other = b.first > a.first || (b.first == a.first && b.index < a.index);
     const Race& w = other ? b : a;
-    return {w.first, fmaxf(w.second, other ? a.first : b.first), fmaxf(a.lower, b.lower), w.index};
+    return {w.first, fmaxf(w.second, other ? a.first : b.first), fmaxf(a.lower, b.lower), w.index, a.zero < b.zero ? a.zero : b.zero};
 }
 __device__ __forceinline__ Race lane_race(Race v) {
 #pragma unroll
     for (int mask = 32; mask > 0; mask >>= 1)
-        v = join(v, Race{__shfl_xor(v.first, mask, 64), __shfl_xor(v.second, mask, 64), __shfl_xor(v.lower, mask, 64), __shfl_xor(v.index, mask, 64)});
+        v = join(v, Race{__shfl_xor(v.first, mask, 64), __shfl_xor(v.second, mask, 64), __shfl_xor(v.lower, mask, 64), __shfl_xor(v.index, mask, 64), v.zero});
+    if (__ballot(v.zero != kNone) != 0) {
+#pragma unroll
+        for (int mask = 32; mask > 0; mask >>= 1) {
+            const int zero = __shfl_xor(v.zero, mask, 64);
+            v.zero = zero < v.zero ? zero : v.zero;
+        }
+    }
     return v;
 }
+// The index of the largest value, the lowest of equal ones; -1: the bounds do not tell. An upper bound of 0 beside noise below 0 is one of a value that may be 0.
+__device__ __forceinline__ int winner(const Race& v) {
+    const bool zeros = v.zero != kNone;
+    if (v.first > 0.0f) return v.second < v.lower && (v.lower > 0.0f || !zeros) ? v.index : -1;
+    if (zeros) return v.first < 0.0f || v.index > v.zero ? v.zero : -1;
+    return v.second < v.lower ? v.index : -1;
+}
+// Noise of a size for which bounds neither overflow nor vanish. Any other leaves the draw to float64.
+constexpr float kLeastNoise = 1e-24f, kMostNoise = 1e12f;
 
 __device__ __forceinline__ uint64_t two_words(float a, float b) { return static_cast<uint64_t>(__float_as_uint(b)) << 32 | __float_as_uint(a); }
 
@@ -330,22 +353,28 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
         if (verdict != kTaken) break;
     }
     int64_t token = -100;
+    const float* noise = p.noise + n * p.noise_row;
     if (greedy) {
         if (split != 0) return;
-        if (largest[taken] != 0) token = static_cast<int64_t>(~static_cast<uint32_t>(largest[taken]));
+        if (largest[taken] != 0) {      // r is 1 there and 0 elsewhere
+            token = static_cast<int64_t>(~static_cast<uint32_t>(largest[taken]));
+            const float e = noise[token];
+            if (fabsf(e) == INFINITY) token = 0;
+            else if (!(e > 0.0f || __float_as_uint(e) == 0u) && p.V > 1) token = token == 0;
+        }
     } else {
-        const T *x = row_of<T>(p, n, taken), *y = taken < length && p.draft_logits != nullptr ? row_of<T>(p, n, p.K + 1 + taken) : nullptr;
         const int64_t drafted = taken < length ? p.drafts[static_cast<int64_t>(n) * p.K + taken] : -1;
-        const float* noise = p.noise + n * p.noise_row;
-        const float2 a = stats[taken], b = y != nullptr ? stats[p.K + 1 + taken] : make_float2(0.0f, 1.0f);
+        const float2 a = stats[taken];
+        const T *x = row_of<T>(p, n, taken), *y = taken < length && p.draft_logits != nullptr ? row_of<T>(p, n, p.K + 1 + taken) : nullptr;
+        float2 b = y != nullptr ? stats[p.K + 1 + taken] : make_float2(0.0f, 1.0f);
         // A draft without a distribution that was turned down: p without it, since p is at most 1.
-        const int64_t passed = y == nullptr ? drafted : -1;
-        const float c = center(a.x), c2 = center(b.x), part = 1.0f / a.y, part2 = 1.0f / b.y;
+        const int passed = y == nullptr && drafted >= 0 && drafted < p.V ? static_cast<int>(drafted) : -1;
         const int begin = split * p.draw_span, end = begin + p.draw_span < p.V ? begin + p.draw_span : p.V;
-        Race mine{0.0f, 0.0f, 0.0f, 0x7fffffff};
+        Race mine = nobody();
         Raw<T, VEC> raw, raw2;
         Raw<float, 4> e[VEC / 4];
-        float bar = 0.0f;
+        float bar = -INFINITY;
+        bool odd = false;
         int at = begin + static_cast<int>(threadIdx.x) * VEC;
         const auto fetch = [&](int from) {
             raw.load(x, from, end - from);
@@ -354,37 +383,66 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
             for (int u = 0; u < VEC / 4; ++u) e[u].load(noise, from + 4 * u, end - from - 4 * u);
         };
         fetch(at);
+        if (!(b.y > 0.0f && b.y < INFINITY)) y = nullptr, b = make_float2(0.0f, 1.0f);        // nothing of it is left to take from p
+        const float c = center(a.x), c2 = center(b.x), part = 1.0f / a.y, part2 = 1.0f / b.y;
         for (int from = begin; from < end; from += BLOCK * VEC, at += BLOCK * VEC) {        // together: the wave shares what it has seen
             float v[VEC], v2[VEC], inverse[VEC], rough[VEC];
             const int left = end - at;
+            uint32_t least_bits = 0xffffffffu, most_bits = 0u;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                v[j] = j < left ? raw[j] : -INFINITY;
+                const float one = j < left ? e[j / 4][j % 4] : 1.0f;
+                v[j] = j < left && at + j != passed ? raw[j] : -INFINITY;
                 v2[j] = y != nullptr && j < left ? raw2[j] : -INFINITY;
-                inverse[j] = j < left ? __builtin_amdgcn_rcpf(e[j / 4][j % 4]) : 0.0f;
+                inverse[j] = __builtin_amdgcn_rcpf(one);
+                const uint32_t bits = __float_as_uint(one);
+                least_bits = least_bits < bits ? least_bits : bits, most_bits = most_bits > bits ? most_bits : bits;
             }
+            // As whole numbers the bits of positive floats are in order, and those of negative ones and NaN behind.
+            const bool usual = least_bits >= __float_as_uint(kLeastNoise) && most_bits <= __float_as_uint(kMostNoise);
             if (from + BLOCK * VEC < end) fetch(at + BLOCK * VEC);
-            // What the wave has seen beats most elements by far, by their shares without corrections, off by less than 2^-14.
-            constexpr float kRough = 6.2e-5f;
-            float least = 0.0f;
+            // What the wave has seen beats most elements by far, by their shares without corrections, off by less than 2^-14, and what vanishes in float32.
+            constexpr float kRough = 6.2e-5f, kVanishing = 1e-37f;
+            bool alive[VEC];            // may have more than 0
+            if (__ballot(!usual) == 0) {
+                float least = 0.0f;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float share = __builtin_amdgcn_exp2f((v[j] - c) * slope.high) * part, theirs = y != nullptr ? __builtin_amdgcn_exp2f((v2[j] - c2) * slope.high) * part2 : 0.0f;
-                const float middle = at + j == passed ? 0.0f : (share - theirs) * inverse[j], width = (share + theirs) * (inverse[j] * kRough);
-                least = fmaxf(least, middle - width);
-                rough[j] = middle + width;
+                for (int j = 0; j < VEC; ++j) {
+                    const float share = __builtin_amdgcn_exp2f((v[j] - c) * slope.high) * part, theirs = y != nullptr ? __builtin_amdgcn_exp2f((v2[j] - c2) * slope.high) * part2 : 0.0f;
+                    const float middle = (share - theirs) * inverse[j], width = fmaf(share + theirs, kRough, kVanishing) * inverse[j];
+                    least = fmaxf(least, middle - width);
+                    rough[j] = fmaxf(middle + width, 0.0f);
+                    alive[j] = rough[j] > 0.0f && v[j] > -INFINITY;
+                }
+                bar = fmaxf(bar, lane_max(least));
+            } else {
+                float least = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float share = __builtin_amdgcn_exp2f((v[j] - c) * slope.high) * part, theirs = y != nullptr ? __builtin_amdgcn_exp2f((v2[j] - c2) * slope.high) * part2 : 0.0f;
+                    const float width = fmaf(share + theirs, kRough, kVanishing), most = fmaxf((share - theirs) + width, 0.0f), few = fmaxf((share - theirs) - width, 0.0f);
+                    const bool negative = inverse[j] < 0.0f;
+                    rough[j] = (negative ? few : most) * inverse[j];
+                    if (j < left) least = fmaxf(least, (negative ? most : few) * inverse[j]);
+                    alive[j] = most > 0.0f && v[j] > -INFINITY;
+                    odd = odd || !(fabsf(inverse[j]) >= 0.999f / kMostNoise && fabsf(inverse[j]) <= 1.001f / kLeastNoise);
+                }
+                bar = fmaxf(bar, lane_max(least));
             }
-            bar = fmaxf(bar, lane_max(least));
+            const bool none = mine.zero == kNone;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                if (rough[j] >= bar && rough[j] > 0.0f && at + j != passed) {
+                // Of those that are 0 a lane's first one counts.
+                if (rough[j] >= bar && (alive[j] || none)) {
                     const float p1 = share_of(v[j], c, slope) * part, p2 = y != nullptr ? share_of(v2[j], c2, slope) * part2 : 0.0f;
-                    const float r = p1 - p2, unsure = fmaf(p1, doubt(v[j] - c, slope), p2 > 0.0f ? p2 * doubt(v2[j] - c2, slope) : 0.0f);
-                    const float upper = (r + unsure) * inverse[j];
-                    if (p1 > 0.0f && upper > 0.0f) mine = join(mine, Race{upper, 0.0f, (r - unsure) * inverse[j], at + j});
+                    const float r = p1 - p2, unsure = fmaf(p1, doubt(v[j] - c, slope), p2 > 0.0f ? p2 * doubt(v2[j] - c2, slope) : 0.0f) + 1e-30f;
+                    const float most = r + unsure, few = fmaxf(r - unsure, 0.0f);
+                    if (v[j] == -INFINITY || most <= 0.0f) mine.zero = j < left && at + j < mine.zero ? at + j : mine.zero;
+                    else mine = join(mine, Race{(inverse[j] < 0.0f ? few : most) * inverse[j], -INFINITY, (inverse[j] < 0.0f ? most : few) * inverse[j], at + j, kNone});
                 }
             }
         }
+        if (odd) mine.first = mine.second = INFINITY;
         mine = lane_race(mine);
         if (lane == 0) races[wave] = mine;
         __syncthreads();
@@ -392,26 +450,30 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
         if (p.draw_splits > 1) {
             // Parts are written and read past the dies' own caches and counted once they have arrived (a fence in place of that, which empties a die's cache, took 23 of 45 us a
             // workgroup at 256 x 128000).
-            uint64_t* parts = p.parts + static_cast<int64_t>(n) * p.draw_splits * 2;
+            uint64_t* parts = p.parts + static_cast<int64_t>(n) * p.draw_splits * 3;
             if (threadIdx.x == 0) {
-                __hip_atomic_store(parts + 2 * split, two_words(mine.first, mine.second), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                __hip_atomic_store(parts + 2 * split + 1, two_words(mine.lower, __int_as_float(mine.index)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(parts + 3 * split, two_words(mine.first, mine.second), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(parts + 3 * split + 1, two_words(mine.lower, __int_as_float(mine.index)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(parts + 3 * split + 2, static_cast<uint64_t>(mine.zero), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
                 last = __hip_atomic_fetch_add(p.arrived + n, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == static_cast<uint32_t>(p.draw_splits - 1);
             }
             __syncthreads();
             if (!last) return;
-            mine = Race{0.0f, 0.0f, 0.0f, 0x7fffffff};
+            mine = nobody();
             if (lane < p.draw_splits) {
-                const uint64_t one = __hip_atomic_load(parts + 2 * lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                const uint64_t two = __hip_atomic_load(parts + 2 * lane + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                const uint64_t one = __hip_atomic_load(parts + 3 * lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                const uint64_t two = __hip_atomic_load(parts + 3 * lane + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                const uint64_t three = __hip_atomic_load(parts + 3 * lane + 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 mine = Race{__uint_as_float(static_cast<uint32_t>(one)), __uint_as_float(static_cast<uint32_t>(one >> 32)), __uint_as_float(static_cast<uint32_t>(two)),
-                            static_cast<int>(two >> 32)};
+                            static_cast<int>(two >> 32), static_cast<int>(three)};
             }
             mine = lane_race(mine);
         }
-        if (mine.first > 0.0f && mine.second < mine.lower) token = mine.index;
-        else if (a.y > 0.0f && a.y < INFINITY) token = exact_draw<T, BLOCK>(x, y, static_cast<int>(y == nullptr && drafted >= 0 && drafted < p.V ? drafted : -1), p.V, a.x, b.x, temperature, noise);
+        if (a.y > 0.0f && a.y < INFINITY) {
+            token = winner(mine);
+            if (token < 0) token = exact_draw<T, BLOCK>(x, y, passed, p.V, a.x, b.x, temperature, noise);
+        }
     }
     if (static_cast<int>(threadIdx.x) <= p.K) {
         const int j = threadIdx.x;
@@ -467,7 +529,7 @@ extern "C" size_t snnf_draft_verification_workspace_bytes(int N, int K, int V, i
     const int rows = draft_logits ? 2 * K + 1 : K + 1;
     const VerifyShape s = verify_shape(N, rows, V);
     const size_t pieces = static_cast<size_t>(N) * rows * s.splits;
-    return rounded(pieces * 8) + rounded(pieces * 8) + static_cast<size_t>(N) * s.draw_splits * 16 + rounded(static_cast<size_t>(N) * 4);
+    return rounded(pieces * 8) + rounded(pieces * 8) + static_cast<size_t>(N) * s.draw_splits * 24 + rounded(static_cast<size_t>(N) * 4);
 }
 
 extern "C" int snnf_draft_verification(const void* logits, int64_t logits_row, int64_t logits_step, const void* draft_logits, int64_t draft_row, int64_t draft_step, int N,
@@ -496,7 +558,7 @@ extern "C" int snnf_draft_verification(const void* logits, int64_t logits_row, i
     p.stats = reinterpret_cast<float2*>(space);
     p.largest = reinterpret_cast<uint64_t*>(space += rounded(pieces * 8));
     p.parts = reinterpret_cast<uint64_t*>(space += rounded(pieces * 8));
-    p.arrived = reinterpret_cast<uint32_t*>(space + static_cast<size_t>(N) * s.draw_splits * 16);
+    p.arrived = reinterpret_cast<uint32_t*>(space + static_cast<size_t>(N) * s.draw_splits * 24);
     p.tokens = tokens, p.accepted = accepted;
     hipStream_t hs = as_stream(stream);
     if (dtype == SNNF_F32) launch_verification<float>(p, hs);

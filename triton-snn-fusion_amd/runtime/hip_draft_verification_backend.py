@@ -57,15 +57,17 @@ def run_hip_draft_verification(logits: torch.Tensor, drafts: torch.Tensor, unifo
     logits: [N, K + 1, V] float32, bfloat16 or float16, the target's at each draft and behind the last; rows may lie any distance apart. Minus infinity masks an entry.
     drafts: [N, K] int64 or int32; one outside [0, V) does not stand. K is at most 64 and may be 0 (a draw alone).
     uniforms: [N, K] float32 in [0, 1): draft x stands if uniform * q(x) < p(x), p = softmax(logits / temperature), q the draft's.
-    noise: [N, V] float32, positive, exponentially distributed (`torch.empty(N, V, device=...).exponential_()`): the token is the one of the largest
-        r / noise, the lowest index where they are equal; r = p behind drafts that all stand, else max(p - q, 0) (p, should nothing be left).
+    noise: [N, V] float32, exponentially distributed (`torch.empty(N, V, device=...).exponential_()`): the token is the one of the largest
+        r / noise, the lowest index where they are equal; r = p behind drafts that all stand, else max(p - q, 0) (p, should nothing be left). Taken as it is
+        written whatever the noise: an entry of r = 0 (a masked one, too) has 0 and is the largest where no entry of r > 0 has noise above 0; r > 0 over NaN is left out.
     draft_logits: [N, K, V] of logits' type, what drafts were drawn from, at the same temperature. None: drafts without a distribution, q(x) = 1.
     temperature: a number, or [N] float32. Where it is not above 0 the request is answered greedily: drafts stand while they are the largest logit (the
-        lowest index among equals), and so is the token behind them.
+        lowest index among equals), and p is 1 there and 0 elsewhere for the token behind them.
     lengths: [N] int32 or int64, clamped to 0..K, how many drafts each request has; what lies behind them is not read.
 
     Decisions are those of exact arithmetic on the given numbers: where float32 cannot tell two apart they are worked out in float64. A target's row of
-    which nothing is left (masked, or not finite) lets no draft stand, and its token is -100. What a recurrent state takes of such a step is `lengths=accepted + 1`.
+    which nothing is left (masked, or not finite) lets no draft stand, and its token is -100. A draft's row of which nothing is left stands for no
+    distribution: its draft does not stand, and r = p. What a recurrent state takes of such a step is `lengths=accepted + 1`.
     Nothing is differentiable.
     """
     module = native(logits)
