@@ -394,6 +394,7 @@ struct DeltaRule : torch::autograd::Function<DeltaRule> {
         const Tensor space = bytes ? empty({static_cast<int64_t>(bytes)}, at::kByte, q) : Tensor();
         const snnf_heads view = heads(out);
         check_status(snnf_delta_rule(&c, &view, last.data_ptr<float>(), marks ? marks->data_ptr<float>() : nullptr, data_of(space), bytes, stream_of(q)));
+        if (state_out.defined() && !state_out.is_inference()) state_out.unsafeGetTensorImpl()->bump_version();      // a graph that kept what it held before has to notice
         return {std::move(out), std::move(last)};
     }
     static variable_list forward(AutogradContext* ctx, Tensor q, Tensor k, Tensor v, Maybe gate, Maybe beta, Maybe state, Maybe starts, Maybe lengths, double scale) {

@@ -107,6 +107,8 @@ def _forward(query, key, value, gate, beta, state, scale, starts, lengths, state
         space = workspace(nbytes, query)
         _lib.check("snnf_delta_rule", lib.snnf_delta_rule(ctypes.byref(call), ctypes.byref(_heads(out)), last.data_ptr(), _lib.ptr(marks), _lib.ptr(space), nbytes,
                                                           _lib.current_stream(query.device)))
+    if state_out is not None and not state_out.is_inference():
+        torch.autograd.graph.increment_version(state_out)      # a graph that kept what it held before has to notice
     return out, last, marks
 
 
@@ -160,7 +162,8 @@ def run_hip_delta_rule(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
     starts: [T, N] bool. Where set, the state is dropped before the step (several documents packed into one sequence).
     lengths: [N] int32 or int64, clamped to 0..T. Steps from there on are padding: what the operands hold there does not matter, out is 0, the state stays. Drafted
         tokens that are not accepted are left out this way: lengths is their number and one.
-    state_out: memory for the returned state, contiguous, without gradients; may be state itself.
+    state_out: memory for the returned state, contiguous, without gradients; may be state itself. Written in place as by an operation of torch: a backward pass that
+        needs what it held before raises.
 
     Up to 16 steps without gradients are taken one by one, others in chunks of 64. Infinities and NaN of states and values stay in their columns, reach no
     step before them and none behind a start; those of keys, beta and gates, and of any operand in the gradients, may reach every step of their chunk.
