@@ -75,12 +75,16 @@ __device__ __forceinline__ float sum_of(const float (&v)[VEC]) {        // in pa
     else return (v[0] + v[1]) + (v[2] + v[3]);
 }
 
+// Temperatures whose slope and what it makes of logits float32 holds; those beyond are worked out in float64, with statistics of the nearest of these.
+constexpr float kColdest = 1e-30f, kHottest = 1e30f;
+__device__ __forceinline__ bool extreme(float temperature) { return temperature < kColdest || temperature > kHottest; }
+
 // 1 / temperature in powers of two, as the sum of two numbers.
 struct Slope {
     float high, low;
 };
 __device__ __forceinline__ Slope slope_of(float temperature) {
-    const double slope = 1.4426950408889634074 / temperature;
+    const double slope = 1.4426950408889634074 / fminf(fmaxf(temperature, kColdest), kHottest);
     const float high = static_cast<float>(slope);
     return {high, static_cast<float>(slope - high)};
 }
@@ -194,10 +198,13 @@ __device__ __forceinline__ V over_block(V v, Op op) {
     }
     return shared[0];
 }
+__device__ __forceinline__ double exact_share(float x, float M, double temperature) {      // a masked entry has none at an infinite temperature either
+    return x == -INFINITY ? 0.0 : exp((static_cast<double>(x) - M) / temperature);
+}
 template <typename T, int BLOCK>
 __device__ double exact_sum(const T* x, int V, float M, double temperature) {
     double s = 0.0;
-    for (int i = threadIdx.x; i < V; i += BLOCK) s += exp((static_cast<double>(to_float(x[i])) - M) / temperature);
+    for (int i = threadIdx.x; i < V; i += BLOCK) s += exact_share(to_float(x[i]), M, temperature);
     return over_block<BLOCK>(s, [](double a, double b) { return a + b; });
 }
 struct Candidate {
@@ -211,8 +218,8 @@ __device__ int exact_draw(const T* x, const T* y, int passed, int V, float M, fl
         Candidate best{0.0, -1};
         int some = 0;
         for (int i = threadIdx.x; i < V; i += BLOCK) {
-            double r = exp((static_cast<double>(to_float(x[i])) - M) / temperature) / s;
-            if (round == 0) r -= y != nullptr ? exp((static_cast<double>(to_float(y[i])) - M2) / temperature) / s2 : (i == passed ? 1.0 : 0.0);
+            double r = exact_share(to_float(x[i]), M, temperature) / s;
+            if (round == 0) r -= y != nullptr ? exact_share(to_float(y[i]), M2, temperature) / s2 : (i == passed ? 1.0 : 0.0);
             const double v = r > 0.0 ? r / static_cast<double>(noise[i]) : 0.0;
             some |= r > 0.0;
             if (best.index < 0 ? v == v : v > best.value) best = Candidate{v, i};
@@ -280,7 +287,7 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
     if (n >= p.N) return;
     const int length = drafts_of(p, n), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const float temperature = temperature_of(p, n);
-    const bool greedy = !(temperature > 0.0f);
+    const bool greedy = !(temperature > 0.0f), beyond = extreme(temperature);
     const Slope slope = slope_of(greedy ? 1.0f : temperature);
     // What the verdicts need of the drafts, sent for before the statistics.
     int64_t drafted_here = -1;
@@ -329,7 +336,7 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
                     unsure += doubt(theirs_logit - center(q.x), slope);
                 }
                 verdict = theirs < mine ? kTaken : kRefused;
-                if (fabsf(theirs - mine) <= unsure * (theirs + mine)) verdict = kDoubtful;
+                if (fabsf(theirs - mine) <= unsure * (theirs + mine) || (beyond && stats[j].y > 0.0f && stats[j].y < INFINITY)) verdict = kDoubtful;
             }
         }
         verdicts[j] = verdict;
@@ -342,11 +349,11 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
             const int64_t x = p.drafts[static_cast<int64_t>(n) * p.K + taken];
             const T *a = row_of<T>(p, n, taken), *b = p.draft_logits == nullptr ? nullptr : row_of<T>(p, n, p.K + 1 + taken);
             const float M = stats[taken].x;
-            const double mine = exp((static_cast<double>(to_float(a[x])) - M) / temperature) / exact_sum<T, BLOCK>(a, p.V, M, temperature);
+            const double mine = exact_share(to_float(a[x]), M, temperature) / exact_sum<T, BLOCK>(a, p.V, M, temperature);
             double theirs = p.uniforms[static_cast<int64_t>(n) * p.K + taken];
             if (b != nullptr) {
                 const float M2 = stats[p.K + 1 + taken].x;
-                theirs *= exp((static_cast<double>(to_float(b[x])) - M2) / temperature) / exact_sum<T, BLOCK>(b, p.V, M2, temperature);
+                theirs *= exact_share(to_float(b[x]), M2, temperature) / exact_sum<T, BLOCK>(b, p.V, M2, temperature);
             }
             verdict = theirs < mine ? kTaken : kRefused;
         }
@@ -374,7 +381,7 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
         Raw<T, VEC> raw, raw2;
         Raw<float, 4> e[VEC / 4];
         float bar = -INFINITY;
-        bool odd = false;
+        bool odd = beyond;
         int at = begin + static_cast<int>(threadIdx.x) * VEC;
         const auto fetch = [&](int from) {
             raw.load(x, from, end - from);

@@ -61,7 +61,7 @@ def run_hip_draft_verification(logits: torch.Tensor, drafts: torch.Tensor, unifo
         r / noise, the lowest index where they are equal; r = p behind drafts that all stand, else max(p - q, 0) (p, should nothing be left). Taken as it is
         written whatever the noise: an entry of r = 0 (a masked one, too) has 0 and is the largest where no entry of r > 0 has noise above 0; r > 0 over NaN is left out.
     draft_logits: [N, K, V] of logits' type, what drafts were drawn from, at the same temperature. None: drafts without a distribution, q(x) = 1.
-    temperature: a number, or [N] float32. Where it is not above 0 the request is answered greedily: drafts stand while they are the largest logit (the
+    temperature: a number, rounded to float32, or [N] float32; infinity makes what is not masked equal. Where it is not above 0 the request is answered greedily: drafts stand while they are the largest logit (the
         lowest index among equals), and p is 1 there and 0 elsewhere for the token behind them.
     lengths: [N] int32 or int64, clamped to 0..K, how many drafts each request has; what lies behind them is not read.
 
