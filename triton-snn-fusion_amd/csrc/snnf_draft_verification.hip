@@ -2,12 +2,12 @@
 // distribution), token x is accepted while u q(x) < p(x); the place behind the accepted ones gets argmax_i r_i / e_i over exponential noise e, which draws i with
 // probability r_i / sum r: r = p behind all drafts, max(p - q, 0) where one was turned down. So every token is distributed as p. The argmax is taken as it is written, whatever the noise: an
 // entry of r = 0 has 0 and is the largest where no entry has noise above 0.
-// Two launches: (M, s) = (max x, sum exp((x - M) / temperature)) of every row, then the decisions and one more pass over the row that is drawn from. Bound by memory; few rows are
-// split over workgroups. 256 requests of 4 drafts x 128000 bfloat16 with both distributions take 168 us, of them 120 the first launch: 590 MB at 4.9 TB/s, next to what 295 million exponents
-// take of the vector units; one request of 4 x 32000 takes 12, the second launch's chain of statistics, drafted logits, verdicts, row and join.
-// A decision is that of exact arithmetic: float32 gives each number with a bound of its error, 10^-6, and where two cannot be told apart the workgroup goes over the rows again in
-// float64. That takes several times as long as the rest, so that the bound matters: exponents are products in two parts, sums are compensated. (In the sums, plain exponents will do: the slope's rounding is the same
-// for all and makes 2^-25.5 of the exponent, of which a sum has at most log2 V on average.)
+// Two launches: (r, s) = an r near the largest x / temperature and sum exp(x / temperature - r) of every row, then the decisions and one more pass over the row that is drawn from. Bound by
+// memory; few rows are split over workgroups. 256 requests of 4 drafts x 128000 bfloat16 with both distributions take 168 us, of them 120 the first launch: 590 MB at 4.9 TB/s, next to what 295
+// million exponents take of the vector units; one request of 4 x 32000 takes 12, the second launch's chain of statistics, drafted logits, verdicts, row and join.
+// A decision is that of float64 on the given numbers: float32 gives each number with a bound of its error (`sum_doubt`, `share_doubt`), and where two cannot be told apart the workgroup goes
+// over the rows again in float64. That takes several times as long as the rest (765 us in place of 164 at 256 x 4 x 128000, two of 150 calls on random numbers), so that the bounds matter. Exponents are powers of two, x * slope - r in one rounding; r is a whole number, so that
+// sums for different r are brought together exactly; sums are compensated in a thread and float64 from there on.
 #include "snnf_sequence.h"
 
 namespace snnf {
@@ -26,7 +26,7 @@ struct VerifyArgs {
     int N, K, V, rows;                  // rows of a request: K + 1 of the target, then the draft's
     int splits, span;                   // of a row in the first launch
     int draw_splits, draw_span;         // and in the second
-    float2* stats;                      // [request][row][split]: M, s
+    float2* stats;                      // [request][row][split]: r, s
     uint64_t* largest;                  // [request][row][split]: key of the largest logit
     uint64_t* parts;                    // [request][split]: the two largest upper bounds; the largest lower bound, index; the lowest index of those that are 0
     uint32_t* arrived;                  // [request]
@@ -45,9 +45,6 @@ __device__ __forceinline__ const T* row_of(const VerifyArgs& p, int n, int row) 
     return row <= p.K ? static_cast<const T*>(p.logits) + n * p.logits_row + row * p.logits_step
                       : static_cast<const T*>(p.draft_logits) + n * p.draft_row + (row - p.K - 1) * p.draft_step;
 }
-
-// What is subtracted where nothing but minus infinity has been seen.
-__device__ __forceinline__ float center(float M) { return M == -INFINITY ? 0.0f : M; }
 
 // A key orders by value, equal ones by the lower index; 0: nothing that could be drawn (minus infinity and NaN).
 __device__ __forceinline__ uint64_t key_of(float x, int index) {
@@ -88,17 +85,42 @@ __device__ __forceinline__ Slope slope_of(float temperature) {
     const float high = static_cast<float>(slope);
     return {high, static_cast<float>(slope - high)};
 }
-// exp((x - M) / temperature): what the exponent's rounding loses is put back to first order. Off by some 2^-22, and by 2^-24 of the exponent where x - M is rounded.
-__device__ __forceinline__ float share_of(float x, float c, const Slope& slope) {
+// 2^(x slope - r), with c = r / slope.high: what leaving out slope.low would change of it but not of the others it is compared with is put back. Off by `share_doubt`.
+__device__ __forceinline__ float exponent_of(float x, float r, const Slope& slope) { return fmaf(x, slope.high, -r); }
+__device__ __forceinline__ float share_of(float x, float r, float c, const Slope& slope) {
     constexpr float kLn2 = 0.69314718055994530942f;
-    const float d = x - c, z = d * slope.high, e = __builtin_amdgcn_exp2f(z);
-    return e == 0.0f ? 0.0f : fmaf(e, fmaf(d, slope.low, fmaf(d, slope.high, -z)) * kLn2, e);
+    const float e = __builtin_amdgcn_exp2f(exponent_of(x, r, slope));
+    return e == 0.0f ? 0.0f : fmaf(e, (x - c) * slope.low * kLn2, e);
+}
+
+// Statistics of several parts brought together: s of each times a power of two. r is infinite where the largest x * slope is beyond kLargest in magnitude; s is 0 then where all is masked, above 0
+// where it is not, and in any case NaN where a number is NaN or infinite. Beyond kLargest c is too coarse, too; such rows are worked out in float64.
+constexpr float kLargest = 4194304.0f;
+template <typename F>
+__device__ __forceinline__ F brought(F s, float from, float to) {
+    return from == to ? s : static_cast<F>(ldexp(s, static_cast<int>(fmaxf(from - to, -1000.0f))));
+}
+__device__ __forceinline__ bool something(const float2& stats) { return stats.y > 0.0f && stats.y < INFINITY; }
+template <int MASK>
+__device__ __forceinline__ double across(double v) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    const uint32_t low = __float_as_uint(snnf::across<MASK>(__uint_as_float(static_cast<uint32_t>(bits)))), high = __float_as_uint(snnf::across<MASK>(__uint_as_float(static_cast<uint32_t>(bits >> 32))));
+    return __builtin_bit_cast(double, static_cast<uint64_t>(high) << 32 | low);
+}
+__device__ __forceinline__ double lane_sum(double v) {
+    v += across<1>(v);
+    v += across<2>(v);
+    v += across<4>(v);
+    v += across<8>(v);
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
 }
 
 template <typename T, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void verify_rows_kernel(VerifyArgs p) {
     constexpr int VEC = kVec<T>, WAVES = BLOCK / 64, BATCH = 2;
-    __shared__ float maxima[WAVES], sums[WAVES];
+    __shared__ float maxima[WAVES];
+    __shared__ double sums[WAVES];
     __shared__ uint64_t keys[WAVES];
     const uint32_t group = group_index();
     const int split = group % p.splits, place = group / p.splits, row = place % p.rows, n = place / p.rows;
@@ -141,9 +163,11 @@ __global__ __launch_bounds__(BLOCK) void verify_rows_kernel(VerifyArgs p) {
         return;
     }
     const Slope slope = slope_of(temperature);
-    float M = -INFINITY, s = 0.0f, lost = 0.0f;
+    // r: rises as soon as an element would have more than 2 and stays a whole number, so that s is multiplied by powers of two.
+    const int first = at;
+    float M = -INFINITY, r = -INFINITY, s = 0.0f, lost = 0.0f;
     for (; at < end; at += BATCH * BLOCK * VEC) {
-        float v[BATCH][VEC], most = M;
+        float v[BATCH][VEC];
 #pragma unroll
         for (int u = 0; u < BATCH; ++u) now[u] = next[u];
         if (at + BATCH * BLOCK * VEC < end) fetch(at + BATCH * BLOCK * VEC);
@@ -152,36 +176,60 @@ __global__ __launch_bounds__(BLOCK) void verify_rows_kernel(VerifyArgs p) {
 #pragma unroll
         for (int u = 0; u < BATCH; ++u)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) most = fmaxf(most, v[u][j]);
-        const float c = center(most);
-        const float f = share_of(M, c, slope);
-        s *= f, lost *= f;
-        M = most;
+            for (int j = 0; j < VEC; ++j) M = fmaxf(M, v[u][j]);
+        const float top = M * slope.high;
+        if (!(top - r <= 1.0f) && fabsf(top) < kLargest) {
+            const float higher = __builtin_rintf(top);
+            s = brought(s, r, higher), lost = brought(lost, r, higher);
+            r = higher;
+        }
+        const float subtracted = r == -INFINITY ? 0.0f : r;
 #pragma unroll
         for (int u = 0; u < BATCH; ++u) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[u][j] = __builtin_amdgcn_exp2f((v[u][j] - c) * slope.high);
+            for (int j = 0; j < VEC; ++j) v[u][j] = __builtin_amdgcn_exp2f(exponent_of(v[u][j], subtracted, slope));
             const float more = sum_of<VEC>(v[u]) - lost, now_s = s + more;
             lost = (now_s - s) - more;
             s = now_s;
         }
     }
-    const float most = lane_max(M);
+    if (M > -INFINITY && !(fabsf(M * slope.high) < kLargest)) {
+        bool broken = M == INFINITY;
+        for (at = first; at < end; at += BATCH * BLOCK * VEC) {
+            fetch(at);
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                float v[VEC];
+                take<T>(v, next[u], end - at - u * BLOCK * VEC);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) broken = broken || v[j] != v[j];
+            }
+        }
+        r = M > 0.0f ? INFINITY : -INFINITY, s = broken ? __builtin_nanf("") : 1.0f, lost = 0.0f;
+    }
+    const float most = lane_max(r);
     if (lane == 0) maxima[wave] = most;
     __syncthreads();
     const float all = lane_max(maxima[lane % WAVES], WAVES < 4 ? 4 : WAVES);
-    s = lane_sum(s * share_of(M, center(all), slope));
-    if (lane == 0) sums[wave] = s;
+    const double sum = lane_sum(brought(static_cast<double>(s) - static_cast<double>(lost), r, all));
+    if (lane == 0) sums[wave] = sum;
     __syncthreads();
     if (threadIdx.x == 0) {
-        s = sums[0];
-        for (int w = 1; w < WAVES; ++w) s += sums[w];
-        p.stats[static_cast<int64_t>(place) * p.splits + split] = make_float2(all, s);
+        double both = sums[0];
+        for (int w = 1; w < WAVES; ++w) both += sums[w];
+        p.stats[static_cast<int64_t>(place) * p.splits + split] = make_float2(all, static_cast<float>(both));
     }
 }
 
-// Relative error of a share over the sum: 4 x 10^-7 of the sum's exponents, some 8 roundings, and that of x - M (of float32 logits).
-__device__ __forceinline__ float doubt(float d, const Slope& slope) { return 1.2e-6f + 6e-8f * fminf(fabsf(d * slope.high), 1000.0f); }
+// Bounds of relative errors, in units u = 2^-24. A share: ln 2 for each power of two of the exponent, which is rounded once, 2 for the power itself (1.43 measured over all exponents from -125
+// to 126), 8 for the correction, three products, a quotient, a difference and the reciprocal of the noise. A sum: in the worst case all exponents are rounded the same way, as those of
+// equal logits are, and slope.low is missing from all: ln 2 (1 + |slope.low / slope.high| / u) for each power of two. Weighted by the shares those are the row's entropy at most, log2 V, and 2
+// for elements above r and r itself; then 2 for the powers, 3 for adding 8 of them, 3 for the compensated sum, 2 where it becomes float32.
+__device__ __forceinline__ float share_doubt(float exponent) { return (10.0f + 0.7f * fminf(fabsf(exponent), 1000.0f)) * 0x1p-24f; }
+__device__ __forceinline__ float sum_doubt(const Slope& slope, int V) {
+    const float bits = static_cast<float>(32 - __builtin_clz(V));
+    return (10.0f + 0.7f * (bits + 2.0f) * (1.0f + fabsf(slope.low / slope.high) * 0x1p24f)) * 0x1p-24f;
+}
 
 // ------------------------------------------------------------------------------------------------------------------
 // In float64, by a workgroup
@@ -202,6 +250,12 @@ __device__ __forceinline__ double exact_share(float x, float M, double temperatu
     return x == -INFINITY ? 0.0 : exp((static_cast<double>(x) - M) / temperature);
 }
 template <typename T, int BLOCK>
+__device__ float exact_top(const T* x, int V) {
+    float M = -INFINITY;
+    for (int i = threadIdx.x; i < V; i += BLOCK) M = fmaxf(M, to_float(x[i]));
+    return over_block<BLOCK>(M, [](float a, float b) { return fmaxf(a, b); });
+}
+template <typename T, int BLOCK>
 __device__ double exact_sum(const T* x, int V, float M, double temperature) {
     double s = 0.0;
     for (int i = threadIdx.x; i < V; i += BLOCK) s += exact_share(to_float(x[i]), M, temperature);
@@ -212,7 +266,8 @@ struct Candidate {
     int index;
 };
 template <typename T, int BLOCK>
-__device__ int exact_draw(const T* x, const T* y, int passed, int V, float M, float M2, double temperature, const float* noise) {
+__device__ int exact_draw(const T* x, const T* y, int passed, int V, double temperature, const float* noise) {
+    const float M = exact_top<T, BLOCK>(x, V), M2 = y != nullptr ? exact_top<T, BLOCK>(y, V) : 0.0f;
     const double s = exact_sum<T, BLOCK>(x, V, M, temperature), s2 = y != nullptr ? exact_sum<T, BLOCK>(y, V, M2, temperature) : 1.0;
     for (int round = 0; round < 2; ++round) {       // where nothing is left beside the draft's share: from p
         Candidate best{0.0, -1};
@@ -289,6 +344,7 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
     const float temperature = temperature_of(p, n);
     const bool greedy = !(temperature > 0.0f), beyond = extreme(temperature);
     const Slope slope = slope_of(greedy ? 1.0f : temperature);
+    const float per_sum = sum_doubt(slope, p.V);
     // What the verdicts need of the drafts, sent for before the statistics.
     int64_t drafted_here = -1;
     float logit = 0.0f, theirs_logit = 0.0f, uniform = 0.0f;
@@ -311,12 +367,13 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
             for (int i = 1; i < p.splits; ++i) best = larger(best, p.largest[at + i]);
             largest[row] = best;
         } else {
-            float M = -INFINITY, s = 0.0f;
+            float r = -INFINITY;
+            double s = 0.0;
 #pragma unroll 4
-            for (int i = 0; i < p.splits; ++i) M = fmaxf(M, p.stats[at + i].x);
+            for (int i = 0; i < p.splits; ++i) r = fmaxf(r, p.stats[at + i].x);
 #pragma unroll 4
-            for (int i = 0; i < p.splits; ++i) s += p.stats[at + i].y * share_of(p.stats[at + i].x, center(M), slope);
-            stats[row] = make_float2(M, s);
+            for (int i = 0; i < p.splits; ++i) s += brought(static_cast<double>(p.stats[at + i].y), p.stats[at + i].x, r);
+            stats[row] = make_float2(r, static_cast<float>(s));
         }
     }
     __syncthreads();
@@ -328,15 +385,17 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
             if (greedy) {
                 verdict = largest[j] != 0 && static_cast<int64_t>(~static_cast<uint32_t>(largest[j])) == drafted_here ? kTaken : kRefused;
             } else {
-                const float c = center(stats[j].x), mine = share_of(logit, c, slope) / stats[j].y;
-                float theirs = uniform, unsure = doubt(logit - c, slope);
+                const float2 a = stats[j], b = p.draft_logits != nullptr ? stats[p.K + 1 + j] : make_float2(0.0f, 1.0f);
+                const float mine = share_of(logit, a.x, a.x / slope.high, slope) / a.y;
+                float theirs = uniform, unsure = per_sum + share_doubt(exponent_of(logit, a.x, slope));
                 if (p.draft_logits != nullptr) {
-                    const float2 q = stats[p.K + 1 + j];
-                    theirs *= share_of(theirs_logit, center(q.x), slope) / q.y;
-                    unsure += doubt(theirs_logit - center(q.x), slope);
+                    theirs *= share_of(theirs_logit, b.x, b.x / slope.high, slope) / b.y;
+                    unsure += per_sum + share_doubt(exponent_of(theirs_logit, b.x, slope));
                 }
-                verdict = theirs < mine ? kTaken : kRefused;
-                if (fabsf(theirs - mine) <= unsure * (theirs + mine) || (beyond && stats[j].y > 0.0f && stats[j].y < INFINITY)) verdict = kDoubtful;
+                verdict = something(a) && something(b) && theirs < mine ? kTaken : kRefused;
+                // a bound, or numbers that vanish in float32
+                if (something(a) && something(b) && (beyond || fabsf(a.x) == INFINITY || fabsf(b.x) == INFINITY || !(fabsf(theirs - mine) > unsure * (theirs + mine)) || fmaxf(theirs, mine) < 1e-30f))
+                    verdict = uniform == uniform ? kDoubtful : kRefused;
             }
         }
         verdicts[j] = verdict;
@@ -348,11 +407,11 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
         if (verdict == kDoubtful) {
             const int64_t x = p.drafts[static_cast<int64_t>(n) * p.K + taken];
             const T *a = row_of<T>(p, n, taken), *b = p.draft_logits == nullptr ? nullptr : row_of<T>(p, n, p.K + 1 + taken);
-            const float M = stats[taken].x;
+            const float M = exact_top<T, BLOCK>(a, p.V);
             const double mine = exact_share(to_float(a[x]), M, temperature) / exact_sum<T, BLOCK>(a, p.V, M, temperature);
             double theirs = p.uniforms[static_cast<int64_t>(n) * p.K + taken];
             if (b != nullptr) {
-                const float M2 = stats[p.K + 1 + taken].x;
+                const float M2 = exact_top<T, BLOCK>(b, p.V);
                 theirs *= exact_share(to_float(b[x]), M2, temperature) / exact_sum<T, BLOCK>(b, p.V, M2, temperature);
             }
             verdict = theirs < mine ? kTaken : kRefused;
@@ -381,7 +440,6 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
         Raw<T, VEC> raw, raw2;
         Raw<float, 4> e[VEC / 4];
         float bar = -INFINITY;
-        bool odd = beyond;
         int at = begin + static_cast<int>(threadIdx.x) * VEC;
         const auto fetch = [&](int from) {
             raw.load(x, from, end - from);
@@ -390,8 +448,10 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
             for (int u = 0; u < VEC / 4; ++u) e[u].load(noise, from + 4 * u, end - from - 4 * u);
         };
         fetch(at);
-        if (!(b.y > 0.0f && b.y < INFINITY)) y = nullptr, b = make_float2(0.0f, 1.0f);        // nothing of it is left to take from p
-        const float c = center(a.x), c2 = center(b.x), part = 1.0f / a.y, part2 = 1.0f / b.y;
+        if (!something(b)) y = nullptr, b = make_float2(0.0f, 1.0f);        // nothing of it is left to take from p
+        const float c = a.x / slope.high, c2 = b.x / slope.high, part = 1.0f / a.y, part2 = 1.0f / b.y;
+        const float of_sums = y != nullptr ? per_sum : 0.0f;        // what all of p have in common changes no order
+        bool odd = beyond || fabsf(a.x) == INFINITY || fabsf(b.x) == INFINITY;
         for (int from = begin; from < end; from += BLOCK * VEC, at += BLOCK * VEC) {        // together: the wave shares what it has seen
             float v[VEC], v2[VEC], inverse[VEC], rough[VEC];
             const int left = end - at;
@@ -415,7 +475,7 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
                 float least = 0.0f;
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const float share = __builtin_amdgcn_exp2f((v[j] - c) * slope.high) * part, theirs = y != nullptr ? __builtin_amdgcn_exp2f((v2[j] - c2) * slope.high) * part2 : 0.0f;
+                    const float share = __builtin_amdgcn_exp2f(exponent_of(v[j], a.x, slope)) * part, theirs = y != nullptr ? __builtin_amdgcn_exp2f(exponent_of(v2[j], b.x, slope)) * part2 : 0.0f;
                     const float middle = (share - theirs) * inverse[j], width = fmaf(share + theirs, kRough, kVanishing) * inverse[j];
                     least = fmaxf(least, middle - width);
                     rough[j] = fmaxf(middle + width, 0.0f);
@@ -426,7 +486,7 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
                 float least = -INFINITY;
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const float share = __builtin_amdgcn_exp2f((v[j] - c) * slope.high) * part, theirs = y != nullptr ? __builtin_amdgcn_exp2f((v2[j] - c2) * slope.high) * part2 : 0.0f;
+                    const float share = __builtin_amdgcn_exp2f(exponent_of(v[j], a.x, slope)) * part, theirs = y != nullptr ? __builtin_amdgcn_exp2f(exponent_of(v2[j], b.x, slope)) * part2 : 0.0f;
                     const float width = fmaf(share + theirs, kRough, kVanishing), most = fmaxf((share - theirs) + width, 0.0f), few = fmaxf((share - theirs) - width, 0.0f);
                     const bool negative = inverse[j] < 0.0f;
                     rough[j] = (negative ? few : most) * inverse[j];
@@ -441,8 +501,8 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
             for (int j = 0; j < VEC; ++j) {
                 // Of those that are 0 a lane's first one counts.
                 if (rough[j] >= bar && (alive[j] || none)) {
-                    const float p1 = share_of(v[j], c, slope) * part, p2 = y != nullptr ? share_of(v2[j], c2, slope) * part2 : 0.0f;
-                    const float r = p1 - p2, unsure = fmaf(p1, doubt(v[j] - c, slope), p2 > 0.0f ? p2 * doubt(v2[j] - c2, slope) : 0.0f) + 1e-30f;
+                    const float p1 = share_of(v[j], a.x, c, slope) * part, p2 = y != nullptr ? share_of(v2[j], b.x, c2, slope) * part2 : 0.0f;
+                    const float r = p1 - p2, unsure = fmaf(p1, of_sums + share_doubt(exponent_of(v[j], a.x, slope)), p2 > 0.0f ? p2 * (of_sums + share_doubt(exponent_of(v2[j], b.x, slope))) : 0.0f) + 1e-30f;
                     const float most = r + unsure, few = fmaxf(r - unsure, 0.0f);
                     if (v[j] == -INFINITY || most <= 0.0f) mine.zero = j < left && at + j < mine.zero ? at + j : mine.zero;
                     else mine = join(mine, Race{(inverse[j] < 0.0f ? few : most) * inverse[j], -INFINITY, (inverse[j] < 0.0f ? most : few) * inverse[j], at + j, kNone});
@@ -477,9 +537,9 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
             }
             mine = lane_race(mine);
         }
-        if (a.y > 0.0f && a.y < INFINITY) {
+        if (something(a)) {
             token = winner(mine);
-            if (token < 0) token = exact_draw<T, BLOCK>(x, y, passed, p.V, a.x, b.x, temperature, noise);
+            if (token < 0) token = exact_draw<T, BLOCK>(x, y, passed, p.V, temperature, noise);
         }
     }
     if (static_cast<int>(threadIdx.x) <= p.K) {

@@ -65,7 +65,8 @@ def run_hip_draft_verification(logits: torch.Tensor, drafts: torch.Tensor, unifo
         lowest index among equals), and p is 1 there and 0 elsewhere for the token behind them.
     lengths: [N] int32 or int64, clamped to 0..K, how many drafts each request has; what lies behind them is not read.
 
-    Decisions are those of exact arithmetic on the given numbers: where float32 cannot tell two apart they are worked out in float64. A target's row of
+    Decisions are those of float64 on the given numbers: float32 comes with bounds of its error, and a request of which it cannot tell two numbers apart is
+    worked out again in float64, which adds 0.6 ms at 128000 logits (on random numbers, in one call of 256 requests in a hundred). A target's row of
     which nothing is left (masked, or not finite) lets no draft stand, and its token is -100. A draft's row of which nothing is left stands for no
     distribution: its draft does not stand, and r = p. What a recurrent state takes of such a step is `lengths=accepted + 1`.
     Nothing is differentiable.
