@@ -126,12 +126,11 @@ __host__ __device__ __forceinline__ constexpr int block_pieces(int ranks) { retu
 __host__ __device__ __forceinline__ constexpr int block_words(int ranks) { return block_pieces(ranks) * 256; }
 __host__ __device__ __forceinline__ constexpr int block_vectors(int ranks) { return kBlocks * (3 + ranks) * 256; }
 
-// Terms of what the output alone depends on: scores, and the state and corrections that they multiply. What the gradients of queries and keys are made of, too.
+// Terms of what the output alone depends on: scores, and the state and corrections that they multiply. A call whose gradients will be wanted has as many of what the gradients of queries, keys
+// and gates are products of (RANKS below): 2 where all of those are rounded to 16 bits, 3 where gates are float32, whose gradients float32 are, too. In the gradient of gates those of queries and keys cancel: with
+// one term of the states for bfloat16 it had been off by 1.5 to 2.8 times bfloat16's rounding (and 120 of 1590 us of a training pass of 4096 x 4 x 16 heads shorter), with two terms of everything
+// float32 gates' by 1 to 4 x 10^-5 of its size (with three by 0.5 to 1.4 x 10^-6; forward and backward of 4096 x 4 x 16 heads of 128 bfloat16 take 1512 in place of 1113 us then).
 template <typename T> inline constexpr int kOutputRanks = sizeof(T) == 4 ? 3 : 2;
-
-// Of the states that the gradients of queries and keys are products of. (One term for bfloat16 would have saved 120 of 1590 us of a training pass of 4096 x 4 x 16 heads and left the gradient of
-// gates, in which those of queries and keys cancel, off by 1.5 to 2.8 times its rounding.)
-template <typename T> inline constexpr int kMarkRanks = kOutputRanks<T>;
 
 // What the walks leave for the gradients, as the terms of which those are products. States [rank][value column][32 KS elements of a key], value columns up to what a walk's workgroups have; the 64 bytes
 // of 32 elements lie at a place that depends on the column, so that columns read side by side from LDS come from different banks.
@@ -445,14 +444,14 @@ template <typename T, int WAVES> struct Tile {
 };
 
 // A chunk's block on its way to LDS.
-template <int PIECES, int WAVES> struct StagedBlock {
+template <int PIECES, int WAVES, int LAST> struct StagedBlock {     // the first PIECES - 1 and piece LAST
     static constexpr int kCount = (PIECES + WAVES - 1) / WAVES;
     u32x4a words[kCount];
     __device__ __forceinline__ void load(const uint32_t* from) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
         for (int i = 0; i < kCount; ++i)
-            if (wave + i * WAVES < PIECES) words[i] = *reinterpret_cast<const u32x4a*>(from + (wave + i * WAVES) * 256 + lane * 4);
+            if (wave + i * WAVES < PIECES) words[i] = *reinterpret_cast<const u32x4a*>(from + (wave + i * WAVES < PIECES - 1 ? wave + i * WAVES : LAST) * 256 + lane * 4);
     }
     __device__ __forceinline__ void store(uint32_t* lds) const {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -464,10 +463,11 @@ template <int PIECES, int WAVES> struct StagedBlock {
 // Threads of a walk's workgroup: with one term to an element four waves more, which load.
 template <typename T> __host__ __device__ __forceinline__ constexpr int walk_threads(int waves) { return 64 * (waves + (kTerms<T> == 1 ? 4 : 0)); }
 // What a walk reads of a chunk: keys, queries, values (or the gradient of what is read) and the chunk's block, without queries and scores if not ALL; through registers...
+template <int PIECES, bool ALL> inline constexpr int kTaken = ALL ? PIECES : kBlocks * 3 + 1;      // of a block's pieces: without the scores if not ALL
 template <typename T, int KS, int WAVES, int PIECES, bool ALL> struct StagedChunk {
     Staged<T, 4 * KS, 64 * WAVES> k, q;
     Staged<T, 2 * WAVES, 64 * WAVES> v;
-    StagedBlock<PIECES, WAVES> block;
+    StagedBlock<kTaken<PIECES, ALL>, WAVES, PIECES - 1> block;
     __device__ __forceinline__ void load(const DeltaArgs& p, const T* keys, const T* queries, const T* values, int64_t step, int rows, int width, const uint32_t* from) {
         k.load(keys, p.k.step, rows, p.DK, p.near_keys);
         if constexpr (ALL) q.load(queries, p.q.step, rows, p.DK, p.near_keys);
@@ -489,7 +489,7 @@ template <typename T, int KS, int WAVES, int PIECES, bool ALL = true> struct Chu
     struct Buffers {
         uint16_t keys[Rows<T, KS>::kSize], queries[Rows<T, KS>::kSize];
         T tile[Tile<T, WAVES>::kSize];
-        uint32_t block[PIECES * 256];
+        uint32_t block[kTaken<PIECES, ALL> * 256];
     };
     struct Chunk {                      // its first row of keys, queries and values, and how many rows and values there are
         const T *keys, *queries, *values;
@@ -528,9 +528,9 @@ template <typename T, int KS, int WAVES, int PIECES, bool ALL = true> struct Chu
             }
             const uint32_t at = lds_address(to.block) + wave * 1024;
 #pragma unroll
-            for (int i = 0; i < (PIECES + W - 1) / W; ++i) {
+            for (int i = 0; i < (kTaken<PIECES, ALL> + W - 1) / W; ++i) {
                 const int piece = wave + i * W;
-                if (piece < PIECES && (ALL || piece < kBlocks * 3 || piece == PIECES - 1)) to_lds(c.block + piece * 256, lane * 16u, at + i * W * 1024);
+                if (piece < kTaken<PIECES, ALL>) to_lds(c.block + (piece < kTaken<PIECES, ALL> - 1 ? piece : PIECES - 1) * 256, lane * 16u, at + i * W * 1024);
             }
         }
     }
@@ -647,7 +647,7 @@ __device__ __forceinline__ bool part_of_head(int heads, int parts, int* head, in
 inline dim3 head_grid(int heads, int parts) { return grid_of(static_cast<int64_t>((heads + 7) / 8 * 8) * parts); }
 
 // Fragments, decays and inverses of all chunks; transposed for the backward pass.
-template <typename T, int KS, bool BACKWARD> void launch_chunks(const DeltaArgs& p, hipStream_t stream);
+template <typename T, int KS, int RANKS, bool BACKWARD> void launch_chunks(const DeltaArgs& p, hipStream_t stream);
 
 // Workgroups to a segment on its first walk, and what joins the states (backward: from the last segment on).
 inline int transfer_parts(int waves, int KS, int DV) { return (DV + 16 * waves - 1) / (16 * waves) + (2 * KS + waves - 1) / waves; }
@@ -659,7 +659,7 @@ void set_segments(DeltaArgs& p, const snnf_delta_rule_call* call, bool backward,
 int check_delta(const char* name, const snnf_delta_rule_call* call);
 DeltaArgs delta_args(const snnf_delta_rule_call* call);
 int64_t delta_chunks(const snnf_delta_rule_call* call);
-int delta_ranks(const snnf_delta_rule_call* call);
+int delta_ranks(const snnf_delta_rule_call* call, bool training);
 int64_t delta_mark_elements(const snnf_delta_rule_call* call);
 // Whether a chunk's rows lie within reach of 31-bit offsets, and, where they go to LDS as they are, on 16 bytes.
 inline bool near_by(const HeadView& x, int dtype, bool read) {

@@ -28,9 +28,9 @@ __device__ __forceinline__ f32x4 multiply_f32(const f32x4& a, const f32x4& b, f3
     return c;
 }
 
-template <typename T, int KS, bool BACKWARD>
+template <typename T, int KS, int RANKS, bool BACKWARD>
 __global__ __launch_bounds__(256, kTerms<T> == 3 ? 2 : 4) void delta_chunk_kernel(DeltaArgs p) {
-    constexpr int RANKS = BACKWARD ? 3 : kOutputRanks<T>, TERMS = kTerms<T>;
+    constexpr int TERMS = kTerms<T>;
     constexpr int kMatrix = kChunk * kPitch, kFragments = 4 * KS * TERMS * 256;
     __shared__ alignas(16) uint32_t shared[kFragments > 2 * kMatrix ? kFragments : 2 * kMatrix];     // keys, then the matrices
     // L below the diagonal, the scores transposed above it, four columns to the right: score [i][c] at [c][i + 4]
@@ -232,11 +232,11 @@ __global__ __launch_bounds__(256, kTerms<T> == 3 ? 2 : 4) void delta_chunk_kerne
 // A prompt of 8192 steps x 16 heads of 128 bfloat16, 8 segments: chunks 34, first walk 80, states 18, second walk 68 us; in one go chunks and walk took 634.
 enum Walk { kOutputs, kTraining, kTransfer };
 
-template <typename T, int KS, int WAVES, Walk WALK>
+template <typename T, int KS, int WAVES, int RANKS, Walk WALK>
 __global__ __launch_bounds__(kTerms<T> == 1 && walk_threads<T>(WAVES) <= 512 ? 512 : walk_threads<T>(WAVES)) void delta_walk_kernel(DeltaArgs p) {
     using Lds = Rows<T, KS>;
     using Values = Tile<T, WAVES>;
-    constexpr int RANKS = kOutputRanks<T>, TERMS = kTerms<T>, PIPE = TERMS == 1 ? 2 : 1;
+    constexpr int TERMS = kTerms<T>, PIPE = TERMS == 1 ? 2 : 1;
     constexpr bool TRAIN = WALK == kTraining, TRANSFER = WALK == kTransfer;
     using Reader = ChunkReader<T, KS, WAVES, block_pieces(RANKS), !TRANSFER>;
     __shared__ alignas(16) typename Reader::Buffers lds[Reader::kBuffers];
@@ -302,7 +302,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 && walk_threads<T>(WAVES) <= 512 ? 5
         typename Reader::Buffers& here = lds[chunk % Reader::kBuffers];
         const uint16_t *keys = here.keys, *queries = here.queries;
         T* tile = here.tile;
-        const uint32_t *block = here.block, *vectors = block + block_vectors(RANKS);
+        const uint32_t *block = here.block, *vectors = block + block_vectors(TRANSFER ? 0 : RANKS);
         reader.wait(here);
         if constexpr (!Reader::kDirect) fetch(chunk + 1);
         now();
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 && walk_threads<T>(WAVES) <= 512 ? 5
             now();
             if (PIPE == 2 && s + 1 < KS) load(s + 1);
             if constexpr (TRAIN)
-                if (s % 2 == 1) store_marks<KS, kMarkRanks<T>>(p.marks + index * (kMarkRanks<T> * padded_values(p.DV) * 32 * KS), p.DV, mine, s - 1, x[0].t, x[1].t);
+                if (s % 2 == 1) store_marks<KS, RANKS>(p.marks + index * (RANKS * padded_values(p.DV) * 32 * KS), p.DV, mine, s - 1, x[0].t, x[1].t);
             if (s + 1 < KS) x[(s + 1) % 2] = split<3>(state[2 * s + 2], state[2 * s + 3]);
             if (s + 1 == KS) {
 #pragma unroll
@@ -688,32 +688,34 @@ __global__ __launch_bounds__(64 * KS) void delta_step_kernel(DeltaArgs p) {
 // ------------------------------------------------------------------------------------------------------------------
 // Launch
 // ------------------------------------------------------------------------------------------------------------------
-template <typename T, int KS, int WAVES>
-void launch_walk(const DeltaArgs& p, hipStream_t stream) {
-    const dim3 grid(head_grid(p.N * p.HV * p.segments, (p.DV + 16 * WAVES - 1) / (16 * WAVES))), block(walk_threads<T>(WAVES));
-    if (p.marks != nullptr) delta_walk_kernel<T, KS, WAVES, kTraining><<<grid, block, 0, stream>>>(p);
-    else delta_walk_kernel<T, KS, WAVES, kOutputs><<<grid, block, 0, stream>>>(p);
+template <typename T, int KS, int WAVES, int RANKS, Walk WALK>
+void launch_walk(const DeltaArgs& p, int segments, int parts, hipStream_t stream) {
+    delta_walk_kernel<T, KS, WAVES, RANKS, WALK><<<head_grid(p.N * p.HV * segments, parts), dim3(walk_threads<T>(WAVES)), 0, stream>>>(p);
 }
 
-template <typename T, int KS>
-void launch_forward(const DeltaArgs& p, hipStream_t stream) {
-    if (p.blocks == nullptr) {
-        delta_step_kernel<T, KS><<<head_grid(p.N * p.HV, (p.DV + 63) / 64), dim3(64 * KS), 0, stream>>>(p);
-        return;
-    }
-    launch_chunks<T, KS, false>(p, stream);
+template <typename T, int KS, int RANKS, Walk WALK>
+void launch_walks(const DeltaArgs& p, hipStream_t stream) {
+    launch_chunks<T, KS, RANKS, false>(p, stream);
     if (p.segments > 1) {
         constexpr int WAVES = sizeof(T) == 2 ? 8 : 4;
-        delta_walk_kernel<T, KS, WAVES, kTransfer><<<head_grid(p.N * p.HV * (p.segments - 1), transfer_parts(WAVES, KS, p.DV)), dim3(walk_threads<T>(WAVES)), 0, stream>>>(p);
+        launch_walk<T, KS, WAVES, RANKS, kTransfer>(p, p.segments - 1, transfer_parts(WAVES, KS, p.DV), stream);
         launch_join<KS>(p, false, stream);
     }
     if constexpr (kTerms<T> == 1) {
         if (two_waves(p)) {
-            launch_walk<T, KS, 2>(p, stream);
+            launch_walk<T, KS, 2, RANKS, WALK>(p, p.segments, (p.DV + 31) / 32, stream);
             return;
         }
     }
-    launch_walk<T, KS, 4>(p, stream);
+    launch_walk<T, KS, 4, RANKS, WALK>(p, p.segments, (p.DV + 63) / 64, stream);
+}
+
+template <typename T, int KS>
+void launch_forward(const DeltaArgs& p, int ranks, hipStream_t stream) {
+    if (p.blocks == nullptr) delta_step_kernel<T, KS><<<head_grid(p.N * p.HV, (p.DV + 63) / 64), dim3(64 * KS), 0, stream>>>(p);
+    else if (p.marks == nullptr) launch_walks<T, KS, kOutputRanks<T>, kOutputs>(p, stream);
+    else if (ranks == 3) launch_walks<T, KS, 3, kTraining>(p, stream);
+    else if constexpr (kOutputRanks<T> == 2) launch_walks<T, KS, 2, kTraining>(p, stream);
 }
 
 }  // namespace
@@ -751,16 +753,16 @@ void set_segments(DeltaArgs& p, const snnf_delta_rule_call* c, bool backward, fl
     p.between = workspace + static_cast<int64_t>(p.N) * p.HV * (p.segments - 1) * transfer_floats(c->key_size <= 64 ? 2 : 4, p.DV);
 }
 
-template <typename T, int KS, bool BACKWARD>
+template <typename T, int KS, int RANKS, bool BACKWARD>
 void launch_chunks(const DeltaArgs& p, hipStream_t stream) {
-    delta_chunk_kernel<T, KS, BACKWARD><<<grid_of(static_cast<int64_t>(p.N) * p.HV * p.chunks), dim3(256), 0, stream>>>(p);
+    delta_chunk_kernel<T, KS, RANKS, BACKWARD><<<grid_of(static_cast<int64_t>(p.N) * p.HV * p.chunks), dim3(256), 0, stream>>>(p);
 }
-template void launch_chunks<float, 2, true>(const DeltaArgs&, hipStream_t);
-template void launch_chunks<float, 4, true>(const DeltaArgs&, hipStream_t);
-template void launch_chunks<bf16_t, 2, true>(const DeltaArgs&, hipStream_t);
-template void launch_chunks<bf16_t, 4, true>(const DeltaArgs&, hipStream_t);
-template void launch_chunks<f16_t, 2, true>(const DeltaArgs&, hipStream_t);
-template void launch_chunks<f16_t, 4, true>(const DeltaArgs&, hipStream_t);
+template void launch_chunks<float, 2, 3, true>(const DeltaArgs&, hipStream_t);
+template void launch_chunks<float, 4, 3, true>(const DeltaArgs&, hipStream_t);
+template void launch_chunks<bf16_t, 2, 3, true>(const DeltaArgs&, hipStream_t);
+template void launch_chunks<bf16_t, 4, 3, true>(const DeltaArgs&, hipStream_t);
+template void launch_chunks<f16_t, 2, 3, true>(const DeltaArgs&, hipStream_t);
+template void launch_chunks<f16_t, 4, 3, true>(const DeltaArgs&, hipStream_t);
 
 int check_delta(const char* name, const snnf_delta_rule_call* c) {
     if (c == nullptr) return fail(SNNF_ERR_INVALID_ARGUMENT, "%s: no call", name);
@@ -797,8 +799,8 @@ DeltaArgs delta_args(const snnf_delta_rule_call* c) {
     return p;
 }
 
-int delta_ranks(const snnf_delta_rule_call* c) { return c->dtype == SNNF_F32 ? kOutputRanks<float> : kOutputRanks<bf16_t>; }
-int64_t delta_mark_elements(const snnf_delta_rule_call* c) { return mark_elements(c->dtype == SNNF_F32 ? kMarkRanks<float> : (c->dtype == SNNF_F16 ? kMarkRanks<f16_t> : kMarkRanks<bf16_t>), c->key_size <= 64 ? 2 : 4, c->value_size); }
+int delta_ranks(const snnf_delta_rule_call* c, bool training) { return c->dtype == SNNF_F32 || (training && c->gate_dtype == SNNF_F32) ? 3 : 2; }
+int64_t delta_mark_elements(const snnf_delta_rule_call* c) { return mark_elements(delta_ranks(c, true), c->key_size <= 64 ? 2 : 4, c->value_size); }
 int64_t delta_chunks(const snnf_delta_rule_call* c) {
     return static_cast<int64_t>(c->N) * c->value_heads * ((c->T + kChunk - 1) / kChunk);
 }
@@ -809,12 +811,12 @@ using namespace snnf;
 
 extern "C" size_t snnf_delta_rule_workspace_bytes(const snnf_delta_rule_call* call, int training) {
     if (check_delta("snnf_delta_rule_workspace_bytes", call) != SNNF_OK || (!training && call->T <= kFewSteps)) return 0;
-    return static_cast<size_t>(delta_chunks(call)) * block_words(delta_ranks(call)) * 4 + delta_segment_floats(call, false) * 4;
+    return static_cast<size_t>(delta_chunks(call)) * block_words(delta_ranks(call, training != 0)) * 4 + delta_segment_floats(call, false) * 4;
 }
 
 extern "C" size_t snnf_delta_rule_marks_bytes(const snnf_delta_rule_call* call) {
     if (check_delta("snnf_delta_rule_marks_bytes", call) != SNNF_OK) return 0;
-    return static_cast<size_t>(delta_chunks(call)) * (delta_mark_elements(call) + delta_elements(delta_ranks(call), call->value_size)) * sizeof(uint16_t);
+    return static_cast<size_t>(delta_chunks(call)) * (delta_mark_elements(call) + delta_elements(delta_ranks(call, true), call->value_size)) * sizeof(uint16_t);
 }
 
 extern "C" int snnf_delta_rule(const snnf_delta_rule_call* call, const snnf_heads* out, float* state_out, void* marks, void* workspace, size_t workspace_bytes,
@@ -832,7 +834,7 @@ extern "C" int snnf_delta_rule(const snnf_delta_rule_call* call, const snnf_head
         if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
             return fail(SNNF_ERR_WORKSPACE, "snnf_delta_rule: workspace of %zu bytes needed, got %zu", need, workspace_bytes);
         p.blocks = static_cast<uint32_t*>(workspace);
-        set_segments(p, call, false, reinterpret_cast<float*>(p.blocks + delta_chunks(call) * block_words(delta_ranks(call))));
+        set_segments(p, call, false, reinterpret_cast<float*>(p.blocks + delta_chunks(call) * block_words(delta_ranks(call, marks != nullptr))));
     }
     if (marks != nullptr) {
         if (!aligned_to(marks, 16)) return fail(SNNF_ERR_INVALID_ARGUMENT, "snnf_delta_rule: marks must lie on 16 bytes");
@@ -842,8 +844,9 @@ extern "C" int snnf_delta_rule(const snnf_delta_rule_call* call, const snnf_head
     p.near_values = p.near_values && near_by(p.out, call->dtype, false);
     hipStream_t hs = as_stream(stream);
     const bool small = call->key_size <= 64;
-    if (call->dtype == SNNF_F32) small ? launch_forward<float, 2>(p, hs) : launch_forward<float, 4>(p, hs);
-    else if (call->dtype == SNNF_BF16) small ? launch_forward<bf16_t, 2>(p, hs) : launch_forward<bf16_t, 4>(p, hs);
-    else small ? launch_forward<f16_t, 2>(p, hs) : launch_forward<f16_t, 4>(p, hs);
+    const int ranks = delta_ranks(call, marks != nullptr);
+    if (call->dtype == SNNF_F32) small ? launch_forward<float, 2>(p, ranks, hs) : launch_forward<float, 4>(p, ranks, hs);
+    else if (call->dtype == SNNF_BF16) small ? launch_forward<bf16_t, 2>(p, ranks, hs) : launch_forward<bf16_t, 4>(p, ranks, hs);
+    else small ? launch_forward<f16_t, 2>(p, ranks, hs) : launch_forward<f16_t, 4>(p, ranks, hs);
     return check_launch("snnf_delta_rule");
 }

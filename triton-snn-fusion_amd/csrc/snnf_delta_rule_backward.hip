@@ -18,9 +18,9 @@ namespace {
 // As the walk forward, with R in accumulators: 4096 x 4 x 16 heads of 128 bfloat16 305 us, 4.8 a chunk.
 // In segments where heads are few, as the walk forward: a segment's effect on R is A^T R + B, and a first walk (TRANSFER) takes the identity and no gradient of its outputs for A^T, the
 // gradient of its outputs and no R for B.
-template <typename T, int KS, int WAVES, bool TRANSFER>
+template <typename T, int KS, int WAVES, int RANKS, bool TRANSFER>
 __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_kernel(DeltaArgs p) {
-    constexpr int RANKS = kOutputRanks<T>, TERMS = kTerms<T>, PIPE = TERMS == 1 ? 2 : 1;
+    constexpr int TERMS = kTerms<T>, PIPE = TERMS == 1 ? 2 : 1;
     using Lds = Rows<T, KS>;
     using Values = Tile<T, WAVES>;
     using Reader = ChunkReader<T, KS, WAVES, block_pieces(3)>;
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
             now();
             x[s % 2] = split<3>(later[2 * s], later[2 * s + 1]);
             if constexpr (!TRANSFER)
-                if (s % 2 == 1) store_marks<KS, kMarkRanks<T>>(p.later + index * (kMarkRanks<T> * padded_values(p.DV) * 32 * KS), p.DV, mine, s - 1, x[0].t, x[1].t);
+                if (s % 2 == 1) store_marks<KS, RANKS>(p.later + index * (RANKS * padded_values(p.DV) * 32 * KS), p.DV, mine, s - 1, x[0].t, x[1].t);
 #pragma unroll
             for (int rank = 2; rank >= 0; --rank)
 #pragma unroll
@@ -274,10 +274,10 @@ __device__ __forceinline__ void store_gate(const DeltaArgs& p, const HeadView& x
     else static_cast<T*>(const_cast<void*>(x.data))[at] = from_float<T>(v);
 }
 
-// Of tensors of 16 bits the logarithm is rounded to float32: a decay by 2^-10 is off by 2^-21 then.
-template <typename T>
+// Where all gradients are rounded to 16 bits the logarithm is rounded to float32: a decay by 2^-10 is off by 2^-21 then.
+template <bool FINE>
 __device__ __forceinline__ float decay_apart(const Sum& one, const Sum& other, bool ahead) {
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (FINE) {
         return ahead ? decay_between(other, one) : decay_between(one, other);
     } else {
         const float x = (one.large - other.large) + (one.small - other.small);
@@ -286,13 +286,13 @@ __device__ __forceinline__ float decay_apart(const Sum& one, const Sum& other, b
 }
 
 // Two waves to 16 steps: the first works out dL, the second dP, and each has half of the head's elements of everything else; they exchange dL and dP through LDS. A workgroup takes one chunk after the
-// other, each in pieces of 32 value columns and then a last one of keys and queries; with bfloat16 four more waves load the next piece while one is worked on.
+// other, each in pieces of 32 value columns and then a last one of keys and queries; with bfloat16, two terms to what the walks left, four more waves load the next piece while one is worked on.
 // Bound by memory and by the phases between barriers: 4096 chunks of 128 bfloat16 elements read and write 1.2 GB in 370 us (3.2 TB/s; without waves of their own for the loads 435).
-template <typename T, int KS> struct GradientPieces {
-    static constexpr int RANKS = kOutputRanks<T>, TERMS = kTerms<T>, MARKS = kMarkRanks<T>, BUFFERS = TERMS == 1 ? 2 : 1;     // by the room in LDS
+template <typename T, int KS, int RANKS> struct GradientPieces {
+    static constexpr int TERMS = kTerms<T>, BUFFERS = TERMS == 1 && RANKS == 2 ? 2 : 1;     // by the room in LDS
     static constexpr int THREADS = BUFFERS == 2 ? 768 : 512;
     struct Slice {                      // 32 value columns of everything
-        uint16_t marks[MARKS][1024 * KS], later[MARKS][1024 * KS], deltas[RANKS][kChunk * 32], pulls[RANKS][kChunk * 32], douts[TERMS][kChunk * 32];
+        uint16_t marks[RANKS][1024 * KS], later[RANKS][1024 * KS], deltas[RANKS][kChunk * 32], pulls[RANKS][kChunk * 32], douts[TERMS][kChunk * 32];
     };
     struct Heads {
         uint16_t keys[Rows<T, KS>::kSize], queries[Rows<T, KS>::kSize];
@@ -305,11 +305,11 @@ template <typename T, int KS> struct GradientPieces {
 };
 
 // SHARED: whether value heads share queries and keys, whose gradients are their sums then, held over the chunks of a head's members.
-template <typename T, int KS, bool SHARED>
-__global__ __launch_bounds__((GradientPieces<T, KS>::THREADS)) void delta_gradient_kernel(DeltaArgs p) {
+template <typename T, int KS, int RANKS, bool SHARED>
+__global__ __launch_bounds__((GradientPieces<T, KS, RANKS>::THREADS)) void delta_gradient_kernel(DeltaArgs p) {
     using Lds = Rows<T, KS>;
-    using Pieces = GradientPieces<T, KS>;
-    constexpr int RANKS = Pieces::RANKS, TERMS = Pieces::TERMS, MARKS = Pieces::MARKS, BUFFERS = Pieces::BUFFERS;
+    using Pieces = GradientPieces<T, KS, RANKS>;
+    constexpr int TERMS = Pieces::TERMS, BUFFERS = Pieces::BUFFERS;
     constexpr bool LOADERS = BUFFERS == 2;
     __shared__ alignas(16) typename Pieces::Piece lds[BUFFERS];
     __shared__ alignas(16) Sum total[kChunk];
@@ -351,9 +351,9 @@ __global__ __launch_bounds__((GradientPieces<T, KS>::THREADS)) void delta_gradie
         constexpr int WAVES = LOADERS ? 4 : 8;
         const int from_wave = wave % WAVES;
         const int64_t index = index_of(x);
-        const uint16_t *marks = p.marks + index * (MARKS * columns * 32 * KS), *later = p.later + index * (MARKS * columns * 32 * KS);
+        const uint16_t *marks = p.marks + index * (RANKS * columns * 32 * KS), *later = p.later + index * (RANKS * columns * 32 * KS);
 #pragma unroll
-        for (int r = 0; r < MARKS; ++r)
+        for (int r = 0; r < RANKS; ++r)
 #pragma unroll
             for (int i = 0; i < (2 * KS + WAVES - 1) / WAVES; ++i)
                 if (from_wave + WAVES * i < 2 * KS) {
@@ -405,8 +405,8 @@ __global__ __launch_bounds__((GradientPieces<T, KS>::THREADS)) void delta_gradie
         if constexpr (TERMS == 1) {
             if (p.near_keys) {
                 const uint32_t* zeros = p.blocks + index_of(x) * block_words(3) + block_vectors(3) + kZeros;
-                rows_to_lds<4 * KS, THREADS / 64>(w, reinterpret_cast<const uint16_t*>(keys), p.k.step, x.rows, p.DK, zeros, to.keys);
-                rows_to_lds<4 * KS, THREADS / 64>(w, reinterpret_cast<const uint16_t*>(queries), p.q.step, x.rows, p.DK, zeros, to.queries);
+                rows_to_lds<4 * KS, THREADS / 64>(LOADERS ? w : wave, reinterpret_cast<const uint16_t*>(keys), p.k.step, x.rows, p.DK, zeros, to.keys);
+                rows_to_lds<4 * KS, THREADS / 64>(LOADERS ? w : wave, reinterpret_cast<const uint16_t*>(queries), p.q.step, x.rows, p.DK, zeros, to.queries);
                 return;
             }
         }
@@ -518,7 +518,7 @@ __global__ __launch_bounds__((GradientPieces<T, KS>::THREADS)) void delta_gradie
             }
 #pragma unroll
             for (int d = 0; d < KS; ++d) {
-                const Terms<MARKS> x = state_columns<MARKS, KS>(here.marks[0], team * KS + d), y = state_columns<MARKS, KS>(here.later[0], team * KS + d);
+                const Terms<RANKS> x = state_columns<RANKS, KS>(here.marks[0], team * KS + d), y = state_columns<RANKS, KS>(here.later[0], team * KS + d);
                 if (d == w) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) dot = fmaf(term_sum(x, j), term_sum(y, j), dot);
@@ -557,7 +557,7 @@ __global__ __launch_bounds__((GradientPieces<T, KS>::THREADS)) void delta_gradie
             for (int r = 0; r < 4; ++r) {
                 const int x = at + r;
                 const Sum other = {sums[r / 2][r % 2 * 2], sums[r / 2][r % 2 * 2 + 1]};
-                const float d = parts[r] == mine_part ? decay_apart<T>(mine_total, other, x <= own) : 0.0f;
+                const float d = parts[r] == mine_part ? decay_apart<RANKS == 3>(mine_total, other, x <= own) : 0.0f;
                 if (team == 0) {
                     by_row[j][r] = x == own ? 0.0f : kept(-d * beta * others[r], x < own ? by_row[j][r] : by_column[j][r]);
                 } else {
@@ -679,23 +679,29 @@ __global__ __launch_bounds__((GradientPieces<T, KS>::THREADS)) void delta_gradie
     }
 }
 
-template <typename T, int KS>
+template <typename T, int KS, int RANKS>
 void launch_backward(const DeltaArgs& p, hipStream_t stream) {
-    launch_chunks<T, KS, true>(p, stream);
+    launch_chunks<T, KS, 3, true>(p, stream);
     if (p.segments > 1) {
-        delta_walk_back_kernel<T, KS, 4, true><<<head_grid(p.N * p.HV * (p.segments - 1), transfer_parts(4, KS, p.DV)), dim3(walk_threads<T>(4)), 0, stream>>>(p);
+        delta_walk_back_kernel<T, KS, 4, 3, true><<<head_grid(p.N * p.HV * (p.segments - 1), transfer_parts(4, KS, p.DV)), dim3(walk_threads<T>(4)), 0, stream>>>(p);
         launch_join<KS>(p, true, stream);
     }
     bool narrow = false;
     if constexpr (kTerms<T> == 1) {
         narrow = two_waves(p);
-        if (narrow) delta_walk_back_kernel<T, KS, 2, false><<<head_grid(p.N * p.HV * p.segments, (p.DV + 31) / 32), dim3(walk_threads<T>(2)), 0, stream>>>(p);
+        if (narrow) delta_walk_back_kernel<T, KS, 2, RANKS, false><<<head_grid(p.N * p.HV * p.segments, (p.DV + 31) / 32), dim3(walk_threads<T>(2)), 0, stream>>>(p);
     }
-    if (!narrow) delta_walk_back_kernel<T, KS, 4, false><<<head_grid(p.N * p.HV * p.segments, (p.DV + 63) / 64), dim3(walk_threads<T>(4)), 0, stream>>>(p);
+    if (!narrow) delta_walk_back_kernel<T, KS, 4, RANKS, false><<<head_grid(p.N * p.HV * p.segments, (p.DV + 63) / 64), dim3(walk_threads<T>(4)), 0, stream>>>(p);
     const int64_t places = static_cast<int64_t>(p.N) * p.H * p.chunks, units = compute_units();
-    const dim3 grid(static_cast<unsigned>(places < units ? places : units)), block(GradientPieces<T, KS>::THREADS);
-    if (p.HV > p.H) delta_gradient_kernel<T, KS, true><<<grid, block, 0, stream>>>(p);
-    else delta_gradient_kernel<T, KS, false><<<grid, block, 0, stream>>>(p);
+    const dim3 grid(static_cast<unsigned>(places < units ? places : units)), block(GradientPieces<T, KS, RANKS>::THREADS);
+    if (p.HV > p.H) delta_gradient_kernel<T, KS, RANKS, true><<<grid, block, 0, stream>>>(p);
+    else delta_gradient_kernel<T, KS, RANKS, false><<<grid, block, 0, stream>>>(p);
+}
+template <typename T>
+void launch_backward(const DeltaArgs& p, int ranks, hipStream_t stream) {
+    const bool small = p.DK <= 64;
+    if (ranks == 3) small ? launch_backward<T, 2, 3>(p, stream) : launch_backward<T, 4, 3>(p, stream);
+    else if constexpr (kOutputRanks<T> == 2) small ? launch_backward<T, 2, 2>(p, stream) : launch_backward<T, 4, 2>(p, stream);
 }
 
 }  // namespace
@@ -706,7 +712,7 @@ using namespace snnf;
 extern "C" size_t snnf_delta_rule_backward_workspace_bytes(const snnf_delta_rule_call* call) {
     if (check_delta("snnf_delta_rule_backward_workspace_bytes", call) != SNNF_OK) return 0;
     return static_cast<size_t>(delta_chunks(call)) *
-           (block_words(3) * 4 + (delta_mark_elements(call) + delta_elements(delta_ranks(call), call->value_size)) * sizeof(uint16_t)) +
+           (block_words(3) * 4 + (delta_mark_elements(call) + delta_elements(delta_ranks(call, true), call->value_size)) * sizeof(uint16_t)) +
            delta_segment_floats(call, true) * 4;
 }
 
@@ -735,11 +741,11 @@ extern "C" int snnf_delta_rule_backward(const snnf_delta_rule_call* call, const 
     p.blocks = static_cast<uint32_t*>(workspace);
     p.later = reinterpret_cast<uint16_t*>(p.blocks + chunks * block_words(3));
     p.pulls = p.later + chunks * delta_mark_elements(call);
-    set_segments(p, call, true, reinterpret_cast<float*>(p.pulls + chunks * delta_elements(delta_ranks(call), call->value_size)));
+    set_segments(p, call, true, reinterpret_cast<float*>(p.pulls + chunks * delta_elements(delta_ranks(call, true), call->value_size)));
     hipStream_t hs = as_stream(stream);
-    const bool small = call->key_size <= 64;
-    if (call->dtype == SNNF_F32) small ? launch_backward<float, 2>(p, hs) : launch_backward<float, 4>(p, hs);
-    else if (call->dtype == SNNF_BF16) small ? launch_backward<bf16_t, 2>(p, hs) : launch_backward<bf16_t, 4>(p, hs);
-    else small ? launch_backward<f16_t, 2>(p, hs) : launch_backward<f16_t, 4>(p, hs);
+    const int ranks = delta_ranks(call, true);
+    if (call->dtype == SNNF_F32) launch_backward<float>(p, ranks, hs);
+    else if (call->dtype == SNNF_BF16) launch_backward<bf16_t>(p, ranks, hs);
+    else launch_backward<f16_t>(p, ranks, hs);
     return check_launch("snnf_delta_rule_backward");
 }

@@ -156,7 +156,8 @@ def run_hip_delta_rule(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
         multiple of H, and value head j works with key and query head j // (Hv // H). Dk is at most 128, Dv at most 1024.
     gate: [T, N, Hv], the logarithm of the decay (None: no decay), at most 0 in earnest. Below -104, where less than 2^-149 would be left, the state is dropped as by a start.
     beta: [T, N, Hv], how much of a step's correction is taken (None: 1). With keys of length 1 at most, states stay bounded for beta up to 2.
-        gate and beta are both of query's type or both float32.
+        gate and beta are both of query's type or both float32. Gradients of float32 ones are float32's own beside 16-bit queries, too: products of the
+        training passes then have three bfloat16 terms in place of two (4096 steps x 4 x 16 heads of 128: 1.51 ms in place of 1.11, 605 MB kept in place of 403).
     state: [N, Hv, Dk, Dv] float32 before the first step (None: zeros). The returned state is float32 and, unless state_out is given, new memory.
     scale: of the outputs, 1 / sqrt(Dk) if None.
     starts: [T, N] bool. Where set, the state is dropped before the step (several documents packed into one sequence).
