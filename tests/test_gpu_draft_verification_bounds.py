@@ -105,3 +105,20 @@ def test_logits_of_any_size(hip_ops, dtype):
     r[:, 4] = 0.0
     assert got.accepted[:8].tolist() == [0] * 8 and torch.equal(got.tokens[:6, 0].cpu(), (r / noise.double())[:6].argmax(1))
     assert got.tokens[6:].tolist() == [[-100] * 2] * 2 + [[4, -100]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("temperature", [1.0, 2.0 ** -10])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_logits_around_the_largest_that_float32_takes(hip_ops, sign, temperature):
+    """2^22 powers of two, where rows are left to float64: numbers on both sides of it weigh as they are."""
+    V, N = 6000, 40
+    g = gen(8)
+    logits = (sign * 2.0 ** 22 * math.log(2.0) + torch.cat([torch.linspace(-10.0, 10.0, N - 8), torch.linspace(-1200.0, 1200.0, 8)])[:, None, None] + torch.randn(N, 2, V, generator=g) * 2).mul(temperature).float()
+    drafts, uniforms, noise = torch.randint(0, V, (N, 1), generator=g), torch.rand(N, 1, generator=g) * 2e-4, torch.empty(N, V).exponential_(generator=g)
+    p = torch.softmax(logits.double() / temperature, -1)
+    want = (uniforms.double() < p[:, 0].gather(1, drafts))[:, 0]
+    r = torch.where(want[:, None], p[:, 1], p[:, 0].scatter(1, drafts, 0.0))
+    got = run(logits.to(DEV), drafts.to(DEV), uniforms.to(DEV), noise.to(DEV), temperature=temperature)
+    assert 5 < int(want.sum()) < 35 and torch.equal(got.accepted.cpu().bool(), want)
+    assert torch.equal(got.tokens.cpu().gather(1, want.long()[:, None])[:, 0], (r / noise.double()).argmax(1))

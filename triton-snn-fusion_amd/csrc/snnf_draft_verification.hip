@@ -96,6 +96,7 @@ __device__ __forceinline__ float share_of(float x, float r, float c, const Slope
 // Statistics of several parts brought together: s of each times a power of two. r is infinite where the largest x * slope is beyond kLargest in magnitude; s is 0 then where all is masked, above 0
 // where it is not, and in any case NaN where a number is NaN or infinite. Beyond kLargest c is too coarse, too; such rows are worked out in float64.
 constexpr float kLargest = 4194304.0f;
+__device__ __forceinline__ bool coarse(float r) { return !(fabsf(r) <= kLargest - 1024.0f); }      // or so near that parts of the row may be beyond and count
 template <typename F>
 __device__ __forceinline__ F brought(F s, float from, float to) {
     return from == to ? s : static_cast<F>(ldexp(s, static_cast<int>(fmaxf(from - to, -1000.0f))));
@@ -394,7 +395,7 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
                 }
                 verdict = something(a) && something(b) && theirs < mine ? kTaken : kRefused;
                 // a bound, or numbers that vanish in float32
-                if (something(a) && something(b) && (beyond || fabsf(a.x) == INFINITY || fabsf(b.x) == INFINITY || !(fabsf(theirs - mine) > unsure * (theirs + mine)) || fmaxf(theirs, mine) < 1e-30f))
+                if (something(a) && something(b) && (beyond || coarse(a.x) || coarse(b.x) || !(fabsf(theirs - mine) > unsure * (theirs + mine)) || fmaxf(theirs, mine) < 1e-30f))
                     verdict = uniform == uniform ? kDoubtful : kRefused;
             }
         }
@@ -451,7 +452,7 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
         if (!something(b)) y = nullptr, b = make_float2(0.0f, 1.0f);        // nothing of it is left to take from p
         const float c = a.x / slope.high, c2 = b.x / slope.high, part = 1.0f / a.y, part2 = 1.0f / b.y;
         const float of_sums = y != nullptr ? per_sum : 0.0f;        // what all of p have in common changes no order
-        bool odd = beyond || fabsf(a.x) == INFINITY || fabsf(b.x) == INFINITY;
+        bool odd = beyond || coarse(a.x) || coarse(b.x);
         for (int from = begin; from < end; from += BLOCK * VEC, at += BLOCK * VEC) {        // together: the wave shares what it has seen
             float v[VEC], v2[VEC], inverse[VEC], rough[VEC];
             const int left = end - at;
