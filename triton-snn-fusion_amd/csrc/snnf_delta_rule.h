@@ -76,6 +76,14 @@ __device__ __forceinline__ f32x4 product(const Terms<NA>& a, const Terms<NB>& b,
     return c;
 }
 
+// Over the four rows of 16 lanes
+__device__ __forceinline__ float sum_of_rows(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
 // Nothing is moved across by the compiler, which would put loads off until their values are needed.
 __device__ __forceinline__ void now() { __builtin_amdgcn_sched_barrier(0); }
 
@@ -259,7 +267,8 @@ template <typename T, int KS> struct Rows {
 };
 
 // 16 bytes a lane from memory to LDS, a lane's behind the one before it: `lds` is the first lane's byte address. Written out, since the compiler lets every later read of LDS wait for what it
-// knows to be on its way there; whoever reads waits (`arrived`) and passes a barrier first.
+// knows to be on its way there; whoever reads waits (`arrived`) and passes a barrier first. m0 cannot be named as overwritten: the compiler keeps it from its registers and writes it
+// itself only for what these kernels do not hold (registers with an index that varies, messages, other loads to LDS); its listing of them has no m0 but these.
 __device__ __forceinline__ void to_lds(const void* from, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(lds) : "memory");
 }

@@ -14,7 +14,7 @@ namespace {
 // The backward pass wants transposes: of the scores, and of (I + diag(beta) L)^-1, whose transpose turns a gradient of beta delta into that of the rows in front.
 // A workgroup to a chunk of a value head, a wave to 16 rows. The inverse: blocks on the diagonal by substitution, those below by products in float32. Bound by the chain of loads, substitution,
 // three joins of blocks and stores, of which four workgroups to a CU overlap, for which registers and LDS just do (17 KB of LDS more for a matrix of scores, and 100 bytes of spilled registers a thread with them,
-// 181 us in place of 122): 8192 chunks of 128 bfloat16 elements 122 us, 390 MB at 3.2 TB/s.
+// 181 us in place of 122): 8192 chunks of 128 bfloat16 elements, two thirds of them of steps that are there, 122 us. 4096 whole ones, 264 MB of heads and fragments, 78 us (3.4 TB/s).
 constexpr int kPitch = 68;              // of a [64 x 64] matrix in LDS: rows start 4 banks apart
 
 // rows 16 a.., columns 16 b + 4 (lane / 16) + 0..3 of lane % 16's row
@@ -543,14 +543,8 @@ __global__ __launch_bounds__(64 * KS) void delta_join_kernel(DeltaArgs p, int ba
 // ------------------------------------------------------------------------------------------------------------------
 // Step by step, in float32: 64 columns of the state to a workgroup, 8 rows and 4 columns to a thread. k . S and q . S are summed over the rows in one
 // exchange; out = scale (q . S + (q . k) beta delta). One step is bound by memory, 33.7 MB for 16 requests x 16 heads of 128 x 128 in 8.4 us (4.0 TB/s, a launch's start and end among them), each further one by the
-// vector units, 0.9 us: chunks are faster from some 20 steps on (16 steps 23.2 us, 17 as a chunk 29.7; one request 16.8 and 19.6).
-__device__ __forceinline__ float sum_of_rows(float v) {      // over the four rows of 16 lanes
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
+// vector units, 0.9 us. 16 steps take 23.2 us and 17 as a chunk 29.7 (one request 16.8 and 19.6), so that 17 to some 20 would be faster step by step; they go in chunks since the steps' operands
+// go to LDS at once, a piece of one step to a thread, of which there are as many as 16 steps have pieces.
 // Of four numbers at once: row g of 16 lanes gets the sum of the g-th.
 __device__ __forceinline__ float sums_of_rows(float a, float b, float c, float d) {
     const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);

@@ -213,12 +213,6 @@ __global__ __launch_bounds__(kTerms<T> == 1 ? 512 : 256) void delta_walk_back_ke
 // ------------------------------------------------------------------------------------------------------------------
 // Of queries and keys transposed, [DK x steps]: a wave owns 16 steps as columns, so that dP and dL, contracted over steps next, are multiplied as they lie in
 // accumulators. Those are worked out twice, with the wave's steps as rows and as columns of the matrix.
-__device__ __forceinline__ float over_groups(float v) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
 // A row of 32 value columns in LDS: [term][64 rows][32], 16 bytes at a place that depends on the row.
 __device__ __forceinline__ uint32_t value_place(int row, int slot) { return static_cast<uint32_t>(row * 32 + 8 * slot_of<4>(row, slot)); }
 template <int N>
@@ -624,10 +618,10 @@ __global__ __launch_bounds__((GradientPieces<T, KS, RANKS>::THREADS)) void delta
                 dk_all[d] += dk[d];
             }
         }
-        sum = over_groups(sum);
-        tail = over_groups(tail);
-        dbeta = over_groups(dbeta);
-        zv = over_groups(zv);
+        sum = sum_of_rows(sum);
+        tail = sum_of_rows(tail);
+        dbeta = sum_of_rows(dbeta);
+        zv = sum_of_rows(zv);
         dot = lane_sum(dot);
         const int first = item.chunk * kChunk, hv = item.h * members + item.member, t_own = first + own;
         if (group == 0) {
