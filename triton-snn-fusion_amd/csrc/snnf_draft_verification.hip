@@ -3,8 +3,8 @@
 // probability r_i / sum r: r = p behind all drafts, max(p - q, 0) where one was turned down. So every token is distributed as p. The argmax is taken as it is written, whatever the noise: an
 // entry of r = 0 has 0 and is the largest where no entry has noise above 0.
 // Two launches: (r, s) = an r near the largest x / temperature and sum exp(x / temperature - r) of every row, then the decisions and one more pass over the row that is drawn from. Bound by
-// memory; few rows are split over workgroups. 256 requests of 4 drafts x 128000 bfloat16 with both distributions take 168 us, of them 120 the first launch: 590 MB at 4.9 TB/s, next to what 295
-// million exponents take of the vector units; one request of 4 x 32000 takes 12, the second launch's chain of statistics, drafted logits, verdicts, row and join.
+// memory; few rows are split over workgroups. 256 requests of 4 drafts x 128000 bfloat16 with both distributions take 167 us, of them 114 the first launch: 590 MB at 5.2 TB/s, next to what 295
+// million exponents take of the vector units; one request of 4 x 32000 takes 12.9, the second launch's chain of statistics, drafted logits, verdicts, row and join.
 // A decision is that of float64 on the given numbers: float32 gives each number with a bound of its error (`sum_doubt`, `share_doubt`), and where two cannot be told apart the workgroup goes
 // over the rows again in float64. That takes several times as long as the rest (765 us in place of 164 at 256 x 4 x 128000, two of 150 calls on random numbers), so that the bounds matter. Exponents are powers of two, x * slope - r in one rounding; r is a whole number, so that
 // sums for different r are brought together exactly; sums are compensated in a thread and float64 from there on.
@@ -565,7 +565,7 @@ void split_row(int64_t rows, int64_t wanted, int least, int V, int* splits, int*
     *splits = (V + *span - 1) / *span;
 }
 // Few rows are split until four workgroups to a CU have a piece each (32 x 8 x 32000 float32: 17.7 us, with two 19.2), but pieces are of some rounds of a workgroup at least: 4096 elements in
-// the first launch (one request of 4 x 32000: 4096 12.8, 8192 13.0, 16384 13.9 us), 2048 in the second, whose pieces follow a chain of their own (2048 11.9, 4096 13.0, 8192 15.4).
+// the first launch (one request of 4 x 32000: 4096 12.8, 8192 13.0, 16384 13.9 us), 2048 in the second, whose pieces follow a chain of their own (2048 11.9, 4096 13.0, 8192 15.4; these and those above as measured when the draw had exponential noise alone, which made it 1 us shorter).
 VerifyShape verify_shape(int64_t N, int rows, int V) {
     VerifyShape s;
     split_row(N * rows, compute_units() * 4, 4096, V, &s.splits, &s.span);
