@@ -63,7 +63,7 @@ def noises(N, V, g):
 @pytest.mark.gpu
 @pytest.mark.parametrize("draft", [True, False])
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("V", [2, 300, 9001, 70000])
+@pytest.mark.parametrize("V", [1, 2, 300, 9001, 70000])
 def test_noise_that_is_not_exponential(hip_ops, V, dtype, draft):
     N = 6
     for i, (what, noise) in enumerate(noises(N, V, gen(V))):

@@ -427,7 +427,7 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
             token = static_cast<int64_t>(~static_cast<uint32_t>(largest[taken]));
             const float e = noise[token];
             if (fabsf(e) == INFINITY) token = 0;
-            else if (!(e > 0.0f || __float_as_uint(e) == 0u) && p.V > 1) token = token == 0;
+            else if (!(e > 0.0f || __float_as_uint(e) == 0u) && (p.V > 1 || e != e)) token = p.V > 1 ? token == 0 : -100;
         }
     } else {
         const int64_t drafted = taken < length ? p.drafts[static_cast<int64_t>(n) * p.K + taken] : -1;
